@@ -439,6 +439,146 @@ kc_status kc_learn_apply(kc_handle* h, const double* sums, const double* row_sum
  * order) into host memory; waits for the device. */
 kc_status kc_copy_weights(kc_handle* h, uint64_t offset, uint64_t count, float* host);
 
+/* ---------------------------------------------------------------------------
+ * Drawing answers, the loss of drawn answers, and gradient clipping. The
+ * reference draws from a question's whole distribution (sampleRow, forward/
+ * sampling.ts:41-57) and learns unclipped; these entry points are additions
+ * beside kc_select / kc_select_batch, kc_backward* and kc_learn_*.
+ *
+ * Rows. A row is one question's scores (any additive units: a mask's -1e30
+ * included) or its distribution p. Two layouts:
+ *   frames > 0: a packed batch as kc_forward_batch_device leaves it: frame f's
+ *     [Q_f, R_f] block at p_off[f] (elements of values and of every output
+ *     laid out like it), its first question at q_off[f]; q_off NULL = one row
+ *     a frame. rows may exceed q_off[frames]: the rows behind the last frame
+ *     are left alone, so a captured graph can be replayed on smaller batches.
+ *     row_len bounds the longest row (0 = KC_MAX_BANK); a row longer than that
+ *     is refused by itself (KC_NO_SELECTION, loss 0, nothing else written).
+ *   frames = 0: dense [rows, row_len], row i at values + i * row_pitch
+ *     elements (0 = row_len).
+ * An entry is out of the row's support when it is NaN, a score at or below
+ * -1e29 (f16: also -65504, the type's lowest), or a p that is not above 0;
+ * +infinity counts as the largest finite f32. */
+#define KC_DTYPE_F32 0
+#define KC_DTYPE_F16 1
+#define KC_DTYPE_BF16 2
+#define KC_DTYPE_F64 3            /* kc_clip_grads only */
+#define KC_ROWS_SCORES 0
+#define KC_ROWS_P 1               /* f32 probabilities, as kc_forward_batch returns them */
+#define KC_MAX_ROW 262128u        /* longest row the row entry points take */
+
+typedef struct kc_rows_view {
+  const void* values;
+  const uint64_t* q_off;   /* [frames+1] or NULL */
+  const uint64_t* p_off;   /* [frames+1] */
+  uint32_t rows, frames;
+  uint64_t row_len, row_pitch;
+  int32_t dtype, kind;     /* KC_DTYPE_F32 / F16 / BF16, KC_ROWS_* */
+} kc_rows_view;
+
+/* The policy a row is drawn from, applied in this order. With m the row's
+ * largest value: weights w_j = exp((v_j - m) / temperature), or for p
+ * (p_j / m)^(1 / temperature); top_k keeps the k largest (0 = off); top_p the
+ * shortest prefix in descending order that holds top_p of what top_k left
+ * (1 = off; the largest entry always stays); min_p the entries with w_j >=
+ * min_p times the largest (0 = off). Ties go to the lowest index. Entries
+ * with w_j < exp(-700) are dropped. pi_j = w_j / sum of the kept. Temperature
+ * 0 keeps the first largest entry alone. The row_* arrays ([rows] or NULL)
+ * replace a limit row by row; there, a temperature that is not above 0 means
+ * 0, a NaN top_p or min_p cuts nothing. Weights and their sums are 64-bit, in
+ * a fixed order: equal calls give equal bits. */
+typedef struct kc_sampling {
+  float temperature;
+  uint32_t top_k;
+  float top_p, min_p;
+  const float* row_temperature;
+  const uint32_t* row_top_k;
+  const float* row_top_p;
+  const float* row_min_p;
+} kc_sampling;
+
+/* What a draw writes; every pointer may be NULL but not all of them. */
+typedef struct kc_draw_out {
+  uint32_t* index;   /* [rows] the drawn entry; KC_NO_SELECTION for an empty row */
+  uint32_t* kept;    /* [rows] entries the policy kept */
+  float* logp;       /* [rows] log pi of the drawn entry; -infinity for an empty row */
+  float* p;          /* pi, laid out like the rows (dense: p_pitch elements a row, 0 = row_len); 0 off the support.
+                        May be the f32 values themselves. */
+  uint64_t p_pitch;
+  uint64_t p_capacity, q_capacity; /* elements of p and of the per-row arrays (kc_draw_batch only) */
+} kc_draw_out;
+
+/* One draw a row: the first entry in bank order whose running pi passes
+ * uniforms[row] in [0, 1) (DEVICE f64 [rows]; values outside are clamped), as
+ * sampleRow walks it; uniforms NULL: the first largest entry. DEVICE pointers
+ * throughout; one launch on the handle's stream, no allocation, no wait, so it
+ * can be captured. The handle's resident batch stays resident. */
+kc_status kc_draw_device(kc_handle* h, const kc_rows_view* rows, const kc_sampling* sampling, const double* uniforms,
+                         const kc_draw_out* out);
+/* The same for one question x bank matrix in HOST memory (a kc_select result:
+ * p [q, r] with r <= KC_MAX_BANK); every pointer is a host pointer. */
+kc_status kc_draw(kc_handle* h, uint32_t q, uint32_t r, const float* p, const kc_sampling* sampling,
+                  const double* uniforms, const kc_draw_out* out);
+/* The last kc_forward_batch / kc_select_batch batch's distributions, still
+ * resident on the device, drawn under `sampling` (HOST row_* arrays and
+ * uniforms, [batch questions]) into HOST outputs laid out like that batch's.
+ * Refused (KC_ERR_INVALID_ARG) under kc_select_batch's conditions. The draw is
+ * exact for the p rows it reads; at KC_PRECISION_CERTIFIED those carry that
+ * path's ~1e-6. */
+kc_status kc_draw_batch(kc_handle* h, const kc_sampling* sampling, const double* uniforms, const kc_draw_out* out);
+
+/* The loss of drawn answers under the policy that drew them, and its gradient
+ * by the scores (the kept set taken as constant):
+ *   loss = -advantage * log pi(action) - entropy_coef * H(pi)
+ *   grad_j = row_weight * (advantage * (pi_j - [j = action])
+ *            + entropy_coef * pi_j * (log pi_j + H)) / temperature
+ * for kept j, 0 elsewhere, rounded once to the scores' type. A row whose
+ * action is KC_NO_TARGET, outside the row or not kept, and a row at temperature
+ * 0, has loss 0 and gradient 0 (logp: 0 without a target, -infinity for an
+ * action the policy cannot take). DEVICE pointers; queued like kc_draw_device. */
+typedef struct kc_policy_loss_view {
+  const uint32_t* actions;  /* [rows] */
+  const float* advantage;   /* [rows] */
+  const float* row_weight;  /* [rows] or NULL (1): the loss's own upstream gradient */
+  float entropy_coef;
+  float* loss;              /* [rows] or NULL */
+  float* logp;              /* [rows] or NULL */
+  float* entropy;           /* [rows] or NULL; 0 for an empty row */
+  void* grad;               /* the scores' type and layout (dense: grad_pitch, 0 = row_len), or NULL; may be the scores themselves */
+  uint64_t grad_pitch;
+} kc_policy_loss_view;
+kc_status kc_policy_loss(kc_handle* h, const kc_rows_view* rows, const kc_sampling* sampling,
+                         const kc_policy_loss_view* loss);
+
+/* The policy kc_backward and kc_backward_batch_device differentiate from the
+ * next call on: the targets' policy term becomes (pi - onehot) / temperature
+ * over pi's support, nothing for a target that pi does not hold (an AWAY
+ * target keeps its own weighting, with pi for p). NULL: the whole softmax at
+ * temperature 1, as the reference. Scalar limits only; temperature above 0.
+ * The policy output, the value head and the readings stay those of p. */
+kc_status kc_set_policy(kc_handle* h, const kc_sampling* sampling);
+
+/* The global norm of many gradients and clipping by it:
+ *   norm = sqrt(sum_t weight_t^2 * |in_t|^2), scale = min(1, max_norm / norm)
+ *   (1 when the norm is not finite), out_t = in_t * scale.
+ * grads: HOST array of DEVICE tensors, contiguous, KC_DTYPE_*; out NULL = the
+ * tensor only counts, out = in clips in place; outputs must not overlap other
+ * tensors. max_norm >= 0 (+infinity: the norm alone decides nothing).
+ * workspace: DEVICE, kc_clip_workspace(count) bytes, the caller's own for as
+ * long as the call runs (two captured graphs need two). result: DEVICE [2]
+ * norm, scale (f64). Sums are 64-bit in a fixed order. Queued on the handle's
+ * stream; no allocation, no wait. */
+typedef struct kc_grad_view {
+  const void* in;
+  void* out;
+  uint64_t n;
+  double weight;
+  int32_t dtype;
+} kc_grad_view;
+uint64_t kc_clip_workspace(uint64_t count);
+kc_status kc_clip_grads(kc_handle* h, const kc_grad_view* grads, uint64_t count, double max_norm, void* workspace,
+                        uint64_t workspace_bytes, double* result);
+
 /* KRY1 checkpoints (host/checkpoint.ts:17-116): 11 little-endian u32 header
  * words (magic "KRY1" = 0x4b525931, version 1, hiddenSize, ffnSize,
  * encoderBlocks, mixerBlocks, headCount, headDim, routeKindCount, tokenRows

@@ -10,12 +10,14 @@ from .frame import (FrameBatch, HostFrame, HostFrameError, HostRecord, HostToken
                     compile_active_frame, pack_frame_batch, pack_host_frame, record_ranges)
 from .model import (BRAIN_FORWARD_CONFIG, RECORD_WIDTH, BrainForwardConfig, BrainForwardWeights,
                     create_brain_forward_weights, embedding_table_bases, weight_layout)
+from .policy import GradList, Sampling
 
 __all__ = [
     "FrameBatch", "HostFrame", "HostFrameError", "HostRecord", "HostToken", "PAD_TOKEN", "QUERY_BAND",
     "RECORD_WIDTH", "compile_active_frame", "pack_frame_batch", "pack_host_frame", "record_ranges",
     "BRAIN_FORWARD_CONFIG", "BrainForwardConfig", "BrainForwardWeights", "create_brain_forward_weights",
-    "embedding_table_bases", "weight_layout", "cuda_backend", "CudaBrainBackend", "BrainSession",
+    "embedding_table_bases", "weight_layout", "cuda_backend", "CudaBrainBackend", "BrainSession", "GradList",
+    "Sampling",
 ]
 
 

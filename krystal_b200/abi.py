@@ -31,6 +31,9 @@ KC_NO_TARGET = 0xFFFFFFFF
 KC_AWAY_TARGET = 0x80000000
 KC_LEARN_STATS = 8
 KC_NO_WORD = 0xFFFFFFFF
+KC_DTYPE_F32, KC_DTYPE_F16, KC_DTYPE_BF16, KC_DTYPE_F64 = 0, 1, 2, 3
+KC_ROWS_SCORES, KC_ROWS_P = 0, 1
+KC_MAX_ROW = 262128
 CHECKPOINT_REFUSALS = {1: "not a krystal checkpoint", 2: "a later checkpoint format", 3: "a different geometry",
                        4: "a different vocabulary", 5: "truncated"}
 
@@ -43,7 +46,8 @@ EXPORTS = ("kc_abi_version", "kc_create", "kc_sync", "kc_encode", "kc_select", "
            "kc_stream_poll", "kc_stream_clock_ms", "kc_stream_last_error", "kc_stream_destroy",
            "kc_stream_push_many", "kc_load_checkpoint", "kc_save_checkpoint", "kc_select_batch",
            "kc_inject_wait_expiry", "kc_learn_plan", "kc_learn_accumulate_rows", "kc_learn_apply",
-           "kc_copy_weights", "kc_stream_create_ex", "kc_stream_read_stats")
+           "kc_copy_weights", "kc_stream_create_ex", "kc_stream_read_stats", "kc_draw_device", "kc_draw",
+           "kc_draw_batch", "kc_policy_loss", "kc_set_policy", "kc_clip_workspace", "kc_clip_grads")
 
 
 class KrystalCudaError(RuntimeError):
@@ -176,6 +180,31 @@ class KcStageTimes(C.Structure):
         return {n: getattr(self, n) for n, _ in self._fields_}
 
 
+class KcRowsView(C.Structure):
+    _fields_ = [("values", P), ("q_off", P), ("p_off", P), ("rows", C.c_uint32), ("frames", C.c_uint32),
+                ("row_len", C.c_uint64), ("row_pitch", C.c_uint64), ("dtype", C.c_int32), ("kind", C.c_int32)]
+
+
+class KcSampling(C.Structure):
+    _fields_ = [("temperature", C.c_float), ("top_k", C.c_uint32), ("top_p", C.c_float), ("min_p", C.c_float),
+                ("row_temperature", P), ("row_top_k", P), ("row_top_p", P), ("row_min_p", P)]
+
+
+class KcDrawOut(C.Structure):
+    _fields_ = [("index", P), ("kept", P), ("logp", P), ("p", P), ("p_pitch", C.c_uint64),
+                ("p_capacity", C.c_uint64), ("q_capacity", C.c_uint64)]
+
+
+class KcPolicyLossView(C.Structure):
+    _fields_ = [("actions", P), ("advantage", P), ("row_weight", P), ("entropy_coef", C.c_float), ("loss", P),
+                ("logp", P), ("entropy", P), ("grad", P), ("grad_pitch", C.c_uint64)]
+
+
+class KcGradView(C.Structure):
+    # `in` is a Python keyword
+    _fields_ = [("in_", P), ("out", P), ("n", C.c_uint64), ("weight", C.c_double), ("dtype", C.c_int32)]
+
+
 _lib = None
 
 
@@ -241,13 +270,22 @@ def load(path: str | os.PathLike | None = None) -> C.CDLL:
     lib.kc_destroy.restype = None
     lib.kc_last_error.argtypes = [P]
     lib.kc_last_error.restype = C.c_char_p
+    lib.kc_draw_device.argtypes = [P, C.POINTER(KcRowsView), C.POINTER(KcSampling), P, C.POINTER(KcDrawOut)]
+    lib.kc_draw.argtypes = [P, C.c_uint32, C.c_uint32, P, C.POINTER(KcSampling), P, C.POINTER(KcDrawOut)]
+    lib.kc_draw_batch.argtypes = [P, C.POINTER(KcSampling), P, C.POINTER(KcDrawOut)]
+    lib.kc_policy_loss.argtypes = [P, C.POINTER(KcRowsView), C.POINTER(KcSampling), C.POINTER(KcPolicyLossView)]
+    lib.kc_set_policy.argtypes = [P, C.POINTER(KcSampling)]
+    lib.kc_clip_workspace.argtypes = [C.c_uint64]
+    lib.kc_clip_workspace.restype = C.c_uint64
+    lib.kc_clip_grads.argtypes = [P, P, C.c_uint64, C.c_double, P, C.c_uint64, P]
     for name in ("kc_create", "kc_sync", "kc_encode", "kc_select", "kc_forward_batch", "kc_forward_batch_device",
                  "kc_set_stream", "kc_synchronize", "kc_profile", "kc_profile_read", "kc_select_noalloc",
                  "kc_set_precision", "kc_backward", "kc_backward_batch_device", "kc_learn_frame_stats",
                  "kc_learn_accumulate", "kc_stream_create", "kc_stream_push", "kc_stream_flush", "kc_stream_poll",
                  "kc_stream_push_many", "kc_load_checkpoint", "kc_save_checkpoint", "kc_select_batch",
                  "kc_inject_wait_expiry", "kc_learn_plan", "kc_learn_accumulate_rows", "kc_learn_apply",
-                 "kc_copy_weights", "kc_stream_create_ex", "kc_stream_read_stats"):
+                 "kc_copy_weights", "kc_stream_create_ex", "kc_stream_read_stats", "kc_draw_device", "kc_draw",
+                 "kc_draw_batch", "kc_policy_loss", "kc_set_policy", "kc_clip_grads"):
         getattr(lib, name).restype = C.c_int
     _lib = lib
     return lib

@@ -27,6 +27,7 @@ import numpy as np
 from . import abi
 from .frame import FrameBatch, HostFrame
 from .model import BrainForwardConfig, BrainForwardWeights
+from .policy import GradList, Sampling
 
 
 @dataclass
@@ -89,6 +90,16 @@ class MaskRule:
     band_allow: np.ndarray  # u32 [Q]
 
 
+@dataclass
+class Draw:
+    """One draw a question from its tempered and cut distribution (policy.Sampling)."""
+
+    index: np.ndarray  # [Q] u32, KC_NO_SELECTION for an empty row
+    p: np.ndarray      # the policy, laid out like the distributions it was cut from
+    logp: np.ndarray   # [Q] log probability of the drawn entry
+    kept: np.ndarray   # [Q] u32 entries the policy kept
+
+
 def _f32(a) -> np.ndarray:
     return np.ascontiguousarray(a, dtype=np.float32)
 
@@ -141,6 +152,7 @@ class CudaBrainBackend:
         h = C.c_void_p()
         abi.check(self._lib.kc_create(C.byref(cfg), C.byref(views.view), device, C.byref(h)))
         self._h = h
+        self.policy: Sampling | None = None  # what the backward differentiates (set_policy)
 
     # --- BrainBackend -----------------------------------------------------
     def encode(self, frame: HostFrame) -> EncodedFrame:
@@ -310,11 +322,91 @@ class CudaBrainBackend:
         abi.check(self._lib.kc_select_noalloc(self._h, q, r, query_output, bank_keys, bank_values, mask, p, index,
                                               gather), self._h)
 
+    # --- drawing from a tempered and cut policy -----------------------------------
+    def draw(self, rows: abi.KcRowsView, sampling: Sampling, uniforms: int | None = None, index: int | None = None,
+             kept: int | None = None, logp: int | None = None, p: int | None = None, p_pitch: int = 0) -> None:
+        """kc_draw_device: one draw a row of DEVICE rows (policy.ragged_rows,
+        policy.dense_rows), by uniforms (f64) or, without, the first largest
+        entry. Outputs are raw device pointers; queued on the handle's stream."""
+        out = abi.KcDrawOut(index, kept, logp, p, p_pitch, 0, 0)
+        abi.check(self._lib.kc_draw_device(self._h, C.byref(rows), C.byref(sampling.device_struct()), uniforms,
+                                           C.byref(out)), self._h)
+
+    def draw_rows(self, p, q: int, sampling: Sampling, uniforms=None) -> Draw:
+        """kc_draw: one draw a question from a host [q, r] distribution (a
+        Selection's p)."""
+        p = _f32(p)
+        r = p.size // max(1, q)
+        if p.size != q * r:
+            raise ValueError(f"p must hold {q} rows of one length")
+        s, keep = sampling.host_struct(q)
+        u = self._uniforms(uniforms, q)
+        res = Draw(np.empty(q, np.uint32), np.empty(q * r, np.float32), np.empty(q, np.float32), np.empty(q, np.uint32))
+        out = abi.KcDrawOut(res.index.ctypes.data, res.kept.ctypes.data, res.logp.ctypes.data, res.p.ctypes.data, 0,
+                            res.p.size, q)
+        abi.check(self._lib.kc_draw(self._h, q, r, p.ctypes.data, C.byref(s), abi.ptr(u), C.byref(out)), self._h)
+        return res
+
+    def draw_batch(self, sampling: Sampling, uniforms=None) -> Draw:
+        """kc_draw_batch: the last forward_batch / select_batch batch's
+        distributions drawn under `sampling`, without selecting them again."""
+        last = getattr(self, "_last_batch_sizes", None)
+        if last is None:
+            raise RuntimeError("no batch has been run through forward_batch on this backend")
+        total_p, nq, _ = last
+        s, keep = sampling.host_struct(nq)
+        u = self._uniforms(uniforms, nq)
+        res = Draw(np.empty(nq, np.uint32), np.empty(total_p, np.float32), np.empty(nq, np.float32),
+                   np.empty(nq, np.uint32))
+        out = abi.KcDrawOut(res.index.ctypes.data, res.kept.ctypes.data, res.logp.ctypes.data, res.p.ctypes.data, 0,
+                            res.p.size, nq)
+        abi.check(self._lib.kc_draw_batch(self._h, C.byref(s), abi.ptr(u), C.byref(out)), self._h)
+        return res
+
+    @staticmethod
+    def _uniforms(uniforms, rows: int):
+        if uniforms is None:
+            return None
+        u = np.ascontiguousarray(uniforms, dtype=np.float64)
+        if u.size != rows:
+            raise ValueError(f"uniforms must have one entry per question ({rows})")
+        return u
+
+    def policy_loss(self, rows: abi.KcRowsView, sampling: Sampling, actions: int, advantage: int,
+                    entropy_coef: float = 0.0, row_weight: int | None = None, loss: int | None = None,
+                    logp: int | None = None, entropy: int | None = None, grad: int | None = None,
+                    grad_pitch: int = 0) -> None:
+        """kc_policy_loss: the loss of drawn answers under the policy that drew
+        them, and its gradient by the scores (raw device pointers)."""
+        v = abi.KcPolicyLossView(actions, advantage, row_weight, entropy_coef, loss, logp, entropy, grad, grad_pitch)
+        abi.check(self._lib.kc_policy_loss(self._h, C.byref(rows), C.byref(sampling.device_struct()), C.byref(v)),
+                  self._h)
+
+    def set_policy(self, sampling: Sampling | None) -> None:
+        """kc_set_policy: the policy the backward differentiates from now on
+        (None: the whole softmax at temperature 1)."""
+        s = C.byref(sampling.device_struct()) if sampling is not None else None
+        abi.check(self._lib.kc_set_policy(self._h, s), self._h)
+        self.policy = sampling
+
+    def clip_grads(self, grads: GradList, max_norm: float, result: int) -> None:
+        """kc_clip_grads: the list's global norm, and its gradients scaled to
+        max_norm; result: a device pointer to two f64, norm and scale."""
+        if grads.device.index != self.device:
+            raise ValueError(f"the gradients lie on {grads.device}, the backend on cuda:{self.device}")
+        abi.check(self._lib.kc_clip_grads(self._h, grads.address, grads.count, max_norm, grads.workspace.data_ptr(),
+                                          grads.workspace_bytes, result), self._h)
+
     # --- packed ragged batches ------------------------------------------------
     def forward_batch(self, batch: FrameBatch, rule: MaskRule | None = None, uniforms=None,
                       want_query_output: bool = False, p_capacity: int | None = None, word_ids=None,
-                      word_alpha: float = 0.0, out: dict | None = None, mask=None) -> dict:
+                      word_alpha: float = 0.0, out: dict | None = None, mask=None,
+                      sampling: Sampling | None = None) -> dict:
         """Pack, encode and select a whole batch; host arrays in and out.
+        sampling: draw each question's answer from its tempered and cut
+        distribution (uniforms; without them the first largest entry): "index"
+        and "p" are then the draw's and the policy's, with "logp" and "kept"
+        beside them.
         word_ids [records*8] / word_alpha: the same-word bias (WordBias).
         mask: an explicit selection mask laid out like p (frame f's [Q_f, R_f]
         block at p_off[f]; NEG_INF blocked, 0 open), for a grammar that is not
@@ -328,7 +420,7 @@ class CudaBrainBackend:
         sa = ba = u = None
         if rule is not None:
             sa, ba = _u32(rule.schema_allow), _u32(rule.band_allow)
-        if uniforms is not None:
+        if uniforms is not None and sampling is None:
             u = np.ascontiguousarray(uniforms, dtype=np.float64)
         wid = _u32(word_ids) if word_ids is not None else None
         if wid is not None and wid.size != batch.records * 8:
@@ -364,18 +456,27 @@ class CudaBrainBackend:
         self._last_batch_sizes = (int(bo.total_p), int(bo.total_q), batch.frames)
         if qo is not None:
             res["query_output"] = qo[:bo.total_q * self.config.hidden_size]
+        return res if sampling is None else self._drawn(res, sampling, uniforms)
+
+    def _drawn(self, res: dict, sampling: Sampling, uniforms) -> dict:
+        """A batch result with its answers drawn from the resident batch."""
+        d = self.draw_batch(sampling, uniforms)
+        res["p"][:] = d.p
+        res["index"][:] = d.index
+        res.update(logp=d.logp, kept=d.kept)
         return res
 
     def select_batch(self, rule: MaskRule | None = None, uniforms=None, out: dict | None = None,
-                     mask=None) -> dict:
+                     mask=None, sampling: Sampling | None = None) -> dict:
         """kc_select_batch: the last forward_batch's batch selected again under
         `rule` and/or `uniforms` (per question), without encoding it again
-        (consider once, choose many: host/session.ts:128-176). `out` as for
-        forward_batch; without it the result arrays are sized from that batch."""
+        (consider once, choose many: host/session.ts:128-176). `out` and
+        `sampling` as for forward_batch; without `out` the result arrays are
+        sized from that batch."""
         sa = ba = u = None
         if rule is not None:
             sa, ba = _u32(rule.schema_allow), _u32(rule.band_allow)
-        if uniforms is not None:
+        if uniforms is not None and sampling is None:
             u = np.ascontiguousarray(uniforms, dtype=np.float64)
         m = _f32(mask) if mask is not None else None
         sv = abi.KcBatchSelectView(abi.ptr(sa), abi.ptr(ba), abi.ptr(u), abi.ptr(m))
@@ -390,8 +491,9 @@ class CudaBrainBackend:
         bo = abi.KcBatchOut(p.ctypes.data, p.size, idx.ctypes.data, idx.size, p_off.ctypes.data, q_off.ctypes.data,
                             None, 0, 0, 0, 0)
         abi.check(self._lib.kc_select_batch(self._h, C.byref(sv), C.byref(bo)), self._h)
-        return {"p": p[:bo.total_p], "index": idx[:bo.total_q], "p_off": p_off, "q_off": q_off,
-                "total_t": bo.total_t, "total_r": bo.total_r}
+        res = {"p": p[:bo.total_p], "index": idx[:bo.total_q], "p_off": p_off, "q_off": q_off,
+               "total_t": bo.total_t, "total_r": bo.total_r}
+        return res if sampling is None else self._drawn(res, sampling, uniforms)
 
     def forward_batch_device(self, frames: int, records: int, rec_off: int, token_ids: int, field_roles: int,
                              schema_ids: int, band_ids: int, schema_allow: int | None = None,

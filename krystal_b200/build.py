@@ -22,7 +22,7 @@ NVCC_FLAGS = [
     # the exact path must not contract a*b+c: JavaScript never does
     "--fmad=false",
     "-Xcompiler", "-fPIC,-O2",
-    "-shared",
+    "-shared", "--threads", "4",
 ]
 
 
@@ -34,7 +34,7 @@ def nvcc() -> str:
 
 
 def sources() -> list[Path]:
-    return sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + [ROOT / "include" / "krystal_cuda.h"]
+    return sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + [ROOT / "include" / "krystal_cuda.h"]
 
 
 def needs_build() -> bool:
@@ -49,7 +49,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         return LIB
     OUT_DIR.mkdir(exist_ok=True)
     tmp = LIB.with_suffix(".so.tmp")
-    cmd = [nvcc(), *NVCC_FLAGS, "-I", str(ROOT / "include"), "-o", str(tmp), str(CSRC / "krystal_cuda.cu")]
+    cmd = [nvcc(), *NVCC_FLAGS, "-I", str(ROOT / "include"), "-o", str(tmp), *map(str, sorted(CSRC.glob("*.cu")))]
     if verbose:
         print(" ".join(cmd), file=sys.stderr)
     subprocess.run(cmd, check=True)

@@ -195,6 +195,10 @@ struct SelBackArgs {
   float* dig;                // [Q,128]
   float* dag;                // [Q,128]
   float* dscore;             // [P]
+  // the policy the targets' term differentiates (kc_set_policy): pi laid out
+  // like p, and 1 / temperature; null: p itself
+  const float* pi;
+  double inv_temperature;
 };
 
 __global__ void __launch_bounds__(256) k_sel_back_scores(SelBackArgs a) {
@@ -239,12 +243,20 @@ __global__ void __launch_bounds__(256) k_sel_back_scores(SelBackArgs a) {
   const bool valid = raw != KC_INVALID;
   const bool away = valid && raw >= 0x80000000u;
   const uint32_t target = away ? raw - 0x80000000u : raw;
-  const double p_away = away && target < uint32_t(R) ? double(ps[target]) : 0.0;
+  const float* pol = a.pi ? a.pi + po : ps;
+  const bool held = !a.pi || target >= uint32_t(R) || pol[target] > 0.0f;  // a target pi does not hold moves nothing
+  const double p_away = away && target < uint32_t(R) ? double(pol[target]) : 0.0;
   const double sc = away ? p_away / js_max(1.0 - p_away, 1e-6) : 0.0;
   for (int j = tid; j < R; j += 256) {
     const double pij = ps[j];
     const double one = uint32_t(j) == target ? 1.0 : 0.0;
-    const double pg = !valid ? 0.0 : away ? sc * (one - pij) : pij - one;
+    double pg = 0.0;
+    if (!a.pi) {
+      pg = !valid ? 0.0 : away ? sc * (one - pij) : pij - one;
+    } else if (valid && held && pol[j] > 0.0f) {
+      const double pj = pol[j];
+      pg = (away ? sc * (one - pj) : pj - one) * a.inv_temperature;
+    }
     a.dscore[po + j] = f32(pij * (double(f32(s64[j])) - row_sum) + pg);
   }
 }

@@ -1,0 +1,192 @@
+// clip.cuh — the global norm of many gradient tensors, and clipping by it:
+// norm = sqrt(sum_t weight_t^2 sum_i g_ti^2), scale = min(1, max_norm / norm)
+// (1 where the norm is not finite: what follows sees the gradients as they
+// are), out_ti = g_ti * scale, rounded once to the tensor's type.
+//
+// Two launches: k_norm leaves one partial sum a CTA, k_scale adds the partial
+// sums again in every CTA (a few KB from L2) and scales. All sums are 64-bit
+// and in an order that the sizes alone decide; there are no atomics. The work
+// is cut into chunks of 32 KB of one tensor; CTA b takes chunks b, b + grid, ...
+// and k_scale takes them from the last back, so that what k_norm read last is
+// still in L2.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "policy_args.h"
+
+namespace kc {
+namespace clip {
+
+constexpr int kThreads = 512;
+constexpr uint32_t kChunkBytes = 32768;
+
+template <uint32_t N>
+struct Table {
+  Tensor t[N];
+  uint32_t count, chunks;
+};
+
+__host__ __device__ constexpr uint32_t dtype_bytes(int d) { return d == kF32 ? 4u : d == kF64 ? 8u : 2u; }
+
+struct Piece {
+  const Tensor* t;
+  uint64_t first;  // element
+  uint32_t n;      // elements
+};
+
+template <uint32_t N>
+__device__ __forceinline__ Piece piece_of(const Table<N>& tb, uint32_t chunk) {
+  uint32_t lo = 0, hi = tb.count;
+  while (hi - lo > 1) {
+    const uint32_t mid = (lo + hi) / 2;
+    if (tb.t[mid].chunk0 <= chunk) lo = mid; else hi = mid;
+  }
+  Piece p;
+  p.t = &tb.t[lo];
+  const uint32_t per = kChunkBytes / dtype_bytes(p.t->dtype);
+  p.first = uint64_t(chunk - p.t->chunk0) * per;
+  p.n = uint32_t(min(uint64_t(per), p.t->n - p.first));
+  return p;
+}
+
+__device__ __forceinline__ double wide(float v) { return double(v); }
+__device__ __forceinline__ double wide(double v) { return v; }
+__device__ __forceinline__ double wide(__half v) { return double(__half2float(v)); }
+__device__ __forceinline__ double wide(__nv_bfloat16 v) { return double(__bfloat162float(v)); }
+__device__ __forceinline__ float scaled(float v, double s) { return v * float(s); }
+__device__ __forceinline__ double scaled(double v, double s) { return v * s; }
+__device__ __forceinline__ __half scaled(__half v, double s) { return __float2half_rn(__half2float(v) * float(s)); }
+__device__ __forceinline__ __nv_bfloat16 scaled(__nv_bfloat16 v, double s) {
+  return __float2bfloat16_rn(__bfloat162float(v) * float(s));
+}
+
+// Elements of a piece ahead of its first 16-byte boundary.
+template <typename T>
+__device__ __forceinline__ uint32_t head_of(const T* p, uint32_t n) {
+  const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(p) & 15);
+  return min(n, off ? uint32_t((16 - off) / sizeof(T)) : 0u);
+}
+
+template <typename T>
+__device__ __forceinline__ double square_sum(const T* in, uint32_t n) {
+  constexpr int V = 16 / int(sizeof(T));
+  const uint32_t head = head_of(in, n), vecs = (n - head) / V;
+  double acc[2] = {0.0, 0.0};
+  const uint4* src = reinterpret_cast<const uint4*>(in + head);
+#pragma unroll 4
+  for (uint32_t i = threadIdx.x; i < vecs; i += kThreads) {
+    const uint4 raw = src[i];
+    alignas(16) T v[V];
+    *reinterpret_cast<uint4*>(v) = raw;
+#pragma unroll
+    for (int e = 0; e < V; e++) {
+      const double d = wide(v[e]);
+      acc[e & 1] = fma(d, d, acc[e & 1]);
+    }
+  }
+  const uint32_t loose = n - vecs * V;  // the head, then the tail
+  for (uint32_t i = threadIdx.x; i < loose; i += kThreads) {
+    const double d = wide(in[i < head ? i : i + vecs * V]);
+    acc[0] = fma(d, d, acc[0]);
+  }
+  return acc[0] + acc[1];
+}
+
+template <typename T>
+__device__ __forceinline__ void scale_piece(const T* in, T* out, uint32_t n, double scale) {
+  constexpr int V = 16 / int(sizeof(T));
+  if ((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(out)) & 15) {
+    for (uint32_t i = threadIdx.x; i < n; i += kThreads) out[i] = scaled(in[i], scale);
+    return;
+  }
+  const uint32_t head = head_of(in, n), vecs = (n - head) / V;
+  const uint4* src = reinterpret_cast<const uint4*>(in + head);
+  uint4* dst = reinterpret_cast<uint4*>(out + head);
+#pragma unroll 4
+  for (uint32_t i = threadIdx.x; i < vecs; i += kThreads) {
+    alignas(16) T v[V];
+    *reinterpret_cast<uint4*>(v) = src[i];
+#pragma unroll
+    for (int e = 0; e < V; e++) v[e] = scaled(v[e], scale);
+    dst[i] = *reinterpret_cast<uint4*>(v);
+  }
+  const uint32_t loose = n - vecs * V;
+  for (uint32_t i = threadIdx.x; i < loose; i += kThreads) {
+    const uint32_t at = i < head ? i : i + vecs * V;
+    out[at] = scaled(in[at], scale);
+  }
+}
+
+// The CTA's sum, in thread order by warps; valid in every thread.
+__device__ __forceinline__ double cta_sum(double v, double* red) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (lane == 0) red[warp] = v;
+  __syncthreads();
+  v = lane < kThreads / 32 ? red[lane] : 0.0;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+template <uint32_t N>
+__global__ void __launch_bounds__(kThreads) k_norm(const __grid_constant__ Table<N> tb, double* __restrict__ partial) {
+  __shared__ double red[kThreads / 32];
+  double sum = 0.0;
+  for (uint32_t c = blockIdx.x; c < tb.chunks; c += gridDim.x) {
+    const Piece p = piece_of(tb, c);
+    double s = 0.0;
+    switch (p.t->dtype) {
+      case kF32: s = square_sum(static_cast<const float*>(p.t->in) + p.first, p.n); break;
+      case kF16: s = square_sum(static_cast<const __half*>(p.t->in) + p.first, p.n); break;
+      case kBF16: s = square_sum(static_cast<const __nv_bfloat16*>(p.t->in) + p.first, p.n); break;
+      default: s = square_sum(static_cast<const double*>(p.t->in) + p.first, p.n); break;
+    }
+    sum = fma(p.t->weight * p.t->weight, s, sum);
+  }
+  sum = cta_sum(sum, red);
+  if (threadIdx.x == 0) partial[blockIdx.x] = sum;
+}
+
+template <uint32_t N>
+__global__ void __launch_bounds__(kThreads) k_scale(const __grid_constant__ Table<N> tb,
+                                                    const double* __restrict__ partial, uint32_t partials,
+                                                    double max_norm, double* __restrict__ result, int first) {
+  __shared__ double red[kThreads / 32];
+  double sum = 0.0;
+  for (uint32_t i = threadIdx.x; i < partials; i += kThreads) sum += partial[i];
+  const double norm = sqrt(cta_sum(sum, red));
+  const bool cut = norm > max_norm && norm <= 1.7976931348623157e308;
+  const double scale = cut ? max_norm / norm : 1.0;
+  if (first && blockIdx.x == 0 && threadIdx.x == 0) {
+    result[0] = norm;
+    result[1] = scale;
+  }
+  for (uint32_t r = blockIdx.x; r < tb.chunks; r += gridDim.x) {
+    const Piece p = piece_of(tb, tb.chunks - 1 - r);
+    if (!p.t->out || (!cut && p.t->out == p.t->in)) continue;
+    switch (p.t->dtype) {
+      case kF32:
+        scale_piece(static_cast<const float*>(p.t->in) + p.first, static_cast<float*>(p.t->out) + p.first, p.n, scale);
+        break;
+      case kF16:
+        scale_piece(static_cast<const __half*>(p.t->in) + p.first, static_cast<__half*>(p.t->out) + p.first, p.n,
+                    scale);
+        break;
+      case kBF16:
+        scale_piece(static_cast<const __nv_bfloat16*>(p.t->in) + p.first,
+                    static_cast<__nv_bfloat16*>(p.t->out) + p.first, p.n, scale);
+        break;
+      default:
+        scale_piece(static_cast<const double*>(p.t->in) + p.first, static_cast<double*>(p.t->out) + p.first, p.n,
+                    scale);
+        break;
+    }
+  }
+}
+
+}  // namespace clip
+}  // namespace kc

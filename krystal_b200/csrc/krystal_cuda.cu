@@ -21,6 +21,7 @@
 #include <cstdio>
 #include <cstring>
 #include <mutex>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -34,6 +35,7 @@
 #include "learn.cuh"
 #include "ozaki.cuh"
 #include "pack.cuh"
+#include "policy_args.h"
 #include "tc_gemm.cuh"
 
 namespace {
@@ -129,9 +131,15 @@ struct BackWs {
   DevBuf learn_partial;
   // the device learn step's rollback copy, health words and readback
   DevBuf learn_backup, learn_health, learn_out;
+  DevBuf pol;  // pi of every p row, when kc_set_policy names a policy
   // the last batch differentiated: its frame count and the selection it ran under
   uint32_t frames = 0;
   const float* mask_used = nullptr;
+};
+
+// A host draw's staged inputs and its results (kc_draw, kc_draw_batch).
+struct DrawWs {
+  DevBuf values, uniforms, temperature, top_k, top_p, min_p, index, kept, logp, p;
 };
 
 enum Stage { kStPack, kStEmbed, kStEncGemm, kStEncAttn, kStPool, kStMixer, kStSelector, kStFallback, kStEncFfn,
@@ -192,6 +200,10 @@ struct kc_handle {
   Workspace ws;      // the batch
   Workspace ws_fb;   // frames recomputed on the exact path
   BackWs bw;         // the backward
+  DrawWs dw;         // host draws
+  bool policy_on = false;  // the backward differentiates `policy` (kc_set_policy)
+  kc_sampling policy{};
+  std::vector<kc::clip::Tensor> clip_list;  // kc_clip_grads' tensors, reused
   DevBuf wt;         // transposed copies of the block and selector matrices (page layout)
   bool wt_blocks_dirty = true;  // the blocks' transposed copies are stale
   bool wt_sel_dirty = true;     // the selector's transposed copies are stale
@@ -1569,6 +1581,8 @@ struct DeviceGuard {
 // The backward of every frame of a packed batch (backward.cuh), after an
 // exact forward that saves what the backward reads. `sel`, `targets`,
 // `valence` are device arrays or null. Results stay in h->bw and ws.p.
+kc_status policy_rows(kc_handle* h, Workspace& ws, uint32_t frames, const kc::FrameTotals& tot, float* pi);
+
 kc_status backward_batch(kc_handle* h, const DevBatch& b, const float* sel, const uint32_t* targets,
                          const double* valence, kc::FrameTotals* tot_out, bool exact) {
   // The GEMMs run on the tensor cores unless the handle or the caller asks
@@ -1658,6 +1672,12 @@ kc_status backward_batch(kc_handle* h, const DevBatch& b, const float* sel, cons
   float* dquery = P<float>(bw.dquery);
   float* dbk = P<float>(bw.dbk);
   float* dbv = P<float>(bw.dbv);
+  const float* pi = nullptr;  // the policy the targets' term differentiates; null: p
+  if (h->policy_on && PP) {
+    KC_TRY(need(bw.pol, PP * 4), "workspace");
+    KC_CHECK(policy_rows(h, ws, F, tot, P<float>(bw.pol)));
+    pi = P<float>(bw.pol);
+  }
   {
     ProfScope ps(h, kStSelector);
     if (Q) {
@@ -1673,7 +1693,7 @@ kc_status backward_batch(kc_handle* h, const DevBatch& b, const float* sel, cons
     h->launches += 2;
     if (Q) {
       kc::SelBackArgs sb{geo, p, bv, h->w + d.off_val, P<float>(bw.dpred), targets, dquery, P<float>(bw.dig),
-                         P<float>(bw.dag), P<float>(bw.dscore)};
+                         P<float>(bw.dag), P<float>(bw.dscore), pi, pi ? 1.0 / double(h->policy.temperature) : 1.0};
       kc::k_sel_back_scores<<<unsigned(Q), 256, size_t(tot.max_r) * 12, h->stream>>>(sb);
       kc::k_sel_back_dq<<<unsigned(Q), 128, 0, h->stream>>>(geo, P<float>(bw.dscore), P<float>(ws.sk), h_scale,
                                                            P<float>(bw.dqp));
@@ -2789,4 +2809,5 @@ const char* kc_last_error(kc_handle* h) { return h ? h->err.c_str() : g_create_e
 
 }  // extern "C"
 
+#include "policy_abi.cuh"
 #include "stream.cuh"

@@ -1,0 +1,68 @@
+// policy.cu — the launchers of the policy rows (policy.cuh, by element type) and
+// of the gradient clipping (clip.cuh).
+#include <algorithm>
+
+#include "clip.cuh"
+#include "policy_args.h"
+
+namespace kc {
+namespace pol {
+
+cudaError_t launch_draw(const DrawArg& a, int dtype, cudaStream_t stream, uint64_t* launches) {
+  if (a.r.rows == 0) return cudaSuccess;
+  ++*launches;
+  return dtype == kF32 ? draw_f32(a, stream) : dtype == kF16 ? draw_f16(a, stream) : draw_bf16(a, stream);
+}
+
+cudaError_t launch_policy_loss(const LossArg& a, int dtype, cudaStream_t stream, uint64_t* launches) {
+  if (a.r.rows == 0) return cudaSuccess;
+  ++*launches;
+  return dtype == kF32 ? loss_f32(a, stream) : dtype == kF16 ? loss_f16(a, stream) : loss_bf16(a, stream);
+}
+
+}  // namespace pol
+
+namespace clip {
+namespace {
+
+template <uint32_t N>
+unsigned fill(Table<N>& tb, Tensor* t, uint32_t count) {
+  uint64_t chunk = 0;
+  for (uint32_t i = 0; i < count; i++) {
+    tb.t[i] = t[i];
+    tb.t[i].chunk0 = uint32_t(chunk);
+    const uint64_t per = kChunkBytes / dtype_bytes(t[i].dtype);
+    chunk += (t[i].n + per - 1) / per;
+  }
+  tb.count = count;
+  tb.chunks = uint32_t(chunk);
+  return tb.chunks;
+}
+
+}  // namespace
+
+cudaError_t launch_clip(Tensor* t, uint64_t count, double max_norm, double* workspace, double* result, int sms,
+                        cudaStream_t stream, uint64_t* launches) {
+  const uint32_t most = std::min<uint32_t>(kMaxCtas, uint32_t(sms) * 4);
+  static thread_local Table<kTable> tb;
+  uint32_t partials = 0;
+  for (int pass = 0; pass < 2; pass++) {
+    bool first = true;
+    for (uint64_t at = 0; at < count || first; at += kTable) {
+      const uint32_t chunks = fill(tb, t + at, uint32_t(std::min<uint64_t>(kTable, count - at)));
+      const unsigned grid = std::max(1u, std::min(most, chunks));
+      if (pass == 0) {
+        k_norm<kTable><<<grid, kThreads, 0, stream>>>(tb, workspace + partials);
+        partials += grid;
+      } else {
+        k_scale<kTable><<<grid, kThreads, 0, stream>>>(tb, workspace, partials, max_norm, result, first ? 1 : 0);
+      }
+      ++*launches;
+      first = false;
+    }
+  }
+  return cudaGetLastError();
+}
+
+}  // namespace clip
+}  // namespace kc

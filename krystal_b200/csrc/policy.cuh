@@ -1,0 +1,670 @@
+// policy.cuh — what a host does with the rows of scores or probabilities a
+// selection leaves: draw an answer from a tempered and cut distribution
+// (k_draw), and the loss of drawn answers with its gradient (k_policy_loss).
+// The selector itself draws from the whole softmax (sampleRow, forward/
+// sampling.ts:41-57); the cuts have no counterpart in the reference.
+//
+// One row v_0 .. v_{n-1}. An entry is open unless it is NaN, a score at or
+// below -1e29 (f16: also the type's lowest value) or a probability that is
+// not above 0. With m the largest open value and T the temperature,
+//
+//   x_j = (v_j - m) / T          (probabilities: (log v_j - log m) / T)
+//   w_j = e^{x_j}                (probabilities at T = 1: v_j itself)
+//
+// and then, in this order, top-k keeps the k largest, top-p the shortest
+// prefix in descending order whose mass reaches top_p of what top-k left,
+// min-p the entries with w_j >= min_p * max w (ties always to the lowest
+// index); entries with x_j < -700 cannot be drawn and are dropped. pi_j =
+// w_j / Z over what is kept.
+//
+// Which entries are kept, and which one a uniform hits, are decisions: they
+// are taken from 64-bit weights summed in a fixed order, so a row's answer
+// does not depend on how the row was split, and equals the definition's to
+// about n * 1e-15 of probability. No entry is sorted: a cut is the largest
+// value t with count(v >= t) >= k, or mass(v >= t) >= top_p * total, found by
+// halving the range of values between snapped row entries.
+//
+// A row lives in registers: E entries a thread, one warp a row up to 1024
+// entries, a CTA to 32768, a cluster of CTAs beyond. Warp g of the row's
+// group owns the contiguous segment [32 E g, 32 E (g + 1)), in chunks of one
+// 16-byte load a lane, so that bank order is (warp, chunk, lane, entry) and a
+// prefix sum needs one warp scan a chunk.
+#pragma once
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "policy_args.h"
+
+namespace kc {
+namespace pol {
+
+constexpr double kDropped = -700.0;  // e^x stays a normal number above it
+
+template <typename T> struct Lowest { static constexpr float open_above = -1e29f; };
+template <> struct Lowest<__half> { static constexpr float open_above = -65504.0f; };
+
+__device__ __forceinline__ float as_f32(float v) { return v; }
+__device__ __forceinline__ float as_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float as_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// f32 values as u32 keys in the same order; 0 is kept for "not in the row's
+// support" (no finite value maps to it).
+__device__ __forceinline__ uint32_t key_of(float v) {
+  const uint32_t b = __float_as_uint(v + 0.0f);  // -0 joins +0
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? (k ^ 0x80000000u) : ~k);
+}
+
+// e^x for -700 <= x <= 0 in 64 bits, by a table of 2^{i/32} (Tang, "Table-
+// driven implementation of the exponential function", ACM TOMS 15(2), 1989):
+// x = (32 q + i) ln2/32 + r, |r| <= ln2/64, and e^r by its Taylor polynomial
+// of degree 5 (the first term left out is below 3e-15). Lane i holds 2^{i/32}
+// and the lanes fetch each other's by a shuffle, so every lane of the warp
+// calls this together.
+__device__ __forceinline__ double exp64(double x, double tab) {
+  constexpr double kBig = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer
+  const double t = fma(x, 46.166241308446828384, kBig);  // 32 / ln 2
+  const int n = __double2loint(t);
+  const double r = fma(t - kBig, -0.021660849392498290195, x);  // ln 2 / 32
+  double p = fma(r, 1.0 / 120.0, 1.0 / 24.0);
+  p = fma(r, p, 1.0 / 6.0);
+  p = fma(r, p, 0.5);
+  p = fma(r, p, 1.0);
+  p = fma(r, p, 1.0);
+  const double s = __shfl_sync(0xffffffffu, tab, n & 31) * p;
+  return __hiloint2double(__double2hiint(s) + ((n >> 5) << 20), __double2loint(s));
+}
+
+// Tempered probabilities take their logarithm here, out of line: the call sits
+// in every loop over a row's entries.
+static __device__ __noinline__ double log64(double v) { return log(v); }
+
+__device__ __forceinline__ double warp_add(double v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+// Inclusive prefix over the lanes.
+__device__ __forceinline__ double warp_scan(double v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double y = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += y;
+  }
+  return v;
+}
+__device__ __forceinline__ uint32_t warp_scan(uint32_t v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t y = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += y;
+  }
+  return v;
+}
+
+// Reductions over a row's group of W warps in each of CL CTAs. Every thread
+// of the group calls each of them the same number of times; sums add the
+// warps, then the CTAs, in order. The slots alternate between two buffers, so
+// one barrier a reduction is enough: a slot is written again only after the
+// next reduction's barrier, which every reader of it has passed.
+template <int W, int CL>
+struct Group {
+  struct Shared {
+    double d[2][W > 1 ? W : 1];
+    uint32_t u[2][3][W > 1 ? W : 1];
+    double cd[2][CL];
+    uint32_t cu[2][3][CL];
+  };
+  Shared& s;
+  int lane, warp, rank, buf;
+
+  __device__ Group(Shared& sh, int l, int w) : s(sh), lane(l), warp(w), rank(0), buf(0) {
+    if constexpr (CL > 1) {
+      rank = int(cooperative_groups::this_cluster().block_rank());
+      cooperative_groups::this_cluster().sync();  // a CTA's shared memory is written once it runs
+    }
+  }
+  __device__ int segment() const { return rank * W + warp; }
+
+  // (sum, min, max) of three values at once
+  __device__ void counts(uint32_t& add, uint32_t& mn, uint32_t& mx) {
+    add = __reduce_add_sync(0xffffffffu, add);
+    mn = __reduce_min_sync(0xffffffffu, mn);
+    mx = __reduce_max_sync(0xffffffffu, mx);
+    if constexpr (W > 1) {
+      buf ^= 1;
+      if (lane == 0) { s.u[buf][0][warp] = add; s.u[buf][1][warp] = mn; s.u[buf][2][warp] = mx; }
+      __syncthreads();
+      const bool in = lane < W;
+      add = __reduce_add_sync(0xffffffffu, in ? s.u[buf][0][lane] : 0u);
+      mn = __reduce_min_sync(0xffffffffu, in ? s.u[buf][1][lane] : 0xffffffffu);
+      mx = __reduce_max_sync(0xffffffffu, in ? s.u[buf][2][lane] : 0u);
+    }
+    if constexpr (CL > 1) {
+      namespace cg = cooperative_groups;
+      cg::cluster_group cl = cg::this_cluster();
+      if (warp == 0 && lane < CL) {
+        uint32_t* dst = cl.map_shared_rank(&s.cu[0][0][0], lane) + buf * 3 * CL;
+        dst[rank] = add; dst[CL + rank] = mn; dst[2 * CL + rank] = mx;
+      }
+      cl.sync();
+      const bool in = lane < CL;
+      add = __reduce_add_sync(0xffffffffu, in ? s.cu[buf][0][lane] : 0u);
+      mn = __reduce_min_sync(0xffffffffu, in ? s.cu[buf][1][lane] : 0xffffffffu);
+      mx = __reduce_max_sync(0xffffffffu, in ? s.cu[buf][2][lane] : 0u);
+    }
+  }
+  // The group's sum of one value a thread; *before (if asked for) gets the
+  // sum over the warps ahead of this one in bank order.
+  __device__ double sum(double v, double* before = nullptr) {
+    v = warp_add(v);
+    if constexpr (W > 1) {
+      buf ^= 1;
+      if (lane == 0) s.d[buf][warp] = v;
+      __syncthreads();
+      const double sc = warp_scan(lane < W ? s.d[buf][lane] : 0.0, lane);
+      if (before) *before = warp ? __shfl_sync(0xffffffffu, sc, warp - 1) : 0.0;
+      v = __shfl_sync(0xffffffffu, sc, W - 1);
+    } else if (before) {
+      *before = 0.0;
+    }
+    if constexpr (CL > 1) {
+      namespace cg = cooperative_groups;
+      cg::cluster_group cl = cg::this_cluster();
+      if (warp == 0 && lane < CL) cl.map_shared_rank(&s.cd[0][0], lane)[buf * CL + rank] = v;
+      cl.sync();
+      const double sc = warp_scan(lane < CL ? s.cd[buf][lane] : 0.0, lane);
+      const double ahead = __shfl_sync(0xffffffffu, sc, rank ? rank - 1 : 0);
+      if (before && rank) *before += ahead;
+      v = __shfl_sync(0xffffffffu, sc, CL - 1);
+    }
+    return v;
+  }
+  // The sum over the warps ahead of this one of a value the warp agrees on.
+  __device__ uint32_t ahead(uint32_t v) {
+    uint32_t before = 0;
+    if constexpr (W > 1) {
+      buf ^= 1;
+      if (lane == 0) s.u[buf][0][warp] = v;
+      __syncthreads();
+      const uint32_t sc = warp_scan(lane < W ? s.u[buf][0][lane] : 0u, lane);
+      before = warp ? __shfl_sync(0xffffffffu, sc, warp - 1) : 0u;
+      v = __shfl_sync(0xffffffffu, sc, W - 1);
+    }
+    if constexpr (CL > 1) {
+      namespace cg = cooperative_groups;
+      cg::cluster_group cl = cg::this_cluster();
+      if (warp == 0 && lane < CL) cl.map_shared_rank(&s.cu[0][0][0], lane)[buf * 3 * CL + rank] = v;
+      cl.sync();
+      const uint32_t sc = warp_scan(lane < CL ? s.cu[buf][0][lane] : 0u, lane);
+      const uint32_t others = __shfl_sync(0xffffffffu, sc, rank ? rank - 1 : 0);
+      if (rank) before += others;
+    }
+    return before;
+  }
+};
+
+// Where a row lies. The frame of a ragged row is found by a 32-way search of
+// q_off (three probes for 4096 frames). False: the row lies behind the last
+// frame's questions, and nothing of it exists.
+struct RowAt {
+  uint64_t in, out;
+  uint64_t n;
+};
+__device__ __forceinline__ bool locate(const RowsArg& r, uint64_t out_pitch, uint32_t row, int lane, RowAt* at) {
+  if (r.frames == 0) {
+    *at = RowAt{row * r.pitch, row * out_pitch, r.row_len};
+    return true;
+  }
+  uint32_t lo = row;
+  uint64_t first = row, count = 1;
+  if (r.q_off) {
+    uint32_t hi = r.frames;
+    lo = 0;
+    if (row >= r.q_off[hi]) return false;
+    while (hi - lo > 1) {
+      const uint32_t step = (hi - lo + 31) / 32;
+      const uint64_t probe = uint64_t(lo) + uint64_t(lane) * step;
+      const uint32_t below = __popc(__ballot_sync(0xffffffffu, probe < hi && r.q_off[probe < hi ? probe : lo] <= row));
+      lo += (below - 1) * step;
+      hi = min(hi, lo + step);
+    }
+    first = r.q_off[lo];
+    count = r.q_off[lo + 1] - first;
+  } else if (row >= r.frames) {
+    return false;
+  }
+  const uint64_t p0 = r.p_off[lo], block = r.p_off[lo + 1] - p0;
+  uint64_t n;
+  if ((block | count) >> 32) n = block / count;
+  else n = uint32_t(block) / uint32_t(count);
+  const uint64_t at0 = p0 + (row - first) * n;
+  *at = RowAt{at0, at0, n};
+  return true;
+}
+
+struct Cut {
+  double inv_t;     // 0: the largest entry alone
+  uint32_t k;       // 0: off
+  double top_p;     // >= 1: off
+  double min_p;     // <= 0: off
+};
+__device__ __forceinline__ Cut cut_of(const CutArg& c, uint32_t row) {
+  const float t = c.row_temperature ? c.row_temperature[row] : c.temperature;
+  const float p = c.row_top_p ? c.row_top_p[row] : c.top_p;
+  const float m = c.row_min_p ? c.row_min_p[row] : c.min_p;
+  Cut o;
+  o.inv_t = t > 0.0f ? 1.0 / double(t) : 0.0;
+  o.k = c.row_top_k ? c.row_top_k[row] : c.top_k;
+  o.top_p = p < 1.0f ? fmax(double(p), 0.0) : 2.0;  // a NaN cuts nothing
+  o.min_p = m > 0.0f ? fmin(double(m), 1.0) : 0.0;
+  if (!(t > 0.0f)) o.k = 1;
+  return o;
+}
+
+// A row's entries in registers, and its cut.
+template <typename T, int E, int W, int CL>
+struct Row {
+  static constexpr int V = 16 / int(sizeof(T));
+  static constexpr int kChunks = E / V;
+  static constexpr uint32_t kCap = uint32_t(32) * E * W * CL;
+  static_assert(E % V == 0, "a thread holds whole vectors");
+
+  Group<W, CL> g;
+  uint32_t k[E];  // keys; 0: not in the support
+  double tab;     // 2^{lane/32}
+  double m, log_m, inv_t;
+  bool power;     // probabilities at a temperature other than 1: x from logarithms
+  bool plain_p;   // probabilities at T = 1: the weights are the values
+  int i0;         // index of this lane's first entry of chunk 0
+
+  __device__ Row(typename Group<W, CL>::Shared& sh, int lane, int warp) : g(sh, lane, warp) {
+    tab = exp2(double(lane) * (1.0 / 32.0));
+  }
+
+  __device__ int at(int c) const { return i0 + c * 32 * V; }
+
+  // Loads n entries from row. A lane's 16-byte loads start on 16-byte
+  // boundaries; a vector that reaches past either end of the row is read
+  // entry by entry.
+  __device__ void load(const T* row, uint32_t n, int kind) {
+    const int shift = int((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+    i0 = g.segment() * 32 * E + g.lane * V - shift;
+#pragma unroll
+    for (int c = 0; c < kChunks; c++) {
+      const int i = at(c);
+      alignas(16) T v[V];
+      bool in[V];
+      if (i >= 0 && i + V <= int(n)) {
+        *reinterpret_cast<uint4*>(v) = __ldcs(reinterpret_cast<const uint4*>(row + i));
+#pragma unroll
+        for (int e = 0; e < V; e++) in[e] = true;
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+          in[e] = i + e >= 0 && i + e < int(n);
+          v[e] = in[e] ? row[i + e] : from_f32<T>(0.0f);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < V; e++) {
+        const float f = as_f32(v[e]);
+        const bool open = in[e] && (kind == kKindP ? f > 0.0f : f > Lowest<T>::open_above);
+        k[c * V + e] = open ? key_of(fminf(f, 3.402823466e38f)) : 0u;
+      }
+    }
+  }
+
+  // The tempered log weight, and the weight, of a key in the support.
+  __device__ double x_of(uint32_t key) const {
+    const double v = double(value_of(key));
+    return power ? (log64(v) - log_m) * inv_t : (v - m) * inv_t;
+  }
+  // Every lane of the warp calls this together; 0 for key 0 and for dropped entries.
+  __device__ double weight(uint32_t key) const {
+    if (plain_p) return key ? double(value_of(key)) : 0.0;
+    const double x = key ? x_of(key) : 0.0;
+    const double w = exp64(fmax(x, kDropped), tab);
+    return key && x >= kDropped ? w : 0.0;
+  }
+
+  // The pivot between two values of the row: halfway in value for scores,
+  // halfway in exponent and mantissa for probabilities (which span decades);
+  // after a dozen steps the two alternate, so that no row takes more than
+  // about 70 steps whatever its values.
+  __device__ static uint32_t pivot(uint32_t lo, uint32_t hi, int step, int kind) {
+    const bool by_value = step < 12 ? kind != kKindP : (step & 1);
+    uint32_t p = lo + (hi - lo + 1) / 2;
+    if (by_value) p = key_of(0.5f * value_of(lo) + 0.5f * value_of(hi));
+    return min(max(p, lo + 1), hi);
+  }
+
+  // Drops the entries below the cut t and all but the first `ties` at it.
+  __device__ void apply(uint32_t t, uint32_t ties, uint32_t all) {
+    if (ties >= all) {
+#pragma unroll
+      for (int e = 0; e < E; e++)
+        if (k[e] < t) k[e] = 0u;
+      return;
+    }
+    uint32_t mine = 0;
+#pragma unroll
+    for (int e = 0; e < E; e++) mine += k[e] == t;
+    uint32_t seen = g.ahead(__reduce_add_sync(0xffffffffu, mine));
+#pragma unroll
+    for (int c = 0; c < kChunks; c++) {
+      uint32_t in = 0;
+#pragma unroll
+      for (int e = 0; e < V; e++) in += k[c * V + e] == t;
+      const uint32_t incl = warp_scan(in, g.lane);
+      uint32_t r = seen + incl - in;
+#pragma unroll
+      for (int e = 0; e < V; e++) {
+        const uint32_t key = k[c * V + e];
+        if (key == t) {
+          if (r >= ties) k[c * V + e] = 0u;
+          r++;
+        } else if (key < t) {
+          k[c * V + e] = 0u;
+        }
+      }
+      seen += __shfl_sync(0xffffffffu, incl, 31);
+    }
+  }
+
+  // The temperature and the cuts; afterwards k[e] != 0 exactly for what top-k
+  // and top-p keep (min-p and the dropping are left to the weights' pass).
+  // Returns the open entries before the cuts.
+  __device__ uint32_t cut(const Cut& c, int kind) {
+    uint32_t open = 0, lo = 0xffffffffu, hi = 0u;
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      open += k[e] != 0u;
+      if (k[e]) lo = min(lo, k[e]);
+      hi = max(hi, k[e]);
+    }
+    g.counts(open, lo, hi);
+    plain_p = kind == kKindP && c.inv_t == 1.0;
+    power = kind == kKindP && !plain_p;
+    inv_t = c.inv_t;
+    if (open == 0) { m = log_m = 0.0; return 0; }
+    m = double(value_of(hi));
+    log_m = kind == kKindP ? log64(m) : 0.0;
+    const uint32_t top = hi;
+    if (c.k && c.k < open) {
+      // the largest t with count(k >= t) >= c.k; `above`: count(k > t's bracket)
+      uint32_t cur = top, above = 0, at_lo = open;
+      for (int step = 0; cur != lo; step++) {
+        const uint32_t p = pivot(lo, cur, step, kind);
+        uint32_t n = 0, mn = 0xffffffffu, mx = 0u;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+          if (k[e] >= p) { n++; mn = min(mn, k[e]); }
+          else mx = max(mx, k[e]);
+        }
+        g.counts(n, mn, mx);
+        if (n >= c.k) { lo = mn; at_lo = n; }
+        else { cur = mx; above = n; }
+      }
+      apply(lo, c.k - above, at_lo - above);
+    }
+    if (c.top_p < 1.0) {
+      double part = 0.0;
+#pragma unroll
+      for (int e = 0; e < E; e++)
+        if (__any_sync(0xffffffffu, k[e] != 0u)) part += weight(k[e]);
+      const double goal = c.top_p * g.sum(part);
+      // the largest t with mass(k >= t) >= goal
+      uint32_t cur = top;
+      double above = 0.0;
+      for (int step = 0; cur != lo; step++) {
+        const uint32_t p = pivot(lo, cur, step, kind);
+        double mass = 0.0;
+        uint32_t n = 0, mn = 0xffffffffu, mx = 0u;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+          const bool in = k[e] >= p && k[e] <= cur;
+          if (__any_sync(0xffffffffu, in)) mass += weight(in ? k[e] : 0u);
+          if (k[e] >= p) mn = min(mn, k[e]);
+          else mx = max(mx, k[e]);
+        }
+        mass = above + g.sum(mass);
+        g.counts(n, mn, mx);
+        if (mass >= goal) lo = mn;
+        else { cur = mx; above = mass; }
+      }
+      uint32_t ties = 0, mn = 0xffffffffu, mx = 0u;
+#pragma unroll
+      for (int e = 0; e < E; e++) ties += k[e] == lo;
+      g.counts(ties, mn, mx);
+      const double w = weight(lo);
+      const double need = w > 0.0 ? ceil((goal - above) / w) : 1.0;
+      apply(lo, need < 1.0 ? 1u : need >= double(ties) ? ties : uint32_t(need), ties);
+    }
+    return open;
+  }
+};
+
+template <typename T, int E, int W, int CL>
+__global__ void __launch_bounds__(W == 1 ? 128 : W * 32) k_draw(DrawArg a) {
+  using R = Row<T, E, W, CL>;
+  constexpr int V = R::V;
+  __shared__ typename Group<W, CL>::Shared sh;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t row = W == 1 ? blockIdx.x * 4 + warp : blockIdx.x / CL;
+  if (row >= a.r.rows) return;
+  RowAt at;
+  if (!locate(a.r, a.out_pitch, row, lane, &at)) return;
+  R r(sh, lane, W == 1 ? 0 : warp);
+  const bool fits = at.n <= a.r.row_len && at.n + V - 1 <= R::kCap;
+  const uint32_t n = fits ? uint32_t(at.n) : 0u;
+  const T* in = static_cast<const T*>(a.r.values) + at.in;
+  r.load(in, n, a.r.kind);
+  const Cut c = cut_of(a.c, row);
+  r.cut(c, a.r.kind);
+  // the weights, their prefix sums chunk by chunk in bank order
+  const double floor_w = c.min_p * (r.plain_p ? r.m : 1.0);
+  double incl[R::kChunks], run = 0.0;
+  uint32_t kept = 0, last = 0u;
+#pragma unroll
+  for (int ch = 0; ch < R::kChunks; ch++) {
+    double s = 0.0;
+#pragma unroll
+    for (int e = 0; e < V; e++) {
+      uint32_t& key = r.k[ch * V + e];
+      if (__any_sync(0xffffffffu, key != 0u)) {
+        const double w = r.weight(key);
+        if (!(w > 0.0) || w < floor_w) key = 0u;
+        if (key) {
+          s += w;
+          kept++;
+          last = uint32_t(r.at(ch) + e) + 1u;
+        }
+      }
+    }
+    const double sc = warp_scan(s, lane);
+    incl[ch] = run + sc;
+    run += __shfl_sync(0xffffffffu, sc, 31);
+  }
+  double before;
+  const double z = r.g.sum(lane == 31 ? run : 0.0, &before);
+  // the first entry whose prefix passes u z, or (no u) the first largest
+  uint32_t hit = 0xffffffffu;
+  if (a.uniforms) {
+    // cum > u z by the sign of u z - cum, whose one rounding keeps it: u on an
+    // entry's edge falls where the reals put it
+    const double u = fmin(fmax(a.uniforms[row], 0.0), 1.0);
+#pragma unroll
+    for (int ch = 0; ch < R::kChunks; ch++) {
+      const bool past = fma(u, z, -(before + incl[ch])) < 0.0;
+      if (hit == 0xffffffffu && __any_sync(0xffffffffu, past)) {
+        // the first such lane walks its entries from the prefix ahead of it
+        const int who = __ffs(__ballot_sync(0xffffffffu, past)) - 1;
+        double ws[V], own = 0.0;
+#pragma unroll
+        for (int e = 0; e < V; e++) own += ws[e] = r.weight(r.k[ch * V + e]);
+        double cum = before + (incl[ch] - own);
+        uint32_t found = 0xffffffffu;
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+          cum += ws[e];
+          if (found == 0xffffffffu && r.k[ch * V + e] && fma(u, z, -cum) < 0.0) found = uint32_t(r.at(ch) + e);
+        }
+        if (found == 0xffffffffu) {  // a last bit short: the lane's last kept entry
+#pragma unroll
+          for (int e = 0; e < V; e++)
+            if (r.k[ch * V + e]) found = uint32_t(r.at(ch) + e);
+        }
+        hit = __shfl_sync(0xffffffffu, found, who);
+      }
+    }
+  } else {
+    const uint32_t top = key_of(float(r.m));
+#pragma unroll
+    for (int e = E - 1; e >= 0; e--)
+      if (r.k[e] == top) hit = uint32_t(r.at(e / V) + e % V);
+  }
+  r.g.counts(kept, hit, last);
+  if (kept && hit == 0xffffffffu) hit = last - 1u;
+  // the owner of the entry writes the row's answer
+  const bool lead = r.g.segment() == 0 && lane == 0;
+  if (kept == 0) {
+    if (lead) {
+      if (a.index) a.index[row] = kNone;
+      if (a.logp) a.logp[row] = -INFINITY;
+      if (a.kept) a.kept[row] = 0u;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      const bool mine = uint32_t(r.at(e / V) + e % V) == hit && r.k[e];
+      if (__any_sync(0xffffffffu, mine)) {
+        const double w = r.weight(r.k[e]);
+        if (mine) {
+          if (a.index) a.index[row] = hit;
+          if (a.logp) a.logp[row] = float(log64(w / z));
+        }
+      }
+    }
+    if (lead && a.kept) a.kept[row] = kept;
+  }
+  if (a.p && fits) {
+    const double inv = kept ? 1.0 / z : 0.0;
+    float* out = a.p + at.out;
+#pragma unroll
+    for (int ch = 0; ch < R::kChunks; ch++) {
+      const int i = r.at(ch);
+      alignas(16) float v[V];
+#pragma unroll
+      for (int e = 0; e < V; e++) {
+        const uint32_t key = r.k[ch * V + e];
+        v[e] = 0.0f;
+        if (__any_sync(0xffffffffu, key != 0u)) v[e] = float(r.weight(key) * inv);
+      }
+      if (i >= 0 && i + V <= int(n) && (reinterpret_cast<uintptr_t>(out + i) & 15) == 0) {
+#pragma unroll
+        for (int e = 0; e < V; e += 4) *reinterpret_cast<float4*>(out + i + e) = *reinterpret_cast<float4*>(v + e);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; e++)
+          if (i + e >= 0 && i + e < int(n)) out[i + e] = v[e];
+      }
+    }
+  }
+}
+
+// loss = -A log pi(a) - beta H(pi), H = log Z - sum w x / Z, and
+// dloss/dv_j = (A (pi_j - [j = a]) + beta pi_j (log pi_j + H)) / T for what is
+// kept, 0 elsewhere, times the row's weight.
+template <typename T, int E, int W, int CL>
+__global__ void __launch_bounds__(W == 1 ? 128 : W * 32) k_policy_loss(LossArg a) {
+  using R = Row<T, E, W, CL>;
+  constexpr int V = R::V;
+  __shared__ typename Group<W, CL>::Shared sh;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t row = W == 1 ? blockIdx.x * 4 + warp : blockIdx.x / CL;
+  if (row >= a.r.rows) return;
+  RowAt at;
+  if (!locate(a.r, a.out_pitch, row, lane, &at)) return;
+  R r(sh, lane, W == 1 ? 0 : warp);
+  const bool fits = at.n <= a.r.row_len && at.n + V - 1 <= R::kCap;
+  const uint32_t n = fits ? uint32_t(at.n) : 0u;
+  const T* in = static_cast<const T*>(a.r.values) + at.in;
+  r.load(in, n, kKindScores);
+  const Cut c = cut_of(a.c, row);
+  r.cut(c, kKindScores);
+  const uint32_t act = a.actions[row];
+  const bool asked = act != kNone;
+  double part = 0.0, px = 0.0, xa = 0.0;
+  uint32_t kept = 0, live = 0xffffffffu, dummy = 0u;
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    uint32_t& key = r.k[e];
+    if (__any_sync(0xffffffffu, key != 0u)) {
+      const double w = r.weight(key);
+      if (!(w > 0.0) || w < c.min_p) key = 0u;
+      if (key) {
+        const double x = r.x_of(key);
+        part += w;
+        px = fma(w, x, px);
+        kept++;
+        if (uint32_t(r.at(e / V) + e % V) == act) { live = 0u; xa = x; }
+      }
+    }
+  }
+  const double z = r.g.sum(part);
+  const double sx = r.g.sum(px);
+  xa = r.g.sum(xa);
+  r.g.counts(kept, live, dummy);
+  const double log_z = kept ? log64(z) : 0.0;
+  const double h = kept ? log_z - sx / z : 0.0;
+  const double logp = xa - log_z;
+  // a temperature that is not positive has one answer and no gradient
+  const bool learns = asked && live == 0u && c.inv_t > 0.0;
+  const double adv = double(a.advantage[row]), beta = double(a.beta);
+  const double rw = a.row_weight ? double(a.row_weight[row]) : 1.0;
+  if (r.g.segment() == 0 && lane == 0) {
+    if (a.loss) a.loss[row] = learns ? float(-adv * logp - beta * h) : 0.0f;
+    if (a.logp) a.logp[row] = !asked ? 0.0f : live == 0u ? float(logp) : -INFINITY;
+    if (a.entropy) a.entropy[row] = float(h);
+  }
+  if (!a.grad || !fits) return;
+  T* out = static_cast<T*>(a.grad) + at.out;
+  const double g0 = rw * c.inv_t, inv_z = kept ? 1.0 / z : 0.0, base = h - log_z;
+#pragma unroll
+  for (int ch = 0; ch < R::kChunks; ch++) {
+    const int i = r.at(ch);
+    alignas(16) T v[V];
+#pragma unroll
+    for (int e = 0; e < V; e++) {
+      const uint32_t key = r.k[ch * V + e];
+      double d = 0.0;
+      if (learns && __any_sync(0xffffffffu, key != 0u)) {
+        const double pi = r.weight(key) * inv_z;
+        if (key) {
+          const double one = uint32_t(i + e) == act ? 1.0 : 0.0;
+          d = g0 * fma(adv, pi - one, beta * pi * (r.x_of(key) + base));
+        }
+      }
+      v[e] = from_f32<T>(float(d));
+    }
+    if (i >= 0 && i + V <= int(n) && (reinterpret_cast<uintptr_t>(out + i) & 15) == 0) {
+      *reinterpret_cast<uint4*>(out + i) = *reinterpret_cast<uint4*>(v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; e++)
+        if (i + e >= 0 && i + e < int(n)) out[i + e] = v[e];
+    }
+  }
+}
+
+}  // namespace pol
+}  // namespace kc

@@ -1,0 +1,9 @@
+// policy_bf16.cu — the policy rows of bf16 values.
+#include "policy_launch.cuh"
+
+namespace kc {
+namespace pol {
+cudaError_t draw_bf16(const DrawArg& a, cudaStream_t s) { return draw_as<__nv_bfloat16>(a, s); }
+cudaError_t loss_bf16(const LossArg& a, cudaStream_t s) { return loss_as<__nv_bfloat16>(a, s); }
+}  // namespace pol
+}  // namespace kc

@@ -1,0 +1,9 @@
+// policy_f16.cu — the policy rows of f16 values.
+#include "policy_launch.cuh"
+
+namespace kc {
+namespace pol {
+cudaError_t draw_f16(const DrawArg& a, cudaStream_t s) { return draw_as<__half>(a, s); }
+cudaError_t loss_f16(const LossArg& a, cudaStream_t s) { return loss_as<__half>(a, s); }
+}  // namespace pol
+}  // namespace kc

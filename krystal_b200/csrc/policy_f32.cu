@@ -1,0 +1,9 @@
+// policy_f32.cu — the policy rows of f32 values.
+#include "policy_launch.cuh"
+
+namespace kc {
+namespace pol {
+cudaError_t draw_f32(const DrawArg& a, cudaStream_t s) { return draw_as<float>(a, s); }
+cudaError_t loss_f32(const LossArg& a, cudaStream_t s) { return loss_as<float>(a, s); }
+}  // namespace pol
+}  // namespace kc

@@ -41,6 +41,7 @@ from . import abi
 from .backend import CudaBrainBackend, WeightChanges
 from .frame import FrameBatch, pack_host_frame
 from .model import BrainForwardWeights
+from .policy import GradList, Sampling
 from .session import selection_mask
 
 NO_TARGET = abi.KC_NO_TARGET
@@ -58,6 +59,13 @@ class LearnOptions:
     unfreeze_pool: bool = False
     unfreeze_tokens: bool = False
     token_rate: float = 0.1
+    # Beyond the reference. sampling: the policy the answers were drawn from
+    # (BrainSession.think(sampling=...)), which the update then differentiates;
+    # None: the whole softmax. max_update_norm: the actor's update (selector,
+    # pool and table rows, each with its rate) is scaled down to this global
+    # norm; the critic keeps its own rate.
+    sampling: Sampling | None = None
+    max_update_norm: float = math.inf
 
 
 @dataclass
@@ -83,6 +91,7 @@ class LearnReport:
     update_applied: bool
     rejected: str | None = None
     health: dict = field(default_factory=dict)
+    update_norm: float | None = None  # the actor's global norm before clipping, when max_update_norm asks for it
 
 
 @dataclass
@@ -171,6 +180,11 @@ def apply_update(weights: BrainForwardWeights, sums: np.ndarray, plan: UpdatePla
     hh = h * h
     s_wq, s_wk = sums[:hh], sums[hh:2 * hh]
     s_pool, s_dv = sums[2 * hh:2 * hh + 2 * h], sums[2 * hh + 2 * h:2 * hh + 5 * h]
+    if math.isfinite(options.max_update_norm):
+        parts = [s_wq, s_wk] + ([s_pool] if options.unfreeze_pool else [])
+        norm = math.sqrt(sum(float(np.dot(s, s)) for s in parts))
+        if math.isfinite(norm) and norm > options.max_update_norm:
+            s_wq, s_wk, s_pool = (s * (options.max_update_norm / norm) for s in (s_wq, s_wk, s_pool))
     before = (weights.selector.wq.copy(), weights.selector.wk.copy(), weights.value_head_wv.copy(),
               weights.pool.copy())
     lr = options.learning_rate
@@ -277,6 +291,8 @@ class BatchLearner:
         self.stream = torch.cuda.Stream(device=self.dev)
         self.rows_buf = None  # [table rows * H + table rows] f64: row sums, then touched flags
         self._pinned = {}
+        self.norm = torch.zeros(2, dtype=torch.float64, device=self.dev)  # the update's norm and scale
+        self.clip_list = self.clip_key = None
 
     def _to_device(self, name: str, a: np.ndarray):
         """a host array through a reused pinned buffer, copied without waiting."""
@@ -308,12 +324,15 @@ class BatchLearner:
         cur = torch.cuda.current_stream(self.dev)
         run = cur if cur.cuda_stream else self.stream
         prev = self.be.stream_ptr()
+        prev_policy = self.be.policy
         self.be.set_stream(run.cuda_stream)
         try:
+            self.be.set_policy(options.sampling)
             with torch.cuda.stream(run):
                 return self._step(frames, records, rec_off, token_ids, field_roles, schema_ids, band_ids, rewards,
                                   answered, targets, selection, schema_allow, band_allow, options, global_frames)
         finally:
+            self.be.set_policy(prev_policy)
             self.be.set_stream(prev)
 
     def _step(self, frames, records, rec_off, token_ids, field_roles, schema_ids, band_ids, rewards, answered,
@@ -357,6 +376,8 @@ class BatchLearner:
             dist.all_reduce(self.sums, group=self.group)
             if row_sums is not None:
                 dist.all_reduce(self.rows_buf, group=self.group)
+        if math.isfinite(options.max_update_norm):
+            self._clip(options, row_sums)
         result = self.be.learn_apply(self.sums.data_ptr(), row_sums.data_ptr() if row_sums is not None else None,
                                      touched.data_ptr() if touched is not None else None,
                                      self.report.data_ptr(), opts)
@@ -366,7 +387,24 @@ class BatchLearner:
         health = dict(semantic_embedding_max_abs=float(result[3]), selector_max_abs=float(result[4]),
                       value_max_abs=float(result[5]), pool_max_abs=float(result[6]), finite=bool(result[2]))
         return LearnReport(int(report[0]), float(report[4]), float(report[5]), int(report[2]), int(report[3]),
-                           float(report[6]), float(report[7]), bool(result[0]), rejected, health)
+                           float(report[6]), float(report[7]), bool(result[0]), rejected, health,
+                           float(self.norm[0]) if math.isfinite(options.max_update_norm) else None)
+
+    def _clip(self, options: LearnOptions, row_sums) -> None:
+        """The actor's sums scaled to max_update_norm, in place: after the
+        all-reduce, so every rank finds the same norm."""
+        key = (bool(options.unfreeze_pool), options.token_rate if row_sums is not None else None)
+        if self.clip_key != key:
+            h = self.be.config.hidden_size
+            parts, weights = [self.sums[:2 * h * h]], [1.0]
+            if options.unfreeze_pool:
+                parts.append(self.sums[2 * h * h:2 * h * h + 2 * h])
+                weights.append(1.0)
+            if row_sums is not None:
+                parts.append(row_sums)
+                weights.append(options.token_rate)
+            self.clip_list, self.clip_key = GradList(parts, weights=weights), key
+        self.be.clip_grads(self.clip_list, options.max_update_norm, self.norm.data_ptr())
 
     def _read_back(self, options: LearnOptions, moved: bool) -> None:
         """The host's arrays as the device page left them."""

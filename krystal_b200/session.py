@@ -20,6 +20,7 @@ from .checkpoint import decode_checkpoint, encode_checkpoint
 from .frame import HostFrame, pack_host_frame
 from .model import BRAIN_FORWARD_CONFIG, BrainForwardConfig, BrainForwardWeights, create_brain_forward_weights, \
     validate_brain_forward_weights
+from .policy import Sampling
 
 NEG_INF = np.float32(-1e30)  # forward/oracle.ts:36
 
@@ -67,14 +68,21 @@ class Deliberation:
         self._encoded = encoded
 
     def choose(self, allows: Callable[[int, int], bool] | None = None,
-               sample: Callable[[int], float] | None = None) -> ThinkResult:
+               sample: Callable[[int], float] | None = None, sampling: Sampling | None = None) -> ThinkResult:
+        """Each question's answer under its grammar: the most probable record, or
+        a draw by `sample`. With `sampling` the answer comes from the tempered
+        and cut policy, which is then the distribution reported."""
         active = self.frame.active
         q, r = active.query_records.size, active.bank_records.size
         if self._encoded is None:
             return ThinkResult([], self.frame)
         mask = selection_mask(active, allows)
         uniforms = None if sample is None else np.array([sample(i) for i in range(q)], dtype=np.float64)
-        sel = self._session.backend.select(self._encoded, mask=mask, uniforms=uniforms, gather=False)
+        be = self._session.backend
+        if sampling is None:
+            sel = be.select(self._encoded, mask=mask, uniforms=uniforms, gather=False)
+        else:
+            sel = be.draw_rows(be.select(self._encoded, mask=mask, gather=False).p, q, sampling, uniforms)
         out = []
         for i in range(q):
             chosen = int(sel.index[i])
@@ -102,8 +110,8 @@ class BrainSession:
             return Deliberation(frame, self, None)
         return Deliberation(frame, self, self.backend.encode(frame))
 
-    def think(self, records: Sequence, allows=None, sample=None) -> ThinkResult:
-        return self.consider(records).choose(allows, sample)
+    def think(self, records: Sequence, allows=None, sample=None, sampling: Sampling | None = None) -> ThinkResult:
+        return self.consider(records).choose(allows, sample, sampling)
 
     def learn(self, experiences: Sequence, options=None):
         """session.ts:195-197: one pass over remembered turns (learnFromExperience),
