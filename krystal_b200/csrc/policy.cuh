@@ -83,9 +83,42 @@ __device__ __forceinline__ double exp64(double x, double tab) {
   return __hiloint2double(__double2hiint(s) + ((n >> 5) << 20), __double2loint(s));
 }
 
-// Tempered probabilities take their logarithm here, out of line: the call sits
-// in every loop over a row's entries.
+// log v in 64 bits for a positive f32 v, by a table of 32 mantissa intervals
+// (Tang, "Table-driven implementation of the logarithm function", ACM TOMS
+// 16(4), 1990): v = 2^e m, c_i = 1 / (the middle of m's interval), r = m c_i - 1,
+// |r| <= 1/65, log v = e ln 2 - log c_i + log(1 + r) by its series to r^8
+// (the first term left out is below 6e-18). Lane i holds c_i and -log c_i;
+// every lane of the warp calls this together.
+__device__ __forceinline__ double log_tab(float v, double c, double neg_log_c) {
+  const double d = double(v);
+  const int hi = __double2hiint(d);
+  const int i = (hi >> 15) & 31;
+  const double m = __hiloint2double((hi & 0xfffff) | 0x3ff00000, __double2loint(d));
+  const double ci = __shfl_sync(0xffffffffu, c, i), li = __shfl_sync(0xffffffffu, neg_log_c, i);
+  const double r = fma(m, ci, -1.0);
+  double p = fma(r, -1.0 / 8.0, 1.0 / 7.0);
+  p = fma(r, p, -1.0 / 6.0);
+  p = fma(r, p, 1.0 / 5.0);
+  p = fma(r, p, -1.0 / 4.0);
+  p = fma(r, p, 1.0 / 3.0);
+  p = fma(r, p, -0.5);
+  p = fma(r, p, 1.0);
+  return fma(double((hi >> 20) - 1023), 0.69314718055994530942, fma(r, p, li));
+}
+
+// One logarithm a row or two, out of line.
 static __device__ __noinline__ double log64(double v) { return log(v); }
+
+__device__ __forceinline__ float exp2_fast(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float log2_fast(float v) {
+  float r;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
 
 __device__ __forceinline__ double warp_add(double v) {
 #pragma unroll
@@ -188,6 +221,23 @@ struct Group {
     }
     return v;
   }
+  // The group's sum of one u32 a thread whose warp sums stay below 2^32.
+  __device__ double sum_u32(uint32_t v) {
+    v = __reduce_add_sync(0xffffffffu, v);
+    if constexpr (W > 1 || CL > 1) return sum(lane == 0 ? double(v) : 0.0);
+    return double(v);
+  }
+  // The same, with the minimum and maximum of two more.
+  __device__ double masses(uint32_t add, uint32_t& mn, uint32_t& mx) {
+    if constexpr (W > 1 || CL > 1) {
+      const double v = sum_u32(add);
+      uint32_t none = 0;
+      counts(none, mn, mx);
+      return v;
+    }
+    counts(add, mn, mx);
+    return double(add);
+  }
   // The sum over the warps ahead of this one of a value the warp agrees on.
   __device__ uint32_t ahead(uint32_t v) {
     uint32_t before = 0;
@@ -276,21 +326,48 @@ struct Row {
   static constexpr int V = 16 / int(sizeof(T));
   static constexpr int kChunks = E / V;
   static constexpr uint32_t kCap = uint32_t(32) * E * W * CL;
-  static_assert(E % V == 0, "a thread holds whole vectors");
+  static constexpr bool kCached = E <= 32;  // the registers hold a weight an entry beside the keys
+  static_assert(E % V == 0 && kChunks <= 32, "a thread holds whole vectors");
 
   Group<W, CL> g;
-  uint32_t k[E];  // keys; 0: not in the support
-  double tab;     // 2^{lane/32}
+  uint32_t k[E];   // keys; 0: not in the support
+  uint32_t live;   // chunks of this warp that hold an entry of the support
+  double tab;      // 2^{lane/32}
+  double c_tab, l_tab;  // log_tab's table, for tempered probabilities
   double m, log_m, inv_t;
-  bool power;     // probabilities at a temperature other than 1: x from logarithms
-  bool plain_p;   // probabilities at T = 1: the weights are the values
-  int i0;         // index of this lane's first entry of chunk 0
+  bool power;      // probabilities at a temperature other than 1: x from logarithms
+  bool plain_p;    // probabilities at T = 1: the weights are the values
+  int i0;          // index of this lane's first entry of chunk 0
 
   __device__ Row(typename Group<W, CL>::Shared& sh, int lane, int warp) : g(sh, lane, warp) {
     tab = exp2(double(lane) * (1.0 / 32.0));
+    c_tab = 1.0 / (1.0 + (lane + 0.5) * (1.0 / 32.0));
+    l_tab = 0.0;
   }
 
   __device__ int at(int c) const { return i0 + c * 32 * V; }
+  __device__ uint32_t index(int e) const { return uint32_t(at(e / V) + e % V); }
+
+  // f(entry) for every entry of the chunks that hold any; the warp together.
+  template <typename F>
+  __device__ __forceinline__ void each(F f) {
+#pragma unroll
+    for (int c = 0; c < kChunks; c++)
+      if (live >> c & 1u) {
+#pragma unroll
+        for (int e = 0; e < V; e++) f(c * V + e);
+      }
+  }
+  __device__ void find_live() {
+    live = 0;
+#pragma unroll
+    for (int c = 0; c < kChunks; c++) {
+      uint32_t any = 0;
+#pragma unroll
+      for (int e = 0; e < V; e++) any |= k[c * V + e];
+      if (__any_sync(0xffffffffu, any != 0u)) live |= 1u << c;
+    }
+  }
 
   // Loads n entries from row. A lane's 16-byte loads start on 16-byte
   // boundaries; a vector that reaches past either end of the row is read
@@ -321,19 +398,23 @@ struct Row {
         k[c * V + e] = open ? key_of(fminf(f, 3.402823466e38f)) : 0u;
       }
     }
+    find_live();
   }
 
-  // The tempered log weight, and the weight, of a key in the support.
+  // The tempered log weight of a key in the support (a key outside it: some
+  // number). Every lane of the warp calls this together.
   __device__ double x_of(uint32_t key) const {
-    const double v = double(value_of(key));
-    return power ? (log64(v) - log_m) * inv_t : (v - m) * inv_t;
+    const float v = value_of(key ? key : 0xbf800000u);
+    return power ? (log_tab(v, c_tab, l_tab) - log_m) * inv_t : (double(v) - m) * inv_t;
   }
-  // Every lane of the warp calls this together; 0 for key 0 and for dropped entries.
+  // The weight of an x, and of a key; 0 for key 0 and for dropped entries.
+  __device__ double weight_of(uint32_t key, double x) const {
+    const double w = exp64(fmin(fmax(x, kDropped), 0.0), tab);
+    return key && x >= kDropped ? w : 0.0;
+  }
   __device__ double weight(uint32_t key) const {
     if (plain_p) return key ? double(value_of(key)) : 0.0;
-    const double x = key ? x_of(key) : 0.0;
-    const double w = exp64(fmax(x, kDropped), tab);
-    return key && x >= kDropped ? w : 0.0;
+    return weight_of(key, x_of(key));
   }
 
   // The pivot between two values of the row: halfway in value for scores,
@@ -347,36 +428,71 @@ struct Row {
     return min(max(p, lo + 1), hi);
   }
 
-  // Drops the entries below the cut t and all but the first `ties` at it.
+  // Drops the entries below the cut t and all but the first `ties` of the
+  // `all` at it.
   __device__ void apply(uint32_t t, uint32_t ties, uint32_t all) {
     if (ties >= all) {
+      each([&](int e) { if (k[e] < t) k[e] = 0u; });
+    } else {
+      uint32_t mine = 0;
+      each([&](int e) { mine += k[e] == t; });
+      uint32_t seen = g.ahead(__reduce_add_sync(0xffffffffu, mine));
 #pragma unroll
-      for (int e = 0; e < E; e++)
-        if (k[e] < t) k[e] = 0u;
-      return;
-    }
-    uint32_t mine = 0;
+      for (int c = 0; c < kChunks; c++) {
+        uint32_t in = 0;
 #pragma unroll
-    for (int e = 0; e < E; e++) mine += k[e] == t;
-    uint32_t seen = g.ahead(__reduce_add_sync(0xffffffffu, mine));
+        for (int e = 0; e < V; e++) in += k[c * V + e] == t;
+        const uint32_t incl = warp_scan(in, g.lane);
+        uint32_t r = seen + incl - in;
 #pragma unroll
-    for (int c = 0; c < kChunks; c++) {
-      uint32_t in = 0;
-#pragma unroll
-      for (int e = 0; e < V; e++) in += k[c * V + e] == t;
-      const uint32_t incl = warp_scan(in, g.lane);
-      uint32_t r = seen + incl - in;
-#pragma unroll
-      for (int e = 0; e < V; e++) {
-        const uint32_t key = k[c * V + e];
-        if (key == t) {
-          if (r >= ties) k[c * V + e] = 0u;
-          r++;
-        } else if (key < t) {
-          k[c * V + e] = 0u;
+        for (int e = 0; e < V; e++) {
+          const uint32_t key = k[c * V + e];
+          if (key == t) {
+            if (r >= ties) k[c * V + e] = 0u;
+            r++;
+          } else if (key < t) {
+            k[c * V + e] = 0u;
+          }
         }
+        seen += __shfl_sync(0xffffffffu, incl, 31);
       }
-      seen += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    find_live();
+  }
+
+  // top-p's search by approximate weights: f32 exponentials in units of 2^-20
+  // of the largest, summed as integers. An entry above half a unit has |x| <=
+  // 21 ln 2; three f32 roundings of the exponent and ex2's 2^-22 put its weight
+  // within 3e-6, and for probabilities lg2's 2^-22 of log2 v and of log2 m add
+  // 3.4e-7 (|log2 m| + 21 T) / T. A mass that clears the goal by `err` of the
+  // total and half a unit an entry is on its side for certain; the first pivot
+  // that does not leaves [lo, cur] to the 64-bit search. What it usually
+  // leaves is one value.
+  __device__ void narrow(double top_p, uint32_t open, int kind, uint32_t& lo, uint32_t& cur) {
+    uint32_t q[E], all = 0;
+    const float mv = float(m), it = float(inv_t) * (kind == kKindP ? 1.0f : 1.44269504f);
+    const float mu = kind == kKindP ? log2_fast(mv) : mv;
+    each([&](int e) {
+      const float v = value_of(k[e] ? k[e] : 0xbf800000u);
+      const float u = ((kind == kKindP ? log2_fast(v) : v) - mu) * it;
+      q[e] = k[e] ? __float2uint_rn(exp2_fast(fminf(u, 0.0f)) * 1048576.0f) : 0u;
+      all += q[e];
+    });
+    const double total = g.sum_u32(all);
+    const double goal = top_p * total;
+    const double err = (1e-5 + 1e-5 * inv_t + 4e-7 * fabs(double(mu)) * (kind == kKindP ? inv_t : 0.0)) * total +
+                       0.5 * open + 1.0;
+    for (int step = 0; cur != lo; step++) {
+      const uint32_t p = pivot(lo, cur, step, kind);
+      uint32_t mass = 0, mn = 0xffffffffu, mx = 0u;
+      each([&](int e) {
+        if (k[e] >= p) { mass += q[e]; mn = min(mn, k[e]); }
+        else mx = max(mx, k[e]);
+      });
+      const double a = g.masses(mass, mn, mx);
+      if (a >= goal + err) lo = mn;
+      else if (a < goal - err) cur = mx;
+      else return;
     }
   }
 
@@ -385,69 +501,82 @@ struct Row {
   // Returns the open entries before the cuts.
   __device__ uint32_t cut(const Cut& c, int kind) {
     uint32_t open = 0, lo = 0xffffffffu, hi = 0u;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
+    each([&](int e) {
       open += k[e] != 0u;
       if (k[e]) lo = min(lo, k[e]);
       hi = max(hi, k[e]);
-    }
+    });
     g.counts(open, lo, hi);
     plain_p = kind == kKindP && c.inv_t == 1.0;
     power = kind == kKindP && !plain_p;
     inv_t = c.inv_t;
     if (open == 0) { m = log_m = 0.0; return 0; }
     m = double(value_of(hi));
-    log_m = kind == kKindP ? log64(m) : 0.0;
+    log_m = 0.0;
+    if (power) {
+      l_tab = -log64(c_tab);
+      log_m = log_tab(value_of(hi), c_tab, l_tab);
+    }
     const uint32_t top = hi;
+    uint32_t left = open;
     if (c.k && c.k < open) {
       // the largest t with count(k >= t) >= c.k; `above`: count(k > t's bracket)
       uint32_t cur = top, above = 0, at_lo = open;
       for (int step = 0; cur != lo; step++) {
         const uint32_t p = pivot(lo, cur, step, kind);
         uint32_t n = 0, mn = 0xffffffffu, mx = 0u;
-#pragma unroll
-        for (int e = 0; e < E; e++) {
+        each([&](int e) {
           if (k[e] >= p) { n++; mn = min(mn, k[e]); }
           else mx = max(mx, k[e]);
-        }
+        });
         g.counts(n, mn, mx);
         if (n >= c.k) { lo = mn; at_lo = n; }
         else { cur = mx; above = n; }
       }
       apply(lo, c.k - above, at_lo - above);
+      left = c.k;
     }
     if (c.top_p < 1.0) {
-      double part = 0.0;
-#pragma unroll
-      for (int e = 0; e < E; e++)
-        if (__any_sync(0xffffffffu, k[e] != 0u)) part += weight(k[e]);
-      const double goal = c.top_p * g.sum(part);
       // the largest t with mass(k >= t) >= goal
       uint32_t cur = top;
-      double above = 0.0;
-      for (int step = 0; cur != lo; step++) {
-        const uint32_t p = pivot(lo, cur, step, kind);
-        double mass = 0.0;
-        uint32_t n = 0, mn = 0xffffffffu, mx = 0u;
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-          const bool in = k[e] >= p && k[e] <= cur;
-          if (__any_sync(0xffffffffu, in)) mass += weight(in ? k[e] : 0u);
-          if (k[e] >= p) mn = min(mn, k[e]);
-          else mx = max(mx, k[e]);
-        }
-        mass = above + g.sum(mass);
-        g.counts(n, mn, mx);
-        if (mass >= goal) lo = mn;
-        else { cur = mx; above = mass; }
-      }
+      if constexpr (kCached) narrow(c.top_p, left, kind, lo, cur);
       uint32_t ties = 0, mn = 0xffffffffu, mx = 0u;
-#pragma unroll
-      for (int e = 0; e < E; e++) ties += k[e] == lo;
+      each([&](int e) { ties += k[e] == lo; });
       g.counts(ties, mn, mx);
-      const double w = weight(lo);
-      const double need = w > 0.0 ? ceil((goal - above) / w) : 1.0;
-      apply(lo, need < 1.0 ? 1u : need >= double(ties) ? ties : uint32_t(need), ties);
+      if (cur != lo || ties > 1) {
+        double part = 0.0, over = 0.0;
+        each([&](int e) {
+          const double w = weight(k[e]);
+          part += w;
+          if (k[e] > cur) over += w;
+        });
+        const double goal = c.top_p * g.sum(part);
+        double above = g.sum(over);
+        for (int step = 0; cur != lo; step++) {
+          const uint32_t p = pivot(lo, cur, step, kind);
+          double mass = 0.0;
+          uint32_t n = 0;
+          mn = 0xffffffffu, mx = 0u;
+          each([&](int e) {
+            const bool in = k[e] >= p && k[e] <= cur;
+            if (__any_sync(0xffffffffu, in)) mass += weight(in ? k[e] : 0u);
+            if (k[e] >= p) mn = min(mn, k[e]);
+            else mx = max(mx, k[e]);
+          });
+          mass = above + g.sum(mass);
+          g.counts(n, mn, mx);
+          if (mass >= goal) lo = mn;
+          else { cur = mx; above = mass; }
+        }
+        ties = 0, mn = 0xffffffffu, mx = 0u;
+        each([&](int e) { ties += k[e] == lo; });
+        g.counts(ties, mn, mx);
+        const double w = weight(lo);
+        const double need = w > 0.0 ? ceil((goal - above) / w) : 1.0;
+        apply(lo, need < 1.0 ? 1u : need >= double(ties) ? ties : uint32_t(need), ties);
+      } else {
+        apply(lo, 1u, 1u);
+      }
     }
     return open;
   }
@@ -472,28 +601,33 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) k_draw(DrawArg a) {
   r.cut(c, a.r.kind);
   // the weights, their prefix sums chunk by chunk in bank order
   const double floor_w = c.min_p * (r.plain_p ? r.m : 1.0);
-  double incl[R::kChunks], run = 0.0;
+  double incl[R::kChunks], w[R::kCached ? E : 1], run = 0.0;
   uint32_t kept = 0, last = 0u;
 #pragma unroll
   for (int ch = 0; ch < R::kChunks; ch++) {
+    incl[ch] = run;
+    if (!(r.live >> ch & 1u)) continue;
     double s = 0.0;
 #pragma unroll
-    for (int e = 0; e < V; e++) {
-      uint32_t& key = r.k[ch * V + e];
-      if (__any_sync(0xffffffffu, key != 0u)) {
-        const double w = r.weight(key);
-        if (!(w > 0.0) || w < floor_w) key = 0u;
-        if (key) {
-          s += w;
-          kept++;
-          last = uint32_t(r.at(ch) + e) + 1u;
-        }
+    for (int e = ch * V; e < ch * V + V; e++) {
+      double we = r.weight(r.k[e]);
+      if (we < floor_w) we = 0.0;
+      if (!(we > 0.0)) r.k[e] = 0u;
+      if constexpr (R::kCached) w[e] = we;
+      s += we;
+      if (r.k[e]) {
+        kept++;
+        last = r.index(e) + 1u;
       }
     }
     const double sc = warp_scan(s, lane);
     incl[ch] = run + sc;
     run += __shfl_sync(0xffffffffu, sc, 31);
   }
+  auto weight = [&](int e) {
+    if constexpr (R::kCached) return w[e];
+    else return r.weight(r.k[e]);
+  };
   double before;
   const double z = r.g.sum(lane == 31 ? run : 0.0, &before);
   // the first entry whose prefix passes u z, or (no u) the first largest
@@ -504,24 +638,24 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) k_draw(DrawArg a) {
     const double u = fmin(fmax(a.uniforms[row], 0.0), 1.0);
 #pragma unroll
     for (int ch = 0; ch < R::kChunks; ch++) {
-      const bool past = fma(u, z, -(before + incl[ch])) < 0.0;
+      const bool past = (r.live >> ch & 1u) && fma(u, z, -(before + incl[ch])) < 0.0;
       if (hit == 0xffffffffu && __any_sync(0xffffffffu, past)) {
         // the first such lane walks its entries from the prefix ahead of it
         const int who = __ffs(__ballot_sync(0xffffffffu, past)) - 1;
         double ws[V], own = 0.0;
 #pragma unroll
-        for (int e = 0; e < V; e++) own += ws[e] = r.weight(r.k[ch * V + e]);
+        for (int e = 0; e < V; e++) own += ws[e] = weight(ch * V + e);
         double cum = before + (incl[ch] - own);
         uint32_t found = 0xffffffffu;
 #pragma unroll
         for (int e = 0; e < V; e++) {
           cum += ws[e];
-          if (found == 0xffffffffu && r.k[ch * V + e] && fma(u, z, -cum) < 0.0) found = uint32_t(r.at(ch) + e);
+          if (found == 0xffffffffu && r.k[ch * V + e] && fma(u, z, -cum) < 0.0) found = r.index(ch * V + e);
         }
         if (found == 0xffffffffu) {  // a last bit short: the lane's last kept entry
 #pragma unroll
           for (int e = 0; e < V; e++)
-            if (r.k[ch * V + e]) found = uint32_t(r.at(ch) + e);
+            if (r.k[ch * V + e]) found = r.index(ch * V + e);
         }
         hit = __shfl_sync(0xffffffffu, found, who);
       }
@@ -530,7 +664,7 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) k_draw(DrawArg a) {
     const uint32_t top = key_of(float(r.m));
 #pragma unroll
     for (int e = E - 1; e >= 0; e--)
-      if (r.k[e] == top) hit = uint32_t(r.at(e / V) + e % V);
+      if (r.k[e] == top) hit = r.index(e);
   }
   r.g.counts(kept, hit, last);
   if (kept && hit == 0xffffffffu) hit = last - 1u;
@@ -543,17 +677,16 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) k_draw(DrawArg a) {
       if (a.kept) a.kept[row] = 0u;
     }
   } else {
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-      const bool mine = uint32_t(r.at(e / V) + e % V) == hit && r.k[e];
+    r.each([&](int e) {
+      const bool mine = r.index(e) == hit && r.k[e];
       if (__any_sync(0xffffffffu, mine)) {
-        const double w = r.weight(r.k[e]);
+        const double we = weight(e);
         if (mine) {
           if (a.index) a.index[row] = hit;
-          if (a.logp) a.logp[row] = float(log64(w / z));
+          if (a.logp) a.logp[row] = float(log64(we / z));
         }
       }
-    }
+    });
     if (lead && a.kept) a.kept[row] = kept;
   }
   if (a.p && fits) {
@@ -565,9 +698,8 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) k_draw(DrawArg a) {
       alignas(16) float v[V];
 #pragma unroll
       for (int e = 0; e < V; e++) {
-        const uint32_t key = r.k[ch * V + e];
         v[e] = 0.0f;
-        if (__any_sync(0xffffffffu, key != 0u)) v[e] = float(r.weight(key) * inv);
+        if (r.live >> ch & 1u) v[e] = float(weight(ch * V + e) * inv);
       }
       if (i >= 0 && i + V <= int(n) && (reinterpret_cast<uintptr_t>(out + i) & 15) == 0) {
 #pragma unroll
@@ -605,21 +737,21 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) k_policy_loss(LossArg a
   const bool asked = act != kNone;
   double part = 0.0, px = 0.0, xa = 0.0;
   uint32_t kept = 0, live = 0xffffffffu, dummy = 0u;
-#pragma unroll
-  for (int e = 0; e < E; e++) {
+  double ws[R::kCached ? E : 1];
+  r.each([&](int e) {
     uint32_t& key = r.k[e];
-    if (__any_sync(0xffffffffu, key != 0u)) {
-      const double w = r.weight(key);
-      if (!(w > 0.0) || w < c.min_p) key = 0u;
-      if (key) {
-        const double x = r.x_of(key);
-        part += w;
-        px = fma(w, x, px);
-        kept++;
-        if (uint32_t(r.at(e / V) + e % V) == act) { live = 0u; xa = x; }
-      }
+    const double x = r.x_of(key);
+    double w = r.weight_of(key, x);
+    if (w < c.min_p) w = 0.0;
+    if (!(w > 0.0)) key = 0u;
+    if constexpr (R::kCached) ws[e] = w;
+    part += w;
+    px = fma(w, key ? x : 0.0, px);
+    if (key) {
+      kept++;
+      if (r.index(e) == act) { live = 0u; xa = x; }
     }
-  }
+  });
   const double z = r.g.sum(part);
   const double sx = r.g.sum(px);
   xa = r.g.sum(xa);
@@ -647,12 +779,13 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) k_policy_loss(LossArg a
     for (int e = 0; e < V; e++) {
       const uint32_t key = r.k[ch * V + e];
       double d = 0.0;
-      if (learns && __any_sync(0xffffffffu, key != 0u)) {
-        const double pi = r.weight(key) * inv_z;
-        if (key) {
-          const double one = uint32_t(i + e) == act ? 1.0 : 0.0;
-          d = g0 * fma(adv, pi - one, beta * pi * (r.x_of(key) + base));
-        }
+      if (learns && (r.live >> ch & 1u)) {
+        const double x = r.x_of(key);
+        double pi;
+        if constexpr (R::kCached) pi = ws[ch * V + e] * inv_z;
+        else pi = r.weight_of(key, x) * inv_z;
+        const double one = uint32_t(i + e) == act ? 1.0 : 0.0;
+        if (key) d = g0 * fma(adv, pi - one, beta * pi * (x + base));
       }
       v[e] = from_f32<T>(float(d));
     }

@@ -32,18 +32,22 @@ cudaError_t go(void (*kernel)(A), const A& a, int w, int cl, cudaStream_t stream
 template <typename T>
 inline cudaError_t draw_as(const DrawArg& a, cudaStream_t s) {
   const uint64_t need = a.r.row_len + 16 / sizeof(T) - 1;
+  constexpr int kMid = sizeof(T) == 4 ? 20 : 24;  // the largest bank, misaligned, in 8 warps
   if (need <= 256) return go(k_draw<T, 8, 1, 1>, a, 1, 1, s);
   if (need <= 1024) return go(k_draw<T, 32, 1, 1>, a, 1, 1, s);
-  if (need <= 8192) return go(k_draw<T, 32, 8, 1>, a, 8, 1, s);
+  if (need <= 8 * 32 * kMid) return go(k_draw<T, kMid, 8, 1>, a, 8, 1, s);
+  if (need <= 16384) return go(k_draw<T, 32, 16, 1>, a, 16, 1, s);
   if (need <= 32768) return go(k_draw<T, 64, 16, 1>, a, 16, 1, s);
   return go(k_draw<T, 64, 16, 8>, a, 16, 8, s);
 }
 template <typename T>
 inline cudaError_t loss_as(const LossArg& a, cudaStream_t s) {
   const uint64_t need = a.r.row_len + 16 / sizeof(T) - 1;
+  constexpr int kMid = sizeof(T) == 4 ? 20 : 24;
   if (need <= 256) return go(k_policy_loss<T, 8, 1, 1>, a, 1, 1, s);
   if (need <= 1024) return go(k_policy_loss<T, 32, 1, 1>, a, 1, 1, s);
-  if (need <= 8192) return go(k_policy_loss<T, 32, 8, 1>, a, 8, 1, s);
+  if (need <= 8 * 32 * kMid) return go(k_policy_loss<T, kMid, 8, 1>, a, 8, 1, s);
+  if (need <= 16384) return go(k_policy_loss<T, 32, 16, 1>, a, 16, 1, s);
   if (need <= 32768) return go(k_policy_loss<T, 64, 16, 1>, a, 16, 1, s);
   return go(k_policy_loss<T, 64, 16, 8>, a, 16, 8, s);
 }
