@@ -799,5 +799,241 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) k_policy_loss(LossArg a
   }
 }
 
+// ---------------------------------------------------------------------------
+// The policy loss over the whole softmax, nothing cut: no decision hangs on a
+// last bit, so the row stays as it was loaded (NV 16-byte vectors a thread) and
+// its exponentials are f32. With u_j = (v_j - m) log2(e) / T, taken as one
+// fma of v_j (the rounding of m log2(e) / T is common to all and cancels),
+//   Z = sum 2^u, S = sum 2^u u, log pi_j = ln 2 (u_j - log2 Z),
+//   H = ln 2 (log2 Z - S / Z), and the gradient is
+//   2^u_j (u_j B + C) with B = g beta ln 2 / (T Z), C = g (A + beta (H - ln Z)) / (T Z)
+// but for -g A / T more at the action. Sums: four f32 partial sums of at most
+// 16 terms a thread, joined in 64 bits. Arithmetic on pairs (f32x2).
+//
+// Masked entries need no test where they vanish by themselves: NaN and what
+// lies below the mask's floor is raised to it as the row is loaded, and 2^u is
+// 0 if (m - floor) log2(e) / T >= 200. A row where that does not hold (a
+// largest score near the floor, f16 at a temperature of hundreds), that holds
+// +infinity, or whose m log2(e) / T is 1e5 or more (its rounding, 2^-24 of it,
+// would not stay far below 1) tests every entry and subtracts m first.
+// ---------------------------------------------------------------------------
+struct Pair { float x, y; };
+__device__ __forceinline__ unsigned long long pack2(float x, float y) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ Pair unpack2(unsigned long long v) {
+  Pair p;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(p.x), "=f"(p.y) : "l"(v));
+  return p;
+}
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// What masked entries are raised to: a value of the type at or below open_above.
+template <typename T> struct Floor { static constexpr float value = -1.00025555e30f; };  // a bf16 value
+template <> struct Floor<__half> { static constexpr float value = -65504.0f; };
+
+
+// Raises a vector's entries to the floor (a NaN too) and takes their largest into mx.
+__device__ __forceinline__ void raise(float* v, float& mx) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    v[e] = fmaxf(v[e], Floor<float>::value);
+    mx = fmaxf(mx, v[e]);
+  }
+}
+template <typename T, typename T2>
+__device__ __forceinline__ void raise_pairs(T2* v, T2 floor2, float& mx) {
+  T2 top = floor2;
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    v[e] = __hmax2(v[e], floor2);
+    top = __hmax2(top, v[e]);
+  }
+  mx = fmaxf(mx, fmaxf(as_f32(T(top.x)), as_f32(T(top.y))));
+}
+__device__ __forceinline__ void raise(__half* v, float& mx) {
+  raise_pairs<__half>(reinterpret_cast<__half2*>(v), __float2half2_rn(Floor<__half>::value), mx);
+}
+__device__ __forceinline__ void raise(__nv_bfloat16* v, float& mx) {
+  raise_pairs<__nv_bfloat16>(reinterpret_cast<__nv_bfloat162*>(v), __float2bfloat162_rn(Floor<__nv_bfloat16>::value), mx);
+}
+__device__ __forceinline__ void store2(float* d, Pair r) { d[0] = r.x; d[1] = r.y; }
+__device__ __forceinline__ void store2(__half* d, Pair r) {
+  *reinterpret_cast<__half2*>(d) = __floats2half2_rn(r.x, r.y);
+}
+__device__ __forceinline__ void store2(__nv_bfloat16* d, Pair r) {
+  *reinterpret_cast<__nv_bfloat162*>(d) = __floats2bfloat162_rn(r.x, r.y);
+}
+
+template <typename T, int NV, int W, int CL>
+__global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W == 16 ? 2 : 1) k_policy_whole(LossArg a) {
+  constexpr int V = 16 / int(sizeof(T));
+  constexpr uint32_t kCap = uint32_t(32) * V * NV * W * CL;
+  __shared__ typename Group<W, CL>::Shared sh;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t row = W == 1 ? blockIdx.x * 4 + warp : blockIdx.x / CL;
+  if (row >= a.r.rows) return;
+  RowAt at;
+  if (!locate(a.r, a.out_pitch, row, lane, &at)) return;
+  Group<W, CL> g(sh, lane, W == 1 ? 0 : warp);
+  const bool fits = at.n <= a.r.row_len && at.n + V - 1 <= kCap;
+  const int n = fits ? int(at.n) : 0;
+  const T* in = static_cast<const T*>(a.r.values) + at.in;
+  const int shift = int((reinterpret_cast<uintptr_t>(in) & 15) / sizeof(T));
+  const int i0 = g.segment() * 32 * V * NV + lane * V - shift;
+  constexpr float floor_v = Floor<T>::value;
+
+  // the row, masked entries raised to the floor; its largest
+  alignas(16) T v[NV][V];
+  float mx = -INFINITY;
+#pragma unroll
+  for (int c = 0; c < NV; c++) {
+    const int i = i0 + c * 32 * V;
+    if (i >= 0 && i + V <= n) {
+      *reinterpret_cast<uint4*>(v[c]) = __ldcs(reinterpret_cast<const uint4*>(in + i));
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; e++) v[c][e] = i + e >= 0 && i + e < n ? in[i + e] : from_f32<T>(floor_v);
+    }
+    raise(v[c], mx);
+  }
+  // the action's value, before anything is written: grad may lie over values
+  const uint32_t act = a.actions[row];
+  const bool asked = act != kNone;
+  const float va = act < uint32_t(n) ? as_f32(in[act]) : floor_v;
+  uint32_t none = 0, mn = mx == INFINITY ? 0u : 1u, top = key_of(fminf(mx, 3.402823466e38f));
+  g.counts(none, mn, top);  // mn 0: the row holds +infinity
+  const float m = value_of(top);
+  const float t_row = a.c.row_temperature ? a.c.row_temperature[row] : a.c.temperature;
+  const double inv_t = t_row > 0.0f ? 1.0 / double(t_row) : 0.0;
+  const float sc = float(inv_t * 1.4426950408889634074);  // log2(e) / T
+  const bool any = m > Lowest<T>::open_above;
+  const bool open_t = t_row > 0.0f;
+  const bool plain = mn != 0u && (m - Lowest<T>::open_above) * sc >= 200.0f && fabsf(m * sc) < 1e5f && sc < 1e6f;
+  const float off = -m * sc;
+  auto u_of = [&](float f) { return plain ? fmaf(f, sc, off) : (fminf(f, m) - m) * sc; };
+
+  // Z and S
+  double z = 0.0, s = 0.0;
+  if (plain) {
+    const unsigned long long sc2 = pack2(sc, sc), off2 = pack2(off, off);
+    unsigned long long za[2] = {0ull, 0ull}, sa[2] = {0ull, 0ull};
+#pragma unroll
+    for (int c = 0; c < NV; c++)
+#pragma unroll
+      for (int e = 0; e < V; e += 2) {
+        const unsigned long long u = fma2(pack2(as_f32(v[c][e]), as_f32(v[c][e + 1])), sc2, off2);
+        const Pair up = unpack2(u);
+        const unsigned long long w = pack2(exp2_fast(up.x), exp2_fast(up.y));
+        za[(e >> 1) & 1] = add2(za[(e >> 1) & 1], w);
+        sa[(e >> 1) & 1] = fma2(w, u, sa[(e >> 1) & 1]);
+      }
+    const Pair z0 = unpack2(za[0]), z1 = unpack2(za[1]), s0 = unpack2(sa[0]), s1 = unpack2(sa[1]);
+    z = (double(z0.x) + double(z0.y)) + (double(z1.x) + double(z1.y));
+    s = (double(s0.x) + double(s0.y)) + (double(s1.x) + double(s1.y));
+  } else if (any) {
+#pragma unroll
+    for (int c = 0; c < NV; c++)
+#pragma unroll
+      for (int e = 0; e < V; e++) {
+        const float f = as_f32(v[c][e]);
+        if (f > Lowest<T>::open_above) {
+          const float u = fmaxf(u_of(f), -2000.0f), w = exp2_fast(u);
+          z += double(w);
+          s += double(w) * double(u);
+        }
+      }
+  }
+  z = g.sum(z);
+  s = g.sum(s);
+
+  // the row's answer
+  const float ua = u_of(fminf(va, 3.402823466e38f));
+  bool live = asked && va > Lowest<T>::open_above && double(ua) * 0.69314718055994530942 >= kDropped;
+  if (!open_t) {  // temperature 0: the first largest entry alone
+    uint32_t first = 0xffffffffu;
+#pragma unroll
+    for (int c = 0; c < NV; c++)
+#pragma unroll
+      for (int e = 0; e < V; e++)
+        if (fminf(as_f32(v[c][e]), 3.402823466e38f) == m) first = min(first, uint32_t(i0 + c * 32 * V + e));
+    uint32_t zero = 0;
+    none = 0;
+    g.counts(none, first, zero);
+    live = asked && any && first == act;
+  }
+  const double lg_z = any ? log2(z) : 0.0;
+  const double h = any && open_t ? 0.69314718055994530942 * (lg_z - s / z) : 0.0;
+  const double logp = open_t ? 0.69314718055994530942 * (double(ua) - lg_z) : 0.0;
+  const bool learns = asked && live && open_t;
+  const double adv = double(a.advantage[row]), beta = double(a.beta);
+  const double gt = (a.row_weight ? double(a.row_weight[row]) : 1.0) * inv_t;
+  if (g.segment() == 0 && lane == 0) {
+    if (a.loss) a.loss[row] = learns ? float(-adv * logp - beta * h) : 0.0f;
+    if (a.logp) a.logp[row] = !asked ? 0.0f : live ? float(logp) : -INFINITY;
+    if (a.entropy) a.entropy[row] = float(h);
+  }
+  if (!a.grad || !fits) return;
+  T* out = static_cast<T*>(a.grad) + at.out;
+  const double over = learns ? gt / z : 0.0;
+  const float B = float(over * beta * 0.69314718055994530942);
+  const float C = float(over * (adv + beta * (h - 0.69314718055994530942 * lg_z)));
+  const bool quick = plain && fabsf(B) < 10.0f;
+  const unsigned long long sc2 = pack2(sc, sc), off2 = pack2(off, off), B2 = pack2(B, B), C2 = pack2(C, C);
+#pragma unroll
+  for (int c = 0; c < NV; c++) {
+    const int i = i0 + c * 32 * V;
+    alignas(16) T d[V];
+    if (quick) {
+#pragma unroll
+      for (int e = 0; e < V; e += 2) {
+        const unsigned long long u = fma2(pack2(as_f32(v[c][e]), as_f32(v[c][e + 1])), sc2, off2);
+        const Pair up = unpack2(u);
+        const Pair r = unpack2(mul2(pack2(exp2_fast(up.x), exp2_fast(up.y)), fma2(u, B2, C2)));
+        store2(d + e, r);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; e++) {
+        const float f = as_f32(v[c][e]), u = fmaxf(u_of(f), -2000.0f);
+        d[e] = from_f32<T>(learns && f > Lowest<T>::open_above ? exp2_fast(u) * fmaf(u, B, C) : 0.0f);
+      }
+    }
+    // the action's entry, and its lane's alone, gets the rest
+    if (learns && act - uint32_t(i) < uint32_t(V)) {
+#pragma unroll
+      for (int e = 0; e < V; e++)
+        if (uint32_t(i + e) == act) {
+          const double x = 0.69314718055994530942 * double(ua);
+          const double pi = exp(x - 0.69314718055994530942 * lg_z);
+          d[e] = from_f32<T>(float(gt * fma(adv, pi - 1.0, beta * pi * (logp + h))));
+        }
+    }
+    if (i >= 0 && i + V <= n && (reinterpret_cast<uintptr_t>(out + i) & 15) == 0) {
+      *reinterpret_cast<uint4*>(out + i) = *reinterpret_cast<uint4*>(d);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; e++)
+        if (i + e >= 0 && i + e < n) out[i + e] = d[e];
+    }
+  }
+}
+
 }  // namespace pol
 }  // namespace kc

@@ -41,7 +41,22 @@ inline cudaError_t draw_as(const DrawArg& a, cudaStream_t s) {
   return go(k_draw<T, 64, 16, 8>, a, 16, 8, s);
 }
 template <typename T>
+inline cudaError_t whole_as(const LossArg& a, cudaStream_t s) {
+  constexpr int V = 16 / sizeof(T);
+  const uint64_t need = a.r.row_len + V - 1;
+  if (need <= 256) return go(k_policy_whole<T, 8 / V, 1, 1>, a, 1, 1, s);
+  if (need <= 1024) return go(k_policy_whole<T, 32 / V, 1, 1>, a, 1, 1, s);
+  if (need <= 6144) return go(k_policy_whole<T, 24 / V, 8, 1>, a, 8, 1, s);
+  if (need <= 16384) return go(k_policy_whole<T, 32 / V, 16, 1>, a, 16, 1, s);
+  constexpr int W = V == 4 ? 32 : 16;  // 8 vectors a thread
+  if (need <= 32768) return go(k_policy_whole<T, 8, W, 1>, a, W, 1, s);
+  return go(k_policy_whole<T, 8, W, 8>, a, W, 8, s);
+}
+template <typename T>
 inline cudaError_t loss_as(const LossArg& a, cudaStream_t s) {
+  const CutArg& c = a.c;
+  if (!c.top_k && !c.row_top_k && !(c.top_p < 1.0f) && !c.row_top_p && !(c.min_p > 0.0f) && !c.row_min_p)
+    return whole_as<T>(a, s);
   const uint64_t need = a.r.row_len + 16 / sizeof(T) - 1;
   constexpr int kMid = sizeof(T) == 4 ? 20 : 24;
   if (need <= 256) return go(k_policy_loss<T, 8, 1, 1>, a, 1, 1, s);

@@ -8,6 +8,15 @@ covered by a factor of 1.001, values below f32's normal range by 2^-149. A
 log probability is a difference of numbers up to 700, exact to about 1e-12.
 Gradients: half a step of their type of the value; the terms that cancel in
 it are 64-bit, below 1e-12 of the largest.
+
+Where nothing is cut, the loss works in f32 (whole_tolerances). A weight 2^u
+is off by ex2's 2^-22 and by one rounding of u, |u| ln 2 2^-24, of itself; a
+partial sum has at most 16 terms, 2^-20. The mean of |u| under pi is at most
+L = log2 n (H <= ln n), so Z is within 2^-20 + 2^-22 + 0.7 2^-24 L < 2^-19 of
+itself for L <= 18, and log Z within 2^-18. log pi(a) adds its own u's
+rounding, 2^-24 of it; H = ln 2 (log2 Z - S / Z) has S / Z within 2^-18 of
+at most L + 2, and 0.7 2^-24 E[u^2] <= 2^-24 (L + 2)^2 < 2^-19 (L + 2) on top.
+A gradient is pi's error of its terms, and H's.
 """
 import numpy as np
 import pytest
@@ -76,7 +85,7 @@ def near(got, want, half, tiny=0.0):
     got, want = np.asarray(got, np.float64), np.asarray(want, np.float64)
     inf = np.isinf(want)
     assert np.array_equal(got[inf], want[inf])
-    got, want = got[~inf], want[~inf]
+    got, want, tiny = got[~inf], want[~inf], np.broadcast_to(tiny, want.shape)[~inf]
     bad = ~(np.abs(got - want) <= half * 1.001 * np.abs(want) + tiny)
     assert not bad.any(), (got[bad][:4], want[bad][:4])
 
@@ -349,6 +358,11 @@ def test_policy_loss(be, n, dtype):
         for i in range(rows):
             row = ref.policy(wide(v[i]), t, k, p, mp, f16=dtype == "f16")
             L, l, e, g = ref.loss(row, n, int(act[i]), float(adv[i]), float(np.float32(beta)), t, float(w[i]))
+            if c in (0, 3):
+                stat, part = whole_tolerances(row, n, float(adv[i]), beta, float(w[i]) / t, l)
+                near([float(lo[i]), float(lp[i]), float(h[i])], [L, l, e], HALF["f32"], stat)
+                near(got[i], g, HALF[dtype], TINY[dtype] + part)
+                continue
             near([float(lo[i]), float(lp[i]), float(h[i])], [L, l, e], HALF["f32"], 1e-11 * (1 + abs(float(adv[i]))))
             size = (abs(float(adv[i])) + beta * (np.log(n) + 1)) * float(w[i]) / t  # of the terms that cancel
             near(got[i], g, HALF[dtype], TINY[dtype] + 1e-11 * size)
@@ -357,6 +371,64 @@ def test_policy_loss(be, n, dtype):
                        grad_pitch=src.pitch)
         be.synchronize()
         assert bool((src.view() == grad.view()).all()) and src.rest_untouched()
+
+
+def whole_tolerances(row, n, adv, beta, scale, logp):
+    """What f32 weights add to half a step: of (loss, logp, entropy), and of each gradient."""
+    j, pi, logpi = row
+    h = -float((pi * logpi).sum()) if j.size else 0.0
+    logp = logp if np.isfinite(logp) else 0.0
+    e_logp, e_h = 2.0 ** -18 + 2.0 ** -22 * abs(logp), 2.0 ** -17 * (np.log2(n) + 2)
+    part = np.zeros(n)
+    part[j] = scale * pi * ((abs(adv) + beta * (np.abs(logpi) + h)) * (2.0 ** -17 + 2.0 ** -22 * np.abs(logpi))
+                            + beta * e_h)
+    return np.array([abs(adv) * e_logp + beta * e_h, e_logp, e_h]), part
+
+
+def whole_loss(be, v, dtype, act, adv, beta, temps):
+    """The uncut loss of v with a temperature a row, against the plain form."""
+    rows, n = v.shape
+    dv, dt = v.cuda(), on_gpu(np.asarray(temps, np.float32))
+    da, dadv = on_gpu(np.asarray(act, np.int32)), on_gpu(np.asarray(adv, np.float32))
+    lo, lp, h = (torch.zeros(rows, device="cuda") for _ in range(3))
+    grad = torch.zeros_like(dv)
+    torch.cuda.synchronize()
+    be.policy_loss(policy.dense_rows(dv.data_ptr(), dtype, rows, n), policy.Sampling(row_temperature=dt.data_ptr()),
+                   da.data_ptr(), dadv.data_ptr(), beta, loss=lo.data_ptr(), logp=lp.data_ptr(), entropy=h.data_ptr(),
+                   grad=grad.data_ptr())
+    be.synchronize()
+    got = grad.double().cpu().numpy()
+    for i in range(rows):
+        t = float(np.float32(temps[i]))
+        t = t if t > 0 else 0.0
+        row = ref.policy(wide(v[i]), t, f16=dtype == "f16")
+        L, l, e, g = ref.loss(row, n, int(act[i]), float(np.float32(adv[i])), float(np.float32(beta)), t)
+        stat, part = whole_tolerances(row, n, float(adv[i]), beta, 1.0 / t if t else 0.0, l)
+        near([float(lo[i]), float(lp[i]), float(h[i])], [L, l, e], HALF["f32"], stat)
+        near(got[i], g, HALF[dtype], TINY[dtype] + part)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", [40, 900, 5000])
+def test_whole_softmax_where_masks_do_not_vanish_by_themselves(be, dtype, n):
+    """Rows whose masked entries a plain exponential would let through: hot
+    temperatures, largest scores next to the mask's floor, infinities, and
+    temperatures of 0 and infinity."""
+    rng = np.random.default_rng(n)
+    v = scores(rng, 9, n, dtype, 0.3)
+    v[1, :n // 2] = float("inf")
+    if dtype == "f16":
+        v[2] = torch.where(torch.from_numpy(rng.random(n) < 0.5), torch.tensor(-65504.0), torch.tensor(-65472.0)).half()
+    else:
+        v[2] = torch.where(torch.from_numpy(rng.random(n) < 0.5), torch.tensor(-1e30), torch.tensor(-9.5e28)).to(v.dtype)
+    v[3] = torch.from_numpy(np.where(rng.random(n) < 0.5, np.nan, 1.0)).to(v.dtype)
+    v[5, 7], v[5, 9] = 50.0, 50.0
+    act = [int(ref.support(wide(r), f16=dtype == "f16")[:1].sum()) for r in v]
+    act[5] = 9  # a later one of two largest
+    temps = [700.0, 1.0, 1.0, 0.5, 1.0, 0.0, 1e25, np.inf, np.nan]
+    whole_loss(be, v, dtype, act, rng.normal(size=9), 0.1, temps)
+    act[5] = 7
+    whole_loss(be, v, dtype, act, rng.normal(size=9), 0.0, temps)
 
 
 def test_loss_gradient_against_differences(be):
