@@ -262,6 +262,76 @@ struct Group {
   }
 };
 
+// Writes a row's entries of T, a 16-byte vector a lane and chunk, to an address
+// that need not be aligned as the vectors are. With out + i + delta on a
+// 16-byte boundary, a lane stores its own entries from delta on and the next
+// lane's (lane 31: the next chunk's lane 0) up to delta: whole vectors again,
+// for four shuffles and a shift in registers. What the row's and the warp's
+// ends leave is written entry by entry. The warp calls put for its chunks in
+// order, then finish.
+template <typename T>
+struct RowWriter {
+  static constexpr int V = 16 / int(sizeof(T));
+  T* out;
+  int n, lane, delta, prev_i;
+  uint4 prev;
+  bool have;
+
+  __device__ RowWriter(T* o, int len, int l, int i0) : out(o), n(len), lane(l), have(false) {
+    delta = int((16 - (reinterpret_cast<uintptr_t>(o + i0) & 15)) & 15) / int(sizeof(T));
+  }
+  __device__ void some(const uint4& d, int i, int from, int to) {
+    const T* e = reinterpret_cast<const T*>(&d);
+#pragma unroll
+    for (int j = 0; j < V; j++)
+      if (j >= from && j < to && i + j >= 0 && i + j < n) out[i + j] = e[j];
+  }
+  __device__ void whole(const uint4& d, int i) {
+    if (i >= 0 && i + V <= n) __stcs(reinterpret_cast<uint4*>(out + i), d);
+    else some(d, i, 0, V);
+  }
+  __device__ void emit(const uint4& next, bool last) {
+    const uint4 s = lane == 0 ? next : prev;
+    uint32_t a[8] = {prev.x, prev.y, prev.z, prev.w, 0u, 0u, 0u, 0u};
+    const int from = (lane + 1) & 31;
+    a[4] = __shfl_sync(0xffffffffu, s.x, from);
+    a[5] = __shfl_sync(0xffffffffu, s.y, from);
+    a[6] = __shfl_sync(0xffffffffu, s.z, from);
+    a[7] = __shfl_sync(0xffffffffu, s.w, from);
+    const int words = delta * int(sizeof(T)) / 4;
+    if (words & 2) {
+#pragma unroll
+      for (int j = 0; j < 6; j++) a[j] = a[j + 2];
+    }
+    if (words & 1) {
+#pragma unroll
+      for (int j = 0; j < 5; j++) a[j] = a[j + 1];
+    }
+    if (sizeof(T) == 2 && (delta & 1)) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) a[j] = __byte_perm(a[j], a[j + 1], 0x5432);
+    }
+    const uint4 d = make_uint4(a[0], a[1], a[2], a[3]);
+    if (last && lane == 31) some(d, prev_i + delta, 0, V - delta);
+    else whole(d, prev_i + delta);
+  }
+  __device__ void put(const T* v, int i) {
+    const uint4 d = *reinterpret_cast<const uint4*>(v);
+    if (delta == 0) {
+      whole(d, i);
+      return;
+    }
+    if (have) emit(d, false);
+    else if (lane == 0) some(d, i, 0, delta);
+    prev = d;
+    prev_i = i;
+    have = true;
+  }
+  __device__ void finish() {
+    if (delta && have) emit(prev, true);
+  }
+};
+
 // Where a row lies. The frame of a ragged row is found by a 32-way search of
 // q_off (three probes for 4096 frames). False: the row lies behind the last
 // frame's questions, and nothing of it exists.
@@ -771,6 +841,7 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) k_policy_loss(LossArg a
   if (!a.grad || !fits) return;
   T* out = static_cast<T*>(a.grad) + at.out;
   const double g0 = rw * c.inv_t, inv_z = kept ? 1.0 / z : 0.0, base = h - log_z;
+  RowWriter<T> writer(out, int(n), lane, r.i0);
 #pragma unroll
   for (int ch = 0; ch < R::kChunks; ch++) {
     const int i = r.at(ch);
@@ -789,14 +860,9 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) k_policy_loss(LossArg a
       }
       v[e] = from_f32<T>(float(d));
     }
-    if (i >= 0 && i + V <= int(n) && (reinterpret_cast<uintptr_t>(out + i) & 15) == 0) {
-      *reinterpret_cast<uint4*>(out + i) = *reinterpret_cast<uint4*>(v);
-    } else {
-#pragma unroll
-      for (int e = 0; e < V; e++)
-        if (i + e >= 0 && i + e < int(n)) out[i + e] = v[e];
-    }
+    writer.put(v, i);
   }
+  writer.finish();
 }
 
 // ---------------------------------------------------------------------------
@@ -995,6 +1061,7 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W == 16 ? 2 : 1) k_poli
   const float B = float(over * beta * 0.69314718055994530942);
   const float C = float(over * (adv + beta * (h - 0.69314718055994530942 * lg_z)));
   const bool quick = plain && fabsf(B) < 10.0f;
+  RowWriter<T> writer(out, n, lane, i0);
   const unsigned long long sc2 = pack2(sc, sc), off2 = pack2(off, off), B2 = pack2(B, B), C2 = pack2(C, C);
 #pragma unroll
   for (int c = 0; c < NV; c++) {
@@ -1025,14 +1092,9 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W == 16 ? 2 : 1) k_poli
           d[e] = from_f32<T>(float(gt * fma(adv, pi - 1.0, beta * pi * (logp + h))));
         }
     }
-    if (i >= 0 && i + V <= n && (reinterpret_cast<uintptr_t>(out + i) & 15) == 0) {
-      *reinterpret_cast<uint4*>(out + i) = *reinterpret_cast<uint4*>(d);
-    } else {
-#pragma unroll
-      for (int e = 0; e < V; e++)
-        if (i + e >= 0 && i + e < n) out[i + e] = d[e];
-    }
+    writer.put(d, i);
   }
+  writer.finish();
 }
 
 }  // namespace pol
