@@ -1939,6 +1939,7 @@ kc_status kc_create(const kc_config* config, const kc_weights_view* weights, int
       (e = cudaFuncSetAttribute(kc::oz::k_oz_gemm<kc::kEpiGate>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                 kc::oz::kSmem)))
     return bail(e, "smem");
+  if ((e = kc::pol::prepare())) return bail(e, "smem");
   s = do_sync(h, weights, nullptr);
   if (s) {
     std::string m = h->err;

@@ -8,6 +8,12 @@
 namespace kc {
 namespace pol {
 
+cudaError_t prepare() {
+  cudaError_t e;
+  if ((e = prepare_f32()) || (e = prepare_f16()) || (e = prepare_bf16())) return e;
+  return cudaSuccess;
+}
+
 cudaError_t launch_draw(const DrawArg& a, int dtype, cudaStream_t stream, uint64_t* launches) {
   if (a.r.rows == 0) return cudaSuccess;
   ++*launches;

@@ -34,6 +34,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "policy_args.h"
 
@@ -153,6 +155,8 @@ struct Group {
   struct Shared {
     double d[2][W > 1 ? W : 1];
     uint32_t u[2][3][W > 1 ? W : 1];
+    float2 f[2][W > 1 ? W : 1];
+    float2 cf[2][CL];
     double cd[2][CL];
     uint32_t cu[2][3][CL];
   };
@@ -221,6 +225,50 @@ struct Group {
     }
     return v;
   }
+  __device__ uint32_t largest(uint32_t v) {
+    v = __reduce_max_sync(0xffffffffu, v);
+    if constexpr (W > 1) {
+      buf ^= 1;
+      if (lane == 0) s.u[buf][0][warp] = v;
+      __syncthreads();
+      v = __reduce_max_sync(0xffffffffu, lane < W ? s.u[buf][0][lane] : 0u);
+    }
+    if constexpr (CL > 1) {
+      namespace cg = cooperative_groups;
+      cg::cluster_group cl = cg::this_cluster();
+      if (warp == 0 && lane < CL) cl.map_shared_rank(&s.cu[0][0][0], lane)[buf * 3 * CL + rank] = v;
+      cl.sync();
+      v = __reduce_max_sync(0xffffffffu, lane < CL ? s.cu[buf][0][lane] : 0u);
+    }
+    return v;
+  }
+  // The group's sums of two f32, by trees of at most 5 levels a step.
+  static __device__ float2 warp_pair(float2 v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+      v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+    }
+    return v;
+  }
+  __device__ float2 pair_sum(float2 v) {
+    const float2 nil = make_float2(0.0f, 0.0f);
+    v = warp_pair(v);
+    if constexpr (W > 1) {
+      buf ^= 1;
+      if (lane == 0) s.f[buf][warp] = v;
+      __syncthreads();
+      v = warp_pair(lane < W ? s.f[buf][lane] : nil);
+    }
+    if constexpr (CL > 1) {
+      namespace cg = cooperative_groups;
+      cg::cluster_group cl = cg::this_cluster();
+      if (warp == 0 && lane < CL) cl.map_shared_rank(&s.cf[0][0], lane)[buf * CL + rank] = v;
+      cl.sync();
+      v = warp_pair(lane < CL ? s.cf[buf][lane] : nil);
+    }
+    return v;
+  }
   // The group's sum of one u32 a thread whose warp sums stay below 2^32.
   __device__ double sum_u32(uint32_t v) {
     v = __reduce_add_sync(0xffffffffu, v);
@@ -261,6 +309,35 @@ struct Group {
     return before;
   }
 };
+
+// A 16-byte vector as four words: entry e of it, and two results as a word.
+template <typename T> __device__ __forceinline__ float entry(const uint32_t* w, int e);
+template <> __device__ __forceinline__ float entry<float>(const uint32_t* w, int e) { return __uint_as_float(w[e]); }
+template <> __device__ __forceinline__ float entry<__nv_bfloat16>(const uint32_t* w, int e) {
+  return __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+}
+template <> __device__ __forceinline__ float entry<__half>(const uint32_t* w, int e) {
+  return __half2float(__ushort_as_half(static_cast<unsigned short>(e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xffffu)));
+}
+template <typename T> __device__ __forceinline__ void set2(uint32_t* w, int e, float x, float y);
+template <> __device__ __forceinline__ void set2<float>(uint32_t* w, int e, float x, float y) {
+  w[e] = __float_as_uint(x);
+  w[e + 1] = __float_as_uint(y);
+}
+template <> __device__ __forceinline__ void set2<__half>(uint32_t* w, int e, float x, float y) {
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w[e / 2]) : "f"(y), "f"(x));
+}
+template <> __device__ __forceinline__ void set2<__nv_bfloat16>(uint32_t* w, int e, float x, float y) {
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[e / 2]) : "f"(y), "f"(x));
+}
+
+// The word w with the first (second) entry of x; an f32 word is one entry.
+template <typename T> __device__ __forceinline__ uint32_t first_of(uint32_t x, uint32_t w) {
+  return sizeof(T) == 4 ? x : (w & 0xffff0000u) | (x & 0xffffu);
+}
+template <typename T> __device__ __forceinline__ uint32_t second_of(uint32_t x, uint32_t w) {
+  return sizeof(T) == 4 ? x : (w & 0xffffu) | (x & 0xffff0000u);
+}
 
 // Writes a row's entries of T, a 16-byte vector a lane and chunk, to an address
 // that need not be aligned as the vectors are. With out + i + delta on a
@@ -315,8 +392,8 @@ struct RowWriter {
     if (last && lane == 31) some(d, prev_i + delta, 0, V - delta);
     else whole(d, prev_i + delta);
   }
-  __device__ void put(const T* v, int i) {
-    const uint4 d = *reinterpret_cast<const uint4*>(v);
+  __device__ void put(const uint32_t* w, int i) {
+    const uint4 d = make_uint4(w[0], w[1], w[2], w[3]);
     if (delta == 0) {
       whole(d, i);
       return;
@@ -845,7 +922,8 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) k_policy_loss(LossArg a
 #pragma unroll
   for (int ch = 0; ch < R::kChunks; ch++) {
     const int i = r.at(ch);
-    alignas(16) T v[V];
+    float f[V];
+    uint32_t v[4];
 #pragma unroll
     for (int e = 0; e < V; e++) {
       const uint32_t key = r.k[ch * V + e];
@@ -858,8 +936,10 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) k_policy_loss(LossArg a
         const double one = uint32_t(i + e) == act ? 1.0 : 0.0;
         if (key) d = g0 * fma(adv, pi - one, beta * pi * (x + base));
       }
-      v[e] = from_f32<T>(float(d));
+      f[e] = float(d);
     }
+#pragma unroll
+    for (int e = 0; e < V; e += 2) set2<T>(v, e, f[e], f[e + 1]);
     writer.put(v, i);
   }
   writer.finish();
@@ -867,14 +947,14 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) k_policy_loss(LossArg a
 
 // ---------------------------------------------------------------------------
 // The policy loss over the whole softmax, nothing cut: no decision hangs on a
-// last bit, so the row stays as it was loaded (NV 16-byte vectors a thread) and
-// its exponentials are f32. With u_j = (v_j - m) log2(e) / T, taken as one
+// last bit, so the row stays as it was loaded (a warp's registers, NV 16-byte
+// vectors a lane; longer rows: k_policy_long) and its exponentials are f32. With u_j = (v_j - m) log2(e) / T, taken as one
 // fma of v_j (the rounding of m log2(e) / T is common to all and cancels),
 //   Z = sum 2^u, S = sum 2^u u, log pi_j = ln 2 (u_j - log2 Z),
 //   H = ln 2 (log2 Z - S / Z), and the gradient is
 //   2^u_j (u_j B + C) with B = g beta ln 2 / (T Z), C = g (A + beta (H - ln Z)) / (T Z)
-// but for -g A / T more at the action. Sums: four f32 partial sums of at most
-// 16 terms a thread, joined in 64 bits. Arithmetic on pairs (f32x2).
+// but for -g A / T more at the action. Sums: eight f32 partial sums of at most
+// 16 terms a thread, joined by trees. Arithmetic on pairs (f32x2).
 //
 // Masked entries need no test where they vanish by themselves: NaN and what
 // lies below the mask's floor is raised to it as the row is loaded, and 2^u is
@@ -916,39 +996,41 @@ template <> struct Floor<__half> { static constexpr float value = -65504.0f; };
 
 
 // Raises a vector's entries to the floor (a NaN too) and takes their largest into mx.
-__device__ __forceinline__ void raise(float* v, float& mx) {
+template <typename T> __device__ __forceinline__ void raise(uint32_t* w, float& mx);
+template <> __device__ __forceinline__ void raise<float>(uint32_t* w, float& mx) {
 #pragma unroll
   for (int e = 0; e < 4; e++) {
-    v[e] = fmaxf(v[e], Floor<float>::value);
-    mx = fmaxf(mx, v[e]);
+    const float f = fmaxf(__uint_as_float(w[e]), Floor<float>::value);
+    w[e] = __float_as_uint(f);
+    mx = fmaxf(mx, f);
   }
 }
-template <typename T, typename T2>
-__device__ __forceinline__ void raise_pairs(T2* v, T2 floor2, float& mx) {
-  T2 top = floor2;
+template <> __device__ __forceinline__ void raise<__half>(uint32_t* w, float& mx) {
+  const __half2 low = __float2half2_rn(Floor<__half>::value);
+  __half2 top = low;
 #pragma unroll
   for (int e = 0; e < 4; e++) {
-    v[e] = __hmax2(v[e], floor2);
-    top = __hmax2(top, v[e]);
+    const __half2 f = __hmax2(*reinterpret_cast<__half2*>(w + e), low);
+    w[e] = *reinterpret_cast<const uint32_t*>(&f);
+    top = __hmax2(top, f);
   }
-  mx = fmaxf(mx, fmaxf(as_f32(T(top.x)), as_f32(T(top.y))));
+  mx = fmaxf(mx, fmaxf(__low2float(top), __high2float(top)));
 }
-__device__ __forceinline__ void raise(__half* v, float& mx) {
-  raise_pairs<__half>(reinterpret_cast<__half2*>(v), __float2half2_rn(Floor<__half>::value), mx);
-}
-__device__ __forceinline__ void raise(__nv_bfloat16* v, float& mx) {
-  raise_pairs<__nv_bfloat16>(reinterpret_cast<__nv_bfloat162*>(v), __float2bfloat162_rn(Floor<__nv_bfloat16>::value), mx);
-}
-__device__ __forceinline__ void store2(float* d, Pair r) { d[0] = r.x; d[1] = r.y; }
-__device__ __forceinline__ void store2(__half* d, Pair r) {
-  *reinterpret_cast<__half2*>(d) = __floats2half2_rn(r.x, r.y);
-}
-__device__ __forceinline__ void store2(__nv_bfloat16* d, Pair r) {
-  *reinterpret_cast<__nv_bfloat162*>(d) = __floats2bfloat162_rn(r.x, r.y);
+template <> __device__ __forceinline__ void raise<__nv_bfloat16>(uint32_t* w, float& mx) {
+  const __nv_bfloat162 low = __float2bfloat162_rn(Floor<__nv_bfloat16>::value);
+  __nv_bfloat162 top = low;
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const __nv_bfloat162 f = __hmax2(*reinterpret_cast<__nv_bfloat162*>(w + e), low);
+    w[e] = *reinterpret_cast<const uint32_t*>(&f);
+    top = __hmax2(top, f);
+  }
+  mx = fmaxf(mx, fmaxf(__low2float(top), __high2float(top)));
 }
 
-template <typename T, int NV, int W, int CL>
-__global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W == 16 ? 2 : 1) k_policy_whole(LossArg a) {
+template <typename T, int NV>
+__global__ void __launch_bounds__(128) k_policy_whole(LossArg a) {
+  constexpr int W = 1, CL = 1;
   constexpr int V = 16 / int(sizeof(T));
   constexpr uint32_t kCap = uint32_t(32) * V * NV * W * CL;
   __shared__ typename Group<W, CL>::Shared sh;
@@ -966,135 +1048,359 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32, W == 16 ? 2 : 1) k_poli
   constexpr float floor_v = Floor<T>::value;
 
   // the row, masked entries raised to the floor; its largest
-  alignas(16) T v[NV][V];
+  uint32_t v[NV][4];
   float mx = -INFINITY;
 #pragma unroll
   for (int c = 0; c < NV; c++) {
     const int i = i0 + c * 32 * V;
     if (i >= 0 && i + V <= n) {
-      *reinterpret_cast<uint4*>(v[c]) = __ldcs(reinterpret_cast<const uint4*>(in + i));
+      const uint4 q = __ldcs(reinterpret_cast<const uint4*>(in + i));
+      v[c][0] = q.x; v[c][1] = q.y; v[c][2] = q.z; v[c][3] = q.w;
     } else {
+      float f[V];
 #pragma unroll
-      for (int e = 0; e < V; e++) v[c][e] = i + e >= 0 && i + e < n ? in[i + e] : from_f32<T>(floor_v);
+      for (int e = 0; e < V; e++) f[e] = i + e >= 0 && i + e < n ? as_f32(in[i + e]) : floor_v;
+#pragma unroll
+      for (int e = 0; e < V; e += 2) set2<T>(v[c], e, f[e], f[e + 1]);
     }
-    raise(v[c], mx);
   }
+#pragma unroll
+  for (int c = 0; c < NV; c++) raise<T>(v[c], mx);
   // the action's value, before anything is written: grad may lie over values
   const uint32_t act = a.actions[row];
   const bool asked = act != kNone;
   const float va = act < uint32_t(n) ? as_f32(in[act]) : floor_v;
-  uint32_t none = 0, mn = mx == INFINITY ? 0u : 1u, top = key_of(fminf(mx, 3.402823466e38f));
-  g.counts(none, mn, top);  // mn 0: the row holds +infinity
-  const float m = value_of(top);
+  constexpr float kLn2 = 0.69314718055994530942f, kMost = 3.402823466e38f;
+  const uint32_t top = g.largest(key_of(mx));
+  const bool endless = top == 0xff800000u;  // the row holds +infinity
+  const float m = endless ? kMost : value_of(top);
   const float t_row = a.c.row_temperature ? a.c.row_temperature[row] : a.c.temperature;
-  const double inv_t = t_row > 0.0f ? 1.0 / double(t_row) : 0.0;
-  const float sc = float(inv_t * 1.4426950408889634074);  // log2(e) / T
-  const bool any = m > Lowest<T>::open_above;
-  const bool open_t = t_row > 0.0f;
-  const bool plain = mn != 0u && (m - Lowest<T>::open_above) * sc >= 200.0f && fabsf(m * sc) < 1e5f && sc < 1e6f;
+  const bool open_t = t_row > 0.0f, any = m > Lowest<T>::open_above;
+  const float sc = open_t ? 1.44269504088896340736f / t_row : 0.0f;  // log2(e) / T
+  const bool plain = !endless && (m - Lowest<T>::open_above) * sc >= 200.0f && fabsf(m * sc) < 1e5f && sc < 1e6f;
   const float off = -m * sc;
   auto u_of = [&](float f) { return plain ? fmaf(f, sc, off) : (fminf(f, m) - m) * sc; };
 
   // Z and S
-  double z = 0.0, s = 0.0;
+  float2 zs = make_float2(0.0f, 0.0f);
   if (plain) {
     const unsigned long long sc2 = pack2(sc, sc), off2 = pack2(off, off);
-    unsigned long long za[2] = {0ull, 0ull}, sa[2] = {0ull, 0ull};
+    unsigned long long za[4] = {0ull, 0ull, 0ull, 0ull}, sa[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
     for (int c = 0; c < NV; c++)
 #pragma unroll
       for (int e = 0; e < V; e += 2) {
-        const unsigned long long u = fma2(pack2(as_f32(v[c][e]), as_f32(v[c][e + 1])), sc2, off2);
+        const int k = (c * V + e) / 2 & 3;
+        const unsigned long long u = fma2(pack2(entry<T>(v[c], e), entry<T>(v[c], e + 1)), sc2, off2);
         const Pair up = unpack2(u);
         const unsigned long long w = pack2(exp2_fast(up.x), exp2_fast(up.y));
-        za[(e >> 1) & 1] = add2(za[(e >> 1) & 1], w);
-        sa[(e >> 1) & 1] = fma2(w, u, sa[(e >> 1) & 1]);
+        za[k] = add2(za[k], w);
+        sa[k] = fma2(w, u, sa[k]);
       }
-    const Pair z0 = unpack2(za[0]), z1 = unpack2(za[1]), s0 = unpack2(sa[0]), s1 = unpack2(sa[1]);
-    z = (double(z0.x) + double(z0.y)) + (double(z1.x) + double(z1.y));
-    s = (double(s0.x) + double(s0.y)) + (double(s1.x) + double(s1.y));
+    const Pair z1 = unpack2(add2(add2(za[0], za[1]), add2(za[2], za[3])));
+    const Pair s1 = unpack2(add2(add2(sa[0], sa[1]), add2(sa[2], sa[3])));
+    zs = make_float2(z1.x + z1.y, s1.x + s1.y);
   } else if (any) {
+    double z = 0.0, s = 0.0;
 #pragma unroll
     for (int c = 0; c < NV; c++)
 #pragma unroll
       for (int e = 0; e < V; e++) {
-        const float f = as_f32(v[c][e]);
+        const float f = entry<T>(v[c], e);
         if (f > Lowest<T>::open_above) {
           const float u = fmaxf(u_of(f), -2000.0f), w = exp2_fast(u);
           z += double(w);
           s += double(w) * double(u);
         }
       }
+    zs = make_float2(float(z), float(s));
   }
-  z = g.sum(z);
-  s = g.sum(s);
+  zs = g.pair_sum(zs);
+  // the widened entries are made again below, not kept: 16-bit rows would take
+  // twice the registers
+#pragma unroll
+  for (int c = 0; c < NV; c++) asm volatile("" : "+r"(v[c][0]), "+r"(v[c][1]), "+r"(v[c][2]), "+r"(v[c][3]));
 
   // the row's answer
-  const float ua = u_of(fminf(va, 3.402823466e38f));
-  bool live = asked && va > Lowest<T>::open_above && double(ua) * 0.69314718055994530942 >= kDropped;
+  const float ua = u_of(fminf(va, kMost));
+  bool live = asked && va > Lowest<T>::open_above && ua * kLn2 >= float(kDropped);
   if (!open_t) {  // temperature 0: the first largest entry alone
     uint32_t first = 0xffffffffu;
 #pragma unroll
     for (int c = 0; c < NV; c++)
 #pragma unroll
       for (int e = 0; e < V; e++)
-        if (fminf(as_f32(v[c][e]), 3.402823466e38f) == m) first = min(first, uint32_t(i0 + c * 32 * V + e));
-    uint32_t zero = 0;
-    none = 0;
+        if (fminf(entry<T>(v[c], e), kMost) == m) first = min(first, uint32_t(i0 + c * 32 * V + e));
+    uint32_t zero = 0, none = 0;
     g.counts(none, first, zero);
     live = asked && any && first == act;
   }
-  const double lg_z = any ? log2(z) : 0.0;
-  const double h = any && open_t ? 0.69314718055994530942 * (lg_z - s / z) : 0.0;
-  const double logp = open_t ? 0.69314718055994530942 * (double(ua) - lg_z) : 0.0;
+  const float lg_z = any ? log2f(zs.x) : 0.0f, inv_z = any ? 1.0f / zs.x : 0.0f;
+  const float h = any && open_t ? kLn2 * (lg_z - zs.y * inv_z) : 0.0f;
+  const float logp = open_t ? kLn2 * (ua - lg_z) : 0.0f;
   const bool learns = asked && live && open_t;
-  const double adv = double(a.advantage[row]), beta = double(a.beta);
-  const double gt = (a.row_weight ? double(a.row_weight[row]) : 1.0) * inv_t;
+  const float adv = a.advantage[row], beta = a.beta;
   if (g.segment() == 0 && lane == 0) {
-    if (a.loss) a.loss[row] = learns ? float(-adv * logp - beta * h) : 0.0f;
-    if (a.logp) a.logp[row] = !asked ? 0.0f : live ? float(logp) : -INFINITY;
-    if (a.entropy) a.entropy[row] = float(h);
+    if (a.loss) a.loss[row] = learns ? fmaf(-adv, logp, -beta * h) : 0.0f;
+    if (a.logp) a.logp[row] = !asked ? 0.0f : live ? logp : -INFINITY;
+    if (a.entropy) a.entropy[row] = h;
   }
   if (!a.grad || !fits) return;
   T* out = static_cast<T*>(a.grad) + at.out;
-  const double over = learns ? gt / z : 0.0;
-  const float B = float(over * beta * 0.69314718055994530942);
-  const float C = float(over * (adv + beta * (h - 0.69314718055994530942 * lg_z)));
+  const float gt = learns ? (a.row_weight ? a.row_weight[row] : 1.0f) / t_row : 0.0f;
+  const float over = gt * inv_z;
+  const float B = over * beta * kLn2, C = over * fmaf(beta, h - kLn2 * lg_z, adv);
   const bool quick = plain && fabsf(B) < 10.0f;
   RowWriter<T> writer(out, n, lane, i0);
   const unsigned long long sc2 = pack2(sc, sc), off2 = pack2(off, off), B2 = pack2(B, B), C2 = pack2(C, C);
 #pragma unroll
   for (int c = 0; c < NV; c++) {
     const int i = i0 + c * 32 * V;
-    alignas(16) T d[V];
+    uint32_t d[4];
     if (quick) {
 #pragma unroll
       for (int e = 0; e < V; e += 2) {
-        const unsigned long long u = fma2(pack2(as_f32(v[c][e]), as_f32(v[c][e + 1])), sc2, off2);
+        const unsigned long long u = fma2(pack2(entry<T>(v[c], e), entry<T>(v[c], e + 1)), sc2, off2);
         const Pair up = unpack2(u);
         const Pair r = unpack2(mul2(pack2(exp2_fast(up.x), exp2_fast(up.y)), fma2(u, B2, C2)));
-        store2(d + e, r);
+        set2<T>(d, e, r.x, r.y);
       }
     } else {
+      float f[V];
 #pragma unroll
       for (int e = 0; e < V; e++) {
-        const float f = as_f32(v[c][e]), u = fmaxf(u_of(f), -2000.0f);
-        d[e] = from_f32<T>(learns && f > Lowest<T>::open_above ? exp2_fast(u) * fmaf(u, B, C) : 0.0f);
+        const float x = entry<T>(v[c], e), u = fmaxf(u_of(x), -2000.0f);
+        f[e] = learns && x > Lowest<T>::open_above ? exp2_fast(u) * fmaf(u, B, C) : 0.0f;
       }
+#pragma unroll
+      for (int e = 0; e < V; e += 2) set2<T>(d, e, f[e], f[e + 1]);
     }
     // the action's entry, and its lane's alone, gets the rest
     if (learns && act - uint32_t(i) < uint32_t(V)) {
+      // (in 64 bits: pi - 1 is the row's largest gradient)
+      const double pi = double(exp2_fast(ua)) / double(zs.x), scale = double(a.row_weight ? a.row_weight[row] : 1.0f) / t_row;
+      const float x = float(scale * fma(double(adv), pi - 1.0, double(beta) * pi * (double(logp) + h)));
 #pragma unroll
-      for (int e = 0; e < V; e++)
-        if (uint32_t(i + e) == act) {
-          const double x = 0.69314718055994530942 * double(ua);
-          const double pi = exp(x - 0.69314718055994530942 * lg_z);
-          d[e] = from_f32<T>(float(gt * fma(adv, pi - 1.0, beta * pi * (logp + h))));
-        }
+      for (int e = 0; e < V; e += 2) {
+        uint32_t w[4];
+        set2<T>(w, e, x, x);
+        if (uint32_t(i + e) == act) d[e * int(sizeof(T)) / 4] = first_of<T>(w[e * int(sizeof(T)) / 4], d[e * int(sizeof(T)) / 4]);
+        if (uint32_t(i + e + 1) == act) d[(e + 1) * int(sizeof(T)) / 4] = second_of<T>(w[(e + 1) * int(sizeof(T)) / 4], d[(e + 1) * int(sizeof(T)) / 4]);
+      }
     }
     writer.put(d, i);
   }
   writer.finish();
+}
+
+
+// The same for longer rows, which stay in shared memory as they were loaded:
+// CL CTAs of NT threads a row, each with its segment of 16-byte vectors. The
+// loops are rolled (a row in registers would unroll them over its whole length,
+// and the instruction cache then bounds them), three CTAs an SM overlap one
+// row's loads with another's arithmetic, and the last pass reads the row at the
+// gradient's alignment, so that every store is a whole vector.
+struct WholeRow {
+  float sc, off, m;
+  bool plain;
+  __device__ float u_of(float f) const { return plain ? fmaf(f, sc, off) : (fminf(f, m) - m) * sc; }
+};
+
+// The vector that starts O entries behind w[0]: O of the next one's. O = 0: w itself.
+template <typename T, int WORDS>
+__device__ __forceinline__ void shifted(const uint4& x, const uint4& y, bool odd, uint32_t* d) {
+  const uint32_t a[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+  for (int j = 0; j < 4; j++)
+    d[j] = sizeof(T) == 2 && odd ? __byte_perm(a[j + WORDS], a[j + WORDS + 1], 0x5432) : a[j + WORDS];
+}
+
+template <typename T, int NT, int CL>
+__global__ void __launch_bounds__(NT) k_policy_long(LossArg a, uint32_t seg_vecs) {
+  constexpr int V = 16 / int(sizeof(T)), W = NT / 32;
+  extern __shared__ uint4 sm_all[];
+  uint4* sm = sm_all + 1;  // one vector ahead of the segment and two behind it may be read
+  __shared__ typename Group<W, CL>::Shared sh;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t row = blockIdx.x / CL;
+  RowAt at;
+  if (!locate(a.r, a.out_pitch, row, lane, &at)) return;
+  Group<W, CL> g(sh, lane, warp);
+  constexpr float kLn2 = 0.69314718055994530942f, kMost = 3.402823466e38f, floor_v = Floor<T>::value;
+  const bool fits = at.n <= a.r.row_len && at.n + V - 1 <= uint64_t(seg_vecs) * V * CL;
+  const int n = fits ? int(at.n) : 0;
+  const T* in = static_cast<const T*>(a.r.values) + at.in;
+  const int shift = int((reinterpret_cast<uintptr_t>(in) & 15) / sizeof(T));
+  const int vecs = (n + shift + V - 1) / V;  // of the row, its misaligned ends included
+  const int v0 = g.rank * int(seg_vecs);     // this CTA's first
+  // one more is loaded where another CTA's segment follows
+  const int mine = max(0, min(int(seg_vecs), vecs - v0)), have = max(0, min(int(seg_vecs) + 1, vecs - v0));
+  const int i0 = v0 * V - shift;
+
+  // the row, masked entries raised to the floor; its largest
+  float mx = -INFINITY;
+#pragma unroll 4
+  for (int j = tid; j < have; j += NT) {
+    const int i = i0 + j * V;
+    uint32_t w[4];
+    if (i >= 0 && i + V <= n) {
+      const uint4 q = __ldcs(reinterpret_cast<const uint4*>(in + i));
+      w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
+    } else {
+      float f[V];
+#pragma unroll
+      for (int e = 0; e < V; e++) f[e] = i + e >= 0 && i + e < n ? as_f32(in[i + e]) : floor_v;
+#pragma unroll
+      for (int e = 0; e < V; e += 2) set2<T>(w, e, f[e], f[e + 1]);
+    }
+    raise<T>(w, mx);
+    sm[j] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  // the action's value, before anything is written: grad may lie over values
+  const uint32_t act = a.actions[row];
+  const bool asked = act != kNone;
+  const float va = act < uint32_t(n) ? as_f32(in[act]) : floor_v;
+  const uint32_t top = g.largest(key_of(fmaxf(mx, floor_v)));
+  const bool endless = top == 0xff800000u;  // the row holds +infinity
+  const float m = endless ? kMost : value_of(top);
+  const float t_row = a.c.row_temperature ? a.c.row_temperature[row] : a.c.temperature;
+  const bool open_t = t_row > 0.0f, any = m > Lowest<T>::open_above;
+  const float sc = open_t ? 1.44269504088896340736f / t_row : 0.0f;  // log2(e) / T
+  const bool plain = !endless && (m - Lowest<T>::open_above) * sc >= 200.0f && fabsf(m * sc) < 1e5f && sc < 1e6f;
+  const WholeRow wr{sc, -m * sc, m, plain};
+  const unsigned long long sc2 = pack2(sc, sc), off2 = pack2(wr.off, wr.off);
+
+  // Z and S
+  float2 zs = make_float2(0.0f, 0.0f);
+  if (plain) {
+    unsigned long long za[4] = {0ull, 0ull, 0ull, 0ull}, sa[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll 2
+    for (int j = tid; j < mine; j += NT) {
+      const uint4 q = sm[j];
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int e = 0; e < V; e += 2) {
+        const unsigned long long u = fma2(pack2(entry<T>(w, e), entry<T>(w, e + 1)), sc2, off2);
+        const Pair up = unpack2(u);
+        const unsigned long long x = pack2(exp2_fast(up.x), exp2_fast(up.y));
+        za[e / 2 & 3] = add2(za[e / 2 & 3], x);
+        sa[e / 2 & 3] = fma2(x, u, sa[e / 2 & 3]);
+      }
+    }
+    const Pair z1 = unpack2(add2(add2(za[0], za[1]), add2(za[2], za[3])));
+    const Pair s1 = unpack2(add2(add2(sa[0], sa[1]), add2(sa[2], sa[3])));
+    zs = make_float2(z1.x + z1.y, s1.x + s1.y);
+  } else if (any) {
+    double z = 0.0, s = 0.0;
+    for (int j = tid; j < mine; j += NT) {
+      const uint4 q = sm[j];
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int e = 0; e < V; e++) {
+        const float f = entry<T>(w, e);
+        if (f > Lowest<T>::open_above) {
+          const float u = fmaxf(wr.u_of(f), -2000.0f), x = exp2_fast(u);
+          z += double(x);
+          s += double(x) * double(u);
+        }
+      }
+    }
+    zs = make_float2(float(z), float(s));
+  }
+  zs = g.pair_sum(zs);
+
+  // the row's answer
+  const float ua = wr.u_of(fminf(va, kMost));
+  bool live = asked && va > Lowest<T>::open_above && ua * kLn2 >= float(kDropped);
+  if (!open_t) {  // temperature 0: the first largest entry alone
+    uint32_t first = 0xffffffffu, zero = 0, none = 0;
+    for (int j = tid; j < mine; j += NT) {
+      const uint4 q = sm[j];
+      const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int e = 0; e < V; e++)
+        if (fminf(entry<T>(w, e), kMost) == m) first = min(first, uint32_t(i0 + j * V + e));
+    }
+    g.counts(none, first, zero);
+    live = asked && any && first == act;
+  }
+  const float lg_z = any ? log2f(zs.x) : 0.0f, inv_z = any ? 1.0f / zs.x : 0.0f;
+  const float h = any && open_t ? kLn2 * (lg_z - zs.y * inv_z) : 0.0f;
+  const float logp = open_t ? kLn2 * (ua - lg_z) : 0.0f;
+  const bool learns = asked && live && open_t;
+  const float adv = a.advantage[row], beta = a.beta;
+  if (g.rank == 0 && tid == 0) {
+    if (a.loss) a.loss[row] = learns ? fmaf(-adv, logp, -beta * h) : 0.0f;
+    if (a.logp) a.logp[row] = !asked ? 0.0f : live ? logp : -INFINITY;
+    if (a.entropy) a.entropy[row] = h;
+  }
+  if (!a.grad || !fits) return;
+  T* out = static_cast<T*>(a.grad) + at.out;
+  const float rw = a.row_weight ? a.row_weight[row] : 1.0f, gt = learns ? rw / t_row : 0.0f, over = gt * inv_z;
+  const float B = over * beta * kLn2, C = over * fmaf(beta, h - kLn2 * lg_z, adv);
+  const bool quick = plain && fabsf(B) < 10.0f;
+  const unsigned long long B2 = pack2(B, B), C2 = pack2(C, C);
+  // Group j of the gradient starts at entry q = i0 + j V + skew of the row, on a
+  // 16-byte boundary of out: entries skew.. of vector j and those of j + 1
+  // ahead of skew. Groups belong to the CTA that holds their first vector;
+  // the first CTA has the one that starts ahead of the row, too.
+  const int skew = int((16 - (reinterpret_cast<uintptr_t>(out + i0) & 15)) & 15) / int(sizeof(T));
+  const int words = skew * int(sizeof(T)) / 4;
+  const bool odd = sizeof(T) == 2 && (skew & 1);
+  auto groups = [&](auto w_) {
+    constexpr int WORDS = decltype(w_)::value;
+#pragma unroll 2
+    for (int j = tid - (skew && g.rank == 0 ? 1 : 0); j < mine; j += NT) {
+      const int i = i0 + j * V + skew;
+      uint32_t w[4], d[4];
+      const uint4 x = sm[j];
+      shifted<T, WORDS>(x, WORDS || odd ? sm[j + 1] : x, odd, w);
+      if (quick) {
+#pragma unroll
+        for (int e = 0; e < V; e += 2) {
+          const unsigned long long u = fma2(pack2(entry<T>(w, e), entry<T>(w, e + 1)), sc2, off2);
+          const Pair up = unpack2(u);
+          const Pair r = unpack2(mul2(pack2(exp2_fast(up.x), exp2_fast(up.y)), fma2(u, B2, C2)));
+          set2<T>(d, e, r.x, r.y);
+        }
+      } else {
+        float f[V];
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+          const float x = entry<T>(w, e), u = fmaxf(wr.u_of(x), -2000.0f);
+          f[e] = learns && x > Lowest<T>::open_above ? exp2_fast(u) * fmaf(u, B, C) : 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < V; e += 2) set2<T>(d, e, f[e], f[e + 1]);
+      }
+      // the action's entry gets the rest, in 64 bits: pi - 1 is the row's largest gradient
+      if (learns && act - uint32_t(i) < uint32_t(V)) {
+        const double pi = double(exp2_fast(ua)) / double(zs.x), scale = double(rw) / t_row;
+        const float x = float(scale * fma(double(adv), pi - 1.0, double(beta) * pi * (double(logp) + h)));
+        uint32_t y[4];
+#pragma unroll
+        for (int e = 0; e < V; e += 2) {
+          set2<T>(y, e, x, x);
+          constexpr int S = int(sizeof(T));
+          if (uint32_t(i + e) == act) d[e * S / 4] = first_of<T>(y[e * S / 4], d[e * S / 4]);
+          if (uint32_t(i + e + 1) == act) d[(e + 1) * S / 4] = second_of<T>(y[(e + 1) * S / 4], d[(e + 1) * S / 4]);
+        }
+      }
+      if (i >= 0 && i + V <= n) {
+        __stcs(reinterpret_cast<uint4*>(out + i), make_uint4(d[0], d[1], d[2], d[3]));
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; e++)
+          if (i + e >= 0 && i + e < n) out[i + e] = from_f32<T>(entry<T>(d, e));
+      }
+    }
+  };
+  switch (words) {
+    case 0: groups(std::integral_constant<int, 0>{}); break;
+    case 1: groups(std::integral_constant<int, 1>{}); break;
+    case 2: groups(std::integral_constant<int, 2>{}); break;
+    default: groups(std::integral_constant<int, 3>{}); break;
+  }
 }
 
 }  // namespace pol

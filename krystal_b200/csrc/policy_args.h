@@ -60,6 +60,13 @@ cudaError_t loss_f32(const LossArg& a, cudaStream_t s);
 cudaError_t loss_f16(const LossArg& a, cudaStream_t s);
 cudaError_t loss_bf16(const LossArg& a, cudaStream_t s);
 
+cudaError_t prepare_f32();
+cudaError_t prepare_f16();
+cudaError_t prepare_bf16();
+
+// What the kernels need once on each device (the current one).
+cudaError_t prepare();
+
 // One launch each on `stream`; *launches counts it.
 cudaError_t launch_draw(const DrawArg& a, int dtype, cudaStream_t stream, uint64_t* launches);
 cudaError_t launch_policy_loss(const LossArg& a, int dtype, cudaStream_t stream, uint64_t* launches);

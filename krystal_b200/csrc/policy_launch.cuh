@@ -40,17 +40,53 @@ inline cudaError_t draw_as(const DrawArg& a, cudaStream_t s) {
   if (need <= 32768) return go(k_draw<T, 64, 16, 1>, a, 16, 1, s);
   return go(k_draw<T, 64, 16, 8>, a, 16, 8, s);
 }
+// Rows that k_policy_long keeps in shared memory: CL CTAs of NT threads a row,
+// up to kShort bytes a row 128 threads, up to kLong 256 (three CTAs an SM),
+// beyond that a cluster of 8 x 512.
+constexpr uint64_t kShort = 16384, kLong = 73728;
+template <typename T>
+constexpr size_t long_smem(uint64_t row_len, int cl) {
+  constexpr uint64_t V = 16 / sizeof(T);
+  return (((row_len + 2 * V - 2) / V + cl - 1) / cl + 4) * 16;
+}
+template <typename T>
+cudaError_t prepare_as() {
+  const auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
+  cudaError_t e;
+  if ((e = cudaFuncSetAttribute(k_policy_long<T, 128, 1>, attr, int(long_smem<T>(kShort / sizeof(T), 1)))) ||
+      (e = cudaFuncSetAttribute(k_policy_long<T, 256, 1>, attr, int(long_smem<T>(kLong / sizeof(T), 1)))) ||
+      (e = cudaFuncSetAttribute(k_policy_long<T, 512, 8>, attr, int(long_smem<T>(kMaxRow, 8)))))
+    return e;
+  return cudaSuccess;
+}
+template <typename T, int NT, int CL>
+cudaError_t go_long(const LossArg& a, cudaStream_t stream) {
+  const size_t smem = long_smem<T>(a.r.row_len, CL);
+  const uint32_t seg = uint32_t(smem / 16 - 4);
+  cudaLaunchConfig_t cfg{};
+  const uint64_t ctas = uint64_t(a.r.rows) * CL;
+  if (ctas > 0x7fffffffu) return cudaErrorInvalidConfiguration;
+  cfg.gridDim = dim3(unsigned(ctas));
+  cfg.blockDim = dim3(NT);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CL;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CL > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, k_policy_long<T, NT, CL>, a, seg);
+}
 template <typename T>
 inline cudaError_t whole_as(const LossArg& a, cudaStream_t s) {
   constexpr int V = 16 / sizeof(T);
   const uint64_t need = a.r.row_len + V - 1;
-  if (need <= 256) return go(k_policy_whole<T, 8 / V, 1, 1>, a, 1, 1, s);
-  if (need <= 1024) return go(k_policy_whole<T, 32 / V, 1, 1>, a, 1, 1, s);
-  if (need <= 6144) return go(k_policy_whole<T, 24 / V, 8, 1>, a, 8, 1, s);
-  if (need <= 16384) return go(k_policy_whole<T, 32 / V, 16, 1>, a, 16, 1, s);
-  constexpr int W = V == 4 ? 32 : 16;  // 8 vectors a thread
-  if (need <= 32768) return go(k_policy_whole<T, 8, W, 1>, a, W, 1, s);
-  return go(k_policy_whole<T, 8, W, 8>, a, W, 8, s);
+  if (need <= 256) return go(k_policy_whole<T, 8 / V>, a, 1, 1, s);
+  if (need <= 1024) return go(k_policy_whole<T, 32 / V>, a, 1, 1, s);
+  if (need * sizeof(T) <= kShort) return go_long<T, 128, 1>(a, s);
+  if (need * sizeof(T) <= kLong) return go_long<T, 256, 1>(a, s);
+  return go_long<T, 512, 8>(a, s);
 }
 template <typename T>
 inline cudaError_t loss_as(const LossArg& a, cudaStream_t s) {
