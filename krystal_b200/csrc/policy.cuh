@@ -995,38 +995,40 @@ template <typename T> struct Floor { static constexpr float value = -1.00025555e
 template <> struct Floor<__half> { static constexpr float value = -65504.0f; };
 
 
-// Raises a vector's entries to the floor (a NaN too) and takes their largest into mx.
-template <typename T> __device__ __forceinline__ void raise(uint32_t* w, float& mx);
-template <> __device__ __forceinline__ void raise<float>(uint32_t* w, float& mx) {
+// The largest of a thread's vectors; raise() also raises a vector's entries to
+// the floor, a NaN too.
+template <typename T> struct Top;
+template <> struct Top<float> {
+  float top = Floor<float>::value;
+  __device__ __forceinline__ void raise(uint32_t* w) {
 #pragma unroll
-  for (int e = 0; e < 4; e++) {
-    const float f = fmaxf(__uint_as_float(w[e]), Floor<float>::value);
-    w[e] = __float_as_uint(f);
-    mx = fmaxf(mx, f);
+    for (int e = 0; e < 4; e++) {
+      const float f = fmaxf(__uint_as_float(w[e]), Floor<float>::value);
+      w[e] = __float_as_uint(f);
+      top = fmaxf(top, f);
+    }
   }
-}
-template <> __device__ __forceinline__ void raise<__half>(uint32_t* w, float& mx) {
-  const __half2 low = __float2half2_rn(Floor<__half>::value);
-  __half2 top = low;
+  __device__ __forceinline__ float value() const { return top; }
+};
+template <typename T2> struct TopPairs {
+  T2 low, top;
+  __device__ __forceinline__ TopPairs(T2 l) : low(l), top(l) {}
+  __device__ __forceinline__ void raise(uint32_t* w) {
 #pragma unroll
-  for (int e = 0; e < 4; e++) {
-    const __half2 f = __hmax2(*reinterpret_cast<__half2*>(w + e), low);
-    w[e] = *reinterpret_cast<const uint32_t*>(&f);
-    top = __hmax2(top, f);
+    for (int e = 0; e < 4; e++) {
+      const T2 f = __hmax2(*reinterpret_cast<T2*>(w + e), low);
+      w[e] = *reinterpret_cast<const uint32_t*>(&f);
+      top = __hmax2(top, f);
+    }
   }
-  mx = fmaxf(mx, fmaxf(__low2float(top), __high2float(top)));
-}
-template <> __device__ __forceinline__ void raise<__nv_bfloat16>(uint32_t* w, float& mx) {
-  const __nv_bfloat162 low = __float2bfloat162_rn(Floor<__nv_bfloat16>::value);
-  __nv_bfloat162 top = low;
-#pragma unroll
-  for (int e = 0; e < 4; e++) {
-    const __nv_bfloat162 f = __hmax2(*reinterpret_cast<__nv_bfloat162*>(w + e), low);
-    w[e] = *reinterpret_cast<const uint32_t*>(&f);
-    top = __hmax2(top, f);
-  }
-  mx = fmaxf(mx, fmaxf(__low2float(top), __high2float(top)));
-}
+  __device__ __forceinline__ float value() const { return fmaxf(__low2float(top), __high2float(top)); }
+};
+template <> struct Top<__half> : TopPairs<__half2> {
+  __device__ __forceinline__ Top() : TopPairs(__float2half2_rn(Floor<__half>::value)) {}
+};
+template <> struct Top<__nv_bfloat16> : TopPairs<__nv_bfloat162> {
+  __device__ __forceinline__ Top() : TopPairs(__float2bfloat162_rn(Floor<__nv_bfloat16>::value)) {}
+};
 
 template <typename T, int NV>
 __global__ void __launch_bounds__(128) k_policy_whole(LossArg a) {
@@ -1049,7 +1051,6 @@ __global__ void __launch_bounds__(128) k_policy_whole(LossArg a) {
 
   // the row, masked entries raised to the floor; its largest
   uint32_t v[NV][4];
-  float mx = -INFINITY;
 #pragma unroll
   for (int c = 0; c < NV; c++) {
     const int i = i0 + c * 32 * V;
@@ -1064,8 +1065,10 @@ __global__ void __launch_bounds__(128) k_policy_whole(LossArg a) {
       for (int e = 0; e < V; e += 2) set2<T>(v[c], e, f[e], f[e + 1]);
     }
   }
+  Top<T> highest;
 #pragma unroll
-  for (int c = 0; c < NV; c++) raise<T>(v[c], mx);
+  for (int c = 0; c < NV; c++) highest.raise(v[c]);
+  const float mx = highest.value();
   // the action's value, before anything is written: grad may lie over values
   const uint32_t act = a.actions[row];
   const bool asked = act != kNone;
@@ -1237,25 +1240,32 @@ __global__ void __launch_bounds__(NT) k_policy_long(LossArg a, uint32_t seg_vecs
   const int mine = max(0, min(int(seg_vecs), vecs - v0)), have = max(0, min(int(seg_vecs) + 1, vecs - v0));
   const int i0 = v0 * V - shift;
 
-  // the row, masked entries raised to the floor; its largest
-  float mx = -INFINITY;
-#pragma unroll 4
+  // the row, by asynchronous copies that are all in flight at once
   for (int j = tid; j < have; j += NT) {
     const int i = i0 + j * V;
-    uint32_t w[4];
     if (i >= 0 && i + V <= n) {
-      const uint4 q = __ldcs(reinterpret_cast<const uint4*>(in + i));
-      w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
+      cp_async16(sm + j, in + i);
     } else {
       float f[V];
+      uint32_t w[4];
 #pragma unroll
       for (int e = 0; e < V; e++) f[e] = i + e >= 0 && i + e < n ? as_f32(in[i + e]) : floor_v;
 #pragma unroll
       for (int e = 0; e < V; e += 2) set2<T>(w, e, f[e], f[e + 1]);
+      sm[j] = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    raise<T>(w, mx);
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  // masked entries raised to the floor (a thread's own vectors: no barrier); the largest
+  Top<T> highest;
+#pragma unroll 4
+  for (int j = tid; j < have; j += NT) {
+    const uint4 q = sm[j];
+    uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    highest.raise(w);
     sm[j] = make_uint4(w[0], w[1], w[2], w[3]);
   }
+  const float mx = highest.value();
   // the action's value, before anything is written: grad may lie over values
   const uint32_t act = a.actions[row];
   const bool asked = act != kNone;
