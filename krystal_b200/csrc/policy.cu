@@ -14,16 +14,16 @@ cudaError_t prepare() {
   return cudaSuccess;
 }
 
-cudaError_t launch_draw(const DrawArg& a, int dtype, cudaStream_t stream, uint64_t* launches) {
+cudaError_t launch_draw(const DrawArg& a, int dtype, int sms, cudaStream_t stream, uint64_t* launches) {
   if (a.r.rows == 0) return cudaSuccess;
   ++*launches;
-  return dtype == kF32 ? draw_f32(a, stream) : dtype == kF16 ? draw_f16(a, stream) : draw_bf16(a, stream);
+  return dtype == kF32 ? draw_f32(a, sms, stream) : dtype == kF16 ? draw_f16(a, sms, stream) : draw_bf16(a, sms, stream);
 }
 
-cudaError_t launch_policy_loss(const LossArg& a, int dtype, cudaStream_t stream, uint64_t* launches) {
+cudaError_t launch_policy_loss(const LossArg& a, int dtype, int sms, cudaStream_t stream, uint64_t* launches) {
   if (a.r.rows == 0) return cudaSuccess;
   ++*launches;
-  return dtype == kF32 ? loss_f32(a, stream) : dtype == kF16 ? loss_f16(a, stream) : loss_bf16(a, stream);
+  return dtype == kF32 ? loss_f32(a, sms, stream) : dtype == kF16 ? loss_f16(a, sms, stream) : loss_bf16(a, sms, stream);
 }
 
 }  // namespace pol

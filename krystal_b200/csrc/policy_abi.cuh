@@ -28,7 +28,7 @@ kc_status check_sampling(kc_handle* h, const kc_sampling* s, bool learns) {
 }
 
 kc::pol::CutArg cut_arg(const kc_sampling* s) {
-  return kc::pol::CutArg{s->temperature, s->top_k, s->top_p, s->min_p,
+  return kc::pol::CutArg{s->temperature > 0.0f ? 1.0 / double(s->temperature) : 0.0, s->temperature, s->top_k, s->top_p, s->min_p,
                          s->row_temperature, s->row_top_k, s->row_top_p, s->row_min_p};
 }
 
@@ -81,7 +81,7 @@ kc_status draw_rows(kc_handle* h, const kc_rows_view* v, const kc_sampling* s, c
   a.kept = out->kept;
   a.logp = out->logp;
   a.p = out->p;
-  KC_TRY(kc::pol::launch_draw(a, v->dtype, h->stream, &h->launches), "draw launch");
+  KC_TRY(kc::pol::launch_draw(a, v->dtype, h->sms, h->stream, &h->launches), "draw launch");
   return KC_OK;
 }
 
@@ -208,7 +208,7 @@ kc_status kc_policy_loss(kc_handle* h, const kc_rows_view* rows, const kc_sampli
   a.logp = loss->logp;
   a.entropy = loss->entropy;
   a.grad = loss->grad;
-  KC_TRY(kc::pol::launch_policy_loss(a, rows->dtype, h->stream, &h->launches), "policy loss launch");
+  KC_TRY(kc::pol::launch_policy_loss(a, rows->dtype, h->sms, h->stream, &h->launches), "policy loss launch");
   return KC_OK;
 }
 

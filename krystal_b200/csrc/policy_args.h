@@ -24,6 +24,7 @@ struct RowsArg {
 };
 
 struct CutArg {
+  double inv_temperature;  // 1 / temperature, 0 at 0
   float temperature;
   uint32_t top_k;
   float top_p, min_p;
@@ -53,12 +54,12 @@ struct LossArg {
 };
 
 // By element type (policy_f32.cu, policy_f16.cu, policy_bf16.cu).
-cudaError_t draw_f32(const DrawArg& a, cudaStream_t s);
-cudaError_t draw_f16(const DrawArg& a, cudaStream_t s);
-cudaError_t draw_bf16(const DrawArg& a, cudaStream_t s);
-cudaError_t loss_f32(const LossArg& a, cudaStream_t s);
-cudaError_t loss_f16(const LossArg& a, cudaStream_t s);
-cudaError_t loss_bf16(const LossArg& a, cudaStream_t s);
+cudaError_t draw_f32(const DrawArg& a, int sms, cudaStream_t s);
+cudaError_t draw_f16(const DrawArg& a, int sms, cudaStream_t s);
+cudaError_t draw_bf16(const DrawArg& a, int sms, cudaStream_t s);
+cudaError_t loss_f32(const LossArg& a, int sms, cudaStream_t s);
+cudaError_t loss_f16(const LossArg& a, int sms, cudaStream_t s);
+cudaError_t loss_bf16(const LossArg& a, int sms, cudaStream_t s);
 
 cudaError_t prepare_f32();
 cudaError_t prepare_f16();
@@ -68,8 +69,8 @@ cudaError_t prepare_bf16();
 cudaError_t prepare();
 
 // One launch each on `stream`; *launches counts it.
-cudaError_t launch_draw(const DrawArg& a, int dtype, cudaStream_t stream, uint64_t* launches);
-cudaError_t launch_policy_loss(const LossArg& a, int dtype, cudaStream_t stream, uint64_t* launches);
+cudaError_t launch_draw(const DrawArg& a, int dtype, int sms, cudaStream_t stream, uint64_t* launches);
+cudaError_t launch_policy_loss(const LossArg& a, int dtype, int sms, cudaStream_t stream, uint64_t* launches);
 
 }  // namespace pol
 

@@ -1,0 +1,754 @@
+// policy_cut.cuh — rows with cuts: the draws (k_draw, k_draw_small) and the
+// policy loss (k_policy_loss, k_policy_loss_small).
+//
+// A row is loaded into registers, E entries a thread: a warp up to 256 entries,
+// a CTA to 32768, a cluster of 8 CTAs beyond. Warp g of the row's group owns
+// the contiguous segment [32 E g, 32 E (g + 1)), in chunks of one 16-byte load
+// a lane, so that bank order is (warp, chunk, lane, entry).
+//
+// What the cuts leave is usually short: a bank's grammar admits few records,
+// and top-k and top-p keep few. So a row is first gathered: its open entries,
+// or with top-k those at or above a lower bound of the k-th largest, go to a
+// list in shared memory in bank order, and if it holds at most kList entries
+// one warp does everything else on it, with one entry a lane and slice
+// (Row<8, 1, 1, 1>). The lower bound is the k-th largest of the chunks' maxima:
+// k chunks reach it, so k entries do. Rows whose list would be longer stay
+// spread over their group.
+#pragma once
+#include "policy.cuh"
+
+namespace kc {
+namespace pol {
+
+constexpr uint32_t kList = 256;
+constexpr uint32_t kListTopK = 208;  // top-k up to this looks for a list
+
+struct List {
+  uint32_t key[kList], where[kList];  // a key, and its index in the row
+};
+
+// Open entries of a row, their smallest and largest key.
+struct Stats {
+  uint32_t open, lo, hi;
+};
+
+// A row's entries (V of them in a vector; V = 1: a gathered list), and its cut.
+template <int E, int V, int W, int CL>
+struct Row {
+  static constexpr int kChunks = E / V;
+  static constexpr uint32_t kCap = uint32_t(32) * E * W * CL;
+  static constexpr bool kCached = E <= 32;  // the registers hold a weight an entry beside the keys
+  static_assert(E % V == 0 && kChunks <= 32, "a thread holds whole vectors");
+
+  Group<W, CL> g;
+  const Tables& t;
+  uint32_t k[E];   // keys; 0: not in the support
+  uint32_t live;   // chunks of this warp that hold an entry of the support
+  int slices;      // of a list: 32 entries each
+  double m, log_m, inv_t;
+  bool power;      // probabilities at a temperature other than 1: x from logarithms
+  bool plain_p;    // probabilities at T = 1: the weights are the values
+  int i0;          // index of this lane's first entry of chunk 0
+  const uint32_t* where;  // a list's indices
+
+  __device__ Row(typename Group<W, CL>::Shared& sh, const Tables& tables, int lane, int warp)
+      : g(sh, lane, warp), t(tables) {}
+
+  __device__ int at(int c) const { return i0 + c * 32 * V; }
+  __device__ uint32_t index(int e) const {
+    if constexpr (V == 1) return where[e * 32 + g.lane];
+    else return uint32_t(at(e / V) + e % V);
+  }
+
+  // f(entry) for every entry of the chunks that hold any; the warp together.
+  template <typename F>
+  __device__ __forceinline__ void each(F f) {
+#pragma unroll
+    for (int c = 0; c < kChunks; c++) {
+      if constexpr (V == 1) {
+        if (c >= slices) break;
+      }
+      if (V == 1 || (live >> c & 1u)) {
+#pragma unroll
+        for (int e = 0; e < V; e++) f(c * V + e);
+      }
+    }
+  }
+  __device__ void find_live() {
+    if constexpr (V == 1) return;
+    live = 0;
+#pragma unroll
+    for (int c = 0; c < kChunks; c++) {
+      uint32_t any = 0;
+#pragma unroll
+      for (int e = 0; e < V; e++) any |= k[c * V + e];
+      if (__any_sync(0xffffffffu, any != 0u)) live |= 1u << c;
+    }
+  }
+
+  // Loads n entries from row. A lane's 16-byte loads start on 16-byte
+  // boundaries; a vector that reaches past either end of the row is read
+  // entry by entry.
+  template <typename T>
+  __device__ void load(const T* row, uint32_t n, int kind) {
+    static_assert(V == 16 / int(sizeof(T)), "a vector is 16 bytes");
+    const int shift = int((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+    i0 = g.segment() * 32 * E + g.lane * V - shift;
+#pragma unroll
+    for (int c = 0; c < kChunks; c++) {
+      const int i = at(c);
+      if (i >= 0 && i + V <= int(n)) {
+        const uint4 q = __ldcs(reinterpret_cast<const uint4*>(row + i));
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int e = 0; e < V; e++) k[c * V + e] = open_key<T>(entry<T>(w, e), kind);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; e++)
+          k[c * V + e] = i + e >= 0 && i + e < int(n) ? open_key<T>(as_f32(row[i + e]), kind) : 0u;
+      }
+    }
+    find_live();
+  }
+  // Takes up a list of n entries.
+  __device__ void take(const List& list, uint32_t n) {
+    where = list.where;
+    slices = int((n + 31) / 32);
+#pragma unroll
+    for (int c = 0; c < kChunks; c++) {
+      const uint32_t j = uint32_t(c) * 32 + g.lane;
+      k[c] = j < n ? list.key[j] : 0u;
+    }
+  }
+  __device__ bool in_use(int c) const { return V == 1 ? c < slices : (live >> c & 1u); }
+
+  __device__ Stats stats() {
+    Stats s{0u, 0xffffffffu, 0u};
+    each([&](int e) {
+      s.open += k[e] != 0u;
+      if (k[e]) s.lo = min(s.lo, k[e]);
+      s.hi = max(s.hi, k[e]);
+    });
+    g.counts(s.open, s.lo, s.hi);
+    return s;
+  }
+
+  // A key that at least `want` entries reach, few more: see the head of the file.
+  __device__ uint32_t lower_bound(uint32_t want, const Stats& s, int kind) {
+    uint32_t best[kChunks], lo = 0xffffffffu, cur = 0u, all = 0u;
+#pragma unroll
+    for (int c = 0; c < kChunks; c++) {
+      best[c] = 0u;
+#pragma unroll
+      for (int e = 0; e < V; e++) best[c] = max(best[c], k[c * V + e]);
+      all += best[c] != 0u;
+      if (best[c]) lo = min(lo, best[c]);
+      cur = max(cur, best[c]);
+    }
+    g.counts(all, lo, cur);
+    if (all < want) return s.lo;
+    for (int step = 0; cur != lo; step++) {
+      const uint32_t p = pivot(lo, cur, step, kind);
+      uint32_t n = 0, mn = 0xffffffffu, mx = 0u;
+#pragma unroll
+      for (int c = 0; c < kChunks; c++) {
+        if (best[c] >= p) { n++; mn = min(mn, best[c]); }
+        else mx = max(mx, best[c]);
+      }
+      g.counts(n, mn, mx);
+      if (n >= want) {
+        lo = mn;
+        if (n <= want + want / 16 + 4) break;
+      } else {
+        cur = mx;
+      }
+    }
+    return lo;
+  }
+
+  // The entries at or above `from` into the list, in bank order; the caller
+  // knows that they fit. A barrier has to follow.
+  __device__ void gather(uint32_t from, List* list) {
+    uint32_t mine = 0;
+    each([&](int e) { mine += k[e] >= from; });
+    uint32_t seen = g.ahead(__reduce_add_sync(0xffffffffu, mine));
+#pragma unroll
+    for (int c = 0; c < kChunks; c++) {
+      if (!in_use(c)) continue;
+      uint32_t in = 0;
+#pragma unroll
+      for (int e = 0; e < V; e++) in += k[c * V + e] >= from;
+      const uint32_t incl = warp_scan(in, g.lane);
+      uint32_t r = seen + incl - in;
+#pragma unroll
+      for (int e = 0; e < V; e++)
+        if (k[c * V + e] >= from) {
+          list->key[r] = k[c * V + e];
+          list->where[r] = index(c * V + e);
+          r++;
+        }
+      seen += __shfl_sync(0xffffffffu, incl, 31);
+    }
+  }
+
+  // The tempered log weight of a key in the support (a key outside it: some
+  // number). Every lane of the warp calls this together.
+  __device__ double x_of(uint32_t key) const {
+    const float v = value_of(key ? key : 0xbf800000u);
+    return power ? (log_tab(v, t.c, t.l) - log_m) * inv_t : (double(v) - m) * inv_t;
+  }
+  // The weight of an x, and of a key; 0 for key 0 and for dropped entries.
+  __device__ double weight_of(uint32_t key, double x) const {
+    const double w = exp64(fmin(fmax(x, kDropped), 0.0), t.e2);
+    return key && x >= kDropped ? w : 0.0;
+  }
+  __device__ double weight(uint32_t key) const {
+    if (plain_p) return key ? double(value_of(key)) : 0.0;
+    return weight_of(key, x_of(key));
+  }
+
+  // The pivot between two values of the row: halfway in value for scores,
+  // halfway in exponent and mantissa for probabilities (which span decades);
+  // after a dozen steps the two alternate, so that no row takes more than
+  // about 70 steps whatever its values.
+  __device__ static uint32_t pivot(uint32_t lo, uint32_t hi, int step, int kind) {
+    const bool by_value = step < 12 ? kind != kKindP : (step & 1);
+    uint32_t p = lo + (hi - lo + 1) / 2;
+    if (by_value) p = key_of(0.5f * value_of(lo) + 0.5f * value_of(hi));
+    return min(max(p, lo + 1), hi);
+  }
+
+  // Drops the entries below the cut c and all but the first `ties` of the
+  // `all` at it.
+  __device__ void apply(uint32_t cut, uint32_t ties, uint32_t all) {
+    if (ties >= all) {
+      each([&](int e) { if (k[e] < cut) k[e] = 0u; });
+    } else {
+      uint32_t mine = 0;
+      each([&](int e) { mine += k[e] == cut; });
+      uint32_t seen = g.ahead(__reduce_add_sync(0xffffffffu, mine));
+#pragma unroll
+      for (int c = 0; c < kChunks; c++) {
+        if (!in_use(c)) continue;
+        uint32_t in = 0;
+#pragma unroll
+        for (int e = 0; e < V; e++) in += k[c * V + e] == cut;
+        const uint32_t incl = warp_scan(in, g.lane);
+        uint32_t r = seen + incl - in;
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+          const uint32_t key = k[c * V + e];
+          if (key == cut) {
+            if (r >= ties) k[c * V + e] = 0u;
+            r++;
+          } else if (key < cut) {
+            k[c * V + e] = 0u;
+          }
+        }
+        seen += __shfl_sync(0xffffffffu, incl, 31);
+      }
+    }
+    find_live();
+  }
+
+  // top-p's search by approximate weights: f32 exponentials in units of 2^-20
+  // of the largest, summed as integers. An entry above half a unit has |x| <=
+  // 21 ln 2; three f32 roundings of the exponent and ex2's 2^-22 put its weight
+  // within 3e-6, and for probabilities lg2's 2^-22 of log2 v and of log2 m add
+  // 3.4e-7 (|log2 m| + 21 T) / T. A mass that clears the goal by `err` of the
+  // total and half a unit an entry is on its side for certain; the first pivot
+  // that does not leaves [lo, cur] to the 64-bit search. What it usually
+  // leaves is one value.
+  __device__ void narrow(double top_p, uint32_t open, int kind, uint32_t& lo, uint32_t& cur) {
+    uint32_t q[E], all = 0;
+    const float mv = float(m), it = float(inv_t) * (kind == kKindP ? 1.0f : 1.44269504f);
+    const float mu = kind == kKindP ? log2_fast(mv) : mv;
+    each([&](int e) {
+      const float v = value_of(k[e] ? k[e] : 0xbf800000u);
+      const float u = ((kind == kKindP ? log2_fast(v) : v) - mu) * it;
+      q[e] = k[e] ? __float2uint_rn(exp2_fast(fminf(u, 0.0f)) * 1048576.0f) : 0u;
+      all += q[e];
+    });
+    const double total = g.sum_u32(all);
+    const double goal = top_p * total;
+    const double err = (1e-5 + 1e-5 * inv_t + 4e-7 * fabs(double(mu)) * (kind == kKindP ? inv_t : 0.0)) * total +
+                       0.5 * open + 1.0;
+    const double above = goal + err, below = goal - err;
+    for (int step = 0; cur != lo; step++) {
+      const uint32_t p = pivot(lo, cur, step, kind);
+      uint32_t mass = 0, mn = 0xffffffffu, mx = 0u;
+      each([&](int e) {
+        if (k[e] >= p) { mass += q[e]; mn = min(mn, k[e]); }
+        else mx = max(mx, k[e]);
+      });
+      const double a = g.masses(mass, mn, mx);
+      if (a >= above) lo = mn;
+      else if (a < below) cur = mx;
+      else return;
+    }
+  }
+
+  // What the weights need of the row: s.hi is its largest key.
+  __device__ void begin(const Cut& c, const Stats& s, int kind) {
+    plain_p = kind == kKindP && c.inv_t == 1.0;
+    power = kind == kKindP && !plain_p;
+    inv_t = c.inv_t;
+    m = s.open ? double(value_of(s.hi)) : 0.0;
+    log_m = power && s.open ? log_tab(value_of(s.hi), t.c, t.l) : 0.0;
+  }
+
+  // The cuts; afterwards k[e] != 0 exactly for what top-k and top-p keep (min-p
+  // and the dropping are left to the weights' pass).
+  __device__ void cut(const Cut& c, const Stats& s, int kind) {
+    if (s.open == 0) return;
+    uint32_t left = s.open, lo = s.lo;
+    const uint32_t top = s.hi;
+    if (c.k && c.k < s.open) {
+      // the largest t with count(k >= t) >= c.k; `above`: count(k > t's bracket)
+      uint32_t cur = top, above = 0, at_lo = s.open;
+      for (int step = 0; cur != lo; step++) {
+        const uint32_t p = pivot(lo, cur, step, kind);
+        uint32_t n = 0, mn = 0xffffffffu, mx = 0u;
+        each([&](int e) {
+          if (k[e] >= p) { n++; mn = min(mn, k[e]); }
+          else mx = max(mx, k[e]);
+        });
+        g.counts(n, mn, mx);
+        if (n >= c.k) { lo = mn; at_lo = n; }
+        else { cur = mx; above = n; }
+      }
+      apply(lo, c.k - above, at_lo - above);
+      left = c.k;
+    }
+    if (c.top_p < 1.0) {
+      // the largest t with mass(k >= t) >= goal
+      uint32_t cur = top;
+      if constexpr (kCached) narrow(c.top_p, left, kind, lo, cur);
+      uint32_t ties = 0, mn = 0xffffffffu, mx = 0u;
+      each([&](int e) { ties += k[e] == lo; });
+      g.counts(ties, mn, mx);
+      if (cur != lo || ties > 1) {
+        double part = 0.0, over = 0.0;
+        each([&](int e) {
+          const double w = weight(k[e]);
+          part += w;
+          if (k[e] > cur) over += w;
+        });
+        const double goal = c.top_p * g.sum(part);
+        double above = g.sum(over);
+        for (int step = 0; cur != lo; step++) {
+          const uint32_t p = pivot(lo, cur, step, kind);
+          double mass = 0.0;
+          uint32_t n = 0;
+          mn = 0xffffffffu, mx = 0u;
+          each([&](int e) {
+            const bool in = k[e] >= p && k[e] <= cur;
+            if (__any_sync(0xffffffffu, in)) mass += weight(in ? k[e] : 0u);
+            if (k[e] >= p) mn = min(mn, k[e]);
+            else mx = max(mx, k[e]);
+          });
+          mass = above + g.sum(mass);
+          g.counts(n, mn, mx);
+          if (mass >= goal) lo = mn;
+          else { cur = mx; above = mass; }
+        }
+        ties = 0, mn = 0xffffffffu, mx = 0u;
+        each([&](int e) { ties += k[e] == lo; });
+        g.counts(ties, mn, mx);
+        const double w = weight(lo);
+        const double need = w > 0.0 ? ceil((goal - above) / w) : 1.0;
+        apply(lo, need < 1.0 ? 1u : need >= double(ties) ? ties : uint32_t(need), ties);
+      } else {
+        apply(lo, 1u, 1u);
+      }
+    }
+  }
+};
+
+using ListRow = Row<kList / 32, 1, 1, 1>;
+
+// The cuts of a list of up to 32 S entries by sorting its keys (a bitonic
+// network over the lanes): both cuts are then prefixes, and their masses one
+// scan of exact weights. Against the search this is a third of the
+// instructions for 32 entries and half for 64; the ties go by bank order as
+// there.
+template <int S>
+__device__ __forceinline__ void cut_sorted(ListRow& r, const Cut& c) {
+  const int lane = r.g.lane;
+  uint32_t k[S];
+#pragma unroll
+  for (int s = 0; s < S; s++) k[s] = r.k[s];
+#pragma unroll
+  for (int size = 2; size <= 32 * S; size *= 2) {
+#pragma unroll
+    for (int stride = size / 2; stride; stride /= 2) {
+      if (stride == 32) {
+        const uint32_t a = max(k[0], k[S - 1]), b = min(k[0], k[S - 1]);
+        k[0] = a;
+        k[S - 1] = b;
+      } else {
+#pragma unroll
+        for (int s = 0; s < S; s++) {
+          const uint32_t o = __shfl_xor_sync(0xffffffffu, k[s], stride);
+          const bool falling = size == 64 ? true : (((s * 32 + lane) & size) == 0);
+          k[s] = falling == ((lane & stride) == 0) ? max(k[s], o) : min(k[s], o);
+        }
+      }
+    }
+  }
+  // position p = 32 s + lane of the descending order; those past top-k weigh nothing
+  const uint32_t most = c.k ? c.k : 32u * S;
+  uint32_t keep = 0;
+  if (c.top_p < 1.0) {
+    double w[S], before[S], run = 0.0;
+#pragma unroll
+    for (int s = 0; s < S; s++) {
+      w[s] = r.weight(uint32_t(s * 32 + lane) < most ? k[s] : 0u);
+      const double sc = warp_scan(w[s], lane);
+      before[s] = run + (sc - w[s]);
+      run += __shfl_sync(0xffffffffu, sc, 31);
+    }
+    const double goal = c.top_p * run;
+#pragma unroll
+    for (int s = 0; s < S; s++) {
+      const uint32_t p = uint32_t(s * 32 + lane);
+      keep += __popc(__ballot_sync(0xffffffffu, k[s] && p < most && (before[s] < goal || p == 0)));
+    }
+  } else {
+#pragma unroll
+    for (int s = 0; s < S; s++) keep += __popc(__ballot_sync(0xffffffffu, k[s] && uint32_t(s * 32 + lane) < most));
+  }
+  if (keep == 0) return;
+  uint32_t cut = __shfl_sync(0xffffffffu, k[0], (keep - 1) & 31);
+  if (S > 1 && keep > 32) cut = __shfl_sync(0xffffffffu, k[S - 1], (keep - 1) & 31);
+  uint32_t ties = 0, all = 0;
+#pragma unroll
+  for (int s = 0; s < S; s++) {
+    const uint32_t at = __ballot_sync(0xffffffffu, k[s] == cut);
+    all += __popc(at);
+    ties += __popc(at & __ballot_sync(0xffffffffu, uint32_t(s * 32 + lane) < keep));
+  }
+  r.apply(cut, ties, all);
+}
+
+// A list's cuts, from its n entries.
+__device__ __forceinline__ void cut_list(ListRow& r, const Cut& c, const Stats& s, uint32_t n, int kind) {
+  if (!(c.k && c.k < n) && !(c.top_p < 1.0)) return;
+  if (n <= 32) cut_sorted<1>(r, c);
+  else if (n <= 64) cut_sorted<2>(r, c);
+  else r.cut(c, s, kind);
+}
+
+// The draw of a row after its cuts. A list's pi go into a row that was cleared.
+template <typename R, int V>
+__device__ __forceinline__ void finish(R& r, const Cut& c, const DrawArg& a, uint32_t row, const RowAt& at, int n,
+                                       bool fits) {
+  constexpr int E = sizeof(r.k) / 4;
+  const int lane = r.g.lane;
+  // the weights, their prefix sums chunk by chunk in bank order
+  const double floor_w = c.min_p * (r.plain_p ? r.m : 1.0);
+  double incl[R::kChunks], w[R::kCached ? E : 1], run = 0.0;
+  uint32_t kept = 0, last = 0u;
+#pragma unroll
+  for (int ch = 0; ch < R::kChunks; ch++) {
+    incl[ch] = run;
+    if (!r.in_use(ch)) continue;
+    double s = 0.0;
+#pragma unroll
+    for (int e = ch * V; e < ch * V + V; e++) {
+      double we = r.weight(r.k[e]);
+      if (we < floor_w) we = 0.0;
+      if (!(we > 0.0)) r.k[e] = 0u;
+      if constexpr (R::kCached) w[e] = we;
+      s += we;
+      if (r.k[e]) {
+        kept++;
+        last = r.index(e) + 1u;
+      }
+    }
+    const double sc = warp_scan(s, lane);
+    incl[ch] = run + sc;
+    run += __shfl_sync(0xffffffffu, sc, 31);
+  }
+  auto weight = [&](int e) {
+    if constexpr (R::kCached) return w[e];
+    else return r.weight(r.k[e]);
+  };
+  double before;
+  const double z = r.g.sum(lane == 31 ? run : 0.0, &before);
+  // the first entry whose prefix passes u z, or (no u) the first largest
+  uint32_t hit = 0xffffffffu;
+  if (a.uniforms) {
+    // cum > u z by the sign of u z - cum, whose one rounding keeps it: u on an
+    // entry's edge falls where the reals put it
+    const double u = fmin(fmax(a.uniforms[row], 0.0), 1.0);
+#pragma unroll
+    for (int ch = 0; ch < R::kChunks; ch++) {
+      const bool past = r.in_use(ch) && fma(u, z, -(before + incl[ch])) < 0.0;
+      if (hit == 0xffffffffu && __any_sync(0xffffffffu, past)) {
+        // the first such lane walks its entries from the prefix ahead of it
+        const int who = __ffs(__ballot_sync(0xffffffffu, past)) - 1;
+        double ws[V], own = 0.0;
+#pragma unroll
+        for (int e = 0; e < V; e++) own += ws[e] = weight(ch * V + e);
+        double cum = before + (incl[ch] - own);
+        uint32_t found = 0xffffffffu;
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+          cum += ws[e];
+          if (found == 0xffffffffu && r.k[ch * V + e] && fma(u, z, -cum) < 0.0) found = r.index(ch * V + e);
+        }
+        if (found == 0xffffffffu) {  // a last bit short: the lane's last kept entry
+#pragma unroll
+          for (int e = 0; e < V; e++)
+            if (r.k[ch * V + e]) found = r.index(ch * V + e);
+        }
+        hit = __shfl_sync(0xffffffffu, found, who);
+      }
+    }
+  } else {
+    const uint32_t top = key_of(float(r.m));
+    r.each([&](int e) {
+      if (r.k[e] == top) hit = min(hit, r.index(e));
+    });
+  }
+  r.g.counts(kept, hit, last);
+  if (kept && hit == 0xffffffffu) hit = last - 1u;
+  const double inv = kept ? 1.0 / z : 0.0;
+  // the owner of the entry writes the row's answer
+  const bool lead = r.g.segment() == 0 && lane == 0;
+  if (kept == 0) {
+    if (lead) {
+      if (a.index) a.index[row] = kNone;
+      if (a.logp) a.logp[row] = -INFINITY;
+      if (a.kept) a.kept[row] = 0u;
+    }
+  } else {
+    double drawn = 0.0;
+    r.each([&](int e) {
+      const bool mine = r.k[e] && r.index(e) == hit;
+      if (__any_sync(0xffffffffu, mine)) {
+        const double we = weight(e);
+        if (mine) drawn = we;
+      }
+    });
+    if (drawn > 0.0) {
+      if (a.index) a.index[row] = hit;
+      if (a.logp) a.logp[row] = float(log64(drawn * inv));
+    }
+    if (lead && a.kept) a.kept[row] = kept;
+  }
+  if (!a.p || !fits) return;
+  float* out = a.p + at.out;
+  if constexpr (V == 1) {
+    r.each([&](int e) {
+      if (r.k[e]) out[r.index(e)] = float(weight(e) * inv);
+    });
+  } else {
+#pragma unroll
+    for (int ch = 0; ch < R::kChunks; ch++) {
+      const int i = r.at(ch);
+      alignas(16) float v[V];
+#pragma unroll
+      for (int e = 0; e < V; e++) {
+        v[e] = 0.0f;
+        if (r.in_use(ch)) v[e] = float(weight(ch * V + e) * inv);
+      }
+      if (i >= 0 && i + V <= n && (reinterpret_cast<uintptr_t>(out + i) & 15) == 0) {
+#pragma unroll
+        for (int e = 0; e < V; e += 4) *reinterpret_cast<float4*>(out + i + e) = *reinterpret_cast<float4*>(v + e);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; e++)
+          if (i + e >= 0 && i + e < n) out[i + e] = v[e];
+      }
+    }
+  }
+}
+
+// The loss of a row after its cuts, and its gradient:
+//   loss = -A log pi(a) - beta H(pi), H = log Z - sum w x / Z,
+//   dloss/dv_j = (A (pi_j - [j = a]) + beta pi_j (log pi_j + H)) / T
+// for what is kept, 0 elsewhere, times the row's weight.
+template <typename T, typename R, int V>
+__device__ __forceinline__ void finish(R& r, const Cut& c, const LossArg& a, uint32_t row, const RowAt& at, int n,
+                                       bool fits) {
+  constexpr int E = sizeof(r.k) / 4;
+  const int lane = r.g.lane;
+  const uint32_t act = a.actions[row];
+  const bool asked = act != kNone;
+  double part = 0.0, px = 0.0, xa = 0.0;
+  uint32_t kept = 0, live = 0xffffffffu, dummy = 0u;
+  double ws[R::kCached ? E : 1];
+  r.each([&](int e) {
+    uint32_t& key = r.k[e];
+    const double x = r.x_of(key);
+    double w = r.weight_of(key, x);
+    if (w < c.min_p) w = 0.0;
+    if (!(w > 0.0)) key = 0u;
+    if constexpr (R::kCached) ws[e] = w;
+    part += w;
+    px = fma(w, key ? x : 0.0, px);
+    if (key) {
+      kept++;
+      if (r.index(e) == act) { live = 0u; xa = x; }
+    }
+  });
+  const double z = r.g.sum(part);
+  const double sx = r.g.sum(px);
+  xa = r.g.sum(xa);
+  r.g.counts(kept, live, dummy);
+  const double log_z = kept ? log64(z) : 0.0, inv_z = kept ? 1.0 / z : 0.0;
+  const double h = kept ? log_z - sx * inv_z : 0.0;
+  const double logp = xa - log_z;
+  // a temperature that is not positive has one answer and no gradient
+  const bool learns = asked && live == 0u && c.inv_t > 0.0;
+  const double adv = double(a.advantage[row]), beta = double(a.beta);
+  if (r.g.segment() == 0 && lane == 0) {
+    if (a.loss) a.loss[row] = learns ? float(-adv * logp - beta * h) : 0.0f;
+    if (a.logp) a.logp[row] = !asked ? 0.0f : live == 0u ? float(logp) : -INFINITY;
+    if (a.entropy) a.entropy[row] = float(h);
+  }
+  if (!a.grad || !fits) return;
+  T* out = static_cast<T*>(a.grad) + at.out;
+  const double g0 = (a.row_weight ? double(a.row_weight[row]) : 1.0) * c.inv_t, base = h - log_z;
+  auto slope = [&](int e) {
+    const uint32_t key = r.k[e];
+    const double x = r.x_of(key);
+    double pi;
+    if constexpr (R::kCached) pi = ws[e] * inv_z;
+    else pi = r.weight_of(key, x) * inv_z;
+    const double one = key && r.index(e) == act ? 1.0 : 0.0;
+    return key ? float(g0 * fma(adv, pi - one, beta * pi * (x + base))) : 0.0f;
+  };
+  if constexpr (V == 1) {
+    if (learns)
+      r.each([&](int e) {
+        const float d = slope(e);
+        if (r.k[e]) out[r.index(e)] = from_f32<T>(d);
+      });
+  } else {
+    RowWriter<T> writer(out, n, lane, r.i0);
+#pragma unroll
+    for (int ch = 0; ch < R::kChunks; ch++) {
+      float f[V];
+      uint32_t v[4];
+#pragma unroll
+      for (int e = 0; e < V; e++) {
+        f[e] = 0.0f;
+        if (learns && r.in_use(ch)) f[e] = slope(ch * V + e);
+      }
+#pragma unroll
+      for (int e = 0; e < V; e += 2) set2<T>(v, e, f[e], f[e + 1]);
+      writer.put(v, r.at(ch));
+    }
+    writer.finish();
+  }
+}
+
+// The output laid out like the rows, and which of the two finishes it takes.
+template <typename T> __device__ __forceinline__ void clear_out(const DrawArg& a, const RowAt& at, int n, int tid, int threads) {
+  if (a.p) clear_row(a.p + at.out, n, tid, threads);
+}
+template <typename T> __device__ __forceinline__ void clear_out(const LossArg& a, const RowAt& at, int n, int tid, int threads) {
+  if (a.grad) clear_row(static_cast<T*>(a.grad) + at.out, n, tid, threads);
+}
+template <typename T, int V, typename R>
+__device__ __forceinline__ void finish_as(R& r, const Cut& c, const DrawArg& a, uint32_t row, const RowAt& at, int n, bool fits) {
+  finish<R, V>(r, c, a, row, at, n, fits);
+}
+template <typename T, int V, typename R>
+__device__ __forceinline__ void finish_as(R& r, const Cut& c, const LossArg& a, uint32_t row, const RowAt& at, int n, bool fits) {
+  finish<T, R, V>(r, c, a, row, at, n, fits);
+}
+
+// Rows of up to 256 entries: a warp a row, always by its list; a warp goes on
+// to the rows behind, so that its tables are made once.
+template <typename T, typename Arg>
+__global__ void __launch_bounds__(128) k_policy_small(Arg a) {
+  constexpr int V = 16 / int(sizeof(T));
+  __shared__ List lists[4];
+  __shared__ typename Group<1, 1>::Shared none;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const Tables tables(lane, a.r.kind == kKindP);
+  List& list = lists[warp];
+  for (uint32_t row = blockIdx.x * 4 + warp; row < a.r.rows; row += gridDim.x * 4) {
+    RowAt at;
+    if (!locate(a.r, a.out_pitch, row, lane, &at)) return;
+    const bool fits = at.n <= a.r.row_len && at.n + V - 1 <= kList;
+    const int n = fits ? int(at.n) : 0;
+    const T* in = static_cast<const T*>(a.r.values) + at.in;
+    const Cut c = cut_of(a.c, row);
+    uint32_t count = 0;
+    {
+      Row<8, V, 1, 1> whole(none, tables, lane, 0);
+      whole.load(in, uint32_t(n), a.r.kind);
+      uint32_t open = 0;
+      whole.each([&](int e) { open += whole.k[e] != 0u; });
+      count = __reduce_add_sync(0xffffffffu, open);
+      if (fits) clear_out<T>(a, at, n, lane, 32);
+      whole.gather(1u, &list);
+    }
+    __syncwarp();
+    ListRow r(none, tables, lane, 0);
+    r.take(list, count);
+    const Stats s = r.stats();
+    r.begin(c, s, a.r.kind);
+    cut_list(r, c, s, count, a.r.kind);
+    finish_as<T, 1>(r, c, a, row, at, n, fits);
+    __syncwarp();  // the list is written again for the next row
+  }
+}
+
+// Longer rows: CL CTAs of W warps a row.
+template <typename T, int E, int W, int CL, typename Arg>
+__global__ void __launch_bounds__(W * 32) k_policy_rows(Arg a) {
+  constexpr int V = 16 / int(sizeof(T));
+  using R = Row<E, V, W, CL>;
+  __shared__ typename Group<W, CL>::Shared sh;
+  __shared__ typename Group<1, 1>::Shared none;
+  __shared__ List list;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t row = blockIdx.x / CL;
+  RowAt at;
+  if (!locate(a.r, a.out_pitch, row, lane, &at)) return;
+  const Tables tables(lane, a.r.kind == kKindP);
+  R r(sh, tables, lane, warp);
+  const bool fits = at.n <= a.r.row_len && at.n + V - 1 <= R::kCap;
+  const uint32_t n = fits ? uint32_t(at.n) : 0u;
+  r.load(static_cast<const T*>(a.r.values) + at.in, n, a.r.kind);
+  const Cut c = cut_of(a.c, row);
+  Stats s = r.stats();
+  uint32_t from = s.lo, count = s.open;
+  if (s.open > kList && c.k && c.k <= kListTopK) {
+    from = r.lower_bound(c.k, s, a.r.kind);
+    count = 0;
+    uint32_t mn = 0, mx = 0;
+    r.each([&](int e) { count += r.k[e] >= from; });
+    r.g.counts(count, mn, mx);
+  }
+  if (count <= kList) {
+    List* to = &list;
+    if constexpr (CL > 1) to = cooperative_groups::this_cluster().map_shared_rank(&list, 0);
+    r.gather(from ? from : 1u, to);
+    if (fits) clear_out<T>(a, at, int(n), r.g.rank * W * 32 + int(threadIdx.x), W * 32 * CL);
+    if constexpr (CL > 1) cooperative_groups::this_cluster().sync();
+    else __syncthreads();
+    if (r.g.segment() != 0) return;
+    ListRow l(none, tables, lane, 0);
+    l.take(list, count);
+    const Stats ls = l.stats();
+    l.begin(c, ls, a.r.kind);
+    cut_list(l, c, ls, count, a.r.kind);
+    finish_as<T, 1>(l, c, a, row, at, int(n), fits);
+    return;
+  }
+  s.lo = from;
+  s.open = count;
+  r.begin(c, s, a.r.kind);
+  r.cut(c, s, a.r.kind);
+  finish_as<T, V>(r, c, a, row, at, int(n), fits);
+}
+
+}  // namespace pol
+}  // namespace kc

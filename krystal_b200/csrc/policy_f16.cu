@@ -3,8 +3,8 @@
 
 namespace kc {
 namespace pol {
-cudaError_t draw_f16(const DrawArg& a, cudaStream_t s) { return draw_as<__half>(a, s); }
-cudaError_t loss_f16(const LossArg& a, cudaStream_t s) { return loss_as<__half>(a, s); }
+cudaError_t draw_f16(const DrawArg& a, int sms, cudaStream_t s) { return draw_as<__half>(a, sms, s); }
+cudaError_t loss_f16(const LossArg& a, int sms, cudaStream_t s) { return loss_as<__half>(a, sms, s); }
 cudaError_t prepare_f16() { return prepare_as<__half>(); }
 }  // namespace pol
 }  // namespace kc

@@ -3,8 +3,8 @@
 
 namespace kc {
 namespace pol {
-cudaError_t draw_f32(const DrawArg& a, cudaStream_t s) { return draw_as<float>(a, s); }
-cudaError_t loss_f32(const LossArg& a, cudaStream_t s) { return loss_as<float>(a, s); }
+cudaError_t draw_f32(const DrawArg& a, int sms, cudaStream_t s) { return draw_as<float>(a, sms, s); }
+cudaError_t loss_f32(const LossArg& a, int sms, cudaStream_t s) { return loss_as<float>(a, sms, s); }
 cudaError_t prepare_f32() { return prepare_as<float>(); }
 }  // namespace pol
 }  // namespace kc

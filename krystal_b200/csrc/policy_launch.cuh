@@ -2,7 +2,10 @@
 // for one element type; policy_f32.cu, policy_f16.cu and policy_bf16.cu
 // instantiate it, a file a type so that they compile side by side.
 #pragma once
-#include "policy.cuh"
+#include <algorithm>
+
+#include "policy_cut.cuh"
+#include "policy_whole.cuh"
 
 namespace kc {
 namespace pol {
@@ -29,17 +32,25 @@ cudaError_t go(void (*kernel)(A), const A& a, int w, int cl, cudaStream_t stream
 }
 
 // The group that holds the longest row, a vector's misalignment included.
-template <typename T>
-inline cudaError_t draw_as(const DrawArg& a, cudaStream_t s) {
+template <typename T, typename A>
+cudaError_t cut_as(const A& a, int sms, cudaStream_t s) {
   const uint64_t need = a.r.row_len + 16 / sizeof(T) - 1;
   constexpr int kMid = sizeof(T) == 4 ? 20 : 24;  // the largest bank, misaligned, in 8 warps
-  if (need <= 256) return go(k_draw<T, 8, 1, 1>, a, 1, 1, s);
-  if (need <= 1024) return go(k_draw<T, 32, 1, 1>, a, 1, 1, s);
-  if (need <= 8 * 32 * kMid) return go(k_draw<T, kMid, 8, 1>, a, 8, 1, s);
-  if (need <= 16384) return go(k_draw<T, 32, 16, 1>, a, 16, 1, s);
-  if (need <= 32768) return go(k_draw<T, 64, 16, 1>, a, 16, 1, s);
-  return go(k_draw<T, 64, 16, 8>, a, 16, 8, s);
+  if (need <= kList) {
+    const uint64_t ctas = (uint64_t(a.r.rows) + 3) / 4;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(std::min<uint64_t>(ctas, uint64_t(sms) * 8)));
+    cfg.blockDim = dim3(128);
+    cfg.stream = s;
+    return cudaLaunchKernelEx(&cfg, k_policy_small<T, A>, a);
+  }
+  if (need <= 1024) return go(k_policy_rows<T, 8, 4, 1, A>, a, 4, 1, s);
+  if (need <= 8 * 32 * kMid) return go(k_policy_rows<T, kMid, 8, 1, A>, a, 8, 1, s);
+  if (need <= 16384) return go(k_policy_rows<T, 32, 16, 1, A>, a, 16, 1, s);
+  if (need <= 32768) return go(k_policy_rows<T, 64, 16, 1, A>, a, 16, 1, s);
+  return go(k_policy_rows<T, 64, 16, 8, A>, a, 16, 8, s);
 }
+
 // Rows that k_policy_long keeps in shared memory: CL CTAs of NT threads a row,
 // up to kShort bytes a row 128 threads, up to kLong 256 (three CTAs an SM),
 // beyond that a cluster of 8 x 512.
@@ -89,18 +100,15 @@ inline cudaError_t whole_as(const LossArg& a, cudaStream_t s) {
   return go_long<T, 512, 8>(a, s);
 }
 template <typename T>
-inline cudaError_t loss_as(const LossArg& a, cudaStream_t s) {
+inline cudaError_t draw_as(const DrawArg& a, int sms, cudaStream_t s) {
+  return cut_as<T>(a, sms, s);
+}
+template <typename T>
+inline cudaError_t loss_as(const LossArg& a, int sms, cudaStream_t s) {
   const CutArg& c = a.c;
   if (!c.top_k && !c.row_top_k && !(c.top_p < 1.0f) && !c.row_top_p && !(c.min_p > 0.0f) && !c.row_min_p)
     return whole_as<T>(a, s);
-  const uint64_t need = a.r.row_len + 16 / sizeof(T) - 1;
-  constexpr int kMid = sizeof(T) == 4 ? 20 : 24;
-  if (need <= 256) return go(k_policy_loss<T, 8, 1, 1>, a, 1, 1, s);
-  if (need <= 1024) return go(k_policy_loss<T, 32, 1, 1>, a, 1, 1, s);
-  if (need <= 8 * 32 * kMid) return go(k_policy_loss<T, kMid, 8, 1>, a, 8, 1, s);
-  if (need <= 16384) return go(k_policy_loss<T, 32, 16, 1>, a, 16, 1, s);
-  if (need <= 32768) return go(k_policy_loss<T, 64, 16, 1>, a, 16, 1, s);
-  return go(k_policy_loss<T, 64, 16, 8>, a, 16, 8, s);
+  return cut_as<T>(a, sms, s);
 }
 
 }  // namespace pol
