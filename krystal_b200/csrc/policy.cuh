@@ -175,10 +175,14 @@ struct Group {
     double cd[2][CL];
     uint32_t cu[2][3][CL];
   };
-  Shared& s;
+  Shared* s;
   int lane, warp, rank, buf;
 
-  __device__ Group(Shared& sh, int l, int w) : s(sh), lane(l), warp(w), rank(0), buf(0) {
+  // One warp shares nothing.
+  __device__ explicit Group(int l) : s(nullptr), lane(l), warp(0), rank(0), buf(0) {
+    static_assert(W == 1 && CL == 1, "a group of several warps needs shared memory");
+  }
+  __device__ Group(Shared& sh, int l, int w) : s(&sh), lane(l), warp(w), rank(0), buf(0) {
     if constexpr (CL > 1) {
       rank = int(cooperative_groups::this_cluster().block_rank());
       cooperative_groups::this_cluster().sync();  // a CTA's shared memory is written once it runs
@@ -193,25 +197,25 @@ struct Group {
     mx = __reduce_max_sync(0xffffffffu, mx);
     if constexpr (W > 1) {
       buf ^= 1;
-      if (lane == 0) { s.u[buf][0][warp] = add; s.u[buf][1][warp] = mn; s.u[buf][2][warp] = mx; }
+      if (lane == 0) { s->u[buf][0][warp] = add; s->u[buf][1][warp] = mn; s->u[buf][2][warp] = mx; }
       __syncthreads();
       const bool in = lane < W;
-      add = __reduce_add_sync(0xffffffffu, in ? s.u[buf][0][lane] : 0u);
-      mn = __reduce_min_sync(0xffffffffu, in ? s.u[buf][1][lane] : 0xffffffffu);
-      mx = __reduce_max_sync(0xffffffffu, in ? s.u[buf][2][lane] : 0u);
+      add = __reduce_add_sync(0xffffffffu, in ? s->u[buf][0][lane] : 0u);
+      mn = __reduce_min_sync(0xffffffffu, in ? s->u[buf][1][lane] : 0xffffffffu);
+      mx = __reduce_max_sync(0xffffffffu, in ? s->u[buf][2][lane] : 0u);
     }
     if constexpr (CL > 1) {
       namespace cg = cooperative_groups;
       cg::cluster_group cl = cg::this_cluster();
       if (warp == 0 && lane < CL) {
-        uint32_t* dst = cl.map_shared_rank(&s.cu[0][0][0], lane) + buf * 3 * CL;
+        uint32_t* dst = cl.map_shared_rank(&s->cu[0][0][0], lane) + buf * 3 * CL;
         dst[rank] = add; dst[CL + rank] = mn; dst[2 * CL + rank] = mx;
       }
       cl.sync();
       const bool in = lane < CL;
-      add = __reduce_add_sync(0xffffffffu, in ? s.cu[buf][0][lane] : 0u);
-      mn = __reduce_min_sync(0xffffffffu, in ? s.cu[buf][1][lane] : 0xffffffffu);
-      mx = __reduce_max_sync(0xffffffffu, in ? s.cu[buf][2][lane] : 0u);
+      add = __reduce_add_sync(0xffffffffu, in ? s->cu[buf][0][lane] : 0u);
+      mn = __reduce_min_sync(0xffffffffu, in ? s->cu[buf][1][lane] : 0xffffffffu);
+      mx = __reduce_max_sync(0xffffffffu, in ? s->cu[buf][2][lane] : 0u);
     }
   }
   // The group's sum of one value a thread; *before (if asked for) gets the
@@ -220,9 +224,9 @@ struct Group {
     v = warp_add(v);
     if constexpr (W > 1) {
       buf ^= 1;
-      if (lane == 0) s.d[buf][warp] = v;
+      if (lane == 0) s->d[buf][warp] = v;
       __syncthreads();
-      const double sc = warp_scan(lane < W ? s.d[buf][lane] : 0.0, lane);
+      const double sc = warp_scan(lane < W ? s->d[buf][lane] : 0.0, lane);
       if (before) *before = warp ? __shfl_sync(0xffffffffu, sc, warp - 1) : 0.0;
       v = __shfl_sync(0xffffffffu, sc, W - 1);
     } else if (before) {
@@ -231,9 +235,9 @@ struct Group {
     if constexpr (CL > 1) {
       namespace cg = cooperative_groups;
       cg::cluster_group cl = cg::this_cluster();
-      if (warp == 0 && lane < CL) cl.map_shared_rank(&s.cd[0][0], lane)[buf * CL + rank] = v;
+      if (warp == 0 && lane < CL) cl.map_shared_rank(&s->cd[0][0], lane)[buf * CL + rank] = v;
       cl.sync();
-      const double sc = warp_scan(lane < CL ? s.cd[buf][lane] : 0.0, lane);
+      const double sc = warp_scan(lane < CL ? s->cd[buf][lane] : 0.0, lane);
       const double ahead = __shfl_sync(0xffffffffu, sc, rank ? rank - 1 : 0);
       if (before && rank) *before += ahead;
       v = __shfl_sync(0xffffffffu, sc, CL - 1);
@@ -244,16 +248,33 @@ struct Group {
     v = __reduce_max_sync(0xffffffffu, v);
     if constexpr (W > 1) {
       buf ^= 1;
-      if (lane == 0) s.u[buf][0][warp] = v;
+      if (lane == 0) s->u[buf][0][warp] = v;
       __syncthreads();
-      v = __reduce_max_sync(0xffffffffu, lane < W ? s.u[buf][0][lane] : 0u);
+      v = __reduce_max_sync(0xffffffffu, lane < W ? s->u[buf][0][lane] : 0u);
     }
     if constexpr (CL > 1) {
       namespace cg = cooperative_groups;
       cg::cluster_group cl = cg::this_cluster();
-      if (warp == 0 && lane < CL) cl.map_shared_rank(&s.cu[0][0][0], lane)[buf * 3 * CL + rank] = v;
+      if (warp == 0 && lane < CL) cl.map_shared_rank(&s->cu[0][0][0], lane)[buf * 3 * CL + rank] = v;
       cl.sync();
-      v = __reduce_max_sync(0xffffffffu, lane < CL ? s.cu[buf][0][lane] : 0u);
+      v = __reduce_max_sync(0xffffffffu, lane < CL ? s->cu[buf][0][lane] : 0u);
+    }
+    return v;
+  }
+  __device__ uint32_t total(uint32_t v) {
+    v = __reduce_add_sync(0xffffffffu, v);
+    if constexpr (W > 1) {
+      buf ^= 1;
+      if (lane == 0) s->u[buf][0][warp] = v;
+      __syncthreads();
+      v = __reduce_add_sync(0xffffffffu, lane < W ? s->u[buf][0][lane] : 0u);
+    }
+    if constexpr (CL > 1) {
+      namespace cg = cooperative_groups;
+      cg::cluster_group cl = cg::this_cluster();
+      if (warp == 0 && lane < CL) cl.map_shared_rank(&s->cu[0][0][0], lane)[buf * 3 * CL + rank] = v;
+      cl.sync();
+      v = __reduce_add_sync(0xffffffffu, lane < CL ? s->cu[buf][0][lane] : 0u);
     }
     return v;
   }
@@ -271,16 +292,16 @@ struct Group {
     v = warp_pair(v);
     if constexpr (W > 1) {
       buf ^= 1;
-      if (lane == 0) s.f[buf][warp] = v;
+      if (lane == 0) s->f[buf][warp] = v;
       __syncthreads();
-      v = warp_pair(lane < W ? s.f[buf][lane] : nil);
+      v = warp_pair(lane < W ? s->f[buf][lane] : nil);
     }
     if constexpr (CL > 1) {
       namespace cg = cooperative_groups;
       cg::cluster_group cl = cg::this_cluster();
-      if (warp == 0 && lane < CL) cl.map_shared_rank(&s.cf[0][0], lane)[buf * CL + rank] = v;
+      if (warp == 0 && lane < CL) cl.map_shared_rank(&s->cf[0][0], lane)[buf * CL + rank] = v;
       cl.sync();
-      v = warp_pair(lane < CL ? s.cf[buf][lane] : nil);
+      v = warp_pair(lane < CL ? s->cf[buf][lane] : nil);
     }
     return v;
   }
@@ -306,18 +327,18 @@ struct Group {
     uint32_t before = 0;
     if constexpr (W > 1) {
       buf ^= 1;
-      if (lane == 0) s.u[buf][0][warp] = v;
+      if (lane == 0) s->u[buf][0][warp] = v;
       __syncthreads();
-      const uint32_t sc = warp_scan(lane < W ? s.u[buf][0][lane] : 0u, lane);
+      const uint32_t sc = warp_scan(lane < W ? s->u[buf][0][lane] : 0u, lane);
       before = warp ? __shfl_sync(0xffffffffu, sc, warp - 1) : 0u;
       v = __shfl_sync(0xffffffffu, sc, W - 1);
     }
     if constexpr (CL > 1) {
       namespace cg = cooperative_groups;
       cg::cluster_group cl = cg::this_cluster();
-      if (warp == 0 && lane < CL) cl.map_shared_rank(&s.cu[0][0][0], lane)[buf * 3 * CL + rank] = v;
+      if (warp == 0 && lane < CL) cl.map_shared_rank(&s->cu[0][0][0], lane)[buf * 3 * CL + rank] = v;
       cl.sync();
-      const uint32_t sc = warp_scan(lane < CL ? s.cu[buf][0][lane] : 0u, lane);
+      const uint32_t sc = warp_scan(lane < CL ? s->cu[buf][0][lane] : 0u, lane);
       const uint32_t others = __shfl_sync(0xffffffffu, sc, rank ? rank - 1 : 0);
       if (rank) before += others;
     }
@@ -448,7 +469,17 @@ struct RowAt {
   uint64_t in, out;
   uint64_t n;
 };
-__device__ __forceinline__ bool locate(const RowsArg& r, uint64_t out_pitch, uint32_t row, int lane, RowAt* at) {
+// Row `before` of frame f, whose block holds count rows.
+__device__ __forceinline__ void block(const RowsArg& r, uint32_t f, uint64_t count, uint64_t before, RowAt* at) {
+  const uint64_t p0 = r.p_off[f], size = r.p_off[f + 1] - p0;
+  uint64_t n;
+  if ((size | count) >> 32) n = size / count;
+  else n = uint32_t(size) / uint32_t(count);
+  at->in = at->out = p0 + before * n;
+  at->n = n;
+}
+__device__ __forceinline__ bool locate(const RowsArg& r, uint64_t out_pitch, uint32_t row, int lane, RowAt* at,
+                                       uint32_t* frame = nullptr) {
   if (r.frames == 0) {
     *at = RowAt{row * r.pitch, row * out_pitch, r.row_len};
     return true;
@@ -471,14 +502,49 @@ __device__ __forceinline__ bool locate(const RowsArg& r, uint64_t out_pitch, uin
   } else if (row >= r.frames) {
     return false;
   }
-  const uint64_t p0 = r.p_off[lo], block = r.p_off[lo + 1] - p0;
-  uint64_t n;
-  if ((block | count) >> 32) n = block / count;
-  else n = uint32_t(block) / uint32_t(count);
-  const uint64_t at0 = p0 + (row - first) * n;
-  *at = RowAt{at0, at0, n};
+  if (frame) *frame = lo;
+  block(r, lo, count, row - first, at);
   return true;
 }
+
+// The rows from one on, in order: the frame is searched for once.
+struct Walk {
+  RowAt at;
+  uint64_t end;    // the row behind the frame's last
+  uint32_t frame;
+
+  __device__ __forceinline__ bool start(const RowsArg& r, uint64_t out_pitch, uint32_t row, int lane) {
+    if (!locate(r, out_pitch, row, lane, &at, &frame)) return false;
+    pitch_out = out_pitch;
+    end = r.frames == 0 ? ~0ull : r.q_off ? r.q_off[frame + 1] : uint64_t(row) + 1;
+    return true;
+  }
+  // To the next row; false behind the last frame.
+  __device__ __forceinline__ bool step(const RowsArg& r, uint32_t row) {
+    if (r.frames == 0) {
+      at.in += r.pitch;
+      at.out += pitch_out;
+      return true;
+    }
+    if (row < end) {
+      at.in += at.n;
+      at.out = at.in;
+      return true;
+    }
+    uint64_t count = 1;
+    do {  // frames without questions hold no rows
+      if (++frame >= r.frames) return false;
+      const uint64_t from = end;
+      end = r.q_off ? r.q_off[frame + 1] : uint64_t(row) + 1;
+      count = r.q_off ? end - from : 1;
+    } while (row >= end);
+    block(r, frame, count, 0, &at);
+    return true;
+  }
+
+ private:
+  uint64_t pitch_out;
+};
 
 struct Cut {
   double inv_t;     // 0: the largest entry alone

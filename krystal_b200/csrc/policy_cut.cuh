@@ -11,7 +11,7 @@
 // or with top-k those at or above a lower bound of the k-th largest, go to a
 // list in shared memory in bank order, and if it holds at most kList entries
 // one warp does everything else on it, with one entry a lane and slice
-// (Row<8, 1, 1, 1>). The lower bound is the k-th largest of the chunks' maxima:
+// of 32 (ListRow). The lower bound is the k-th largest of the chunks' maxima:
 // k chunks reach it, so k entries do. Rows whose list would be longer stay
 // spread over their group.
 #pragma once
@@ -23,8 +23,10 @@ namespace pol {
 constexpr uint32_t kList = 256;
 constexpr uint32_t kListTopK = 208;  // top-k up to this looks for a list
 
+constexpr int kPairs = 64;  // lists up to this are cut by comparing all pairs
 struct List {
   uint32_t key[kList], where[kList];  // a key, and its index in the row
+  double w[kPairs];
 };
 
 // Open entries of a row, their smallest and largest key.
@@ -45,6 +47,7 @@ struct Row {
   uint32_t k[E];   // keys; 0: not in the support
   uint32_t live;   // chunks of this warp that hold an entry of the support
   int slices;      // of a list: 32 entries each
+  uint32_t top;    // the largest key
   double m, log_m, inv_t;
   bool power;      // probabilities at a temperature other than 1: x from logarithms
   bool plain_p;    // probabilities at T = 1: the weights are the values
@@ -53,6 +56,7 @@ struct Row {
 
   __device__ Row(typename Group<W, CL>::Shared& sh, const Tables& tables, int lane, int warp)
       : g(sh, lane, warp), t(tables) {}
+  __device__ Row(int lane, const Tables& tables) : g(lane), t(tables) {}  // one warp
 
   __device__ int at(int c) const { return i0 + c * 32 * V; }
   __device__ uint32_t index(int e) const {
@@ -120,6 +124,18 @@ struct Row {
       k[c] = j < n ? list.key[j] : 0u;
     }
   }
+  // The stats of a list of n entries; lo only where the search will need it.
+  __device__ Stats list_stats(uint32_t n, bool need_lo) {
+    Stats s{n, 0u, 0u};
+    uint32_t lo = 0xffffffffu;
+    each([&](int e) {
+      s.hi = max(s.hi, k[e]);
+      if (k[e]) lo = min(lo, k[e]);
+    });
+    s.hi = __reduce_max_sync(0xffffffffu, s.hi);
+    s.lo = need_lo ? __reduce_min_sync(0xffffffffu, lo) : 0u;
+    return s;
+  }
   __device__ bool in_use(int c) const { return V == 1 ? c < slices : (live >> c & 1u); }
 
   __device__ Stats stats() {
@@ -135,32 +151,27 @@ struct Row {
 
   // A key that at least `want` entries reach, few more: see the head of the file.
   __device__ uint32_t lower_bound(uint32_t want, const Stats& s, int kind) {
-    uint32_t best[kChunks], lo = 0xffffffffu, cur = 0u, all = 0u;
+    uint32_t best[kChunks], n = 0;
 #pragma unroll
     for (int c = 0; c < kChunks; c++) {
       best[c] = 0u;
 #pragma unroll
       for (int e = 0; e < V; e++) best[c] = max(best[c], k[c * V + e]);
-      all += best[c] != 0u;
-      if (best[c]) lo = min(lo, best[c]);
-      cur = max(cur, best[c]);
+      n += best[c] != 0u;
     }
-    g.counts(all, lo, cur);
-    if (all < want) return s.lo;
-    for (int step = 0; cur != lo; step++) {
+    if (g.total(n) < want) return s.lo;
+    uint32_t lo = s.lo, cur = s.hi;  // count(best >= lo) >= want; cur + 1 does not reach it
+    for (int step = 0; cur > lo && step < 40; step++) {
       const uint32_t p = pivot(lo, cur, step, kind);
-      uint32_t n = 0, mn = 0xffffffffu, mx = 0u;
+      n = 0;
 #pragma unroll
-      for (int c = 0; c < kChunks; c++) {
-        if (best[c] >= p) { n++; mn = min(mn, best[c]); }
-        else mx = max(mx, best[c]);
-      }
-      g.counts(n, mn, mx);
+      for (int c = 0; c < kChunks; c++) n += best[c] >= p;
+      n = g.total(n);
       if (n >= want) {
-        lo = mn;
+        lo = p;
         if (n <= want + want / 16 + 4) break;
       } else {
-        cur = mx;
+        cur = p - 1;
       }
     }
     return lo;
@@ -191,20 +202,25 @@ struct Row {
     }
   }
 
-  // The tempered log weight of a key in the support (a key outside it: some
-  // number). Every lane of the warp calls this together.
+  // The tempered log weight of a key in the support. Every lane of the warp
+  // calls this, and weight, together.
   __device__ double x_of(uint32_t key) const {
-    const float v = value_of(key ? key : 0xbf800000u);
+    const float v = value_of(key);
     return power ? (log_tab(v, t.c, t.l) - log_m) * inv_t : (double(v) - m) * inv_t;
   }
-  // The weight of an x, and of a key; 0 for key 0 and for dropped entries.
-  __device__ double weight_of(uint32_t key, double x) const {
-    const double w = exp64(fmin(fmax(x, kDropped), 0.0), t.e2);
-    return key && x >= kDropped ? w : 0.0;
+  // x of a key (outside the support: 0), and the weight: 0 for key 0 and for
+  // dropped entries.
+  __device__ double weight(uint32_t key, double& x) const {
+    x = x_of(key ? key : top);
+    const bool in = key && x >= kDropped;
+    if (!in) x = 0.0;
+    const double w = exp64(x, t.e2);
+    return in ? w : 0.0;
   }
   __device__ double weight(uint32_t key) const {
     if (plain_p) return key ? double(value_of(key)) : 0.0;
-    return weight_of(key, x_of(key));
+    double x;
+    return weight(key, x);
   }
 
   // The pivot between two values of the row: halfway in value for scores,
@@ -293,8 +309,9 @@ struct Row {
     plain_p = kind == kKindP && c.inv_t == 1.0;
     power = kind == kKindP && !plain_p;
     inv_t = c.inv_t;
-    m = s.open ? double(value_of(s.hi)) : 0.0;
-    log_m = power && s.open ? log_tab(value_of(s.hi), t.c, t.l) : 0.0;
+    top = s.open ? s.hi : 0xbf800000u;  // (some number)
+    m = double(value_of(top));
+    log_m = power ? log_tab(value_of(top), t.c, t.l) : 0.0;
   }
 
   // The cuts; afterwards k[e] != 0 exactly for what top-k and top-p keep (min-p
@@ -365,81 +382,156 @@ struct Row {
   }
 };
 
-using ListRow = Row<kList / 32, 1, 1, 1>;
+template <int S> using ListRow = Row<S, 1, 1, 1>;
 
-// The cuts of a list of up to 32 S entries by sorting its keys (a bitonic
-// network over the lanes): both cuts are then prefixes, and their masses one
-// scan of exact weights. Against the search this is a third of the
-// instructions for 32 entries and half for 64; the ties go by bank order as
-// there.
+// The cuts of a list of up to 32 S entries, without a search: every lane sums
+// up, over the list in shared memory, the entries ahead of its own in
+// descending order (ties in bank order): how many, for top-k, and their exact
+// weights, for top-p. w: the lanes' weights, left at 0 for what is cut.
 template <int S>
-__device__ __forceinline__ void cut_sorted(ListRow& r, const Cut& c) {
+__device__ __forceinline__ void cut_pairs(ListRow<S>& r, const Cut& c, const uint32_t* key, double* shared_w, int n,
+                                          double* w) {
   const int lane = r.g.lane;
-  uint32_t k[S];
+  if (c.k && c.k < uint32_t(n)) {
+    uint32_t bar[S], rank[S];
 #pragma unroll
-  for (int s = 0; s < S; s++) k[s] = r.k[s];
+    for (int s = 0; s < S; s++) {
+      bar[s] = r.k[s];
+      rank[s] = 0u;
+    }
+#pragma unroll 4
+    for (int j = 0; j < n; j++) {
+      const uint32_t kj = key[j];
 #pragma unroll
-  for (int size = 2; size <= 32 * S; size *= 2) {
-#pragma unroll
-    for (int stride = size / 2; stride; stride /= 2) {
-      if (stride == 32) {
-        const uint32_t a = max(k[0], k[S - 1]), b = min(k[0], k[S - 1]);
-        k[0] = a;
-        k[S - 1] = b;
-      } else {
-#pragma unroll
-        for (int s = 0; s < S; s++) {
-          const uint32_t o = __shfl_xor_sync(0xffffffffu, k[s], stride);
-          const bool falling = size == 64 ? true : (((s * 32 + lane) & size) == 0);
-          k[s] = falling == ((lane & stride) == 0) ? max(k[s], o) : min(k[s], o);
-        }
+      for (int s = 0; s < S; s++) {
+        bar[s] += j == s * 32 + lane;  // behind itself, an equal entry is not ahead
+        rank[s] += kj >= bar[s];
       }
     }
+#pragma unroll
+    for (int s = 0; s < S; s++)
+      if (rank[s] >= c.k) {
+        r.k[s] = 0u;
+        w[s] = 0.0;
+      }
   }
-  // position p = 32 s + lane of the descending order; those past top-k weigh nothing
-  const uint32_t most = c.k ? c.k : 32u * S;
-  uint32_t keep = 0;
   if (c.top_p < 1.0) {
-    double w[S], before[S], run = 0.0;
+    uint32_t bar[S];
+    double ahead[S], mine = 0.0;
 #pragma unroll
     for (int s = 0; s < S; s++) {
-      w[s] = r.weight(uint32_t(s * 32 + lane) < most ? k[s] : 0u);
-      const double sc = warp_scan(w[s], lane);
-      before[s] = run + (sc - w[s]);
-      run += __shfl_sync(0xffffffffu, sc, 31);
+      bar[s] = r.k[s];
+      ahead[s] = 0.0;
+      shared_w[s * 32 + lane] = w[s];
+      mine += w[s];
     }
-    const double goal = c.top_p * run;
+    __syncwarp();
+    const double goal = c.top_p * warp_add(mine);
+#pragma unroll 4
+    for (int j = 0; j < n; j++) {
+      const uint32_t kj = key[j];
+      const double wj = shared_w[j];
+#pragma unroll
+      for (int s = 0; s < S; s++) {
+        bar[s] += j == s * 32 + lane;
+        if (kj >= bar[s]) ahead[s] += wj;
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < S; s++)
+      if (!(ahead[s] < goal) && r.k[s] != r.top) {
+        r.k[s] = 0u;
+        w[s] = 0.0;
+      }
+    // the largest entry stays whatever top_p is: the first of its value
+    uint32_t seen = 0u;
 #pragma unroll
     for (int s = 0; s < S; s++) {
-      const uint32_t p = uint32_t(s * 32 + lane);
-      keep += __popc(__ballot_sync(0xffffffffu, k[s] && p < most && (before[s] < goal || p == 0)));
+      const uint32_t at = __ballot_sync(0xffffffffu, r.k[s] == r.top);
+      const bool first = !seen && at && lane == __ffs(at) - 1;
+      if (r.k[s] == r.top && !first && !(ahead[s] < goal)) {
+        r.k[s] = 0u;
+        w[s] = 0.0;
+      }
+      seen |= at;
     }
-  } else {
-#pragma unroll
-    for (int s = 0; s < S; s++) keep += __popc(__ballot_sync(0xffffffffu, k[s] && uint32_t(s * 32 + lane) < most));
   }
-  if (keep == 0) return;
-  uint32_t cut = __shfl_sync(0xffffffffu, k[0], (keep - 1) & 31);
-  if (S > 1 && keep > 32) cut = __shfl_sync(0xffffffffu, k[S - 1], (keep - 1) & 31);
-  uint32_t ties = 0, all = 0;
+}
+
+// What a draw found: the entry (kNone: an empty row), its pi, and how many entries were kept.
+struct Drawn {
+  uint32_t hit, kept;
+  double pi;
+};
+__device__ __forceinline__ void report(const DrawArg& a, uint32_t row, const Drawn& d) {
+  if (a.index) a.index[row] = d.hit;
+  if (a.logp) a.logp[row] = d.hit == kNone ? -INFINITY : float(log64(d.pi));
+  if (a.kept) a.kept[row] = d.kept;
+}
+
+// The draw of a list after its cuts, every lane with the answer; pi go into a
+// row that was cleared. A lane and slice holds one entry, so the entry that a
+// uniform hits is the first one whose prefix passes it.
+template <int S>
+__device__ __forceinline__ Drawn draw_list(ListRow<S>& r, const Cut& c, const DrawArg& a, const RowAt& at, bool fits,
+                                           double u, double* w) {
+  const int lane = r.g.lane;
+  const double floor_w = c.min_p * (r.plain_p ? r.m : 1.0);
+  double incl[S], z = 0.0;
+  uint32_t kept[S];
 #pragma unroll
   for (int s = 0; s < S; s++) {
-    const uint32_t at = __ballot_sync(0xffffffffu, k[s] == cut);
-    all += __popc(at);
-    ties += __popc(at & __ballot_sync(0xffffffffu, uint32_t(s * 32 + lane) < keep));
+    incl[s] = 0.0;
+    kept[s] = 0u;
+    if (!r.in_use(s)) continue;
+    if (w[s] < floor_w) w[s] = 0.0;
+    kept[s] = __ballot_sync(0xffffffffu, w[s] > 0.0);
+    const double sc = warp_scan(w[s], lane);
+    incl[s] = z + sc;
+    z += __shfl_sync(0xffffffffu, sc, 31);
   }
-  r.apply(cut, ties, all);
+  Drawn d{kNone, 0u, 0.0};
+#pragma unroll
+  for (int s = 0; s < S; s++) d.kept += __popc(kept[s]);
+  if (d.kept == 0) return d;
+  const double inv = 1.0 / z;
+  // u z < cum by the sign of u z - cum, whose one rounding keeps it: u on an
+  // entry's edge falls where the reals put it. No u: the first largest entry,
+  // whose weight is the largest there is.
+  int at_s = -1, at_lane = 0;
+#pragma unroll
+  for (int s = 0; s < S; s++) {
+    const bool past = a.uniforms ? fma(u, z, -incl[s]) < 0.0 : r.k[s] == r.top;
+    const uint32_t who = kept[s] & __ballot_sync(0xffffffffu, past);
+    if (at_s < 0 && who) {
+      at_s = s;
+      at_lane = __ffs(who) - 1;
+    }
+  }
+  if (at_s < 0) {  // u of 1, or a last bit short of it: the last kept entry
+#pragma unroll
+    for (int s = 0; s < S; s++)
+      if (kept[s]) {
+        at_s = s;
+        at_lane = 31 - __clz(kept[s]);
+      }
+  }
+  double we = 0.0;
+#pragma unroll
+  for (int s = 0; s < S; s++)
+    if (s == at_s) we = __shfl_sync(0xffffffffu, w[s], at_lane);
+  d.hit = r.where[at_s * 32 + at_lane];
+  d.pi = we * inv;
+  if (a.p && fits) {
+    float* out = a.p + at.out;
+#pragma unroll
+    for (int s = 0; s < S; s++)
+      if (kept[s] >> lane & 1u) out[r.where[s * 32 + lane]] = float(w[s] * inv);
+  }
+  return d;
 }
 
-// A list's cuts, from its n entries.
-__device__ __forceinline__ void cut_list(ListRow& r, const Cut& c, const Stats& s, uint32_t n, int kind) {
-  if (!(c.k && c.k < n) && !(c.top_p < 1.0)) return;
-  if (n <= 32) cut_sorted<1>(r, c);
-  else if (n <= 64) cut_sorted<2>(r, c);
-  else r.cut(c, s, kind);
-}
-
-// The draw of a row after its cuts. A list's pi go into a row that was cleared.
+// The draw of a row that stayed spread over its group, after its cuts.
 template <typename R, int V>
 __device__ __forceinline__ void finish(R& r, const Cut& c, const DrawArg& a, uint32_t row, const RowAt& at, int n,
                                        bool fits) {
@@ -507,9 +599,8 @@ __device__ __forceinline__ void finish(R& r, const Cut& c, const DrawArg& a, uin
       }
     }
   } else {
-    const uint32_t top = key_of(float(r.m));
     r.each([&](int e) {
-      if (r.k[e] == top) hit = min(hit, r.index(e));
+      if (r.k[e] == r.top) hit = min(hit, r.index(e));
     });
   }
   r.g.counts(kept, hit, last);
@@ -540,28 +631,22 @@ __device__ __forceinline__ void finish(R& r, const Cut& c, const DrawArg& a, uin
   }
   if (!a.p || !fits) return;
   float* out = a.p + at.out;
-  if constexpr (V == 1) {
-    r.each([&](int e) {
-      if (r.k[e]) out[r.index(e)] = float(weight(e) * inv);
-    });
-  } else {
 #pragma unroll
-    for (int ch = 0; ch < R::kChunks; ch++) {
-      const int i = r.at(ch);
-      alignas(16) float v[V];
+  for (int ch = 0; ch < R::kChunks; ch++) {
+    const int i = r.at(ch);
+    alignas(16) float v[V];
 #pragma unroll
-      for (int e = 0; e < V; e++) {
-        v[e] = 0.0f;
-        if (r.in_use(ch)) v[e] = float(weight(ch * V + e) * inv);
-      }
-      if (i >= 0 && i + V <= n && (reinterpret_cast<uintptr_t>(out + i) & 15) == 0) {
+    for (int e = 0; e < V; e++) {
+      v[e] = 0.0f;
+      if (r.in_use(ch)) v[e] = float(weight(ch * V + e) * inv);
+    }
+    if (i >= 0 && i + V <= n && (reinterpret_cast<uintptr_t>(out + i) & 15) == 0) {
 #pragma unroll
-        for (int e = 0; e < V; e += 4) *reinterpret_cast<float4*>(out + i + e) = *reinterpret_cast<float4*>(v + e);
-      } else {
+      for (int e = 0; e < V; e += 4) *reinterpret_cast<float4*>(out + i + e) = *reinterpret_cast<float4*>(v + e);
+    } else {
 #pragma unroll
-        for (int e = 0; e < V; e++)
-          if (i + e >= 0 && i + e < n) out[i + e] = v[e];
-      }
+      for (int e = 0; e < V; e++)
+        if (i + e >= 0 && i + e < n) out[i + e] = v[e];
     }
   }
 }
@@ -582,8 +667,7 @@ __device__ __forceinline__ void finish(R& r, const Cut& c, const LossArg& a, uin
   double ws[R::kCached ? E : 1];
   r.each([&](int e) {
     uint32_t& key = r.k[e];
-    const double x = r.x_of(key);
-    double w = r.weight_of(key, x);
+    double x, w = r.weight(key, x);
     if (w < c.min_p) w = 0.0;
     if (!(w > 0.0)) key = 0u;
     if constexpr (R::kCached) ws[e] = w;
@@ -614,10 +698,13 @@ __device__ __forceinline__ void finish(R& r, const Cut& c, const LossArg& a, uin
   const double g0 = (a.row_weight ? double(a.row_weight[row]) : 1.0) * c.inv_t, base = h - log_z;
   auto slope = [&](int e) {
     const uint32_t key = r.k[e];
-    const double x = r.x_of(key);
-    double pi;
-    if constexpr (R::kCached) pi = ws[e] * inv_z;
-    else pi = r.weight_of(key, x) * inv_z;
+    double x, pi;
+    if constexpr (R::kCached) {
+      x = r.x_of(key ? key : r.top);
+      pi = ws[e] * inv_z;
+    } else {
+      pi = r.weight(key, x) * inv_z;
+    }
     const double one = key && r.index(e) == act ? 1.0 : 0.0;
     return key ? float(g0 * fma(adv, pi - one, beta * pi * (x + base))) : 0.0f;
   };
@@ -662,92 +749,227 @@ __device__ __forceinline__ void finish_as(R& r, const Cut& c, const LossArg& a, 
   finish<T, R, V>(r, c, a, row, at, n, fits);
 }
 
-// Rows of up to 256 entries: a warp a row, always by its list; a warp goes on
-// to the rows behind, so that its tables are made once.
-template <typename T, typename Arg>
-__global__ void __launch_bounds__(128) k_policy_small(Arg a) {
-  constexpr int V = 16 / int(sizeof(T));
-  __shared__ List lists[4];
-  __shared__ typename Group<1, 1>::Shared none;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const Tables tables(lane, a.r.kind == kKindP);
-  List& list = lists[warp];
-  for (uint32_t row = blockIdx.x * 4 + warp; row < a.r.rows; row += gridDim.x * 4) {
-    RowAt at;
-    if (!locate(a.r, a.out_pitch, row, lane, &at)) return;
-    const bool fits = at.n <= a.r.row_len && at.n + V - 1 <= kList;
-    const int n = fits ? int(at.n) : 0;
-    const T* in = static_cast<const T*>(a.r.values) + at.in;
-    const Cut c = cut_of(a.c, row);
-    uint32_t count = 0;
-    {
-      Row<8, V, 1, 1> whole(none, tables, lane, 0);
-      whole.load(in, uint32_t(n), a.r.kind);
-      uint32_t open = 0;
-      whole.each([&](int e) { open += whole.k[e] != 0u; });
-      count = __reduce_add_sync(0xffffffffu, open);
-      if (fits) clear_out<T>(a, at, n, lane, 32);
-      whole.gather(1u, &list);
+// What a warp keeps of its rows' answers until it writes them: lane i has the
+// draw of row first + i, so that the logarithms of 32 rows are one evaluation.
+// A loss needs its own at once.
+template <typename Arg> struct Answers {
+  __device__ double uniform(const Arg&, uint32_t) { return 0.0; }
+  template <typename T, int S>
+  __device__ void take(ListRow<S>& r, const Cut& c, const Arg& a, uint32_t row, const RowAt& at, bool fits, double, double*) {
+    finish<T, ListRow<S>, 1>(r, c, a, row, at, int(at.n), fits);
+  }
+  __device__ void done(const Arg&, uint32_t, int) {}
+};
+template <> struct Answers<DrawArg> {
+  Drawn mine{kNone, 0u, 0.0};
+  int held = 0;
+  __device__ double uniform(const DrawArg& a, uint32_t row) {
+    return a.uniforms ? fmin(fmax(a.uniforms[row], 0.0), 1.0) : 0.0;
+  }
+  template <typename T, int S>
+  __device__ __forceinline__ void take(ListRow<S>& r, const Cut& c, const DrawArg& a, uint32_t row, const RowAt& at, bool fits, double u, double* w) {
+    const Drawn d = draw_list<S>(r, c, a, at, fits, u, w);
+    if (r.g.lane == held) mine = d;
+    if (++held == 32) done(a, row, r.g.lane);
+  }
+  // Writes what is held, the last of it row's.
+  __device__ void done(const DrawArg& a, uint32_t row, int lane) {
+    if (lane < held) report(a, row + 1 - held + lane, mine);
+    held = 0;
+  }
+};
+
+// Everything after the gathering, by one warp on a list of n <= 32 S entries.
+template <typename T, int S, typename Arg>
+__device__ __forceinline__ void list_as(List& list, uint32_t n, const Tables& tables, int lane, const Cut& c,
+                                        const Arg& a, uint32_t row, const RowAt& at, bool fits, double u,
+                                        Answers<Arg>& answers) {
+  ListRow<S> r(lane, tables);
+  r.take(list, n);
+  const bool cuts = (c.k && c.k < n) || c.top_p < 1.0;
+  const Stats s = r.list_stats(n, cuts && S > 2);
+  r.begin(c, s, a.r.kind);
+  double w[S];
+  if constexpr (S <= kPairs / 32) {
+#pragma unroll
+    for (int e = 0; e < S; e++) w[e] = r.weight(r.k[e]);
+    if (cuts) cut_pairs<S>(r, c, list.key, list.w, int(n), w);
+  } else {
+    if (cuts) r.cut(c, s, a.r.kind);
+#pragma unroll
+    for (int e = 0; e < S; e++) {
+      w[e] = 0.0;
+      if (r.in_use(e)) w[e] = r.weight(r.k[e]);
     }
+  }
+  answers.template take<T, S>(r, c, a, row, at, fits, u, w);
+}
+template <typename T, typename Arg>
+__device__ __forceinline__ void list_row(List& list, uint32_t n, const Tables& tables, int lane, const Cut& c,
+                                         const Arg& a, uint32_t row, const RowAt& at, bool fits, double u,
+                                         Answers<Arg>& answers) {
+  if (n <= 32) list_as<T, 1>(list, n, tables, lane, c, a, row, at, fits, u, answers);
+  else if (n <= 64) list_as<T, 2>(list, n, tables, lane, c, a, row, at, fits, u, answers);
+  else list_as<T, 8>(list, n, tables, lane, c, a, row, at, fits, u, answers);
+}
+
+// Rows of up to 256 entries: a warp a row, always by its list. A warp takes a
+// run of rows one after another: its tables are made once, the frame is
+// searched for once, and the next row's entries and uniform are fetched while
+// it works.
+constexpr int kSmallCtas = 6;  // an SM
+template <typename T, typename Arg>
+__global__ void __launch_bounds__(128, kSmallCtas) k_policy_small(const __grid_constant__ Arg a) {
+  constexpr int V = 16 / int(sizeof(T)), kVecs = int(kList) / 32 / V;
+  __shared__ List lists[4];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t warps = gridDim.x * 4, each = (a.r.rows + warps - 1) / warps;
+  const uint32_t first = (blockIdx.x * 4 + warp) * each, end = min(a.r.rows, first + each);
+  if (first >= a.r.rows) return;
+  Walk walk;
+  if (!walk.start(a.r, a.out_pitch, first, lane)) return;
+  const Tables tables(lane, a.r.kind == kKindP);
+  Answers<Arg> answers;
+  List& list = lists[warp];
+  // A lane's vectors of the row; a vector that reaches past either end of the
+  // row is read entry by entry, with NaN, which no row's support holds, outside.
+  uint32_t q[kVecs][4];
+  double u;
+  auto fits = [&](const RowAt& at) { return at.n <= a.r.row_len && at.n + V - 1 <= kList; };
+  auto fetch = [&](const RowAt& at, uint32_t row) {
+    const int n = fits(at) ? int(at.n) : 0;
+    const T* in = static_cast<const T*>(a.r.values) + at.in;
+    const int i0 = lane * V - int((reinterpret_cast<uintptr_t>(in) & 15) / sizeof(T));
+#pragma unroll
+    for (int v = 0; v < kVecs; v++) {
+      const int i = i0 + v * 32 * V;
+      if (i >= 0 && i + V <= n) {
+        const uint4 x = __ldcs(reinterpret_cast<const uint4*>(in + i));
+        q[v][0] = x.x; q[v][1] = x.y; q[v][2] = x.z; q[v][3] = x.w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) q[v][e] = 0xffffffffu;
+        if (i + V > 0 && i < n) {
+          float f[V];
+#pragma unroll
+          for (int e = 0; e < V; e++) f[e] = i + e >= 0 && i + e < n ? as_f32(in[i + e]) : __uint_as_float(0x7fc00000u);
+#pragma unroll
+          for (int e = 0; e < V; e += 2) set2<T>(q[v], e, f[e], f[e + 1]);
+        }
+      }
+    }
+    u = answers.uniform(a, row);
+  };
+  fetch(walk.at, first);
+  for (uint32_t row = first; row < end; row++) {
+    const RowAt at = walk.at;
+    const bool ok = fits(at);
+    const T* in = static_cast<const T*>(a.r.values) + at.in;
+    const int i0 = lane * V - int((reinterpret_cast<uintptr_t>(in) & 15) / sizeof(T));
+    // the open entries into the list, in bank order
+    uint32_t count = 0;
+#pragma unroll
+    for (int v = 0; v < kVecs; v++) {
+      uint32_t k[V], ahead = 0, all = 0;
+#pragma unroll
+      for (int e = 0; e < V; e++) {
+        k[e] = open_key<T>(entry<T>(q[v], e), a.r.kind);
+        const uint32_t b = __ballot_sync(0xffffffffu, k[e] != 0u);
+        ahead += __popc(b & ((1u << lane) - 1u));
+        all += __popc(b);
+      }
+      uint32_t r = count + ahead;
+#pragma unroll
+      for (int e = 0; e < V; e++)
+        if (k[e]) {
+          list.key[r] = k[e];
+          list.where[r] = uint32_t(i0 + v * 32 * V + e);
+          r++;
+        }
+      count += all;
+    }
+    // (grad and p may lie over the values: this row's have been read)
+    if (ok) clear_out<T>(a, at, int(at.n), lane, 32);
+    const double u_row = u;
+    const bool more = row + 1 < end && walk.step(a.r, row + 1);
+    if (more) fetch(walk.at, row + 1);
     __syncwarp();
-    ListRow r(none, tables, lane, 0);
-    r.take(list, count);
-    const Stats s = r.stats();
-    r.begin(c, s, a.r.kind);
-    cut_list(r, c, s, count, a.r.kind);
-    finish_as<T, 1>(r, c, a, row, at, n, fits);
+    list_row<T>(list, count, tables, lane, cut_of(a.c, row), a, row, at, ok, u_row, answers);
+    if (!more) {
+      answers.done(a, row, lane);
+      return;
+    }
     __syncwarp();  // the list is written again for the next row
   }
 }
 
-// Longer rows: CL CTAs of W warps a row.
+// Longer rows: CL CTAs of W warps a row. A CTA on its own (CL = 1) takes
+// `batch` rows, one after another up to their lists, which its warps then
+// finish side by side: one warp at the end of one row would leave the SM idle.
+constexpr int kBatch = 8;
 template <typename T, int E, int W, int CL, typename Arg>
-__global__ void __launch_bounds__(W * 32) k_policy_rows(Arg a) {
-  constexpr int V = 16 / int(sizeof(T));
+__global__ void __launch_bounds__(W * 32, E <= 24 && W <= 8 ? 24 / W : 1) k_policy_rows(const __grid_constant__ Arg a,
+                                                                                       uint32_t batch) {
+  constexpr int V = 16 / int(sizeof(T)), kLists = CL > 1 ? 1 : W < kBatch ? W : kBatch;
   using R = Row<E, V, W, CL>;
   __shared__ typename Group<W, CL>::Shared sh;
-  __shared__ typename Group<1, 1>::Shared none;
-  __shared__ List list;
+  __shared__ List lists[kLists];
+  __shared__ struct { RowAt at; uint32_t row, count; } todo[kLists];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t row = blockIdx.x / CL;
-  RowAt at;
-  if (!locate(a.r, a.out_pitch, row, lane, &at)) return;
   const Tables tables(lane, a.r.kind == kKindP);
-  R r(sh, tables, lane, warp);
+  uint32_t made = 0;
+  for (uint32_t b = 0; b < batch; b++) {
+    const uint32_t row = blockIdx.x / CL * batch + b;
+    RowAt at;
+    if (row >= a.r.rows || !locate(a.r, a.out_pitch, row, lane, &at)) break;
+    R r(sh, tables, lane, warp);
+    const bool fits = at.n <= a.r.row_len && at.n + V - 1 <= R::kCap;
+    const uint32_t n = fits ? uint32_t(at.n) : 0u;
+    r.load(static_cast<const T*>(a.r.values) + at.in, n, a.r.kind);
+    const Cut c = cut_of(a.c, row);
+    Stats s = r.stats();
+    uint32_t from = s.lo, count = s.open;
+    if (s.open > kList && c.k && c.k <= kListTopK) {
+      from = r.lower_bound(c.k, s, a.r.kind);
+      uint32_t mn = 0xffffffffu, mx = 0;
+      count = 0;
+      r.each([&](int e) {
+        if (r.k[e] >= from) { count++; mn = min(mn, r.k[e]); }
+      });
+      r.g.counts(count, mn, mx);
+      from = mn;
+    }
+    if (count <= kList) {
+      List* to = &lists[made];
+      if constexpr (CL > 1) to = cooperative_groups::this_cluster().map_shared_rank(to, 0);
+      r.gather(from, to);
+      // (grad and p may lie over the values: this row's have been read)
+      if (fits) clear_out<T>(a, at, int(n), r.g.rank * W * 32 + int(threadIdx.x), W * 32 * CL);
+      if (threadIdx.x == 0) {
+        todo[made].at = at;
+        todo[made].row = row;
+        todo[made].count = count;
+      }
+      made++;
+    } else {
+      s.lo = from;
+      s.open = count;
+      r.begin(c, s, a.r.kind);
+      r.cut(c, s, a.r.kind);
+      finish_as<T, V>(r, c, a, row, at, int(n), fits);
+    }
+    if (W > 1 && b + 1 < batch) __syncthreads();  // the group's slots start again with the next row
+  }
+  if constexpr (CL > 1) cooperative_groups::this_cluster().sync();
+  else __syncthreads();
+  if (warp >= int(made) || (CL > 1 && cooperative_groups::this_cluster().block_rank() != 0)) return;
+  const RowAt at = todo[warp].at;
+  const uint32_t row = todo[warp].row;
   const bool fits = at.n <= a.r.row_len && at.n + V - 1 <= R::kCap;
-  const uint32_t n = fits ? uint32_t(at.n) : 0u;
-  r.load(static_cast<const T*>(a.r.values) + at.in, n, a.r.kind);
-  const Cut c = cut_of(a.c, row);
-  Stats s = r.stats();
-  uint32_t from = s.lo, count = s.open;
-  if (s.open > kList && c.k && c.k <= kListTopK) {
-    from = r.lower_bound(c.k, s, a.r.kind);
-    count = 0;
-    uint32_t mn = 0, mx = 0;
-    r.each([&](int e) { count += r.k[e] >= from; });
-    r.g.counts(count, mn, mx);
-  }
-  if (count <= kList) {
-    List* to = &list;
-    if constexpr (CL > 1) to = cooperative_groups::this_cluster().map_shared_rank(&list, 0);
-    r.gather(from ? from : 1u, to);
-    if (fits) clear_out<T>(a, at, int(n), r.g.rank * W * 32 + int(threadIdx.x), W * 32 * CL);
-    if constexpr (CL > 1) cooperative_groups::this_cluster().sync();
-    else __syncthreads();
-    if (r.g.segment() != 0) return;
-    ListRow l(none, tables, lane, 0);
-    l.take(list, count);
-    const Stats ls = l.stats();
-    l.begin(c, ls, a.r.kind);
-    cut_list(l, c, ls, count, a.r.kind);
-    finish_as<T, 1>(l, c, a, row, at, int(n), fits);
-    return;
-  }
-  s.lo = from;
-  s.open = count;
-  r.begin(c, s, a.r.kind);
-  r.cut(c, s, a.r.kind);
-  finish_as<T, V>(r, c, a, row, at, int(n), fits);
+  Answers<Arg> answers;
+  list_row<T>(lists[warp], todo[warp].count, tables, lane, cut_of(a.c, row), a, row, at, fits,
+              answers.uniform(a, row), answers);
+  answers.done(a, row, lane);
 }
 
 }  // namespace pol

@@ -10,25 +10,35 @@
 namespace kc {
 namespace pol {
 
-// One launch of kernel K over the rows, CL CTAs a row (W > 1) or four rows a
-// CTA (W = 1).
+// One warp a row, four rows a CTA.
 template <typename A>
-cudaError_t go(void (*kernel)(A), const A& a, int w, int cl, cudaStream_t stream) {
+cudaError_t go_warps(void (*kernel)(A), const A& a, cudaStream_t stream) {
   cudaLaunchConfig_t cfg{};
-  cfg.blockDim = dim3(w == 1 ? 128 : unsigned(w) * 32);
-  const uint64_t ctas = w == 1 ? (uint64_t(a.r.rows) + 3) / 4 : uint64_t(a.r.rows) * cl;
+  cfg.blockDim = dim3(128);
+  cfg.gridDim = dim3(unsigned((uint64_t(a.r.rows) + 3) / 4));
+  cfg.stream = stream;
+  return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
+// A launch of k_policy_rows. Rows are batched only where every SM has work
+// without it, twice over.
+template <typename T, int E, int W, int CL, typename A>
+cudaError_t go_rows(const A& a, int sms, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg{};
+  const uint32_t most = CL > 1 ? 1u : uint32_t(std::min(W, kBatch));
+  const uint32_t batch = std::max(1u, std::min(most, a.r.rows / (uint32_t(sms) * 4u)));
+  const uint64_t ctas = (uint64_t(a.r.rows) + batch - 1) / batch * CL;
   if (ctas > 0x7fffffffu) return cudaErrorInvalidConfiguration;
   cfg.gridDim = dim3(unsigned(ctas));
+  cfg.blockDim = dim3(W * 32);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
-  if (cl > 1) {
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = unsigned(cl);
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-  }
-  return cudaLaunchKernelEx(&cfg, kernel, a);
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CL;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = CL > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, k_policy_rows<T, E, W, CL, A>, a, batch);
 }
 
 // The group that holds the longest row, a vector's misalignment included.
@@ -39,16 +49,16 @@ cudaError_t cut_as(const A& a, int sms, cudaStream_t s) {
   if (need <= kList) {
     const uint64_t ctas = (uint64_t(a.r.rows) + 3) / 4;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(unsigned(std::min<uint64_t>(ctas, uint64_t(sms) * 8)));
+    cfg.gridDim = dim3(unsigned(std::min<uint64_t>(ctas, uint64_t(sms) * kSmallCtas)));
     cfg.blockDim = dim3(128);
     cfg.stream = s;
     return cudaLaunchKernelEx(&cfg, k_policy_small<T, A>, a);
   }
-  if (need <= 1024) return go(k_policy_rows<T, 8, 4, 1, A>, a, 4, 1, s);
-  if (need <= 8 * 32 * kMid) return go(k_policy_rows<T, kMid, 8, 1, A>, a, 8, 1, s);
-  if (need <= 16384) return go(k_policy_rows<T, 32, 16, 1, A>, a, 16, 1, s);
-  if (need <= 32768) return go(k_policy_rows<T, 64, 16, 1, A>, a, 16, 1, s);
-  return go(k_policy_rows<T, 64, 16, 8, A>, a, 16, 8, s);
+  if (need <= 1024) return go_rows<T, 8, 4, 1>(a, sms, s);
+  if (need <= 8 * 32 * kMid) return go_rows<T, kMid, 8, 1>(a, sms, s);
+  if (need <= 16384) return go_rows<T, 32, 16, 1>(a, sms, s);
+  if (need <= 32768) return go_rows<T, 64, 16, 1>(a, sms, s);
+  return go_rows<T, 64, 16, 8>(a, sms, s);
 }
 
 // Rows that k_policy_long keeps in shared memory: CL CTAs of NT threads a row,
@@ -93,8 +103,8 @@ template <typename T>
 inline cudaError_t whole_as(const LossArg& a, cudaStream_t s) {
   constexpr int V = 16 / sizeof(T);
   const uint64_t need = a.r.row_len + V - 1;
-  if (need <= 256) return go(k_policy_whole<T, 8 / V>, a, 1, 1, s);
-  if (need <= 1024) return go(k_policy_whole<T, 32 / V>, a, 1, 1, s);
+  if (need <= 256) return go_warps(k_policy_whole<T, 8 / V>, a, s);
+  if (need <= 1024) return go_warps(k_policy_whole<T, 32 / V>, a, s);
   if (need * sizeof(T) <= kShort) return go_long<T, 128, 1>(a, s);
   if (need * sizeof(T) <= kLong) return go_long<T, 256, 1>(a, s);
   return go_long<T, 512, 8>(a, s);
