@@ -45,29 +45,36 @@ unsigned fill(Table<N>& tb, Tensor* t, uint32_t count) {
   return tb.chunks;
 }
 
-}  // namespace
-
-cudaError_t launch_clip(Tensor* t, uint64_t count, double max_norm, double* workspace, double* result, int sms,
-                        cudaStream_t stream, uint64_t* launches) {
+template <uint32_t N>
+cudaError_t run(Tensor* t, uint64_t count, double max_norm, double* workspace, double* result, int sms,
+                cudaStream_t stream, uint64_t* launches) {
   const uint32_t most = std::min<uint32_t>(kMaxCtas, uint32_t(sms) * 4);
-  static thread_local Table<kTable> tb;
+  static thread_local Table<N> tb;
   uint32_t partials = 0;
   for (int pass = 0; pass < 2; pass++) {
     bool first = true;
-    for (uint64_t at = 0; at < count || first; at += kTable) {
-      const uint32_t chunks = fill(tb, t + at, uint32_t(std::min<uint64_t>(kTable, count - at)));
+    for (uint64_t at = 0; at < count || first; at += N) {
+      const uint32_t chunks = fill(tb, t + at, uint32_t(std::min<uint64_t>(N, count - at)));
       const unsigned grid = std::max(1u, std::min(most, chunks));
       if (pass == 0) {
-        k_norm<kTable><<<grid, kThreads, 0, stream>>>(tb, workspace + partials);
+        k_norm<N><<<grid, kThreads, 0, stream>>>(tb, workspace + partials);
         partials += grid;
       } else {
-        k_scale<kTable><<<grid, kThreads, 0, stream>>>(tb, workspace, partials, max_norm, result, first ? 1 : 0);
+        k_scale<N><<<grid, kThreads, 0, stream>>>(tb, workspace, partials, max_norm, result, first ? 1 : 0);
       }
       ++*launches;
       first = false;
     }
   }
   return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_clip(Tensor* t, uint64_t count, double max_norm, double* workspace, double* result, int sms,
+                        cudaStream_t stream, uint64_t* launches) {
+  return count <= kShortTable ? run<kShortTable>(t, count, max_norm, workspace, result, sms, stream, launches)
+                              : run<kTable>(t, count, max_norm, workspace, result, sms, stream, launches);
 }
 
 }  // namespace clip

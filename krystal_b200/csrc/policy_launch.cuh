@@ -47,9 +47,10 @@ cudaError_t cut_as(const A& a, int sms, cudaStream_t s) {
   const uint64_t need = a.r.row_len + 16 / sizeof(T) - 1;
   constexpr int kMid = sizeof(T) == 4 ? 20 : 24;  // the largest bank, misaligned, in 8 warps
   if (need <= kList) {
-    const uint64_t ctas = (uint64_t(a.r.rows) + 3) / 4;
+    // a row a warp, or runs of rows once there are eight for every warp that fits
+    const uint64_t ctas = (uint64_t(a.r.rows) + 3) / 4, fit = uint64_t(sms) * kSmallCtas;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(unsigned(std::min<uint64_t>(ctas, uint64_t(sms) * kSmallCtas)));
+    cfg.gridDim = dim3(unsigned(ctas > 8 * fit ? fit : ctas));
     cfg.blockDim = dim3(128);
     cfg.stream = s;
     return cudaLaunchKernelEx(&cfg, k_policy_small<T, A>, a);
