@@ -6,9 +6,11 @@
 // Two launches: k_norm leaves one partial sum a CTA, k_scale adds the partial
 // sums again in every CTA (a few KB from L2) and scales. All sums are 64-bit
 // and in an order that the sizes alone decide; there are no atomics. The work
-// is cut into chunks of 32 KB of one tensor; CTA b takes chunks b, b + grid, ...
-// and k_scale takes them from the last back, so that what k_norm read last is
-// still in L2.
+// is cut into chunks of one tensor, 8 to 128 KB so that about one falls to each
+// CTA of a small list and a large one pays for few searches of its table; CTA b
+// takes chunks b, b + grid, ... and k_scale takes them from the last back, so
+// that what k_norm read last is still in L2. k_scale is launched while k_norm
+// runs and waits for it on the device.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -20,12 +22,12 @@ namespace kc {
 namespace clip {
 
 constexpr int kThreads = 512;
-constexpr uint32_t kChunkBytes = 32768;
+constexpr uint32_t kMinChunk = 8192, kMaxChunk = 131072;  // bytes
 
 template <uint32_t N>
 struct Table {
   Tensor t[N];
-  uint32_t count, chunks;
+  uint32_t count, chunks, chunk_bytes;
 };
 
 __host__ __device__ constexpr uint32_t dtype_bytes(int d) { return d == kF32 ? 4u : d == kF64 ? 8u : 2u; }
@@ -45,7 +47,7 @@ __device__ __forceinline__ Piece piece_of(const Table<N>& tb, uint32_t chunk) {
   }
   Piece p;
   p.t = &tb.t[lo];
-  const uint32_t per = kChunkBytes / dtype_bytes(p.t->dtype);
+  const uint32_t per = tb.chunk_bytes / dtype_bytes(p.t->dtype);
   p.first = uint64_t(chunk - p.t->chunk0) * per;
   p.n = uint32_t(min(uint64_t(per), p.t->n - p.first));
   return p;
@@ -75,7 +77,7 @@ __device__ __forceinline__ double square_sum(const T* in, uint32_t n) {
   const uint32_t head = head_of(in, n), vecs = (n - head) / V;
   double acc[2] = {0.0, 0.0};
   const uint4* src = reinterpret_cast<const uint4*>(in + head);
-#pragma unroll 4
+#pragma unroll 8
   for (uint32_t i = threadIdx.x; i < vecs; i += kThreads) {
     const uint4 raw = src[i];
     alignas(16) T v[V];
@@ -135,6 +137,7 @@ __device__ __forceinline__ double cta_sum(double v, double* red) {
 template <uint32_t N>
 __global__ void __launch_bounds__(kThreads) k_norm(const __grid_constant__ Table<N> tb, double* __restrict__ partial) {
   __shared__ double red[kThreads / 32];
+  cudaTriggerProgrammaticLaunchCompletion();
   double sum = 0.0;
   for (uint32_t c = blockIdx.x; c < tb.chunks; c += gridDim.x) {
     const Piece p = piece_of(tb, c);
@@ -156,6 +159,7 @@ __global__ void __launch_bounds__(kThreads) k_scale(const __grid_constant__ Tabl
                                                     const double* __restrict__ partial, uint32_t partials,
                                                     double max_norm, double* __restrict__ result, int first) {
   __shared__ double red[kThreads / 32];
+  cudaGridDependencySynchronize();  // k_norm has ended and its partial sums are here
   double sum = 0.0;
   for (uint32_t i = threadIdx.x; i < partials; i += kThreads) sum += partial[i];
   const double norm = sqrt(cta_sum(sum, red));

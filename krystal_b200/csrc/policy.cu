@@ -32,12 +32,15 @@ namespace clip {
 namespace {
 
 template <uint32_t N>
-unsigned fill(Table<N>& tb, Tensor* t, uint32_t count) {
-  uint64_t chunk = 0;
+unsigned fill(Table<N>& tb, Tensor* t, uint32_t count, uint32_t ctas) {
+  uint64_t bytes = 0, chunk = 0;
+  for (uint32_t i = 0; i < count; i++) bytes += t[i].n * dtype_bytes(t[i].dtype);
+  tb.chunk_bytes = kMinChunk;
+  while (tb.chunk_bytes < kMaxChunk && uint64_t(tb.chunk_bytes) * ctas < bytes) tb.chunk_bytes *= 2;
   for (uint32_t i = 0; i < count; i++) {
     tb.t[i] = t[i];
     tb.t[i].chunk0 = uint32_t(chunk);
-    const uint64_t per = kChunkBytes / dtype_bytes(t[i].dtype);
+    const uint64_t per = tb.chunk_bytes / dtype_bytes(t[i].dtype);
     chunk += (t[i].n + per - 1) / per;
   }
   tb.count = count;
@@ -54,13 +57,24 @@ cudaError_t run(Tensor* t, uint64_t count, double max_norm, double* workspace, d
   for (int pass = 0; pass < 2; pass++) {
     bool first = true;
     for (uint64_t at = 0; at < count || first; at += N) {
-      const uint32_t chunks = fill(tb, t + at, uint32_t(std::min<uint64_t>(N, count - at)));
+      const uint32_t chunks = fill(tb, t + at, uint32_t(std::min<uint64_t>(N, count - at)), most);
       const unsigned grid = std::max(1u, std::min(most, chunks));
       if (pass == 0) {
         k_norm<N><<<grid, kThreads, 0, stream>>>(tb, workspace + partials);
         partials += grid;
       } else {
-        k_scale<N><<<grid, kThreads, 0, stream>>>(tb, workspace, partials, max_norm, result, first ? 1 : 0);
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(grid);
+        cfg.blockDim = dim3(kThreads);
+        cfg.stream = stream;
+        cudaLaunchAttribute early[1];
+        early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        early[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = early;
+        cfg.numAttrs = first && at + N >= count ? 1 : 0;  // one launch of each: the one ahead is k_norm's
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, k_scale<N>, tb, static_cast<const double*>(workspace), partials,
+                                                 max_norm, result, first ? 1 : 0);
+        if (e) return e;
       }
       ++*launches;
       first = false;
