@@ -733,6 +733,13 @@ __device__ __forceinline__ void finish(R& r, const Cut& c, const LossArg& a, uin
   }
 }
 
+// Whether a row keeps the stated bound and the group holds it, misaligned as it is.
+template <typename T>
+__device__ __forceinline__ bool row_fits(const RowsArg& r, const RowAt& at, uint32_t cap) {
+  const uint32_t shift = uint32_t((reinterpret_cast<uintptr_t>(static_cast<const T*>(r.values) + at.in) & 15) / sizeof(T));
+  return at.n <= r.row_len && at.n + shift <= cap;
+}
+
 // The output laid out like the rows, and which of the two finishes it takes.
 template <typename T> __device__ __forceinline__ void clear_out(const DrawArg& a, const RowAt& at, int n, int tid, int threads) {
   if (a.p) clear_row(a.p + at.out, n, tid, threads);
@@ -923,7 +930,7 @@ __global__ void __launch_bounds__(W * 32, E <= 24 && W <= 8 ? 24 / W : 1) k_poli
     RowAt at;
     if (row >= a.r.rows || !locate(a.r, a.out_pitch, row, lane, &at)) break;
     R r(sh, tables, lane, warp);
-    const bool fits = at.n <= a.r.row_len && at.n + V - 1 <= R::kCap;
+    const bool fits = row_fits<T>(a.r, at, R::kCap);
     const uint32_t n = fits ? uint32_t(at.n) : 0u;
     r.load(static_cast<const T*>(a.r.values) + at.in, n, a.r.kind);
     const Cut c = cut_of(a.c, row);
@@ -965,7 +972,7 @@ __global__ void __launch_bounds__(W * 32, E <= 24 && W <= 8 ? 24 / W : 1) k_poli
   if (warp >= int(made) || (CL > 1 && cooperative_groups::this_cluster().block_rank() != 0)) return;
   const RowAt at = todo[warp].at;
   const uint32_t row = todo[warp].row;
-  const bool fits = at.n <= a.r.row_len && at.n + V - 1 <= R::kCap;
+  const bool fits = row_fits<T>(a.r, at, R::kCap);
   Answers<Arg> answers;
   list_row<T>(lists[warp], todo[warp].count, tables, lane, cut_of(a.c, row), a, row, at, fits,
               answers.uniform(a, row), answers);

@@ -44,9 +44,11 @@ cudaError_t go_rows(const A& a, int sms, cudaStream_t stream) {
 // The group that holds the longest row, a vector's misalignment included.
 template <typename T, typename A>
 cudaError_t cut_as(const A& a, int sms, cudaStream_t s) {
-  const uint64_t need = a.r.row_len + 16 / sizeof(T) - 1;
+  constexpr uint64_t V = 16 / sizeof(T);
+  const bool aligned = a.r.frames == 0 && a.r.pitch % V == 0 && (reinterpret_cast<uintptr_t>(a.r.values) & 15) == 0;
+  const uint64_t need = a.r.row_len + (aligned ? 0 : V - 1);
   constexpr int kMid = sizeof(T) == 4 ? 20 : 24;  // the largest bank, misaligned, in 8 warps
-  if (need <= kList) {
+  if (a.r.row_len + V - 1 <= kList) {
     // a row a warp, or runs of rows once there are eight for every warp that fits
     const uint64_t ctas = (uint64_t(a.r.rows) + 3) / 4, fit = uint64_t(sms) * kSmallCtas;
     cudaLaunchConfig_t cfg{};
@@ -59,6 +61,8 @@ cudaError_t cut_as(const A& a, int sms, cudaStream_t s) {
   if (need <= 8 * 32 * kMid) return go_rows<T, kMid, 8, 1>(a, sms, s);
   if (need <= 16384) return go_rows<T, 32, 16, 1>(a, sms, s);
   if (need <= 32768) return go_rows<T, 64, 16, 1>(a, sms, s);
+  // half the CTAs where they hold the row: 32 rows are one wave of them
+  if (need <= 131072) return go_rows<T, 64, 16, 4>(a, sms, s);
   return go_rows<T, 64, 16, 8>(a, sms, s);
 }
 
