@@ -322,8 +322,9 @@ struct Group {
     counts(add, mn, mx);
     return double(add);
   }
-  // The sum over the warps ahead of this one of a value the warp agrees on.
-  __device__ uint32_t ahead(uint32_t v) {
+  // The sum over the warps ahead of this one of a value the warp agrees on;
+  // *all (if asked for) gets the group's sum.
+  __device__ uint32_t ahead(uint32_t v, uint32_t* all = nullptr) {
     uint32_t before = 0;
     if constexpr (W > 1) {
       buf ^= 1;
@@ -341,7 +342,9 @@ struct Group {
       const uint32_t sc = warp_scan(lane < CL ? s->cu[buf][0][lane] : 0u, lane);
       const uint32_t others = __shfl_sync(0xffffffffu, sc, rank ? rank - 1 : 0);
       if (rank) before += others;
+      v = __shfl_sync(0xffffffffu, sc, CL - 1);
     }
+    if (all) *all = v;
     return before;
   }
 };

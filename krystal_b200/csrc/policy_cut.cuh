@@ -177,12 +177,13 @@ struct Row {
     return lo;
   }
 
-  // The entries at or above `from` into the list, in bank order; the caller
-  // knows that they fit. A barrier has to follow.
-  __device__ void gather(uint32_t from, List* list) {
-    uint32_t mine = 0;
+  // The entries at or above `from` into the list, in bank order, if they fit;
+  // how many there are. A barrier has to follow.
+  __device__ uint32_t gather(uint32_t from, List* list) {
+    uint32_t mine = 0, all;
     each([&](int e) { mine += k[e] >= from; });
-    uint32_t seen = g.ahead(__reduce_add_sync(0xffffffffu, mine));
+    uint32_t seen = g.ahead(__reduce_add_sync(0xffffffffu, mine), &all);
+    if (all > kList) return all;
 #pragma unroll
     for (int c = 0; c < kChunks; c++) {
       if (!in_use(c)) continue;
@@ -200,6 +201,7 @@ struct Row {
         }
       seen += __shfl_sync(0xffffffffu, incl, 31);
     }
+    return all;
   }
 
   // The tempered log weight of a key in the support. Every lane of the warp
@@ -936,20 +938,15 @@ __global__ void __launch_bounds__(W * 32, E <= 24 && W <= 8 ? 24 / W : 1) k_poli
     const Cut c = cut_of(a.c, row);
     Stats s = r.stats();
     uint32_t from = s.lo, count = s.open;
+    List* to = &lists[made];
+    if constexpr (CL > 1) to = cooperative_groups::this_cluster().map_shared_rank(to, 0);
     if (s.open > kList && c.k && c.k <= kListTopK) {
       from = r.lower_bound(c.k, s, a.r.kind);
-      uint32_t mn = 0xffffffffu, mx = 0;
-      count = 0;
-      r.each([&](int e) {
-        if (r.k[e] >= from) { count++; mn = min(mn, r.k[e]); }
-      });
-      r.g.counts(count, mn, mx);
-      from = mn;
+      count = r.gather(from, to);
+    } else if (s.open <= kList) {
+      r.gather(from, to);
     }
     if (count <= kList) {
-      List* to = &lists[made];
-      if constexpr (CL > 1) to = cooperative_groups::this_cluster().map_shared_rank(to, 0);
-      r.gather(from, to);
       // (grad and p may lie over the values: this row's have been read)
       if (fits) clear_out<T>(a, at, int(n), r.g.rank * W * 32 + int(threadIdx.x), W * 32 * CL);
       if (threadIdx.x == 0) {
@@ -959,8 +956,15 @@ __global__ void __launch_bounds__(W * 32, E <= 24 && W <= 8 ? 24 / W : 1) k_poli
       }
       made++;
     } else {
-      s.lo = from;
-      s.open = count;
+      if (from != s.lo) {  // top-k's search starts from the smallest entry at or above the bound
+        uint32_t mn = 0xffffffffu, none = 0, mx = 0;
+        r.each([&](int e) {
+          if (r.k[e] >= from) mn = min(mn, r.k[e]);
+        });
+        r.g.counts(none, mn, mx);
+        s.lo = mn;
+        s.open = count;
+      }
       r.begin(c, s, a.r.kind);
       r.cut(c, s, a.r.kind);
       finish_as<T, V>(r, c, a, row, at, int(n), fits);

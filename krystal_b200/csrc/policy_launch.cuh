@@ -20,13 +20,23 @@ cudaError_t go_warps(void (*kernel)(A), const A& a, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
-// A launch of k_policy_rows. Rows are batched only where every SM has work
-// without it, twice over.
+// A launch of k_policy_rows. The batch is the one whose waves of CTAs take
+// least: a batch costs its rows up to their lists, and about one and a half
+// more rows for finishing them side by side.
 template <typename T, int E, int W, int CL, typename A>
 cudaError_t go_rows(const A& a, int sms, cudaStream_t stream) {
   cudaLaunchConfig_t cfg{};
   const uint32_t most = CL > 1 ? 1u : uint32_t(std::min(W, kBatch));
-  const uint32_t batch = std::max(1u, std::min(most, a.r.rows / (uint32_t(sms) * 4u)));
+  const uint64_t fit = uint64_t(sms) * (W <= 8 ? 24 / W : 1);
+  uint32_t batch = 1;
+  double least = 1e300;
+  for (uint32_t b = 1; b <= most; b++) {
+    const double waves = double(((uint64_t(a.r.rows) + b - 1) / b + fit - 1) / fit);
+    if (waves * (b + 1.5) < least) {
+      least = waves * (b + 1.5);
+      batch = b;
+    }
+  }
   const uint64_t ctas = (uint64_t(a.r.rows) + batch - 1) / batch * CL;
   if (ctas > 0x7fffffffu) return cudaErrorInvalidConfiguration;
   cfg.gridDim = dim3(unsigned(ctas));
