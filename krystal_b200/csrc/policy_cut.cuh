@@ -657,9 +657,10 @@ __device__ __forceinline__ void finish(R& r, const Cut& c, const DrawArg& a, uin
 //   loss = -A log pi(a) - beta H(pi), H = log Z - sum w x / Z,
 //   dloss/dv_j = (A (pi_j - [j = a]) + beta pi_j (log pi_j + H)) / T
 // for what is kept, 0 elsewhere, times the row's weight.
+// given: a list's weights, 0 for what is cut.
 template <typename T, typename R, int V>
 __device__ __forceinline__ void finish(R& r, const Cut& c, const LossArg& a, uint32_t row, const RowAt& at, int n,
-                                       bool fits) {
+                                       bool fits, const double* given = nullptr) {
   constexpr int E = sizeof(r.k) / 4;
   const int lane = r.g.lane;
   const uint32_t act = a.actions[row];
@@ -669,7 +670,13 @@ __device__ __forceinline__ void finish(R& r, const Cut& c, const LossArg& a, uin
   double ws[R::kCached ? E : 1];
   r.each([&](int e) {
     uint32_t& key = r.k[e];
-    double x, w = r.weight(key, x);
+    double x, w;
+    if constexpr (V == 1) {
+      x = r.x_of(key ? key : r.top);
+      w = given[e];
+    } else {
+      w = r.weight(key, x);
+    }
     if (w < c.min_p) w = 0.0;
     if (!(w > 0.0)) key = 0u;
     if constexpr (R::kCached) ws[e] = w;
@@ -764,8 +771,8 @@ __device__ __forceinline__ void finish_as(R& r, const Cut& c, const LossArg& a, 
 template <typename Arg> struct Answers {
   __device__ double uniform(const Arg&, uint32_t) { return 0.0; }
   template <typename T, int S>
-  __device__ void take(ListRow<S>& r, const Cut& c, const Arg& a, uint32_t row, const RowAt& at, bool fits, double, double*) {
-    finish<T, ListRow<S>, 1>(r, c, a, row, at, int(at.n), fits);
+  __device__ void take(ListRow<S>& r, const Cut& c, const Arg& a, uint32_t row, const RowAt& at, bool fits, double, double* w) {
+    finish<T, ListRow<S>, 1>(r, c, a, row, at, int(at.n), fits, w);
   }
   __device__ void done(const Arg&, uint32_t, int) {}
 };
