@@ -60,7 +60,7 @@ cudaError_t cut_as(const A& a, int sms, cudaStream_t s) {
   constexpr int kMid = sizeof(T) == 4 ? 20 : 24;  // the largest bank, misaligned, in 8 warps
   if (a.r.row_len + V - 1 <= kList) {
     // a row a warp, or runs of rows once there are eight for every warp that fits
-    const uint64_t ctas = (uint64_t(a.r.rows) + 3) / 4, fit = uint64_t(sms) * kSmallCtas;
+    const uint64_t ctas = (uint64_t(a.r.rows) + 3) / 4, fit = uint64_t(sms) * kSmallCtas<A>;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(unsigned(ctas > 8 * fit ? fit : ctas));
     cfg.blockDim = dim3(128);

@@ -498,3 +498,112 @@ def test_captured_draw_replays_on_new_inputs(be):
             want = ref.loss(row, n, j, 1.0, float(np.float32(0.1)), limits(dict(temperature=0.9))[0])[3]
             near(grad[i].cpu().numpy(), want, HALF["f32"], 1e-11)
     g.reset()
+
+
+def check_ragged(be, v, dtype, where, view, cut, u, total, spare=0, kind="scores"):
+    """A packed batch's draws against the plain form; `spare` rows behind the last question."""
+    t, k, p, mp = limits(cut)
+    rows = len(where)
+    du = on_gpu(u)
+    idx, kept = (torch.full((rows + spare,), -9, dtype=torch.int32, device="cuda") for _ in range(2))
+    logp, out = torch.full((rows + spare,), 9.0, device="cuda"), torch.full((total + 3,), 9.0, device="cuda")
+    torch.cuda.synchronize()
+    be.draw(view, sampling(cut), du.data_ptr(), index=idx.data_ptr(), kept=kept.data_ptr(), logp=logp.data_ptr(),
+            p=out.data_ptr())
+    be.synchronize()
+    idx, kept, logp, out = (x.cpu().numpy() for x in (idx, kept, logp, out))
+    assert (idx[rows:] == -9).all() and (kept[rows:] == -9).all() and (logp[rows:] == 9).all() and (out[total:] == 9).all()
+    for i, (at, n) in enumerate(where):
+        row = ref.policy(wide(v[at:at + n]), t, k, p, mp, kind, dtype == "f16")
+        want = np.zeros(n)
+        want[row[0]] = row[1]
+        j, lp = ref.draw(row, u[i])
+        assert (int(idx[i]), int(kept[i])) == (j, row[0].size), i
+        near(out[at:at + n], want, HALF["f32"], TINY["f32"])
+        near([logp[i]], [lp], HALF["f32"], 2e-12)
+
+
+@pytest.mark.parametrize("rows", [30, 3000, 45000])
+def test_runs_of_short_rows(be, rows):
+    """Many short rows: a warp walks through a run of them, over frames without
+    questions and without a bank, and stops behind the last."""
+    rng = np.random.default_rng(rows)
+    frames = rows // 3
+    q, r = rng.integers(0, 7, frames), rng.integers(0, 20, frames)
+    q[rng.random(frames) < 0.2] = 0
+    q_off = np.concatenate([[0], np.cumsum(q)]).astype(np.uint64)
+    p_off = np.concatenate([[0], np.cumsum(q * r)]).astype(np.uint64)
+    v = scores(rng, 1, int(p_off[-1]), "f32")[0]
+    where = [(int(p_off[f]) + i * int(r[f]), int(r[f])) for f in range(frames) for i in range(int(q[f]))]
+    dv, dq, dp = v.cuda(), on_gpu(q_off.view(np.int64)), on_gpu(p_off.view(np.int64))
+    spare = rows // 4 + 1
+    view = policy.ragged_rows(dv.data_ptr(), "f32", len(where) + spare, frames, dq.data_ptr(), dp.data_ptr(), 20)
+    check_ragged(be, v, "f32", where, view, dict(temperature=0.8, top_k=7, top_p=0.8), rng.random(len(where) + spare),
+                 int(p_off[-1]), spare)
+
+
+@pytest.mark.parametrize("open_", [1, 32, 33, 64, 65, 128, 129, 250])
+def test_lists_of_every_length(be, open_):
+    """What the mask leaves of a row is gathered: every size of list, each cut, with ties."""
+    rng = np.random.default_rng(open_)
+    for n, dtype in ((250, "f32"), (900, "bf16"), (5000, "f16"), (40000, "bf16")):
+        v = np.full((4, n), -np.inf, np.float32)
+        for i in range(4):
+            at = np.sort(rng.choice(n, open_, replace=False))
+            v[i, at] = rng.normal(0, 2, open_) if i % 2 else np.round(rng.normal(0, 1, open_))
+        t = torch.from_numpy(v).to(TYPES[dtype])
+        for cut in (dict(), dict(top_k=open_ // 2 + 1), dict(top_p=0.8, temperature=1.3),
+                    dict(top_k=open_ // 3 + 1, top_p=0.7, min_p=0.05), dict(temperature=0.0)):
+            check_draw(be, t, dtype, cut, rng.random(4), offset=3, pitch=n + 2)
+
+
+@pytest.mark.parametrize("n,dtype", [(1000, "f32"), (4096, "bf16"), (12000, "f32"), (30000, "f16"), (100000, "bf16"),
+                                     (200000, "f32")])
+def test_top_k_bounds_that_hold_too_much(be, n, dtype):
+    """Rows of few values: the lower bound of the k-th largest admits more than
+    a list, and the row stays spread over its group; and k beyond any list."""
+    rng = np.random.default_rng(n)
+    few = np.round(rng.normal(0, 0.6, (3, n))).astype(np.float32)
+    few[1] = 1.0
+    few[2, 5] = 9.0
+    t = torch.from_numpy(few).to(TYPES[dtype])
+    for cut in (dict(top_k=50), dict(top_k=2), dict(top_k=200, top_p=0.6), dict(top_k=n // 2, top_p=0.9),
+                dict(top_k=n - 1)):
+        check_draw(be, t, dtype, cut, rng.random(3))
+    u = torch.from_numpy(rng.normal(0, 2, (3, n)).astype(np.float32)).to(TYPES[dtype])
+    for cut in (dict(top_k=207), dict(top_k=209), dict(top_k=208, top_p=0.5), dict(top_k=1, top_p=0.5)):
+        check_draw(be, u, dtype, cut, rng.random(3))
+
+
+@pytest.mark.parametrize("rows,n", [(3000, 700), (1500, 1500)])
+def test_batches_of_long_rows(be, rows, n):
+    """Enough long rows that a CTA takes several: lists, rows that stay spread,
+    empty rows and the rows behind the last question side by side."""
+    rng = np.random.default_rng(rows)
+    lens = rng.integers(0, n + 1, rows)
+    off = np.concatenate([[0], np.cumsum(lens)]).astype(np.int64)
+    v = scores(rng, 1, int(off[-1]), "bf16", 0.5)[0]
+    v[off[7]:off[40]] = v[off[7]:off[40]].round()  # many ties
+    where = [(int(off[i]), int(lens[i])) for i in range(rows)]
+    dv, dp = v.cuda(), on_gpu(off)
+    spare = 9
+    view = policy.ragged_rows(dv.data_ptr(), "bf16", rows + spare, rows, None, dp.data_ptr(), n)
+    for cut in (dict(top_k=60, top_p=0.9), dict(temperature=0.7, top_p=0.8)):
+        check_ragged(be, v, "bf16", where, view, cut, rng.random(rows + spare), int(off[-1]), spare)
+
+
+def test_draws_over_the_values_themselves(be):
+    """p may be the f32 values: short rows, lists of long ones, and spread rows."""
+    rng = np.random.default_rng(6)
+    for rows, n, cut in ((40, 200, dict(top_p=0.9)), (700, 1500, dict(top_k=20)), (5, 9000, dict(top_p=0.95)),
+                         (3, 50000, dict(top_k=30)), (2, 50000, dict(top_p=0.9))):
+        v = scores(rng, rows, n, "f32").cuda()
+        u = on_gpu(rng.random(rows))
+        want = torch.zeros(rows, n, device="cuda")
+        idx = [torch.zeros(rows, dtype=torch.int32, device="cuda") for _ in range(2)]
+        torch.cuda.synchronize()
+        view = policy.dense_rows(v.data_ptr(), "f32", rows, n)
+        be.draw(view, sampling(cut), u.data_ptr(), index=idx[0].data_ptr(), p=want.data_ptr())
+        be.draw(view, sampling(cut), u.data_ptr(), index=idx[1].data_ptr(), p=v.data_ptr())
+        be.synchronize()
+        assert torch.equal(v, want) and torch.equal(idx[0], idx[1])
