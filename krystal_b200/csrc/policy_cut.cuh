@@ -765,15 +765,54 @@ __device__ __forceinline__ void finish_as(R& r, const Cut& c, const LossArg& a, 
   finish<T, R, V>(r, c, a, row, at, n, fits);
 }
 
-// What a warp keeps of its rows' answers until it writes them: lane i has the
+// The finish of a list whose weights are known: a draw to be reported, or a
+// loss that has been written.
+template <typename T, int S>
+__device__ __forceinline__ Drawn finish_list(ListRow<S>& r, const Cut& c, const DrawArg& a, uint32_t, const RowAt& at,
+                                             bool fits, double u, double* w) {
+  return draw_list<S>(r, c, a, at, fits, u, w);
+}
+template <typename T, int S>
+__device__ __forceinline__ Drawn finish_list(ListRow<S>& r, const Cut& c, const LossArg& a, uint32_t row,
+                                             const RowAt& at, bool fits, double, double* w) {
+  finish<T, ListRow<S>, 1>(r, c, a, row, at, int(at.n), fits, w);
+  return Drawn{kNone, 0u, 0.0};
+}
+
+// Everything after the gathering, by one warp on a list of n <= 32 S entries.
+template <typename T, int S, typename Arg>
+__device__ __forceinline__ Drawn list_as(List& list, uint32_t n, const Tables& tables, int lane, const Cut& c,
+                                         const Arg& a, uint32_t row, const RowAt& at, bool fits, double u) {
+  ListRow<S> r(lane, tables);
+  r.take(list, n);
+  const bool cuts = (c.k && c.k < n) || c.top_p < 1.0;
+  constexpr bool pairs = S <= kPairs / 32;
+  const Stats s = r.list_stats(n, cuts && !pairs);
+  r.begin(c, s, a.r.kind);
+  if (!pairs && cuts) r.cut(c, s, a.r.kind);
+  double w[S];
+#pragma unroll
+  for (int e = 0; e < S; e++) {
+    w[e] = 0.0;
+    if (r.in_use(e)) w[e] = r.weight(r.k[e]);
+  }
+  if constexpr (pairs) {
+    if (cuts) cut_pairs<S>(r, c, list.key, list.w, int(n), w);
+  }
+  return finish_list<T, S>(r, c, a, row, at, fits, u, w);
+}
+template <typename T, typename Arg>
+__device__ __forceinline__ Drawn list_row(List& list, uint32_t n, const Tables& tables, int lane, const Cut& c,
+                                          const Arg& a, uint32_t row, const RowAt& at, bool fits, double u) {
+  if (n <= uint32_t(kPairs)) return list_as<T, kPairs / 32>(list, n, tables, lane, c, a, row, at, fits, u);
+  return list_as<T, kList / 32>(list, n, tables, lane, c, a, row, at, fits, u);
+}
+
+// What a warp keeps of its rows' draws until it writes them: lane i has the
 // draw of row first + i, so that the logarithms of 32 rows are one evaluation.
-// A loss needs its own at once.
 template <typename Arg> struct Answers {
   __device__ double uniform(const Arg&, uint32_t) { return 0.0; }
-  template <typename T, int S>
-  __device__ void take(ListRow<S>& r, const Cut& c, const Arg& a, uint32_t row, const RowAt& at, bool fits, double, double* w) {
-    finish<T, ListRow<S>, 1>(r, c, a, row, at, int(at.n), fits, w);
-  }
+  __device__ void take(const Drawn&, const Arg&, uint32_t, int) {}
   __device__ void done(const Arg&, uint32_t, int) {}
 };
 template <> struct Answers<DrawArg> {
@@ -782,11 +821,9 @@ template <> struct Answers<DrawArg> {
   __device__ double uniform(const DrawArg& a, uint32_t row) {
     return a.uniforms ? fmin(fmax(a.uniforms[row], 0.0), 1.0) : 0.0;
   }
-  template <typename T, int S>
-  __device__ __forceinline__ void take(ListRow<S>& r, const Cut& c, const DrawArg& a, uint32_t row, const RowAt& at, bool fits, double u, double* w) {
-    const Drawn d = draw_list<S>(r, c, a, at, fits, u, w);
-    if (r.g.lane == held) mine = d;
-    if (++held == 32) done(a, row, r.g.lane);
+  __device__ __forceinline__ void take(const Drawn& d, const DrawArg& a, uint32_t row, int lane) {
+    if (lane == held) mine = d;
+    if (++held == 32) done(a, row, lane);
   }
   // Writes what is held, the last of it row's.
   __device__ void done(const DrawArg& a, uint32_t row, int lane) {
@@ -795,46 +832,12 @@ template <> struct Answers<DrawArg> {
   }
 };
 
-// Everything after the gathering, by one warp on a list of n <= 32 S entries.
-template <typename T, int S, typename Arg>
-__device__ __forceinline__ void list_as(List& list, uint32_t n, const Tables& tables, int lane, const Cut& c,
-                                        const Arg& a, uint32_t row, const RowAt& at, bool fits, double u,
-                                        Answers<Arg>& answers) {
-  ListRow<S> r(lane, tables);
-  r.take(list, n);
-  const bool cuts = (c.k && c.k < n) || c.top_p < 1.0;
-  const Stats s = r.list_stats(n, cuts && S > 2);
-  r.begin(c, s, a.r.kind);
-  double w[S];
-  if constexpr (S <= kPairs / 32) {
-#pragma unroll
-    for (int e = 0; e < S; e++) w[e] = r.weight(r.k[e]);
-    if (cuts) cut_pairs<S>(r, c, list.key, list.w, int(n), w);
-  } else {
-    if (cuts) r.cut(c, s, a.r.kind);
-#pragma unroll
-    for (int e = 0; e < S; e++) {
-      w[e] = 0.0;
-      if (r.in_use(e)) w[e] = r.weight(r.k[e]);
-    }
-  }
-  answers.template take<T, S>(r, c, a, row, at, fits, u, w);
-}
-template <typename T, typename Arg>
-__device__ __forceinline__ void list_row(List& list, uint32_t n, const Tables& tables, int lane, const Cut& c,
-                                         const Arg& a, uint32_t row, const RowAt& at, bool fits, double u,
-                                         Answers<Arg>& answers) {
-  if (n <= 32) list_as<T, 1>(list, n, tables, lane, c, a, row, at, fits, u, answers);
-  else if (n <= 64) list_as<T, 2>(list, n, tables, lane, c, a, row, at, fits, u, answers);
-  else list_as<T, 8>(list, n, tables, lane, c, a, row, at, fits, u, answers);
-}
-
 // Rows of up to 256 entries: a warp a row, always by its list. A warp takes a
 // run of rows one after another: its tables are made once, the frame is
 // searched for once, and the next row's entries and uniform are fetched while
 // it works.
 // CTAs an SM. More warps hide more of a row's latency, more registers spill
-// less: 34810 drawn rows took 98, 109 and 102 us with 6, 7 and 8, the loss of
+// less: 34810 drawn rows took 95, 109 and 102 us with 6, 7 and 8, the loss of
 // 4096 rows 20.6, 18.1 and 19.6.
 template <typename Arg> constexpr int kSmallCtas = 6;
 template <> constexpr int kSmallCtas<LossArg> = 7;
@@ -914,7 +917,7 @@ __global__ void __launch_bounds__(128, kSmallCtas<Arg>) k_policy_small(const __g
     const bool more = row + 1 < end && walk.step(a.r, row + 1);
     if (more) fetch(walk.at, row + 1);
     __syncwarp();
-    list_row<T>(list, count, tables, lane, cut_of(a.c, row), a, row, at, ok, u_row, answers);
+    answers.take(list_row<T>(list, count, tables, lane, cut_of(a.c, row), a, row, at, ok, u_row), a, row, lane);
     if (!more) {
       answers.done(a, row, lane);
       return;
@@ -989,8 +992,8 @@ __global__ void __launch_bounds__(W * 32, E <= 24 && W <= 8 ? 24 / W : 1) k_poli
   const uint32_t row = todo[warp].row;
   const bool fits = row_fits<T>(a.r, at, R::kCap);
   Answers<Arg> answers;
-  list_row<T>(lists[warp], todo[warp].count, tables, lane, cut_of(a.c, row), a, row, at, fits,
-              answers.uniform(a, row), answers);
+  answers.take(list_row<T>(lists[warp], todo[warp].count, tables, lane, cut_of(a.c, row), a, row, at, fits,
+                           answers.uniform(a, row)), a, row, lane);
   answers.done(a, row, lane);
 }
 
