@@ -550,7 +550,8 @@ struct Walk {
 };
 
 struct Cut {
-  double inv_t;     // 0: the largest entry alone
+  double inv_t;
+  bool greedy;      // a temperature that is not above 0: the first largest entry alone
   uint32_t k;       // 0: off
   double top_p;     // >= 1: off
   double min_p;     // <= 0: off
@@ -564,7 +565,8 @@ __device__ __forceinline__ Cut cut_of(const CutArg& c, uint32_t row) {
   o.k = c.row_top_k ? c.row_top_k[row] : c.top_k;
   o.top_p = p < 1.0f ? fmax(double(p), 0.0) : 2.0;  // a NaN cuts nothing
   o.min_p = m > 0.0f ? fmin(double(m), 1.0) : 0.0;
-  if (!(t > 0.0f)) o.k = 1;
+  o.greedy = !(t > 0.0f);
+  if (o.greedy) o.k = 1;
   return o;
 }
 

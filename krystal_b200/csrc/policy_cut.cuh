@@ -694,8 +694,7 @@ __device__ __forceinline__ void finish(R& r, const Cut& c, const LossArg& a, uin
   const double log_z = kept ? log64(z) : 0.0, inv_z = kept ? 1.0 / z : 0.0;
   const double h = kept ? log_z - sx * inv_z : 0.0;
   const double logp = xa - log_z;
-  // a temperature that is not positive has one answer and no gradient
-  const bool learns = asked && live == 0u && c.inv_t > 0.0;
+  const bool learns = asked && live == 0u && !c.greedy;  // one answer has no gradient
   const double adv = double(a.advantage[row]), beta = double(a.beta);
   if (r.g.segment() == 0 && lane == 0) {
     if (a.loss) a.loss[row] = learns ? float(-adv * logp - beta * h) : 0.0f;
@@ -837,7 +836,7 @@ template <> struct Answers<DrawArg> {
 // searched for once, and the next row's entries and uniform are fetched while
 // it works.
 // CTAs an SM. More warps hide more of a row's latency, more registers spill
-// less: 34810 drawn rows took 95, 109 and 102 us with 6, 7 and 8, the loss of
+// less: 34818 drawn rows took 95, 109 and 102 us with 6, 7 and 8, the loss of
 // 4096 rows 20.6, 18.1 and 19.6.
 template <typename Arg> constexpr int kSmallCtas = 6;
 template <> constexpr int kSmallCtas<LossArg> = 7;

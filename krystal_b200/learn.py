@@ -67,6 +67,10 @@ class LearnOptions:
     sampling: Sampling | None = None
     max_update_norm: float = math.inf
 
+    def __post_init__(self):
+        if not self.max_update_norm >= 0:
+            raise ValueError("max_update_norm must be a number, 0 or above")
+
 
 @dataclass
 class HostExperience:

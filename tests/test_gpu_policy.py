@@ -607,3 +607,119 @@ def test_draws_over_the_values_themselves(be):
         be.draw(view, sampling(cut), u.data_ptr(), index=idx[1].data_ptr(), p=v.data_ptr())
         be.synchronize()
         assert torch.equal(v, want) and torch.equal(idx[0], idx[1])
+
+
+@pytest.mark.parametrize("n", [50, 700, 5000])
+def test_loss_limits_row_by_row(be, n):
+    """Cut losses with a temperature a row: 0, NaN and negative have one answer,
+    infinity weighs every kept entry alike."""
+    rng = np.random.default_rng(n)
+    rows = 8
+    v = scores(rng, rows, n, "f32")
+    temps = np.array([0.5, 0.0, np.nan, -1.0, 0.9, np.inf, 2.0, 1.0], np.float32)
+    ks = rng.integers(1, n, rows).astype(np.int32)
+    act = np.array([int(np.argmax(np.nan_to_num(wide(r), nan=-1e300, neginf=-1e300))) for r in v], np.int32)
+    adv = rng.normal(size=rows).astype(np.float32)
+    dev = [on_gpu(x) for x in (temps, ks, act, adv)]
+    dv, grad = v.cuda(), torch.full((rows, n), 9.0, device="cuda")
+    lo, lp, h = (torch.full((rows,), 9.0, device="cuda") for _ in range(3))
+    torch.cuda.synchronize()
+    s = policy.Sampling(row_temperature=dev[0].data_ptr(), row_top_k=dev[1].data_ptr())
+    be.policy_loss(policy.dense_rows(dv.data_ptr(), "f32", rows, n), s, dev[2].data_ptr(), dev[3].data_ptr(), 0.1,
+                   loss=lo.data_ptr(), logp=lp.data_ptr(), entropy=h.data_ptr(), grad=grad.data_ptr())
+    be.synchronize()
+    for i in range(rows):
+        t = float(temps[i]) if temps[i] > 0 else 0.0
+        row = ref.policy(wide(v[i]), t, int(ks[i]))
+        L, l, e, g = ref.loss(row, n, int(act[i]), float(adv[i]), float(np.float32(0.1)), t)
+        near([float(lo[i]), float(lp[i]), float(h[i])], [L, l, e], HALF["f32"], 4e-11)
+        near(grad[i].cpu().numpy(), g, HALF["f32"], 4e-11)
+
+
+def test_offsets_past_32_bits(be):
+    """Rows, packed blocks and outputs that start behind 2^32 elements."""
+    rng = np.random.default_rng(1)
+    n, far = 300, (1 << 32) + 5
+    buf = torch.empty(far + 4 * n, dtype=torch.bfloat16, device="cuda")
+    out = torch.empty(far + 4 * n, dtype=torch.float32, device="cuda")
+    grad = torch.empty(far + 4 * n, dtype=torch.bfloat16, device="cuda")
+    v = scores(rng, 2, n, "bf16")
+    u = rng.random(2)
+    idx = torch.zeros(2, dtype=torch.int32, device="cuda")
+    act, adv = torch.zeros(2, dtype=torch.int32, device="cuda"), torch.ones(2, device="cuda")
+    du, s = on_gpu(u), policy.Sampling(0.9, 40, 0.9)
+    views = [(policy.dense_rows(buf.data_ptr(), "bf16", 2, n, far), [0, far], far),
+             (policy.ragged_rows(buf.data_ptr(), "bf16", 2, 1, None, 0, n), [far, far + n], 0)]
+    q, p = torch.tensor([0, 2], device="cuda"), torch.tensor([far, far + 2 * n], device="cuda")
+    views[1][0].q_off, views[1][0].p_off = q.data_ptr(), p.data_ptr()
+    for view, starts, pitch in views:
+        for i, at in enumerate(starts):
+            buf[at:at + n] = v[i].cuda()
+            out[at:at + n] = 9.0
+            grad[at:at + n] = 9.0
+        torch.cuda.synchronize()
+        be.draw(view, s, du.data_ptr(), index=idx.data_ptr(), p=out.data_ptr(), p_pitch=pitch)
+        act.copy_(idx)
+        torch.cuda.synchronize()
+        be.policy_loss(view, s, idx.data_ptr(), adv.data_ptr(), 0.0, grad=grad.data_ptr(), grad_pitch=pitch)
+        be.synchronize()
+        for i, at in enumerate(starts):
+            t, k, tp, _ = limits(dict(temperature=0.9, top_k=40, top_p=0.9))
+            row = ref.policy(wide(v[i]), t, k, tp)
+            want = np.zeros(n)
+            want[row[0]] = row[1]
+            assert int(idx[i]) == ref.draw(row, u[i])[0]
+            near(out[at:at + n].cpu().numpy(), want, HALF["f32"], TINY["f32"])
+            g = ref.loss(row, n, int(idx[i]), 1.0, 0.0, t)[3]
+            near(grad[at:at + n].double().cpu().numpy(), g, HALF["bf16"], TINY["bf16"] + 1e-11)
+
+
+FIRST_CALL = """
+import numpy as np, torch
+from krystal_b200 import BRAIN_FORWARD_CONFIG, GradList, Sampling, create_brain_forward_weights, cuda_backend, policy
+cfg = BRAIN_FORWARD_CONFIG.with_token_rows(np.arange(64, dtype=np.uint32))
+be = cuda_backend(0)(cfg, create_brain_forward_weights(cfg, 1))
+v = {n: torch.randn(3, n, device="cuda") for n in (40, 900, 5000, 60000)}
+u = torch.rand(3, dtype=torch.float64, device="cuda")
+adv = torch.ones(3, device="cuda")
+idx = {n: torch.zeros(3, dtype=torch.int32, device="cuda") for n in v}
+grad = {n: [torch.zeros_like(x) for _ in range(2)] for n, x in v.items()}
+res = torch.zeros(2, dtype=torch.float64, device="cuda")
+lst = GradList([g[0] for g in grad.values()])
+side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+be.set_stream(side.cuda_stream)
+cut = Sampling(0.9, 20, 0.9)
+with torch.cuda.graph(graph, stream=side):
+    for n, x in v.items():
+        rows = policy.dense_rows(x.data_ptr(), "f32", 3, n)
+        be.draw(rows, cut, u.data_ptr(), index=idx[n].data_ptr())
+        for s, g in zip((cut, Sampling()), grad[n]):
+            be.policy_loss(rows, s, idx[n].data_ptr(), adv.data_ptr(), 0.1, grad=g.data_ptr())
+    be.clip_grads(lst, 0.5, res.data_ptr())
+graph.replay()
+torch.cuda.synchronize()
+captured = [t.clone() for n in v for t in (idx[n], *grad[n])] + [res.clone()]
+for n, x in v.items():
+    rows = policy.dense_rows(x.data_ptr(), "f32", 3, n)
+    be.draw(rows, cut, u.data_ptr(), index=idx[n].data_ptr())
+    for s, g in zip((cut, Sampling()), grad[n]):
+        be.policy_loss(rows, s, idx[n].data_ptr(), adv.data_ptr(), 0.1, grad=g.data_ptr())
+be.clip_grads(lst, 0.5, res.data_ptr())
+torch.cuda.synchronize()
+now = [t for n in v for t in (idx[n], *grad[n])] + [res]
+assert all(torch.equal(a, b) for a, b in zip(captured, now))
+assert float(res[0]) > 0 and all(bool((i >= 0).all()) for i in idx.values())
+graph.reset()
+be.destroy()
+print("captured first calls agree")
+"""
+
+
+def test_the_first_calls_of_a_process_can_be_captured():
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured first calls agree" in r.stdout, r.stderr[-2000:]

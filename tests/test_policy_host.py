@@ -122,3 +122,12 @@ def test_host_update_is_clipped_to_the_actors_norm(unfreeze_pool):
         for a, b in ((w.selector.wq, free.selector.wq), (w.selector.wk, free.selector.wk), (w.pool, free.pool)):
             assert np.abs(a - b).max() <= 2.0 ** -24  # weights below 1: one f32 rounding
         assert np.array_equal(w.value_head_wv, free.value_head_wv)
+
+
+def test_learn_options_are_checked():
+    for bad in (math.nan, -1.0, -math.inf):
+        with pytest.raises(ValueError, match="max_update_norm"):
+            LearnOptions(max_update_norm=bad)
+    with pytest.raises(ValueError, match="max_update_norm"):
+        replace(LearnOptions(), max_update_norm=-2.0)
+    assert LearnOptions().max_update_norm == math.inf and LearnOptions().sampling is None
