@@ -41,6 +41,8 @@ struct Row {
   static constexpr uint32_t kCap = uint32_t(32) * E * W * CL;
   static constexpr bool kCached = E <= 32;  // the registers hold a weight an entry beside the keys
   static_assert(E % V == 0 && kChunks <= 32, "a thread holds whole vectors");
+  static constexpr float kUnit = 1048576.0f;
+  static_assert(32 * E <= 2048, "a warp's units fit 32 bits");
 
   Group<W, CL> g;
   const Tables& t;
@@ -270,7 +272,7 @@ struct Row {
   }
 
   // top-p's search by approximate weights: f32 exponentials in units of 2^-20
-  // of the largest, summed as integers. An entry above half a unit has |x| <=
+  // of the largest, summed as integers (a warp's at most 2^31). An entry above half a unit has |x| <=
   // 21 ln 2; three f32 roundings of the exponent and ex2's 2^-22 put its weight
   // within 3e-6, and for probabilities lg2's 2^-22 of log2 v and of log2 m add
   // 3.4e-7 (|log2 m| + 21 T) / T. A mass that clears the goal by `err` of the
@@ -278,14 +280,18 @@ struct Row {
   // that does not leaves [lo, cur] to the 64-bit search. What it usually
   // leaves is one value.
   __device__ void narrow(double top_p, uint32_t open, int kind, uint32_t& lo, uint32_t& cur) {
-    uint32_t q[E], all = 0;
+    uint32_t q[kCached ? E : 1], all = 0;
     const float mv = float(m), it = float(inv_t) * (kind == kKindP ? 1.0f : 1.44269504f);
     const float mu = kind == kKindP ? log2_fast(mv) : mv;
-    each([&](int e) {
-      const float v = value_of(k[e] ? k[e] : 0xbf800000u);
+    auto units = [&](uint32_t key) {
+      const float v = value_of(key);
       const float u = ((kind == kKindP ? log2_fast(v) : v) - mu) * it;
-      q[e] = k[e] ? __float2uint_rn(exp2_fast(fminf(u, 0.0f)) * 1048576.0f) : 0u;
-      all += q[e];
+      return __float2uint_rn(exp2_fast(fminf(u, 0.0f)) * kUnit);
+    };
+    each([&](int e) {
+      const uint32_t x = k[e] ? units(k[e]) : 0u;
+      if constexpr (kCached) q[e] = x;
+      all += x;
     });
     const double total = g.sum_u32(all);
     const double goal = top_p * total;
@@ -296,8 +302,13 @@ struct Row {
       const uint32_t p = pivot(lo, cur, step, kind);
       uint32_t mass = 0, mn = 0xffffffffu, mx = 0u;
       each([&](int e) {
-        if (k[e] >= p) { mass += q[e]; mn = min(mn, k[e]); }
-        else mx = max(mx, k[e]);
+        if (k[e] >= p) {
+          if constexpr (kCached) mass += q[e];
+          else mass += units(k[e]);
+          mn = min(mn, k[e]);
+        } else {
+          mx = max(mx, k[e]);
+        }
       });
       const double a = g.masses(mass, mn, mx);
       if (a >= above) lo = mn;
@@ -342,7 +353,7 @@ struct Row {
     if (c.top_p < 1.0) {
       // the largest t with mass(k >= t) >= goal
       uint32_t cur = top;
-      if constexpr (kCached) narrow(c.top_p, left, kind, lo, cur);
+      narrow(c.top_p, left, kind, lo, cur);
       uint32_t ties = 0, mn = 0xffffffffu, mx = 0u;
       each([&](int e) { ties += k[e] == lo; });
       g.counts(ties, mn, mx);
@@ -928,9 +939,11 @@ __global__ void __launch_bounds__(128, kSmallCtas<Arg>) k_policy_small(const __g
 // Longer rows: CL CTAs of W warps a row. A CTA on its own (CL = 1) takes
 // `batch` rows, one after another up to their lists, which its warps then
 // finish side by side: one warp at the end of one row would leave the SM idle.
+// FIT CTAs share an SM: three of eight warps where lists are what rows come to
+// (top-k), two where a row stays in its registers (top-p alone).
 constexpr int kBatch = 8;
-template <typename T, int E, int W, int CL, typename Arg>
-__global__ void __launch_bounds__(W * 32, E <= 24 && W <= 8 ? 24 / W : 1) k_policy_rows(const __grid_constant__ Arg a,
+template <typename T, int E, int W, int CL, int FIT, typename Arg>
+__global__ void __launch_bounds__(W * 32, FIT) k_policy_rows(const __grid_constant__ Arg a,
                                                                                        uint32_t batch) {
   constexpr int V = 16 / int(sizeof(T)), kLists = CL > 1 ? 1 : W < kBatch ? W : kBatch;
   using R = Row<E, V, W, CL>;

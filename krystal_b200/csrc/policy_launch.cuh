@@ -23,11 +23,11 @@ cudaError_t go_warps(void (*kernel)(A), const A& a, cudaStream_t stream) {
 // A launch of k_policy_rows. The batch is the one whose waves of CTAs take
 // least: a batch costs its rows up to their lists, and about one and a half
 // more rows for finishing them side by side.
-template <typename T, int E, int W, int CL, typename A>
+template <typename T, int E, int W, int CL, int FIT, typename A>
 cudaError_t go_rows(const A& a, int sms, cudaStream_t stream) {
   cudaLaunchConfig_t cfg{};
   const uint32_t most = CL > 1 ? 1u : uint32_t(std::min(W, kBatch));
-  const uint64_t fit = uint64_t(sms) * (W <= 8 ? 24 / W : 1);
+  const uint64_t fit = uint64_t(sms) * FIT;
   uint32_t batch = 1;
   double least = 1e300;
   for (uint32_t b = 1; b <= most; b++) {
@@ -48,7 +48,7 @@ cudaError_t go_rows(const A& a, int sms, cudaStream_t stream) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = CL > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, k_policy_rows<T, E, W, CL, A>, a, batch);
+  return cudaLaunchKernelEx(&cfg, k_policy_rows<T, E, W, CL, FIT, A>, a, batch);
 }
 
 // The group that holds the longest row, a vector's misalignment included.
@@ -67,15 +67,16 @@ cudaError_t cut_as(const A& a, int sms, cudaStream_t s) {
     cfg.stream = s;
     return cudaLaunchKernelEx(&cfg, k_policy_small<T, A>, a);
   }
-  if (need <= 1024) return go_rows<T, 8, 4, 1>(a, sms, s);
-  if (need <= 8 * 32 * kMid) return go_rows<T, kMid, 8, 1>(a, sms, s);
-  if (need <= 16384) return go_rows<T, 32, 16, 1>(a, sms, s);
-  if (need <= 32768) return go_rows<T, 64, 16, 1>(a, sms, s);
+  if (need <= 1024) return go_rows<T, 8, 4, 1, 6>(a, sms, s);
+  if (need <= 8 * 32 * kMid)
+    return a.c.top_k || a.c.row_top_k ? go_rows<T, kMid, 8, 1, 3>(a, sms, s) : go_rows<T, kMid, 8, 1, 2>(a, sms, s);
+  if (need <= 16384) return go_rows<T, 32, 16, 1, 1>(a, sms, s);
+  if (need <= 32768) return go_rows<T, 64, 16, 1, 1>(a, sms, s);
   // the fewest CTAs that hold the row: 32 rows of 131071 took 46 us in clusters
   // of 4, one wave, and 63 in clusters of 8
-  if (need <= 65536) return go_rows<T, 64, 16, 2>(a, sms, s);
-  if (need <= 131072) return go_rows<T, 64, 16, 4>(a, sms, s);
-  return go_rows<T, 64, 16, 8>(a, sms, s);
+  if (need <= 65536) return go_rows<T, 64, 16, 2, 1>(a, sms, s);
+  if (need <= 131072) return go_rows<T, 64, 16, 4, 1>(a, sms, s);
+  return go_rows<T, 64, 16, 8, 1>(a, sms, s);
 }
 
 // Rows that k_policy_long keeps in shared memory: CL CTAs of NT threads a row,
