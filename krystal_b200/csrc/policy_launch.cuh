@@ -20,14 +20,20 @@ cudaError_t go_warps(void (*kernel)(A), const A& a, cudaStream_t stream) {
   return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
-// A launch of k_policy_rows. The batch is the one whose waves of CTAs take
-// least: a batch costs its rows up to their lists, and about one and a half
-// more rows for finishing them side by side.
-template <typename T, int E, int W, int CL, int FIT, typename A>
-cudaError_t go_rows(const A& a, int sms, cudaStream_t stream) {
-  cudaLaunchConfig_t cfg{};
+// A launch of k_policy_rows: `need` entries a row at most, misaligned as they
+// may be. The batch is the one whose waves of CTAs take least: a batch costs
+// its rows up to their lists, and about one and a half more rows for finishing
+// them side by side.
+constexpr uint32_t kRowEntries = 32768;  // a CTA holds: 4 bytes of key and 2 of place an entry
+constexpr size_t kRowSmem = size_t(kRowEntries) * 6;
+template <typename T, int W, int CL, typename A>
+cudaError_t go_rows(const A& a, uint64_t need, int sms, cudaStream_t stream) {
+  constexpr uint64_t per = uint64_t(32) * (16 / sizeof(T)) * W * CL;
+  const uint32_t chunks = uint32_t((need + per - 1) / per);
+  const size_t smem = size_t(chunks) * per / CL * 6;
   const uint32_t most = CL > 1 ? 1u : uint32_t(std::min(W, kBatch));
-  const uint64_t fit = uint64_t(sms) * FIT;
+  // CTAs that share an SM: by their threads, and by their shared memory (a list is 2.5 KB)
+  const uint64_t fit = uint64_t(sms) * std::max<uint64_t>(1, std::min<uint64_t>(32 / W, 230000 / (smem + most * 2700 + 2048)));
   uint32_t batch = 1;
   double least = 1e300;
   for (uint32_t b = 1; b <= most; b++) {
@@ -38,9 +44,11 @@ cudaError_t go_rows(const A& a, int sms, cudaStream_t stream) {
     }
   }
   const uint64_t ctas = (uint64_t(a.r.rows) + batch - 1) / batch * CL;
-  if (ctas > 0x7fffffffu) return cudaErrorInvalidConfiguration;
+  if (ctas > 0x7fffffffu || smem > kRowSmem) return cudaErrorInvalidConfiguration;
+  cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(ctas));
   cfg.blockDim = dim3(W * 32);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -48,7 +56,20 @@ cudaError_t go_rows(const A& a, int sms, cudaStream_t stream) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = CL > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, k_policy_rows<T, E, W, CL, FIT, A>, a, batch);
+  return cudaLaunchKernelEx(&cfg, k_policy_rows<T, W, CL, A>, a, batch, chunks);
+}
+template <typename T, typename A>
+cudaError_t prepare_rows() {
+  const auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
+  cudaError_t e;
+  if ((e = cudaFuncSetAttribute(k_policy_rows<T, 4, 1, A>, attr, int(kRowSmem))) ||
+      (e = cudaFuncSetAttribute(k_policy_rows<T, 8, 1, A>, attr, int(kRowSmem))) ||
+      (e = cudaFuncSetAttribute(k_policy_rows<T, 16, 1, A>, attr, int(kRowSmem))) ||
+      (e = cudaFuncSetAttribute(k_policy_rows<T, 16, 2, A>, attr, int(kRowSmem))) ||
+      (e = cudaFuncSetAttribute(k_policy_rows<T, 16, 4, A>, attr, int(kRowSmem))) ||
+      (e = cudaFuncSetAttribute(k_policy_rows<T, 16, 8, A>, attr, int(kRowSmem))))
+    return e;
+  return cudaSuccess;
 }
 
 // The group that holds the longest row, a vector's misalignment included.
@@ -57,7 +78,6 @@ cudaError_t cut_as(const A& a, int sms, cudaStream_t s) {
   constexpr uint64_t V = 16 / sizeof(T);
   const bool aligned = a.r.frames == 0 && a.r.pitch % V == 0 && (reinterpret_cast<uintptr_t>(a.r.values) & 15) == 0;
   const uint64_t need = a.r.row_len + (aligned ? 0 : V - 1);
-  constexpr int kMid = sizeof(T) == 4 ? 20 : 24;  // the largest bank, misaligned, in 8 warps
   if (a.r.row_len + V - 1 <= kList) {
     // a row a warp, or runs of rows once there are eight for every warp that fits
     const uint64_t ctas = (uint64_t(a.r.rows) + 3) / 4, fit = uint64_t(sms) * kSmallCtas<A>;
@@ -67,16 +87,14 @@ cudaError_t cut_as(const A& a, int sms, cudaStream_t s) {
     cfg.stream = s;
     return cudaLaunchKernelEx(&cfg, k_policy_small<T, A>, a);
   }
-  if (need <= 1024) return go_rows<T, 8, 4, 1, 6>(a, sms, s);
-  if (need <= 8 * 32 * kMid)
-    return a.c.top_k || a.c.row_top_k ? go_rows<T, kMid, 8, 1, 3>(a, sms, s) : go_rows<T, kMid, 8, 1, 2>(a, sms, s);
-  if (need <= 16384) return go_rows<T, 32, 16, 1, 1>(a, sms, s);
-  if (need <= 32768) return go_rows<T, 64, 16, 1, 1>(a, sms, s);
+  if (need <= 2048) return go_rows<T, 4, 1>(a, need, sms, s);
+  if (need <= 8192) return go_rows<T, 8, 1>(a, need, sms, s);
+  if (need <= kRowEntries) return go_rows<T, 16, 1>(a, need, sms, s);
   // the fewest CTAs that hold the row: 32 rows of 131071 took 46 us in clusters
   // of 4, one wave, and 63 in clusters of 8
-  if (need <= 65536) return go_rows<T, 64, 16, 2, 1>(a, sms, s);
-  if (need <= 131072) return go_rows<T, 64, 16, 4, 1>(a, sms, s);
-  return go_rows<T, 64, 16, 8, 1>(a, sms, s);
+  if (need <= 2 * kRowEntries) return go_rows<T, 16, 2>(a, need, sms, s);
+  if (need <= 4 * kRowEntries) return go_rows<T, 16, 4>(a, need, sms, s);
+  return go_rows<T, 16, 8>(a, need, sms, s);
 }
 
 // Rows that k_policy_long keeps in shared memory: CL CTAs of NT threads a row,
@@ -96,6 +114,7 @@ cudaError_t prepare_as() {
       (e = cudaFuncSetAttribute(k_policy_long<T, 256, 1>, attr, int(long_smem<T>(kLong / sizeof(T), 1)))) ||
       (e = cudaFuncSetAttribute(k_policy_long<T, 512, 8>, attr, int(long_smem<T>(kMaxRow, 8)))))
     return e;
+  if ((e = prepare_rows<T, DrawArg>()) || (e = prepare_rows<T, LossArg>())) return e;
   return cudaSuccess;
 }
 template <typename T, int NT, int CL>
