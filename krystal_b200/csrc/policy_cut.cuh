@@ -156,6 +156,8 @@ struct WideRow : Scale {
         place(reinterpret_cast<uint16_t*>(sm + W * n * 32 * (V / 4)) + warp * n * 32 * V), chunks(n), live(0), kept(0) {}
 
   __device__ int at(int c) const { return base + c * 32 * V + g.lane * V; }
+  // Until the row is packed, the places' memory holds each vector's largest key.
+  __device__ uint32_t* best() const { return reinterpret_cast<uint32_t*>(place); }
   __device__ void get(int c, uint32_t* k) const {
 #pragma unroll
     for (int j = 0; j < V / 4; j++) {
@@ -216,11 +218,12 @@ struct WideRow : Scale {
 #pragma unroll
           for (int e = 0; e < V; e += 2) set2<T>(w[u], e, f[e], f[e + 1]);
         }
-        uint32_t k[V], any = 0;
+        uint32_t k[V], most = 0;
 #pragma unroll
-        for (int e = 0; e < V; e++) any |= k[e] = open_key<T>(entry<T>(w[u], e), kind);
+        for (int e = 0; e < V; e++) most = max(most, k[e] = open_key<T>(entry<T>(w[u], e), kind));
         put(c0 + u, k);
-        if (__any_sync(0xffffffffu, any != 0u)) live |= 1u << (c0 + u);
+        best()[(c0 + u) * 32 + g.lane] = most;
+        if (__any_sync(0xffffffffu, most != 0u)) live |= 1u << (c0 + u);
       }
     }
   }
@@ -240,12 +243,8 @@ struct WideRow : Scale {
   __device__ uint32_t lower_bound(uint32_t want, const Stats& s, int kind) {
     auto reach = [&](uint32_t p) {  // vectors whose largest reaches p
       uint32_t n = 0;
-      each([&](int, const uint32_t* k) {
-        uint32_t best = k[0];
-#pragma unroll
-        for (int e = 1; e < V; e++) best = max(best, k[e]);
-        n += best >= p;
-      });
+#pragma unroll 4
+      for (int c = 0; c < chunks; c++) n += best()[c * 32 + g.lane] >= p;
       return g.total(n);
     };
     if (reach(s.lo) < want) return s.lo;
