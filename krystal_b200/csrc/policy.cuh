@@ -22,7 +22,8 @@
 // does not depend on how the row was split, and equals the definition's to
 // about n * 1e-15 of probability. No entry is sorted: a cut is the largest
 // value t with count(v >= t) >= k, or mass(v >= t) >= top_p * total, found by
-// halving the range of values between snapped row entries.
+// halving the range of values between snapped row entries, or in a short list
+// by adding up, for each entry, what lies ahead of it.
 //
 // This file: layouts, arithmetic and reductions; policy_cut.cuh: the rows with
 // cuts and the draws; policy_whole.cuh: the loss where nothing is cut.

@@ -838,12 +838,11 @@ template <> struct Answers<DrawArg> {
 // searched for once, and the next row's entries and uniform are fetched while
 // it works.
 // CTAs an SM. More warps hide more of a row's latency, more registers spill
-// less: 34818 drawn rows took 95, 109 and 102 us with 6, 7 and 8, the loss of
-// 4096 rows 20.6, 18.1 and 19.6.
-template <typename Arg> constexpr int kSmallCtas = 6;
-template <> constexpr int kSmallCtas<LossArg> = 7;
+// less: 34818 drawn rows took 95, 97, 105 and 96 us with 5 to 8, the loss of
+// 4096 rows between 19 and 20.
+constexpr int kSmallCtas = 6;
 template <typename T, typename Arg>
-__global__ void __launch_bounds__(128, kSmallCtas<Arg>) k_policy_small(const __grid_constant__ Arg a) {
+__global__ void __launch_bounds__(128, kSmallCtas) k_policy_small(const __grid_constant__ Arg a) {
   constexpr int V = 16 / int(sizeof(T)), kVecs = int(kList) / 32 / V;
   __shared__ List lists[4];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
