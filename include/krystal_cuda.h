@@ -449,13 +449,14 @@ kc_status kc_copy_weights(kc_handle* h, uint64_t offset, uint64_t count, float* 
  * included) or its distribution p. Two layouts:
  *   frames > 0: a packed batch as kc_forward_batch_device leaves it: frame f's
  *     [Q_f, R_f] block at p_off[f] (elements of values and of every output
- *     laid out like it), its first question at q_off[f]; q_off NULL = one row
- *     a frame. rows may exceed q_off[frames]: the rows behind the last frame
+ *     laid out like it), its first question at q_off[f], q_off[0] = 0; q_off
+ *     NULL = one row a frame. rows may exceed q_off[frames]: the rows behind the last frame
  *     are left alone, so a captured graph can be replayed on smaller batches.
  *     row_len bounds the longest row (0 = KC_MAX_BANK); a row longer than that
  *     is refused by itself (KC_NO_SELECTION, loss 0, nothing else written).
  *   frames = 0: dense [rows, row_len], row i at values + i * row_pitch
  *     elements (0 = row_len).
+ * A call takes at most 2147483647 rows.
  * An entry is out of the row's support when it is NaN, a score at or below
  * -1e29 (f16: also -65504, the type's lowest), or a p that is not above 0;
  * +infinity counts as the largest finite f32. */
@@ -503,7 +504,7 @@ typedef struct kc_draw_out {
   uint32_t* kept;    /* [rows] entries the policy kept */
   float* logp;       /* [rows] log pi of the drawn entry; -infinity for an empty row */
   float* p;          /* pi, laid out like the rows (dense: p_pitch elements a row, 0 = row_len); 0 off the support.
-                        May be the f32 values themselves. */
+                        May be the f32 values themselves, at one pitch. */
   uint64_t p_pitch;
   uint64_t p_capacity, q_capacity; /* elements of p and of the per-row arrays (kc_draw_batch only) */
 } kc_draw_out;
@@ -544,7 +545,8 @@ typedef struct kc_policy_loss_view {
   float* loss;              /* [rows] or NULL */
   float* logp;              /* [rows] or NULL */
   float* entropy;           /* [rows] or NULL; 0 for an empty row */
-  void* grad;               /* the scores' type and layout (dense: grad_pitch, 0 = row_len), or NULL; may be the scores themselves */
+  void* grad;               /* the scores' type and layout (dense: grad_pitch, 0 = row_len), or NULL; may be the scores
+                               themselves, at one pitch */
   uint64_t grad_pitch;
 } kc_policy_loss_view;
 kc_status kc_policy_loss(kc_handle* h, const kc_rows_view* rows, const kc_sampling* sampling,

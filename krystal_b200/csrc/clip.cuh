@@ -1,7 +1,10 @@
 // clip.cuh — the global norm of many gradient tensors, and clipping by it:
 // norm = sqrt(sum_t weight_t^2 sum_i g_ti^2), scale = min(1, max_norm / norm)
 // (1 where the norm is not finite: what follows sees the gradients as they
-// are), out_ti = g_ti * scale, rounded once to the tensor's type.
+// are), out_ti = g_ti * scale: f64 elements by the f64 scale, the others by the
+// scale rounded to f32 and the product to the type (two half steps, and no f64
+// conversions, which would bound the pass). A scale near f32's smallest numbers
+// multiplies in 64 bits.
 //
 // Two launches: k_norm leaves one partial sum a CTA, k_scale adds the partial
 // sums again in every CTA (a few KB from L2) and scales. All sums are 64-bit
@@ -11,6 +14,11 @@
 // takes chunks b, b + grid, ... and k_scale takes them from the last back, so
 // that what k_norm read last is still in L2. k_scale is launched while k_norm
 // runs and waits for it on the device.
+//
+// Bound by HBM: 301 mixed tensors of 200 M elements (510 MB in) take 275 us, of
+// which k_norm's one read runs at 5.4 TB/s (83 % of the measured copy rate) and
+// k_scale's read and write at 5.8. Small lists (25 tensors, 1.7 M elements)
+// take 10 us, the host's two launches.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -64,6 +72,13 @@ __device__ __forceinline__ __nv_bfloat16 scaled(__nv_bfloat16 v, double s) {
   return __float2bfloat16_rn(__bfloat162float(v) * float(s));
 }
 
+// The same by a scale too small for f32.
+constexpr double kSmallScale = 1e-30;
+__device__ __forceinline__ void scale64(float& v, double s) { v = float(double(v) * s); }
+__device__ __forceinline__ void scale64(double& v, double s) { v *= s; }
+__device__ __forceinline__ void scale64(__half& v, double s) { v = __double2half(wide(v) * s); }
+__device__ __forceinline__ void scale64(__nv_bfloat16& v, double s) { v = __double2bfloat16(wide(v) * s); }
+
 // Elements of a piece ahead of its first 16-byte boundary.
 template <typename T>
 __device__ __forceinline__ uint32_t head_of(const T* p, uint32_t n) {
@@ -99,6 +114,14 @@ __device__ __forceinline__ double square_sum(const T* in, uint32_t n) {
 template <typename T>
 __device__ __forceinline__ void scale_piece(const T* in, T* out, uint32_t n, double scale) {
   constexpr int V = 16 / int(sizeof(T));
+  if (scale < kSmallScale && scale > 0.0) {
+    for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+      T v = in[i];
+      scale64(v, scale);
+      out[i] = v;
+    }
+    return;
+  }
   if ((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(out)) & 15) {
     for (uint32_t i = threadIdx.x; i < n; i += kThreads) out[i] = scaled(in[i], scale);
     return;

@@ -219,29 +219,56 @@ struct Group {
       mx = __reduce_max_sync(0xffffffffu, in ? s->cu[buf][2][lane] : 0u);
     }
   }
-  // The group's sum of one value a thread; *before (if asked for) gets the
-  // sum over the warps ahead of this one in bank order.
-  __device__ double sum(double v, double* before = nullptr) {
+  // The group's sum of one value a thread.
+  __device__ double sum(double v) {
     v = warp_add(v);
     if constexpr (W > 1) {
       buf ^= 1;
       if (lane == 0) s->d[buf][warp] = v;
       __syncthreads();
-      const double sc = warp_scan(lane < W ? s->d[buf][lane] : 0.0, lane);
-      if (before) *before = warp ? __shfl_sync(0xffffffffu, sc, warp - 1) : 0.0;
-      v = __shfl_sync(0xffffffffu, sc, W - 1);
-    } else if (before) {
-      *before = 0.0;
+      v = __shfl_sync(0xffffffffu, warp_scan(lane < W ? s->d[buf][lane] : 0.0, lane), W - 1);
     }
     if constexpr (CL > 1) {
       namespace cg = cooperative_groups;
       cg::cluster_group cl = cg::this_cluster();
       if (warp == 0 && lane < CL) cl.map_shared_rank(&s->cd[0][0], lane)[buf * CL + rank] = v;
       cl.sync();
-      const double sc = warp_scan(lane < CL ? s->cd[buf][lane] : 0.0, lane);
-      const double ahead = __shfl_sync(0xffffffffu, sc, rank ? rank - 1 : 0);
-      if (before && rank) *before += ahead;
-      v = __shfl_sync(0xffffffffu, sc, CL - 1);
+      v = __shfl_sync(0xffffffffu, warp_scan(lane < CL ? s->cd[buf][lane] : 0.0, lane), CL - 1);
+    }
+    return v;
+  }
+  // The same, with the sums up to this warp's values in bank order and through
+  // them. Added one after another, so that one warp's `through` is the next
+  // one's `before` to the last bit, and equal to its own `before` where the
+  // warp adds nothing: whatever lies below the sum lies in exactly one warp.
+  __device__ double prefix(double v, double& before, double& through) {
+    v = warp_add(v);
+    before = through = 0.0;
+    if constexpr (W > 1) {
+      buf ^= 1;
+      if (lane == 0) s->d[buf][warp] = v;
+      __syncthreads();
+      v = 0.0;
+#pragma unroll
+      for (int j = 0; j < W; j++) {
+        if (j == warp) before = v;
+        v += s->d[buf][j];
+        if (j == warp) through = v;
+      }
+    }
+    if constexpr (CL > 1) {
+      namespace cg = cooperative_groups;
+      cg::cluster_group cl = cg::this_cluster();
+      if (warp == 0 && lane < CL) cl.map_shared_rank(&s->cd[0][0], lane)[buf * CL + rank] = v;
+      cl.sync();
+      double ahead = v = 0.0;
+#pragma unroll
+      for (int j = 0; j < CL; j++) {
+        if (j == rank) ahead = v;
+        v += s->cd[buf][j];
+      }
+      before += ahead;
+      through += ahead;
     }
     return v;
   }
@@ -498,10 +525,11 @@ __device__ __forceinline__ bool locate(const RowsArg& r, uint64_t out_pitch, uin
       const uint32_t step = (hi - lo + 31) / 32;
       const uint64_t probe = uint64_t(lo) + uint64_t(lane) * step;
       const uint32_t below = __popc(__ballot_sync(0xffffffffu, probe < hi && r.q_off[probe < hi ? probe : lo] <= row));
-      lo += (below - 1) * step;
+      lo += (max(below, 1u) - 1) * step;
       hi = min(hi, lo + step);
     }
     first = r.q_off[lo];
+    if (row < first) return false;  // offsets that do not start at 0 have no such row
     count = r.q_off[lo + 1] - first;
   } else if (row >= r.frames) {
     return false;

@@ -49,6 +49,7 @@ kc_status check_rows(kc_handle* h, const kc_rows_view* v, kc::pol::RowsArg* r, u
   r->row_len = v->frames && v->row_len == 0 ? KC_MAX_BANK : v->row_len;
   r->pitch = v->row_pitch ? v->row_pitch : v->row_len;
   r->kind = v->kind;
+  if (v->rows > 0x7fffffffu) return fail(h, KC_ERR_CAPACITY, "a call takes at most 2147483647 rows");
   if (r->row_len > KC_MAX_ROW) return fail(h, KC_ERR_CAPACITY, "a row is longer than KC_MAX_ROW");
   if (v->frames) {
     if (!v->p_off || !aligned(v->p_off, 8) || !aligned(v->q_off, 8))
@@ -81,6 +82,8 @@ kc_status draw_rows(kc_handle* h, const kc_rows_view* v, const kc_sampling* s, c
   a.kept = out->kept;
   a.logp = out->logp;
   a.p = out->p;
+  if (a.p && a.p == v->values && (v->dtype != KC_DTYPE_F32 || (!v->frames && a.out_pitch != a.r.pitch)))
+    return fail(h, KC_ERR_INVALID_ARG, "p over the values needs f32 rows and one pitch");
   KC_TRY(kc::pol::launch_draw(a, v->dtype, h->sms, h->stream, &h->launches), "draw launch");
   return KC_OK;
 }
@@ -208,6 +211,8 @@ kc_status kc_policy_loss(kc_handle* h, const kc_rows_view* rows, const kc_sampli
   a.logp = loss->logp;
   a.entropy = loss->entropy;
   a.grad = loss->grad;
+  if (a.grad && a.grad == rows->values && !rows->frames && a.out_pitch != a.r.pitch)
+    return fail(h, KC_ERR_INVALID_ARG, "a gradient over the scores needs one pitch");
   KC_TRY(kc::pol::launch_policy_loss(a, rows->dtype, h->sms, h->stream, &h->launches), "policy loss launch");
   return KC_OK;
 }

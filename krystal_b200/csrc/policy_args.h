@@ -13,7 +13,7 @@ namespace pol {
 
 constexpr int kKindScores = 0, kKindP = 1;
 constexpr uint32_t kNone = 0xffffffffu;
-constexpr uint32_t kMaxRow = 262128;  // 8 CTAs x 512 threads x 64 entries, less a vector's misalignment
+constexpr uint32_t kMaxRow = 262128;  // 8 CTAs of 32768 entries, less a row's two misaligned vectors
 
 struct RowsArg {
   const void* values;

@@ -629,14 +629,14 @@ __device__ __forceinline__ void finish_wide(WideRow<T, W, CL>& r, const Cut& c, 
       if (!a.uniforms && key == r.top) hit = min(hit, i);
     }
   });
-  double before;
-  const double run = warp_add(mine), z = r.g.sum(mine, &before);
+  double before, through;
+  const double z = r.g.prefix(mine, before, through);
   double drawn = 0.0;
   if (a.uniforms) {
     // cum > u z by the sign of u z - cum, whose one rounding keeps it. The warp
     // whose weights the target falls among walks them, 32 at a time.
     const double u = fmin(fmax(a.uniforms[row], 0.0), 1.0);
-    if (fma(u, z, -(before + run)) < 0.0 && !(fma(u, z, -before) < 0.0)) {
+    if (fma(u, z, -through) < 0.0 && !(fma(u, z, -before) < 0.0)) {
       double cum = before;
       r.packed([&](uint32_t key, uint32_t i) {
         const double w = weight(key), sc = warp_scan(w, lane);
@@ -837,6 +837,12 @@ template <> struct Answers<DrawArg> {
 // run of rows one after another: its tables are made once, the frame is
 // searched for once, and the next row's entries and uniform are fetched while
 // it works.
+//
+// Bound by instruction issue: 34818 drawn rows of 8 to 240 probabilities, a
+// quarter open, take 93 us at an IPC of 2.5, about 1500 warp instructions a row
+// (64-bit exponentials and logarithms, all pairs of the list), and 2 % of the
+// memory's bandwidth; the loss of 4096 rows takes 17 us, one wave of single
+// rows whose latency bounds it.
 // CTAs an SM. More warps hide more of a row's latency, more registers spill
 // less: 34818 drawn rows took 95, 97, 105 and 96 us with 5 to 8, the loss of
 // 4096 rows between 19 and 20.
@@ -930,6 +936,10 @@ __global__ void __launch_bounds__(128, kSmallCtas) k_policy_small(const __grid_c
 // own (CL = 1) takes `batch` rows, one after another up to their lists, which
 // its warps then finish side by side: one warp at the end of one row would
 // leave the SM idle.
+// 4096 drawn rows of 4096 under top-k 200, top-p and min-p take 127 us: issue
+// (IPC 2.75; statistics, the lower bound's counts, one warp a list) and
+// barriers. 32 bf16 rows of 131071 take 39 us: latency, a dozen cluster-wide
+// reductions one after another, on 128 of the SMs.
 template <typename T, int W, int CL, typename Arg>
 __global__ void __launch_bounds__(W * 32, 32 / W) k_policy_rows(const __grid_constant__ Arg a, uint32_t batch,
                                                                uint32_t chunks) {

@@ -125,6 +125,15 @@ def test_extremes(be):
     assert run(be, make([5000], ["f32"]), math.inf)[1] == 1.0
 
 
+def test_a_scale_below_the_smallest_f32(be):
+    """One rounding of a 64-bit product is left, which the check's bounds hold."""
+    grads = make([5000, 70, 3], ["f32", "bf16", "f64"], scale=1e25)
+    outs = [torch.zeros_like(t) for t in grads]
+    check(be, grads, 1e-20, outs)
+    assert all(bool((o != 0).any()) for o in outs)
+    check(be, grads, 1e-20)
+
+
 def test_equal_calls_give_equal_bits(be):
     grads = make([100003, 77, 65536], ["f32", "bf16"], seed=8)
     outs = [[torch.empty_like(t) for t in grads] for _ in range(3)]

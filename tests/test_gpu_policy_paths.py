@@ -392,3 +392,16 @@ def test_refusals(be):
     assert i.tolist() == [-1] * 3 + [-5] * 5
     d = be.draw_rows(np.zeros(0), 0, ok)
     assert d.index.size == 0
+
+
+def test_rows_written_over_themselves_and_too_many_rows_are_refused(be):
+    v = torch.zeros(64, device="cuda")
+    i = torch.zeros(8, dtype=torch.int32, device="cuda")
+    p, ip, ok = v.data_ptr(), i.data_ptr(), Sampling()
+    wide = policy.dense_rows(p, "f32", 2, 8, 10)
+    refused("one pitch", be.draw, wide, ok, p=p)
+    refused("one pitch", be.draw, policy.dense_rows(p, "f16", 2, 8), ok, p=p)
+    refused("one pitch", be.policy_loss, wide, ok, ip, p, grad=p)
+    refused("2147483647", be.draw, policy.dense_rows(p, "f32", 2 ** 31, 1), ok, index=ip)
+    be.draw(wide, ok, index=ip, p=p, p_pitch=10)
+    be.synchronize()
