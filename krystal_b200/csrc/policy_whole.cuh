@@ -9,8 +9,9 @@ namespace pol {
 // ---------------------------------------------------------------------------
 // The policy loss over the whole softmax, nothing cut: no decision hangs on a
 // last bit, so the row stays as it was loaded (a warp's registers, NV 16-byte
-// vectors a lane; longer rows: k_policy_long) and its exponentials are f32. With u_j = (v_j - m) log2(e) / T, taken as one
-// fma of v_j (the rounding of m log2(e) / T is common to all and cancels),
+// vectors a lane; longer rows: k_policy_long) and its exponentials are f32. With
+// u_j = (v_j - m) log2(e) / T, taken as one fma of v_j (the rounding of
+// m log2(e) / T is common to all and cancels),
 //   Z = sum 2^u, S = sum 2^u u, log pi_j = ln 2 (u_j - log2 Z),
 //   H = ln 2 (log2 Z - S / Z), and the gradient is
 //   2^u_j (u_j B + C) with B = g beta ln 2 / (T Z), C = g (A + beta (H - ln Z)) / (T Z)
@@ -55,7 +56,6 @@ __device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigne
 template <typename T> struct Floor { static constexpr float value = -1.00025555e30f; };  // a bf16 value
 template <> struct Floor<__half> { static constexpr float value = -65504.0f; };
 
-
 // The largest of a thread's vectors; raise() also raises a vector's entries to
 // the floor, a NaN too.
 template <typename T> struct Top;
@@ -91,23 +91,45 @@ template <> struct Top<__nv_bfloat16> : TopPairs<__nv_bfloat162> {
   __device__ __forceinline__ Top() : TopPairs(__float2bfloat162_rn(Floor<__nv_bfloat16>::value)) {}
 };
 
+struct WholeRow {
+  float sc, off, m;
+  bool plain;
+  __device__ float u_of(float f) const { return plain ? fmaf(f, sc, off) : (fminf(f, m) - m) * sc; }
+};
+
+// log2(e) / T; a T below 5e-39 keeps it finite, so that the largest entry's u is 0.
+__device__ __forceinline__ float scale_of(float t) { return fminf(1.44269504088896340736f / t, 3.402823466e38f); }
+
+// The gradient entry by entry in 64 bits: where a factor of the quick form
+// could overflow before the product does, and at the action, where pi - 1 is
+// the row's largest gradient.
+struct WholeSlope {
+  float rw, t, z, lg_z, h, adv, beta;
+  __device__ __forceinline__ float of(float u) const {
+    const double w = double(exp2_fast(u)), e = 0.69314718055994530942 * (double(u) - double(lg_z)) + double(h);
+    return float(double(rw) / double(t) * (w / double(z) * fma(double(beta), e, double(adv))));
+  }
+  __device__ __forceinline__ float of_action(float u, float logp) const {
+    const double pi = double(exp2_fast(u)) / double(z);
+    return float(double(rw) / double(t) * fma(double(adv), pi - 1.0, double(beta) * pi * (double(logp) + h)));
+  }
+};
+
 template <typename T, int NV>
 __global__ void __launch_bounds__(128) k_policy_whole(LossArg a) {
-  constexpr int W = 1, CL = 1;
   constexpr int V = 16 / int(sizeof(T));
-  constexpr uint32_t kCap = uint32_t(32) * V * NV * W * CL;
-  __shared__ typename Group<W, CL>::Shared sh;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t row = W == 1 ? blockIdx.x * 4 + warp : blockIdx.x / CL;
+  constexpr uint32_t kCap = uint32_t(32) * V * NV;
+  const int lane = threadIdx.x & 31;
+  const uint32_t row = blockIdx.x * 4 + (threadIdx.x >> 5);
   if (row >= a.r.rows) return;
   RowAt at;
   if (!locate(a.r, a.out_pitch, row, lane, &at)) return;
-  Group<W, CL> g(sh, lane, W == 1 ? 0 : warp);
+  Group<1, 1> g(lane);
   const bool fits = at.n <= a.r.row_len && at.n + V - 1 <= kCap;
   const int n = fits ? int(at.n) : 0;
   const T* in = static_cast<const T*>(a.r.values) + at.in;
   const int shift = int((reinterpret_cast<uintptr_t>(in) & 15) / sizeof(T));
-  const int i0 = g.segment() * 32 * V * NV + lane * V - shift;
+  const int i0 = lane * V - shift;
   constexpr float floor_v = Floor<T>::value;
 
   // the row, masked entries raised to the floor; its largest
@@ -140,10 +162,10 @@ __global__ void __launch_bounds__(128) k_policy_whole(LossArg a) {
   const float m = endless ? kMost : value_of(top);
   const float t_row = a.c.row_temperature ? a.c.row_temperature[row] : a.c.temperature;
   const bool open_t = t_row > 0.0f, any = m > Lowest<T>::open_above;
-  const float sc = open_t ? 1.44269504088896340736f / t_row : 0.0f;  // log2(e) / T
+  const float sc = open_t ? scale_of(t_row) : 0.0f;
   const bool plain = !endless && (m - Lowest<T>::open_above) * sc >= 200.0f && fabsf(m * sc) < 1e5f && sc < 1e6f;
   const float off = -m * sc;
-  auto u_of = [&](float f) { return plain ? fmaf(f, sc, off) : (fminf(f, m) - m) * sc; };
+  const WholeRow row_of{sc, off, m, plain};
 
   // Z and S
   float2 zs = make_float2(0.0f, 0.0f);
@@ -172,7 +194,7 @@ __global__ void __launch_bounds__(128) k_policy_whole(LossArg a) {
       for (int e = 0; e < V; e++) {
         const float f = entry<T>(v[c], e);
         if (f > Lowest<T>::open_above) {
-          const float u = fmaxf(u_of(f), -2000.0f), w = exp2_fast(u);
+          const float u = fmaxf(row_of.u_of(f), -2000.0f), w = exp2_fast(u);
           z += double(w);
           s += double(w) * double(u);
         }
@@ -186,7 +208,7 @@ __global__ void __launch_bounds__(128) k_policy_whole(LossArg a) {
   for (int c = 0; c < NV; c++) asm volatile("" : "+r"(v[c][0]), "+r"(v[c][1]), "+r"(v[c][2]), "+r"(v[c][3]));
 
   // the row's answer
-  const float ua = u_of(fminf(va, kMost));
+  const float ua = row_of.u_of(fminf(va, kMost));
   bool live = asked && va > Lowest<T>::open_above && ua * kLn2 >= float(kDropped);
   if (!open_t) {  // temperature 0: the first largest entry alone
     uint32_t first = 0xffffffffu;
@@ -204,15 +226,15 @@ __global__ void __launch_bounds__(128) k_policy_whole(LossArg a) {
   const float logp = open_t ? kLn2 * (ua - lg_z) : 0.0f;
   const bool learns = asked && live && open_t;
   const float adv = a.advantage[row], beta = a.beta;
-  if (g.segment() == 0 && lane == 0) {
+  if (lane == 0) {
     if (a.loss) a.loss[row] = learns ? fmaf(-adv, logp, -beta * h) : 0.0f;
     if (a.logp) a.logp[row] = !asked ? 0.0f : live ? logp : -INFINITY;
     if (a.entropy) a.entropy[row] = h;
   }
   if (!a.grad || !fits) return;
   T* out = static_cast<T*>(a.grad) + at.out;
-  const float gt = learns ? (a.row_weight ? a.row_weight[row] : 1.0f) / t_row : 0.0f;
-  const float over = gt * inv_z;
+  const float rw = a.row_weight ? a.row_weight[row] : 1.0f, gt = learns ? rw / t_row : 0.0f, over = gt * inv_z;
+  const WholeSlope slope{rw, t_row, zs.x, lg_z, h, adv, beta};
   const float B = over * beta * kLn2, C = over * fmaf(beta, h - kLn2 * lg_z, adv);
   const bool quick = plain && fabsf(B) < 10.0f;
   RowWriter<T> writer(out, n, lane, i0);
@@ -233,17 +255,15 @@ __global__ void __launch_bounds__(128) k_policy_whole(LossArg a) {
       float f[V];
 #pragma unroll
       for (int e = 0; e < V; e++) {
-        const float x = entry<T>(v[c], e), u = fmaxf(u_of(x), -2000.0f);
-        f[e] = learns && x > Lowest<T>::open_above ? exp2_fast(u) * fmaf(u, B, C) : 0.0f;
+        const float x = entry<T>(v[c], e);
+        f[e] = learns && x > Lowest<T>::open_above ? slope.of(fmaxf(row_of.u_of(x), -2000.0f)) : 0.0f;
       }
 #pragma unroll
       for (int e = 0; e < V; e += 2) set2<T>(d, e, f[e], f[e + 1]);
     }
     // the action's entry, and its lane's alone, gets the rest
     if (learns && act - uint32_t(i) < uint32_t(V)) {
-      // (in 64 bits: pi - 1 is the row's largest gradient)
-      const double pi = double(exp2_fast(ua)) / double(zs.x), scale = double(a.row_weight ? a.row_weight[row] : 1.0f) / t_row;
-      const float x = float(scale * fma(double(adv), pi - 1.0, double(beta) * pi * (double(logp) + h)));
+      const float x = slope.of_action(ua, logp);
 #pragma unroll
       for (int e = 0; e < V; e += 2) {
         uint32_t w[4];
@@ -257,19 +277,6 @@ __global__ void __launch_bounds__(128) k_policy_whole(LossArg a) {
   writer.finish();
 }
 
-
-// The same for longer rows, which stay in shared memory as they were loaded:
-// CL CTAs of NT threads a row, each with its segment of 16-byte vectors. The
-// loops are rolled (a row in registers would unroll them over its whole length,
-// and the instruction cache then bounds them), three CTAs an SM overlap one
-// row's loads with another's arithmetic, and the last pass reads the row at the
-// gradient's alignment, so that every store is a whole vector.
-struct WholeRow {
-  float sc, off, m;
-  bool plain;
-  __device__ float u_of(float f) const { return plain ? fmaf(f, sc, off) : (fminf(f, m) - m) * sc; }
-};
-
 // The vector that starts O entries behind w[0]: O of the next one's. O = 0: w itself.
 template <typename T, int WORDS>
 __device__ __forceinline__ void shifted(const uint4& x, const uint4& y, bool odd, uint32_t* d) {
@@ -279,6 +286,15 @@ __device__ __forceinline__ void shifted(const uint4& x, const uint4& y, bool odd
     d[j] = sizeof(T) == 2 && odd ? __byte_perm(a[j + WORDS], a[j + WORDS + 1], 0x5432) : a[j + WORDS];
 }
 
+// The same for longer rows, which stay in shared memory as they were loaded:
+// CL CTAs of NT threads a row, each with its segment of 16-byte vectors. The
+// loops are rolled (a row in registers would unroll them over its whole length,
+// and the instruction cache then bounds them), three CTAs an SM overlap one
+// row's loads with another's arithmetic, and the last pass reads the row at the
+// gradient's alignment, so that every store is a whole vector. 4096 bf16 rows of
+// 32001 take 120 us, 4.4 TB/s and two thirds of what one read and one write cost
+// at the measured copy rate: two exponentials an entry keep their pipe busy half
+// the time, and a CTA's own load, arithmetic and store follow each other.
 template <typename T, int NT, int CL>
 __global__ void __launch_bounds__(NT) k_policy_long(LossArg a, uint32_t seg_vecs) {
   constexpr int V = 16 / int(sizeof(T)), W = NT / 32;
@@ -336,7 +352,7 @@ __global__ void __launch_bounds__(NT) k_policy_long(LossArg a, uint32_t seg_vecs
   const float m = endless ? kMost : value_of(top);
   const float t_row = a.c.row_temperature ? a.c.row_temperature[row] : a.c.temperature;
   const bool open_t = t_row > 0.0f, any = m > Lowest<T>::open_above;
-  const float sc = open_t ? 1.44269504088896340736f / t_row : 0.0f;  // log2(e) / T
+  const float sc = open_t ? scale_of(t_row) : 0.0f;
   const bool plain = !endless && (m - Lowest<T>::open_above) * sc >= 200.0f && fabsf(m * sc) < 1e5f && sc < 1e6f;
   const WholeRow wr{sc, -m * sc, m, plain};
   const unsigned long long sc2 = pack2(sc, sc), off2 = pack2(wr.off, wr.off);
@@ -408,6 +424,7 @@ __global__ void __launch_bounds__(NT) k_policy_long(LossArg a, uint32_t seg_vecs
   if (!a.grad || !fits) return;
   T* out = static_cast<T*>(a.grad) + at.out;
   const float rw = a.row_weight ? a.row_weight[row] : 1.0f, gt = learns ? rw / t_row : 0.0f, over = gt * inv_z;
+  const WholeSlope slope{rw, t_row, zs.x, lg_z, h, adv, beta};
   const float B = over * beta * kLn2, C = over * fmaf(beta, h - kLn2 * lg_z, adv);
   const bool quick = plain && fabsf(B) < 10.0f;
   const unsigned long long B2 = pack2(B, B), C2 = pack2(C, C);
@@ -418,15 +435,16 @@ __global__ void __launch_bounds__(NT) k_policy_long(LossArg a, uint32_t seg_vecs
   const int skew = int((16 - (reinterpret_cast<uintptr_t>(out + i0) & 15)) & 15) / int(sizeof(T));
   const int words = skew * int(sizeof(T)) / 4;
   const bool odd = sizeof(T) == 2 && (skew & 1);
-  auto groups = [&](auto w_) {
+  const int ahead = skew && g.rank == 0 ? 1 : 0;
+  auto groups = [&](auto w_, auto quick_) {
     constexpr int WORDS = decltype(w_)::value;
 #pragma unroll 2
-    for (int j = tid - (skew && g.rank == 0 ? 1 : 0); j < mine; j += NT) {
+    for (int j = tid - ahead; j < mine; j += NT) {
       const int i = i0 + j * V + skew;
       uint32_t w[4], d[4];
       const uint4 x = sm[j];
       shifted<T, WORDS>(x, WORDS || odd ? sm[j + 1] : x, odd, w);
-      if (quick) {
+      if constexpr (decltype(quick_)::value) {
 #pragma unroll
         for (int e = 0; e < V; e += 2) {
           const unsigned long long u = fma2(pack2(entry<T>(w, e), entry<T>(w, e + 1)), sc2, off2);
@@ -438,24 +456,11 @@ __global__ void __launch_bounds__(NT) k_policy_long(LossArg a, uint32_t seg_vecs
         float f[V];
 #pragma unroll
         for (int e = 0; e < V; e++) {
-          const float x = entry<T>(w, e), u = fmaxf(wr.u_of(x), -2000.0f);
-          f[e] = learns && x > Lowest<T>::open_above ? exp2_fast(u) * fmaf(u, B, C) : 0.0f;
+          const float x = entry<T>(w, e);
+          f[e] = learns && x > Lowest<T>::open_above ? slope.of(fmaxf(wr.u_of(x), -2000.0f)) : 0.0f;
         }
 #pragma unroll
         for (int e = 0; e < V; e += 2) set2<T>(d, e, f[e], f[e + 1]);
-      }
-      // the action's entry gets the rest, in 64 bits: pi - 1 is the row's largest gradient
-      if (learns && act - uint32_t(i) < uint32_t(V)) {
-        const double pi = double(exp2_fast(ua)) / double(zs.x), scale = double(rw) / t_row;
-        const float x = float(scale * fma(double(adv), pi - 1.0, double(beta) * pi * (double(logp) + h)));
-        uint32_t y[4];
-#pragma unroll
-        for (int e = 0; e < V; e += 2) {
-          set2<T>(y, e, x, x);
-          constexpr int S = int(sizeof(T));
-          if (uint32_t(i + e) == act) d[e * S / 4] = first_of<T>(y[e * S / 4], d[e * S / 4]);
-          if (uint32_t(i + e + 1) == act) d[(e + 1) * S / 4] = second_of<T>(y[(e + 1) * S / 4], d[(e + 1) * S / 4]);
-        }
       }
       if (i >= 0 && i + V <= n) {
         __stcs(reinterpret_cast<uint4*>(out + i), make_uint4(d[0], d[1], d[2], d[3]));
@@ -466,11 +471,21 @@ __global__ void __launch_bounds__(NT) k_policy_long(LossArg a, uint32_t seg_vecs
       }
     }
   };
-  switch (words) {
-    case 0: groups(std::integral_constant<int, 0>{}); break;
-    case 1: groups(std::integral_constant<int, 1>{}); break;
-    case 2: groups(std::integral_constant<int, 2>{}); break;
-    default: groups(std::integral_constant<int, 3>{}); break;
+  auto pass = [&](auto quick_) {  // (two loops: one with the test inside would hold what both need)
+    switch (words) {
+      case 0: groups(std::integral_constant<int, 0>{}, quick_); break;
+      case 1: groups(std::integral_constant<int, 1>{}, quick_); break;
+      case 2: groups(std::integral_constant<int, 2>{}, quick_); break;
+      default: groups(std::integral_constant<int, 3>{}, quick_); break;
+    }
+  };
+  if (quick) pass(std::true_type{});
+  else pass(std::false_type{});
+  // the action's entry gets the rest, from the thread that wrote its group
+  if (learns) {
+    const int to_act = int(act) - i0 - skew + V, j = to_act / V - 1;
+    if (to_act >= 0 && j >= -ahead && j < mine && (j + ahead) % NT == tid)
+      out[act] = from_f32<T>(slope.of_action(ua, logp));
   }
 }
 

@@ -592,6 +592,47 @@ def test_batches_of_long_rows(be, rows, n):
         check_ragged(be, v, "bf16", where, view, cut, rng.random(rows + spare), int(off[-1]), spare)
 
 
+@pytest.mark.parametrize("n", [4096, 60000])
+def test_uniforms_at_the_borders_of_the_warps(be, n):
+    """Nothing is cut, so the row stays spread over its group, and uniforms step
+    by last bits over every border a split into 32 could have. A last bit of
+    the sums may move the answer to the border's other entry, no further."""
+    rng = np.random.default_rng(n)
+    p = (rng.random(n) ** 3 + 1e-6).astype(np.float32)
+    p[rng.random(n) < 0.02] = 0.0
+    cum = np.cumsum(p.astype(np.longdouble))
+    borders = np.unique(np.concatenate([np.arange(1, 32) * n // 32, np.arange(512, n, 512), np.arange(1024, n, 1024)]))
+    if n > 4096:
+        borders = borders[rng.permutation(borders.size)[:24]]
+    u, where = [], []
+    for b in borders:
+        mid = float(cum[b - 1] / cum[-1])
+        for k in range(-20, 21):
+            u.append(mid + k * np.spacing(mid))
+            where.append(b)
+    rows = len(u)
+    v = on_gpu(p).expand(rows, n).contiguous()
+    du, idx = on_gpu(np.array(u)), torch.zeros(rows, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    be.draw(policy.dense_rows(v.data_ptr(), "f32", rows, n, kind="p"), policy.Sampling(), du.data_ptr(),
+            index=idx.data_ptr())
+    be.synchronize()
+    open_ = np.flatnonzero(p > 0)
+    for got, b in zip(idx.tolist(), where):
+        at = int(np.searchsorted(open_, b))  # the first open entry at or behind the border
+        assert got in open_[max(at - 1, 0):at + 1], (got, b)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", [40, 900, 5000])
+def test_whole_softmax_at_the_smallest_temperatures(be, dtype, n):
+    """1 / T beyond f32: one entry has all of the mass, no gradient is left."""
+    v = scores(np.random.default_rng(n), 4, n, dtype, 0.3)
+    v[:, 5] = 40.0
+    temps = [1e-38, 1e-40, 2.0 ** -149, 3e-39]
+    whole_loss(be, v, dtype, [5, 5, 5, 6], [1.0, -2.0, 0.5, 1.0], 0.1, temps)
+
+
 def test_draws_over_the_values_themselves(be):
     """p may be the f32 values: short rows, lists of long ones, and spread rows."""
     rng = np.random.default_rng(6)
