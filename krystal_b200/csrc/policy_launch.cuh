@@ -100,9 +100,15 @@ cudaError_t cut_as(const A& a, int sms, cudaStream_t s) {
 }
 
 // Rows that k_policy_long keeps in shared memory: CL CTAs of NT threads a row,
-// up to kShort bytes a row 128 threads, up to kLong 256 (three CTAs an SM),
-// beyond that a cluster of 8 x 512.
-constexpr uint64_t kShort = 16384, kLong = 73728;
+// up to kSmall bytes a row 64 threads, up to kShort 128, up to kLong 256 (three
+// CTAs an SM), beyond that a cluster of 8 x 512. Few threads a row, and so many
+// rows an SM, hide one row's reductions behind another's loads: 16384 bf16 rows
+// of 8000 take 109 us on 64 threads and 121 on 128; 8192 of 13000 104 on 64 and
+// 88 on 128; 4096 of 17000 66 on 128 and 68 on 256; 4096 of 25001 100 on 128, 88
+// on 256 and 98 on 384. Up to 1024 entries a warp keeps the row in registers:
+// 65536 bf16 rows of 1000 take 98 us, and 197 in shared memory; of 1100 to 2000
+// a row in registers is the slower one (102 and 78 us).
+constexpr uint64_t kSmall = 16384, kShort = 32768, kLong = 73728;
 template <typename T>
 constexpr size_t long_smem(uint64_t row_len, int cl) {
   constexpr uint64_t V = 16 / sizeof(T);
@@ -112,7 +118,8 @@ template <typename T>
 cudaError_t prepare_as() {
   const auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
   cudaError_t e;
-  if ((e = cudaFuncSetAttribute(k_policy_long<T, 128, 1>, attr, int(long_smem<T>(kShort / sizeof(T), 1)))) ||
+  if ((e = cudaFuncSetAttribute(k_policy_long<T, 64, 1>, attr, int(long_smem<T>(kSmall / sizeof(T), 1)))) ||
+      (e = cudaFuncSetAttribute(k_policy_long<T, 128, 1>, attr, int(long_smem<T>(kShort / sizeof(T), 1)))) ||
       (e = cudaFuncSetAttribute(k_policy_long<T, 256, 1>, attr, int(long_smem<T>(kLong / sizeof(T), 1)))) ||
       (e = cudaFuncSetAttribute(k_policy_long<T, 512, 8>, attr, int(long_smem<T>(kMaxRow, 8)))))
     return e;
@@ -143,7 +150,9 @@ inline cudaError_t whole_as(const LossArg& a, cudaStream_t s) {
   constexpr int V = 16 / sizeof(T);
   const uint64_t need = a.r.row_len + V - 1;
   if (need <= 256) return go_warps(k_policy_whole<T, 8 / V>, a, s);
+  if (need <= 512) return go_warps(k_policy_whole<T, 16 / V>, a, s);
   if (need <= 1024) return go_warps(k_policy_whole<T, 32 / V>, a, s);
+  if (need * sizeof(T) <= kSmall) return go_long<T, 64, 1>(a, s);
   if (need * sizeof(T) <= kShort) return go_long<T, 128, 1>(a, s);
   if (need * sizeof(T) <= kLong) return go_long<T, 256, 1>(a, s);
   return go_long<T, 512, 8>(a, s);

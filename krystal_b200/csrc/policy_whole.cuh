@@ -15,8 +15,8 @@ namespace pol {
 //   Z = sum 2^u, S = sum 2^u u, log pi_j = ln 2 (u_j - log2 Z),
 //   H = ln 2 (log2 Z - S / Z), and the gradient is
 //   2^u_j (u_j B + C) with B = g beta ln 2 / (T Z), C = g (A + beta (H - ln Z)) / (T Z)
-// but for -g A / T more at the action. Sums: eight f32 partial sums of at most
-// 16 terms a thread, joined by trees. Arithmetic on pairs (f32x2).
+// but for -g A / T more at the action. Sums: four or eight f32 partial sums
+// of at most 18 terms a thread, joined by trees. Arithmetic on pairs (f32x2).
 //
 // Masked entries need no test where they vanish by themselves: NaN and what
 // lies below the mask's floor is raised to it as the row is loaded, and 2^u is

@@ -382,6 +382,9 @@ def whole_tolerances(row, n, adv, beta, scale, logp):
     part = np.zeros(n)
     part[j] = scale * pi * ((abs(adv) + beta * (np.abs(logpi) + h)) * (2.0 ** -17 + 2.0 ** -22 * np.abs(logpi))
                             + beta * e_h)
+    # A weight below 2^-126 is 0: such a pi is off by at most 2^-126 (Z is 1 or
+    # more), and pi |log pi|, which grows with pi there, by 126 ln 2 times that.
+    part[j] += scale * 2.0 ** -126 * (abs(adv) + beta * (88 + h))
     return np.array([abs(adv) * e_logp + beta * e_h, e_logp, e_h]), part
 
 
@@ -403,6 +406,8 @@ def whole_loss(be, v, dtype, act, adv, beta, temps):
         t = t if t > 0 else 0.0
         row = ref.policy(wide(v[i]), t, f16=dtype == "f16")
         L, l, e, g = ref.loss(row, n, int(act[i]), float(np.float32(adv[i])), float(np.float32(beta)), t)
+        if dtype == "f16":  # half a step above 65504 and beyond, f16 rounds to infinity
+            g = np.where(np.abs(g) >= 65520.0, np.copysign(np.inf, g), g)
         stat, part = whole_tolerances(row, n, float(adv[i]), beta, 1.0 / t if t else 0.0, l)
         near([float(lo[i]), float(lp[i]), float(h[i])], [L, l, e], HALF["f32"], stat)
         near(got[i], g, HALF[dtype], TINY[dtype] + part)
@@ -621,6 +626,21 @@ def test_uniforms_at_the_borders_of_the_warps(be, n):
     for got, b in zip(idx.tolist(), where):
         at = int(np.searchsorted(open_, b))  # the first open entry at or behind the border
         assert got in open_[max(at - 1, 0):at + 1], (got, b)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", [249, 301, 505, 1017, 2001, 3501, 7001, 8185, 13001, 16377, 30001])
+def test_whole_softmax_at_every_group(be, dtype, n):
+    """Odd rows, each at an alignment of its own, on both sides of the group
+    sizes' borders; the large advantage takes the gradient's 64-bit form."""
+    rng = np.random.default_rng(n)
+    v = scores(rng, 7, n, dtype, 0.2)
+    act = [int(ref.support(wide(r), f16=dtype == "f16")[-1:].sum()) for r in v]
+    adv, temps = rng.normal(size=7), np.array([1.0, 0.6, 0.05, 1.0, 1.0, 2.5, 0.3])
+    adv[2] = 1e4
+    whole_loss(be, v, dtype, act, adv, 0.1, temps)
+    if dtype != "f16":  # f16 gradients end at 65504
+        whole_loss(be, v, dtype, act, adv, 300.0, temps)
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
