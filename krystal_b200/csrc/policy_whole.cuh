@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(128) k_policy_whole(LossArg a) {
   const float rw = a.row_weight ? a.row_weight[row] : 1.0f, gt = learns ? rw / t_row : 0.0f, over = gt * inv_z;
   const WholeSlope slope{rw, t_row, zs.x, lg_z, h, adv, beta};
   const float B = over * beta * kLn2, C = learns ? over * fmaf(beta, h - kLn2 * lg_z, adv) : 0.0f;  // (adv may be NaN)
-  const bool quick = plain && fabsf(B) < 10.0f;
+  const bool quick = plain && fabsf(B) < 10.0f && fabsf(C) < 1e30f;  // (a vanished weight times infinity)
   RowWriter<T> writer(out, n, lane, i0);
   const unsigned long long sc2 = pack2(sc, sc), off2 = pack2(off, off), B2 = pack2(B, B), C2 = pack2(C, C);
 #pragma unroll
@@ -426,7 +426,7 @@ __global__ void __launch_bounds__(NT) k_policy_long(LossArg a, uint32_t seg_vecs
   const float rw = a.row_weight ? a.row_weight[row] : 1.0f, gt = learns ? rw / t_row : 0.0f, over = gt * inv_z;
   const WholeSlope slope{rw, t_row, zs.x, lg_z, h, adv, beta};
   const float B = over * beta * kLn2, C = learns ? over * fmaf(beta, h - kLn2 * lg_z, adv) : 0.0f;  // (adv may be NaN)
-  const bool quick = plain && fabsf(B) < 10.0f;
+  const bool quick = plain && fabsf(B) < 10.0f && fabsf(C) < 1e30f;  // (a vanished weight times infinity)
   const unsigned long long B2 = pack2(B, B), C2 = pack2(C, C);
   // Group j of the gradient starts at entry q = i0 + j V + skew of the row, on a
   // 16-byte boundary of out: entries skew.. of vector j and those of j + 1

@@ -69,3 +69,84 @@ def test_a_row_without_an_answer_has_no_gradient_whatever_its_factors(be, n, dty
     assert np.isfinite(h).all()
     for i in (0, len(rows) + 1):  # the rows beside them learn
         assert np.isfinite(lo[i]) and lo[i] != 0 and bool(torch.isfinite(g[i]).all()) and float(g[i, 1]) != 0
+
+
+def plain_gradient(v, act, adv, beta, t, weight, f16):
+    """The uncut gradient of one row in 64 bits, and the size of the terms that
+    cancel in it; 0 for masked entries whatever the factors, and everywhere
+    where the action's weight is below e^-700, which cannot be drawn."""
+    v = v.double().numpy()
+    j = np.flatnonzero(v > (-65504.0 if f16 else -1e29))
+    j = j[(v[j] - v[j].max()) / t >= -700.0]
+    x = (v[j] - v[j].max()) / t
+    w = np.exp(x)
+    pi, logpi = w / w.sum(), x - np.log(w.sum())
+    h = -(pi * logpi).sum()
+    d = adv * pi + beta * pi * (logpi + h)
+    d[j == act] -= adv
+    g, size = np.zeros(v.size), np.zeros(v.size)
+    if act not in j:
+        return j, pi, g, size
+    g[j] = weight * d / t
+    size[j] = abs(weight) / t * (abs(adv) * (pi + (j == act)) + abs(beta) * pi * (np.abs(logpi) + h))
+    return j, pi, g, size
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", LENGTHS)
+@pytest.mark.parametrize("beta", [0.0, 0.1])
+def test_gradients_whose_factors_leave_f32(be, n, dtype, beta):
+    """weight * advantage / T beyond f32: masked entries stay 0, and so do those
+    whose weight is 0 in 64 bits; the others are rounded from 64-bit products,
+    to infinity where they leave their type. A weight is off by 2^-17 of itself
+    (f32 sums and ex2, as for every uncut row) and below 2^-126 it is 0; half a
+    step of the type on top."""
+    rng = np.random.default_rng(n)
+    v = torch.from_numpy(rng.normal(0, 1.5, (6, n)).astype(np.float32))
+    v[:, ::5] = -np.inf
+    v[:, 1::5] -= 2000.0  # e^-2000 is 0 in 64 bits
+    v[:, 2::10] -= 60.0   # pi about 1e-27: finite gradients
+    v = v.to(TYPES[dtype])
+    likely = v.float()[:, 3::5]
+    act = (likely.argmin(1) * 5 + 3).tolist()  # not the largest: a gradient is left at T = 1e-3
+    temps = [1.0, 0.7, 1.0, 2.0, 1e-3, 0.5]
+    adv, weight = [1e30, -1e25, 3e38, 1e20, -2e36, 1e38], [1e25, 1e30, 4.0, 1e33, 1.0, -1e38]
+    half = {"f32": 2.0 ** -24, "bf16": 2.0 ** -8, "f16": 2.0 ** -11}[dtype]
+    tiny = {"f32": 2.0 ** -149, "bf16": 2.0 ** -133, "f16": 2.0 ** -24}[dtype]
+    most = float(torch.finfo(TYPES[dtype]).max)
+    f = lambda x: float(np.float32(x))  # noqa: E731
+    beta = f(beta)
+    g = policy_loss(be, v, dtype, act, adv, weight, temps, beta)[3].double().numpy()
+    for i in range(6):
+        t = f(temps[i])
+        j, pi, want, size = plain_gradient(v[i], act[i], f(adv[i]), beta, t, f(weight[i]), dtype == "f16")
+        assert not np.isnan(g[i]).any()
+        off = np.ones(n, bool)
+        off[j] = False
+        assert (g[i][off] == 0).all() and (g[i][want == 0] == 0).all()
+        # pi's error: 2^-17 of itself, more by the rounding of x where |x| is large; all of it where the weight is 0
+        x = np.zeros(n)
+        x[j] = np.abs(np.log(np.maximum(pi, 1e-320)))
+        slack = size * (2.0 ** -17 + 2.0 ** -22 * x) + half * 1.001 * np.abs(want)
+        gone = np.zeros(n, bool)
+        gone[j] = pi < 2.0 ** -125
+        sure = (np.abs(want) + slack < most) & ~gone
+        assert (np.abs(g[i] - want)[sure] <= slack[sure] + tiny).all()
+        over = (np.abs(want) - slack > 2 * most) & ~gone
+        assert (g[i][over] == np.copysign(np.inf, want[over])).all()
+        assert over.any() or act[i] not in j
+
+
+@pytest.mark.parametrize("cut", CUTS)
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", LENGTHS)
+def test_masked_entries_have_no_gradient_whatever_the_factors(be, n, dtype, cut):
+    rng = np.random.default_rng(n)
+    v = torch.from_numpy(rng.normal(0, 1.5, (4, n)).astype(np.float32))
+    v[:, 1] = v.amax(1) + 0.5
+    v[:, ::3] = torch.tensor([-np.inf, np.nan, -1e30, np.nan], dtype=torch.float32)[:, None]
+    inf = np.inf
+    g = policy_loss(be, v.to(TYPES[dtype]), dtype, [1] * 4, [np.nan, inf, -inf, 1.0], [1.0, 1.0, 2.0, inf],
+                    cut=cut)[3]
+    assert bool((g[:, ::3] == 0).all())
+    assert not bool(torch.isfinite(g[:, 1]).any())
