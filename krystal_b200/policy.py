@@ -93,8 +93,9 @@ class GradList:
     """The gradients of one global norm: contiguous CUDA tensors of one device,
     where each clipped gradient goes (None: in place), and each one's factor
     in the norm. The list holds its tensors and its workspace; it is built once
-    for gradients that stay where they are. Two captured graphs that may run at
-    once need a list each."""
+    for gradients that stay where they are. The backend holds a list whose clip
+    is still queued. Two captured graphs that may run at once need a list each,
+    and a graph's list has to live as long as the graph."""
 
     def __init__(self, tensors, outs=None, weights=None):
         import torch
