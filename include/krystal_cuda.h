@@ -554,9 +554,10 @@ kc_status kc_policy_loss(kc_handle* h, const kc_rows_view* rows, const kc_sampli
 
 /* The policy kc_backward and kc_backward_batch_device differentiate from the
  * next call on: the targets' policy term becomes (pi - onehot) / temperature
- * over pi's support, nothing for a target that pi does not hold (an AWAY
- * target keeps its own weighting, with pi for p). NULL: the whole softmax at
- * temperature 1, as the reference. Scalar limits only; temperature above 0.
+ * over pi's support, nothing for a target that pi does not hold: cut off,
+ * outside the row, or of a pi that is 0 in f32 (an AWAY target keeps its own
+ * weighting, with pi for p). NULL: the whole softmax at temperature 1, as the
+ * reference (where a target outside the row pushes every entry down). Scalar limits only; temperature above 0.
  * The policy output, the value head and the readings stay those of p. */
 kc_status kc_set_policy(kc_handle* h, const kc_sampling* sampling);
 

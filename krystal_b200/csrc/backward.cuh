@@ -244,7 +244,8 @@ __global__ void __launch_bounds__(256) k_sel_back_scores(SelBackArgs a) {
   const bool away = valid && raw >= 0x80000000u;
   const uint32_t target = away ? raw - 0x80000000u : raw;
   const float* pol = a.pi ? a.pi + po : ps;
-  const bool held = !a.pi || target >= uint32_t(R) || pol[target] > 0.0f;  // a target pi does not hold moves nothing
+  // under a policy, a target that pi does not hold (one outside the row, too) moves nothing
+  const bool held = !a.pi || (target < uint32_t(R) && pol[target] > 0.0f);
   const double p_away = away && target < uint32_t(R) ? double(pol[target]) : 0.0;
   const double sc = away ? p_away / js_max(1.0 - p_away, 1e-6) : 0.0;
   for (int j = tid; j < R; j += 256) {
