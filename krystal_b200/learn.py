@@ -61,7 +61,8 @@ class LearnOptions:
     token_rate: float = 0.1
     # Beyond the reference. sampling: the policy the answers were drawn from
     # (BrainSession.think(sampling=...)), which the update then differentiates;
-    # None: the whole softmax. max_update_norm: the actor's update (selector,
+    # None: the backend's own (set_policy; the whole softmax where none is
+    # set). max_update_norm: the actor's update (selector,
     # pool and table rows, each with its rate) is scaled down to this global
     # norm; the critic keeps its own rate.
     sampling: Sampling | None = None
@@ -331,12 +332,14 @@ class BatchLearner:
         prev_policy = self.be.policy
         self.be.set_stream(run.cuda_stream)
         try:
-            self.be.set_policy(options.sampling)
+            if options.sampling is not None:
+                self.be.set_policy(options.sampling)
             with torch.cuda.stream(run):
                 return self._step(frames, records, rec_off, token_ids, field_roles, schema_ids, band_ids, rewards,
                                   answered, targets, selection, schema_allow, band_allow, options, global_frames)
         finally:
-            self.be.set_policy(prev_policy)
+            if options.sampling is not None:
+                self.be.set_policy(prev_policy)
             self.be.set_stream(prev)
 
     def _step(self, frames, records, rec_off, token_ids, field_roles, schema_ids, band_ids, rewards, answered,
