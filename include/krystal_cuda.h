@@ -525,7 +525,10 @@ kc_status kc_draw(kc_handle* h, uint32_t q, uint32_t r, const float* p, const kc
  * uniforms, [batch questions]) into HOST outputs laid out like that batch's.
  * Refused (KC_ERR_INVALID_ARG) under kc_select_batch's conditions. The draw is
  * exact for the p rows it reads; at KC_PRECISION_CERTIFIED those carry that
- * path's ~1e-6. */
+ * path's ~1e-6 and no frame is recomputed for the draw: it may differ from the
+ * exact path's where a cut or the uniform lies that close to a border. Draws
+ * of the whole distribution match the exact path's if the batch was selected
+ * with the same uniforms, the first largest entry if it was without. */
 kc_status kc_draw_batch(kc_handle* h, const kc_sampling* sampling, const double* uniforms, const kc_draw_out* out);
 
 /* The loss of drawn answers under the policy that drew them, and its gradient

@@ -354,7 +354,9 @@ class CudaBrainBackend:
 
     def draw_batch(self, sampling: Sampling, uniforms=None) -> Draw:
         """kc_draw_batch: the last forward_batch / select_batch batch's
-        distributions drawn under `sampling`, without selecting them again."""
+        distributions drawn under `sampling`, without selecting them again.
+        Exact for the p that batch left on the device: at the certified
+        precision those carry ~1e-6, and no frame is recomputed for a draw."""
         last = getattr(self, "_last_batch_sizes", None)
         if last is None:
             raise RuntimeError("no batch has been run through forward_batch on this backend")
@@ -445,7 +447,12 @@ class CudaBrainBackend:
         sampling: draw each question's answer from its tempered and cut
         distribution (uniforms; without them the first largest entry): "index"
         and "p" are then the draw's and the policy's, with "logp" and "kept"
-        beside them.
+        beside them. At the certified precision (the default) the first largest
+        entry and draws from the whole distribution (Sampling()) match the
+        exact path's; a tempered or cut draw is exact for the p it is taken
+        from, which carry that path's ~1e-6, and may fall otherwise where a
+        cut or the uniform lies that close to a border.
+        set_precision("exact") where it must not.
         word_ids [records*8] / word_alpha: the same-word bias (WordBias).
         mask: an explicit selection mask laid out like p (frame f's [Q_f, R_f]
         block at p_off[f]; NEG_INF blocked, 0 open), for a grammar that is not
@@ -459,8 +466,13 @@ class CudaBrainBackend:
         sa = ba = u = None
         if rule is not None:
             sa, ba = _u32(rule.schema_allow), _u32(rule.band_allow)
-        if uniforms is not None and sampling is None:
+        if uniforms is not None and (sampling is None or sampling.whole):
+            # (with a policy that cuts nothing, too: the certified path's draws are settled in the selection)
             u = np.ascontiguousarray(uniforms, dtype=np.float64)
+            if sampling is not None and hasattr(self, "_last_batch_sizes"):  # (else refused below)
+                self._uniforms(u, self._last_batch_sizes[1])
+            if sampling is not None:
+                self._uniforms(u, int((band == 5).sum()))
         wid = _u32(word_ids) if word_ids is not None else None
         if wid is not None and wid.size != batch.records * 8:
             raise ValueError("word_ids must hold one label per token slot (records * 8)")
@@ -515,7 +527,8 @@ class CudaBrainBackend:
         sa = ba = u = None
         if rule is not None:
             sa, ba = _u32(rule.schema_allow), _u32(rule.band_allow)
-        if uniforms is not None and sampling is None:
+        if uniforms is not None and (sampling is None or sampling.whole):
+            # (with a policy that cuts nothing, too: the certified path's draws are settled in the selection)
             u = np.ascontiguousarray(uniforms, dtype=np.float64)
         m = _f32(mask) if mask is not None else None
         sv = abi.KcBatchSelectView(abi.ptr(sa), abi.ptr(ba), abi.ptr(u), abi.ptr(m))

@@ -39,6 +39,13 @@ class Sampling:
     row_top_p: object = None
     row_min_p: object = None
 
+    @property
+    def whole(self) -> bool:
+        """Whether every row is drawn from its whole distribution, as it is."""
+        rows = (self.row_temperature, self.row_top_k, self.row_top_p, self.row_min_p)
+        return (all(r is None for r in rows) and self.temperature == 1 and self.top_k == 0 and self.top_p >= 1
+                and self.min_p == 0)
+
     def device_struct(self) -> abi.KcSampling:
         return abi.KcSampling(self.temperature, self.top_k, self.top_p, self.min_p, self.row_temperature,
                               self.row_top_k, self.row_top_p, self.row_min_p)
