@@ -486,8 +486,9 @@ typedef struct kc_rows_view {
  * with w_j < exp(-700) are dropped. pi_j = w_j / sum of the kept. Temperature
  * 0 keeps the first largest entry alone. The row_* arrays ([rows] or NULL)
  * replace a limit row by row; there, a temperature that is not above 0 means
- * 0, a NaN top_p or min_p cuts nothing. Weights and their sums are 64-bit, in
- * a fixed order: equal calls give equal bits. */
+ * 0, a NaN top_p or min_p cuts nothing. Weights and their sums are 64-bit (f32
+ * in a kc_policy_loss that cuts nothing), in a fixed order: equal calls give
+ * equal bits. */
 typedef struct kc_sampling {
   float temperature;
   uint32_t top_k;
@@ -536,7 +537,11 @@ kc_status kc_draw_batch(kc_handle* h, const kc_sampling* sampling, const double*
  *   loss = -advantage * log pi(action) - entropy_coef * H(pi)
  *   grad_j = row_weight * (advantage * (pi_j - [j = action])
  *            + entropy_coef * pi_j * (log pi_j + H)) / temperature
- * for kept j, 0 elsewhere, rounded once to the scores' type. A row whose
+ * for kept j, 0 elsewhere, rounded to f32 and then to the scores' type. Where
+ * nothing is cut, weights and sums are f32: pi within 2^-17 of itself, log pi
+ * within 2^-18 and H within 2^-17 (log2 n + 2); where the action holds half of
+ * the mass or more, 1 - pi(action), log pi(action) and H are formed from the
+ * others' weights and lie within 2^-15 of themselves. A row whose
  * action is KC_NO_TARGET, outside the row or not kept, and a row at temperature
  * 0, has loss 0 and gradient 0 (logp: 0 without a target, -infinity for an
  * action the policy cannot take). DEVICE pointers; queued like kc_draw_device. */

@@ -138,6 +138,12 @@ __device__ __forceinline__ float log2_fast(float v) {
   return r;
 }
 
+__device__ __forceinline__ float rcp_fast(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
 __device__ __forceinline__ double warp_add(double v) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -396,6 +402,18 @@ template <> __device__ __forceinline__ void set2<__half>(uint32_t* w, int e, flo
 }
 template <> __device__ __forceinline__ void set2<__nv_bfloat16>(uint32_t* w, int e, float x, float y) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[e / 2]) : "f"(y), "f"(x));
+}
+
+// Entry e of a vector set to x (by masks: an index would move the vector to local memory).
+template <typename T> __device__ __forceinline__ void set_entry(uint32_t* w, uint32_t e, float x) {
+  uint32_t d[2];
+  set2<T>(d, 0, x, x);
+  const uint32_t part = sizeof(T) == 4 ? 0xffffffffu : e & 1 ? 0xffff0000u : 0xffffu;
+#pragma unroll
+  for (uint32_t j = 0; j < 4; j++) {
+    const uint32_t hit = e * uint32_t(sizeof(T)) / 4 == j ? part : 0u;
+    w[j] = (w[j] & ~hit) | (d[0] & hit);
+  }
 }
 
 // The word w with the first (second) entry of x; an f32 word is one entry.

@@ -17,6 +17,10 @@ namespace pol {
 //   2^u_j (u_j B + C) with B = g beta ln 2 / (T Z), C = g (A + beta (H - ln Z)) / (T Z)
 // but for -g A / T more at the action. Sums: four or eight f32 partial sums
 // of at most 18 terms a thread, joined by trees. Arithmetic on pairs (f32x2).
+// The sums are taken without the action's entry (raised to the masks' floor in
+// its place) and its terms added last: with O the others' sum of weights, a
+// confident row's log pi(a) = -log1p(O / w_a) and its gradient's pi - 1 = -O / Z
+// at the action come without cancellation, to the weights' own accuracy.
 //
 // Masked entries need no test where they vanish by themselves: NaN and what
 // lies below the mask's floor is raised to it as the row is loaded, and 2^u is
@@ -97,21 +101,44 @@ struct WholeRow {
   __device__ float u_of(float f) const { return plain ? fmaf(f, sc, off) : (fminf(f, m) - m) * sc; }
 };
 
+// The row's scalars from the others' sums O and S and the action's u (0 weight
+// without one): Z, its logarithm and inverse, log pi(a) and H. Where the action
+// has half of the mass or more both come from terms that do not cancel,
+// H = -pi_a log pi_a - ln 2 (S - O log2 Z) / Z.
+struct WholeSums {
+  float others, w, lg_z, inv_z, logp, h;
+  __device__ __forceinline__ float z() const { return others + w; }
+  __device__ __forceinline__ WholeSums(float2 zs, float ua, bool apart, bool any, bool open_t) {
+    constexpr float kLn2 = 0.69314718055994530942f;
+    others = zs.x;
+    ua = fmaxf(ua, -2000.0f);
+    w = apart ? exp2_fast(ua) : 0.0f;
+    lg_z = any ? log2f(z()) : 0.0f;
+    inv_z = any ? rcp_fast(z()) : 0.0f;
+    logp = open_t ? kLn2 * (ua - lg_z) : 0.0f;
+    h = any && open_t ? kLn2 * (lg_z - fmaf(w, ua, zs.y) * inv_z) : 0.0f;
+    if (apart && others <= w) {
+      logp = -log1pf(others * rcp_fast(w));
+      h = fmaf(kLn2 * inv_z, fmaf(others, lg_z, -zs.y), -w * inv_z * logp);
+    }
+  }
+};
+
 // log2(e) / T; a T below 5e-39 keeps it finite, so that the largest entry's u is 0.
 __device__ __forceinline__ float scale_of(float t) { return fminf(1.44269504088896340736f / t, 3.402823466e38f); }
 
 // The gradient entry by entry in 64 bits: where a factor of the quick form
-// could overflow before the product does, and at the action, where pi - 1 is
-// the row's largest gradient.
+// could overflow before the product does, and at the action.
 struct WholeSlope {
-  float rw, t, z, lg_z, h, adv, beta;
+  float rw, t, adv, beta;
+  const WholeSums& s;
   __device__ __forceinline__ float of(float u) const {
-    const double w = double(exp2_fast(u)), e = 0.69314718055994530942 * (double(u) - double(lg_z)) + double(h);
-    return float(double(rw) / double(t) * (w / double(z) * fma(double(beta), e, double(adv))));
+    const double w = double(exp2_fast(u)), e = 0.69314718055994530942 * (double(u) - double(s.lg_z)) + double(s.h);
+    return float(double(rw) / double(t) * (w / double(s.z()) * fma(double(beta), e, double(adv))));
   }
-  __device__ __forceinline__ float of_action(float u, float logp) const {
-    const double pi = double(exp2_fast(u)) / double(z);
-    return float(double(rw) / double(t) * fma(double(adv), pi - 1.0, double(beta) * pi * (double(logp) + h)));
+  __device__ __forceinline__ float of_action() const {
+    const double w = double(s.w), o = double(s.others);
+    return float(double(rw) * (double(beta) * w * (double(s.logp) + double(s.h)) - double(adv) * o) / (double(t) * (o + w)));
   }
 };
 
@@ -131,6 +158,7 @@ __global__ void __launch_bounds__(128) k_policy_whole(LossArg a) {
   const int shift = int((reinterpret_cast<uintptr_t>(in) & 15) / sizeof(T));
   const int i0 = lane * V - shift;
   constexpr float floor_v = Floor<T>::value;
+  const uint32_t act = a.actions[row];
 
   // the row, masked entries raised to the floor; its largest
   uint32_t v[NV][4];
@@ -152,8 +180,13 @@ __global__ void __launch_bounds__(128) k_policy_whole(LossArg a) {
 #pragma unroll
   for (int c = 0; c < NV; c++) highest.raise(v[c]);
   const float mx = highest.value();
+  // the action is summed apart
+#pragma unroll
+  for (int c = 0; c < NV; c++) {
+    const uint32_t e = act - uint32_t(i0 + c * 32 * V);
+    if (e < uint32_t(V)) set_entry<T>(v[c], e, floor_v);
+  }
   // the action's value, before anything is written: grad may lie over values
-  const uint32_t act = a.actions[row];
   const bool asked = act != kNone;
   const float va = act < uint32_t(n) ? as_f32(in[act]) : floor_v;
   constexpr float kLn2 = 0.69314718055994530942f, kMost = 3.402823466e38f;
@@ -166,8 +199,7 @@ __global__ void __launch_bounds__(128) k_policy_whole(LossArg a) {
   const bool plain = !endless && (m - Lowest<T>::open_above) * sc >= 200.0f && fabsf(m * sc) < 1e5f && sc < 1e6f;
   const float off = -m * sc;
   const WholeRow row_of{sc, off, m, plain};
-
-  // Z and S
+  // Z and S of the others
   float2 zs = make_float2(0.0f, 0.0f);
   if (plain) {
     const unsigned long long sc2 = pack2(sc, sc), off2 = pack2(off, off);
@@ -209,9 +241,10 @@ __global__ void __launch_bounds__(128) k_policy_whole(LossArg a) {
 
   // the row's answer
   const float ua = row_of.u_of(fminf(va, kMost));
+  const WholeSums sums(zs, ua, va > Lowest<T>::open_above, any, open_t);
   bool live = asked && va > Lowest<T>::open_above && ua * kLn2 >= float(kDropped);
   if (!open_t) {  // temperature 0: the first largest entry alone
-    uint32_t first = 0xffffffffu;
+    uint32_t first = va > Lowest<T>::open_above && fminf(va, kMost) == m ? act : 0xffffffffu;
 #pragma unroll
     for (int c = 0; c < NV; c++)
 #pragma unroll
@@ -221,9 +254,7 @@ __global__ void __launch_bounds__(128) k_policy_whole(LossArg a) {
     g.counts(none, first, zero);
     live = asked && any && first == act;
   }
-  const float lg_z = any ? log2f(zs.x) : 0.0f, inv_z = any ? 1.0f / zs.x : 0.0f;
-  const float h = any && open_t ? kLn2 * (lg_z - zs.y * inv_z) : 0.0f;
-  const float logp = open_t ? kLn2 * (ua - lg_z) : 0.0f;
+  const float lg_z = sums.lg_z, inv_z = sums.inv_z, h = sums.h, logp = sums.logp;
   const bool learns = asked && live && open_t;
   const float adv = a.advantage[row], beta = a.beta;
   if (lane == 0) {
@@ -233,8 +264,9 @@ __global__ void __launch_bounds__(128) k_policy_whole(LossArg a) {
   }
   if (!a.grad || !fits) return;
   T* out = static_cast<T*>(a.grad) + at.out;
-  const float rw = a.row_weight ? a.row_weight[row] : 1.0f, gt = learns ? rw / t_row : 0.0f, over = gt * inv_z;
-  const WholeSlope slope{rw, t_row, zs.x, lg_z, h, adv, beta};
+  const float rw = a.row_weight ? a.row_weight[row] : 1.0f;
+  const float over = learns ? rw * (kLn2 * sc) * inv_z : 0.0f;  // rw / (T Z), for the quick form alone
+  const WholeSlope slope{rw, t_row, adv, beta, sums};
   const float B = over * beta * kLn2, C = learns ? over * fmaf(beta, h - kLn2 * lg_z, adv) : 0.0f;  // (adv may be NaN)
   const bool quick = plain && fabsf(B) < 10.0f && fabsf(C) < 1e30f;  // (a vanished weight times infinity)
   RowWriter<T> writer(out, n, lane, i0);
@@ -263,7 +295,7 @@ __global__ void __launch_bounds__(128) k_policy_whole(LossArg a) {
     }
     // the action's entry, and its lane's alone, gets the rest
     if (learns && act - uint32_t(i) < uint32_t(V)) {
-      const float x = slope.of_action(ua, logp);
+      const float x = slope.of_action();
 #pragma unroll
       for (int e = 0; e < V; e += 2) {
         uint32_t w[4];
@@ -316,6 +348,7 @@ __global__ void __launch_bounds__(NT) k_policy_long(LossArg a, uint32_t seg_vecs
   // one more is loaded where another CTA's segment follows
   const int mine = max(0, min(int(seg_vecs), vecs - v0)), have = max(0, min(int(seg_vecs) + 1, vecs - v0));
   const int i0 = v0 * V - shift;
+  const uint32_t act = a.actions[row];
 
   // the row, by asynchronous copies that are all in flight at once
   for (int j = tid; j < have; j += NT) {
@@ -343,8 +376,15 @@ __global__ void __launch_bounds__(NT) k_policy_long(LossArg a, uint32_t seg_vecs
     sm[j] = make_uint4(w[0], w[1], w[2], w[3]);
   }
   const float mx = highest.value();
+  // the action is summed apart
+  const int at_act = act < uint32_t(n) ? int(act) - i0 : -1;
+  if (at_act >= 0 && at_act < mine * V && at_act / V % NT == tid) {
+    const uint4 q = sm[at_act / V];
+    uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    set_entry<T>(w, uint32_t(at_act % V), floor_v);
+    sm[at_act / V] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
   // the action's value, before anything is written: grad may lie over values
-  const uint32_t act = a.actions[row];
   const bool asked = act != kNone;
   const float va = act < uint32_t(n) ? as_f32(in[act]) : floor_v;
   const uint32_t top = g.largest(key_of(fmaxf(mx, floor_v)));
@@ -357,7 +397,7 @@ __global__ void __launch_bounds__(NT) k_policy_long(LossArg a, uint32_t seg_vecs
   const WholeRow wr{sc, -m * sc, m, plain};
   const unsigned long long sc2 = pack2(sc, sc), off2 = pack2(wr.off, wr.off);
 
-  // Z and S
+  // Z and S of the others
   float2 zs = make_float2(0.0f, 0.0f);
   if (plain) {
     unsigned long long za[4] = {0ull, 0ull, 0ull, 0ull}, sa[4] = {0ull, 0ull, 0ull, 0ull};
@@ -398,9 +438,10 @@ __global__ void __launch_bounds__(NT) k_policy_long(LossArg a, uint32_t seg_vecs
 
   // the row's answer
   const float ua = wr.u_of(fminf(va, kMost));
+  const WholeSums sums(zs, ua, va > Lowest<T>::open_above, any, open_t);
   bool live = asked && va > Lowest<T>::open_above && ua * kLn2 >= float(kDropped);
   if (!open_t) {  // temperature 0: the first largest entry alone
-    uint32_t first = 0xffffffffu, zero = 0, none = 0;
+    uint32_t first = va > Lowest<T>::open_above && fminf(va, kMost) == m ? act : 0xffffffffu, zero = 0, none = 0;
     for (int j = tid; j < mine; j += NT) {
       const uint4 q = sm[j];
       const uint32_t w[4] = {q.x, q.y, q.z, q.w};
@@ -411,9 +452,7 @@ __global__ void __launch_bounds__(NT) k_policy_long(LossArg a, uint32_t seg_vecs
     g.counts(none, first, zero);
     live = asked && any && first == act;
   }
-  const float lg_z = any ? log2f(zs.x) : 0.0f, inv_z = any ? 1.0f / zs.x : 0.0f;
-  const float h = any && open_t ? kLn2 * (lg_z - zs.y * inv_z) : 0.0f;
-  const float logp = open_t ? kLn2 * (ua - lg_z) : 0.0f;
+  const float lg_z = sums.lg_z, inv_z = sums.inv_z, h = sums.h, logp = sums.logp;
   const bool learns = asked && live && open_t;
   const float adv = a.advantage[row], beta = a.beta;
   if (g.rank == 0 && tid == 0) {
@@ -423,8 +462,9 @@ __global__ void __launch_bounds__(NT) k_policy_long(LossArg a, uint32_t seg_vecs
   }
   if (!a.grad || !fits) return;
   T* out = static_cast<T*>(a.grad) + at.out;
-  const float rw = a.row_weight ? a.row_weight[row] : 1.0f, gt = learns ? rw / t_row : 0.0f, over = gt * inv_z;
-  const WholeSlope slope{rw, t_row, zs.x, lg_z, h, adv, beta};
+  const float rw = a.row_weight ? a.row_weight[row] : 1.0f;
+  const float over = learns ? rw * (kLn2 * sc) * inv_z : 0.0f;  // rw / (T Z), for the quick form alone
+  const WholeSlope slope{rw, t_row, adv, beta, sums};
   const float B = over * beta * kLn2, C = learns ? over * fmaf(beta, h - kLn2 * lg_z, adv) : 0.0f;  // (adv may be NaN)
   const bool quick = plain && fabsf(B) < 10.0f && fabsf(C) < 1e30f;  // (a vanished weight times infinity)
   const unsigned long long B2 = pack2(B, B), C2 = pack2(C, C);
@@ -485,7 +525,7 @@ __global__ void __launch_bounds__(NT) k_policy_long(LossArg a, uint32_t seg_vecs
   if (learns) {
     const int to_act = int(act) - i0 - skew + V, j = to_act / V - 1;
     if (to_act >= 0 && j >= -ahead && j < mine && (j + ahead) % NT == tid)
-      out[act] = from_f32<T>(slope.of_action(ua, logp));
+      out[act] = from_f32<T>(slope.of_action());
   }
 }
 

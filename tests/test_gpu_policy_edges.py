@@ -1,5 +1,6 @@
 """The policy loss where factors are not finite or leave f32: rows that must
-have no gradient, masked entries, and gradients whose factors overflow."""
+have no gradient, masked entries, and gradients whose factors overflow; and
+confident rows, where pi - 1 and log pi are small."""
 import numpy as np
 import pytest
 
@@ -150,3 +151,45 @@ def test_masked_entries_have_no_gradient_whatever_the_factors(be, n, dtype, cut)
                     cut=cut)[3]
     assert bool((g[:, ::3] == 0).all())
     assert not bool(torch.isfinite(g[:, 1]).any())
+
+
+@pytest.mark.parametrize("dtype,at", [("f32", 0.0), ("f16", 0.0), ("bf16", 0.0), ("f32", 1e6)])
+@pytest.mark.parametrize("n", LENGTHS)
+def test_confident_rows_keep_their_small_gradient(be, n, dtype, at):
+    """The action holds all but 1e-3 to 1e-12 of the mass. Its gradient, the loss
+    and the entropy are as exact as the others' weights: an f32 exponent x is
+    off by 2^-23 |x| (log2(e) / T in f32) and its own rounding, |x| <= 35, the
+    weight by ex2's 2^-22 and the sum's 18 terms: below 2^-16 of each, which
+    makes 2^-15 of what is made of them; half a step of the type on top. At 1e6
+    (f32) the largest score is subtracted first."""
+    rng = np.random.default_rng(n)
+    gap = np.array([8.0, 14.0, 20.0, 30.0]) + np.log(n)
+    v = np.round(rng.uniform(-2, 0, (4, n)) - gap[:, None], 0 if at else 3)  # (f32 steps of 1e6 are 2^-4)
+    act = [n - 1, 0, n // 2, n // 3]
+    v[np.arange(4), act] = 0.0
+    v[:, 7 % n] = -np.inf if 7 not in act else v[:, 7]
+    v = torch.from_numpy((v + at).astype(np.float32)).to(TYPES[dtype])
+    adv, weight = [1.0, -0.7, 2.0, 1.5], [1.0, 1.0, 3.0, 0.25]
+    half = {"f32": 2.0 ** -24, "bf16": 2.0 ** -8, "f16": 2.0 ** -11}[dtype]
+    tiny = {"f32": 2.0 ** -149, "bf16": 2.0 ** -133, "f16": 2.0 ** -24}[dtype]
+    for beta in (0.0, 0.125):
+        lo, lp, h, g = policy_loss(be, v, dtype, act, adv, weight, beta=beta)
+        g = g.double().numpy()
+        for i in range(4):
+            x = v[i].double().numpy() - float(v[i, act[i]])
+            keep = np.isfinite(x)
+            w = np.where(keep, np.exp(np.where(keep, x, 0.0)), 0.0)
+            others = w.sum() - 1.0 if w.sum() > 1.1 else np.delete(w, act[i]).sum()
+            z = 1.0 + others
+            logp = -np.log1p(others)
+            ent = -logp / z - (np.where(keep, w * (np.where(keep, x, 0.0) + logp), 0.0).sum() - logp) / z
+            a = act[i]
+            want = weight[i] * (-adv[i] * others / z + beta / z * (logp + ent))
+            size = weight[i] * (abs(adv[i]) * others / z + beta / z * (abs(logp) + ent))
+            assert 0 < others < 1e-3
+            assert abs(g[i, a] - want) <= 2.0 ** -15 * size + 1.001 * half * abs(want) + tiny
+            assert abs(lp[i] - logp) <= 2.0 ** -15 * abs(logp)
+            assert abs(h[i] - ent) <= 2.0 ** -15 * ent
+            assert abs(lo[i] - (-adv[i] * logp - beta * ent)) <= 2.0 ** -15 * (abs(adv[i] * logp) + beta * ent)
+            if dtype == "f32" and not beta:  # pi - 1 and the other pi sum to nothing
+                assert abs(g[i].sum()) <= 2.0 ** -14 * abs(want)
