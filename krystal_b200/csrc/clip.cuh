@@ -179,12 +179,13 @@ __global__ void __launch_bounds__(kThreads) k_norm(const __grid_constant__ Table
 
 template <uint32_t N>
 __global__ void __launch_bounds__(kThreads) k_scale(const __grid_constant__ Table<N> tb,
-                                                    const double* __restrict__ partial, uint32_t partials,
+                                                    const double* partial, uint32_t partials,
                                                     double max_norm, double* __restrict__ result, int first) {
   __shared__ double red[kThreads / 32];
   cudaGridDependencySynchronize();  // k_norm has ended and its partial sums are here
   double sum = 0.0;
-  for (uint32_t i = threadIdx.x; i < partials; i += kThreads) sum += partial[i];
+  // (written while this kernel runs, so neither read-only data nor read ahead of the wait: from L2)
+  for (uint32_t i = threadIdx.x; i < partials; i += kThreads) sum += __ldcg(partial + i);
   const double norm = sqrt(cta_sum(sum, red));
   const bool cut = norm > max_norm && norm <= 1.7976931348623157e308;
   const double scale = cut ? max_norm / norm : 1.0;
