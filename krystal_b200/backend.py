@@ -18,6 +18,7 @@ one call) and ``backward_batch_device`` (the backward of a whole batch).
 """
 from __future__ import annotations
 
+import collections
 import ctypes as C
 import threading
 from dataclasses import dataclass, field
@@ -154,8 +155,8 @@ class CudaBrainBackend:
         abi.check(self._lib.kc_create(C.byref(cfg), C.byref(views.view), device, C.byref(h)))
         self._h = h
         self.policy: Sampling | None = None  # what the backward differentiates (set_policy)
-        self._clip: GradList | None = None   # the list clipped last
-        self._clips_queued: list = []        # earlier ones: (list, event behind its last clip, or None)
+        self._clips_dropped = collections.deque()  # what dropped lists held that the stream may not have passed,
+        self._clips_queued: list = []              # and behind an event
         self._clip_lock = threading.Lock()
 
     # --- BrainBackend -----------------------------------------------------
@@ -191,7 +192,8 @@ class CudaBrainBackend:
         if getattr(self, "_h", None):
             self._lib.kc_destroy(self._h)  # waits for the stream
             self._h = None
-            self._clip, self._clips_queued = None, []
+            self._clips_dropped.clear()
+            self._clips_queued = []
 
     def backward(self, frame: HostFrame, selection=None, targets=None,
                  valence_target: float | None = None) -> BackwardResult:
@@ -398,45 +400,43 @@ class CudaBrainBackend:
 
     def clip_grads(self, grads: GradList, max_norm: float, result: int) -> None:
         """kc_clip_grads: the list's global norm, and its gradients scaled to
-        max_norm; result: a device pointer to two f64, norm and scale. The
-        call is queued: the backend holds the list, its gradients and its
-        workspace until the stream has passed it (the list clipped last until
-        another one follows, synchronize or destroy). A captured clip's list is
+        max_norm; result: a device pointer to two f64, norm and scale. The call
+        is queued: when the list is dropped, the backend holds its gradients and
+        its workspace until the stream has passed it (and lets go of them in
+        later calls, in synchronize and in destroy). A captured clip's list is
         the caller's to hold for as long as its graph."""
         if grads.device.index != self.device:
             raise ValueError(f"the gradients lie on {grads.device}, the backend on cuda:{self.device}")
+        grads.queued_on(self)
         abi.check(self._lib.kc_clip_grads(self._h, grads.address, grads.count, max_norm, grads.workspace.data_ptr(),
                                           grads.workspace_bytes, result), self._h)
-        if grads is not self._clip:
-            self._hold_clip(grads)
+        if self._clips_dropped or self._clips_queued:
+            self._release_clips()
 
-    def _hold_clip(self, grads: GradList | None) -> None:
-        """Holds `grads` in the place of the list clipped last, and lets go of the
-        lists whose event has passed. The event is recorded now, behind the
-        former list's last clip (a stream that the handle was moved to waits
-        for the one it left). Nothing is recorded or asked while a graph is
-        captured, where neither is allowed."""
+    def hold_clip(self, parts) -> None:
+        """Takes what a dropped list held (GradList.__del__; no CUDA call: it may
+        run anywhere, in a capture too)."""
+        if self._h:
+            self._clips_dropped.append(parts)
+
+    def _release_clips(self) -> None:
+        """Lets go of the dropped lists whose event has passed. The event is
+        recorded here, behind the list's last clip (a stream that the handle was
+        moved to waits for the one it left). Nothing is recorded or asked while
+        a graph is captured, where neither is allowed."""
+        import torch
         with self._clip_lock:
-            if self._clip is not None:
-                self._clips_queued.append((self._clip, None))
-            self._clip = grads
-            if not self._clips_queued:
-                return
-            import torch
             stream = torch.cuda.ExternalStream(self.stream_ptr(), device=self.device)
             if torch.cuda.is_current_stream_capturing():
                 return
             with torch.cuda.stream(stream):
                 if torch.cuda.is_current_stream_capturing():
                     return
-            waits = []
-            for held, event in self._clips_queued:
-                if event is None:
-                    event = torch.cuda.Event()
-                    event.record(stream)
-                if not event.query():
-                    waits.append((held, event))
-            self._clips_queued = waits
+            while self._clips_dropped:
+                event = torch.cuda.Event()
+                self._clips_queued.append((self._clips_dropped.popleft(), event))
+                event.record(stream)
+            self._clips_queued = [c for c in self._clips_queued if not c[1].query()]
 
     # --- packed ragged batches ------------------------------------------------
     def forward_batch(self, batch: FrameBatch, rule: MaskRule | None = None, uniforms=None,
@@ -569,8 +569,8 @@ class CudaBrainBackend:
 
     def synchronize(self) -> None:
         abi.check(self._lib.kc_synchronize(self._h), self._h)
-        if self._clip is not None or self._clips_queued:
-            self._hold_clip(None)
+        if self._clips_dropped or self._clips_queued:
+            self._release_clips()
 
     def set_precision(self, mode: int | str, tau: float = 0.0) -> None:
         """KC_PRECISION_EXACT / CERTIFIED (default) / FAST for the batch entry points."""

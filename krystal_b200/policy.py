@@ -14,6 +14,7 @@ device entry points do.
 from __future__ import annotations
 
 import ctypes as C
+import weakref
 from dataclasses import dataclass
 
 import numpy as np
@@ -100,8 +101,8 @@ class GradList:
     """The gradients of one global norm: contiguous CUDA tensors of one device,
     where each clipped gradient goes (None: in place), and each one's factor
     in the norm. The list holds its tensors and its workspace; it is built once
-    for gradients that stay where they are. The backend holds a list whose clip
-    is still queued. Two captured graphs that may run at once need a list each,
+    for gradients that stay where they are. A list dropped while its clip is
+    queued leaves both with the backend until the stream has passed them. Two captured graphs that may run at once need a list each,
     and a graph's list has to live as long as the graph."""
 
     def __init__(self, tensors, outs=None, weights=None):
@@ -132,3 +133,14 @@ class GradList:
         self.workspace_bytes = int(abi.load().kc_clip_workspace(self.count))
         self.workspace = torch.empty(self.workspace_bytes // 8, dtype=torch.float64, device=self.device)
         self.address = C.addressof(self.views)
+        self.backends = []  # weak references to those that queued a clip of the list
+
+    def queued_on(self, backend) -> None:
+        if not any(r() is backend for r in self.backends):
+            self.backends.append(weakref.ref(backend))
+
+    def __del__(self):
+        for r in getattr(self, "backends", ()):
+            backend = r()
+            if backend is not None:
+                backend.hold_clip((self.keep, self.workspace))

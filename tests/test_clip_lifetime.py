@@ -21,12 +21,12 @@ class Buffer:
         return 64
 
 
-class List:
-    """What clip_grads reads of a GradList."""
-    device, address, count, workspace_bytes = torch.device("cuda", 0), 64, 1, 64
-
-    def __init__(self):
-        self.workspace = Buffer()
+def grad_list():
+    """A list without a device: its workspace is what has to live."""
+    grads = GradList.__new__(GradList)
+    grads.device, grads.address, grads.count, grads.workspace_bytes = torch.device("cuda", 0), 64, 1, 64
+    grads.workspace, grads.keep, grads.backends = Buffer(), (), []
+    return grads
 
 
 class Device:
@@ -68,8 +68,8 @@ def be(monkeypatch):
 
 
 def clip_a_temporary(be):
-    grads = List()
-    dead = weakref.ref(grads)
+    grads = grad_list()
+    dead = weakref.ref(grads.workspace)
     be.clip_grads(grads, 1.0, 64)
     del grads
     gc.collect()
@@ -83,7 +83,7 @@ def test_a_temporary_list_outlives_its_call(be, monkeypatch):
     second = clip_a_temporary(be)  # nothing has passed yet
     assert first() is not None and second() is not None
     dev.passed = dev.recorded
-    third = clip_a_temporary(be)
+    third = clip_a_temporary(be)  # the first one's event was recorded in the second's call
     assert first() is None and second() is not None and third() is not None
     dev.passed = 10 ** 6
     be.synchronize()
@@ -98,11 +98,11 @@ def test_destroy_lets_go_of_every_list(be, monkeypatch):
     assert all(x() is None for x in lists)
 
 
-def test_a_list_used_again_costs_no_event(be, monkeypatch):
+def test_lists_used_again_cost_no_event(be, monkeypatch):
     dev = Device(monkeypatch)
-    grads = List()
-    for _ in range(5):
-        be.clip_grads(grads, 1.0, 64)
+    lists = [grad_list(), grad_list()]
+    for i in range(6):
+        be.clip_grads(lists[i % 2], 1.0, 64)
     assert dev.recorded == 0 and dev.asked == 0
 
 
@@ -110,13 +110,23 @@ def test_no_event_is_touched_while_a_graph_is_captured(be, monkeypatch):
     dev = Device(monkeypatch)
     before = clip_a_temporary(be)
     dev.capturing = True
-    held = [List(), List()]
+    held = [grad_list(), grad_list()]
     for x in held:
         be.clip_grads(x, 1.0, 64)
-    assert before() is not None
+    assert before() is not None and dev.recorded == 0
     dev.capturing, dev.passed = False, 10 ** 6
     be.clip_grads(held[0], 1.0, 64)
     assert before() is None
+
+
+def test_a_list_outlives_none_of_its_backends(be, monkeypatch):
+    Device(monkeypatch)
+    grads = grad_list()
+    dead = weakref.ref(grads.workspace)
+    be.clip_grads(grads, 1.0, 64)
+    be.destroy()  # has waited for the stream
+    del grads
+    assert dead() is None
 
 
 @pytest.mark.gpu
