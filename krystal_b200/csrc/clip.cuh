@@ -7,7 +7,9 @@
 // multiplies in 64 bits.
 //
 // Two launches: k_norm leaves one partial sum a CTA, k_scale adds the partial
-// sums again in every CTA (a few KB from L2) and scales. All sums are 64-bit
+// sums again in every CTA (a few KB from L2) and scales. Lists of more tensors
+// than a launch's table holds take several of each, and one CTA (k_join) adds
+// the partial sums of them all once. All sums are 64-bit
 // and in an order that the sizes alone decide; there are no atomics. The work
 // is cut into chunks of one tensor, 8 to 128 KB so that about one falls to each
 // CTA of a small list and a large one pays for few searches of its table; CTA b
@@ -177,22 +179,48 @@ __global__ void __launch_bounds__(kThreads) k_norm(const __grid_constant__ Table
   if (threadIdx.x == 0) partial[blockIdx.x] = sum;
 }
 
-template <uint32_t N>
-__global__ void __launch_bounds__(kThreads) k_scale(const __grid_constant__ Table<N> tb,
-                                                    const double* partial, uint32_t partials,
-                                                    double max_norm, double* __restrict__ result, int first) {
-  __shared__ double red[kThreads / 32];
-  cudaGridDependencySynchronize();  // k_norm has ended and its partial sums are here
+// Every thread of the CTA adds the partial sums and gets norm and scale.
+struct Clip {
+  double norm, scale;
+};
+__device__ __forceinline__ Clip join(const double* partial, uint32_t partials, double max_norm, double* red) {
   double sum = 0.0;
-  // (written while this kernel runs, so neither read-only data nor read ahead of the wait: from L2)
+  // (written while k_scale runs, so neither read-only data nor read ahead of its wait: from L2)
   for (uint32_t i = threadIdx.x; i < partials; i += kThreads) sum += __ldcg(partial + i);
   const double norm = sqrt(cta_sum(sum, red));
-  const bool cut = norm > max_norm && norm <= 1.7976931348623157e308;
-  const double scale = cut ? max_norm / norm : 1.0;
-  if (first && blockIdx.x == 0 && threadIdx.x == 0) {
-    result[0] = norm;
-    result[1] = scale;
+  return Clip{norm, norm > max_norm && norm <= 1.7976931348623157e308 ? max_norm / norm : 1.0};
+}
+
+// The norm and scale of a list of several launches, whose scaling launches
+// would otherwise add up all of the list's partial sums in each of their CTAs.
+static __global__ void __launch_bounds__(kThreads) k_join(const double* partial, uint32_t partials, double max_norm,
+                                                          double* __restrict__ result) {
+  __shared__ double red[kThreads / 32];
+  const Clip c = join(partial, partials, max_norm, red);
+  if (threadIdx.x == 0) {
+    result[0] = c.norm;
+    result[1] = c.scale;
   }
+}
+
+// partials 0: k_join has written the result.
+template <uint32_t N>
+__global__ void __launch_bounds__(kThreads) k_scale(const __grid_constant__ Table<N> tb, const double* partial,
+                                                    uint32_t partials, double max_norm, double* result) {
+  __shared__ double red[kThreads / 32];
+  double scale;
+  if (partials) {
+    cudaGridDependencySynchronize();  // k_norm has ended and its partial sums are here
+    const Clip c = join(partial, partials, max_norm, red);
+    scale = c.scale;
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+      result[0] = c.norm;
+      result[1] = scale;
+    }
+  } else {
+    scale = result[1];
+  }
+  const bool cut = scale != 1.0;
   for (uint32_t r = blockIdx.x; r < tb.chunks; r += gridDim.x) {
     const Piece p = piece_of(tb, tb.chunks - 1 - r);
     if (!p.t->out || (!cut && p.t->out == p.t->in)) continue;

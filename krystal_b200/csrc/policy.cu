@@ -53,10 +53,11 @@ cudaError_t run(Tensor* t, uint64_t count, double max_norm, double* workspace, d
                 cudaStream_t stream, uint64_t* launches) {
   const uint32_t most = std::min<uint32_t>(kMaxCtas, uint32_t(sms) * 4);
   static thread_local Table<N> tb;
+  const bool one = count <= N;
   uint32_t partials = 0;
   for (int pass = 0; pass < 2; pass++) {
-    bool first = true;
-    for (uint64_t at = 0; at < count || first; at += N) {
+    uint64_t at = 0;
+    do {
       const uint32_t chunks = fill(tb, t + at, uint32_t(std::min<uint64_t>(N, count - at)), most);
       const unsigned grid = std::max(1u, std::min(most, chunks));
       if (pass == 0) {
@@ -71,13 +72,17 @@ cudaError_t run(Tensor* t, uint64_t count, double max_norm, double* workspace, d
         early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         early[0].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = early;
-        cfg.numAttrs = first && at + N >= count ? 1 : 0;  // one launch of each: the one ahead is k_norm's
-        const cudaError_t e = cudaLaunchKernelEx(&cfg, k_scale<N>, tb, static_cast<const double*>(workspace), partials,
-                                                 max_norm, result, first ? 1 : 0);
+        cfg.numAttrs = one ? 1 : 0;  // the launch ahead is k_norm's
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, k_scale<N>, tb, static_cast<const double*>(workspace),
+                                                 one ? partials : 0u, max_norm, result);
         if (e) return e;
       }
       ++*launches;
-      first = false;
+      at += N;
+    } while (at < count);
+    if (pass == 0 && !one) {
+      k_join<<<1, kThreads, 0, stream>>>(workspace, partials, max_norm, result);
+      ++*launches;
     }
   }
   return cudaGetLastError();
