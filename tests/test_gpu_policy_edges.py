@@ -7,6 +7,7 @@ import pytest
 from krystal_b200 import policy
 from krystal_b200.backend import CudaBrainBackend
 from krystal_b200.model import BRAIN_FORWARD_CONFIG, create_brain_forward_weights
+from tests.test_gpu_policy import scores, whole_loss
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -193,3 +194,16 @@ def test_confident_rows_keep_their_small_gradient(be, n, dtype, at):
             assert abs(lo[i] - (-adv[i] * logp - beta * ent)) <= 2.0 ** -15 * (abs(adv[i] * logp) + beta * ent)
             if dtype == "f32" and not beta:  # pi - 1 and the other pi sum to nothing
                 assert abs(g[i].sum()) <= 2.0 ** -14 * abs(want)
+
+
+@pytest.mark.parametrize("dtype,n", [("f32", 17000), ("f32", 18400), ("bf16", 34000), ("bf16", 36800), ("f16", 36801)])
+def test_rows_whose_threads_add_eighteen_terms(be, dtype, n):
+    """The longest partial sums: 17 and 18 terms a thread, off by 18 2^-24. With
+    ex2's 2^-22 and 0.7 2^-24 log2 n of the exponents' rounding (log2 n <= 15.2)
+    Z is within 2^-18.9 of itself, below the 2^-18 that whole_loss allows of
+    log Z."""
+    rng = np.random.default_rng(n)
+    v = scores(rng, 4, n, dtype, 0.05)
+    act = [int(np.argmax(np.nan_to_num(r.double().numpy(), nan=-1e300, neginf=-1e300))) for r in v]
+    act[1] = int(np.flatnonzero(v[1].double().numpy() > -1e4)[n // 2])
+    whole_loss(be, v, dtype, act, rng.normal(size=4), 0.1, [1.0, 0.8, 5.0, 30.0])
