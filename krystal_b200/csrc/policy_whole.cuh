@@ -111,7 +111,7 @@ struct WholeSums {
   __device__ __forceinline__ WholeSums(float2 zs, float ua, bool apart, bool any, bool open_t) {
     constexpr float kLn2 = 0.69314718055994530942f;
     others = zs.x;
-    ua = fmaxf(ua, -2000.0f);
+    ua = apart ? fmaxf(ua, -2000.0f) : 0.0f;  // (a masked action's u is anything)
     w = apart ? exp2_fast(ua) : 0.0f;
     lg_z = any ? log2f(z()) : 0.0f;
     inv_z = any ? rcp_fast(z()) : 0.0f;

@@ -207,3 +207,28 @@ def test_rows_whose_threads_add_eighteen_terms(be, dtype, n):
     act = [int(np.argmax(np.nan_to_num(r.double().numpy(), nan=-1e300, neginf=-1e300))) for r in v]
     act[1] = int(np.flatnonzero(v[1].double().numpy() > -1e4)[n // 2])
     whole_loss(be, v, dtype, act, rng.normal(size=4), 0.1, [1.0, 0.8, 5.0, 30.0])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", LENGTHS)
+def test_the_entropy_of_rows_whose_action_is_masked(be, n, dtype):
+    """Every sort of mask under the action, and an action outside the row: H is
+    the row's, within 2^-17 (log2 n + 2) as for every uncut row."""
+    rng = np.random.default_rng(n)
+    masks = [np.nan, -np.inf, -1e30, float(np.finfo(np.float32).min), np.nan, np.nan]
+    v = torch.from_numpy(rng.normal(0, 1.5, (6, n)).astype(np.float32))
+    act = [1, 5, n - 2, n // 2, n + 3, -1]
+    for i, a in enumerate(act):
+        if 0 <= a < n:
+            v[i, a] = masks[i]
+    v = v.to(TYPES[dtype])
+    temps = [1.0, 0.5, 2.0, 1.0, 1.0, 1e-3]
+    lo, lp, h, g = policy_loss(be, v, dtype, act, [1.0] * 6, [1.0] * 6, temps)
+    assert (lo == 0).all() and bool((g == 0).all()) and (lp == [-np.inf] * 5 + [0.0]).all()
+    for i in range(6):
+        x = v[i].double().numpy()
+        x = x[x > (-65504.0 if dtype == "f16" else -1e29)]
+        x = (x - x.max()) / float(np.float32(temps[i]))
+        pi = np.exp(x) / np.exp(x).sum()
+        want = float(np.log(np.exp(x).sum()) - (pi * x).sum())
+        assert abs(h[i] - want) <= 2.0 ** -17 * (np.log2(n) + 2)
