@@ -571,7 +571,9 @@ kc_status kc_set_policy(kc_handle* h, const kc_sampling* sampling);
 
 /* The global norm of many gradients and clipping by it:
  *   norm = sqrt(sum_t weight_t^2 * |in_t|^2), scale = min(1, max_norm / norm)
- *   (1 when the norm is not finite), out_t = in_t * scale.
+ *   (1 when the norm is not finite, as it is where an element is not or the
+ *   sum of squares leaves f64: f64 gradients above about 1e154),
+ *   out_t = in_t * scale.
  * grads: HOST array of DEVICE tensors, contiguous, KC_DTYPE_*; out NULL = the
  * tensor only counts, out = in clips in place; outputs must not overlap other
  * tensors. max_norm >= 0 (+infinity: the norm alone decides nothing).

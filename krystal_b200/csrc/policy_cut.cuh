@@ -23,10 +23,20 @@
 namespace kc {
 namespace pol {
 
+// A list is 8 entries a lane, what one warp holds in registers. Top-k up to
+// kListTopK looks for one: the bound admits k entries and those that share
+// their vectors, so a k near 256 leaves more than a list (at 200: 217 to 236 of
+// 4096 f32 entries, which fit, but 246 to 271 of bf16 ones and over 320 of 1024
+// f32 ones) and has counted for nothing. 4096 rows, with the bound and without:
+// 4096 f32 at k = 50 89 and 172 us, at 200 101 and 189; 4096 bf16 at 100 89 and
+// 157, at 200 171 and 160; 1024 f32 at 100 45 and 67, at 200 83 and 73.
 constexpr uint32_t kList = 256;
-constexpr uint32_t kListTopK = 208;  // top-k up to this looks for a list
-constexpr int kPairs = 64;           // lists up to this are cut by comparing all pairs
-constexpr int kBatch = 8;            // rows a CTA takes up to their lists
+constexpr uint32_t kListTopK = 208;
+// Lists up to this are cut by comparing all pairs. 30000 rows under top-p with
+// 32, 64 and 128: of 30 entries 46, 58 and 81 us, of 60 87, 78 and 121, of 120
+// 116, 117 and 204.
+constexpr int kPairs = 64;
+constexpr int kBatch = 8;  // rows a CTA takes up to their lists
 
 struct List {
   uint32_t key[kList], where[kList];  // a key, and its index in the row
@@ -841,9 +851,10 @@ template <> struct Answers<DrawArg> {
 // Bound by instruction issue: 34818 drawn rows of 8 to 240 probabilities, a
 // quarter open, take 93 us at an IPC of 2.5, about 1500 warp instructions a row
 // (64-bit exponentials and logarithms, all pairs of the list), and 2 % of the
-// memory's bandwidth; the loss of 4096 rows takes 17 us, one wave of single
-// rows whose latency bounds it.
-// CTAs an SM. More warps hide more of a row's latency, more registers spill
+// memory's bandwidth; the loss of 4096 rows takes 17 us, the latency of single
+// rows: 1024 CTAs on the 888 that fit, each with its own tables.
+// CTAs an SM (80 registers: f32 draws spill 292 bytes a thread, the others 164
+// to 244). More warps hide more of a row's latency, more registers spill
 // less: 34818 drawn rows took 95, 97, 105 and 96 us with 5 to 8, the loss of
 // 4096 rows between 19 and 20.
 constexpr int kSmallCtas = 6;
@@ -938,8 +949,10 @@ __global__ void __launch_bounds__(128, kSmallCtas) k_policy_small(const __grid_c
 // leave the SM idle.
 // 4096 drawn rows of 4096 under top-k 200, top-p and min-p take 127 us: issue
 // (IPC 2.75; statistics, the lower bound's counts, one warp a list) and
-// barriers. 32 bf16 rows of 131071 take 39 us: latency, a dozen cluster-wide
-// reductions one after another, on 128 of the SMs.
+// barriers. 32 bf16 rows of 131071 with limits of their own take 34 to 42 us:
+// latency, a dozen cluster-wide reductions one after another, on 128 of the SMs.
+// The registers of two CTAs of 16 warps an SM (64) spill 108 to 176 bytes a
+// thread, those of the largest rows' too, whose shared memory leaves one.
 template <typename T, int W, int CL, typename Arg>
 __global__ void __launch_bounds__(W * 32, 32 / W) k_policy_rows(const __grid_constant__ Arg a, uint32_t batch,
                                                                uint32_t chunks) {

@@ -65,7 +65,7 @@ def test_lists_of_many_launches(be, count, share):
     assert scale == (norm * share / got if share < 1 else 1.0)
     for b, o in zip(before, outs):
         want = b.double() * scale
-        assert bool(((o.double() - want).abs() <= 2.0 ** -23 * want.abs()).all())  # the scale's half step and the product's
+        assert bool(((o.double() - want).abs() <= 2.0 ** -23 * want.abs()).all())  # two half steps: scale, product
 
 
 def clip_time(be, count):
@@ -92,3 +92,16 @@ def test_the_time_of_a_long_list_grows_with_its_length(be):
     short, long = clip_time(be, 32768), clip_time(be, 262144)
     print(f"32768 tensors: {short:.3f} ms, 262144: {long:.3f} ms")
     assert long < 12 * short
+
+
+def test_a_sum_of_squares_beyond_f64_scales_nothing(be):
+    """Finite f64 gradients whose squares are not: the norm is infinite, and what
+    follows sees the gradients as they are."""
+    for size, weight in ((1e200, 1.0), (1e100, 1e100)):
+        g = torch.full((1000,), size, dtype=torch.float64, device="cuda")
+        out, res = torch.zeros_like(g), torch.zeros(2, dtype=torch.float64, device="cuda")
+        lst = GradList([g], [out], [weight])
+        torch.cuda.synchronize()
+        be.clip_grads(lst, 1.0, res.data_ptr())
+        be.synchronize()
+        assert res.tolist() == [math.inf, 1.0] and torch.equal(out, g)
