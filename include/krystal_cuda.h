@@ -565,7 +565,8 @@ kc_status kc_policy_loss(kc_handle* h, const kc_rows_view* rows, const kc_sampli
  * over pi's support, nothing for a target that pi does not hold: cut off,
  * outside the row, or of a pi that is 0 in f32 (an AWAY target keeps its own
  * weighting, with pi for p). NULL: the whole softmax at temperature 1, as the
- * reference (where a target outside the row pushes every entry down). Scalar limits only; temperature above 0.
+ * reference (where a target outside the row pushes every entry down). Scalar
+ * limits only; temperature above 0.
  * The policy output, the value head and the readings stay those of p. */
 kc_status kc_set_policy(kc_handle* h, const kc_sampling* sampling);
 

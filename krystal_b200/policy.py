@@ -102,8 +102,9 @@ class GradList:
     where each clipped gradient goes (None: in place), and each one's factor
     in the norm. The list holds its tensors and its workspace; it is built once
     for gradients that stay where they are. A list dropped while its clip is
-    queued leaves both with the backend until the stream has passed them. Two captured graphs that may run at once need a list each,
-    and a graph's list has to live as long as the graph."""
+    queued leaves both with the backend until the stream has passed them. Two
+    captured graphs that may run at once need a list each, and a graph's list
+    has to live as long as the graph."""
 
     def __init__(self, tensors, outs=None, weights=None):
         import torch

@@ -154,15 +154,16 @@ def test_masked_entries_have_no_gradient_whatever_the_factors(be, n, dtype, cut)
     assert not bool(torch.isfinite(g[:, 1]).any())
 
 
-@pytest.mark.parametrize("dtype,at", [("f32", 0.0), ("f16", 0.0), ("bf16", 0.0), ("f32", 1e6)])
+@pytest.mark.parametrize("dtype,at", [("f32", 0.0), ("f16", 0.0), ("bf16", 0.0), ("f32", 1e3), ("f32", 1e6)])
 @pytest.mark.parametrize("n", LENGTHS)
 def test_confident_rows_keep_their_small_gradient(be, n, dtype, at):
     """The action holds all but 1e-3 to 1e-12 of the mass. Its gradient, the loss
     and the entropy are as exact as the others' weights: an f32 exponent x is
     off by 2^-23 |x| (log2(e) / T in f32) and its own rounding, |x| <= 35, the
     weight by ex2's 2^-22 and the sum's 18 terms: below 2^-16 of each, which
-    makes 2^-15 of what is made of them; half a step of the type on top. At 1e6
-    (f32) the largest score is subtracted first."""
+    makes 2^-15 of what is made of them; half a step of the type on top. At 1e3
+    (f32) every exponent holds one rounding of m log2(e) / T, which cancels; at
+    1e6 the largest score is subtracted first."""
     rng = np.random.default_rng(n)
     gap = np.array([8.0, 14.0, 20.0, 30.0]) + np.log(n)
     v = np.round(rng.uniform(-2, 0, (4, n)) - gap[:, None], 0 if at else 3)  # (f32 steps of 1e6 are 2^-4)
