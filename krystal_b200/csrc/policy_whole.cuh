@@ -324,7 +324,7 @@ __device__ __forceinline__ void shifted(const uint4& x, const uint4& y, bool odd
 // and the instruction cache then bounds them), three CTAs an SM overlap one
 // row's loads with another's arithmetic, and the last pass reads the row at the
 // gradient's alignment, so that every store is a whole vector. 4096 bf16 rows of
-// 32001 take 112 to 120 us, 4.4 to 4.7 TB/s, two thirds of the measured copy
+// 32001 take 112 to 124 us, 4.2 to 4.7 TB/s, two thirds of the measured copy
 // rate: two exponentials an entry keep their pipe busy half the time, and a
 // CTA's own load, arithmetic and store follow each other.
 template <typename T, int NT, int CL>
