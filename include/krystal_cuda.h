@@ -593,6 +593,131 @@ uint64_t kc_clip_workspace(uint64_t count);
 kc_status kc_clip_grads(kc_handle* h, const kc_grad_view* grads, uint64_t count, double max_norm, void* workspace,
                         uint64_t workspace_bytes, double* result);
 
+/* ---------------------------------------------------------------------------
+ * The bank cache: keys and values of records, kept on the device in 8 bits from
+ * turn to turn. What a record encodes to depends on the record alone (the
+ * encoder blocks and the pooling see no other), so a bank that grows need not be
+ * encoded again; the reference encodes the whole frame every turn
+ * (host/session.ts:128-147), and these entry points are additions beside it.
+ *
+ * Storage. Pages of KC_CACHE_PAGE rows; a row has kv_heads keys and as many
+ * values of head_dim (32, 64 or 128) codes. Page after page and head after head
+ * two cells of 32 rows: keys [32][head_dim] and values [32][head_dim], a byte a
+ * code, then 32 f32 key scales and 32 f32 value scales. A key's 64-byte halves
+ * change places where head_dim is 128 and bit 2 of its row is set; a value's
+ * byte b lies at b ^ 32 * (row & 3) for 128 dims and b ^ 32 * ((row >> 1) & 1)
+ * for 64. Behind the pages lie their bounds [pages][kv_heads][2][head_dim] f32:
+ * the smallest and the largest of the keys that a page holds.
+ * A row x of a head is stored as scale = max(f32(max |x| / top), 2^-100) and
+ * code = round(f32(x / scale)), halves to the even, top = 127 (KC_CACHE_I8, kept
+ * as code + 128) or 448 (KC_CACHE_E4M3); its value is f32(code * scale). NaN
+ * counts as 0, magnitudes beyond 2^127 as 2^127. The caller owns the storage
+ * (DEVICE, 16-byte aligned, kc_cache_bytes); it need not be cleared.
+ *
+ * Every pointer of these entry points is a DEVICE pointer. They queue work on the
+ * handle's stream, allocate nothing, wait for nothing and can be captured. Equal
+ * calls give equal bits. Rows or questions behind the last sequence's are left
+ * as they were. */
+#define KC_CACHE_I8 0
+#define KC_CACHE_E4M3 1
+#define KC_CACHE_PAGE 64u
+#define KC_CACHE_MAX_SELECT 1638400u  /* rows a sequence may hold where kc_cache_blocks selects */
+
+typedef struct kc_cache_view {
+  void* storage;
+  uint64_t bytes;      /* of storage */
+  uint32_t pages, kv_heads, head_dim;
+  int32_t format;      /* KC_CACHE_* */
+} kc_cache_view;
+
+uint64_t kc_cache_bytes(uint32_t pages, uint32_t kv_heads, uint32_t head_dim);
+
+/* Sequence s (a session's bank) holds lengths[s] rows: row i in page
+ * pages[s * pitch + i / KC_CACHE_PAGE]. A page number outside the cache shuts
+ * its rows out: they are not written, read as 0, attended by nothing. */
+typedef struct kc_page_table {
+  const uint32_t* pages;    /* [sequences, pitch] */
+  const uint32_t* lengths;  /* [sequences] */
+  uint32_t sequences, pitch;
+  uint32_t max_length;      /* bounds the lengths (0 = pitch * KC_CACHE_PAGE); a longer sequence is attended up to it */
+} kc_page_table;
+
+/* Rows [rows, kv_heads, head_dim], pitch elements apart (0 = dense). Sequence s
+ * has rows row_off[s] .. row_off[s+1] - 1 (ascending; NULL: row s). */
+typedef struct kc_cache_rows {
+  void *keys, *values;      /* read from by kc_cache_write, written by kc_cache_read (there either may be NULL) */
+  const uint64_t* row_off;  /* [sequences+1] or NULL */
+  uint64_t rows, pitch;
+  int32_t dtype;            /* KC_DTYPE_F32 / F16 / BF16 */
+} kc_cache_rows;
+
+/* Appends: a sequence's rows become its last ones, lengths[s] counting them
+ * already. A sequence that is cut back and written again is written the same
+ * way. Bounds of the pages written are taken over all rows these hold now. A
+ * page that is written belongs to one sequence of the call. */
+kc_status kc_cache_write(kc_handle* h, const kc_cache_view* cache, const kc_page_table* table, const kc_cache_rows* rows);
+/* Stored values back, rounded to the rows' type: a sequence's last rows, or
+ * (starts [sequences]) those from row starts[s] on. Rows that a sequence does
+ * not hold read as 0. */
+kc_status kc_cache_read(kc_handle* h, const kc_cache_view* cache, const kc_page_table* table, const uint32_t* starts,
+                        const kc_cache_rows* rows);
+
+/* Questions [questions, heads, head_dim], pitch elements apart (0 = dense);
+ * heads / kv_heads neighbouring heads share a key head. Sequence s asks
+ * q_off[s] .. q_off[s+1] - 1 (NULL: question s). Values are finite. */
+typedef struct kc_question_view {
+  const void* q;
+  const uint64_t* q_off;    /* [sequences+1] or NULL */
+  uint32_t questions, heads;
+  uint32_t max_questions;   /* bounds one sequence's questions (0 = questions); those beyond it are left as they were */
+  int32_t dtype;            /* KC_DTYPE_F32 / F16 / BF16 */
+  uint64_t pitch;
+} kc_question_view;
+
+/* The blocks (pages, by their number in the sequence) a question's group of
+ * heads looks at: the `recent` last ones and the best of the others by
+ *   sum over the group's heads of sum_d max(q_d * min_d, q_d * max_d),
+ * which no sum of q . k of a row of the block exceeds (f64; ties and equals to
+ * the lowest block; NaN below all). blocks [questions, kv_heads, count]: in
+ * ascending order, KC_NO_SELECTION behind the last where the sequence has
+ * fewer. recent <= count. */
+kc_status kc_cache_blocks(kc_handle* h, const kc_cache_view* cache, const kc_page_table* table,
+                          const kc_question_view* questions, uint32_t count, uint32_t recent, uint32_t* blocks);
+
+/* Attention: out = sum_j softmax_j(scale * q . k_j + mask_j) v_j over the rows
+ * of the question's sequence, or of the blocks its list names (a block named
+ * twice counts twice; numbers outside the sequence count for nothing). A mask
+ * entry at or below -1e29, or NaN, shuts its row out, larger ones than 1e29 count
+ * as 1e29; rows behind the mask's end are shut out. Nothing left: out 0, lse
+ * -infinity. Scores, sums and statistics are f32; for 16-bit questions the
+ * weights are rounded to 11 bits before they meet the values, for f32 ones to
+ * 22. */
+typedef struct kc_attend_view {
+  void* out;                 /* [questions, heads, head_dim], the questions' type, out_pitch elements apart (0 = dense) */
+  uint64_t out_pitch;
+  float* lse;                /* [questions, heads] log of the sum of exponentials, or NULL */
+  const float* mask;         /* sequence s's [Q_s, R_s] block at mask_off[s], as kc_batch_view.mask, or NULL */
+  const uint64_t* mask_off;  /* [sequences+1] */
+  const uint32_t* blocks;    /* [questions, kv_heads, block_count] (kc_cache_blocks), or NULL: every row */
+  uint32_t block_count;
+  float scale;               /* 0 = 1 / sqrt(head_dim) */
+  void* workspace;           /* kc_cache_attend_workspace bytes, 16-byte aligned, the call's own while it runs */
+  uint64_t workspace_bytes;
+} kc_attend_view;
+uint64_t kc_cache_attend_workspace(kc_handle* h, const kc_cache_view* cache, const kc_page_table* table,
+                                   const kc_question_view* questions, uint32_t block_count);
+kc_status kc_cache_attend(kc_handle* h, const kc_cache_view* cache, const kc_page_table* table,
+                          const kc_question_view* questions, const kc_attend_view* attend);
+
+/* Pointer scores over a cache of one head: scale * q . k_j + mask_j into
+ * sequence s's [Q_s, R_s] block at off[s], f32, -1e30 for rows that the mask (laid
+ * out alike, or NULL; read as above) shuts out or that the sequence does not
+ * hold: rows as kc_draw_device and kc_policy_loss take them. scale 0 =
+ * 1 / sqrt(head_dim). */
+kc_status kc_cache_scores(kc_handle* h, const kc_cache_view* cache, const kc_page_table* table,
+                          const kc_question_view* questions, const uint64_t* off, const float* mask, float scale,
+                          float* scores);
+
 /* KRY1 checkpoints (host/checkpoint.ts:17-116): 11 little-endian u32 header
  * words (magic "KRY1" = 0x4b525931, version 1, hiddenSize, ffnSize,
  * encoderBlocks, mixerBlocks, headCount, headDim, routeKindCount, tokenRows

@@ -34,6 +34,9 @@ KC_NO_WORD = 0xFFFFFFFF
 KC_DTYPE_F32, KC_DTYPE_F16, KC_DTYPE_BF16, KC_DTYPE_F64 = 0, 1, 2, 3
 KC_ROWS_SCORES, KC_ROWS_P = 0, 1
 KC_MAX_ROW = 262128
+KC_CACHE_I8, KC_CACHE_E4M3 = 0, 1
+KC_CACHE_PAGE = 64
+KC_CACHE_MAX_SELECT = 1638400
 CHECKPOINT_REFUSALS = {1: "not a krystal checkpoint", 2: "a later checkpoint format", 3: "a different geometry",
                        4: "a different vocabulary", 5: "truncated"}
 
@@ -47,7 +50,9 @@ EXPORTS = ("kc_abi_version", "kc_create", "kc_sync", "kc_encode", "kc_select", "
            "kc_stream_push_many", "kc_load_checkpoint", "kc_save_checkpoint", "kc_select_batch",
            "kc_inject_wait_expiry", "kc_learn_plan", "kc_learn_accumulate_rows", "kc_learn_apply",
            "kc_copy_weights", "kc_stream_create_ex", "kc_stream_read_stats", "kc_draw_device", "kc_draw",
-           "kc_draw_batch", "kc_policy_loss", "kc_set_policy", "kc_clip_workspace", "kc_clip_grads")
+           "kc_draw_batch", "kc_policy_loss", "kc_set_policy", "kc_clip_workspace", "kc_clip_grads", "kc_cache_bytes",
+           "kc_cache_write", "kc_cache_read", "kc_cache_blocks", "kc_cache_attend_workspace", "kc_cache_attend",
+           "kc_cache_scores")
 
 
 class KrystalCudaError(RuntimeError):
@@ -205,6 +210,31 @@ class KcGradView(C.Structure):
     _fields_ = [("in_", P), ("out", P), ("n", C.c_uint64), ("weight", C.c_double), ("dtype", C.c_int32)]
 
 
+class KcCacheView(C.Structure):
+    _fields_ = [("storage", P), ("bytes", C.c_uint64), ("pages", C.c_uint32), ("kv_heads", C.c_uint32),
+                ("head_dim", C.c_uint32), ("format", C.c_int32)]
+
+
+class KcPageTable(C.Structure):
+    _fields_ = [("pages", P), ("lengths", P), ("sequences", C.c_uint32), ("pitch", C.c_uint32),
+                ("max_length", C.c_uint32)]
+
+
+class KcCacheRows(C.Structure):
+    _fields_ = [("keys", P), ("values", P), ("row_off", P), ("rows", C.c_uint64), ("pitch", C.c_uint64),
+                ("dtype", C.c_int32)]
+
+
+class KcQuestionView(C.Structure):
+    _fields_ = [("q", P), ("q_off", P), ("questions", C.c_uint32), ("heads", C.c_uint32),
+                ("max_questions", C.c_uint32), ("dtype", C.c_int32), ("pitch", C.c_uint64)]
+
+
+class KcAttendView(C.Structure):
+    _fields_ = [("out", P), ("out_pitch", C.c_uint64), ("lse", P), ("mask", P), ("mask_off", P), ("blocks", P),
+                ("block_count", C.c_uint32), ("scale", C.c_float), ("workspace", P), ("workspace_bytes", C.c_uint64)]
+
+
 _lib = None
 
 
@@ -278,6 +308,16 @@ def load(path: str | os.PathLike | None = None) -> C.CDLL:
     lib.kc_clip_workspace.argtypes = [C.c_uint64]
     lib.kc_clip_workspace.restype = C.c_uint64
     lib.kc_clip_grads.argtypes = [P, P, C.c_uint64, C.c_double, P, C.c_uint64, P]
+    cache = [P, C.POINTER(KcCacheView), C.POINTER(KcPageTable)]
+    lib.kc_cache_bytes.argtypes = [C.c_uint32, C.c_uint32, C.c_uint32]
+    lib.kc_cache_bytes.restype = C.c_uint64
+    lib.kc_cache_write.argtypes = cache + [C.POINTER(KcCacheRows)]
+    lib.kc_cache_read.argtypes = cache + [P, C.POINTER(KcCacheRows)]
+    lib.kc_cache_blocks.argtypes = cache + [C.POINTER(KcQuestionView), C.c_uint32, C.c_uint32, P]
+    lib.kc_cache_attend_workspace.argtypes = cache + [C.POINTER(KcQuestionView), C.c_uint32]
+    lib.kc_cache_attend_workspace.restype = C.c_uint64
+    lib.kc_cache_attend.argtypes = cache + [C.POINTER(KcQuestionView), C.POINTER(KcAttendView)]
+    lib.kc_cache_scores.argtypes = cache + [C.POINTER(KcQuestionView), P, P, C.c_float, P]
     for name in ("kc_create", "kc_sync", "kc_encode", "kc_select", "kc_forward_batch", "kc_forward_batch_device",
                  "kc_set_stream", "kc_synchronize", "kc_profile", "kc_profile_read", "kc_select_noalloc",
                  "kc_set_precision", "kc_backward", "kc_backward_batch_device", "kc_learn_frame_stats",
@@ -285,7 +325,8 @@ def load(path: str | os.PathLike | None = None) -> C.CDLL:
                  "kc_stream_push_many", "kc_load_checkpoint", "kc_save_checkpoint", "kc_select_batch",
                  "kc_inject_wait_expiry", "kc_learn_plan", "kc_learn_accumulate_rows", "kc_learn_apply",
                  "kc_copy_weights", "kc_stream_create_ex", "kc_stream_read_stats", "kc_draw_device", "kc_draw",
-                 "kc_draw_batch", "kc_policy_loss", "kc_set_policy", "kc_clip_grads"):
+                 "kc_draw_batch", "kc_policy_loss", "kc_set_policy", "kc_clip_grads", "kc_cache_write", "kc_cache_read",
+                 "kc_cache_blocks", "kc_cache_attend", "kc_cache_scores"):
         getattr(lib, name).restype = C.c_int
     _lib = lib
     return lib

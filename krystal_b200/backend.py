@@ -27,6 +27,7 @@ from typing import Callable, Sequence
 import numpy as np
 
 from . import abi
+from .cache import BankCache
 from .frame import FrameBatch, HostFrame
 from .model import BrainForwardConfig, BrainForwardWeights
 from .policy import GradList, Sampling
@@ -426,7 +427,9 @@ class CudaBrainBackend:
         a graph is captured, where neither is allowed."""
         import torch
         with self._clip_lock:
-            stream = torch.cuda.ExternalStream(self.stream_ptr(), device=self.device)
+            at = self.stream_ptr()
+            stream = (torch.cuda.default_stream(self.device) if at == 1  # cudaStreamLegacy, the default stream's name
+                      else torch.cuda.ExternalStream(at, device=self.device))
             if torch.cuda.is_current_stream_capturing():
                 return
             with torch.cuda.stream(stream):
@@ -437,6 +440,62 @@ class CudaBrainBackend:
                 self._clips_queued.append((self._clips_dropped.popleft(), event))
                 event.record(stream)
             self._clips_queued = [c for c in self._clips_queued if not c[1].query()]
+
+    # --- the bank cache -------------------------------------------------------------
+    def _cache(self, cache: BankCache):
+        if cache.device.index != self.device:
+            raise ValueError(f"the cache lies on {cache.device}, the backend on cuda:{self.device}")
+        cache.queued_on(self)
+        if self._clips_dropped or self._clips_queued:
+            self._release_clips()
+        return C.byref(cache.view)
+
+    def cache_write(self, cache: BankCache, table: abi.KcPageTable, rows: abi.KcCacheRows) -> None:
+        """kc_cache_write: the rows quantised as the last of their sequences
+        (cache.page_table, cache.cache_rows: device pointers); queued on the
+        handle's stream, as the other calls on a cache are."""
+        abi.check(self._lib.kc_cache_write(self._h, self._cache(cache), C.byref(table), C.byref(rows)), self._h)
+
+    def cache_read(self, cache: BankCache, table: abi.KcPageTable, rows: abi.KcCacheRows,
+                   starts: int | None = None) -> None:
+        """kc_cache_read: the sequences' last rows, or those from ``starts`` (u32
+        [sequences], device) on, into rows.keys and rows.values."""
+        abi.check(self._lib.kc_cache_read(self._h, self._cache(cache), C.byref(table), starts, C.byref(rows)), self._h)
+
+    def cache_blocks(self, cache: BankCache, table: abi.KcPageTable, questions: abi.KcQuestionView, count: int,
+                     recent: int, blocks: int) -> None:
+        """kc_cache_blocks: the ``count`` pages each question's group of heads looks
+        at, the ``recent`` last ones among them, into blocks (u32 [questions,
+        kv_heads, count], device)."""
+        abi.check(self._lib.kc_cache_blocks(self._h, self._cache(cache), C.byref(table), C.byref(questions), count,
+                                            recent, blocks), self._h)
+
+    def attend_workspace(self, cache: BankCache, table: abi.KcPageTable, questions: abi.KcQuestionView,
+                         block_count: int = 0) -> int:
+        """kc_cache_attend_workspace: the bytes of device memory a cache_attend of
+        these arguments needs."""
+        return int(self._lib.kc_cache_attend_workspace(self._h, C.byref(cache.view), C.byref(table),
+                                                       C.byref(questions), block_count))
+
+    def cache_attend(self, cache: BankCache, table: abi.KcPageTable, questions: abi.KcQuestionView, out: int,
+                     out_pitch: int = 0, lse: int | None = None, mask: int | None = None, mask_off: int | None = None,
+                     blocks: int | None = None, block_count: int = 0, scale: float = 0.0,
+                     workspace: int | None = None, workspace_bytes: int = 0) -> None:
+        """kc_cache_attend: attention of the questions over their sequences' rows, or
+        over the blocks that their lists name. Outputs, mask, blocks and workspace
+        are device pointers."""
+        v = abi.KcAttendView(out, out_pitch, lse, mask, mask_off, blocks, block_count, scale, workspace,
+                             workspace_bytes)
+        abi.check(self._lib.kc_cache_attend(self._h, self._cache(cache), C.byref(table), C.byref(questions),
+                                            C.byref(v)), self._h)
+
+    def cache_scores(self, cache: BankCache, table: abi.KcPageTable, questions: abi.KcQuestionView, scores: int,
+                     off: int, mask: int | None = None, scale: float = 0.0) -> None:
+        """kc_cache_scores: pointer scores over a cache of one head, laid out like a
+        batch's p at ``off``: rows that ``draw`` and ``policy_loss`` take
+        (policy.ragged_rows)."""
+        abi.check(self._lib.kc_cache_scores(self._h, self._cache(cache), C.byref(table), C.byref(questions), off, mask,
+                                            scale, scores), self._h)
 
     # --- packed ragged batches ------------------------------------------------
     def forward_batch(self, batch: FrameBatch, rule: MaskRule | None = None, uniforms=None,

@@ -27,6 +27,7 @@
 
 #include "../../include/krystal_cuda.h"
 #include "backward.cuh"
+#include "cache_args.h"
 #include "common.cuh"
 #include "exact.cuh"
 #include "fast.cuh"
@@ -1940,6 +1941,7 @@ kc_status kc_create(const kc_config* config, const kc_weights_view* weights, int
                                 kc::oz::kSmem)))
     return bail(e, "smem");
   if ((e = kc::pol::prepare())) return bail(e, "smem");
+  if ((e = kc::cache::prepare())) return bail(e, "smem");
   s = do_sync(h, weights, nullptr);
   if (s) {
     std::string m = h->err;
@@ -2811,4 +2813,5 @@ const char* kc_last_error(kc_handle* h) { return h ? h->err.c_str() : g_create_e
 }  // extern "C"
 
 #include "policy_abi.cuh"
+#include "cache_abi.cuh"
 #include "stream.cuh"
