@@ -90,6 +90,20 @@ struct BlockArg {
   uint32_t* blocks;         // [questions][kv heads][count]
 };
 
+// By question type (cache_attend_f32.cu, cache_attend_f16.cu, cache_attend_bf16.cu).
+cudaError_t attend_f32(const AttendArg& a, int sms, cudaStream_t s, uint64_t* launches);
+cudaError_t attend_f16(const AttendArg& a, int sms, cudaStream_t s, uint64_t* launches);
+cudaError_t attend_bf16(const AttendArg& a, int sms, cudaStream_t s, uint64_t* launches);
+cudaError_t scores_f32(const ScoreArg& a, int sms, cudaStream_t s, uint64_t* launches);
+cudaError_t scores_f16(const ScoreArg& a, int sms, cudaStream_t s, uint64_t* launches);
+cudaError_t scores_bf16(const ScoreArg& a, int sms, cudaStream_t s, uint64_t* launches);
+
+cudaError_t prepare_store();
+cudaError_t prepare_f32();
+cudaError_t prepare_f16();
+cudaError_t prepare_bf16();
+
+// What the kernels need once on each device (the current one).
 cudaError_t prepare();
 
 cudaError_t launch_write(const Store& c, const Table& t, const Rows& r, int sms, cudaStream_t s, uint64_t* launches);

@@ -1,0 +1,633 @@
+// cache_attend.cuh — attention and pointer scores of questions over the bank
+// cache, on the tiles of cache_tile.cuh; instantiated by question type
+// (cache_attend_f32.cu, _f16.cu, _bf16.cu).
+//
+// Attention. With s_j the scores in units of log 2, b_j their mask entries and
+// vs_j = f_j 2^e_j the value scales,
+//   t_j = (b_j - B) + s_j + e_j,  B the largest b_j,  M the largest t_j,
+//   x_j = 2^(t_j - M + 8),  l = sum x_j 2^-e_j,  o = sum (x_j f_j) code_j,  out = o / l.
+// The value scales' exponents are in the maximum, so that the weights x_j f_j that
+// are rounded to f16 lie below 2^15 whatever the scales are, and a large scale
+// that the mask or its score puts out of the running does not push the others
+// below f16's range. Subtracting B first keeps the digits of masks far from 0.
+// B, M, l and o run over a warp's cells (M is left alone while it rises by less
+// than 6 binary orders), then over the warps that share a row, then over the parts
+// that a long sequence is cut into.
+//
+// A cell's bytes are read once by the team of warps that needs them, by 16-byte
+// asynchronous copies kStages - 1 cells ahead.
+#pragma once
+#include <algorithm>
+
+#include "cache_tile.cuh"
+
+namespace kc {
+namespace cache {
+namespace {
+
+constexpr int kThreads = 256, kWarps = 8;
+constexpr float kLift = 8.0f, kSlack = 6.0f;
+constexpr int kLeastExp = -80;  // value scales below it keep their digits in f_j; l stays below 2^128
+
+__host__ __device__ constexpr int stages(int dim) { return dim == 32 ? 4 : 3; }
+
+// What a warp needs of one key of a cell: score = product * a * unit + e.
+struct KeyInfo {
+  float a;   // key scale
+  float e;   // exponent of the value scale; -infinity: not attended
+  float f;   // value scale / 2^e
+  float re;  // 2^-e
+};
+
+// The unit of work a team looks at: a sequence's questions (or one question, with
+// a list of its own) against one key head.
+struct Unit {
+  uint32_t seq, q0, rows, len, blocks, kv, row0;  // row0: the team's first row
+  uint64_t stride;                                // of the mask
+  const float* mask;                              // of the unit's first question
+};
+
+// How a launch's warps are shared out: teams of `mg` warps (16 rows each) read the
+// same cells, `kg` teams share a unit's cells, a CTA has hg units.
+struct Shape {
+  uint32_t mg, kg, hg, chunks;  // chunks: of 16 mg rows, that a unit may have
+  uint64_t items;
+};
+
+__device__ __forceinline__ bool unit_of(const AttendArg& a, const Shape& sh, uint64_t item, Unit* u) {
+  if (item >= sh.items) return false;
+  const uint32_t group = a.a.heads / a.c.heads;
+  u->kv = uint32_t(item % a.c.heads);
+  const uint64_t rest = item / a.c.heads;
+  const uint32_t chunk = uint32_t(rest % sh.chunks), which = uint32_t(rest / sh.chunks);
+  uint32_t first, count;
+  if (a.blocks) {  // a question
+    if (a.a.off) {
+      if (which < a.a.off[0] || which >= a.a.off[a.t.seqs]) return false;
+      u->seq = owner_of(a.a.off, a.t.seqs, which);
+      first = uint32_t(a.a.off[u->seq]);
+      count = uint32_t(a.a.off[u->seq + 1]) - first;
+    } else {
+      if (which >= a.t.seqs) return false;
+      u->seq = first = which;
+      count = 1;
+    }
+    if (which - first >= a.a.max_q) return false;
+    u->q0 = which;
+    u->rows = group;
+  } else {  // a sequence
+    u->seq = which;
+    first = a.a.off ? uint32_t(a.a.off[which]) : which;
+    const uint64_t end = a.a.off ? a.a.off[which + 1] : which + 1;
+    count = uint32_t(end - first);
+    u->q0 = first;
+    u->rows = min(count, a.a.max_q) * group;
+  }
+  if (first >= a.a.questions) return false;
+  u->rows = min(u->rows, (a.a.questions - u->q0) * group);
+  u->row0 = chunk * 16 * sh.mg;
+  if (u->row0 >= u->rows) return false;
+  u->len = length_of(a.t, u->seq);
+  u->blocks = (u->len + kPage - 1) / kPage;
+  u->stride = 0;
+  u->mask = nullptr;
+  if (a.mask) {
+    u->stride = (a.mask_off[u->seq + 1] - a.mask_off[u->seq]) / count;
+    u->mask = a.mask + a.mask_off[u->seq] + (u->q0 - first) * u->stride;
+  }
+  return true;
+}
+
+// 16 questions' rows of a warp's results, as the warps of a row, or the parts of a
+// sequence, are joined: [B, M, l, -] and o.
+struct Stat {
+  float b, m, l;
+};
+__device__ __forceinline__ float weight_of(const Stat& s, float b, float m) {
+  return s.m == -INFINITY ? 0.0f : ex2((s.b - b) + (s.m - m));
+}
+
+template <typename T, int FMT>
+__device__ __forceinline__ void put(const AttendArg& a, uint64_t question, uint32_t head, uint32_t dim, float o, float l) {
+  static_cast<T*>(a.out)[question * a.out_pitch + uint64_t(head) * a.c.dim + dim] = from_f32<T>(l > 0.0f ? o / l * widened<FMT>() : 0.0f);
+}
+__device__ __forceinline__ void put_lse(const AttendArg& a, uint64_t question, uint32_t head, const Stat& s) {
+  if (a.lse) a.lse[question * a.a.heads + head] = s.l > 0.0f ? (s.b + s.m - kLift) * kLn2 + logf(s.l) : -INFINITY;
+}
+
+// Part `part` of a row's results in the workspace: o [dim], then B, M, l.
+__device__ __forceinline__ float* part_of(const AttendArg& a, uint64_t question, uint32_t head, uint32_t part) {
+  return a.work + ((question * a.a.heads + head) * a.splits + part) * (a.c.dim + 4);
+}
+
+template <typename T, int D, int FMT>
+__global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void k_attend(AttendArg a, Shape sh) {
+  constexpr int S = stages(D), CB = int(cell_bytes(D)), NB = D / 8;
+  constexpr bool kTwo = sizeof(T) == 4;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ KeyInfo s_info[kWarps][kCell];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+  const uint32_t team = warp / sh.mg, mi = warp % sh.mg;
+  const uint32_t part = blockIdx.y, group = a.a.heads / a.c.heads;
+  Unit u{};
+  const bool live = unit_of(a, sh, uint64_t(blockIdx.x) * sh.hg + team / sh.kg, &u);
+
+  Walk w{};
+  uint32_t parts = 1;
+  if (live) {
+    const uint32_t all = a.blocks ? a.block_count : u.blocks;
+    parts = max(1u, (all + a.chunk - 1) / a.chunk);
+    w.table = a.t.table + uint64_t(u.seq) * a.t.pitch;
+    w.list = a.blocks ? a.blocks + (uint64_t(u.q0) * a.c.heads + u.kv) * a.block_count : nullptr;
+    w.blocks = u.blocks;
+    w.pages = a.c.pages;
+    w.b0 = part * a.chunk;
+    w.cells = w.b0 < all ? 2 * min(a.chunk, all - w.b0) : 0;
+    w.first = team % sh.kg;
+    w.step = sh.kg;
+  }
+  const bool mine = live && part < parts;
+  const uint32_t n = mine ? w.count() : 0;
+  // this lane's rows: their question (from the unit's first) and head
+  const uint32_t row = u.row0 + mi * 16 + g;
+  const bool busy = mine && u.row0 + mi * 16 < u.rows;
+  const bool ok0 = mine && row < u.rows, ok1 = mine && row + 8 < u.rows;
+  const uint32_t i0 = row / group, i1 = (row + 8) / group;
+  QTile<T, D> q;
+  {
+    const T* base = static_cast<const T*>(a.a.q);
+    q.load(ok0 ? base + (u.q0 + i0) * a.a.pitch + (u.kv * group + row % group) * uint64_t(D) : nullptr,
+           ok1 ? base + (u.q0 + i1) * a.a.pitch + (u.kv * group + (row + 8) % group) * uint64_t(D) : nullptr, c,
+           a.scale * kLog2e);
+  }
+  const float* mask0 = u.mask && ok0 ? u.mask + i0 * u.stride : nullptr;
+  const float* mask1 = u.mask && ok1 ? u.mask + i1 * u.stride : nullptr;
+
+  uint8_t* ring = smem + team * (S * CB);
+  auto issue = [&](uint32_t i, uint32_t page) {
+    if (page != kNone) {
+      const uint8_t* src = cell_of<D>(a.c, page, u.kv, w.half(i));
+      uint8_t* dst = ring + (i % S) * CB;
+      for (uint32_t k = mi * 32 + lane; k < CB / 16; k += sh.mg * 32) copy16(dst + 16 * k, src + 16 * k);
+    }
+    copy_commit();
+  };
+
+  float o[NB][4], top[2] = {-INFINITY, -INFINITY}, high[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+#pragma unroll
+  for (int t = 0; t < NB; t++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[t][i] = 0.0f;
+  if (n) w.begin();
+  if (n) {
+#pragma unroll
+    for (uint32_t i = 0; i + 1 < S; i++) {
+      const uint32_t page = w.page_of(0, i);
+      issue(i, i < n ? page : kNone);
+    }
+  }
+  KeyInfo* info = s_info[warp];
+  for (uint32_t i = 0; i < n; i++) {
+    w.advance(i);
+    copy_wait<S - 2>();
+    meet(team, sh.mg);
+    const uint32_t next = w.page_of(i, S - 1), page = w.page_of(i, 0), block = w.block_of(i);
+    issue(i + S - 1, i + S - 1 < n ? next : kNone);
+    if (!busy || page == kNone) continue;
+    const uint8_t* cell = ring + (i % S) * CB;
+    const uint64_t pos = uint64_t(block) * kPage + w.half(i) * kCell;
+    {
+      const float* scales = reinterpret_cast<const float*>(cell + 2 * kCell * D);
+      const float vs = scales[kCell + lane];
+      const bool open = pos + lane < u.len && (!u.mask || pos + lane < u.stride);
+      const uint32_t e = max(__float_as_uint(vs) >> 23, uint32_t(127 + kLeastExp)), es = min(e, 253u);
+      KeyInfo k;
+      k.re = pow2_biased(254u - es);
+      k.f = vs * k.re;
+      k.a = scales[lane] * widened<FMT>();
+      k.e = float(int(es) - 127);
+      if (!open) k = KeyInfo{0.0f, -INFINITY, 0.0f, 0.0f};
+      info[lane] = k;
+    }
+    float s[4][4];
+    key_products<T, D, FMT>(q, cell, g, c, s);
+    __syncwarp();
+#pragma unroll
+    for (int J = 0; J < 4; J++)
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        const KeyInfo ki = info[8 * J + 4 * k + c];
+        s[J][k] = fmaf(s[J][k] * ki.a, q.unit[0], ki.e);
+        s[J][2 + k] = fmaf(s[J][2 + k] * ki.a, q.unit[1], ki.e);
+      }
+    float keep[2] = {1.0f, 1.0f};
+    bool moved = false;
+    if (u.mask) {
+      float bias[4][4], most[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int J = 0; J < 4; J++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const uint64_t at = pos + 8 * J + 4 * (k & 1) + c;
+          const float* m = k < 2 ? mask0 : mask1;
+          const float x = m && at < u.stride && at < u.len ? m[at] : -INFINITY;
+          bias[J][k] = x > kBlocked ? fminf(x, -kBlocked) * kLog2e : -INFINITY;
+          most[k / 2] = fmaxf(most[k / 2], bias[J][k]);
+        }
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 1));
+        most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 2));
+        const float was = top[h];
+        top[h] = fmaxf(was, most[h]);
+        if (was != top[h]) {  // what is summed so far was measured from the former one
+          high[h] += was - top[h];
+          if (was == -INFINITY) high[h] = -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int J = 0; J < 4; J++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) s[J][k] += bias[J][k] == -INFINITY ? -INFINITY : bias[J][k] - top[k / 2];
+    }
+    float most[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int J = 0; J < 4; J++)
+#pragma unroll
+      for (int k = 0; k < 4; k++) most[k / 2] = fmaxf(most[k / 2], s[J][k]);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 1));
+      most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 2));
+      if (most[h] > high[h] + kSlack || (high[h] == -INFINITY && most[h] > -INFINITY)) {
+        keep[h] = high[h] == -INFINITY ? 0.0f : ex2(high[h] - most[h]);
+        high[h] = most[h];
+        moved = true;
+      }
+    }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int t = 0; t < NB; t++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) o[t][k] *= keep[k / 2];
+      sum[0] *= keep[0];
+      sum[1] *= keep[1];
+    }
+    const float from[2] = {high[0] == -INFINITY ? 0.0f : high[0] - kLift, high[1] == -INFINITY ? 0.0f : high[1] - kLift};
+#pragma unroll
+    for (int v = 0; v < 2; v++) {
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int J = 0; J < 2; J++) {
+        const KeyInfo k0 = info[16 * v + 8 * J + c], k1 = info[16 * v + 8 * J + 4 + c];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const float x0 = ex2(s[2 * v + J][2 * h] - from[h]), x1 = ex2(s[2 * v + J][2 * h + 1] - from[h]);
+          sum[h] = fmaf(x1, k1.re, fmaf(x0, k0.re, sum[h]));
+          const float w0 = x0 * k0.f, w1 = x1 * k1.f;
+          hi[2 * J + h] = pack(w0, w1);
+          if (kTwo) {
+            const __half2 t2 = *reinterpret_cast<const __half2*>(&hi[2 * J + h]);
+            lo[2 * J + h] = pack(w0 - __low2float(t2), w1 - __high2float(t2));
+          }
+        }
+      }
+      value_products<D, FMT, kTwo>(hi, lo, cell + kCell * D, v, g, c, o);
+    }
+    __syncwarp();
+  }
+  copy_wait<0>();
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
+    sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
+    if (!u.mask || !live) top[h] = 0.0f;
+  }
+  const Stat st[2] = {{top[0], high[0], sum[0]}, {top[1], high[1], sum[1]}};
+
+  if (sh.kg == 1) {  // a row has one warp
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      if (!(h ? ok1 : ok0)) continue;
+      const uint64_t question = u.q0 + (h ? i1 : i0);
+      const uint32_t head = u.kv * group + (row + 8 * h) % group;
+      if (parts == 1) {
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+#pragma unroll
+          for (int t = 0; t < NB; t++) put<T, FMT>(a, question, head, (2 * c + k) * NB + t, o[t][2 * h + k], st[h].l);
+        if (c == 0) put_lse(a, question, head, st[h]);
+      } else {
+        float* p = part_of(a, question, head, part);
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+#pragma unroll
+          for (int t = 0; t < NB; t++) p[(2 * c + k) * NB + t] = o[t][2 * h + k];
+        if (c == 0) {
+          p[D] = st[h].b;
+          p[D + 1] = st[h].m;
+          p[D + 2] = st[h].l;
+        }
+      }
+    }
+    return;
+  }
+  // the warps of a row meet in shared memory: [warp][16 rows][D + 4]
+  __syncthreads();
+  float* join = reinterpret_cast<float*>(smem);
+  if (busy) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      float* p = join + (warp * 16 + g + 8 * h) * (D + 4);
+#pragma unroll
+      for (int k = 0; k < 2; k++)
+#pragma unroll
+        for (int t = 0; t < NB; t++) p[(2 * c + k) * NB + t] = o[t][2 * h + k];
+      if (c == 0) {
+        p[D] = st[h].b;
+        p[D + 1] = st[h].m;
+        p[D + 2] = st[h].l;
+      }
+    }
+  }
+  __syncthreads();
+  if (!busy) return;
+  // the team kgi of a unit's kg takes every kg-th row of its warps' 16
+  const uint32_t kgi = team % sh.kg, base = (team - kgi) * sh.mg + mi;
+  for (uint32_t r = kgi; r < 16; r += sh.kg) {
+    const uint32_t at = u.row0 + mi * 16 + r;
+    if (at >= u.rows) break;
+    Stat all{-INFINITY, -INFINITY, 0.0f};
+    for (uint32_t k = 0; k < sh.kg; k++) {
+      const float* p = join + ((base + k * sh.mg) * 16 + r) * (D + 4);
+      if (p[D + 1] > -INFINITY) all.b = fmaxf(all.b, p[D]);
+    }
+    for (uint32_t k = 0; k < sh.kg; k++) {
+      const float* p = join + ((base + k * sh.mg) * 16 + r) * (D + 4);
+      if (p[D + 1] > -INFINITY) all.m = fmaxf(all.m, (p[D] - all.b) + p[D + 1]);
+    }
+    float acc[D / 32] = {};
+    for (uint32_t k = 0; k < sh.kg; k++) {
+      const float* p = join + ((base + k * sh.mg) * 16 + r) * (D + 4);
+      const float x = weight_of(Stat{p[D], p[D + 1], p[D + 2]}, all.b, all.m);
+      all.l = fmaf(x, p[D + 2], all.l);
+#pragma unroll
+      for (int e = 0; e < D / 32; e++) acc[e] = fmaf(x, p[lane + 32 * e], acc[e]);
+    }
+    const uint64_t question = u.q0 + at / group;
+    const uint32_t head = u.kv * group + at % group;
+    if (parts == 1) {
+#pragma unroll
+      for (int e = 0; e < D / 32; e++) put<T, FMT>(a, question, head, lane + 32 * e, acc[e], all.l);
+      if (lane == 0) put_lse(a, question, head, all);
+    } else {
+      float* p = part_of(a, question, head, part);
+#pragma unroll
+      for (int e = 0; e < D / 32; e++) p[lane + 32 * e] = acc[e];
+      if (lane == 0) {
+        p[D] = all.b;
+        p[D + 1] = all.m;
+        p[D + 2] = all.l;
+      }
+    }
+  }
+}
+
+// The parts of every row of a cut sequence, joined: a CTA a question and head, the
+// parts shared among its warps, then the warps' sums in their order.
+template <typename T, int D, int FMT>
+__global__ __launch_bounds__(kThreads) void k_join(AttendArg a) {
+  __shared__ float s_o[kWarps][D];
+  __shared__ Stat s_stat[kWarps];
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // before any return: what follows this kernel follows the parts
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t question = blockIdx.x / a.a.heads, head = blockIdx.x % a.a.heads;
+  uint32_t seq = question, nth = 0;
+  if (a.a.off) {
+    if (question < a.a.off[0] || question >= a.a.off[a.t.seqs]) return;
+    seq = owner_of(a.a.off, a.t.seqs, question);
+    nth = uint32_t(question - a.a.off[seq]);
+  } else if (question >= a.t.seqs) {
+    return;
+  }
+  const uint32_t all = a.blocks ? a.block_count : (length_of(a.t, seq) + kPage - 1) / kPage;
+  const uint32_t parts = (all + a.chunk - 1) / a.chunk;
+  if (nth >= a.a.max_q || parts <= 1) return;
+  const float* p = part_of(a, question, head, 0);
+  Stat st{-INFINITY, -INFINITY, 0.0f};
+  float acc[D / 32] = {};
+  for (uint32_t k = warp; k < parts; k += kWarps) {
+    const float* x = p + uint64_t(k) * (D + 4);
+    const Stat other{x[D], x[D + 1], x[D + 2]};
+    if (other.m == -INFINITY) continue;
+    const float b = fmaxf(st.b, other.b);
+    const float m = fmaxf(st.m == -INFINITY ? -INFINITY : (st.b - b) + st.m, (other.b - b) + other.m);
+    const float keep = weight_of(st, b, m), add = weight_of(other, b, m);
+    st = Stat{b, m, fmaf(add, other.l, keep * st.l)};
+#pragma unroll
+    for (int e = 0; e < D / 32; e++) acc[e] = fmaf(add, x[lane + 32 * e], keep * acc[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < D / 32; e++) s_o[warp][lane + 32 * e] = acc[e];
+  if (lane == 0) s_stat[warp] = st;
+  __syncthreads();
+  if (threadIdx.x >= D) return;
+  Stat sum{-INFINITY, -INFINITY, 0.0f};
+  float o = 0.0f;
+  for (int k = 0; k < kWarps; k++)
+    if (s_stat[k].m > -INFINITY) sum.b = fmaxf(sum.b, s_stat[k].b);
+  for (int k = 0; k < kWarps; k++)
+    if (s_stat[k].m > -INFINITY) sum.m = fmaxf(sum.m, (s_stat[k].b - sum.b) + s_stat[k].m);
+  for (int k = 0; k < kWarps; k++) {
+    const float x = weight_of(s_stat[k], sum.b, sum.m);
+    sum.l = fmaf(x, s_stat[k].l, sum.l);
+    o = fmaf(x, s_o[k][threadIdx.x], o);
+  }
+  put<T, FMT>(a, question, head, threadIdx.x, o, sum.l);
+  if (threadIdx.x == 0) put_lse(a, question, head, sum);
+}
+
+inline Shape shape_of(const AttendArg& a, int sms) {
+  const uint32_t group = a.a.heads / a.c.heads;
+  const uint64_t rows = a.blocks || a.block_count ? group : uint64_t(a.a.max_q) * group;
+  const uint64_t units = a.blocks || a.block_count ? a.a.questions : a.t.seqs;
+  const uint32_t blocks = a.block_count ? a.block_count : (a.t.max_len + kPage - 1) / kPage;
+  Shape sh{};
+  sh.mg = rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 8;
+  sh.chunks = uint32_t((rows + 16 * sh.mg - 1) / (16 * sh.mg));
+  sh.items = units * sh.chunks * a.c.heads;
+  // short sequences of many units: a team a unit; else the CTA's teams share one
+  sh.kg = blocks <= 8 && sh.items * sh.mg >= uint64_t(sms) * 16 ? 1 : kWarps / sh.mg;
+  sh.hg = kWarps / (sh.mg * sh.kg);
+  return sh;
+}
+
+template <typename T, int D, int FMT>
+cudaError_t attend_tile(const AttendArg& a, int sms, cudaStream_t s, uint64_t* launches) {
+  const Shape sh = shape_of(a, sms);
+  const uint64_t ctas = (sh.items + sh.hg - 1) / sh.hg;
+  if (ctas == 0) return cudaSuccess;
+  if (ctas > 0x7fffffffull) return cudaErrorInvalidConfiguration;
+  const size_t ring = size_t(kWarps / sh.mg) * stages(D) * cell_bytes(D);
+  const size_t join = sh.kg > 1 ? size_t(kWarps) * 16 * (D + 4) * 4 : 0;
+  k_attend<T, D, FMT><<<dim3(unsigned(ctas), a.splits), kThreads, std::max(ring, join), s>>>(a, sh);
+  ++*launches;
+  cudaError_t e = cudaGetLastError();
+  if (e || a.splits == 1) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(a.a.questions * a.a.heads);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute early[1];
+  early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = early;
+  cfg.numAttrs = 1;
+  ++*launches;
+  return cudaLaunchKernelEx(&cfg, k_join<T, D, FMT>, a);
+}
+
+// --- pointer scores --------------------------------------------------------------
+
+// A warp a cell of a sequence and 16 of its questions at a time; the tile passes
+// through shared memory so that masks are read and scores written 32 to a row.
+template <typename T, int D, int FMT>
+__global__ __launch_bounds__(kThreads) void k_scores(ScoreArg a, uint32_t chunks, uint32_t cells) {
+  constexpr int S = 3, KB = int(kCell) * D, CB = KB + int(kCell) * 4;  // keys and their scales
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float s_tile[kWarps][16][kCell + 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+  const uint32_t seq = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
+  const uint64_t q0 = a.a.off ? a.a.off[seq] : seq, q1 = a.a.off ? a.a.off[seq + 1] : seq + 1;
+  const uint32_t count = uint32_t(q1 - q0), rows = uint32_t(min(uint64_t(min(count, a.a.max_q)), a.a.questions > q0 ? a.a.questions - q0 : 0));
+  const uint32_t row0 = chunk * 16;
+  if (row0 >= rows) return;
+  const uint64_t stride = (a.off[seq + 1] - a.off[seq]) / count;
+  const uint32_t len = uint32_t(min(uint64_t(length_of(a.t, seq)), stride));
+  const uint64_t end = (stride + kCell - 1) / kCell;  // cells of the row, those behind the bank's end included
+  const uint64_t at0 = a.off[seq] + row0 * stride;
+  const uint32_t n_rows = min(16u, rows - row0);
+
+  Walk w{};
+  w.table = a.t.table + uint64_t(seq) * a.t.pitch;
+  w.blocks = (len + kPage - 1) / kPage;
+  w.pages = a.c.pages;
+  w.b0 = blockIdx.y * cells / 2;
+  const uint64_t c0 = uint64_t(blockIdx.y) * cells;
+  if (c0 >= end) return;
+  w.cells = uint32_t(blockIdx.y + 1 == gridDim.y ? end - c0 : min(uint64_t(cells), end - c0));  // the last takes what the table does not bound
+  w.first = warp;
+  w.step = kWarps;
+  const uint32_t n = w.count();
+  QTile<T, D> q;
+  const T* base = static_cast<const T*>(a.a.q) + (q0 + row0) * a.a.pitch;
+  q.load(uint32_t(g) < n_rows ? base + g * a.a.pitch : nullptr, uint32_t(g + 8) < n_rows ? base + (g + 8) * a.a.pitch : nullptr, c, a.scale);
+  if (n == 0) return;
+  uint8_t* ring = smem + warp * (S * CB);
+  auto issue = [&](uint32_t i, uint32_t page) {
+    if (page != kNone) {
+      const uint8_t* src = cell_of<D>(a.c, page, 0, w.half(i));
+      uint8_t* dst = ring + (i % S) * CB;
+#pragma unroll
+      for (int k = 0; k < KB / 512; k++) copy16(dst + 16 * (k * 32 + lane), src + 16 * (k * 32 + lane));
+      if (lane < 8) copy16(dst + KB + 16 * lane, src + 2 * KB + 16 * lane);
+    }
+    copy_commit();
+  };
+  w.begin();
+#pragma unroll
+  for (uint32_t i = 0; i + 1 < S; i++) {
+    const uint32_t page = w.page_of(0, i);
+    issue(i, i < n ? page : kNone);
+  }
+  float (*tile)[kCell + 1] = s_tile[warp];
+  for (uint32_t i = 0; i < n; i++) {
+    w.advance(i);
+    copy_wait<S - 2>();
+    __syncwarp();
+    const uint32_t next = w.page_of(i, S - 1), page = w.page_of(i, 0);
+    issue(i + S - 1, i + S - 1 < n ? next : kNone);
+    const uint64_t pos = (c0 + w.first + uint64_t(w.step) * i) * kCell + lane;
+    float unit = 0.0f;
+    if (page != kNone) {
+      const uint8_t* cell = ring + (i % S) * CB;
+      float s[4][4];
+      key_products<T, D, FMT>(q, cell, g, c, s);
+      unit = reinterpret_cast<const float*>(cell + KB)[lane] * widened<FMT>();
+#pragma unroll
+      for (int J = 0; J < 4; J++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) tile[g + 8 * (k / 2)][8 * J + 4 * (k & 1) + c] = s[J][k] * q.unit[k / 2];
+    }
+    __syncwarp();
+    if (pos < stride) {
+      const bool held = page != kNone && pos < len;
+      float* out = a.scores + at0 + pos;
+      const float* mask = a.mask ? a.mask + at0 + pos : nullptr;
+      for (uint32_t r = 0; r < n_rows; r++) {
+        const float bias = mask ? mask[r * stride] : 0.0f;
+        out[r * stride] = held && bias > kBlocked ? fmaf(tile[r][lane], unit, fminf(bias, -kBlocked)) : kShut;
+      }
+    }
+    __syncwarp();
+  }
+  copy_wait<0>();
+}
+
+template <typename T, int D, int FMT>
+cudaError_t scores_tile(const ScoreArg& a, int sms, cudaStream_t s, uint64_t* launches) {
+  const uint32_t chunks = (a.a.max_q + 15) / 16;
+  const uint64_t ctas = uint64_t(a.t.seqs) * chunks;
+  if (ctas > 0x7fffffffull) return cudaErrorInvalidConfiguration;
+  // rows may be longer than their bank: max_len does not bound them, the table does
+  const uint64_t all = uint64_t(a.t.pitch) * 2;
+  const uint64_t want = std::max<uint64_t>(1, uint64_t(sms) * 12 / std::max<uint64_t>(1, ctas));
+  uint64_t cells = std::max<uint64_t>(kWarps * 2, (all + want - 1) / want);
+  cells = (cells + kWarps * 2 - 1) / (kWarps * 2) * (kWarps * 2);
+  const uint64_t parts = std::max<uint64_t>(1, (all + cells - 1) / cells);
+  if (parts > 65535) return cudaErrorInvalidConfiguration;
+  const size_t smem = size_t(kWarps) * 3 * (kCell * D + kCell * 4);
+  k_scores<T, D, FMT><<<dim3(unsigned(ctas), unsigned(parts)), kThreads, smem, s>>>(a, chunks, uint32_t(cells));
+  ++*launches;
+  return cudaGetLastError();
+}
+
+// --- by type -----------------------------------------------------------------------
+
+template <typename T, int D, int FMT>
+cudaError_t prepare_tile() {
+  const int ring = int(kWarps * stages(D) * cell_bytes(D)), join = kWarps * 16 * (D + 4) * 4;
+  cudaError_t e = cudaFuncSetAttribute(k_attend<T, D, FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize, std::max(ring, join));
+  if (e) return e;
+  return cudaFuncSetAttribute(k_scores<T, D, FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              int(kWarps * 3 * (kCell * D + kCell * 4)));
+}
+
+template <typename T>
+cudaError_t prepare_as() {
+  cudaError_t e;
+  if ((e = prepare_tile<T, 32, kI8>()) || (e = prepare_tile<T, 32, kE4M3>()) || (e = prepare_tile<T, 64, kI8>()) ||
+      (e = prepare_tile<T, 64, kE4M3>()) || (e = prepare_tile<T, 128, kI8>()) || (e = prepare_tile<T, 128, kE4M3>()))
+    return e;
+  return cudaSuccess;
+}
+
+template <typename T>
+cudaError_t attend_as(const AttendArg& a, int sms, cudaStream_t s, uint64_t* launches) {
+  const bool i8 = a.c.format == kI8;
+  if (a.c.dim == 32) return i8 ? attend_tile<T, 32, kI8>(a, sms, s, launches) : attend_tile<T, 32, kE4M3>(a, sms, s, launches);
+  if (a.c.dim == 64) return i8 ? attend_tile<T, 64, kI8>(a, sms, s, launches) : attend_tile<T, 64, kE4M3>(a, sms, s, launches);
+  return i8 ? attend_tile<T, 128, kI8>(a, sms, s, launches) : attend_tile<T, 128, kE4M3>(a, sms, s, launches);
+}
+
+template <typename T>
+cudaError_t scores_as(const ScoreArg& a, int sms, cudaStream_t s, uint64_t* launches) {
+  const bool i8 = a.c.format == kI8;
+  if (a.c.dim == 32) return i8 ? scores_tile<T, 32, kI8>(a, sms, s, launches) : scores_tile<T, 32, kE4M3>(a, sms, s, launches);
+  if (a.c.dim == 64) return i8 ? scores_tile<T, 64, kI8>(a, sms, s, launches) : scores_tile<T, 64, kE4M3>(a, sms, s, launches);
+  return i8 ? scores_tile<T, 128, kI8>(a, sms, s, launches) : scores_tile<T, 128, kE4M3>(a, sms, s, launches);
+}
+
+}  // namespace
+}  // namespace cache
+}  // namespace kc

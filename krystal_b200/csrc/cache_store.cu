@@ -375,7 +375,7 @@ cudaError_t launch_blocks(const BlockArg& a, int, cudaStream_t s, uint64_t* laun
   return cudaGetLastError();
 }
 
-cudaError_t prepare() {
+cudaError_t prepare_store() {
   cudaError_t e;
   const int most = int(kMaxBlocks) * 8;
   if ((e = cudaFuncSetAttribute(k_blocks<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, most)) ||

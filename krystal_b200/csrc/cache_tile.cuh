@@ -1,0 +1,236 @@
+// cache_tile.cuh — a warp's 16 question rows against a cell of 32 cached keys on
+// the tensor cores: fragments of questions and codes, and what a cell needs of
+// its scales. (mma.sync m16n8k16: a serving call has few question rows a key, so
+// that the cache's bytes bound it, and 8-bit codes become f16 in registers, where
+// these instructions take their operands; 5th-generation ones would need them
+// written back to shared memory for tiles of 64 or 128 rows that are mostly empty.)
+//
+// Exactness. Codes are exact in f16. A question row is divided by a power of two
+// that brings its largest element into [1, 2); 16-bit questions are then exact
+// (bits 2^-25 below the largest aside), f32 ones are the sum of two f16 (22 bits,
+// two products). Products accumulate in f32.
+#pragma once
+#include "cache.cuh"
+
+namespace kc {
+namespace cache {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// D = A B + D, A [16][16] and B [16][8] f16, D f32. Lane (g, c) = (lane / 4,
+// lane % 4) holds A's (g, 2c..), (g + 8, 2c..), (g, 2c + 8..), (g + 8, 2c + 8..),
+// B's (2c.., g), (2c + 8.., g) and D's (g, 2c), (g, 2c + 1), (g + 8, 2c), (g + 8, 2c + 1).
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Bytes 0 and 1 (HIGH: 2 and 3) of a word of codes as two f16. i8: 0x6400 + byte
+// is 1024 + byte, less 1152. e4m3: exponent and mantissa moved to an f16's place
+// are the value times 2^-8 (subnormals too); callers multiply it back.
+template <int FMT, bool HIGH>
+__device__ __forceinline__ uint32_t widen(uint32_t w) {
+  if (FMT == kI8) {
+    const uint32_t x = __byte_perm(w, 0x64646464u, HIGH ? 0x4342 : 0x4140);
+    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2{__ushort_as_half(0x6480), __ushort_as_half(0x6480)});
+    return *reinterpret_cast<const uint32_t*>(&y);
+  }
+  const uint32_t x = __byte_perm(w, 0u, HIGH ? 0x3424 : 0x1404);
+  return ((x >> 1) & 0x3f803f80u) | (x & 0x80008000u);
+}
+template <int FMT>
+__device__ __forceinline__ constexpr float widened() { return FMT == kI8 ? 1.0f : 256.0f; }
+
+// 2^x, x an integer in [-126, 127] given as its biased exponent.
+__device__ __forceinline__ float pow2_biased(uint32_t e) { return __uint_as_float(e << 23); }
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The A fragments of a warp's 16 question rows. The dimensions' order within a
+// fragment is the keys': lane c's bytes of a key row, 4 a fragment.
+template <typename T, int D>
+struct QTile {
+  static constexpr bool kTwo = sizeof(T) == 4;  // f32: two f16 a value
+  static constexpr int kSteps = D / 16;
+  uint32_t hi[kSteps][4], lo[kTwo ? kSteps : 1][4];
+  float unit[2];  // what a product of rows g and g + 8 is multiplied by
+
+  // Dimension of element i (0..3) of lane c's piece of fragment s.
+  static __device__ __forceinline__ int dim(int s, int c) {
+    return D == 32 ? 8 * c + 4 * s : D == 64 ? 16 * c + 4 * s : s < 4 ? 16 * c + 4 * s : 64 + 16 * c + 4 * (s - 4);
+  }
+
+  // rows: the two rows of this lane, null where there is none. factor multiplies every score.
+  __device__ __forceinline__ void load(const T* r0, const T* r1, int c, float factor) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const T* r = h ? r1 : r0;
+      float x[kSteps][4], top = 0.0f;
+#pragma unroll
+      for (int s = 0; s < kSteps; s++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          x[s][i] = r ? to_f32(r[dim(s, c) + i]) * (kTwo ? factor : 1.0f) : 0.0f;
+          top = fmaxf(top, fabsf(x[s][i]));
+        }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const uint32_t e = min(max(__float_as_uint(top) >> 23, 1u), 253u);
+      const float down = pow2_biased(254u - e);
+      unit[h] = pow2_biased(e) * (kTwo ? 1.0f : factor);
+#pragma unroll
+      for (int s = 0; s < kSteps; s++)
+#pragma unroll
+        for (int p = 0; p < 2; p++) {
+          const float y0 = x[s][2 * p] * down, y1 = x[s][2 * p + 1] * down;
+          hi[s][2 * p + h] = pack(y0, y1);
+          if (kTwo) {
+            const __half2 top2 = *reinterpret_cast<const __half2*>(&hi[s][2 * p + h]);
+            lo[kTwo ? s : 0][2 * p + h] = pack(y0 - __low2float(top2), y1 - __high2float(top2));
+          }
+        }
+    }
+  }
+};
+
+// s[J] += the 16 rows times the 8 keys of group J of the cell at `keys`. Lane
+// column n of group J stands for row 8 J + n / 2 + 4 (n % 2): the pairs of
+// neighbouring columns that a lane accumulates are then the rows (a, a + 4) that
+// value() pairs, and the quarter-warp's reads fall on different banks.
+template <typename T, int D, int FMT>
+__device__ __forceinline__ void key_products(const QTile<T, D>& q, const uint8_t* keys, int g, int c, float (&s)[4][4]) {
+#pragma unroll
+  for (int J = 0; J < 4; J++) {
+    const uint32_t row = 8 * J + (g >> 1) + ((g & 1) << 2);
+    uint32_t w[D / 16];
+    if constexpr (D == 32) {
+      const uint2 v = *reinterpret_cast<const uint2*>(keys + key_at<D>(row, 8 * c));
+      w[0] = v.x; w[1] = v.y;
+    } else {
+#pragma unroll
+      for (int p = 0; p < D / 64; p++) {
+        const uint4 v = *reinterpret_cast<const uint4*>(keys + key_at<D>(row, 64 * p + 16 * c));
+        w[4 * p] = v.x; w[4 * p + 1] = v.y; w[4 * p + 2] = v.z; w[4 * p + 3] = v.w;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) s[J][i] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < D / 16; k++) {
+      const uint32_t b0 = widen<FMT, false>(w[k]), b1 = widen<FMT, true>(w[k]);
+      mma(s[J], q.hi[k], b0, b1);
+      if constexpr (QTile<T, D>::kTwo) mma(s[J], q.lo[k], b0, b1);
+    }
+  }
+}
+
+// o += the weights of 16 rows for the 16 keys of half u of a cell (A fragments,
+// hi and for f32 questions lo) times their values. Column n of tile t of o stands
+// for dimension n * (D / 8) + t.
+template <int D, int FMT, bool TWO>
+__device__ __forceinline__ void value_products(const uint32_t (&hi)[4], const uint32_t (&lo)[4], const uint8_t* values, int u,
+                                               int g, int c, float (&o)[D / 8][4]) {
+  constexpr int W = D / 32;  // words of 4 dimensions that a lane reads of each of its rows
+  uint32_t w[4][W];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const uint8_t* p = values + value_at<D>(16 * u + c + 4 * i, 4 * W * g);
+    if constexpr (W == 1) {
+      w[i][0] = *reinterpret_cast<const uint32_t*>(p);
+    } else if constexpr (W == 2) {
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
+      w[i][0] = v.x; w[i][1] = v.y;
+    } else {
+      const uint4 v = *reinterpret_cast<const uint4*>(p);
+      w[i][0] = v.x; w[i][1] = v.y; w[i][2] = v.z; w[i][3] = v.w;
+    }
+  }
+#pragma unroll
+  for (int x = 0; x < W; x++)
+#pragma unroll
+    for (int y = 0; y < 2; y++) {  // bytes 2 y and 2 y + 1 of the word
+      const uint32_t p0 = __byte_perm(w[0][x], w[1][x], y ? 0x7362 : 0x5140);
+      const uint32_t p1 = __byte_perm(w[2][x], w[3][x], y ? 0x7362 : 0x5140);
+      const uint32_t b00 = widen<FMT, false>(p0), b01 = widen<FMT, false>(p1);
+      const uint32_t b10 = widen<FMT, true>(p0), b11 = widen<FMT, true>(p1);
+      mma(o[4 * x + 2 * y], hi, b00, b01);
+      mma(o[4 * x + 2 * y + 1], hi, b10, b11);
+      if constexpr (TWO) {
+        mma(o[4 * x + 2 * y], lo, b00, b01);
+        mma(o[4 * x + 2 * y + 1], lo, b10, b11);
+      }
+    }
+}
+
+// 16 bytes, global to shared, asynchronous.
+__device__ __forceinline__ void copy16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+               ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// The warps of a team meet (named barriers 1..8; a team of one needs none).
+__device__ __forceinline__ void meet(uint32_t team, uint32_t warps) {
+  if (warps == 1) __syncwarp();
+  else asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(warps * 32) : "memory");
+}
+
+// The cells a team walks over: cell first + step * i of the blocks from b0 on,
+// 32 at a time in the lanes' registers and 32 ahead, so that no copy waits for a
+// page number.
+struct Walk {
+  const uint32_t* table;  // the sequence's pages
+  const uint32_t* list;   // the question's blocks, or null: every block in turn
+  uint32_t blocks, pages; // of the sequence; of the cache
+  uint32_t b0, cells, first, step;
+  uint32_t block[2], page[2];
+
+  __device__ __forceinline__ uint32_t count() const { return cells > first ? (cells - first + step - 1) / step : 0; }
+  __device__ __forceinline__ uint32_t half(uint32_t i) const { return (first + step * i) & 1u; }
+  __device__ __forceinline__ void fetch(uint32_t batch, int which) {
+    const uint32_t cell = first + step * (batch * 32 + (threadIdx.x & 31));
+    uint32_t b = kNone, p = kNone;
+    if (cell < cells) {
+      b = b0 + (cell >> 1);
+      if (list) b = list[b];
+      if (b < blocks) p = table[b];
+      if (p >= pages) p = kNone;
+    }
+    block[which] = b;
+    page[which] = p;
+  }
+  __device__ __forceinline__ void begin() {
+    fetch(0, 0);
+    fetch(1, 1);
+  }
+  // At the start of step i: the registers move on with it.
+  __device__ __forceinline__ void advance(uint32_t i) {
+    if (i && (i & 31u) == 0) {
+      block[0] = block[1];
+      page[0] = page[1];
+      fetch(i / 32 + 1, 1);
+    }
+  }
+  // The page of step i + ahead (kNone: none), where step i is the current one.
+  __device__ __forceinline__ uint32_t page_of(uint32_t i, uint32_t ahead) const {
+    const uint32_t j = (i & 31u) + ahead;
+    return __shfl_sync(0xffffffffu, j < 32 ? page[0] : page[1], j & 31u);
+  }
+  __device__ __forceinline__ uint32_t block_of(uint32_t i) const { return __shfl_sync(0xffffffffu, block[0], i & 31u); }
+};
+
+}  // namespace cache
+}  // namespace kc
