@@ -29,7 +29,10 @@ constexpr int kThreads = 256, kWarps = 8;
 constexpr float kLift = 8.0f, kSlack = 6.0f;
 constexpr int kLeastExp = -80;  // value scales below it keep their digits in f_j; l stays below 2^128
 
-__host__ __device__ constexpr int stages(int dim) { return dim == 32 ? 4 : 3; }
+// Cells a ring holds; a masked call's has the mask entries of each warp's 16 rows
+// beside them, 36 floats apart so that 8 rows of a column lie on different banks.
+constexpr int kMaskPitch = 36, kMaskBytes = 16 * kMaskPitch * 4;
+__host__ __device__ constexpr int stages(int dim, bool masked) { return masked ? (dim == 32 ? 3 : 2) : dim == 32 ? 4 : 3; }
 
 // What a warp needs of one key of a cell: score = product * a * unit + e.
 struct KeyInfo {
@@ -109,7 +112,7 @@ __device__ __forceinline__ float weight_of(const Stat& s, float b, float m) {
 
 template <typename T, int FMT>
 __device__ __forceinline__ void put(const AttendArg& a, uint64_t question, uint32_t head, uint32_t dim, float o, float l) {
-  static_cast<T*>(a.out)[question * a.out_pitch + uint64_t(head) * a.c.dim + dim] = from_f32<T>(l > 0.0f ? o / l * widened<FMT>() : 0.0f);
+  static_cast<T*>(a.out)[question * a.out_pitch + uint64_t(head) * a.c.dim + dim] = from_f32<T>(l > 0.0f ? o * (widened<FMT>() / l) : 0.0f);
 }
 __device__ __forceinline__ void put_lse(const AttendArg& a, uint64_t question, uint32_t head, const Stat& s) {
   if (a.lse) a.lse[question * a.a.heads + head] = s.l > 0.0f ? (s.b + s.m - kLift) * kLn2 + logf(s.l) : -INFINITY;
@@ -120,9 +123,24 @@ __device__ __forceinline__ float* part_of(const AttendArg& a, uint64_t question,
   return a.work + ((question * a.a.heads + head) * a.splits + part) * (a.c.dim + 4);
 }
 
-template <typename T, int D, int FMT>
+// N values of a row, one after another.
+template <typename T, int N>
+__device__ __forceinline__ void put_run(T* dst, const float (&x)[N], bool wide) {
+  if (wide) {
+    T y[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) y[i] = from_f32<T>(x[i]);
+#pragma unroll
+    for (int i = 0; i < int(N * sizeof(T) / 16); i++) reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(y)[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++) dst[i] = from_f32<T>(x[i]);
+  }
+}
+
+template <typename T, int D, int FMT, bool MASKED>
 __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void k_attend(AttendArg a, Shape sh) {
-  constexpr int S = stages(D), CB = int(cell_bytes(D)), NB = D / 8;
+  constexpr int S = stages(D, MASKED), CB = int(cell_bytes(D)), NB = D / 8;
   constexpr bool kTwo = sizeof(T) == 4;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ KeyInfo s_info[kWarps][kCell];
@@ -160,15 +178,26 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void k_attend(AttendArg
            ok1 ? base + (u.q0 + i1) * a.a.pitch + (u.kv * group + (row + 8) % group) * uint64_t(D) : nullptr, c,
            a.scale * kLog2e);
   }
-  const float* mask0 = u.mask && ok0 ? u.mask + i0 * u.stride : nullptr;
-  const float* mask1 = u.mask && ok1 ? u.mask + i1 * u.stride : nullptr;
-
   uint8_t* ring = smem + team * (S * CB);
-  auto issue = [&](uint32_t i, uint32_t page) {
+  uint8_t* biases = smem + kWarps / sh.mg * (S * CB) + warp * (S * kMaskBytes);  // a masked call's
+  __shared__ uint64_t s_mask[MASKED ? kWarps : 1][16];  // where the rows' masks begin
+  const uint32_t open_end = MASKED ? uint32_t(min(uint64_t(u.len), u.stride)) : u.len;
+  const uint32_t n_rows = busy ? min(16u, u.rows - (u.row0 + mi * 16)) : 0;
+  if (MASKED) {
+    if (lane < 16) s_mask[warp][lane] = uint64_t(u.row0 + mi * 16 + lane) / group * u.stride;
+    __syncwarp();
+  }
+  auto issue = [&](uint32_t i, uint32_t page, uint32_t block) {
     if (page != kNone) {
       const uint8_t* src = cell_of<D>(a.c, page, u.kv, w.half(i));
       uint8_t* dst = ring + (i % S) * CB;
       for (uint32_t k = mi * 32 + lane; k < CB / 16; k += sh.mg * 32) copy16(dst + 16 * k, src + 16 * k);
+      if (MASKED) {
+        const uint64_t pos = uint64_t(block) * kPage + w.half(i) * kCell + lane;
+        uint8_t* to = biases + (i % S) * kMaskBytes + 4 * lane;
+        if (pos < open_end)
+          for (uint32_t r = 0; r < n_rows; r++) copy4(to + r * (4 * kMaskPitch), u.mask + s_mask[warp][r] + pos);
+      }
     }
     copy_commit();
   };
@@ -182,8 +211,8 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void k_attend(AttendArg
   if (n) {
 #pragma unroll
     for (uint32_t i = 0; i + 1 < S; i++) {
-      const uint32_t page = w.page_of(0, i);
-      issue(i, i < n ? page : kNone);
+      const uint32_t page = w.page_of(0, i), block = w.block_of(0, i);
+      issue(i, i < n ? page : kNone, block);
     }
   }
   KeyInfo* info = s_info[warp];
@@ -191,15 +220,15 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void k_attend(AttendArg
     w.advance(i);
     copy_wait<S - 2>();
     meet(team, sh.mg);
-    const uint32_t next = w.page_of(i, S - 1), page = w.page_of(i, 0), block = w.block_of(i);
-    issue(i + S - 1, i + S - 1 < n ? next : kNone);
+    const uint32_t next = w.page_of(i, S - 1), page = w.page_of(i, 0), block = w.block_of(i, 0);
+    issue(i + S - 1, i + S - 1 < n ? next : kNone, MASKED ? w.block_of(i, S - 1) : 0);
     if (!busy || page == kNone) continue;
     const uint8_t* cell = ring + (i % S) * CB;
     const uint64_t pos = uint64_t(block) * kPage + w.half(i) * kCell;
     {
       const float* scales = reinterpret_cast<const float*>(cell + 2 * kCell * D);
       const float vs = scales[kCell + lane];
-      const bool open = pos + lane < u.len && (!u.mask || pos + lane < u.stride);
+      const bool open = pos + lane < open_end;
       const uint32_t e = max(__float_as_uint(vs) >> 23, uint32_t(127 + kLeastExp)), es = min(e, 253u);
       KeyInfo k;
       k.re = pow2_biased(254u - es);
@@ -222,33 +251,33 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void k_attend(AttendArg
       }
     float keep[2] = {1.0f, 1.0f};
     bool moved = false;
-    if (u.mask) {
-      float bias[4][4], most[2] = {-INFINITY, -INFINITY};
+    if (MASKED) {
+      // entries are read twice rather than kept: 16 registers more would spill
+      const float* bias = reinterpret_cast<const float*>(biases + (i % S) * kMaskBytes) + g * kMaskPitch + c;
+      auto entry = [&](int J, int k) {
+        const float x = bias[(k / 2) * 8 * kMaskPitch + 8 * J + 4 * (k & 1)];
+        return s[J][k] > -INFINITY && x > kBlocked ? fminf(x, -kBlocked) * kLog2e : -INFINITY;
+      };
+      float most[2] = {-INFINITY, -INFINITY};
 #pragma unroll
       for (int J = 0; J < 4; J++)
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-          const uint64_t at = pos + 8 * J + 4 * (k & 1) + c;
-          const float* m = k < 2 ? mask0 : mask1;
-          const float x = m && at < u.stride && at < u.len ? m[at] : -INFINITY;
-          bias[J][k] = x > kBlocked ? fminf(x, -kBlocked) * kLog2e : -INFINITY;
-          most[k / 2] = fmaxf(most[k / 2], bias[J][k]);
-        }
+        for (int k = 0; k < 4; k++) most[k / 2] = fmaxf(most[k / 2], entry(J, k));
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 1));
         most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 2));
         const float was = top[h];
         top[h] = fmaxf(was, most[h]);
-        if (was != top[h]) {  // what is summed so far was measured from the former one
-          high[h] += was - top[h];
-          if (was == -INFINITY) high[h] = -INFINITY;
-        }
+        if (was != top[h]) high[h] = was == -INFINITY ? -INFINITY : high[h] + (was - top[h]);  // measured from the new one
       }
 #pragma unroll
       for (int J = 0; J < 4; J++)
 #pragma unroll
-        for (int k = 0; k < 4; k++) s[J][k] += bias[J][k] == -INFINITY ? -INFINITY : bias[J][k] - top[k / 2];
+        for (int k = 0; k < 4; k++) {
+          const float x = entry(J, k);
+          s[J][k] = x > -INFINITY ? s[J][k] + (x - top[k / 2]) : -INFINITY;
+        }
     }
     float most[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -301,33 +330,28 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void k_attend(AttendArg
   for (int h = 0; h < 2; h++) {
     sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
     sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
-    if (!u.mask || !live) top[h] = 0.0f;
+    if (!MASKED) top[h] = 0.0f;
   }
   const Stat st[2] = {{top[0], high[0], sum[0]}, {top[1], high[1], sum[1]}};
 
   if (sh.kg == 1) {  // a row has one warp
+    const bool wide = (reinterpret_cast<uintptr_t>(a.out) | a.out_pitch * sizeof(T)) % 16 == 0;
 #pragma unroll
     for (int h = 0; h < 2; h++) {
       if (!(h ? ok1 : ok0)) continue;
       const uint64_t question = u.q0 + (h ? i1 : i0);
       const uint32_t head = u.kv * group + (row + 8 * h) % group;
+      const float unit = parts > 1 ? 1.0f : st[h].l > 0.0f ? widened<FMT>() / st[h].l : 0.0f;
+      float run[2 * NB];
+#pragma unroll
+      for (int k = 0; k < 2 * NB; k++) run[k] = o[k % NB][2 * h + k / NB] * unit;
       if (parts == 1) {
-#pragma unroll
-        for (int k = 0; k < 2; k++)
-#pragma unroll
-          for (int t = 0; t < NB; t++) put<T, FMT>(a, question, head, (2 * c + k) * NB + t, o[t][2 * h + k], st[h].l);
+        put_run(static_cast<T*>(a.out) + question * a.out_pitch + head * uint64_t(D) + 2 * c * NB, run, wide);
         if (c == 0) put_lse(a, question, head, st[h]);
       } else {
         float* p = part_of(a, question, head, part);
-#pragma unroll
-        for (int k = 0; k < 2; k++)
-#pragma unroll
-          for (int t = 0; t < NB; t++) p[(2 * c + k) * NB + t] = o[t][2 * h + k];
-        if (c == 0) {
-          p[D] = st[h].b;
-          p[D + 1] = st[h].m;
-          p[D + 2] = st[h].l;
-        }
+        put_run(p + 2 * c * NB, run, true);
+        if (c == 0) *reinterpret_cast<float4*>(p + D) = make_float4(st[h].b, st[h].m, st[h].l, 0.0f);
       }
     }
     return;
@@ -393,58 +417,89 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void k_attend(AttendArg
   }
 }
 
-// The parts of every row of a cut sequence, joined: a CTA a question and head, the
-// parts shared among its warps, then the warps' sums in their order.
+// The parts of every row of a cut sequence, joined: `per` warps a question and
+// head, each over its share of the parts, 32 at a time (a lane a part for the
+// weights, then a lane a dimension), then the warps' sums in their order.
 template <typename T, int D, int FMT>
-__global__ __launch_bounds__(kThreads) void k_join(AttendArg a) {
+__global__ __launch_bounds__(kThreads) void k_join(AttendArg a, uint32_t per) {
   __shared__ float s_o[kWarps][D];
   __shared__ Stat s_stat[kWarps];
   asm volatile("griddepcontrol.wait;" ::: "memory");  // before any return: what follows this kernel follows the parts
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t question = blockIdx.x / a.a.heads, head = blockIdx.x % a.a.heads;
+  const uint32_t item = blockIdx.x * (kWarps / per) + warp / per, share = warp % per;
+  const uint32_t question = item / a.a.heads, head = item % a.a.heads;
   uint32_t seq = question, nth = 0;
+  bool live = question < a.a.questions;
   if (a.a.off) {
-    if (question < a.a.off[0] || question >= a.a.off[a.t.seqs]) return;
-    seq = owner_of(a.a.off, a.t.seqs, question);
-    nth = uint32_t(question - a.a.off[seq]);
-  } else if (question >= a.t.seqs) {
-    return;
+    live = live && question >= a.a.off[0] && question < a.a.off[a.t.seqs];
+    if (live) {
+      seq = owner_of(a.a.off, a.t.seqs, question);
+      nth = uint32_t(question - a.a.off[seq]);
+    }
   }
-  const uint32_t all = a.blocks ? a.block_count : (length_of(a.t, seq) + kPage - 1) / kPage;
+  live = live && seq < a.t.seqs && nth < a.a.max_q;
+  const uint32_t all = !live ? 0 : a.blocks ? a.block_count : (length_of(a.t, seq) + kPage - 1) / kPage;
   const uint32_t parts = (all + a.chunk - 1) / a.chunk;
-  if (nth >= a.a.max_q || parts <= 1) return;
-  const float* p = part_of(a, question, head, 0);
+  live = live && parts > 1;
   Stat st{-INFINITY, -INFINITY, 0.0f};
   float acc[D / 32] = {};
-  for (uint32_t k = warp; k < parts; k += kWarps) {
-    const float* x = p + uint64_t(k) * (D + 4);
-    const Stat other{x[D], x[D + 1], x[D + 2]};
-    if (other.m == -INFINITY) continue;
-    const float b = fmaxf(st.b, other.b);
-    const float m = fmaxf(st.m == -INFINITY ? -INFINITY : (st.b - b) + st.m, (other.b - b) + other.m);
-    const float keep = weight_of(st, b, m), add = weight_of(other, b, m);
-    st = Stat{b, m, fmaf(add, other.l, keep * st.l)};
+  if (live) {
+    const float* p = part_of(a, question, head, 0);
+    for (uint32_t k0 = share * 32; k0 < parts; k0 += per * 32) {
+      const uint32_t mine = k0 + lane;
+      Stat other{-INFINITY, -INFINITY, 0.0f};
+      if (mine < parts) {
+        const float4 v = *reinterpret_cast<const float4*>(p + uint64_t(mine) * (D + 4) + D);
+        other = Stat{v.y > -INFINITY ? v.x : -INFINITY, v.y, v.z};
+      }
+      float b = fmaxf(st.b, other.b);
 #pragma unroll
-    for (int e = 0; e < D / 32; e++) acc[e] = fmaf(add, x[lane + 32 * e], keep * acc[e]);
-  }
+      for (int o = 16; o; o >>= 1) b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, o));
+      if (b == -INFINITY) continue;
+      float m = fmaxf(st.m == -INFINITY ? -INFINITY : (st.b - b) + st.m, other.m == -INFINITY ? -INFINITY : (other.b - b) + other.m);
 #pragma unroll
-  for (int e = 0; e < D / 32; e++) s_o[warp][lane + 32 * e] = acc[e];
-  if (lane == 0) s_stat[warp] = st;
-  __syncthreads();
-  if (threadIdx.x >= D) return;
-  Stat sum{-INFINITY, -INFINITY, 0.0f};
-  float o = 0.0f;
-  for (int k = 0; k < kWarps; k++)
-    if (s_stat[k].m > -INFINITY) sum.b = fmaxf(sum.b, s_stat[k].b);
-  for (int k = 0; k < kWarps; k++)
-    if (s_stat[k].m > -INFINITY) sum.m = fmaxf(sum.m, (s_stat[k].b - sum.b) + s_stat[k].m);
-  for (int k = 0; k < kWarps; k++) {
-    const float x = weight_of(s_stat[k], sum.b, sum.m);
-    sum.l = fmaf(x, s_stat[k].l, sum.l);
-    o = fmaf(x, s_o[k][threadIdx.x], o);
+      for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const float keep = weight_of(st, b, m), add = weight_of(other, b, m);
+      float l = add * other.l;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+      st = Stat{b, m, fmaf(keep, st.l, l)};
+#pragma unroll
+      for (int e = 0; e < D / 32; e++) acc[e] *= keep;
+      const uint32_t n = min(32u, parts - k0);
+      const float* x = p + uint64_t(k0) * (D + 4) + lane;
+#pragma unroll 8
+      for (uint32_t k = 0; k < n; k++) {
+        const float y = __shfl_sync(0xffffffffu, add, k);
+#pragma unroll
+        for (int e = 0; e < D / 32; e++) acc[e] = fmaf(y, y > 0.0f ? x[k * (D + 4) + 32 * e] : 0.0f, acc[e]);
+      }
+    }
   }
-  put<T, FMT>(a, question, head, threadIdx.x, o, sum.l);
-  if (threadIdx.x == 0) put_lse(a, question, head, sum);
+  if (per > 1) {
+#pragma unroll
+    for (int e = 0; e < D / 32; e++) s_o[warp][lane + 32 * e] = acc[e];
+    if (lane == 0) s_stat[warp] = st;
+    __syncthreads();
+    if (share) return;
+    Stat sum{-INFINITY, -INFINITY, 0.0f};
+    for (uint32_t k = 0; k < per; k++) sum.b = fmaxf(sum.b, s_stat[warp + k].b);
+    for (uint32_t k = 0; k < per; k++)
+      if (s_stat[warp + k].m > -INFINITY) sum.m = fmaxf(sum.m, (s_stat[warp + k].b - sum.b) + s_stat[warp + k].m);
+#pragma unroll
+    for (int e = 0; e < D / 32; e++) acc[e] = 0.0f;
+    for (uint32_t k = 0; k < per; k++) {
+      const float x = weight_of(s_stat[warp + k], sum.b, sum.m);
+      sum.l = fmaf(x, s_stat[warp + k].l, sum.l);
+#pragma unroll
+      for (int e = 0; e < D / 32; e++) acc[e] = fmaf(x, s_o[warp + k][lane + 32 * e], acc[e]);
+    }
+    st = sum;
+  }
+  if (!live) return;
+#pragma unroll
+  for (int e = 0; e < D / 32; e++) put<T, FMT>(a, question, head, lane + 32 * e, acc[e], st.l);
+  if (lane == 0) put_lse(a, question, head, st);
 }
 
 inline Shape shape_of(const AttendArg& a, int sms) {
@@ -468,14 +523,18 @@ cudaError_t attend_tile(const AttendArg& a, int sms, cudaStream_t s, uint64_t* l
   const uint64_t ctas = (sh.items + sh.hg - 1) / sh.hg;
   if (ctas == 0) return cudaSuccess;
   if (ctas > 0x7fffffffull) return cudaErrorInvalidConfiguration;
-  const size_t ring = size_t(kWarps / sh.mg) * stages(D) * cell_bytes(D);
+  const bool masked = a.mask != nullptr;
+  const size_t ring = stages(D, masked) * (size_t(kWarps / sh.mg) * cell_bytes(D) + (masked ? kWarps * kMaskBytes : 0));
   const size_t join = sh.kg > 1 ? size_t(kWarps) * 16 * (D + 4) * 4 : 0;
-  k_attend<T, D, FMT><<<dim3(unsigned(ctas), a.splits), kThreads, std::max(ring, join), s>>>(a, sh);
+  const dim3 grid(unsigned(ctas), a.splits);
+  if (masked) k_attend<T, D, FMT, true><<<grid, kThreads, std::max(ring, join), s>>>(a, sh);
+  else k_attend<T, D, FMT, false><<<grid, kThreads, std::max(ring, join), s>>>(a, sh);
   ++*launches;
   cudaError_t e = cudaGetLastError();
   if (e || a.splits == 1) return e;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(a.a.questions * a.a.heads);
+  const uint32_t per = a.splits <= 32 ? 1 : kWarps, rows = kWarps / per;
+  cfg.gridDim = dim3((a.a.questions * a.a.heads + rows - 1) / rows);
   cfg.blockDim = dim3(kThreads);
   cfg.stream = s;
   cudaLaunchAttribute early[1];
@@ -484,7 +543,7 @@ cudaError_t attend_tile(const AttendArg& a, int sms, cudaStream_t s, uint64_t* l
   cfg.attrs = early;
   cfg.numAttrs = 1;
   ++*launches;
-  return cudaLaunchKernelEx(&cfg, k_join<T, D, FMT>, a);
+  return cudaLaunchKernelEx(&cfg, k_join<T, D, FMT>, a, per);
 }
 
 // --- pointer scores --------------------------------------------------------------
@@ -548,7 +607,9 @@ __global__ __launch_bounds__(kThreads) void k_scores(ScoreArg a, uint32_t chunks
     const uint32_t next = w.page_of(i, S - 1), page = w.page_of(i, 0);
     issue(i + S - 1, i + S - 1 < n ? next : kNone);
     const uint64_t pos = (c0 + w.first + uint64_t(w.step) * i) * kCell + lane;
-    float unit = 0.0f;
+    float unit = 0.0f, bias[16];  // the cell's mask entries, on their way while it is multiplied
+#pragma unroll
+    for (int r = 0; r < 16; r++) bias[r] = a.mask && uint32_t(r) < n_rows && pos < stride ? a.mask[at0 + r * stride + pos] : 0.0f;
     if (page != kNone) {
       const uint8_t* cell = ring + (i % S) * CB;
       float s[4][4];
@@ -563,11 +624,10 @@ __global__ __launch_bounds__(kThreads) void k_scores(ScoreArg a, uint32_t chunks
     if (pos < stride) {
       const bool held = page != kNone && pos < len;
       float* out = a.scores + at0 + pos;
-      const float* mask = a.mask ? a.mask + at0 + pos : nullptr;
-      for (uint32_t r = 0; r < n_rows; r++) {
-        const float bias = mask ? mask[r * stride] : 0.0f;
-        out[r * stride] = held && bias > kBlocked ? fmaf(tile[r][lane], unit, fminf(bias, -kBlocked)) : kShut;
-      }
+#pragma unroll
+      for (int r = 0; r < 16; r++)
+        if (uint32_t(r) < n_rows)
+          out[r * stride] = held && bias[r] > kBlocked ? fmaf(tile[r][lane], unit, fminf(bias[r], -kBlocked)) : kShut;
     }
     __syncwarp();
   }
@@ -596,9 +656,12 @@ cudaError_t scores_tile(const ScoreArg& a, int sms, cudaStream_t s, uint64_t* la
 
 template <typename T, int D, int FMT>
 cudaError_t prepare_tile() {
-  const int ring = int(kWarps * stages(D) * cell_bytes(D)), join = kWarps * 16 * (D + 4) * 4;
-  cudaError_t e = cudaFuncSetAttribute(k_attend<T, D, FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize, std::max(ring, join));
-  if (e) return e;
+  const int join = kWarps * 16 * (D + 4) * 4;
+  const int plain = kWarps * stages(D, false) * int(cell_bytes(D)), masked = kWarps * stages(D, true) * (int(cell_bytes(D)) + kMaskBytes);
+  cudaError_t e;
+  if ((e = cudaFuncSetAttribute(k_attend<T, D, FMT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, std::max(plain, join))) ||
+      (e = cudaFuncSetAttribute(k_attend<T, D, FMT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, std::max(masked, join))))
+    return e;
   return cudaFuncSetAttribute(k_scores<T, D, FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                               int(kWarps * 3 * (kCell * D + kCell * 4)));
 }

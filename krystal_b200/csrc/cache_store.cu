@@ -1,8 +1,12 @@
 // cache_store.cu — rows quantised into the bank cache, rows read back, and the
 // selection of the blocks whose keys can score highest.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 #include "cache.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace kc {
 namespace cache {
@@ -218,103 +222,185 @@ __device__ __forceinline__ unsigned long long order_key(double s) {
   return b >> 63 ? ~b : b | (1ull << 63);
 }
 
+constexpr uint32_t kAsk = 8;  // questions of a sequence that a cluster scores at once
+
+// The `left` largest of n keys (left < n) of one question, by one warp: a radix
+// select, 8 bits a pass from the highest bit in which two keys differ, until a
+// bin is taken whole. An entry is taken if its key's known bits lie above
+// limit's, or equal them and it is among the first `ties` that do.
+struct Cut {
+  unsigned long long known, limit;
+  uint32_t ties;
+};
+__device__ __forceinline__ Cut cut_of(const unsigned long long* key, uint32_t n, uint32_t left, uint32_t* bin, uint32_t lane) {
+  unsigned long long both = ~0ull, any = 0;
+  for (uint32_t b = lane; b < n; b += 32) {
+    both &= key[b];
+    any |= key[b];
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    both &= __shfl_xor_sync(0xffffffffu, both, o);
+    any |= __shfl_xor_sync(0xffffffffu, any, o);
+  }
+  if (both == any) return Cut{~0ull, any, left};  // all are equal
+  int shift = 64 - __clzll(static_cast<long long>(both ^ any)) - 8;  // of the 8 bits that begin with the first that differs
+  if (shift < 0) shift = 0;
+  Cut c{shift + 8 < 64 ? ~0ull << (shift + 8) : 0ull, 0, left};
+  c.limit = any & c.known;
+  for (;;) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) bin[lane * 8 + i] = 0;
+    __syncwarp();
+    for (uint32_t b = lane; b < n; b += 32)
+      if ((key[b] & c.known) == c.limit) atomicAdd(&bin[uint32_t(key[b] >> shift) & 255u], 1u);
+    __syncwarp();
+    uint32_t own[8], sum = 0;  // lane 0 has the highest bins
+#pragma unroll
+    for (int i = 0; i < 8; i++) sum += own[i] = bin[255 - (lane * 8 + i)];
+    uint32_t upto = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= uint32_t(o)) upto += y;
+    }
+    const uint32_t who = __ffs(__ballot_sync(0xffffffffu, upto >= c.ties)) - 1;
+    uint32_t above = upto - sum, pick = 0, held = 0;
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      if (!found && above + own[i] >= c.ties) {
+        found = true;
+        pick = 255 - (lane * 8 + i);
+        held = own[i];
+      }
+      if (!found) above += own[i];
+    }
+    above = __shfl_sync(0xffffffffu, above, who);
+    pick = __shfl_sync(0xffffffffu, pick, who);
+    held = __shfl_sync(0xffffffffu, held, who);
+    c.ties -= above;
+    c.limit = (c.limit & c.known) | (static_cast<unsigned long long>(pick) << shift);
+    c.known |= 255ull << shift;
+    c.limit &= c.known;
+    if (held == c.ties || shift == 0) return c;
+    shift = shift > 8 ? shift - 8 : 0;
+    __syncwarp();
+  }
+}
+
 // The blocks that a question's group of heads looks at: with q+ and q- the sums
 // of the heads' positive and negative parts,
 //   score_b = sum_d q+_d hi_bd + q-_d lo_bd  >=  sum over heads of any q . k in b.
 // Products of two f32 are exact in f64 and the sums differ from the definition's
-// by about 1e-15 of their terms, so that the choice is the definition's. One CTA
-// a question and key head; the scores stay in shared memory, a radix select finds
-// the count-th largest, and what is taken leaves in block order.
-template <typename T>
-__global__ __launch_bounds__(kThreads) void k_blocks(BlockArg a) {
-  extern __shared__ unsigned long long s_key[];
-  __shared__ double s_q[2][128];
-  __shared__ uint32_t s_bin[256], s_scan[kWarps], s_pick, s_left;
-  const uint32_t head = blockIdx.x % a.c.heads, row = blockIdx.x / a.c.heads, d = a.c.dim;
-  uint32_t seq = row;
-  if (a.a.off) {
-    if (row < a.a.off[0] || row >= a.a.off[a.t.seqs]) return;
-    seq = owner_of(a.a.off, a.t.seqs, row);
-  } else if (row >= a.t.seqs) {
-    return;
-  }
-  const uint32_t n = (length_of(a.t, seq) + kPage - 1) / kPage, group = a.a.heads / a.c.heads;
-  for (uint32_t i = threadIdx.x; i < d; i += kThreads) {
-    double up = 0.0, down = 0.0;
-    for (uint32_t g = 0; g < group; g++) {
-      const double q = to_f32(static_cast<const T*>(a.a.q)[row * a.a.pitch + (head * group + g) * uint64_t(d) + i]);
-      up += q > 0.0 ? q : 0.0;
-      down += q > 0.0 ? 0.0 : q;
-    }
-    s_q[0][i] = up;
-    s_q[1][i] = down;
-  }
-  __syncthreads();
-  for (uint32_t b = threadIdx.x; b < n; b += kThreads) {
-    const uint32_t page = a.t.table[uint64_t(seq) * a.t.pitch + b];
-    double s = -INFINITY;
-    if (b + a.recent >= n) {
-      s = INFINITY;
-    } else if (page < a.c.pages) {
-      const float* lo = a.c.bounds + (uint64_t(page) * a.c.heads + head) * 2 * d;
-      s = 0.0;
-      for (uint32_t i = 0; i < d; i++)
-        s = fma(s_q[0][i], double(lo[d + i]), fma(s_q[1][i], double(lo[i]), s));
-    }
-    s_key[b] = order_key(s);
-  }
-  __syncthreads();
-  // the radix select: `limit` ends as the count-th largest key, `left` as the
-  // number of entries equal to it that are taken
-  unsigned long long limit = 0, known = 0;
-  uint32_t left = min(a.count, n);
-  for (int shift = 56; shift >= 0 && left < n; shift -= 8) {
-    s_bin[threadIdx.x] = 0;
-    __syncthreads();
-    for (uint32_t b = threadIdx.x; b < n; b += kThreads)
-      if ((s_key[b] & known) == limit) atomicAdd(&s_bin[uint32_t(s_key[b] >> shift) & 255u], 1u);
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      uint32_t above = 0, bin = 255;
-      while (above + s_bin[bin] < left) above += s_bin[bin--];
-      s_pick = bin;
-      s_left = left - above;
-    }
-    __syncthreads();
-    left = s_left;
-    limit |= static_cast<unsigned long long>(s_pick) << shift;
-    known |= 255ull << shift;
-    __syncthreads();
-  }
-  uint32_t* out = a.blocks + (uint64_t(row) * a.c.heads + head) * a.count;
-  uint32_t at = 0, even = 0;  // taken before, and equal to the limit before
+// by about 1e-15 of their terms, so that the choice is the definition's.
+//
+// A cluster of CTAs takes up to kAsk questions of a sequence and a key head and
+// reads each block's bounds once for them: 4 lanes a block, 16 bytes of the
+// smallest and of the largest keys a lane and step, so that 8 blocks of a warp are
+// on their way at once. The scores go, as keys that order alike, to the shared
+// memory of the CTA that selects for the question, a warp a question. The newest
+// blocks are the sequence's last, so they follow whatever is selected.
+template <typename T, int D>
+__global__ __launch_bounds__(kThreads) void k_blocks(BlockArg a, uint32_t ask, uint32_t chunks, uint32_t most) {
+  extern __shared__ unsigned long long s_key[];  // [questions of this CTA][most]
+  __shared__ double s_q[kAsk][2][D];
+  __shared__ uint32_t s_bin[kWarps][256];
+  cg::cluster_group cluster = cg::this_cluster();
+  const uint32_t rank = cluster.block_rank(), ctas = cluster.num_blocks();
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (uint32_t b0 = 0; b0 < n; b0 += kThreads) {
-    const uint32_t b = b0 + threadIdx.x;
-    const bool all = a.count >= n;
-    const bool tie = b < n && !all && s_key[b] == limit, more = b < n && (all || s_key[b] > limit);
-    // ranks by two ballots: ties packed in the high half, the others in the low
-    const uint32_t mt = __ballot_sync(0xffffffffu, tie), mm = __ballot_sync(0xffffffffu, more);
-    if (lane == 0) s_scan[warp] = (__popc(mt) << 16) | __popc(mm);
-    __syncthreads();
-    uint32_t before_tie = even, before_more = 0, all_tie = 0, all_more = 0;
-    for (uint32_t w = 0; w < kWarps; w++) {
-      if (w < warp) before_tie += s_scan[w] >> 16, before_more += s_scan[w] & 0xffffu;
-      all_tie += s_scan[w] >> 16;
-      all_more += s_scan[w] & 0xffffu;
+  const uint32_t unit = blockIdx.x / ctas, head = unit % a.c.heads, group = a.a.heads / a.c.heads;
+  const uint32_t chunk = unit / a.c.heads % chunks, seq = unit / a.c.heads / chunks;
+  const uint64_t q0 = a.a.off ? a.a.off[seq] : seq, q1 = a.a.off ? a.a.off[seq + 1] : seq + 1;
+  const uint64_t end = min(min(q0 + a.a.max_q, q1), uint64_t(a.a.questions)), row0 = q0 + chunk * ask;
+  if (row0 >= end) return;  // the whole cluster
+  const uint32_t nq = uint32_t(min(uint64_t(ask), end - row0));
+  const uint32_t n = (length_of(a.t, seq) + kPage - 1) / kPage;
+  const uint32_t last = min(a.recent, n), scored = n > a.count ? n - last : 0;  // blocks that have to be scored
+  for (uint32_t i = threadIdx.x; i < nq * D; i += kThreads) {
+    double up = 0.0, down = 0.0;
+    const T* q = static_cast<const T*>(a.a.q) + (row0 + i / D) * a.a.pitch + head * group * uint64_t(D) + i % D;
+    for (uint32_t g = 0; g < group; g++) {
+      const double x = to_f32(q[g * D]);
+      up += x > 0.0 ? x : 0.0;
+      down += x > 0.0 ? 0.0 : x;
     }
-    const uint32_t under = (1u << lane) - 1;
-    before_tie += __popc(mt & under);
-    before_more += __popc(mm & under);
-    const bool take = more || (tie && before_tie < left);
-    // entries taken before this one: those above the limit, and the ties among the first `left`
-    const uint32_t rank = at + before_more + (min(before_tie, left) - min(even, left));
-    if (take) out[rank] = b;
-    at += all_more + (min(even + all_tie, left) - min(even, left));
-    even += all_tie;
-    __syncthreads();
+    s_q[i / D][0][i % D] = up;
+    s_q[i / D][1][i % D] = down;
   }
-  for (uint32_t i = min(a.count, n) + threadIdx.x; i < a.count; i += kThreads) out[i] = kNone;
+  cluster.sync();
+  const uint32_t part = lane & 3;
+  for (uint32_t b0 = (rank * kWarps + warp) * 8; b0 < scored; b0 += ctas * kWarps * 8) {
+    const uint32_t b = b0 + lane / 4;
+    const uint32_t page = b < scored ? a.t.table[uint64_t(seq) * a.t.pitch + b] : kNone;
+    const bool there = page < a.c.pages;
+    constexpr int F = D / 16;
+    float4 lo[F], hi[F];
+    const float4* bounds = reinterpret_cast<const float4*>(a.c.bounds + (uint64_t(there ? page : 0) * a.c.heads + head) * 2 * D);
+#pragma unroll
+    for (int i = 0; i < F; i++) {
+      lo[i] = bounds[part + 4 * i];
+      hi[i] = bounds[D / 4 + part + 4 * i];
+    }
+    double score[kAsk] = {};
+#pragma unroll
+    for (int i = 0; i < F; i++) {
+      const double l[4] = {lo[i].x, lo[i].y, lo[i].z, lo[i].w}, h[4] = {hi[i].x, hi[i].y, hi[i].z, hi[i].w};
+#pragma unroll
+      for (uint32_t k = 0; k < kAsk; k++) {
+        if (k >= nq) break;
+        const double2* up = reinterpret_cast<const double2*>(&s_q[k][0][4 * (part + 4 * i)]);
+        const double2* down = reinterpret_cast<const double2*>(&s_q[k][1][4 * (part + 4 * i)]);
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          const double2 u = up[j], w = down[j];
+          score[k] = fma(u.x, h[2 * j], fma(w.x, l[2 * j], score[k]));
+          score[k] = fma(u.y, h[2 * j + 1], fma(w.y, l[2 * j + 1], score[k]));
+        }
+      }
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < kAsk; k++) {
+      if (k >= nq) break;
+      double s = score[k];
+      s += __shfl_xor_sync(0xffffffffu, s, 1);
+      s += __shfl_xor_sync(0xffffffffu, s, 2);
+      if (part == k % 4 && b < scored) {
+        unsigned long long* to = cluster.map_shared_rank(s_key, k % ctas);
+        to[uint64_t(k / ctas) * most + b] = order_key(there ? s : -INFINITY);
+      }
+    }
+  }
+  cluster.sync();
+  const uint32_t k = rank + ctas * warp;
+  if (k >= nq) return;
+  const unsigned long long* key = s_key + uint64_t(warp) * most;
+  uint32_t* out = a.blocks + ((row0 + k) * a.c.heads + head) * a.count;
+  const uint32_t under = (1u << lane) - 1;
+  uint32_t at = 0;
+  if (scored == 0) {  // all that there are
+    for (uint32_t b = lane; b < n; b += 32) out[b] = b;
+    at = n;
+  } else {
+    if (a.count > last) {
+      const Cut c = cut_of(key, scored, a.count - last, s_bin[warp], lane);
+      uint32_t even = 0;
+      for (uint32_t b0 = 0; b0 < scored; b0 += 32) {
+        const uint32_t b = b0 + lane;
+        const unsigned long long x = b < scored ? key[b] & c.known : 0;
+        const bool tie = b < scored && x == c.limit, more = b < scored && x > c.limit;
+        const uint32_t ties = __ballot_sync(0xffffffffu, tie);
+        const bool take = more || (tie && even + __popc(ties & under) < c.ties);
+        const uint32_t took = __ballot_sync(0xffffffffu, take);
+        if (take) out[at + __popc(took & under)] = b;
+        at += __popc(took);
+        even += __popc(ties);
+      }
+    }
+    for (uint32_t b = scored + lane; b < n; b += 32) out[at + b - scored] = b;
+    at += n - scored;
+  }
+  for (uint32_t i = at + lane; i < a.count; i += 32) out[i] = kNone;
 }
 
 template <typename T, int D, int FMT>
@@ -364,24 +450,62 @@ cudaError_t launch_read(const Store& c, const Table& t, const Rows& r, int sms, 
   return store(false, c, t, r, sms, s, launches);
 }
 
-cudaError_t launch_blocks(const BlockArg& a, int, cudaStream_t s, uint64_t* launches) {
+namespace {
+
+template <typename T, int D>
+cudaError_t blocks_as(const BlockArg& a, int sms, cudaStream_t s) {
+  const uint32_t most = std::max(1u, (a.t.max_len + kPage - 1) / kPage);
+  uint32_t ask = std::min(kAsk, a.a.max_q);
+  while (ask > 1 && uint64_t(ask) * most > kMaxBlocks) ask--;
+  const uint32_t chunks = (a.a.max_q + ask - 1) / ask;
+  const uint64_t units = uint64_t(a.t.seqs) * chunks * a.c.heads;
+  // few units of long sequences: clusters share a unit's blocks, while each CTA
+  // has a few rounds of its warps' 8 and there is room for two CTAs an SM
+  uint32_t ctas = 1;
+  while (ctas < 8 && units * ctas * 2 <= uint64_t(sms) * 2 && most >= ctas * 2 * kWarps * 8 * 2) ctas *= 2;
+  if (units * ctas > 0x7fffffffull) return cudaErrorInvalidConfiguration;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(units * ctas));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = size_t((ask + ctas - 1) / ctas) * most * 8;
+  cfg.stream = s;
+  cudaLaunchAttribute cluster[1];
+  cluster[0].id = cudaLaunchAttributeClusterDimension;
+  cluster[0].val.clusterDim.x = ctas;
+  cluster[0].val.clusterDim.y = cluster[0].val.clusterDim.z = 1;
+  cfg.attrs = cluster;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, k_blocks<T, D>, a, ask, chunks, most);
+}
+
+template <typename T>
+cudaError_t blocks_dim(const BlockArg& a, int sms, cudaStream_t s) {
+  return a.c.dim == 32 ? blocks_as<T, 32>(a, sms, s) : a.c.dim == 64 ? blocks_as<T, 64>(a, sms, s) : blocks_as<T, 128>(a, sms, s);
+}
+
+template <typename T>
+cudaError_t prepare_blocks() {
+  const int most = int(kMaxBlocks) * 8;
+  cudaError_t e;
+  if ((e = cudaFuncSetAttribute(k_blocks<T, 32>, cudaFuncAttributeMaxDynamicSharedMemorySize, most)) ||
+      (e = cudaFuncSetAttribute(k_blocks<T, 64>, cudaFuncAttributeMaxDynamicSharedMemorySize, most)) ||
+      (e = cudaFuncSetAttribute(k_blocks<T, 128>, cudaFuncAttributeMaxDynamicSharedMemorySize, most)))
+    return e;
+  return cudaSuccess;
+}
+
+}  // namespace
+
+cudaError_t launch_blocks(const BlockArg& a, int sms, cudaStream_t s, uint64_t* launches) {
   if (a.a.questions == 0 || a.t.seqs == 0) return cudaSuccess;
-  const size_t smem = size_t((a.t.max_len + kPage - 1) / kPage) * 8;
-  const unsigned grid = a.a.questions * a.c.heads;
   ++*launches;
-  if (a.a.dtype == kF32) k_blocks<float><<<grid, kThreads, smem, s>>>(a);
-  else if (a.a.dtype == kF16) k_blocks<__half><<<grid, kThreads, smem, s>>>(a);
-  else k_blocks<__nv_bfloat16><<<grid, kThreads, smem, s>>>(a);
-  return cudaGetLastError();
+  return a.a.dtype == kF32 ? blocks_dim<float>(a, sms, s)
+       : a.a.dtype == kF16 ? blocks_dim<__half>(a, sms, s) : blocks_dim<__nv_bfloat16>(a, sms, s);
 }
 
 cudaError_t prepare_store() {
   cudaError_t e;
-  const int most = int(kMaxBlocks) * 8;
-  if ((e = cudaFuncSetAttribute(k_blocks<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, most)) ||
-      (e = cudaFuncSetAttribute(k_blocks<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, most)) ||
-      (e = cudaFuncSetAttribute(k_blocks<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, most)))
-    return e;
+  if ((e = prepare_blocks<float>()) || (e = prepare_blocks<__half>()) || (e = prepare_blocks<__nv_bfloat16>())) return e;
   return cudaSuccess;
 }
 

@@ -178,6 +178,10 @@ __device__ __forceinline__ void copy16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
                ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))), "l"(src) : "memory");
 }
+__device__ __forceinline__ void copy4(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;"
+               ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))), "l"(src) : "memory");
+}
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -229,7 +233,10 @@ struct Walk {
     const uint32_t j = (i & 31u) + ahead;
     return __shfl_sync(0xffffffffu, j < 32 ? page[0] : page[1], j & 31u);
   }
-  __device__ __forceinline__ uint32_t block_of(uint32_t i) const { return __shfl_sync(0xffffffffu, block[0], i & 31u); }
+  __device__ __forceinline__ uint32_t block_of(uint32_t i, uint32_t ahead) const {
+    const uint32_t j = (i & 31u) + ahead;
+    return __shfl_sync(0xffffffffu, j < 32 ? block[0] : block[1], j & 31u);
+  }
 };
 
 }  // namespace cache
