@@ -29,9 +29,10 @@ constexpr int kThreads = 256, kWarps = 8;
 constexpr float kLift = 8.0f, kSlack = 6.0f;
 constexpr int kLeastExp = -80;  // value scales below it keep their digits in f_j; l stays below 2^128
 
-// Cells a ring holds; a masked call's has the mask entries of each warp's 16 rows
-// beside them, 36 floats apart so that 8 rows of a column lie on different banks.
-constexpr int kMaskPitch = 36, kMaskBytes = 16 * kMaskPitch * 4;
+// Cells a ring holds; a masked call's has the mask entries of each warp's rows
+// beside them, 36 floats apart so that what a warp reads at once lies on different banks.
+constexpr int kMaskPitch = 36;
+__host__ __device__ constexpr int mask_bytes(int tiles) { return 8 * tiles * kMaskPitch * 4; }
 __host__ __device__ constexpr int stages(int dim, bool masked) { return masked ? (dim == 32 ? 3 : 2) : dim == 32 ? 4 : 3; }
 
 // What a warp needs of one key of a cell: score = product * a * unit + e.
@@ -50,10 +51,10 @@ struct Unit {
   const float* mask;                              // of the unit's first question
 };
 
-// How a launch's warps are shared out: teams of `mg` warps (16 rows each) read the
-// same cells, `kg` teams share a unit's cells, a CTA has hg units.
+// How a launch's warps are shared out: teams of `mg` warps (8 `tiles` rows each) read
+// the same cells, `kg` teams share a unit's cells, a CTA has hg units.
 struct Shape {
-  uint32_t mg, kg, hg, chunks;  // chunks: of 16 mg rows, that a unit may have
+  uint32_t tiles, mg, kg, hg, chunks;  // chunks: of 8 tiles mg rows, that a unit may have
   uint64_t items;
 };
 
@@ -88,7 +89,7 @@ __device__ __forceinline__ bool unit_of(const AttendArg& a, const Shape& sh, uin
   }
   if (first >= a.a.questions) return false;
   u->rows = min(u->rows, (a.a.questions - u->q0) * group);
-  u->row0 = chunk * 16 * sh.mg;
+  u->row0 = chunk * 8 * sh.tiles * sh.mg;
   if (u->row0 >= u->rows) return false;
   u->len = length_of(a.t, u->seq);
   u->blocks = (u->len + kPage - 1) / kPage;
@@ -101,7 +102,7 @@ __device__ __forceinline__ bool unit_of(const AttendArg& a, const Shape& sh, uin
   return true;
 }
 
-// 16 questions' rows of a warp's results, as the warps of a row, or the parts of a
+// What is known of a row's scores, as the warps of a row, or the parts of a
 // sequence, are joined: [B, M, l, -] and o.
 struct Stat {
   float b, m, l;
@@ -123,24 +124,45 @@ __device__ __forceinline__ float* part_of(const AttendArg& a, uint64_t question,
   return a.work + ((question * a.a.heads + head) * a.splits + part) * (a.c.dim + 4);
 }
 
-// N values of a row, one after another.
+// N values of a row, one after another; wide: the place is 16-byte aligned.
 template <typename T, int N>
 __device__ __forceinline__ void put_run(T* dst, const float (&x)[N], bool wide) {
+  constexpr int bytes = N * int(sizeof(T));
   if (wide) {
-    T y[N];
+    alignas(16) T y[N];
 #pragma unroll
     for (int i = 0; i < N; i++) y[i] = from_f32<T>(x[i]);
+    if constexpr (bytes % 16 == 0) {
 #pragma unroll
-    for (int i = 0; i < int(N * sizeof(T) / 16); i++) reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(y)[i];
+      for (int i = 0; i < bytes / 16; i++) reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(y)[i];
+    } else {
+      *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(y);
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < N; i++) dst[i] = from_f32<T>(x[i]);
   }
 }
 
-template <typename T, int D, int FMT, bool MASKED>
-__global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void k_attend(AttendArg a, Shape sh) {
-  constexpr int S = stages(D, MASKED), CB = int(cell_bytes(D)), NB = D / 8;
+// The cell's bytes, shared out among the MG warps of a team.
+template <int CB, int MG>
+__device__ __forceinline__ void copy_cell(uint8_t* dst, const uint8_t* src, uint32_t thread) {
+#pragma unroll
+  for (int k = 0; k < (CB / 16 + MG * 32 - 1) / (MG * 32); k++) {
+    const uint32_t at = thread + k * MG * 32;
+    if ((k + 1) * MG * 32 <= CB / 16 || at < CB / 16) copy16(dst + 16 * at, src + 16 * at);
+  }
+}
+
+// CTAs of 256 threads that an SM should hold at once: what their rings and their
+// registers (without spilling) leave room for.
+__host__ __device__ constexpr int resident(int dim, int tiles, bool masked) {
+  return dim == 128 || (dim == 64 && tiles == 2 && masked) ? 1 : dim == 32 && tiles == 1 ? 3 : 2;
+}
+
+template <typename T, int D, int FMT, int NT, bool MASKED>
+__global__ __launch_bounds__(kThreads, resident(D, NT, MASKED)) void k_attend(AttendArg a, Shape sh) {
+  constexpr int S = stages(D, MASKED), CB = int(cell_bytes(D)), MT = D / 16, NB = D / 8, R = 8 * NT;
   constexpr bool kTwo = sizeof(T) == 4;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ KeyInfo s_info[kWarps][kCell];
@@ -166,53 +188,63 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void k_attend(AttendArg
   }
   const bool mine = live && part < parts;
   const uint32_t n = mine ? w.count() : 0;
-  // this lane's rows: their question (from the unit's first) and head
-  const uint32_t row = u.row0 + mi * 16 + g;
-  const bool busy = mine && u.row0 + mi * 16 < u.rows;
-  const bool ok0 = mine && row < u.rows, ok1 = mine && row + 8 < u.rows;
-  const uint32_t i0 = row / group, i1 = (row + 8) / group;
-  QTile<T, D> q;
-  {
-    const T* base = static_cast<const T*>(a.a.q);
-    q.load(ok0 ? base + (u.q0 + i0) * a.a.pitch + (u.kv * group + row % group) * uint64_t(D) : nullptr,
-           ok1 ? base + (u.q0 + i1) * a.a.pitch + (u.kv * group + (row + 8) % group) * uint64_t(D) : nullptr, c,
-           a.scale * kLog2e);
-  }
+  if (n) w.begin();
+  const uint32_t row0 = u.row0 + mi * R;  // the warp's first row
+  const uint32_t n_rows = mine && row0 < u.rows ? min(uint32_t(R), u.rows - row0) : 0;
+
   uint8_t* ring = smem + team * (S * CB);
-  uint8_t* biases = smem + kWarps / sh.mg * (S * CB) + warp * (S * kMaskBytes);  // a masked call's
-  __shared__ uint64_t s_mask[MASKED ? kWarps : 1][16];  // where the rows' masks begin
+  uint8_t* biases = smem + kWarps / sh.mg * (S * CB) + warp * (S * mask_bytes(NT));  // a masked call's
+  __shared__ uint64_t s_mask[MASKED ? kWarps : 1][R];  // where the rows' masks begin
   const uint32_t open_end = MASKED ? uint32_t(min(uint64_t(u.len), u.stride)) : u.len;
-  const uint32_t n_rows = busy ? min(16u, u.rows - (u.row0 + mi * 16)) : 0;
   if (MASKED) {
-    if (lane < 16) s_mask[warp][lane] = uint64_t(u.row0 + mi * 16 + lane) / group * u.stride;
+    if (lane < R) s_mask[warp][lane] = uint64_t((row0 + lane) / group) * u.stride;
     __syncwarp();
   }
   auto issue = [&](uint32_t i, uint32_t page, uint32_t block) {
     if (page != kNone) {
       const uint8_t* src = cell_of<D>(a.c, page, u.kv, w.half(i));
       uint8_t* dst = ring + (i % S) * CB;
-      for (uint32_t k = mi * 32 + lane; k < CB / 16; k += sh.mg * 32) copy16(dst + 16 * k, src + 16 * k);
+      const uint32_t thread = mi * 32 + lane;
+      if (sh.mg == 1) copy_cell<CB, 1>(dst, src, thread);
+      else if (sh.mg == 2) copy_cell<CB, 2>(dst, src, thread);
+      else if (sh.mg == 4) copy_cell<CB, 4>(dst, src, thread);
+      else copy_cell<CB, 8>(dst, src, thread);
       if (MASKED) {
         const uint64_t pos = uint64_t(block) * kPage + w.half(i) * kCell + lane;
-        uint8_t* to = biases + (i % S) * kMaskBytes + 4 * lane;
+        uint8_t* to = biases + (i % S) * mask_bytes(NT) + 4 * lane;
         if (pos < open_end)
           for (uint32_t r = 0; r < n_rows; r++) copy4(to + r * (4 * kMaskPitch), u.mask + s_mask[warp][r] + pos);
       }
     }
     copy_commit();
   };
-
-  float o[NB][4], top[2] = {-INFINITY, -INFINITY}, high[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
-#pragma unroll
-  for (int t = 0; t < NB; t++)
-#pragma unroll
-    for (int i = 0; i < 4; i++) o[t][i] = 0.0f;
-  if (n) w.begin();
   if (n) {
 #pragma unroll
     for (uint32_t i = 0; i + 1 < S; i++) {
       const uint32_t page = w.page_of(0, i), block = w.block_of(0, i);
       issue(i, i < n ? page : kNone, block);
+    }
+  }
+  QTile<T, D, NT> q;
+#pragma unroll
+  for (int t = 0; t < NT; t++) {
+    const uint32_t r = row0 + 8 * t + g;
+    q.load(t, uint32_t(8 * t + g) < n_rows ? static_cast<const T*>(a.a.q) + (u.q0 + r / group) * a.a.pitch + (u.kv * group + r % group) * uint64_t(D) : nullptr,
+           c, a.scale * kLog2e);
+  }
+
+  float o[NT][MT][4], top[NT][2], high[NT][2], sum[NT][2];
+#pragma unroll
+  for (int t = 0; t < NT; t++) {
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) o[t][m][i] = 0.0f;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      top[t][h] = MASKED ? -INFINITY : 0.0f;
+      high[t][h] = -INFINITY;
+      sum[t][h] = 0.0f;
     }
   }
   KeyInfo* info = s_info[warp];
@@ -222,184 +254,185 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void k_attend(AttendArg
     meet(team, sh.mg);
     const uint32_t next = w.page_of(i, S - 1), page = w.page_of(i, 0), block = w.block_of(i, 0);
     issue(i + S - 1, i + S - 1 < n ? next : kNone, MASKED ? w.block_of(i, S - 1) : 0);
-    if (!busy || page == kNone) continue;
+    if (!n_rows || page == kNone) continue;
     const uint8_t* cell = ring + (i % S) * CB;
     const uint64_t pos = uint64_t(block) * kPage + w.half(i) * kCell;
     {
       const float* scales = reinterpret_cast<const float*>(cell + 2 * kCell * D);
       const float vs = scales[kCell + lane];
-      const bool open = pos + lane < open_end;
-      const uint32_t e = max(__float_as_uint(vs) >> 23, uint32_t(127 + kLeastExp)), es = min(e, 253u);
+      const uint32_t e = min(max(__float_as_uint(vs) >> 23, uint32_t(127 + kLeastExp)), 253u);
       KeyInfo k;
-      k.re = pow2_biased(254u - es);
+      k.re = pow2_biased(254u - e);
       k.f = vs * k.re;
       k.a = scales[lane] * widened<FMT>();
-      k.e = float(int(es) - 127);
-      if (!open) k = KeyInfo{0.0f, -INFINITY, 0.0f, 0.0f};
+      k.e = float(int(e) - 127);
+      if (pos + lane >= open_end) k = KeyInfo{0.0f, -INFINITY, 0.0f, 0.0f};
       info[lane] = k;
     }
-    float s[4][4];
-    key_products<T, D, FMT>(q, cell, g, c, s);
+    float s[NT][2][4];
+    key_products<T, D, FMT, NT>(q, cell, g, c, s);
     __syncwarp();
+    KeyInfo key[4];  // of keys key_of(g) + 8 j
 #pragma unroll
-    for (int J = 0; J < 4; J++)
+    for (int j = 0; j < 4; j++) {
+      key[j] = info[8 * j + key_of(g)];
 #pragma unroll
-      for (int k = 0; k < 2; k++) {
-        const KeyInfo ki = info[8 * J + 4 * k + c];
-        s[J][k] = fmaf(s[J][k] * ki.a, q.unit[0], ki.e);
-        s[J][2 + k] = fmaf(s[J][2 + k] * ki.a, q.unit[1], ki.e);
-      }
-    float keep[2] = {1.0f, 1.0f};
-    bool moved = false;
+      for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+          s[t][j / 2][2 * (j % 2) + h] = fmaf(s[t][j / 2][2 * (j % 2) + h] * key[j].a, q.unit[t][h], key[j].e);
+    }
     if (MASKED) {
-      // entries are read twice rather than kept: 16 registers more would spill
-      const float* bias = reinterpret_cast<const float*>(biases + (i % S) * kMaskBytes) + g * kMaskPitch + c;
-      auto entry = [&](int J, int k) {
-        const float x = bias[(k / 2) * 8 * kMaskPitch + 8 * J + 4 * (k & 1)];
-        return s[J][k] > -INFINITY && x > kBlocked ? fminf(x, -kBlocked) * kLog2e : -INFINITY;
-      };
-      float most[2] = {-INFINITY, -INFINITY};
+      // entries are read twice rather than kept: their registers would spill
+      const float* bias = reinterpret_cast<const float*>(biases + (i % S) * mask_bytes(NT)) + 2 * c * kMaskPitch + key_of(g);
 #pragma unroll
-      for (int J = 0; J < 4; J++)
-#pragma unroll
-        for (int k = 0; k < 4; k++) most[k / 2] = fmaxf(most[k / 2], entry(J, k));
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 1));
-        most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 2));
-        const float was = top[h];
-        top[h] = fmaxf(was, most[h]);
-        if (was != top[h]) high[h] = was == -INFINITY ? -INFINITY : high[h] + (was - top[h]);  // measured from the new one
-      }
-#pragma unroll
-      for (int J = 0; J < 4; J++)
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-          const float x = entry(J, k);
-          s[J][k] = x > -INFINITY ? s[J][k] + (x - top[k / 2]) : -INFINITY;
-        }
-    }
-    float most[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-    for (int J = 0; J < 4; J++)
-#pragma unroll
-      for (int k = 0; k < 4; k++) most[k / 2] = fmaxf(most[k / 2], s[J][k]);
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-      most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 1));
-      most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 2));
-      if (most[h] > high[h] + kSlack || (high[h] == -INFINITY && most[h] > -INFINITY)) {
-        keep[h] = high[h] == -INFINITY ? 0.0f : ex2(high[h] - most[h]);
-        high[h] = most[h];
-        moved = true;
-      }
-    }
-    if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-      for (int t = 0; t < NB; t++)
-#pragma unroll
-        for (int k = 0; k < 4; k++) o[t][k] *= keep[k / 2];
-      sum[0] *= keep[0];
-      sum[1] *= keep[1];
-    }
-    const float from[2] = {high[0] == -INFINITY ? 0.0f : high[0] - kLift, high[1] == -INFINITY ? 0.0f : high[1] - kLift};
-#pragma unroll
-    for (int v = 0; v < 2; v++) {
-      uint32_t hi[4], lo[4];
-#pragma unroll
-      for (int J = 0; J < 2; J++) {
-        const KeyInfo k0 = info[16 * v + 8 * J + c], k1 = info[16 * v + 8 * J + 4 + c];
+      for (int t = 0; t < NT; t++) {
+        auto entry = [&](int j, int h) {
+          const float x = bias[(8 * t + h) * kMaskPitch + 8 * j];
+          return key[j].e > -INFINITY && x > kBlocked ? fminf(x, -kBlocked) * kLog2e : -INFINITY;
+        };
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-          const float x0 = ex2(s[2 * v + J][2 * h] - from[h]), x1 = ex2(s[2 * v + J][2 * h + 1] - from[h]);
-          sum[h] = fmaf(x1, k1.re, fmaf(x0, k0.re, sum[h]));
-          const float w0 = x0 * k0.f, w1 = x1 * k1.f;
-          hi[2 * J + h] = pack(w0, w1);
-          if (kTwo) {
-            const __half2 t2 = *reinterpret_cast<const __half2*>(&hi[2 * J + h]);
-            lo[2 * J + h] = pack(w0 - __low2float(t2), w1 - __high2float(t2));
+          float most = fmaxf(fmaxf(entry(0, h), entry(1, h)), fmaxf(entry(2, h), entry(3, h)));
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, x));
+          const float was = top[t][h];
+          top[t][h] = fmaxf(was, most);
+          if (was != top[t][h]) high[t][h] = was == -INFINITY ? -INFINITY : high[t][h] + (was - top[t][h]);  // measured from the new one
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const float x = entry(j, h);
+            float& y = s[t][j / 2][2 * (j % 2) + h];
+            y = x > -INFINITY ? y + (x - top[t][h]) : -INFINITY;
           }
         }
       }
-      value_products<D, FMT, kTwo>(hi, lo, cell + kCell * D, v, g, c, o);
+    }
+    bool moved = false;
+    float keep[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        float most = fmaxf(fmaxf(s[t][0][h], s[t][0][2 + h]), fmaxf(s[t][1][h], s[t][1][2 + h]));
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, x));
+        keep[t][h] = 1.0f;
+        if (most > high[t][h] + kSlack) {
+          keep[t][h] = high[t][h] == -INFINITY ? 0.0f : ex2(high[t][h] - most);
+          high[t][h] = most;
+          moved = true;
+        }
+      }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+          for (int k = 0; k < 4; k++) o[t][m][k] *= keep[t][k % 2];
+        sum[t][0] *= keep[t][0];
+        sum[t][1] *= keep[t][1];
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < 2; v++) {
+      uint32_t hi[NT][2], lo[kTwo ? NT : 1][2];
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        const float from[2] = {high[t][0] == -INFINITY ? 0.0f : high[t][0] - kLift, high[t][1] == -INFINITY ? 0.0f : high[t][1] - kLift};
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          const KeyInfo& k = key[2 * v + j];
+          const float x0 = ex2(s[t][v][2 * j] - from[0]), x1 = ex2(s[t][v][2 * j + 1] - from[1]);
+          sum[t][0] = fmaf(x0, k.re, sum[t][0]);
+          sum[t][1] = fmaf(x1, k.re, sum[t][1]);
+          const float w0 = x0 * k.f, w1 = x1 * k.f;
+          const uint32_t h = pack(w0, w1);
+          hi[t][j] = transposed(h);
+          if (kTwo) {
+            const __half2 y = *reinterpret_cast<const __half2*>(&h);
+            lo[kTwo ? t : 0][j] = transposed(pack(w0 - __low2float(y), w1 - __high2float(y)));
+          }
+        }
+      }
+      value_products<D, FMT, NT, kTwo>(hi, lo, cell + kCell * D, v, g, c, o);
     }
     __syncwarp();
   }
   copy_wait<0>();
 #pragma unroll
-  for (int h = 0; h < 2; h++) {
-    sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
-    sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
-    if (!MASKED) top[h] = 0.0f;
-  }
-  const Stat st[2] = {{top[0], high[0], sum[0]}, {top[1], high[1], sum[1]}};
+  for (int t = 0; t < NT; t++)
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) sum[t][h] += __shfl_xor_sync(0xffffffffu, sum[t][h], x);
 
   if (sh.kg == 1) {  // a row has one warp
     const bool wide = (reinterpret_cast<uintptr_t>(a.out) | a.out_pitch * sizeof(T)) % 16 == 0;
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      if (!(h ? ok1 : ok0)) continue;
-      const uint64_t question = u.q0 + (h ? i1 : i0);
-      const uint32_t head = u.kv * group + (row + 8 * h) % group;
-      const float unit = parts > 1 ? 1.0f : st[h].l > 0.0f ? widened<FMT>() / st[h].l : 0.0f;
-      float run[2 * NB];
+    for (int t = 0; t < NT; t++)
 #pragma unroll
-      for (int k = 0; k < 2 * NB; k++) run[k] = o[k % NB][2 * h + k / NB] * unit;
-      if (parts == 1) {
-        put_run(static_cast<T*>(a.out) + question * a.out_pitch + head * uint64_t(D) + 2 * c * NB, run, wide);
-        if (c == 0) put_lse(a, question, head, st[h]);
-      } else {
-        float* p = part_of(a, question, head, part);
-        put_run(p + 2 * c * NB, run, true);
-        if (c == 0) *reinterpret_cast<float4*>(p + D) = make_float4(st[h].b, st[h].m, st[h].l, 0.0f);
+      for (int h = 0; h < 2; h++) {
+        const uint32_t r = 8 * t + 2 * c + h;
+        if (r >= n_rows) continue;
+        const uint64_t question = u.q0 + (row0 + r) / group;
+        const uint32_t head = u.kv * group + (row0 + r) % group;
+        const Stat st{top[t][h], high[t][h], sum[t][h]};
+        const float unit = parts > 1 ? 1.0f : st.l > 0.0f ? widened<FMT>() / st.l : 0.0f;
+        float run[NB];
+#pragma unroll
+        for (int k = 0; k < NB; k++) run[k] = o[t][k / 2][2 * (k % 2) + h] * unit;
+        if (parts == 1) {
+          put_run(static_cast<T*>(a.out) + question * a.out_pitch + head * uint64_t(D) + g * NB, run, wide);
+          if (g == 0) put_lse(a, question, head, st);
+        } else {
+          float* p = part_of(a, question, head, part);
+          put_run(p + g * NB, run, true);
+          if (g == 0) *reinterpret_cast<float4*>(p + D) = make_float4(st.b, st.m, st.l, 0.0f);
+        }
       }
-    }
     return;
   }
-  // the warps of a row meet in shared memory: [warp][16 rows][D + 4]
+  // the warps of a row meet in shared memory: [warp][rows][D + 4]
   __syncthreads();
   float* join = reinterpret_cast<float*>(smem);
-  if (busy) {
+#pragma unroll
+  for (int t = 0; t < NT; t++)
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-      float* p = join + (warp * 16 + g + 8 * h) * (D + 4);
+      const uint32_t r = 8 * t + 2 * c + h;
+      if (r >= n_rows) continue;
+      float* p = join + (warp * R + r) * (D + 4);
+      float run[NB];
 #pragma unroll
-      for (int k = 0; k < 2; k++)
-#pragma unroll
-        for (int t = 0; t < NB; t++) p[(2 * c + k) * NB + t] = o[t][2 * h + k];
-      if (c == 0) {
-        p[D] = st[h].b;
-        p[D + 1] = st[h].m;
-        p[D + 2] = st[h].l;
-      }
+      for (int k = 0; k < NB; k++) run[k] = o[t][k / 2][2 * (k % 2) + h];
+      put_run(p + g * NB, run, true);
+      if (g == 0) *reinterpret_cast<float4*>(p + D) = make_float4(top[t][h], high[t][h], sum[t][h], 0.0f);
     }
-  }
   __syncthreads();
-  if (!busy) return;
-  // the team kgi of a unit's kg takes every kg-th row of its warps' 16
+  // the team kgi of a unit's kg takes every kg-th row of its warps'
   const uint32_t kgi = team % sh.kg, base = (team - kgi) * sh.mg + mi;
-  for (uint32_t r = kgi; r < 16; r += sh.kg) {
-    const uint32_t at = u.row0 + mi * 16 + r;
-    if (at >= u.rows) break;
+  for (uint32_t r = kgi; r < n_rows; r += sh.kg) {
     Stat all{-INFINITY, -INFINITY, 0.0f};
     for (uint32_t k = 0; k < sh.kg; k++) {
-      const float* p = join + ((base + k * sh.mg) * 16 + r) * (D + 4);
+      const float* p = join + ((base + k * sh.mg) * R + r) * (D + 4);
       if (p[D + 1] > -INFINITY) all.b = fmaxf(all.b, p[D]);
     }
     for (uint32_t k = 0; k < sh.kg; k++) {
-      const float* p = join + ((base + k * sh.mg) * 16 + r) * (D + 4);
+      const float* p = join + ((base + k * sh.mg) * R + r) * (D + 4);
       if (p[D + 1] > -INFINITY) all.m = fmaxf(all.m, (p[D] - all.b) + p[D + 1]);
     }
     float acc[D / 32] = {};
     for (uint32_t k = 0; k < sh.kg; k++) {
-      const float* p = join + ((base + k * sh.mg) * 16 + r) * (D + 4);
+      const float* p = join + ((base + k * sh.mg) * R + r) * (D + 4);
       const float x = weight_of(Stat{p[D], p[D + 1], p[D + 2]}, all.b, all.m);
       all.l = fmaf(x, p[D + 2], all.l);
 #pragma unroll
       for (int e = 0; e < D / 32; e++) acc[e] = fmaf(x, p[lane + 32 * e], acc[e]);
     }
-    const uint64_t question = u.q0 + at / group;
-    const uint32_t head = u.kv * group + at % group;
+    const uint64_t question = u.q0 + (row0 + r) / group;
+    const uint32_t head = u.kv * group + (row0 + r) % group;
     if (parts == 1) {
 #pragma unroll
       for (int e = 0; e < D / 32; e++) put<T, FMT>(a, question, head, lane + 32 * e, acc[e], all.l);
@@ -408,11 +441,7 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 1 : 2) void k_attend(AttendArg
       float* p = part_of(a, question, head, part);
 #pragma unroll
       for (int e = 0; e < D / 32; e++) p[lane + 32 * e] = acc[e];
-      if (lane == 0) {
-        p[D] = all.b;
-        p[D + 1] = all.m;
-        p[D + 2] = all.l;
-      }
+      if (lane == 0) *reinterpret_cast<float4*>(p + D) = make_float4(all.b, all.m, all.l, 0.0f);
     }
   }
 }
@@ -502,19 +531,38 @@ __global__ __launch_bounds__(kThreads) void k_join(AttendArg a, uint32_t per) {
   if (lane == 0) put_lse(a, question, head, st);
 }
 
+// Tiles of 8 rows a warp has at most: two of wide f32 rows would not fit the registers.
+template <typename T, int D>
+__host__ __device__ constexpr int most_tiles() { return D > 32 && sizeof(T) == 4 ? 1 : 2; }
+
 inline Shape shape_of(const AttendArg& a, int sms) {
   const uint32_t group = a.a.heads / a.c.heads;
   const uint64_t rows = a.blocks || a.block_count ? group : uint64_t(a.a.max_q) * group;
   const uint64_t units = a.blocks || a.block_count ? a.a.questions : a.t.seqs;
   const uint32_t blocks = a.block_count ? a.block_count : (a.t.max_len + kPage - 1) / kPage;
   Shape sh{};
-  sh.mg = rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 8;
-  sh.chunks = uint32_t((rows + 16 * sh.mg - 1) / (16 * sh.mg));
+  sh.tiles = rows <= 8 || (a.c.dim > 32 && a.a.dtype == kF32) ? 1 : 2;  // most_tiles
+  const uint64_t warps = (rows + 8 * sh.tiles - 1) / (8 * sh.tiles);
+  sh.mg = warps <= 1 ? 1 : warps <= 2 ? 2 : warps <= 4 ? 4 : 8;
+  sh.chunks = uint32_t((warps + sh.mg - 1) / sh.mg);
   sh.items = units * sh.chunks * a.c.heads;
   // short sequences of many units: a team a unit; else the CTA's teams share one
   sh.kg = blocks <= 8 && sh.items * sh.mg >= uint64_t(sms) * 16 ? 1 : kWarps / sh.mg;
   sh.hg = kWarps / (sh.mg * sh.kg);
   return sh;
+}
+
+__host__ __device__ constexpr size_t attend_smem(int dim, int tiles, bool masked, uint32_t teams, bool joins) {
+  const size_t ring = size_t(stages(dim, masked)) * (teams * cell_bytes(dim) + (masked ? kWarps * mask_bytes(tiles) : 0));
+  const size_t join = joins ? size_t(kWarps) * 8 * tiles * (dim + 4) * 4 : 0;
+  return ring > join ? ring : join;
+}
+
+template <typename T, int D, int FMT, int NT>
+void attend_rows(const AttendArg& a, const Shape& sh, dim3 grid, cudaStream_t s) {
+  const size_t smem = attend_smem(D, NT, a.mask != nullptr, kWarps / sh.mg, sh.kg > 1);
+  if (a.mask) k_attend<T, D, FMT, NT, true><<<grid, kThreads, smem, s>>>(a, sh);
+  else k_attend<T, D, FMT, NT, false><<<grid, kThreads, smem, s>>>(a, sh);
 }
 
 template <typename T, int D, int FMT>
@@ -523,12 +571,10 @@ cudaError_t attend_tile(const AttendArg& a, int sms, cudaStream_t s, uint64_t* l
   const uint64_t ctas = (sh.items + sh.hg - 1) / sh.hg;
   if (ctas == 0) return cudaSuccess;
   if (ctas > 0x7fffffffull) return cudaErrorInvalidConfiguration;
-  const bool masked = a.mask != nullptr;
-  const size_t ring = stages(D, masked) * (size_t(kWarps / sh.mg) * cell_bytes(D) + (masked ? kWarps * kMaskBytes : 0));
-  const size_t join = sh.kg > 1 ? size_t(kWarps) * 16 * (D + 4) * 4 : 0;
   const dim3 grid(unsigned(ctas), a.splits);
-  if (masked) k_attend<T, D, FMT, true><<<grid, kThreads, std::max(ring, join), s>>>(a, sh);
-  else k_attend<T, D, FMT, false><<<grid, kThreads, std::max(ring, join), s>>>(a, sh);
+  constexpr int most = most_tiles<T, D>();
+  if (sh.tiles == 1) attend_rows<T, D, FMT, 1>(a, sh, grid, s);
+  else attend_rows<T, D, FMT, most>(a, sh, grid, s);
   ++*launches;
   cudaError_t e = cudaGetLastError();
   if (e || a.splits == 1) return e;
@@ -578,9 +624,10 @@ __global__ __launch_bounds__(kThreads) void k_scores(ScoreArg a, uint32_t chunks
   w.first = warp;
   w.step = kWarps;
   const uint32_t n = w.count();
-  QTile<T, D> q;
+  QTile<T, D, 2> q;
   const T* base = static_cast<const T*>(a.a.q) + (q0 + row0) * a.a.pitch;
-  q.load(uint32_t(g) < n_rows ? base + g * a.a.pitch : nullptr, uint32_t(g + 8) < n_rows ? base + (g + 8) * a.a.pitch : nullptr, c, a.scale);
+#pragma unroll
+  for (int t = 0; t < 2; t++) q.load(t, uint32_t(8 * t + g) < n_rows ? base + (8 * t + g) * a.a.pitch : nullptr, c, a.scale);
   if (n == 0) return;
   uint8_t* ring = smem + warp * (S * CB);
   auto issue = [&](uint32_t i, uint32_t page) {
@@ -612,13 +659,15 @@ __global__ __launch_bounds__(kThreads) void k_scores(ScoreArg a, uint32_t chunks
     for (int r = 0; r < 16; r++) bias[r] = a.mask && uint32_t(r) < n_rows && pos < stride ? a.mask[at0 + r * stride + pos] : 0.0f;
     if (page != kNone) {
       const uint8_t* cell = ring + (i % S) * CB;
-      float s[4][4];
-      key_products<T, D, FMT>(q, cell, g, c, s);
+      float s[2][2][4];
+      key_products<T, D, FMT, 2>(q, cell, g, c, s);
       unit = reinterpret_cast<const float*>(cell + KB)[lane] * widened<FMT>();
 #pragma unroll
-      for (int J = 0; J < 4; J++)
+      for (int t = 0; t < 2; t++)
 #pragma unroll
-        for (int k = 0; k < 4; k++) tile[g + 8 * (k / 2)][8 * J + 4 * (k & 1) + c] = s[J][k] * q.unit[k / 2];
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+          for (int h = 0; h < 2; h++) tile[8 * t + 2 * c + h][8 * j + key_of(g)] = s[t][j / 2][2 * (j % 2) + h] * q.unit[t][h];
     }
     __syncwarp();
     if (pos < stride) {
@@ -656,11 +705,13 @@ cudaError_t scores_tile(const ScoreArg& a, int sms, cudaStream_t s, uint64_t* la
 
 template <typename T, int D, int FMT>
 cudaError_t prepare_tile() {
-  const int join = kWarps * 16 * (D + 4) * 4;
-  const int plain = kWarps * stages(D, false) * int(cell_bytes(D)), masked = kWarps * stages(D, true) * (int(cell_bytes(D)) + kMaskBytes);
+  constexpr int most = most_tiles<T, D>();
+  auto allow = [](auto kernel, int tiles, bool masked) {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(attend_smem(D, tiles, masked, kWarps, true)));
+  };
   cudaError_t e;
-  if ((e = cudaFuncSetAttribute(k_attend<T, D, FMT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, std::max(plain, join))) ||
-      (e = cudaFuncSetAttribute(k_attend<T, D, FMT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, std::max(masked, join))))
+  if ((e = allow(k_attend<T, D, FMT, 1, false>, 1, false)) || (e = allow(k_attend<T, D, FMT, 1, true>, 1, true)) ||
+      (e = allow(k_attend<T, D, FMT, most, false>, most, false)) || (e = allow(k_attend<T, D, FMT, most, true>, most, true)))
     return e;
   return cudaFuncSetAttribute(k_scores<T, D, FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                               int(kWarps * 3 * (kCell * D + kCell * 4)));

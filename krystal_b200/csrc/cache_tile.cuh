@@ -1,9 +1,15 @@
-// cache_tile.cuh — a warp's 16 question rows against a cell of 32 cached keys on
-// the tensor cores: fragments of questions and codes, and what a cell needs of
-// its scales. (mma.sync m16n8k16: a serving call has few question rows a key, so
-// that the cache's bytes bound it, and 8-bit codes become f16 in registers, where
-// these instructions take their operands; 5th-generation ones would need them
-// written back to shared memory for tiles of 64 or 128 rows that are mostly empty.)
+// cache_tile.cuh — a warp's question rows, 8 a tile, against a cell of 32 cached
+// keys on the tensor cores: fragments of questions and codes, and the walk over a
+// sequence's cells. (mma.sync m16n8k16: a serving call has few question rows a
+// key, so that the cache's bytes bound it, and 8-bit codes become f16 in
+// registers, where these instructions take their operands; 5th-generation ones
+// would need them written back to shared memory, for tiles of 64 or 128 rows that
+// are mostly empty.)
+//
+// Keys and values are the 16-row operand A, the questions and the weights the
+// 8-column operand B: S^T = K Q^T, O^T = V^T P^T. A single token's few heads then
+// fill the tile that 16 rows of questions would leave empty; every code is widened
+// once for all of the warp's tiles.
 //
 // Exactness. Codes are exact in f16. A question row is divided by a power of two
 // that brings its largest element into [1, 2); 16-bit questions are then exact
@@ -57,91 +63,111 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// The A fragments of a warp's 16 question rows. The dimensions' order within a
-// fragment is the keys': lane c's bytes of a key row, 4 a fragment.
-template <typename T, int D>
+// An 8 x 8 matrix of f16 transposed over the warp: lane (g, c) gives (g, 2c..),
+// and gets (2c.., g).
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// The key of a 16-key group that lane row g (the A operand's row g, or 8 + g less
+// 8) stands for: neighbouring rows (2c, 2c + 1) are the keys (c, c + 4), so that
+// the four value rows a lane reads with another's are neighbours, and a
+// quarter-warp's key rows fall on different banks.
+__device__ __forceinline__ uint32_t key_of(int g) { return uint32_t(g >> 1) + (uint32_t(g & 1) << 2); }
+
+// The B fragments of a warp's question rows, 8 a tile. The dimensions' order
+// within a fragment is the keys': lane c's bytes of a key row, 4 a fragment.
+template <typename T, int D, int NT>
 struct QTile {
   static constexpr bool kTwo = sizeof(T) == 4;  // f32: two f16 a value
   static constexpr int kSteps = D / 16;
-  uint32_t hi[kSteps][4], lo[kTwo ? kSteps : 1][4];
-  float unit[2];  // what a product of rows g and g + 8 is multiplied by
+  uint32_t hi[NT][kSteps][2], lo[kTwo ? NT : 1][kTwo ? kSteps : 1][2];
+  float unit[NT][2];  // what a product of rows 2c and 2c + 1 of a tile is multiplied by
 
-  // Dimension of element i (0..3) of lane c's piece of fragment s.
+  // Dimension of the first of the 4 elements of lane c's piece of fragment s.
   static __device__ __forceinline__ int dim(int s, int c) {
     return D == 32 ? 8 * c + 4 * s : D == 64 ? 16 * c + 4 * s : s < 4 ? 16 * c + 4 * s : 64 + 16 * c + 4 * (s - 4);
   }
 
-  // rows: the two rows of this lane, null where there is none. factor multiplies every score.
-  __device__ __forceinline__ void load(const T* r0, const T* r1, int c, float factor) {
+  // row: row g of tile t, null where there is none. factor multiplies every score.
+  __device__ __forceinline__ void load(int t, const T* row, int c, float factor) {
+    float x[kSteps][4], top = 0.0f;
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const T* r = h ? r1 : r0;
-      float x[kSteps][4], top = 0.0f;
+    for (int s = 0; s < kSteps; s++)
 #pragma unroll
-      for (int s = 0; s < kSteps; s++)
+      for (int i = 0; i < 4; i++) {
+        x[s][i] = row ? to_f32(row[dim(s, c) + i]) * (kTwo ? factor : 1.0f) : 0.0f;
+        top = fmaxf(top, fabsf(x[s][i]));
+      }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const uint32_t e = min(max(__float_as_uint(top) >> 23, 1u), 253u);
+    const float down = pow2_biased(254u - e), own = pow2_biased(e) * (kTwo ? 1.0f : factor);
+    unit[t][0] = __shfl_sync(0xffffffffu, own, 8 * c);
+    unit[t][1] = __shfl_sync(0xffffffffu, own, 8 * c + 4);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          x[s][i] = r ? to_f32(r[dim(s, c) + i]) * (kTwo ? factor : 1.0f) : 0.0f;
-          top = fmaxf(top, fabsf(x[s][i]));
+    for (int s = 0; s < kSteps; s++)
+#pragma unroll
+      for (int p = 0; p < 2; p++) {
+        const float y0 = x[s][2 * p] * down, y1 = x[s][2 * p + 1] * down;
+        hi[t][s][p] = pack(y0, y1);
+        if (kTwo) {
+          const __half2 h = *reinterpret_cast<const __half2*>(&hi[t][s][p]);
+          lo[kTwo ? t : 0][kTwo ? s : 0][p] = pack(y0 - __low2float(h), y1 - __high2float(h));
         }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const uint32_t e = min(max(__float_as_uint(top) >> 23, 1u), 253u);
-      const float down = pow2_biased(254u - e);
-      unit[h] = pow2_biased(e) * (kTwo ? 1.0f : factor);
-#pragma unroll
-      for (int s = 0; s < kSteps; s++)
-#pragma unroll
-        for (int p = 0; p < 2; p++) {
-          const float y0 = x[s][2 * p] * down, y1 = x[s][2 * p + 1] * down;
-          hi[s][2 * p + h] = pack(y0, y1);
-          if (kTwo) {
-            const __half2 top2 = *reinterpret_cast<const __half2*>(&hi[s][2 * p + h]);
-            lo[kTwo ? s : 0][2 * p + h] = pack(y0 - __low2float(top2), y1 - __high2float(top2));
-          }
-        }
-    }
+      }
   }
 };
 
-// s[J] += the 16 rows times the 8 keys of group J of the cell at `keys`. Lane
-// column n of group J stands for row 8 J + n / 2 + 4 (n % 2): the pairs of
-// neighbouring columns that a lane accumulates are then the rows (a, a + 4) that
-// value() pairs, and the quarter-warp's reads fall on different banks.
-template <typename T, int D, int FMT>
-__device__ __forceinline__ void key_products(const QTile<T, D>& q, const uint8_t* keys, int g, int c, float (&s)[4][4]) {
+// The words of one key row that lane c multiplies, a word a fragment.
+template <int D>
+__device__ __forceinline__ void key_words(const uint8_t* keys, uint32_t row, int c, uint32_t (&w)[D / 16]) {
+  if constexpr (D == 32) {
+    const uint2 v = *reinterpret_cast<const uint2*>(keys + key_at<D>(row, 8 * c));
+    w[0] = v.x; w[1] = v.y;
+  } else {
 #pragma unroll
-  for (int J = 0; J < 4; J++) {
-    const uint32_t row = 8 * J + (g >> 1) + ((g & 1) << 2);
-    uint32_t w[D / 16];
-    if constexpr (D == 32) {
-      const uint2 v = *reinterpret_cast<const uint2*>(keys + key_at<D>(row, 8 * c));
-      w[0] = v.x; w[1] = v.y;
-    } else {
-#pragma unroll
-      for (int p = 0; p < D / 64; p++) {
-        const uint4 v = *reinterpret_cast<const uint4*>(keys + key_at<D>(row, 64 * p + 16 * c));
-        w[4 * p] = v.x; w[4 * p + 1] = v.y; w[4 * p + 2] = v.z; w[4 * p + 3] = v.w;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; i++) s[J][i] = 0.0f;
-#pragma unroll
-    for (int k = 0; k < D / 16; k++) {
-      const uint32_t b0 = widen<FMT, false>(w[k]), b1 = widen<FMT, true>(w[k]);
-      mma(s[J], q.hi[k], b0, b1);
-      if constexpr (QTile<T, D>::kTwo) mma(s[J], q.lo[k], b0, b1);
+    for (int p = 0; p < D / 64; p++) {
+      const uint4 v = *reinterpret_cast<const uint4*>(keys + key_at<D>(row, 64 * p + 16 * c));
+      w[4 * p] = v.x; w[4 * p + 1] = v.y; w[4 * p + 2] = v.z; w[4 * p + 3] = v.w;
     }
   }
 }
 
-// o += the weights of 16 rows for the 16 keys of half u of a cell (A fragments,
-// hi and for f32 questions lo) times their values. Column n of tile t of o stands
-// for dimension n * (D / 8) + t.
-template <int D, int FMT, bool TWO>
-__device__ __forceinline__ void value_products(const uint32_t (&hi)[4], const uint32_t (&lo)[4], const uint8_t* values, int u,
-                                               int g, int c, float (&o)[D / 8][4]) {
-  constexpr int W = D / 32;  // words of 4 dimensions that a lane reads of each of its rows
+// s[t][u] = keys of 16-key group u of the cell at `keys` times the rows of tile t:
+// (key g, rows 2c, 2c + 1), (key g + 8, rows 2c, 2c + 1), keys by key_of.
+template <typename T, int D, int FMT, int NT>
+__device__ __forceinline__ void key_products(const QTile<T, D, NT>& q, const uint8_t* keys, int g, int c, float (&s)[NT][2][4]) {
+#pragma unroll
+  for (int u = 0; u < 2; u++) {
+    uint32_t w0[D / 16], w1[D / 16];
+    key_words<D>(keys, 16 * u + key_of(g), c, w0);
+    key_words<D>(keys, 16 * u + 8 + key_of(g), c, w1);
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) s[t][u][i] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < D / 16; k++) {
+      const uint32_t a[4] = {widen<FMT, false>(w0[k]), widen<FMT, false>(w1[k]), widen<FMT, true>(w0[k]), widen<FMT, true>(w1[k])};
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        mma(s[t][u], a, q.hi[t][k][0], q.hi[t][k][1]);
+        if constexpr (QTile<T, D, NT>::kTwo) mma(s[t][u], a, q.lo[t][k][0], q.lo[t][k][1]);
+      }
+    }
+  }
+}
+
+// o += the values of 16-key group u times the weights of the warp's rows (B
+// fragments, hi and for f32 questions lo). Rows g and g + 8 of tile m of o stand
+// for dimensions (D / 8) g + 2 m and the next.
+template <int D, int FMT, int NT, bool TWO>
+__device__ __forceinline__ void value_products(const uint32_t (&hi)[NT][2], const uint32_t (&lo)[TWO ? NT : 1][2],
+                                               const uint8_t* values, int u, int g, int c, float (&o)[NT][D / 16][4]) {
+  constexpr int W = D / 32;  // words of 4 dimensions that a lane reads of each of its keys
   uint32_t w[4][W];
 #pragma unroll
   for (int i = 0; i < 4; i++) {
@@ -162,13 +188,11 @@ __device__ __forceinline__ void value_products(const uint32_t (&hi)[4], const ui
     for (int y = 0; y < 2; y++) {  // bytes 2 y and 2 y + 1 of the word
       const uint32_t p0 = __byte_perm(w[0][x], w[1][x], y ? 0x7362 : 0x5140);
       const uint32_t p1 = __byte_perm(w[2][x], w[3][x], y ? 0x7362 : 0x5140);
-      const uint32_t b00 = widen<FMT, false>(p0), b01 = widen<FMT, false>(p1);
-      const uint32_t b10 = widen<FMT, true>(p0), b11 = widen<FMT, true>(p1);
-      mma(o[4 * x + 2 * y], hi, b00, b01);
-      mma(o[4 * x + 2 * y + 1], hi, b10, b11);
-      if constexpr (TWO) {
-        mma(o[4 * x + 2 * y], lo, b00, b01);
-        mma(o[4 * x + 2 * y + 1], lo, b10, b11);
+      const uint32_t a[4] = {widen<FMT, false>(p0), widen<FMT, true>(p0), widen<FMT, false>(p1), widen<FMT, true>(p1)};
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        mma(o[t][2 * x + y], a, hi[t][0], hi[t][1]);
+        if constexpr (TWO) mma(o[t][2 * x + y], a, lo[t][0], lo[t][1]);
       }
     }
 }
