@@ -10,9 +10,10 @@
 // are rounded to f16 lie below 2^15 whatever the scales are, and a large scale
 // that the mask or its score puts out of the running does not push the others
 // below f16's range. Subtracting B first keeps the digits of masks far from 0.
-// B, M, l and o run over a warp's cells (M is left alone while it rises by less
-// than 6 binary orders), then over the warps that share a row, then over the parts
-// that a long sequence is cut into.
+// B, M, l and o run over a warp's cells, then over the warps that share a row, then
+// over the parts that a long sequence is cut into. Within a warp M is left alone
+// while no score lies more than 6 binary orders above it, and B within 32, so that
+// most cells take a vote in place of the rows' maxima.
 //
 // A cell's bytes are read once by the team of warps that needs them, by 16-byte
 // asynchronous copies kStages - 1 cells ahead.
@@ -26,14 +27,14 @@ namespace cache {
 namespace {
 
 constexpr int kThreads = 256, kWarps = 8;
-constexpr float kLift = 8.0f, kSlack = 6.0f;
+constexpr float kLift = 8.0f, kSlack = 6.0f, kFar = 32.0f;
 constexpr int kLeastExp = -80;  // value scales below it keep their digits in f_j; l stays below 2^128
 
 // Cells a ring holds; a masked call's has the mask entries of each warp's rows
 // beside them, 36 floats apart so that what a warp reads at once lies on different banks.
 constexpr int kMaskPitch = 36;
 __host__ __device__ constexpr int mask_bytes(int tiles) { return 8 * tiles * kMaskPitch * 4; }
-__host__ __device__ constexpr int stages(int dim, bool masked) { return masked ? (dim == 32 ? 3 : 2) : dim == 32 ? 4 : 3; }
+__host__ __device__ constexpr int stages(int dim, bool masked) { return masked && dim > 32 ? 2 : 3; }
 
 // What a warp needs of one key of a cell: score = product * a * unit + e.
 struct KeyInfo {
@@ -113,7 +114,7 @@ __device__ __forceinline__ float weight_of(const Stat& s, float b, float m) {
 
 template <typename T, int FMT>
 __device__ __forceinline__ void put(const AttendArg& a, uint64_t question, uint32_t head, uint32_t dim, float o, float l) {
-  static_cast<T*>(a.out)[question * a.out_pitch + uint64_t(head) * a.c.dim + dim] = from_f32<T>(l > 0.0f ? o * (widened<FMT>() / l) : 0.0f);
+  static_cast<T*>(a.out)[question * a.out_pitch + uint64_t(head) * a.c.dim + dim] = from_f32<T>(l > 0.0f ? o * (1.0f / l) : 0.0f);
 }
 __device__ __forceinline__ void put_lse(const AttendArg& a, uint64_t question, uint32_t head, const Stat& s) {
   if (a.lse) a.lse[question * a.a.heads + head] = s.l > 0.0f ? (s.b + s.m - kLift) * kLn2 + logf(s.l) : -INFINITY;
@@ -122,6 +123,13 @@ __device__ __forceinline__ void put_lse(const AttendArg& a, uint64_t question, u
 // Part `part` of a row's results in the workspace: o [dim], then B, M, l.
 __device__ __forceinline__ float* part_of(const AttendArg& a, uint64_t question, uint32_t head, uint32_t part) {
   return a.work + ((question * a.a.heads + head) * a.splits + part) * (a.c.dim + 4);
+}
+
+// The largest of a tile row's values: over the lanes of one c.
+__device__ __forceinline__ float row_most(float x) {
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+  return x;
 }
 
 // N values of a row, one after another; wide: the place is 16-byte aligned.
@@ -198,6 +206,9 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED)) void k_attend(At
   const uint32_t open_end = MASKED ? uint32_t(min(uint64_t(u.len), u.stride)) : u.len;
   if (MASKED) {
     if (lane < R) s_mask[warp][lane] = uint64_t((row0 + lane) / group) * u.stride;
+    // rows that are not there are shut: what a vote sees of them must not change from call to call
+    for (uint32_t r = n_rows; r < uint32_t(R); r++)
+      for (int k = 0; k < S; k++) reinterpret_cast<float*>(biases + k * mask_bytes(NT))[r * kMaskPitch + lane] = kShut;
     __syncwarp();
   }
   auto issue = [&](uint32_t i, uint32_t page, uint32_t block) {
@@ -218,11 +229,12 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED)) void k_attend(At
     }
     copy_commit();
   };
+  uint32_t ahead[S - 1];  // the pages of the cells that are on their way
   if (n) {
 #pragma unroll
     for (uint32_t i = 0; i + 1 < S; i++) {
-      const uint32_t page = w.page_of(0, i), block = w.block_of(0, i);
-      issue(i, i < n ? page : kNone, block);
+      ahead[i] = w.page_of(0, i);
+      issue(i, ahead[i], w.block_of(0, i));
     }
   }
   QTile<T, D, NT> q;
@@ -252,8 +264,11 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED)) void k_attend(At
     w.advance(i);
     copy_wait<S - 2>();
     meet(team, sh.mg);
-    const uint32_t next = w.page_of(i, S - 1), page = w.page_of(i, 0), block = w.block_of(i, 0);
-    issue(i + S - 1, i + S - 1 < n ? next : kNone, MASKED ? w.block_of(i, S - 1) : 0);
+    const uint32_t page = ahead[0], block = w.block_of(i, 0);
+#pragma unroll
+    for (int k = 0; k + 2 < S; k++) ahead[k] = ahead[k + 1];
+    ahead[S - 2] = w.page_of(i, S - 1);  // none behind the last
+    issue(i + S - 1, ahead[S - 2], MASKED ? w.block_of(i, S - 1) : 0);
     if (!n_rows || page == kNone) continue;
     const uint8_t* cell = ring + (i % S) * CB;
     const uint64_t pos = uint64_t(block) * kPage + w.half(i) * kCell;
@@ -264,7 +279,7 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED)) void k_attend(At
       KeyInfo k;
       k.re = pow2_biased(254u - e);
       k.f = vs * k.re;
-      k.a = scales[lane] * widened<FMT>();
+      k.a = scales[lane];
       k.e = float(int(e) - 127);
       if (pos + lane >= open_end) k = KeyInfo{0.0f, -INFINITY, 0.0f, 0.0f};
       info[lane] = k;
@@ -283,56 +298,60 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED)) void k_attend(At
           s[t][j / 2][2 * (j % 2) + h] = fmaf(s[t][j / 2][2 * (j % 2) + h] * key[j].a, q.unit[t][h], key[j].e);
     }
     if (MASKED) {
-      // entries are read twice rather than kept: their registers would spill
       const float* bias = reinterpret_cast<const float*>(biases + (i % S) * mask_bytes(NT)) + 2 * c * kMaskPitch + key_of(g);
 #pragma unroll
       for (int t = 0; t < NT; t++) {
-        auto entry = [&](int j, int h) {
-          const float x = bias[(8 * t + h) * kMaskPitch + 8 * j];
-          return key[j].e > -INFINITY && x > kBlocked ? fminf(x, -kBlocked) * kLog2e : -INFINITY;
-        };
+        float x[4][2], most[2];
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-          float most = fmaxf(fmaxf(entry(0, h), entry(1, h)), fmaxf(entry(2, h), entry(3, h)));
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, x));
-          const float was = top[t][h];
-          top[t][h] = fmaxf(was, most);
-          if (was != top[t][h]) high[t][h] = was == -INFINITY ? -INFINITY : high[t][h] + (was - top[t][h]);  // measured from the new one
 #pragma unroll
           for (int j = 0; j < 4; j++) {
-            const float x = entry(j, h);
-            float& y = s[t][j / 2][2 * (j % 2) + h];
-            y = x > -INFINITY ? y + (x - top[t][h]) : -INFINITY;
+            const float y = bias[(8 * t + h) * kMaskPitch + 8 * j];
+            x[j][h] = key[j].e > -INFINITY && y > kBlocked ? fminf(y, -kBlocked) * kLog2e : -INFINITY;
+          }
+          most[h] = fmaxf(fmaxf(x[0][h], x[1][h]), fmaxf(x[2][h], x[3][h]));
+        }
+        if (__any_sync(0xffffffffu, most[0] > top[t][0] + kFar || most[1] > top[t][1] + kFar)) {
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            const float was = top[t][h];
+            top[t][h] = fmaxf(was, row_most(most[h]));
+            if (was != top[t][h]) high[t][h] = was == -INFINITY ? -INFINITY : high[t][h] + (was - top[t][h]);  // measured from the new one
           }
         }
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            float& y = s[t][j / 2][2 * (j % 2) + h];
+            y = x[j][h] > -INFINITY ? y + (x[j][h] - top[t][h]) : -INFINITY;
+          }
       }
     }
-    bool moved = false;
-    float keep[NT][2];
+    float most[NT][2];
+    bool above = false;
 #pragma unroll
     for (int t = 0; t < NT; t++)
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        float most = fmaxf(fmaxf(s[t][0][h], s[t][0][2 + h]), fmaxf(s[t][1][h], s[t][1][2 + h]));
-#pragma unroll
-        for (int x = 4; x < 32; x <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, x));
-        keep[t][h] = 1.0f;
-        if (most > high[t][h] + kSlack) {
-          keep[t][h] = high[t][h] == -INFINITY ? 0.0f : ex2(high[t][h] - most);
-          high[t][h] = most;
-          moved = true;
-        }
+        most[t][h] = fmaxf(fmaxf(s[t][0][h], s[t][0][2 + h]), fmaxf(s[t][1][h], s[t][1][2 + h]));
+        above |= most[t][h] > high[t][h] + kSlack;
       }
-    if (__any_sync(0xffffffffu, moved)) {
+    if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
       for (int t = 0; t < NT; t++) {
+        float keep[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const float now = fmaxf(high[t][h], row_most(most[t][h]));
+          keep[h] = now == high[t][h] ? 1.0f : ex2(high[t][h] - now);
+          high[t][h] = now;
+          sum[t][h] *= keep[h];
+        }
 #pragma unroll
         for (int m = 0; m < MT; m++)
 #pragma unroll
-          for (int k = 0; k < 4; k++) o[t][m][k] *= keep[t][k % 2];
-        sum[t][0] *= keep[t][0];
-        sum[t][1] *= keep[t][1];
+          for (int k = 0; k < 4; k++) o[t][m][k] *= keep[k % 2];
       }
     }
 #pragma unroll
@@ -379,7 +398,7 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED)) void k_attend(At
         const uint64_t question = u.q0 + (row0 + r) / group;
         const uint32_t head = u.kv * group + (row0 + r) % group;
         const Stat st{top[t][h], high[t][h], sum[t][h]};
-        const float unit = parts > 1 ? 1.0f : st.l > 0.0f ? widened<FMT>() / st.l : 0.0f;
+        const float unit = parts > 1 ? 1.0f : st.l > 0.0f ? 1.0f / st.l : 0.0f;
         float run[NB];
 #pragma unroll
         for (int k = 0; k < NB; k++) run[k] = o[t][k / 2][2 * (k % 2) + h] * unit;
@@ -501,7 +520,7 @@ __global__ __launch_bounds__(kThreads) void k_join(AttendArg a, uint32_t per) {
       for (uint32_t k = 0; k < n; k++) {
         const float y = __shfl_sync(0xffffffffu, add, k);
 #pragma unroll
-        for (int e = 0; e < D / 32; e++) acc[e] = fmaf(y, y > 0.0f ? x[k * (D + 4) + 32 * e] : 0.0f, acc[e]);
+        for (int e = 0; e < D / 32; e++) acc[e] = fmaf(y, x[k * (D + 4) + 32 * e], acc[e]);
       }
     }
   }
@@ -661,7 +680,7 @@ __global__ __launch_bounds__(kThreads) void k_scores(ScoreArg a, uint32_t chunks
       const uint8_t* cell = ring + (i % S) * CB;
       float s[2][2][4];
       key_products<T, D, FMT, 2>(q, cell, g, c, s);
-      unit = reinterpret_cast<const float*>(cell + KB)[lane] * widened<FMT>();
+      unit = reinterpret_cast<const float*>(cell + KB)[lane];
 #pragma unroll
       for (int t = 0; t < 2; t++)
 #pragma unroll

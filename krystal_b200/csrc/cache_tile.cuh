@@ -39,8 +39,7 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
 }
 
 // Bytes 0 and 1 (HIGH: 2 and 3) of a word of codes as two f16. i8: 0x6400 + byte
-// is 1024 + byte, less 1152. e4m3: exponent and mantissa moved to an f16's place
-// are the value times 2^-8 (subnormals too); callers multiply it back.
+// is 1024 + byte, less 1152. e4m3: the instruction for it.
 template <int FMT, bool HIGH>
 __device__ __forceinline__ uint32_t widen(uint32_t w) {
   if (FMT == kI8) {
@@ -48,11 +47,11 @@ __device__ __forceinline__ uint32_t widen(uint32_t w) {
     const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2{__ushort_as_half(0x6480), __ushort_as_half(0x6480)});
     return *reinterpret_cast<const uint32_t*>(&y);
   }
-  const uint32_t x = __byte_perm(w, 0u, HIGH ? 0x3424 : 0x1404);
-  return ((x >> 1) & 0x3f803f80u) | (x & 0x80008000u);
+  uint32_t y;
+  const unsigned short x = static_cast<unsigned short>(HIGH ? w >> 16 : w);
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(y) : "h"(x));
+  return y;
 }
-template <int FMT>
-__device__ __forceinline__ constexpr float widened() { return FMT == kI8 ? 1.0f : 256.0f; }
 
 // 2^x, x an integer in [-126, 127] given as its biased exponent.
 __device__ __forceinline__ float pow2_biased(uint32_t e) { return __uint_as_float(e << 23); }
