@@ -11,7 +11,6 @@
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
 
 #include "cache_args.h"
 #include "policy_args.h"
@@ -56,19 +55,27 @@ __device__ __forceinline__ float tame(float x) {
   return x != x ? 0.0f : fminf(fmaxf(x, -kMostValue), kMostValue);
 }
 
-template <int FMT>
-__device__ __forceinline__ uint32_t encode(float x, float scale) {
-  const float y = __fdiv_rn(x, scale);
-  if (FMT == kI8) return uint32_t(__float2int_rn(y) + 128);
-  return __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
-}
+constexpr float kPlainScale = 8.673617379884035e-19f;  // 2^-60: remainders of x / scale stay in f32's range above it
 
+// The values over their scale of a word of four codes.
 template <int FMT>
-__device__ __forceinline__ float decode(uint32_t code) {
-  if (FMT == kI8) return float(int(code) - 128);
-  // the exponent and mantissa of e4m3 in an f16's place are the value times 2^-8
-  const uint32_t h = ((code & 0x80u) << 8) | ((code & 0x7fu) << 7);
-  return __half2float(__ushort_as_half(static_cast<unsigned short>(h))) * 256.0f;
+__device__ __forceinline__ void values_of(uint32_t w, float (&v)[4]) {
+  if (FMT == kI8) {
+    // 0x4b000000 + byte is 2^23 + byte
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      v[i] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + i)) - 8388736.0f;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      uint32_t h;
+      const unsigned short x = static_cast<unsigned short>(i ? w >> 16 : w);
+      asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(x));
+      const __half2 y = *reinterpret_cast<const __half2*>(&h);
+      v[2 * i] = __low2float(y);
+      v[2 * i + 1] = __high2float(y);
+    }
+  }
 }
 
 // Rows that sequence s holds.
@@ -77,13 +84,19 @@ __device__ __forceinline__ uint32_t length_of(const Table& t, uint32_t s) {
   return n < t.max_len ? n : t.max_len;
 }
 
-// The last s with off[s] <= i (off ascending, off[0] <= i).
+// The last s with off[s] <= i (off ascending, off[0] <= i), by a whole warp: 32
+// places are looked at together, so that a thousand sequences take two trips to
+// memory, not ten.
 __device__ __forceinline__ uint32_t owner_of(const uint64_t* off, uint32_t n, uint64_t i) {
-  uint32_t lo = 0, hi = n;
+  const uint32_t lane = threadIdx.x & 31;
+  uint32_t lo = 0, hi = n;  // off[lo] <= i < off[hi], or hi = n
   while (hi - lo > 1) {
-    const uint32_t mid = (lo + hi) / 2;
-    if (off[mid] <= i) lo = mid;
-    else hi = mid;
+    const uint32_t step = (hi - lo + 32) / 33;  // lane k looks at lo + (k + 1) step
+    const uint64_t at = uint64_t(lo) + uint64_t(lane + 1) * step;
+    const uint32_t under = __popc(__ballot_sync(0xffffffffu, at < hi && off[at < hi ? at : lo] <= i));
+    const uint64_t top = uint64_t(lo) + uint64_t(under + 1) * step;
+    if (top < hi) hi = uint32_t(top);
+    lo += under * step;
   }
   return lo;
 }

@@ -15,162 +15,286 @@ namespace {
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr uint32_t kRowsMost = 64;  // source rows a CTA of k_write or k_read looks after
 
-// Row i of a Rows: its sequence and position there; false where there is none.
+// Where the rows of a chunk lie. Called by a whole CTA, for `chunk` rows from
+// `first` on; the first warps fill in the places of a row each.
 struct Place {
   uint32_t seq;
-  int64_t pos;
-  uint64_t nth, count;  // the row's number among its sequence's rows of the call, and their number
+  int64_t pos;           // in the sequence
+  uint64_t nth, count;   // the row's number among its sequence's rows of the call, and their number
+  bool mine, inside;     // a row of the call; at a position that the table has a page for
 };
-__device__ __forceinline__ bool place_of(const Table& t, const Rows& r, uint64_t i, Place* p) {
-  if (i >= r.rows) return false;
+__device__ __forceinline__ Place place_of(const Table& t, const Rows& r, uint64_t first, uint32_t chunk) {
+  Place p{};
+  const uint64_t i = first + threadIdx.x;
+  p.mine = threadIdx.x < chunk && i < r.rows && (r.off ? i >= r.off[0] && i < r.off[t.seqs] : i < t.seqs);
   if (r.off) {
-    if (i < r.off[0] || i >= r.off[t.seqs]) return false;
-    p->seq = owner_of(r.off, t.seqs, i);
-    const uint64_t first = r.off[p->seq];
-    p->nth = i - first;
-    p->count = r.off[p->seq + 1] - first;
+    // the warp's first row by a search, the others among the 32 sequences behind
+    // its owner where these reach far enough
+    const uint32_t lane = threadIdx.x & 31;
+    const uint32_t who = __ballot_sync(0xffffffffu, p.mine);
+    if (!who) return p;
+    const uint32_t base = owner_of(r.off, t.seqs, __shfl_sync(0xffffffffu, i, __ffs(who) - 1));
+    const uint64_t ends = base + 1 + lane <= t.seqs ? r.off[base + 1 + lane] : ~0ull;  // of sequence base + lane
+    const bool near = __shfl_sync(0xffffffffu, ends, 31) > __shfl_sync(0xffffffffu, i, 31 - __clz(who));
+    uint32_t over = 0;  // sequences of the window that end at or before the row
+    if (near) {
+#pragma unroll
+      for (int k = 16; k; k >>= 1) {
+        const uint64_t e = __shfl_sync(0xffffffffu, ends, over + k - 1);
+        if (e <= i) over += k;
+      }
+      p.seq = base + over;
+    } else {
+      for (int k = 0; k < 32; k++) {
+        const uint64_t row = __shfl_sync(0xffffffffu, i, k);
+        if (!(who >> k & 1)) continue;
+        const uint32_t s = owner_of(r.off, t.seqs, row);
+        if (lane == uint32_t(k)) p.seq = s;
+      }
+    }
+    if (p.mine) {
+      const uint64_t from = r.off[p.seq];
+      p.nth = i - from;
+      p.count = r.off[p.seq + 1] - from;
+    }
   } else {
-    if (i >= t.seqs) return false;
-    p->seq = uint32_t(i);
-    p->nth = 0;
-    p->count = 1;
+    p.seq = uint32_t(i);
+    p.count = 1;
   }
-  p->pos = (r.starts ? int64_t(r.starts[p->seq]) : int64_t(t.lengths[p->seq]) - int64_t(p->count)) + int64_t(p->nth);
-  return p->pos >= 0 && p->pos < int64_t(uint64_t(t.pitch) * kPage);
+  if (p.mine) {
+    p.pos = (r.starts ? int64_t(r.starts[p.seq]) : int64_t(t.lengths[p.seq]) - int64_t(p.count)) + int64_t(p.nth);
+    p.inside = p.pos >= 0 && p.pos < int64_t(uint64_t(t.pitch) * kPage);
+  }
+  return p;
 }
 
-// N elements from p as one or two 16-byte loads (WIDE: p is aligned to them), or one by one.
-template <typename T, int N, bool WIDE>
-__device__ __forceinline__ void load(const T* p, float (&x)[N]) {
+// Eight elements as they lie, by 16-byte loads (WIDE: aligned to them) or one by one.
+template <typename T>
+struct Eight {
+  uint4 v[sizeof(T) / 2];
+  __device__ __forceinline__ float at(int i) const { return to_f32(reinterpret_cast<const T*>(v)[i]); }
+};
+template <typename T, bool WIDE>
+__device__ __forceinline__ Eight<T> load8(const T* p) {
+  Eight<T> x;
   if (WIDE) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    const T* e = reinterpret_cast<const T*>(&v);
 #pragma unroll
-    for (int i = 0; i < N; i++) x[i] = to_f32(e[i]);
+    for (int i = 0; i < int(sizeof(T) / 2); i++) x.v[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
   } else {
 #pragma unroll
-    for (int i = 0; i < N; i++) x[i] = to_f32(p[i]);
+    for (int i = 0; i < 8; i++) reinterpret_cast<T*>(x.v)[i] = p[i];
+  }
+  return x;
+}
+
+// The largest of N magnitudes; NaN if one is.
+__device__ __forceinline__ float most_of(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(fabsf(b)));
+  return y;
+}
+
+// x / top rounded to f32: q + (x - q top) / top with q = x / top nearly (Markstein).
+// Where the remainder would leave f32's range the scale's floor holds anyway.
+template <int FMT>
+__device__ __forceinline__ float scale_of(float x) {
+  constexpr float kTop = FMT == kI8 ? kTopI8 : kTopE4M3, kOver = 1.0f / kTop;
+  const float q = x * kOver;
+  return fmaxf(fmaf(fmaf(-q, kTop, x), kOver, q), kLeastScale);
+}
+
+// N codes of a row, 4 a word. The quotient is
+// formed the same way from the rounded reciprocal; for scales so small that the
+// remainder could leave f32's range it is the division itself (not for rows of
+// zeros, which are common).
+template <int FMT, int N>
+__device__ __forceinline__ void codes_of(float (&x)[N], float scale, bool zero, uint32_t (&w)[N / 4]) {
+  float y[N] = {};
+  if (scale > kPlainScale || zero) {
+    const float r = __frcp_rn(scale);
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const float q = x[i] * r;
+      y[i] = fmaf(fmaf(-q, scale, x[i]), r, q);
+    }
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < N; i++) {  // the division stands here once, the registers move on past it
+      const float q = __fdiv_rn(x[0], scale);
+#pragma unroll
+      for (int k = 0; k + 1 < N; k++) {
+        x[k] = x[k + 1];
+        y[k] = y[k + 1];
+      }
+      y[N - 1] = q;
+    }
+  }
+  if (FMT == kI8) {
+    // adding 1.5 * 2^23 leaves the nearest integer, halves to the even, in the low bits
+    uint32_t b[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) b[i] = __float_as_uint(y[i] + (12582912.0f + 128.0f));
+#pragma unroll
+    for (int p = 0; p < N / 4; p++)
+      w[p] = __byte_perm(__byte_perm(b[4 * p], b[4 * p + 1], 0x0040), __byte_perm(b[4 * p + 2], b[4 * p + 3], 0x0040), 0x5410);
+  } else {
+#pragma unroll
+    for (int p = 0; p < N / 4; p++) {
+      uint32_t lo, hi;
+      asm("{.reg .b16 t; cvt.rn.satfinite.e4m3x2.f32 t, %2, %1; cvt.u32.u16 %0, t;}" : "=r"(lo) : "f"(y[4 * p]), "f"(y[4 * p + 1]));
+      asm("{.reg .b16 t; cvt.rn.satfinite.e4m3x2.f32 t, %2, %1; cvt.u32.u16 %0, t;}" : "=r"(hi) : "f"(y[4 * p + 2]), "f"(y[4 * p + 3]));
+      w[p] = __byte_perm(lo, hi, 0x5410);
+    }
   }
 }
 
-// One warp a page and head: the call's rows of that page quantised into its
-// cells, then the bounds of all the rows the page holds. A CTA looks at `chunk`
-// source rows and takes the pages whose first new row is among them, so that
-// every page has one writer and the pages need not be listed beforehand.
+// Bounds that take in the 8 keys' dimensions of two words of codes.
+template <int FMT>
+__device__ __forceinline__ void widen_bounds(const uint32_t (&w)[2], float scale, float (&lo)[8], float (&hi)[8]) {
+#pragma unroll
+  for (int p = 0; p < 2; p++) {
+    float v[4];
+    values_of<FMT>(w[p], v);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      lo[4 * p + i] = fminf(lo[4 * p + i], v[i] * scale);
+      hi[4 * p + i] = fmaxf(hi[4 * p + i], v[i] * scale);
+    }
+  }
+}
+
+// One warp the keys or the values of a page and head: the call's rows of that page
+// quantised into its cells and, with the keys, the bounds of all the rows the page
+// holds. A CTA looks at `chunk` source rows and takes the pages whose first new row
+// is among them, so that every page has one writer and the pages need not be listed
+// beforehand. kAhead passes of 8 elements a lane are on their way together (4 a lane
+// took twice the instructions for f32), and no code of the call's rows is read again.
+constexpr int kWriteThreads = 128;
+
 template <typename T, int D, int FMT, bool WIDE>
-__global__ __launch_bounds__(kThreads) void k_write(Store c, Table t, Rows r, uint32_t chunk) {
-  constexpr int V = 16 / sizeof(T), L = D / V, RP = 32 / L;  // elements a lane, lanes a row, rows a pass
-  __shared__ uint32_t s_count, s_seq[kRowsMost], s_pos[kRowsMost], s_new[kRowsMost], s_held[kRowsMost];
+__global__ __launch_bounds__(kWriteThreads, 7) void k_write(Store c, Table t, Rows r, uint32_t chunk) {
+  constexpr int V = 8, L = D / V, RP = 32 / L;  // elements a lane, lanes a row, rows a pass
+  constexpr int kAhead = sizeof(T) == 4 ? 2 : 4;
+  __shared__ uint32_t s_count, s_seq[kRowsMost], s_pos[kRowsMost], s_new[kRowsMost];
   __shared__ uint64_t s_row[kRowsMost];
   if (threadIdx.x == 0) s_count = 0;
   __syncthreads();
-  if (threadIdx.x < chunk) {
-    const uint64_t i = uint64_t(blockIdx.x) * chunk + threadIdx.x;
-    Place p;
-    if (place_of(t, r, i, &p)) {
-      const uint32_t at = uint32_t(p.pos % kPage);
-      if (at == 0 || p.nth == 0) {
-        const uint32_t k = atomicAdd(&s_count, 1u);
-        s_seq[k] = p.seq;
-        s_pos[k] = uint32_t(p.pos);
-        s_new[k] = uint32_t(min(uint64_t(kPage - at), min(p.count, r.rows - (i - p.nth)) - p.nth));
-        s_held[k] = min(kPage, t.lengths[p.seq] - (uint32_t(p.pos) - at));
-        s_row[k] = i;
-      }
+  if (threadIdx.x < (chunk + 31) / 32 * 32) {
+    const uint64_t i0 = uint64_t(blockIdx.x) * chunk;
+    const Place p = place_of(t, r, i0, chunk);
+    const uint32_t at = uint32_t(p.pos % kPage);
+    if (p.inside && (at == 0 || p.nth == 0)) {
+      const uint32_t k = atomicAdd(&s_count, 1u);
+      s_seq[k] = p.seq;
+      s_pos[k] = uint32_t(p.pos);
+      s_new[k] = uint32_t(min(uint64_t(kPage - at), min(p.count, r.rows - (i0 + threadIdx.x - p.nth)) - p.nth));
+      s_row[k] = i0 + threadIdx.x;
     }
   }
   __syncthreads();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (uint32_t item = warp; item < s_count * c.heads; item += kWarps) {
-    const uint32_t k = item / c.heads, head = item % c.heads;
+  const uint32_t b = (lane % L) * V, sub = lane / L, items = s_count * c.heads * 2;
+  for (uint32_t item = warp; item < items; item += kWriteThreads / 32) {
+    const uint32_t which = item & 1u, k = item / 2 / c.heads, head = item / 2 - k * c.heads;
     const uint32_t page = t.table[uint64_t(s_seq[k]) * t.pitch + s_pos[k] / kPage];
     if (page >= c.pages) continue;
     const uint32_t first = s_pos[k] % kPage, n = s_new[k];
     uint8_t* cells = cell_of<D>(c, page, head, 0);
-    for (uint32_t j0 = 0; j0 < n; j0 += RP) {
-      const uint32_t j = j0 + lane / L, b = (lane % L) * V;
-      const bool there = j < n;
-      const uint32_t row = first + j;
-      uint8_t* cell = cells + (row / kCell) * cell_bytes(D);
+    const T* from = static_cast<const T*>(which ? r.values : r.keys) + s_row[k] * r.pitch + head * D + b;
+    float lo[V], hi[V];
 #pragma unroll
-      for (int which = 0; which < 2; which++) {
-        float x[V];
-        float top = 0.0f;
-        if (there)
-          load<T, V, WIDE>(static_cast<const T*>(which ? r.values : r.keys) + (s_row[k] + j) * r.pitch + head * D + b, x);
-#pragma unroll
-        for (int i = 0; i < V; i++) {
-          x[i] = there ? tame(x[i]) : 0.0f;
-          top = fmaxf(top, fabsf(x[i]));
-        }
-#pragma unroll
-        for (int o = 1; o < L; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float scale = fmaxf(__fdiv_rn(top, FMT == kI8 ? kTopI8 : kTopE4M3), kLeastScale);
-        uint32_t w[V / 4] = {};
-#pragma unroll
-        for (int i = 0; i < V; i++) w[i / 4] |= encode<FMT>(x[i], scale) << (8 * (i % 4));
-        if (there) {
-          const uint32_t rc = row % kCell;
-          uint32_t* dst = reinterpret_cast<uint32_t*>(cell + which * kCell * D + (which ? value_at<D>(rc, b) : key_at<D>(rc, b)));
-#pragma unroll
-          for (int i = 0; i < V / 4; i++) dst[i] = w[i];
-          if (lane % L == 0) reinterpret_cast<float*>(cell + 2 * kCell * D)[which * kCell + rc] = scale;
-        }
-      }
-    }
-    __syncwarp();
-    // the bounds, from the codes as stored: 16 dimensions a lane
-    constexpr int LB = D / 16;
-    float lo[16], hi[16];
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
+    for (int i = 0; i < V; i++) {
       lo[i] = __int_as_float(0x7f800000);
       hi[i] = -lo[i];
     }
-    const uint32_t held = s_held[k], b = (lane % LB) * 16;
-    for (uint32_t row = lane / LB; row < held; row += 32 / LB) {
-      const uint8_t* cell = cells + (row / kCell) * cell_bytes(D);
-      const uint4 v = *reinterpret_cast<const uint4*>(cell + key_at<D>(row % kCell, b));
-      const float scale = reinterpret_cast<const float*>(cell + 2 * kCell * D)[row % kCell];
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    for (uint32_t j0 = 0; j0 < n; j0 += RP * kAhead) {
+      Eight<T> raw[kAhead];
 #pragma unroll
-      for (int i = 0; i < 16; i++) {
-        const float y = decode<FMT>((w[i / 4] >> (8 * (i % 4))) & 0xffu) * scale;
-        lo[i] = fminf(lo[i], y);
-        hi[i] = fmaxf(hi[i], y);
+      for (int x = 0; x < kAhead; x++) {
+        const uint32_t j = j0 + x * RP + sub;
+        raw[x] = j < n ? load8<T, WIDE>(from + j * r.pitch) : Eight<T>{};
       }
+#pragma unroll
+      for (int x = 0; x < kAhead; x++) {
+        if (j0 + x * RP >= n) break;
+        const uint32_t j = j0 + x * RP + sub, row = first + j, rc = row % kCell;
+        float y[V], top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+          y[i] = raw[x].at(i);
+          top = most_of(top, y[i]);
+        }
+        if (!(top <= kMostValue)) {
+          top = 0.0f;
+#pragma unroll
+          for (int i = 0; i < V; i++) {
+            y[i] = tame(y[i]);
+            top = fmaxf(top, fabsf(y[i]));
+          }
+        }
+#pragma unroll
+        for (int o = 1; o < L; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float scale = scale_of<FMT>(top);
+        uint32_t w[V / 4];
+        codes_of<FMT, V>(y, scale, top == 0.0f, w);
+        if (j < n) {
+          uint8_t* cell = cells + (row / kCell) * cell_bytes(D);
+          uint8_t* dst = cell + (which ? kCell * D + value_at<D>(rc, b) : key_at<D>(rc, b));
+          *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+          if (lane % L == 0) reinterpret_cast<float*>(cell + 2 * kCell * D)[which * kCell + rc] = scale;
+          if (!which) widen_bounds<FMT>(w, scale, lo, hi);
+        }
+      }
+    }
+    if (which) continue;
+    // rows that the page held before
+    for (uint32_t r0 = 0; r0 < first; r0 += RP * kAhead) {
+      uint32_t w[kAhead][V / 4];
+      float scale[kAhead];
+#pragma unroll
+      for (int x = 0; x < kAhead; x++) {
+        const uint32_t row = min(r0 + x * RP + sub, first - 1);  // the last one again where there is none
+        const uint8_t* cell = cells + (row / kCell) * cell_bytes(D);
+        const uint2 v = *reinterpret_cast<const uint2*>(cell + key_at<D>(row % kCell, b));
+        w[x][0] = v.x;
+        w[x][1] = v.y;
+        scale[x] = reinterpret_cast<const float*>(cell + 2 * kCell * D)[row % kCell];
+      }
+#pragma unroll
+      for (int x = 0; x < kAhead; x++) widen_bounds<FMT>(w[x], scale[x], lo, hi);
     }
     float* bounds = c.bounds + (uint64_t(page) * c.heads + head) * 2 * D;
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
+    for (int i = 0; i < V; i++)
 #pragma unroll
-      for (int o = LB; o < 32; o <<= 1) {
+      for (int o = L; o < 32; o <<= 1) {
         lo[i] = fminf(lo[i], __shfl_xor_sync(0xffffffffu, lo[i], o));
         hi[i] = fmaxf(hi[i], __shfl_xor_sync(0xffffffffu, hi[i], o));
       }
-      if (lane < LB) {
-        bounds[b + i] = lo[i];
-        bounds[D + b + i] = hi[i];
+    if (lane < L) {
+#pragma unroll
+      for (int p = 0; p < V / 4; p++) {
+        *reinterpret_cast<float4*>(bounds + b + 4 * p) = make_float4(lo[4 * p], lo[4 * p + 1], lo[4 * p + 2], lo[4 * p + 3]);
+        *reinterpret_cast<float4*>(bounds + D + b + 4 * p) = make_float4(hi[4 * p], hi[4 * p + 1], hi[4 * p + 2], hi[4 * p + 3]);
       }
     }
   }
 }
 
-// Rows read back: a CTA looks up where `chunk` rows lie, then its threads copy
-// 16 bytes of output each; rows that the sequence does not hold are 0.
+// Rows read back: a CTA looks up where `chunk` rows lie, then its threads copy 16
+// bytes of output each, of kAhead places at a time; rows that the sequence does
+// not hold are 0.
 template <typename T, int D, int FMT, bool WIDE>
 __global__ __launch_bounds__(kThreads) void k_read(Store c, Table t, Rows r, uint32_t chunk) {
-  constexpr int V = 16 / sizeof(T), L = D / V;
+  constexpr int V = 16 / sizeof(T), L = D / V, kAhead = 4;
   __shared__ uint64_t s_cell[kRowsMost];  // the cell of the row's first head
   __shared__ uint32_t s_at[kRowsMost];    // its row there; kNone: zeros, kNone - 1: not a row of the call
   const uint64_t row0 = uint64_t(blockIdx.x) * chunk;
-  if (threadIdx.x < chunk) {
-    Place p;
-    const uint64_t i = row0 + threadIdx.x;
-    const bool mine = i < r.rows && (r.off ? i >= r.off[0] && i < r.off[t.seqs] : i < t.seqs);
-    uint32_t at = mine ? kNone : kNone - 1;
+  if (threadIdx.x < (chunk + 31) / 32 * 32) {
+    const Place p = place_of(t, r, row0, chunk);
+    uint32_t at = p.mine ? kNone : kNone - 1;
     uint64_t cell = 0;
-    if (place_of(t, r, i, &p) && p.pos < int64_t(t.lengths[p.seq])) {
+    if (p.inside && p.pos < int64_t(t.lengths[p.seq])) {
       const uint32_t page = t.table[uint64_t(p.seq) * t.pitch + uint64_t(p.pos) / kPage];
       if (page < c.pages) {
         at = uint32_t(p.pos % kCell);
@@ -181,37 +305,58 @@ __global__ __launch_bounds__(kThreads) void k_read(Store c, Table t, Rows r, uin
     s_cell[threadIdx.x] = cell;
   }
   __syncthreads();
-  const uint32_t n = chunk * c.heads * L;
-  for (uint32_t e = threadIdx.x; e < n; e += kThreads) {
-    const uint32_t b = e % L * V, head = e / L % c.heads, j = e / (L * c.heads);
-    const uint32_t at = s_at[j];
-    if (at == kNone - 1) continue;
-    const uint8_t* cell = c.cells + (s_cell[j] + head * 2) * cell_bytes(D);
+  // a warp takes 32 / L heads or rows at a time: a place is (row, head), L lanes each
+  const uint32_t b = threadIdx.x % L * V, lanes = kThreads / L, places = chunk * c.heads;
+  for (uint32_t p0 = threadIdx.x / L; p0 < places; p0 += lanes * kAhead) {
+    uint32_t w[kAhead][2][V / 4];
+    float scale[kAhead][2];
+    T* to[kAhead][2];
 #pragma unroll
-    for (int which = 0; which < 2; which++) {
-      T* dst = static_cast<T*>(which ? r.values : r.keys);
-      if (!dst) continue;
-      dst += (row0 + j) * r.pitch + head * D + b;
-      T out[V];
-      uint32_t w[V / 4] = {};
-      float scale = 0.0f;
-      if (at != kNone) {
-        const uint32_t* src =
-            reinterpret_cast<const uint32_t*>(cell + which * kCell * D + (which ? value_at<D>(at, b) : key_at<D>(at, b)));
+    for (int x = 0; x < kAhead; x++) {
+      const uint32_t p = p0 + x * lanes, j = p / c.heads, head = p - j * c.heads;
+      const uint32_t at = p < places ? s_at[j] : kNone - 1;
+      const uint64_t dst = (row0 + j) * r.pitch + head * D + b;
+      to[x][0] = at == kNone - 1 || !r.keys ? nullptr : static_cast<T*>(r.keys) + dst;
+      to[x][1] = at == kNone - 1 || !r.values ? nullptr : static_cast<T*>(r.values) + dst;
+      const uint8_t* cell = c.cells + (at < kCell ? s_cell[j] + head * 2 : 0) * cell_bytes(D);
 #pragma unroll
-        for (int i = 0; i < V / 4; i++) w[i] = src[i];
-        scale = reinterpret_cast<const float*>(cell + 2 * kCell * D)[which * kCell + at];
-      }
+      for (int which = 0; which < 2; which++) {
+        scale[x][which] = 0.0f;
 #pragma unroll
-      for (int i = 0; i < V; i++)
-        out[i] = from_f32<T>(at == kNone ? 0.0f : decode<FMT>((w[i / 4] >> (8 * (i % 4))) & 0xffu) * scale);
-      if (WIDE) {
-        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(out);
-      } else {
-#pragma unroll
-        for (int i = 0; i < V; i++) dst[i] = out[i];
+        for (int i = 0; i < V / 4; i++) w[x][which][i] = FMT == kI8 ? 0x80808080u : 0u;
+        if (at < kCell && to[x][which]) {
+          const uint8_t* src = cell + which * kCell * D + (which ? value_at<D>(at, b) : key_at<D>(at, b));
+          if constexpr (V == 4) {
+            w[x][which][0] = __ldcs(reinterpret_cast<const uint32_t*>(src));
+          } else {
+            const uint2 v = __ldcs(reinterpret_cast<const uint2*>(src));
+            w[x][which][0] = v.x;
+            w[x][which][V / 4 - 1] = v.y;
+          }
+          scale[x][which] = reinterpret_cast<const float*>(cell + 2 * kCell * D)[which * kCell + at];
+        }
       }
     }
+#pragma unroll
+    for (int x = 0; x < kAhead; x++)
+#pragma unroll
+      for (int which = 0; which < 2; which++) {
+        if (!to[x][which]) continue;
+        alignas(16) T out[V];
+#pragma unroll
+        for (int i = 0; i < V / 4; i++) {
+          float value[4];
+          values_of<FMT>(w[x][which][i], value);
+#pragma unroll
+          for (int e = 0; e < 4; e++) out[4 * i + e] = from_f32<T>(value[e] * scale[x][which]);
+        }
+        if (WIDE) {
+          __stcs(reinterpret_cast<uint4*>(to[x][which]), *reinterpret_cast<const uint4*>(out));
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; i++) to[x][which][i] = out[i];
+        }
+      }
   }
 }
 
@@ -413,8 +558,8 @@ cudaError_t store_as(bool write, const Store& c, const Table& t, const Rows& r, 
   const uint64_t grid = (r.rows + chunk - 1) / chunk;
   if (grid > 0x7fffffffull) return cudaErrorInvalidConfiguration;
   if (write) {
-    if (wide) k_write<T, D, FMT, true><<<unsigned(grid), kThreads, 0, s>>>(c, t, r, chunk);
-    else k_write<T, D, FMT, false><<<unsigned(grid), kThreads, 0, s>>>(c, t, r, chunk);
+    if (wide) k_write<T, D, FMT, true><<<unsigned(grid), kWriteThreads, 0, s>>>(c, t, r, chunk);
+    else k_write<T, D, FMT, false><<<unsigned(grid), kWriteThreads, 0, s>>>(c, t, r, chunk);
   } else {
     if (wide) k_read<T, D, FMT, true><<<unsigned(grid), kThreads, 0, s>>>(c, t, r, chunk);
     else k_read<T, D, FMT, false><<<unsigned(grid), kThreads, 0, s>>>(c, t, r, chunk);
