@@ -204,8 +204,10 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED)) void k_attend(At
   uint8_t* biases = smem + kWarps / sh.mg * (S * CB) + warp * (S * mask_bytes(NT));  // a masked call's
   __shared__ uint64_t s_mask[MASKED ? kWarps : 1][R];  // where the rows' masks begin
   const uint32_t open_end = MASKED ? uint32_t(min(uint64_t(u.len), u.stride)) : u.len;
+  bool aligned = false;  // whether every row's mask begins at 16 bytes
   if (MASKED) {
     if (lane < R) s_mask[warp][lane] = uint64_t((row0 + lane) / group) * u.stride;
+    aligned = (reinterpret_cast<uintptr_t>(u.mask) | u.stride * 4) % 16 == 0;
     // rows that are not there are shut: what a vote sees of them must not change from call to call
     for (uint32_t r = n_rows; r < uint32_t(R); r++)
       for (int k = 0; k < S; k++) reinterpret_cast<float*>(biases + k * mask_bytes(NT))[r * kMaskPitch + lane] = kShut;
@@ -221,10 +223,21 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED)) void k_attend(At
       else if (sh.mg == 4) copy_cell<CB, 4>(dst, src, thread);
       else copy_cell<CB, 8>(dst, src, thread);
       if (MASKED) {
-        const uint64_t pos = uint64_t(block) * kPage + w.half(i) * kCell + lane;
-        uint8_t* to = biases + (i % S) * mask_bytes(NT) + 4 * lane;
-        if (pos < open_end)
-          for (uint32_t r = 0; r < n_rows; r++) copy4(to + r * (4 * kMaskPitch), u.mask + s_mask[warp][r] + pos);
+        const uint32_t pos = block * kPage + w.half(i) * kCell;  // below 2^32: the length is
+        uint8_t* to = biases + (i % S) * mask_bytes(NT);
+        if (aligned && pos + kCell <= open_end) {  // 4 rows at a time
+#pragma unroll
+          for (int r = 0; r < R; r += 4)
+            if (uint32_t(r + lane / 8) < n_rows)
+              copy16(to + (r + lane / 8) * (4 * kMaskPitch) + 16 * (lane % 8), u.mask + s_mask[warp][r + lane / 8] + pos + 4 * (lane % 8));
+        } else {
+          const bool in = pos + lane < open_end;
+          for (uint32_t r = 0; r < n_rows; r++) {
+            uint8_t* dst = to + r * (4 * kMaskPitch) + 4 * lane;
+            if (in) copy4(dst, u.mask + s_mask[warp][r] + pos + lane);
+            else *reinterpret_cast<float*>(dst) = kShut;
+          }
+        }
       }
     }
     copy_commit();
@@ -305,11 +318,10 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED)) void k_attend(At
 #pragma unroll
         for (int h = 0; h < 2; h++) {
 #pragma unroll
-          for (int j = 0; j < 4; j++) {
-            const float y = bias[(8 * t + h) * kMaskPitch + 8 * j];
-            x[j][h] = key[j].e > -INFINITY && y > kBlocked ? fminf(y, -kBlocked) * kLog2e : -INFINITY;
-          }
-          most[h] = fmaxf(fmaxf(x[0][h], x[1][h]), fmaxf(x[2][h], x[3][h]));
+          for (int j = 0; j < 4; j++) x[j][h] = bias[(8 * t + h) * kMaskPitch + 8 * j];
+          // a maximum passes NaN over, where it is not the only one: hence kShut
+          most[h] = fminf(fmaxf(fmaxf(fmaxf(kShut, x[0][h]), x[1][h]), fmaxf(x[2][h], x[3][h])), -kBlocked) * kLog2e;
+          if (!(most[h] > kBlocked * kLog2e)) most[h] = -INFINITY;
         }
         if (__any_sync(0xffffffffu, most[0] > top[t][0] + kFar || most[1] > top[t][1] + kFar)) {
 #pragma unroll
@@ -320,12 +332,14 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED)) void k_attend(At
           }
         }
 #pragma unroll
-        for (int j = 0; j < 4; j++)
+        for (int h = 0; h < 2; h++) {
+          const float from = top[t][h] == -INFINITY ? 0.0f : -top[t][h];
 #pragma unroll
-          for (int h = 0; h < 2; h++) {
+          for (int j = 0; j < 4; j++) {
             float& y = s[t][j / 2][2 * (j % 2) + h];
-            y = x[j][h] > -INFINITY ? y + (x[j][h] - top[t][h]) : -INFINITY;
+            y = x[j][h] > kBlocked ? y + (fminf(x[j][h], -kBlocked) * kLog2e + from) : -INFINITY;  // rounded as top is
           }
+        }
       }
     }
     float most[NT][2];
@@ -613,89 +627,103 @@ cudaError_t attend_tile(const AttendArg& a, int sms, cudaStream_t s, uint64_t* l
 
 // --- pointer scores --------------------------------------------------------------
 
-// A warp a cell of a sequence and 16 of its questions at a time; the tile passes
-// through shared memory so that masks are read and scores written 32 to a row.
+// 8 questions a warp, a cell at a time; `mg` warps with as many questions more
+// share the cells that their team brings, kg teams take turns at a sequence's cells
+// (64 f32 questions of 128 a bank of 4096: 8 warps a team; with the cells read once for
+// every 16 questions before, 110 us against 81). The products pass through shared
+// memory so that masks are read and scores written 32 to a row; the mask's entries
+// are on their way while the cell is multiplied.
 template <typename T, int D, int FMT>
-__global__ __launch_bounds__(kThreads) void k_scores(ScoreArg a, uint32_t chunks, uint32_t cells) {
+__global__ __launch_bounds__(kThreads, 2) void k_scores(ScoreArg a, uint32_t mg, uint32_t chunks, uint32_t cells) {
   constexpr int S = 3, KB = int(kCell) * D, CB = KB + int(kCell) * 4;  // keys and their scales
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float s_tile[kWarps][16][kCell + 1];
+  __shared__ float s_tile[kWarps][8][kCell + 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+  const uint32_t team = warp / mg, mi = warp % mg, kg = kWarps / mg;
   const uint32_t seq = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
   const uint64_t q0 = a.a.off ? a.a.off[seq] : seq, q1 = a.a.off ? a.a.off[seq + 1] : seq + 1;
   const uint32_t count = uint32_t(q1 - q0), rows = uint32_t(min(uint64_t(min(count, a.a.max_q)), a.a.questions > q0 ? a.a.questions - q0 : 0));
-  const uint32_t row0 = chunk * 16;
-  if (row0 >= rows) return;
+  if (chunk * 8 * mg >= rows) return;  // the whole CTA
+  const uint32_t row0 = (chunk * mg + mi) * 8, n_rows = row0 < rows ? min(8u, rows - row0) : 0;
   const uint64_t stride = (a.off[seq + 1] - a.off[seq]) / count;
   const uint32_t len = uint32_t(min(uint64_t(length_of(a.t, seq)), stride));
   const uint64_t end = (stride + kCell - 1) / kCell;  // cells of the row, those behind the bank's end included
-  const uint64_t at0 = a.off[seq] + row0 * stride;
-  const uint32_t n_rows = min(16u, rows - row0);
+  const uint64_t c0 = uint64_t(blockIdx.y) * cells;
+  if (c0 >= end) return;
 
   Walk w{};
   w.table = a.t.table + uint64_t(seq) * a.t.pitch;
   w.blocks = (len + kPage - 1) / kPage;
   w.pages = a.c.pages;
-  w.b0 = blockIdx.y * cells / 2;
-  const uint64_t c0 = uint64_t(blockIdx.y) * cells;
-  if (c0 >= end) return;
+  w.b0 = uint32_t(c0 / 2);
   w.cells = uint32_t(blockIdx.y + 1 == gridDim.y ? end - c0 : min(uint64_t(cells), end - c0));  // the last takes what the table does not bound
-  w.first = warp;
-  w.step = kWarps;
+  w.first = team;
+  w.step = kg;
   const uint32_t n = w.count();
-  QTile<T, D, 2> q;
-  const T* base = static_cast<const T*>(a.a.q) + (q0 + row0) * a.a.pitch;
-#pragma unroll
-  for (int t = 0; t < 2; t++) q.load(t, uint32_t(8 * t + g) < n_rows ? base + (8 * t + g) * a.a.pitch : nullptr, c, a.scale);
-  if (n == 0) return;
-  uint8_t* ring = smem + warp * (S * CB);
+  if (n == 0) return;  // the whole team
+  uint8_t* ring = smem + team * (S * CB);
   auto issue = [&](uint32_t i, uint32_t page) {
     if (page != kNone) {
       const uint8_t* src = cell_of<D>(a.c, page, 0, w.half(i));
       uint8_t* dst = ring + (i % S) * CB;
-#pragma unroll
-      for (int k = 0; k < KB / 512; k++) copy16(dst + 16 * (k * 32 + lane), src + 16 * (k * 32 + lane));
-      if (lane < 8) copy16(dst + KB + 16 * lane, src + 2 * KB + 16 * lane);
+      for (uint32_t k = mi * 32 + lane; k < CB / 16; k += mg * 32) copy16(dst + 16 * k, src + 16 * k + (k < KB / 16 ? 0 : KB));
     }
     copy_commit();
   };
   w.begin();
+  uint32_t ahead[S - 1];
 #pragma unroll
   for (uint32_t i = 0; i + 1 < S; i++) {
-    const uint32_t page = w.page_of(0, i);
-    issue(i, i < n ? page : kNone);
+    ahead[i] = w.page_of(0, i);
+    issue(i, ahead[i]);
   }
+  QTile<T, D, 1> q;
+  q.load(0, uint32_t(g) < n_rows ? static_cast<const T*>(a.a.q) + (q0 + row0 + g) * a.a.pitch : nullptr, c, a.scale);
   float (*tile)[kCell + 1] = s_tile[warp];
+  const uint64_t at0 = a.off[seq] + row0 * stride;
   for (uint32_t i = 0; i < n; i++) {
     w.advance(i);
     copy_wait<S - 2>();
-    __syncwarp();
-    const uint32_t next = w.page_of(i, S - 1), page = w.page_of(i, 0);
-    issue(i + S - 1, i + S - 1 < n ? next : kNone);
+    meet(team, mg);
+    const uint32_t page = ahead[0];
+    ahead[0] = ahead[1];
+    ahead[1] = w.page_of(i, S - 1);
+    issue(i + S - 1, ahead[1]);
     const uint64_t pos = (c0 + w.first + uint64_t(w.step) * i) * kCell + lane;
-    float unit = 0.0f, bias[16];  // the cell's mask entries, on their way while it is multiplied
+    const bool there = pos < stride;
+    float bias[8];
+    if (a.mask) {
+      const float* m = a.mask + at0 + pos;
 #pragma unroll
-    for (int r = 0; r < 16; r++) bias[r] = a.mask && uint32_t(r) < n_rows && pos < stride ? a.mask[at0 + r * stride + pos] : 0.0f;
-    if (page != kNone) {
+      for (int r = 0; r < 8; r++) {
+        bias[r] = there && uint32_t(r) < n_rows ? *m : 0.0f;
+        m += stride;
+      }
+    }
+    float unit = 0.0f;
+    if (page != kNone && n_rows) {
       const uint8_t* cell = ring + (i % S) * CB;
-      float s[2][2][4];
-      key_products<T, D, FMT, 2>(q, cell, g, c, s);
+      float s[1][2][4];
+      key_products<T, D, FMT, 1>(q, cell, g, c, s);
       unit = reinterpret_cast<const float*>(cell + KB)[lane];
 #pragma unroll
-      for (int t = 0; t < 2; t++)
+      for (int j = 0; j < 4; j++)
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-#pragma unroll
-          for (int h = 0; h < 2; h++) tile[8 * t + 2 * c + h][8 * j + key_of(g)] = s[t][j / 2][2 * (j % 2) + h] * q.unit[t][h];
+        for (int h = 0; h < 2; h++) tile[2 * c + h][8 * j + key_of(g)] = s[0][j / 2][2 * (j % 2) + h] * q.unit[0][h];
     }
     __syncwarp();
-    if (pos < stride) {
+    if (there) {
       const bool held = page != kNone && pos < len;
       float* out = a.scores + at0 + pos;
 #pragma unroll
-      for (int r = 0; r < 16; r++)
-        if (uint32_t(r) < n_rows)
-          out[r * stride] = held && bias[r] > kBlocked ? fmaf(tile[r][lane], unit, fminf(bias[r], -kBlocked)) : kShut;
+      for (int r = 0; r < 8; r++) {
+        if (uint32_t(r) < n_rows) {
+          float x = kShut;
+          if (held && (!a.mask || bias[r] > kBlocked)) x = fmaf(tile[r][lane], unit, a.mask ? fminf(bias[r], -kBlocked) : 0.0f);
+          *out = x;
+        }
+        out += stride;
+      }
     }
     __syncwarp();
   }
@@ -704,18 +732,19 @@ __global__ __launch_bounds__(kThreads) void k_scores(ScoreArg a, uint32_t chunks
 
 template <typename T, int D, int FMT>
 cudaError_t scores_tile(const ScoreArg& a, int sms, cudaStream_t s, uint64_t* launches) {
-  const uint32_t chunks = (a.a.max_q + 15) / 16;
+  const uint32_t warps = (a.a.max_q + 7) / 8, mg = warps <= 1 ? 1 : warps <= 2 ? 2 : warps <= 4 ? 4 : 8, kg = kWarps / mg;
+  const uint32_t chunks = (warps + mg - 1) / mg;
   const uint64_t ctas = uint64_t(a.t.seqs) * chunks;
   if (ctas > 0x7fffffffull) return cudaErrorInvalidConfiguration;
-  // rows may be longer than their bank: max_len does not bound them, the table does
-  const uint64_t all = uint64_t(a.t.pitch) * 2;
-  const uint64_t want = std::max<uint64_t>(1, uint64_t(sms) * 12 / std::max<uint64_t>(1, ctas));
-  uint64_t cells = std::max<uint64_t>(kWarps * 2, (all + want - 1) / want);
-  cells = (cells + kWarps * 2 - 1) / (kWarps * 2) * (kWarps * 2);
+  // parts of at least a cell a team (two for the pair of a block), for about 8 CTAs
+  // an SM; rows may be longer than their bank: the table bounds the parts
+  const uint64_t all = uint64_t(a.t.pitch) * 2, least = std::max(2u, kg);
+  const uint64_t want = std::max<uint64_t>(1, uint64_t(sms) * 8 / std::max<uint64_t>(1, ctas));
+  const uint64_t cells = (std::max<uint64_t>(least, (all + want - 1) / want) + least - 1) / least * least;
   const uint64_t parts = std::max<uint64_t>(1, (all + cells - 1) / cells);
-  if (parts > 65535) return cudaErrorInvalidConfiguration;
-  const size_t smem = size_t(kWarps) * 3 * (kCell * D + kCell * 4);
-  k_scores<T, D, FMT><<<dim3(unsigned(ctas), unsigned(parts)), kThreads, smem, s>>>(a, chunks, uint32_t(cells));
+  if (parts > 65535 || cells > 0x7fffffffull) return cudaErrorInvalidConfiguration;
+  const size_t smem = size_t(kg) * 3 * (kCell * D + kCell * 4);
+  k_scores<T, D, FMT><<<dim3(unsigned(ctas), unsigned(parts)), kThreads, smem, s>>>(a, mg, chunks, uint32_t(cells));
   ++*launches;
   return cudaGetLastError();
 }
