@@ -689,9 +689,8 @@ kc_status kc_cache_blocks(kc_handle* h, const kc_cache_view* cache, const kc_pag
  * twice counts twice; numbers outside the sequence count for nothing). A mask
  * entry at or below -1e29, or NaN, shuts its row out, larger ones than 1e29 count
  * as 1e29; rows behind the mask's end are shut out. Nothing left: out 0, lse
- * -infinity. Scores, sums and statistics are f32; for 16-bit questions the
- * weights are rounded to 11 bits before they meet the values, for f32 ones to
- * 22. */
+ * -infinity. Scores, sums and statistics are f32; the weights are rounded to 22
+ * bits before they meet the values, to 11 for bf16 questions. */
 typedef struct kc_attend_view {
   void* out;                 /* [questions, heads, head_dim], the questions' type, out_pitch elements apart (0 = dense) */
   uint64_t out_pitch;

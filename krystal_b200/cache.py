@@ -64,7 +64,8 @@ class BankCache:
         return self.storage[size - n:size].view(torch.float32).view(self.pages, self.kv_heads, 2, self.head_dim)
 
     def queued_on(self, backend) -> None:
-        if not any(r() is backend for r in self.backends):
+        if not self.backends or self.backends[-1]() is not backend:
+            self.backends = [r for r in self.backends if r() is not None and r() is not backend]
             self.backends.append(weakref.ref(backend))
 
     def __del__(self):

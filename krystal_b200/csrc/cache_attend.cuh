@@ -19,6 +19,7 @@
 // asynchronous copies kStages - 1 cells ahead.
 #pragma once
 #include <algorithm>
+#include <type_traits>
 
 #include "cache_tile.cuh"
 
@@ -162,16 +163,21 @@ __device__ __forceinline__ void copy_cell(uint8_t* dst, const uint8_t* src, uint
   }
 }
 
+// f16 pieces of a weight: two for f32 questions (22 bits) and for f16 ones, whose
+// output one piece's rounding would reach; bf16 outputs round 8 times more.
+template <typename T>
+__host__ __device__ constexpr int parts_of_weights() { return std::is_same<T, __nv_bfloat16>::value ? 1 : 2; }
+
 // CTAs of 256 threads that an SM should hold at once: what their rings and their
 // registers (without spilling) leave room for.
-__host__ __device__ constexpr int resident(int dim, int tiles, bool masked) {
-  return dim == 128 || (dim == 64 && tiles == 2 && masked) ? 1 : dim == 32 && tiles == 1 ? 3 : 2;
+__host__ __device__ constexpr int resident(int dim, int tiles, bool masked, int weights) {
+  return dim == 128 || (dim == 64 && tiles == 2 && (masked || weights == 2)) ? 1 : dim == 32 && tiles == 1 ? 3 : 2;
 }
 
 template <typename T, int D, int FMT, int NT, bool MASKED>
-__global__ __launch_bounds__(kThreads, resident(D, NT, MASKED)) void k_attend(AttendArg a, Shape sh) {
+__global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<T>())) void k_attend(AttendArg a, Shape sh) {
   constexpr int S = stages(D, MASKED), CB = int(cell_bytes(D)), MT = D / 16, NB = D / 8, R = 8 * NT;
-  constexpr bool kTwo = sizeof(T) == 4;
+  constexpr bool kTwo = parts_of_weights<T>() == 2;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ KeyInfo s_info[kWarps][kCell];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;

@@ -248,11 +248,12 @@ __global__ __launch_bounds__(kWriteThreads, 7) void k_write(Store c, Table t, Ro
     }
     if (which) continue;
     // rows that the page held before
-    for (uint32_t r0 = 0; r0 < first; r0 += RP * kAhead) {
-      uint32_t w[kAhead][V / 4];
-      float scale[kAhead];
+    constexpr int kBack = 8;
+    for (uint32_t r0 = 0; r0 < first; r0 += RP * kBack) {
+      uint32_t w[kBack][V / 4];
+      float scale[kBack];
 #pragma unroll
-      for (int x = 0; x < kAhead; x++) {
+      for (int x = 0; x < kBack; x++) {
         const uint32_t row = min(r0 + x * RP + sub, first - 1);  // the last one again where there is none
         const uint8_t* cell = cells + (row / kCell) * cell_bytes(D);
         const uint2 v = *reinterpret_cast<const uint2*>(cell + key_at<D>(row % kCell, b));
@@ -261,7 +262,7 @@ __global__ __launch_bounds__(kWriteThreads, 7) void k_write(Store c, Table t, Ro
         scale[x] = reinterpret_cast<const float*>(cell + 2 * kCell * D)[row % kCell];
       }
 #pragma unroll
-      for (int x = 0; x < kAhead; x++) widen_bounds<FMT>(w[x], scale[x], lo, hi);
+      for (int x = 0; x < kBack; x++) widen_bounds<FMT>(w[x], scale[x], lo, hi);
     }
     float* bounds = c.bounds + (uint64_t(page) * c.heads + head) * 2 * D;
 #pragma unroll
@@ -369,17 +370,34 @@ __device__ __forceinline__ unsigned long long order_key(double s) {
 
 constexpr uint32_t kAsk = 8;  // questions of a sequence that a cluster scores at once
 
-// The `left` largest of n keys (left < n) of one question, by one warp: a radix
-// select, 8 bits a pass from the highest bit in which two keys differ, until a
-// bin is taken whole. An entry is taken if its key's known bits lie above
-// limit's, or equal them and it is among the first `ties` that do.
+// A group of `warps` warps of a CTA that selects for one question: warp `nth` of
+// it, lane `lane`, meeting at the named barrier `id`.
+struct Group {
+  uint32_t id, warps, nth, lane;
+  __device__ __forceinline__ void meet() const {
+    if (warps == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(warps * 32) : "memory");
+  }
+};
+// What the group shares.
+struct Pick {
+  uint32_t bin[256];
+  unsigned long long both[kWarps], any[kWarps];
+  uint32_t more[kWarps], ties[kWarps];
+};
+
+// The `left` largest of n keys (left < n) of one question: a radix select, 8 bits a
+// pass from the highest bit in which two keys differ, until a bin is taken whole.
+// An entry is taken if its key's known bits lie above limit's, or equal them and it
+// is among the first `ties` that do.
 struct Cut {
   unsigned long long known, limit;
   uint32_t ties;
 };
-__device__ __forceinline__ Cut cut_of(const unsigned long long* key, uint32_t n, uint32_t left, uint32_t* bin, uint32_t lane) {
+__device__ __forceinline__ Cut cut_of(const unsigned long long* key, uint32_t n, uint32_t left, Pick& p, const Group& g) {
   unsigned long long both = ~0ull, any = 0;
-  for (uint32_t b = lane; b < n; b += 32) {
+  const uint32_t thread = g.nth * 32 + g.lane, step = g.warps * 32;
+  for (uint32_t b = thread; b < n; b += step) {
     both &= key[b];
     any |= key[b];
   }
@@ -388,26 +406,33 @@ __device__ __forceinline__ Cut cut_of(const unsigned long long* key, uint32_t n,
     both &= __shfl_xor_sync(0xffffffffu, both, o);
     any |= __shfl_xor_sync(0xffffffffu, any, o);
   }
+  if (g.lane == 0) {
+    p.both[g.nth] = both;
+    p.any[g.nth] = any;
+  }
+  for (uint32_t i = thread; i < 256; i += step) p.bin[i] = 0;
+  g.meet();
+  for (uint32_t w = 0; w < g.warps; w++) {
+    both &= p.both[w];
+    any |= p.any[w];
+  }
   if (both == any) return Cut{~0ull, any, left};  // all are equal
   int shift = 64 - __clzll(static_cast<long long>(both ^ any)) - 8;  // of the 8 bits that begin with the first that differs
   if (shift < 0) shift = 0;
   Cut c{shift + 8 < 64 ? ~0ull << (shift + 8) : 0ull, 0, left};
   c.limit = any & c.known;
   for (;;) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) bin[lane * 8 + i] = 0;
-    __syncwarp();
-    for (uint32_t b = lane; b < n; b += 32)
-      if ((key[b] & c.known) == c.limit) atomicAdd(&bin[uint32_t(key[b] >> shift) & 255u], 1u);
-    __syncwarp();
+    for (uint32_t b = thread; b < n; b += step)
+      if ((key[b] & c.known) == c.limit) atomicAdd(&p.bin[uint32_t(key[b] >> shift) & 255u], 1u);
+    g.meet();
     uint32_t own[8], sum = 0;  // lane 0 has the highest bins
 #pragma unroll
-    for (int i = 0; i < 8; i++) sum += own[i] = bin[255 - (lane * 8 + i)];
+    for (int i = 0; i < 8; i++) sum += own[i] = p.bin[255 - (g.lane * 8 + i)];
     uint32_t upto = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= uint32_t(o)) upto += y;
+      if (g.lane >= uint32_t(o)) upto += y;
     }
     const uint32_t who = __ffs(__ballot_sync(0xffffffffu, upto >= c.ties)) - 1;
     uint32_t above = upto - sum, pick = 0, held = 0;
@@ -416,7 +441,7 @@ __device__ __forceinline__ Cut cut_of(const unsigned long long* key, uint32_t n,
     for (int i = 0; i < 8; i++) {
       if (!found && above + own[i] >= c.ties) {
         found = true;
-        pick = 255 - (lane * 8 + i);
+        pick = 255 - (g.lane * 8 + i);
         held = own[i];
       }
       if (!found) above += own[i];
@@ -430,7 +455,9 @@ __device__ __forceinline__ Cut cut_of(const unsigned long long* key, uint32_t n,
     c.limit &= c.known;
     if (held == c.ties || shift == 0) return c;
     shift = shift > 8 ? shift - 8 : 0;
-    __syncwarp();
+    g.meet();  // the bins are read
+    for (uint32_t i = thread; i < 256; i += step) p.bin[i] = 0;
+    g.meet();
   }
 }
 
@@ -444,13 +471,14 @@ __device__ __forceinline__ Cut cut_of(const unsigned long long* key, uint32_t n,
 // reads each block's bounds once for them: 4 lanes a block, 16 bytes of the
 // smallest and of the largest keys a lane and step, so that 8 blocks of a warp are
 // on their way at once. The scores go, as keys that order alike, to the shared
-// memory of the CTA that selects for the question, a warp a question. The newest
+// memory of the CTA that selects for the question, with as many of its warps as the
+// other questions leave. The newest
 // blocks are the sequence's last, so they follow whatever is selected.
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads) void k_blocks(BlockArg a, uint32_t ask, uint32_t chunks, uint32_t most) {
   extern __shared__ unsigned long long s_key[];  // [questions of this CTA][most]
   __shared__ double s_q[kAsk][2][D];
-  __shared__ uint32_t s_bin[kWarps][256];
+  __shared__ Pick s_pick[kWarps];
   cg::cluster_group cluster = cg::this_cluster();
   const uint32_t rank = cluster.block_rank(), ctas = cluster.num_blocks();
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -474,10 +502,13 @@ __global__ __launch_bounds__(kThreads) void k_blocks(BlockArg a, uint32_t ask, u
     s_q[i / D][1][i % D] = down;
   }
   cluster.sync();
-  const uint32_t part = lane & 3;
-  for (uint32_t b0 = (rank * kWarps + warp) * 8; b0 < scored; b0 += ctas * kWarps * 8) {
-    const uint32_t b = b0 + lane / 4;
-    const uint32_t page = b < scored ? a.t.table[uint64_t(seq) * a.t.pitch + b] : kNone;
+  const uint32_t part = lane & 3, stride = ctas * kWarps * 8;
+  const uint32_t* table = a.t.table + uint64_t(seq) * a.t.pitch;
+  uint32_t b = (rank * kWarps + warp) * 8 + lane / 4;
+  uint32_t ahead = b < scored ? table[b] : kNone;
+  for (uint32_t b0 = (rank * kWarps + warp) * 8; b0 < scored; b0 += stride, b += stride) {
+    const uint32_t page = ahead;
+    ahead = b + stride < scored ? table[b + stride] : kNone;
     const bool there = page < a.c.pages;
     constexpr int F = D / 16;
     float4 lo[F], hi[F];
@@ -517,35 +548,61 @@ __global__ __launch_bounds__(kThreads) void k_blocks(BlockArg a, uint32_t ask, u
     }
   }
   cluster.sync();
-  const uint32_t k = rank + ctas * warp;
-  if (k >= nq) return;
-  const unsigned long long* key = s_key + uint64_t(warp) * most;
+  const uint32_t here = rank < nq ? (nq - rank + ctas - 1) / ctas : 0;  // questions of this CTA
+  if (here == 0) return;
+  Group g{0, here == 1 ? 8u : here == 2 ? 4u : here <= 4 ? 2u : 1u, 0, lane};
+  const uint32_t local = warp / g.warps, k = rank + ctas * local;
+  if (local >= here) return;
+  g.id = 1 + local;
+  g.nth = warp % g.warps;
+  const unsigned long long* key = s_key + uint64_t(local) * most;
   uint32_t* out = a.blocks + ((row0 + k) * a.c.heads + head) * a.count;
-  const uint32_t under = (1u << lane) - 1;
-  uint32_t at = 0;
+  const uint32_t under = (1u << lane) - 1, thread = g.nth * 32 + lane, step = g.warps * 32;
+  uint32_t total = 0;
   if (scored == 0) {  // all that there are
-    for (uint32_t b = lane; b < n; b += 32) out[b] = b;
-    at = n;
+    for (uint32_t x = thread; x < n; x += step) out[x] = x;
+    total = n;
   } else {
-    if (a.count > last) {
-      const Cut c = cut_of(key, scored, a.count - last, s_bin[warp], lane);
-      uint32_t even = 0;
-      for (uint32_t b0 = 0; b0 < scored; b0 += 32) {
-        const uint32_t b = b0 + lane;
-        const unsigned long long x = b < scored ? key[b] & c.known : 0;
-        const bool tie = b < scored && x == c.limit, more = b < scored && x > c.limit;
-        const uint32_t ties = __ballot_sync(0xffffffffu, tie);
-        const bool take = more || (tie && even + __popc(ties & under) < c.ties);
+    total = a.count - last;
+    if (total) {
+      Pick& p = s_pick[local];
+      const Cut c = cut_of(key, scored, total, p, g);
+      // each warp takes a run of the blocks; it begins behind what the warps before it take
+      const uint32_t run = ((scored + 31) / 32 + g.warps - 1) / g.warps * 32, from = g.nth * run, to = min(from + run, scored);
+      uint32_t at = 0, even = 0;
+      if (g.warps > 1) {
+        uint32_t more = 0, ties = 0;
+        for (uint32_t x0 = from; x0 < to; x0 += 32) {
+          const unsigned long long x = x0 + lane < to ? key[x0 + lane] & c.known : 0;
+          more += __popc(__ballot_sync(0xffffffffu, x0 + lane < to && x > c.limit));
+          ties += __popc(__ballot_sync(0xffffffffu, x0 + lane < to && x == c.limit));
+        }
+        if (lane == 0) {
+          p.more[g.nth] = more;
+          p.ties[g.nth] = ties;
+        }
+        g.meet();
+        for (uint32_t w = 0; w < g.nth; w++) {
+          at += p.more[w];
+          even += p.ties[w];
+        }
+        at += min(even, c.ties);
+      }
+      for (uint32_t x0 = from; x0 < to; x0 += 32) {
+        const unsigned long long x = x0 + lane < to ? key[x0 + lane] & c.known : 0;
+        const bool tie = x0 + lane < to && x == c.limit, over = x0 + lane < to && x > c.limit;
+        const uint32_t mask = __ballot_sync(0xffffffffu, tie);
+        const bool take = over || (tie && even + __popc(mask & under) < c.ties);
         const uint32_t took = __ballot_sync(0xffffffffu, take);
-        if (take) out[at + __popc(took & under)] = b;
+        if (take) out[at + __popc(took & under)] = x0 + lane;
         at += __popc(took);
-        even += __popc(ties);
+        even += __popc(mask);
       }
     }
-    for (uint32_t b = scored + lane; b < n; b += 32) out[at + b - scored] = b;
-    at += n - scored;
+    for (uint32_t x = scored + thread; x < n; x += step) out[total + x - scored] = x;
+    total += n - scored;
   }
-  for (uint32_t i = at + lane; i < a.count; i += 32) out[i] = kNone;
+  for (uint32_t x = total + thread; x < a.count; x += step) out[x] = kNone;
 }
 
 template <typename T, int D, int FMT>
