@@ -171,13 +171,13 @@ __host__ __device__ constexpr int parts_of_weights() { return std::is_same<T, __
 // CTAs of 256 threads that an SM should hold at once: what their rings and their
 // registers (without spilling) leave room for.
 __host__ __device__ constexpr int resident(int dim, int tiles, bool masked, int weights) {
-  return dim == 128 || (dim == 64 && tiles == 2 && (masked || weights == 2)) ? 1 : dim == 32 && tiles == 1 ? 3 : 2;
+  return dim == 128 || (dim == 64 && tiles == 2 && (masked || weights == 2)) ? 1 : dim == 32 && tiles == 1 && !masked ? 3 : 2;
 }
 
 template <typename T, int D, int FMT, int NT, bool MASKED>
 __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<T>())) void k_attend(AttendArg a, Shape sh) {
   constexpr int S = stages(D, MASKED), CB = int(cell_bytes(D)), MT = D / 16, NB = D / 8, R = 8 * NT;
-  constexpr bool kTwo = parts_of_weights<T>() == 2;
+  constexpr bool kTwo = parts_of_weights<T>() == 2, kApart = sizeof(T) == 4;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ KeyInfo s_info[kWarps][kCell];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
@@ -374,6 +374,9 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
           for (int k = 0; k < 4; k++) o[t][m][k] *= keep[k % 2];
       }
     }
+    // f32 outputs: a cell's products are summed by themselves. The tensor cores'
+    // sums truncate, and one sum over 16 cells was off by 1.2e-6, this by 4e-7.
+    float part_o[kApart ? NT : 1][kApart ? MT : 1][4] = {};
 #pragma unroll
     for (int v = 0; v < 2; v++) {
       uint32_t hi[NT][2], lo[kTwo ? NT : 1][2];
@@ -395,7 +398,16 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
           }
         }
       }
-      value_products<D, FMT, NT, kTwo>(hi, lo, cell + kCell * D, v, g, c, o);
+      if constexpr (kApart) value_products<D, FMT, NT, kTwo>(hi, lo, cell + kCell * D, v, g, c, part_o);
+      else value_products<D, FMT, NT, kTwo>(hi, lo, cell + kCell * D, v, g, c, o);
+    }
+    if constexpr (kApart) {
+#pragma unroll
+      for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+          for (int k = 0; k < 4; k++) o[t][m][k] += part_o[t][m][k];
     }
     __syncwarp();
   }
