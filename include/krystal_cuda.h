@@ -717,6 +717,42 @@ kc_status kc_cache_scores(kc_handle* h, const kc_cache_view* cache, const kc_pag
                           const kc_question_view* questions, const uint64_t* off, const float* mask, float scale,
                           float* scores);
 
+/* A turn of many sessions whose banks lie in caches: what BrainSession.think
+ * (host/session.ts:128-181) does with a frame, without encoding the records of
+ * earlier turns again. `batch` (DEVICE pointers, as for kc_forward_batch_device)
+ * has a frame a session with the turn's records alone, in any order and of either
+ * kind; table.lengths (sequence f = frame f) count the bank records among them
+ * already. These are appended: what each mixer block attends (its projections of
+ * the pooled bank keys and values) to mixer[block], caches of 4 heads of 32; the
+ * selector's projections of the keys, with the pooled values, to `selector`, one
+ * head of 128; the same table for all. The questions are answered over all rows
+ * that their session holds: p[i] (question i in batch order, table.max_length
+ * entries a row, 0 behind the bank's end) is their distribution or, under
+ * `sampling` (DEVICE row limits; NULL: the whole distribution), their policy;
+ * index as kc_draw_device leaves it, by batch.uniforms or the first largest entry.
+ * batch.mask: [questions, table.max_length] entries, NULL = open; a schema x band
+ * rule is refused (a cache keeps neither).
+ * Products run on the tensor cores at fp32-class accuracy at every precision of
+ * the handle; the banks are 8-bit, so that p lies within a few percent of
+ * kc_forward_batch's and close decisions may differ. The call waits for the
+ * batch's sizes and for the pipeline's error word, and releases the resident
+ * batch. A turn that is refused or fails may have appended: repeat it with the
+ * same lengths. Weight changes do not reach rows that are cached. */
+typedef struct kc_bank_view {
+  const kc_cache_view* mixer;  /* HOST [mixer_blocks] */
+  kc_cache_view selector;
+  kc_page_table table;         /* sequences = batch.frames, max_length <= KC_MAX_ROW */
+} kc_bank_view;
+typedef struct kc_bank_out {
+  float* p;                    /* DEVICE [questions, table.max_length] */
+  uint32_t* index;             /* DEVICE [questions] or NULL */
+  float* logp;                 /* DEVICE [questions] or NULL */
+  uint64_t q_capacity;         /* rows of p, index and logp */
+  uint64_t total_q, total_r;   /* written by the call: questions, bank records appended */
+} kc_bank_out;
+kc_status kc_bank_turn(kc_handle* h, const kc_batch_view* batch, const kc_bank_view* bank, const kc_sampling* sampling,
+                       kc_bank_out* out);
+
 /* KRY1 checkpoints (host/checkpoint.ts:17-116): 11 little-endian u32 header
  * words (magic "KRY1" = 0x4b525931, version 1, hiddenSize, ffnSize,
  * encoderBlocks, mixerBlocks, headCount, headDim, routeKindCount, tokenRows

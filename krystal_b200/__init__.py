@@ -6,6 +6,7 @@ logic the reference keeps on the host (frame packing, weight init, the
 selection mask). The CUDA library is required: constructing a backend raises
 when it is missing; nothing falls back to the CPU.
 """
+from .banks import SessionBanks
 from .cache import BankCache
 from .frame import (FrameBatch, HostFrame, HostFrameError, HostRecord, HostToken, PAD_TOKEN, QUERY_BAND,
                     compile_active_frame, pack_frame_batch, pack_host_frame, record_ranges)
@@ -18,7 +19,7 @@ __all__ = [
     "RECORD_WIDTH", "compile_active_frame", "pack_frame_batch", "pack_host_frame", "record_ranges",
     "BRAIN_FORWARD_CONFIG", "BrainForwardConfig", "BrainForwardWeights", "create_brain_forward_weights",
     "embedding_table_bases", "weight_layout", "cuda_backend", "CudaBrainBackend", "BrainSession", "GradList",
-    "Sampling", "BankCache",
+    "Sampling", "BankCache", "SessionBanks",
 ]
 
 

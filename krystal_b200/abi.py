@@ -52,7 +52,7 @@ EXPORTS = ("kc_abi_version", "kc_create", "kc_sync", "kc_encode", "kc_select", "
            "kc_copy_weights", "kc_stream_create_ex", "kc_stream_read_stats", "kc_draw_device", "kc_draw",
            "kc_draw_batch", "kc_policy_loss", "kc_set_policy", "kc_clip_workspace", "kc_clip_grads", "kc_cache_bytes",
            "kc_cache_write", "kc_cache_read", "kc_cache_blocks", "kc_cache_attend_workspace", "kc_cache_attend",
-           "kc_cache_scores")
+           "kc_cache_scores", "kc_bank_turn")
 
 
 class KrystalCudaError(RuntimeError):
@@ -235,6 +235,15 @@ class KcAttendView(C.Structure):
                 ("block_count", C.c_uint32), ("scale", C.c_float), ("workspace", P), ("workspace_bytes", C.c_uint64)]
 
 
+class KcBankView(C.Structure):
+    _fields_ = [("mixer", C.POINTER(KcCacheView)), ("selector", KcCacheView), ("table", KcPageTable)]
+
+
+class KcBankOut(C.Structure):
+    _fields_ = [("p", P), ("index", P), ("logp", P), ("q_capacity", C.c_uint64), ("total_q", C.c_uint64),
+                ("total_r", C.c_uint64)]
+
+
 _lib = None
 
 
@@ -318,6 +327,8 @@ def load(path: str | os.PathLike | None = None) -> C.CDLL:
     lib.kc_cache_attend_workspace.restype = C.c_uint64
     lib.kc_cache_attend.argtypes = cache + [C.POINTER(KcQuestionView), C.POINTER(KcAttendView)]
     lib.kc_cache_scores.argtypes = cache + [C.POINTER(KcQuestionView), P, P, C.c_float, P]
+    lib.kc_bank_turn.argtypes = [P, C.POINTER(KcBatchView), C.POINTER(KcBankView), C.POINTER(KcSampling),
+                                 C.POINTER(KcBankOut)]
     for name in ("kc_create", "kc_sync", "kc_encode", "kc_select", "kc_forward_batch", "kc_forward_batch_device",
                  "kc_set_stream", "kc_synchronize", "kc_profile", "kc_profile_read", "kc_select_noalloc",
                  "kc_set_precision", "kc_backward", "kc_backward_batch_device", "kc_learn_frame_stats",
@@ -326,7 +337,7 @@ def load(path: str | os.PathLike | None = None) -> C.CDLL:
                  "kc_inject_wait_expiry", "kc_learn_plan", "kc_learn_accumulate_rows", "kc_learn_apply",
                  "kc_copy_weights", "kc_stream_create_ex", "kc_stream_read_stats", "kc_draw_device", "kc_draw",
                  "kc_draw_batch", "kc_policy_loss", "kc_set_policy", "kc_clip_grads", "kc_cache_write", "kc_cache_read",
-                 "kc_cache_blocks", "kc_cache_attend", "kc_cache_scores"):
+                 "kc_cache_blocks", "kc_cache_attend", "kc_cache_scores", "kc_bank_turn"):
         getattr(lib, name).restype = C.c_int
     _lib = lib
     return lib

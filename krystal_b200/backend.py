@@ -497,6 +497,26 @@ class CudaBrainBackend:
         abi.check(self._lib.kc_cache_scores(self._h, self._cache(cache), C.byref(table), C.byref(questions), off, mask,
                                             scale, scores), self._h)
 
+    def bank_turn(self, frames: int, records: int, rec_off: int, token_ids: int, field_roles: int, schema_ids: int,
+                  band_ids: int, mixer: Sequence[BankCache], selector: BankCache, table: abi.KcPageTable, p: int,
+                  q_capacity: int, index: int | None = None, logp: int | None = None, uniforms: int | None = None,
+                  mask: int | None = None, sampling: Sampling | None = None, word_ids: int | None = None,
+                  word_alpha: float = 0.0) -> abi.KcBankOut:
+        """kc_bank_turn: a turn of many sessions whose banks lie in caches (raw
+        device pointers; banks.SessionBanks keeps the caches and their pages)."""
+        if len(mixer) != self.config.mixer_blocks:
+            raise ValueError(f"a bank has a cache per mixer block ({self.config.mixer_blocks})")
+        for c in (*mixer, selector):
+            self._cache(c)
+        views = (abi.KcCacheView * max(1, len(mixer)))(*(c.view for c in mixer))
+        bank = abi.KcBankView(views, selector.view, table)
+        bv = abi.KcBatchView(frames, records, rec_off, token_ids, field_roles, schema_ids, band_ids, None, None,
+                             uniforms, word_ids, float(word_alpha), mask)
+        out = abi.KcBankOut(p, index, logp, q_capacity)
+        s = C.byref(sampling.device_struct()) if sampling is not None else None
+        abi.check(self._lib.kc_bank_turn(self._h, C.byref(bv), C.byref(bank), s, C.byref(out)), self._h)
+        return out
+
     # --- packed ragged batches ------------------------------------------------
     def forward_batch(self, batch: FrameBatch, rule: MaskRule | None = None, uniforms=None,
                       want_query_output: bool = False, p_capacity: int | None = None, word_ids=None,

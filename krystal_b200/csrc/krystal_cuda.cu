@@ -113,6 +113,7 @@ struct Workspace {
   DevBuf tile_row, row_rc;
   // activations
   DevBuf x, qkv, bk, bv, mk, mv, qstate, mq, mh, sq, sk, p, index, gather;
+  DevBuf turn_attend, turn_work, turn_off;  // kc_bank_turn: attention outputs, its workspace, score offsets
   // weight-row scatter staging
   DevBuf rows_val, rows_off;
   // certification flags per frame, and the list of frames to recompute
@@ -1125,11 +1126,12 @@ void launch_select_fast(kc_handle* h, Workspace& ws, const DevBatch& b, const kc
   h->launches++;
 }
 
-// The forward on the tensor cores (tc_gemm.cuh, fast.cuh): the selector
-// raises ws.flags[f] for frames whose decisions it cannot certify.
-kc_status forward_fast(kc_handle* h, Workspace& ws, const DevBatch& b, const kc::FrameTotals& tot) {
+// The records of a packed batch on the tensor cores (tc_gemm.cuh, fast.cuh): the
+// encoder blocks and the poolings, into ws.bk, ws.bv and ws.qstate. Clears the
+// error word and the frames' flags.
+kc_status encode_fast(kc_handle* h, Workspace& ws, const DevBatch& b, const kc::FrameTotals& tot) {
   const Dims& d = h->d;
-  const uint64_t N = b.records, T = tot.t, Q = tot.q, R = tot.r;
+  const uint64_t N = b.records, T = tot.t;
   const uint32_t H = d.h, FF = d.ffn;
   KC_CHECK(build_images(h));
   KC_TRY(cudaMemsetAsync(h->d_err, 0, sizeof(int), h->stream), "memset");
@@ -1141,7 +1143,7 @@ kc_status forward_fast(kc_handle* h, Workspace& ws, const DevBatch& b, const kc:
     launch_embed(h, ws, b, x, T);
   }
   const float attn_scale = float(1.0 / std::sqrt(double(d.hd)));
-  const int enc_m = 0, mix_m = 3 * int(d.enc), sel_m = mix_m + 5 * int(d.mix);
+  const int enc_m = 0;
   if (attn_fusable(h) && d.enc > 0) KC_CHECK(attn_prepare(h, ws, T));
   for (uint32_t blk = 0; blk < d.enc && T > 0; blk++) {
     if (attn_fusable(h)) {  // q|k|v, attention and the residual in one kernel: q|k|v stay on chip
@@ -1184,6 +1186,18 @@ kc_status forward_fast(kc_handle* h, Workspace& ws, const DevBatch& b, const kc:
     kc::k_pool_fast<<<unsigned((N + 7) / 8), 256, 0, h->stream>>>(pa);
     h->launches++;
   }
+  return KC_OK;
+}
+
+// The forward on the tensor cores: the selector raises ws.flags[f] for frames
+// whose decisions it cannot certify.
+kc_status forward_fast(kc_handle* h, Workspace& ws, const DevBatch& b, const kc::FrameTotals& tot) {
+  const Dims& d = h->d;
+  const uint64_t Q = tot.q, R = tot.r;
+  const uint32_t H = d.h;
+  const float attn_scale = float(1.0 / std::sqrt(double(d.hd)));
+  const int mix_m = 3 * int(d.enc), sel_m = mix_m + 5 * int(d.mix);
+  KC_CHECK(encode_fast(h, ws, b, tot));
   // the bank-side projections as planes products: bk once through the
   // selector's Wk (plane 0 of ws.sk, where the selector reads it) and every
   // block's Wk (planes 1..), bv once through every block's Wv (planes of ws.mv)
@@ -2814,4 +2828,5 @@ const char* kc_last_error(kc_handle* h) { return h ? h->err.c_str() : g_create_e
 
 #include "policy_abi.cuh"
 #include "cache_abi.cuh"
+#include "bank_abi.cuh"
 #include "stream.cuh"

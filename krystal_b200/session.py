@@ -113,6 +113,12 @@ class BrainSession:
     def think(self, records: Sequence, allows=None, sample=None, sampling: Sampling | None = None) -> ThinkResult:
         return self.consider(records).choose(allows, sample, sampling)
 
+    def banks(self, pages: int, max_length: int, format: str = "i8"):
+        """Caches for conversations with this brain whose banks grow turn by turn
+        (banks.SessionBanks): a turn encodes its own records alone."""
+        from .banks import SessionBanks
+        return SessionBanks(self.backend, pages, max_length, format)
+
     def learn(self, experiences: Sequence, options=None):
         """session.ts:195-197: one pass over remembered turns (learnFromExperience),
         the backend differentiating and told what moved."""

@@ -13,7 +13,8 @@ from tests import cache_cases as ref
 
 HEADER = Path(__file__).resolve().parent.parent / "include" / "krystal_cuda.h"
 STRUCTS = {"kc_cache_view": "KcCacheView", "kc_page_table": "KcPageTable", "kc_cache_rows": "KcCacheRows",
-           "kc_question_view": "KcQuestionView", "kc_attend_view": "KcAttendView"}
+           "kc_question_view": "KcQuestionView", "kc_attend_view": "KcAttendView", "kc_bank_view": "KcBankView",
+           "kc_bank_out": "KcBankOut"}
 
 
 def test_struct_layouts_match_the_header(tmp_path):
@@ -51,7 +52,9 @@ def test_a_null_handle_is_refused():
     calls = [lib.kc_cache_write(None, c, t, C.byref(rows)), lib.kc_cache_read(None, c, t, None, C.byref(rows)),
              lib.kc_cache_blocks(None, c, t, C.byref(ask), 1, 0, None),
              lib.kc_cache_attend(None, c, t, C.byref(ask), C.byref(view)),
-             lib.kc_cache_scores(None, c, t, C.byref(ask), None, None, 0.0, None)]
+             lib.kc_cache_scores(None, c, t, C.byref(ask), None, None, 0.0, None),
+             lib.kc_bank_turn(None, C.byref(abi.KcBatchView()), C.byref(abi.KcBankView()), None,
+                              C.byref(abi.KcBankOut()))]
     assert calls == [abi.KC_ERR_INVALID_ARG] * len(calls)
     assert b"handle is null" in lib.kc_last_error(None)
     assert lib.kc_cache_attend_workspace(None, c, t, C.byref(ask), 0) == 0
