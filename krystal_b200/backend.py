@@ -428,7 +428,8 @@ class CudaBrainBackend:
         import torch
         with self._clip_lock:
             at = self.stream_ptr()
-            stream = (torch.cuda.default_stream(self.device) if at == 1  # cudaStreamLegacy, the default stream's name
+            # 1 is cudaStreamLegacy, which torch knows as its default stream alone
+            stream = (torch.cuda.default_stream(self.device) if at == 1 and torch.cuda.is_available()
                       else torch.cuda.ExternalStream(at, device=self.device))
             if torch.cuda.is_current_stream_capturing():
                 return

@@ -54,11 +54,21 @@ struct Unit {
 };
 
 // How a launch's warps are shared out: teams of `mg` warps (8 `tiles` rows each) read
-// the same cells, `kg` teams share a unit's cells, a CTA has hg units.
+// the same cells, `kg` teams share a unit's cells, a CTA of `warps` warps has hg units.
 struct Shape {
-  uint32_t tiles, mg, kg, hg, chunks;  // chunks: of 8 tiles mg rows, that a unit may have
+  uint32_t tiles, mg, kg, hg, warps, chunks;  // chunks: of 8 tiles mg rows, that a unit may have
   uint64_t items;
 };
+
+// Row r of a unit: its question (from the unit's first) and its head of the group.
+struct RowId {
+  uint32_t question, head;
+};
+__device__ __forceinline__ RowId row_id(uint32_t r, uint32_t group) {
+  if (group == 1) return RowId{r, 0};  // the same for all: no division
+  const uint32_t q = r / group;
+  return RowId{q, r - q * group};
+}
 
 __device__ __forceinline__ bool unit_of(const AttendArg& a, const Shape& sh, uint64_t item, Unit* u) {
   if (item >= sh.items) return false;
@@ -207,12 +217,12 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
   const uint32_t n_rows = mine && row0 < u.rows ? min(uint32_t(R), u.rows - row0) : 0;
 
   uint8_t* ring = smem + team * (S * CB);
-  uint8_t* biases = smem + kWarps / sh.mg * (S * CB) + warp * (S * mask_bytes(NT));  // a masked call's
+  uint8_t* biases = smem + sh.warps / sh.mg * (S * CB) + warp * (S * mask_bytes(NT));  // a masked call's
   __shared__ uint64_t s_mask[MASKED ? kWarps : 1][R];  // where the rows' masks begin
   const uint32_t open_end = MASKED ? uint32_t(min(uint64_t(u.len), u.stride)) : u.len;
   bool aligned = false;  // whether every row's mask begins at 16 bytes
   if (MASKED) {
-    if (lane < R) s_mask[warp][lane] = uint64_t((row0 + lane) / group) * u.stride;
+    if (lane < R) s_mask[warp][lane] = uint64_t(row_id(row0 + lane, group).question) * u.stride;
     aligned = (reinterpret_cast<uintptr_t>(u.mask) | u.stride * 4) % 16 == 0;
     // rows that are not there are shut: what a vote sees of them must not change from call to call
     for (uint32_t r = n_rows; r < uint32_t(R); r++)
@@ -259,8 +269,8 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
   QTile<T, D, NT> q;
 #pragma unroll
   for (int t = 0; t < NT; t++) {
-    const uint32_t r = row0 + 8 * t + g;
-    q.load(t, uint32_t(8 * t + g) < n_rows ? static_cast<const T*>(a.a.q) + (u.q0 + r / group) * a.a.pitch + (u.kv * group + r % group) * uint64_t(D) : nullptr,
+    const RowId r = row_id(row0 + 8 * t + g, group);
+    q.load(t, uint32_t(8 * t + g) < n_rows ? static_cast<const T*>(a.a.q) + (u.q0 + r.question) * a.a.pitch + (u.kv * group + r.head) * uint64_t(D) : nullptr,
            c, a.scale * kLog2e);
   }
 
@@ -427,8 +437,9 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
       for (int h = 0; h < 2; h++) {
         const uint32_t r = 8 * t + 2 * c + h;
         if (r >= n_rows) continue;
-        const uint64_t question = u.q0 + (row0 + r) / group;
-        const uint32_t head = u.kv * group + (row0 + r) % group;
+        const RowId id = row_id(row0 + r, group);
+        const uint64_t question = u.q0 + id.question;
+        const uint32_t head = u.kv * group + id.head;
         const Stat st{top[t][h], high[t][h], sum[t][h]};
         const float unit = parts > 1 ? 1.0f : st.l > 0.0f ? 1.0f / st.l : 0.0f;
         float run[NB];
@@ -482,8 +493,9 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
 #pragma unroll
       for (int e = 0; e < D / 32; e++) acc[e] = fmaf(x, p[lane + 32 * e], acc[e]);
     }
-    const uint64_t question = u.q0 + (row0 + r) / group;
-    const uint32_t head = u.kv * group + (row0 + r) % group;
+    const RowId id = row_id(row0 + r, group);
+    const uint64_t question = u.q0 + id.question;
+    const uint32_t head = u.kv * group + id.head;
     if (parts == 1) {
 #pragma unroll
       for (int e = 0; e < D / 32; e++) put<T, FMT>(a, question, head, lane + 32 * e, acc[e], all.l);
@@ -597,23 +609,26 @@ inline Shape shape_of(const AttendArg& a, int sms) {
   sh.mg = warps <= 1 ? 1 : warps <= 2 ? 2 : warps <= 4 ? 4 : 8;
   sh.chunks = uint32_t((warps + sh.mg - 1) / sh.mg);
   sh.items = units * sh.chunks * a.c.heads;
-  // short sequences of many units: a team a unit; else the CTA's teams share one
-  sh.kg = blocks <= 8 && sh.items * sh.mg >= uint64_t(sms) * 16 ? 1 : kWarps / sh.mg;
-  sh.hg = kWarps / (sh.mg * sh.kg);
+  // short sequences of many units: a team a unit, in CTAs of 4 warps, which units
+  // of one length leave together; else the CTA's teams share one
+  const bool small = blocks <= 8 && sh.items * sh.mg >= uint64_t(sms) * 16;
+  sh.warps = small && sh.mg <= 4 ? 4 : kWarps;
+  sh.kg = small ? 1 : kWarps / sh.mg;
+  sh.hg = sh.warps / (sh.mg * sh.kg);
   return sh;
 }
 
-__host__ __device__ constexpr size_t attend_smem(int dim, int tiles, bool masked, uint32_t teams, bool joins) {
-  const size_t ring = size_t(stages(dim, masked)) * (teams * cell_bytes(dim) + (masked ? kWarps * mask_bytes(tiles) : 0));
+__host__ __device__ constexpr size_t attend_smem(int dim, int tiles, bool masked, uint32_t warps, uint32_t teams, bool joins) {
+  const size_t ring = size_t(stages(dim, masked)) * (teams * cell_bytes(dim) + (masked ? warps * mask_bytes(tiles) : 0));
   const size_t join = joins ? size_t(kWarps) * 8 * tiles * (dim + 4) * 4 : 0;
   return ring > join ? ring : join;
 }
 
 template <typename T, int D, int FMT, int NT>
 void attend_rows(const AttendArg& a, const Shape& sh, dim3 grid, cudaStream_t s) {
-  const size_t smem = attend_smem(D, NT, a.mask != nullptr, kWarps / sh.mg, sh.kg > 1);
-  if (a.mask) k_attend<T, D, FMT, NT, true><<<grid, kThreads, smem, s>>>(a, sh);
-  else k_attend<T, D, FMT, NT, false><<<grid, kThreads, smem, s>>>(a, sh);
+  const size_t smem = attend_smem(D, NT, a.mask != nullptr, sh.warps, sh.warps / sh.mg, sh.kg > 1);
+  if (a.mask) k_attend<T, D, FMT, NT, true><<<grid, sh.warps * 32, smem, s>>>(a, sh);
+  else k_attend<T, D, FMT, NT, false><<<grid, sh.warps * 32, smem, s>>>(a, sh);
 }
 
 template <typename T, int D, int FMT>
@@ -773,7 +788,7 @@ template <typename T, int D, int FMT>
 cudaError_t prepare_tile() {
   constexpr int most = most_tiles<T, D>();
   auto allow = [](auto kernel, int tiles, bool masked) {
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(attend_smem(D, tiles, masked, kWarps, true)));
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(attend_smem(D, tiles, masked, kWarps, kWarps, true)));
   };
   cudaError_t e;
   if ((e = allow(k_attend<T, D, FMT, 1, false>, 1, false)) || (e = allow(k_attend<T, D, FMT, 1, true>, 1, true)) ||
