@@ -207,6 +207,7 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
     w.pages = a.c.pages;
     w.b0 = part * a.chunk;
     w.cells = w.b0 < all ? 2 * min(a.chunk, all - w.b0) : 0;
+    if (!a.blocks && w.cells) w.cells = min(w.cells, (u.len - w.b0 * kPage + kCell - 1) / kCell);  // a page's second cell may be empty
     w.first = team % sh.kg;
     w.step = sh.kg;
   }
@@ -299,8 +300,19 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
     ahead[S - 2] = w.page_of(i, S - 1);  // none behind the last
     issue(i + S - 1, ahead[S - 2], MASKED ? w.block_of(i, S - 1) : 0);
     if (!n_rows || page == kNone) continue;
-    const uint8_t* cell = ring + (i % S) * CB;
+    uint8_t* cell = ring + (i % S) * CB;
     const uint64_t pos = uint64_t(block) * kPage + w.half(i) * kCell;
+    if (pos >= u.len) continue;
+    if (FMT == kE4M3 && pos + kCell > u.len) {
+      // bytes behind the sequence's last row may be e4m3's NaN, which no weight of
+      // 0 takes away; every warp of a team writes the zeros that it will read
+      const uint32_t held = uint32_t(u.len - pos), n16 = (kCell - held) * D / 16;
+      for (uint32_t k = lane; k < n16; k += 32) {
+        reinterpret_cast<uint4*>(cell + held * D)[k] = uint4{};
+        reinterpret_cast<uint4*>(cell + (kCell + held) * D)[k] = uint4{};
+      }
+      __syncwarp();
+    }
     {
       const float* scales = reinterpret_cast<const float*>(cell + 2 * kCell * D);
       const float vs = scales[kCell + lane];

@@ -40,7 +40,8 @@ def offsets(n):
 class Bank:
     """A cache of sequences of given lengths, in shuffled pages, and what it holds."""
 
-    def __init__(self, be, lengths, kv=4, dim=32, fmt="i8", seed=0, dtype="f32", spread=1.0, spare=3):
+    def __init__(self, be, lengths, kv=4, dim=32, fmt="i8", seed=0, dtype="f32", spread=1.0, spare=3,
+                 fill=0xA5):
         rng = np.random.default_rng(seed)
         self.be, self.lengths, self.kv, self.dim, self.fmt = be, list(lengths), kv, dim, fmt
         self.n = len(self.lengths)
@@ -48,7 +49,7 @@ class Bank:
         count = self.n * self.pitch + spare
         self.pages = rng.permutation(count)[:self.n * self.pitch].reshape(self.n, self.pitch).astype(np.uint32)
         self.cache = BankCache(count, kv, dim, fmt, storage=torch.full(
-            (BankCache.bytes_for(count, kv, dim),), 0xA5, dtype=torch.uint8, device="cuda"))
+            (BankCache.bytes_for(count, kv, dim),), fill, dtype=torch.uint8, device="cuda"))
         total = sum(self.lengths)
         x = rng.normal(0, 1, (2, total, kv, dim)) * np.exp(rng.normal(0, spread, (2, total, kv, 1)))
         x[:, ::29] = 0
@@ -424,6 +425,27 @@ def test_value_scales_of_any_size(be):
         got = a.attend(mask=True)
         b.values[0][7] = 0  # shut out: its size is not the tolerance's
         a.check(got, mask=True)
+
+
+@pytest.mark.parametrize("mask", [False, True])
+@pytest.mark.parametrize("kv,heads,dim", [(4, 4, 32), (2, 8, 64), (1, 40, 128)])
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+def test_what_lies_behind_the_last_row_does_not_matter(be, kv, heads, dim, fmt, mask):
+    """Storage that was never cleared: NaN codes (0x7f, 0xff), NaN and infinite
+    scales behind a sequence's end and in its other rows' neighbours."""
+    got = []
+    for fill in (0x00, 0x7F, 0xFF):
+        b = Bank(be, [0, 1, 37, 64, 100, 300], kv, dim, fmt, fill=fill)
+        a = Asked(b, [2, 1, 9, 1, 20, 3], heads)
+        a.masks()
+        got.append(a.attend(mask=mask))
+        one = Asked(b, [1] * 6, heads)
+        lists = select(b, one, 3, 1)
+        got[-1] += one.attend(blocks=lists, block_count=3) + (lists.cpu().numpy(),)
+    a.check(got[0][:2], mask=mask)
+    for other in got[1:]:
+        for x, y in zip(got[0], other):
+            assert np.array_equal(x, y)
 
 
 def test_masks_beyond_1e29_and_short_masks(be):
