@@ -669,7 +669,8 @@ typedef struct kc_question_view {
   const void* q;
   const uint64_t* q_off;    /* [sequences+1] or NULL */
   uint32_t questions, heads;
-  uint32_t max_questions;   /* bounds one sequence's questions (0 = questions); those beyond it are left as they were */
+  uint32_t max_questions;   /* bounds one sequence's questions (0 = questions); those beyond it are left as they were.
+                               Launches are sized by it: many sequences need it */
   int32_t dtype;            /* KC_DTYPE_F32 / F16 / BF16 */
   uint64_t pitch;
 } kc_question_view;
@@ -690,7 +691,8 @@ kc_status kc_cache_blocks(kc_handle* h, const kc_cache_view* cache, const kc_pag
  * entry at or below -1e29, or NaN, shuts its row out, larger ones than 1e29 count
  * as 1e29; rows behind the mask's end are shut out. Nothing left: out 0, lse
  * -infinity. Scores, sums and statistics are f32; the weights are rounded to 22
- * bits before they meet the values, to 11 for bf16 questions. */
+ * bits before they meet the values, to 11 for bf16 questions. No output overlaps
+ * an input. */
 typedef struct kc_attend_view {
   void* out;                 /* [questions, heads, head_dim], the questions' type, out_pitch elements apart (0 = dense) */
   uint64_t out_pitch;

@@ -104,6 +104,14 @@ kc_status check_ask(kc_handle* h, const kc_question_view* v, const kc::cache::St
   return KC_OK;
 }
 
+// What a launch answered; too many units are the caller's bound on the questions.
+kc_status launched(kc_handle* h, cudaError_t e, const char* what) {
+  if (e == cudaErrorInvalidConfiguration)
+    return fail(h, KC_ERR_CAPACITY, "sequences times max_questions leave the launch's range: bound one sequence's questions");
+  KC_TRY(e, what);
+  return KC_OK;
+}
+
 kc_status check_scale(kc_handle* h, float scale, uint32_t dim, float* out) {
   if (!std::isfinite(scale)) return fail(h, KC_ERR_INVALID_ARG, "scale must be finite");
   *out = scale != 0.0f ? scale : float(1.0 / std::sqrt(double(dim)));
@@ -151,8 +159,7 @@ kc_status kc_cache_blocks(kc_handle* h, const kc_cache_view* cache, const kc_pag
   a.count = count;
   a.recent = recent;
   a.blocks = blocks;
-  KC_TRY(kc::cache::launch_blocks(a, h->sms, h->stream, &h->launches), "block selection launch");
-  return KC_OK;
+  return launched(h, kc::cache::launch_blocks(a, h->sms, h->stream, &h->launches), "block selection launch");
 }
 
 uint64_t kc_cache_attend_workspace(kc_handle* h, const kc_cache_view* cache, const kc_page_table* table,
@@ -179,6 +186,7 @@ kc_status kc_cache_attend(kc_handle* h, const kc_cache_view* cache, const kc_pag
   if (a.a.questions && !v->out) return fail(h, KC_ERR_INVALID_ARG, "attention needs an output");
   if (v->out_pitch && v->out_pitch < width)
     return fail(h, KC_ERR_INVALID_ARG, "the output's pitch is smaller than heads * head_dim");
+  if (v->out && v->out == questions->q) return fail(h, KC_ERR_INVALID_ARG, "attention does not write over its questions");
   if (v->mask && !v->mask_off) return fail(h, KC_ERR_INVALID_ARG, "a mask needs its offsets");
   if ((v->blocks != nullptr) != (v->block_count != 0))
     return fail(h, KC_ERR_INVALID_ARG, "a list of blocks needs its count, and a count its list");
@@ -197,8 +205,7 @@ kc_status kc_cache_attend(kc_handle* h, const kc_cache_view* cache, const kc_pag
   if (need && (!v->workspace || v->workspace_bytes < need))
     return fail(h, KC_ERR_CAPACITY, "the workspace is smaller than kc_cache_attend_workspace");
   a.work = static_cast<float*>(v->workspace);
-  KC_TRY(kc::cache::launch_attend(a, h->sms, h->stream, &h->launches), "attention launch");
-  return KC_OK;
+  return launched(h, kc::cache::launch_attend(a, h->sms, h->stream, &h->launches), "attention launch");
 }
 
 kc_status kc_cache_scores(kc_handle* h, const kc_cache_view* cache, const kc_page_table* table,
@@ -219,8 +226,7 @@ kc_status kc_cache_scores(kc_handle* h, const kc_cache_view* cache, const kc_pag
   a.scores = scores;
   a.off = off;
   a.mask = mask;
-  KC_TRY(kc::cache::launch_scores(a, h->sms, h->stream, &h->launches), "scores launch");
-  return KC_OK;
+  return launched(h, kc::cache::launch_scores(a, h->sms, h->stream, &h->launches), "scores launch");
 }
 
 }  // extern "C"

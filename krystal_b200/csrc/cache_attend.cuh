@@ -70,12 +70,11 @@ __device__ __forceinline__ RowId row_id(uint32_t r, uint32_t group) {
   return RowId{q, r - q * group};
 }
 
-__device__ __forceinline__ bool unit_of(const AttendArg& a, const Shape& sh, uint64_t item, Unit* u) {
+__device__ __forceinline__ bool unit_of(const AttendArg& a, const Shape& sh, uint32_t item, Unit* u) {
   if (item >= sh.items) return false;
-  const uint32_t group = a.a.heads / a.c.heads;
-  u->kv = uint32_t(item % a.c.heads);
-  const uint64_t rest = item / a.c.heads;
-  const uint32_t chunk = uint32_t(rest % sh.chunks), which = uint32_t(rest / sh.chunks);
+  const uint32_t group = a.a.heads / a.c.heads, rest = item / a.c.heads;
+  u->kv = item - rest * a.c.heads;
+  const uint32_t which = sh.chunks == 1 ? rest : rest / sh.chunks, chunk = rest - which * sh.chunks;
   uint32_t first, count;
   if (a.blocks) {  // a question
     if (a.a.off) {
@@ -194,7 +193,7 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
   const uint32_t team = warp / sh.mg, mi = warp % sh.mg;
   const uint32_t part = blockIdx.y, group = a.a.heads / a.c.heads;
   Unit u{};
-  const bool live = unit_of(a, sh, uint64_t(blockIdx.x) * sh.hg + team / sh.kg, &u);
+  const bool live = unit_of(a, sh, blockIdx.x * sh.hg + (sh.kg == 1 ? team : team / sh.kg), &u);
 
   Walk w{};
   uint32_t parts = 1;
@@ -648,7 +647,7 @@ cudaError_t attend_tile(const AttendArg& a, int sms, cudaStream_t s, uint64_t* l
   const Shape sh = shape_of(a, sms);
   const uint64_t ctas = (sh.items + sh.hg - 1) / sh.hg;
   if (ctas == 0) return cudaSuccess;
-  if (ctas > 0x7fffffffull) return cudaErrorInvalidConfiguration;
+  if (sh.items > 0x7fffffffull || a.splits > 65535) return cudaErrorInvalidConfiguration;
   const dim3 grid(unsigned(ctas), a.splits);
   constexpr int most = most_tiles<T, D>();
   if (sh.tiles == 1) attend_rows<T, D, FMT, 1>(a, sh, grid, s);

@@ -702,6 +702,49 @@ def test_a_turn_over_a_cached_bank(be):
         be.set_stream(None)
 
 
+def test_a_cut_sequence_in_a_graph(be):
+    """The join follows the parts it was launched behind, in a graph too, and the
+    workspace is the graph's."""
+    stream = torch.cuda.Stream()
+    b = Bank(be, [9000, 40], 1, 64, spread=0.3)
+    a = Asked(b, [1, 1], 4)
+    out, lse = torch.zeros(2, 4, 64, device="cuda"), torch.zeros(2, 4, device="cuda")
+    size = be.attend_workspace(b.cache, b.table, a.view)
+    assert size > 0
+    work = torch.zeros(size, dtype=torch.uint8, device="cuda")
+    after = torch.zeros_like(out)
+    torch.cuda.synchronize()
+    be.set_stream(stream.cuda_stream)
+    try:
+        def call():
+            be.cache_attend(b.cache, b.table, a.view, out.data_ptr(), lse=lse.data_ptr(), workspace=work.data_ptr(),
+                            workspace_bytes=size)
+        with torch.cuda.stream(stream):
+            call()
+            after.copy_(out)  # what follows the call follows its join
+        torch.cuda.synchronize()
+        assert torch.equal(after, out)
+        a.check((out.cpu().numpy(), lse.cpu().numpy()))
+        first = out.clone()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            call()
+            after.copy_(out)
+        for _ in range(5):
+            out.zero_()
+            after.zero_()
+            work.fill_(0xFF)
+            torch.cuda.synchronize()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(after, first)
+        with pytest.raises(abi.KrystalCudaError, match="workspace"):
+            be.cache_attend(b.cache, b.table, a.view, out.data_ptr(), workspace=work.data_ptr(), workspace_bytes=size - 16)
+        del g
+    finally:
+        be.set_stream(None)
+
+
 def test_offsets_past_32_bits(be):
     """A cache of 5 GB whose last pages hold the rows, and a mask and scores
     behind 2^32 bytes."""
@@ -784,7 +827,7 @@ def test_refusals(be):
     for kw, match in [(dict(out=None), "an output"), (dict(out_pitch=255), "pitch is smaller"), (dict(mask=p(out)), "offsets"),
                       (dict(block_count=2), "list of blocks"), (dict(blocks=p(out)), "list of blocks"),
                       (dict(scale=float("nan")), "finite"), (dict(scale=float("inf")), "finite"), (dict(out=p(out) + 1), "aligned"),
-                      (dict(lse=p(out) + 2), "aligned"), (dict(workspace=p(out) + 4), "16 bytes")]:
+                      (dict(out=p(a.flat)), "over its questions"), (dict(lse=p(out) + 2), "aligned"), (dict(workspace=p(out) + 4), "16 bytes")]:
         refused(match, be.cache_attend, **{**good, **kw})
     blocks = torch.zeros(3, 2, 2, dtype=torch.int32, device="cuda")
     refused("at least one block", be.cache_blocks, b.cache, b.table, a.view, 0, 0, p(blocks))
