@@ -743,7 +743,7 @@ kc_status kc_cache_scores(kc_handle* h, const kc_cache_view* cache, const kc_pag
 typedef struct kc_bank_view {
   const kc_cache_view* mixer;  /* HOST [mixer_blocks] */
   kc_cache_view selector;
-  kc_page_table table;         /* sequences = batch.frames, max_length <= KC_MAX_ROW */
+  kc_page_table table;         /* sequences = batch.frames, max_length (0: pitch * 64) <= KC_MAX_ROW */
 } kc_bank_view;
 typedef struct kc_bank_out {
   float* p;                    /* DEVICE [questions, table.max_length] */

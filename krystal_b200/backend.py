@@ -415,8 +415,8 @@ class CudaBrainBackend:
             self._release_clips()
 
     def hold_clip(self, parts) -> None:
-        """Takes what a dropped list held (GradList.__del__; no CUDA call: it may
-        run anywhere, in a capture too)."""
+        """Takes what a dropped list or cache held (GradList.__del__,
+        BankCache.__del__; no CUDA call: it may run anywhere, in a capture too)."""
         if self._h:
             self._clips_dropped.append(parts)
 

@@ -84,6 +84,8 @@ class SessionBanks:
             raise ValueError("a session takes one turn at a time")
         if not turns:
             return []
+        if masks is not None and len(masks) != len(turns):
+            raise ValueError(f"a mask per turn is needed ({len(turns)})")
         batch = pack_frame_batch([r for _, r in turns])
         rec = np.diff(batch.rec_off.astype(np.int64))
         asks = np.bincount(np.repeat(np.arange(len(turns)), rec), weights=batch.band_ids == QUERY_BAND,

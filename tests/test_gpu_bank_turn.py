@@ -177,6 +177,8 @@ def test_sessions_come_and_go(be):
         banks.turn([("a", asks), ("a", asks)])
     with pytest.raises(ValueError, match="mask must be"):
         banks.turn([("a", asks)], [np.zeros(3)])
+    with pytest.raises(ValueError, match="a mask per turn"):
+        banks.turn([("a", asks)], [])
     with pytest.raises(ValueError, match="one entry per question"):
         banks.turn([("a", asks)], uniforms=[0.5] * 99)
     with pytest.raises(abi.KrystalCudaError, match="tokenRows"):  # refused on the device: nothing is kept of the turn
