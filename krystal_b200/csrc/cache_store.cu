@@ -142,7 +142,8 @@ __device__ __forceinline__ void codes_of(float (&x)[N], float scale, bool zero, 
     for (int p = 0; p < N / 4; p++) {
       uint32_t lo, hi;
       asm("{.reg .b16 t; cvt.rn.satfinite.e4m3x2.f32 t, %2, %1; cvt.u32.u16 %0, t;}" : "=r"(lo) : "f"(y[4 * p]), "f"(y[4 * p + 1]));
-      asm("{.reg .b16 t; cvt.rn.satfinite.e4m3x2.f32 t, %2, %1; cvt.u32.u16 %0, t;}" : "=r"(hi) : "f"(y[4 * p + 2]), "f"(y[4 * p + 3]));
+      asm("{.reg .b16 t; cvt.rn.satfinite.e4m3x2.f32 t, %2, %1; cvt.u32.u16 %0, t;}"
+          : "=r"(hi) : "f"(y[4 * p + 2]), "f"(y[4 * p + 3]));
       w[p] = __byte_perm(lo, hi, 0x5410);
     }
   }
@@ -167,8 +168,9 @@ __device__ __forceinline__ void widen_bounds(const uint32_t (&w)[2], float scale
 // quantised into its cells and, with the keys, the bounds of all the rows the page
 // holds. A CTA looks at `chunk` source rows and takes the pages whose first new row
 // is among them, so that every page has one writer and the pages need not be listed
-// beforehand. kAhead passes of 8 elements a lane are on their way together (4 a lane
-// took twice the instructions for f32), and no code of the call's rows is read again.
+// beforehand; where pages are few, several CTAs share them, each some of the heads.
+// kAhead passes of 8 elements a lane are on their way together (4 a lane took twice
+// the instructions for f32), and no code of the call's rows is read again.
 // 507 000 f32 rows of 4 heads of 32: 157 us, 4.2 TB/s; 250 000 bf16 rows of 8 heads
 // of 128 to e4m3: 489 us, 3.2 TB/s, bound by about 20 instructions an element (the
 // quotient, the code, its value again for the bounds).
@@ -197,7 +199,7 @@ __global__ __launch_bounds__(kWriteThreads, 7) void k_write(Store c, Table t, Ro
   __syncthreads();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t b = (lane % L) * V, sub = lane / L, items = s_count * c.heads * 2;
-  for (uint32_t item = warp; item < items; item += kWriteThreads / 32) {
+  for (uint32_t item = warp * gridDim.y + blockIdx.y; item < items; item += kWriteThreads / 32 * gridDim.y) {
     const uint32_t which = item & 1u, k = item / 2 / c.heads, head = item / 2 - k * c.heads;
     const uint32_t page = t.table[uint64_t(s_seq[k]) * t.pitch + s_pos[k] / kPage];
     if (page >= c.pages) continue;
@@ -620,8 +622,14 @@ cudaError_t store_as(bool write, const Store& c, const Table& t, const Rows& r, 
   const uint64_t grid = (r.rows + chunk - 1) / chunk;
   if (grid > 0x7fffffffull) return cudaErrorInvalidConfiguration;
   if (write) {
-    if (wide) k_write<T, D, FMT, true><<<unsigned(grid), kWriteThreads, 0, s>>>(c, t, r, chunk);
-    else k_write<T, D, FMT, false><<<unsigned(grid), kWriteThreads, 0, s>>>(c, t, r, chunk);
+    // CTAs that share a chunk's pages: until about 6 an SM have one to write, while
+    // each of their 4 warps has something of every page (6700 f16 rows of 8 heads of
+    // 64 written and read: 47 us, 66 with one)
+    const uint64_t pages = r.rows / kPage + std::min<uint64_t>(t.seqs, r.rows);
+    unsigned share = 1;
+    while (share * 2 * (kWriteThreads / 32) <= c.heads * 2 && pages * share < uint64_t(sms) * 6) share *= 2;
+    if (wide) k_write<T, D, FMT, true><<<dim3(unsigned(grid), share), kWriteThreads, 0, s>>>(c, t, r, chunk);
+    else k_write<T, D, FMT, false><<<dim3(unsigned(grid), share), kWriteThreads, 0, s>>>(c, t, r, chunk);
   } else {
     if (wide) k_read<T, D, FMT, true><<<unsigned(grid), kThreads, 0, s>>>(c, t, r, chunk);
     else k_read<T, D, FMT, false><<<unsigned(grid), kThreads, 0, s>>>(c, t, r, chunk);
