@@ -96,7 +96,8 @@ kc_status turn_pass(kc_handle* h, const DevBatch& b, const kc::FrameTotals& tot,
     a.out = ws.turn_attend.p;
     a.work = P<float>(ws.turn_work);
     KC_TRY(kc::cache::launch_attend(a, h->sms, h->stream, &h->launches), "attention launch");
-    k_turn_add<<<unsigned((Q * H / 4 + 255) / 256), 256, 0, h->stream>>>(P<float4>(ws.qstate), P<float4>(ws.turn_attend), Q * H / 4);
+    k_turn_add<<<unsigned((Q * H / 4 + 255) / 256), 256, 0, h->stream>>>(P<float4>(ws.qstate),
+                                                                       P<float4>(ws.turn_attend), Q * H / 4);
     h->launches++;
     KC_CHECK(tc_gemm<kc::tc::kEpiRelu>(h, P<float>(ws.qstate), Q, m0 + 3, P<float>(ws.mh)));
     KC_CHECK(tc_gemm<kc::tc::kEpiResid>(h, P<float>(ws.mh), Q, m0 + 4, P<float>(ws.qstate)));

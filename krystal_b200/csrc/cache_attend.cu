@@ -15,7 +15,8 @@ uint64_t plan_attend(AttendArg& a, int sms) {
   const Shape sh = shape_of(a, sms);
   const uint32_t blocks = std::max(1u, a.block_count ? a.block_count : (a.t.max_len + kPage - 1) / kPage);
   const uint64_t waves = a.block_count || a.t.seqs == 1 ? 1 : 4;
-  const uint64_t ctas = std::max<uint64_t>(1, (sh.items + sh.hg - 1) / sh.hg), places = uint64_t(sms) * (a.c.dim == 128 ? 1 : 2) * (kWarps / sh.warps);
+  const uint64_t ctas = std::max<uint64_t>(1, (sh.items + sh.hg - 1) / sh.hg);
+  const uint64_t places = uint64_t(sms) * (a.c.dim == 128 ? 1 : 2) * (kWarps / sh.warps);
   const uint64_t want = std::max<uint64_t>(1, places * waves / ctas);
   a.chunk = uint32_t(std::max<uint64_t>(2 * sh.kg, (blocks + want - 1) / want));
   a.splits = (blocks + a.chunk - 1) / a.chunk;

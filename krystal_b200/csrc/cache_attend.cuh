@@ -213,7 +213,8 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
     w.pages = a.c.pages;
     w.b0 = part * a.chunk;
     w.cells = w.b0 < all ? 2 * min(a.chunk, all - w.b0) : 0;
-    if (!a.blocks && w.cells) w.cells = min(w.cells, (u.len - w.b0 * kPage + kCell - 1) / kCell);  // a page's second cell may be empty
+    if (!a.blocks && w.cells)  // a page's second cell may be empty
+      w.cells = min(w.cells, (u.len - w.b0 * kPage + kCell - 1) / kCell);
     w.first = team % sh.kg;
     w.step = sh.kg;
   }
@@ -252,7 +253,8 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
 #pragma unroll
           for (int r = 0; r < R; r += 4)
             if (uint32_t(r + lane / 8) < n_rows)
-              copy16(to + (r + lane / 8) * (4 * kMaskPitch) + 16 * (lane % 8), u.mask + s_mask[warp][r + lane / 8] + pos + 4 * (lane % 8));
+              copy16(to + (r + lane / 8) * (4 * kMaskPitch) + 16 * (lane % 8),
+                     u.mask + s_mask[warp][r + lane / 8] + pos + 4 * (lane % 8));
         } else {
           const bool in = pos + lane < open_end;
           for (uint32_t r = 0; r < n_rows; r++) {
@@ -277,8 +279,8 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
 #pragma unroll
   for (int t = 0; t < NT; t++) {
     const RowId r = row_id(row0 + 8 * t + g, group);
-    q.load(t, uint32_t(8 * t + g) < n_rows ? static_cast<const T*>(a.a.q) + (u.q0 + r.question) * a.a.pitch + (u.kv * group + r.head) * uint64_t(D) : nullptr,
-           c, a.scale * kLog2e);
+    const T* at = static_cast<const T*>(a.a.q) + (u.q0 + r.question) * a.a.pitch + (u.kv * group + r.head) * uint64_t(D);
+    q.load(t, uint32_t(8 * t + g) < n_rows ? at : nullptr, c, a.scale * kLog2e);
   }
 
   float o[NT][MT][4], top[NT][2], high[NT][2], sum[NT][2];
@@ -338,11 +340,14 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       key[j] = info[8 * j + key_of(g)];
+      const Pair ka = pair(key[j].a, key[j].a), ke = pair(key[j].e, key[j].e);
 #pragma unroll
-      for (int t = 0; t < NT; t++)
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-          s[t][j / 2][2 * (j % 2) + h] = fmaf(s[t][j / 2][2 * (j % 2) + h] * key[j].a, q.unit[t][h], key[j].e);
+      for (int t = 0; t < NT; t++) {
+        float* x = &s[t][j / 2][2 * (j % 2)];
+        const float2 y = halves(fma2(mul2(pair(x[0], x[1]), ka), pair(q.unit[t][0], q.unit[t][1]), ke));
+        x[0] = y.x;
+        x[1] = y.y;
+      }
     }
     if (MASKED) {
       const float* bias = reinterpret_cast<const float*>(biases + (i % S) * mask_bytes(NT)) + 2 * c * kMaskPitch + key_of(g);
@@ -362,7 +367,8 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
           for (int h = 0; h < 2; h++) {
             const float was = top[t][h];
             top[t][h] = fmaxf(was, row_most(most[h]));
-            if (was != top[t][h]) high[t][h] = was == -INFINITY ? -INFINITY : high[t][h] + (was - top[t][h]);  // measured from the new one
+            if (was != top[t][h])  // M is measured from the new one
+              high[t][h] = was == -INFINITY ? -INFINITY : high[t][h] + (was - top[t][h]);
           }
         }
 #pragma unroll
@@ -410,21 +416,27 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
       uint32_t hi[NT][2], lo[kTwo ? NT : 1][2];
 #pragma unroll
       for (int t = 0; t < NT; t++) {
-        const float from[2] = {high[t][0] == -INFINITY ? 0.0f : high[t][0] - kLift, high[t][1] == -INFINITY ? 0.0f : high[t][1] - kLift};
+        const Pair less = pair(high[t][0] == -INFINITY ? 0.0f : kLift - high[t][0],
+                               high[t][1] == -INFINITY ? 0.0f : kLift - high[t][1]);
+        Pair l = pair(sum[t][0], sum[t][1]);
 #pragma unroll
         for (int j = 0; j < 2; j++) {
           const KeyInfo& k = key[2 * v + j];
-          const float x0 = ex2(s[t][v][2 * j] - from[0]), x1 = ex2(s[t][v][2 * j + 1] - from[1]);
-          sum[t][0] = fmaf(x0, k.re, sum[t][0]);
-          sum[t][1] = fmaf(x1, k.re, sum[t][1]);
-          const float w0 = x0 * k.f, w1 = x1 * k.f;
-          const uint32_t h = pack(w0, w1);
+          const float2 y = halves(add2(pair(s[t][v][2 * j], s[t][v][2 * j + 1]), less));
+          const Pair x = pair(ex2(y.x), ex2(y.y));
+          l = fma2(x, pair(k.re, k.re), l);
+          const Pair w = mul2(x, pair(k.f, k.f));
+          const float2 wf = halves(w);
+          const uint32_t h = pack(wf.x, wf.y);
           hi[t][j] = transposed(h);
           if (kTwo) {
-            const __half2 y = *reinterpret_cast<const __half2*>(&h);
-            lo[kTwo ? t : 0][j] = transposed(pack(w0 - __low2float(y), w1 - __high2float(y)));
+            const __half2 z = *reinterpret_cast<const __half2*>(&h);
+            const float2 rest = halves(fma2(pair(__low2float(z), __high2float(z)), pair(-1.0f, -1.0f), w));
+            lo[kTwo ? t : 0][j] = transposed(pack(rest.x, rest.y));
           }
         }
+        sum[t][0] = halves(l).x;
+        sum[t][1] = halves(l).y;
       }
       if constexpr (kApart) value_products<D, FMT, NT, kTwo>(hi, lo, cell + kCell * D, v, g, c, part_o);
       else value_products<D, FMT, NT, kTwo>(hi, lo, cell + kCell * D, v, g, c, o);
@@ -435,7 +447,11 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
 #pragma unroll
         for (int m = 0; m < MT; m++)
 #pragma unroll
-          for (int k = 0; k < 4; k++) o[t][m][k] += part_o[t][m][k];
+          for (int k = 0; k < 4; k += 2) {
+            const float2 y = halves(add2(pair(o[t][m][k], o[t][m][k + 1]), pair(part_o[t][m][k], part_o[t][m][k + 1])));
+            o[t][m][k] = y.x;
+            o[t][m][k + 1] = y.y;
+          }
     }
     __syncwarp();
   }
@@ -566,7 +582,8 @@ __global__ __launch_bounds__(kThreads) void k_join(AttendArg a, uint32_t per) {
 #pragma unroll
       for (int o = 16; o; o >>= 1) b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, o));
       if (b == -INFINITY) continue;
-      float m = fmaxf(st.m == -INFINITY ? -INFINITY : (st.b - b) + st.m, other.m == -INFINITY ? -INFINITY : (other.b - b) + other.m);
+      float m = fmaxf(st.m == -INFINITY ? -INFINITY : (st.b - b) + st.m,
+                      other.m == -INFINITY ? -INFINITY : (other.b - b) + other.m);
 #pragma unroll
       for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       const float keep = weight_of(st, b, m), add = weight_of(other, b, m);
@@ -694,7 +711,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_scores(ScoreArg a, uint32_t mg,
   const uint32_t team = warp / mg, mi = warp % mg, kg = kWarps / mg;
   const uint32_t seq = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
   const uint64_t q0 = a.a.off ? a.a.off[seq] : seq, q1 = a.a.off ? a.a.off[seq + 1] : seq + 1;
-  const uint32_t count = uint32_t(q1 - q0), rows = uint32_t(min(uint64_t(min(count, a.a.max_q)), a.a.questions > q0 ? a.a.questions - q0 : 0));
+  const uint32_t count = uint32_t(q1 - q0);
+  const uint32_t rows = uint32_t(min(uint64_t(min(count, a.a.max_q)), a.a.questions > q0 ? a.a.questions - q0 : 0));
   if (chunk * 8 * mg >= rows) return;  // the whole CTA
   const uint32_t row0 = (chunk * mg + mi) * 8, n_rows = row0 < rows ? min(8u, rows - row0) : 0;
   const uint64_t stride = (a.off[seq + 1] - a.off[seq]) / count;
@@ -708,7 +726,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_scores(ScoreArg a, uint32_t mg,
   w.blocks = (len + kPage - 1) / kPage;
   w.pages = a.c.pages;
   w.b0 = uint32_t(c0 / 2);
-  w.cells = uint32_t(blockIdx.y + 1 == gridDim.y ? end - c0 : min(uint64_t(cells), end - c0));  // the last takes what the table does not bound
+  // the last part takes what the table does not bound
+  w.cells = uint32_t(blockIdx.y + 1 == gridDim.y ? end - c0 : min(uint64_t(cells), end - c0));
   w.first = team;
   w.step = kg;
   const uint32_t n = w.count();
@@ -807,7 +826,8 @@ template <typename T, int D, int FMT>
 cudaError_t prepare_tile() {
   constexpr int most = most_tiles<T, D>();
   auto allow = [](auto kernel, int tiles, bool masked) {
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(attend_smem(D, tiles, masked, kWarps, kWarps, true)));
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                int(attend_smem(D, tiles, masked, kWarps, kWarps, true)));
   };
   cudaError_t e;
   if ((e = allow(k_attend<T, D, FMT, 1, false>, 1, false)) || (e = allow(k_attend<T, D, FMT, 1, true>, 1, true)) ||

@@ -76,6 +76,34 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
 // quarter-warp's key rows fall on different banks.
 __device__ __forceinline__ uint32_t key_of(int g) { return uint32_t(g >> 1) + (uint32_t(g & 1) << 2); }
 
+// Two f32 in one register pair, and the instructions that take two at once.
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair pair(float a, float b) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 halves(Pair p) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
 // The B fragments of a warp's question rows, 8 a tile. The dimensions' order
 // within a fragment is the keys': lane c's bytes of a key row, 4 a fragment.
 template <typename T, int D, int NT>
