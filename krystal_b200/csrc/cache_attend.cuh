@@ -276,11 +276,12 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
     }
   }
   QTile<T, D, NT> q;
+  const bool wide_q = (reinterpret_cast<uintptr_t>(a.a.q) | a.a.pitch * sizeof(T)) % 16 == 0;
 #pragma unroll
   for (int t = 0; t < NT; t++) {
     const RowId r = row_id(row0 + 8 * t + g, group);
     const T* at = static_cast<const T*>(a.a.q) + (u.q0 + r.question) * a.a.pitch + (u.kv * group + r.head) * uint64_t(D);
-    q.load(t, uint32_t(8 * t + g) < n_rows ? at : nullptr, c, a.scale * kLog2e);
+    q.load(t, uint32_t(8 * t + g) < n_rows ? at : nullptr, wide_q, c, a.scale * kLog2e);
   }
 
   float o[NT][MT][4], top[NT][2], high[NT][2], sum[NT][2];
@@ -749,7 +750,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_scores(ScoreArg a, uint32_t mg,
     issue(i, ahead[i]);
   }
   QTile<T, D, 1> q;
-  q.load(0, uint32_t(g) < n_rows ? static_cast<const T*>(a.a.q) + (q0 + row0 + g) * a.a.pitch : nullptr, c, a.scale);
+  q.load(0, uint32_t(g) < n_rows ? static_cast<const T*>(a.a.q) + (q0 + row0 + g) * a.a.pitch : nullptr,
+         (reinterpret_cast<uintptr_t>(a.a.q) | a.a.pitch * sizeof(T)) % 16 == 0, c, a.scale);
   float (*tile)[kCell + 1] = s_tile[warp];
   const uint64_t at0 = a.off[seq] + row0 * stride;
   for (uint32_t i = 0; i < n; i++) {
