@@ -222,7 +222,7 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
   uint32_t n = mine ? w.count() : 0;
   if (n) w.begin();
   // A list ends with its last block that is there (81 sequences of 3 to 32 rows, lists
-  // of 32 and 8 heads: 55 us, 67 with the empty entries gone through).
+  // of 32 and 8 heads, a CTA each: 55 us, 67 with the empty entries gone through).
   if (a.blocks && n && n <= 64) {
     const uint32_t late = __ballot_sync(0xffffffffu, w.page[1] != kNone), early = __ballot_sync(0xffffffffu, w.page[0] != kNone);
     n = late ? 64 - __clz(late) : 32 - __clz(early);
@@ -644,7 +644,10 @@ inline Shape shape_of(const AttendArg& a, int sms) {
   const uint32_t group = a.a.heads / a.c.heads;
   const uint64_t rows = a.blocks || a.block_count ? group : uint64_t(a.a.max_q) * group;
   const uint64_t units = a.blocks || a.block_count ? a.a.questions : a.t.seqs;
-  const uint32_t blocks = a.block_count ? a.block_count : (a.t.max_len + kPage - 1) / kPage;
+  const uint32_t pages = (a.t.max_len + kPage - 1) / kPage;
+  // a short sequence's list is mostly empty (81 of 3 to 32 rows, lists of 32, 8 heads
+  // of 32: 21 us, 55 with a CTA for each)
+  const uint32_t blocks = a.block_count ? std::min(a.block_count, pages) : pages;
   Shape sh{};
   sh.tiles = rows <= 8 || (a.c.dim > 32 && a.a.dtype == kF32) ? 1 : 2;  // most_tiles
   const uint64_t warps = (rows + 8 * sh.tiles - 1) / (8 * sh.tiles);
