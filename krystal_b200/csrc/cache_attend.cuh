@@ -22,8 +22,8 @@
 // sequences of up to 16384 rows (8 key heads of 128, e4m3) take 109 us, 5.2 TB/s;
 // one f16 token over 400003 rows 42 us, 5.1 TB/s. Many are bound by issue, 400 to
 // 900 instructions a cell and warp: 64 f32 questions over 64 masked banks of 4096
-// (4 heads of 32) take 181 us, of which the exponentials need 15 and the tensor
-// cores 30; 4096 banks of 8 to 240 rows with 1 to 16 questions 90 us, 2.1 TB/s.
+// (4 heads of 32) take 179 us, of which the exponentials need 15 and the tensor
+// cores 30; 4096 banks of 8 to 240 rows with 1 to 16 questions 91 us, 2.1 TB/s.
 #pragma once
 #include <algorithm>
 #include <type_traits>
@@ -708,7 +708,8 @@ cudaError_t attend_tile(const AttendArg& a, int sms, cudaStream_t s, uint64_t* l
 // 8 questions a warp, a cell at a time; `mg` warps with as many questions more
 // share the cells that their team brings, kg teams take turns at a sequence's cells
 // (64 f32 questions of 128 a bank of 4096: 8 warps a team; with the cells read once for
-// every 16 questions before, 110 us against 81). The products pass through shared
+// every 16 questions before, 110 us against 81; 72 since the questions are read 4
+// elements at once). The products pass through shared
 // memory so that masks are read and scores written 32 to a row; the mask's entries
 // are on their way while the cell is multiplied. Bound by issue: 540 instructions a
 // cell and warp, a quarter of them widening i8 keys.

@@ -588,7 +588,8 @@ def test_pointer_scores(be, dim, fmt, dtype, mask):
         got = s[at:at + n]
         assert (got[~ok] == np.float32(-1e30)).all()
         # a sum of d terms that may truncate, 22 bits of an f32 q, and the mask added
-        room = (np.abs(k) @ np.abs(a.q[i, 0]).astype(np.float64)) * sc * (dim * u + 2.0 ** -22) + 4 * u * (np.abs(x) + np.abs(np.where(ok, m, 0)))
+        room = (np.abs(k) @ np.abs(a.q[i, 0]).astype(np.float64)) * sc * (dim * u + 2.0 ** -22)
+        room += 4 * u * (np.abs(x) + np.abs(np.where(ok, m, 0)))
         assert (np.abs(got - x)[ok] <= room[ok]).all(), i
 
 
@@ -827,7 +828,8 @@ def test_refusals(be):
     for kw, match in [(dict(out=None), "an output"), (dict(out_pitch=255), "pitch is smaller"), (dict(mask=p(out)), "offsets"),
                       (dict(block_count=2), "list of blocks"), (dict(blocks=p(out)), "list of blocks"),
                       (dict(scale=float("nan")), "finite"), (dict(scale=float("inf")), "finite"), (dict(out=p(out) + 1), "aligned"),
-                      (dict(out=p(a.flat)), "over its questions"), (dict(lse=p(out) + 2), "aligned"), (dict(workspace=p(out) + 4), "16 bytes")]:
+                      (dict(out=p(a.flat)), "over its questions"), (dict(lse=p(out) + 2), "aligned"),
+                      (dict(workspace=p(out) + 4), "16 bytes")]:
         refused(match, be.cache_attend, **{**good, **kw})
     blocks = torch.zeros(3, 2, 2, dtype=torch.int32, device="cuda")
     refused("at least one block", be.cache_blocks, b.cache, b.table, a.view, 0, 0, p(blocks))
