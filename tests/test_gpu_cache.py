@@ -553,6 +553,21 @@ def test_lists_with_repeats_and_numbers_outside(be):
     a.check(got, lists=[[[int(x) for x in row] for row in lists[i]] for i in range(4)])
 
 
+@pytest.mark.parametrize("dtype,heads,count,mask", [("f32", 4, 20, False), ("bf16", 8, 40, False), ("f16", 4, 32, True)])
+def test_lists_of_many_short_sequences(be, dtype, heads, count, mask):
+    """Lists longer than their sequences: holes, repeats and numbers outside at any place, or nothing at all."""
+    b = Bank(be, [(37 * i) % 131 for i in range(210)], 4, 32, dtype=dtype)
+    a = Asked(b, [3 + i % 2 for i in range(210)], heads, dtype)
+    a.masks()
+    rng = np.random.default_rng(count)
+    lists = rng.integers(0, 4, (a.total, 4, count)).astype(np.uint32)
+    lists[rng.random(lists.shape) < 0.8] = ref.NONE
+    lists[:, 1, 5:] = ref.NONE
+    lists[:, 2, :-1] = ref.NONE
+    lists[::7, 3] = ref.NONE
+    a.check(a.attend(mask=mask, blocks=cuda(lists), block_count=count), mask=mask, lists=lists.tolist())
+
+
 def test_long_lists_are_cut_and_joined(be):
     b = Bank(be, [64 * 700 + 3], 1, 64, spread=0.3)
     a = Asked(b, [1], 4, "f16")
