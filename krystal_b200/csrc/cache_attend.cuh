@@ -15,6 +15,15 @@
 // while no score lies more than 6 binary orders above it, and B within 32, so that
 // most cells take a vote in place of the rows' maxima.
 //
+// Value scales far apart. x_j leaves f32 where t_j lies more than 134 below M. While
+// all e_j lie in -40 .. 24 (rows whose largest value is 1e-10 to 2e9) a row whose
+// x_j is lost has less than 2^-70 of the sum; rows of zeros count as -40, any
+// exponent is theirs. From the first cell with another scale on (the vote on M
+// finds it) a warp takes its cells in the general form, at two exponentials a
+// score: rows of zeros are left out of M, and the sums have a maximum of their own,
+//   l = sum 2^((b_j - B) + s_j - L),  L the largest exponent.
+// Sums that meet, of warps or parts, bring their L (M - 8 where there is none).
+//
 // A cell's bytes are read once by the team of warps that needs them, by 16-byte
 // asynchronous copies two cells ahead (one in masked calls of wide heads).
 //
@@ -36,7 +45,7 @@ namespace {
 
 constexpr int kThreads = 256, kWarps = 8;
 constexpr float kLift = 8.0f, kSlack = 6.0f, kFar = 32.0f;
-constexpr int kLeastExp = -80;  // value scales below it keep their digits in f_j; l stays below 2^128
+constexpr uint32_t kLeastExp = 127 - 40, kMostExp = 127 + 24;  // biased: usual value scales lie between
 
 // Cells a ring holds; a masked call's has the mask entries of each warp's rows
 // beside them, 36 floats apart so that what a warp reads at once lies on different banks.
@@ -47,9 +56,9 @@ __host__ __device__ constexpr int stages(int dim, bool masked) { return masked &
 // What a warp needs of one key of a cell: score = product * a * unit + e.
 struct KeyInfo {
   float a;   // key scale
-  float e;   // exponent of the value scale; -infinity: not attended
+  float e;   // exponent of the value scale; -infinity: not attended, or (general form) a row of zeros
   float f;   // value scale / 2^e
-  float re;  // 2^-e
+  float re;  // 2^-e; 0: not attended
 };
 
 // The unit of work a team looks at: a sequence's questions (or one question, with
@@ -121,23 +130,53 @@ __device__ __forceinline__ bool unit_of(const AttendArg& a, const Shape& sh, uin
 }
 
 // What is known of a row's scores, as the warps of a row, or the parts of a
-// sequence, are joined: [B, M, l, -] and o.
+// sequence, are joined: [B, M, l, L] and o. The sum of the exponentials is
+// l 2^(B + L), what they weigh o 2^(B + M - 8).
 struct Stat {
-  float b, m, l;
+  float b, m, l, low;
 };
-__device__ __forceinline__ float weight_of(const Stat& s, float b, float m) {
-  return s.m == -INFINITY ? 0.0f : ex2((s.b - b) + (s.m - m));
+__device__ __forceinline__ Stat nothing() { return Stat{-INFINITY, -INFINITY, 0.0f, -INFINITY}; }
+__device__ __forceinline__ Stat stat_at(const float* p) {
+  const float4 v = *reinterpret_cast<const float4*>(p);
+  return v.z > 0.0f ? Stat{v.x, v.y, v.z, v.w} : nothing();
+}
+__device__ __forceinline__ float4 packed(const Stat& s) { return make_float4(s.b, s.m, s.l, s.low); }
+// x 2^d where the product is in f32's range, though 2^d may not be.
+__device__ __forceinline__ float times_ex2(float x, float d) {
+  const float y = ex2(0.5f * d);
+  return x * y * y;
+}
+
+// The Stats of `width` neighbouring lanes (a power of two) as one, and what this
+// lane's o is multiplied by. The largest L does for the joined sum: the largest sum
+// is at least 2^(L - 16), since M - 8 lies 16 above its sum's logarithm at most.
+__device__ __forceinline__ Stat joined(const Stat& s, uint32_t width, float* weight) {
+  Stat all = s;
+  for (uint32_t o = width / 2; o; o >>= 1) all.b = fmaxf(all.b, __shfl_xor_sync(0xffffffffu, all.b, o));
+  const bool some = s.l > 0.0f;
+  const float up = some ? s.b - all.b : 0.0f;
+  all.m = up + s.m;
+  all.low = up + s.low;
+  for (uint32_t o = width / 2; o; o >>= 1) {
+    all.m = fmaxf(all.m, __shfl_xor_sync(0xffffffffu, all.m, o));
+    all.low = fmaxf(all.low, __shfl_xor_sync(0xffffffffu, all.low, o));
+  }
+  *weight = s.m == -INFINITY ? 0.0f : ex2(up + (s.m - all.m));
+  all.l = some ? times_ex2(s.l, up + (s.low - all.low)) : 0.0f;
+  for (uint32_t o = width / 2; o; o >>= 1) all.l += __shfl_xor_sync(0xffffffffu, all.l, o);
+  return all;
 }
 
 template <typename T, int FMT>
-__device__ __forceinline__ void put(const AttendArg& a, uint64_t question, uint32_t head, uint32_t dim, float o, float l) {
-  static_cast<T*>(a.out)[question * a.out_pitch + uint64_t(head) * a.c.dim + dim] = from_f32<T>(l > 0.0f ? o * (1.0f / l) : 0.0f);
+__device__ __forceinline__ void put(const AttendArg& a, uint64_t question, uint32_t head, uint32_t dim, float o, const Stat& s) {
+  static_cast<T*>(a.out)[question * a.out_pitch + uint64_t(head) * a.c.dim + dim] =
+      from_f32<T>(s.l > 0.0f ? times_ex2(o * (1.0f / s.l), s.m - kLift - s.low) : 0.0f);
 }
 __device__ __forceinline__ void put_lse(const AttendArg& a, uint64_t question, uint32_t head, const Stat& s) {
-  if (a.lse) a.lse[question * a.a.heads + head] = s.l > 0.0f ? (s.b + s.m - kLift) * kLn2 + logf(s.l) : -INFINITY;
+  if (a.lse) a.lse[question * a.a.heads + head] = s.l > 0.0f ? (s.b + s.low) * kLn2 + logf(s.l) : -INFINITY;
 }
 
-// Part `part` of a row's results in the workspace: o [dim], then B, M, l.
+// Part `part` of a row's results in the workspace: o [dim], then B, M, l, L.
 __device__ __forceinline__ float* part_of(const AttendArg& a, uint64_t question, uint32_t head, uint32_t part) {
   return a.work + ((question * a.a.heads + head) * a.splits + part) * (a.c.dim + 4);
 }
@@ -177,6 +216,19 @@ __device__ __forceinline__ void copy_cell(uint8_t* dst, const uint8_t* src, uint
     const uint32_t at = thread + k * MG * 32;
     if ((k + 1) * MG * 32 <= CB / 16 || at < CB / 16) copy16(dst + 16 * at, src + 16 * at);
   }
+}
+
+// Whether a row of D codes is one of zeros.
+template <int D, int FMT>
+__device__ __forceinline__ bool zero_row(const uint8_t* codes) {
+  uint32_t any = 0;
+#pragma unroll
+  for (int i = 0; i < D / 16; i++) {
+    const uint4 w = reinterpret_cast<const uint4*>(codes)[i];
+    if (FMT == kI8) any |= (w.x ^ 0x80808080u) | (w.y ^ 0x80808080u) | (w.z ^ 0x80808080u) | (w.w ^ 0x80808080u);
+    else any |= (w.x | w.y | w.z | w.w) & 0x7f7f7f7fu;  // 0 and -0
+  }
+  return any == 0;
 }
 
 // f16 pieces of a weight: two for f32 questions (22 bits) and for f16 ones, whose
@@ -305,19 +357,15 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
     }
   }
   KeyInfo* info = s_info[warp];
-  for (uint32_t i = 0; i < n; i++) {
-    w.advance(i);
-    copy_wait<S - 2>();
-    meet(team, sh.mg);
-    const uint32_t page = ahead[0], block = w.block_of(i, 0);
-#pragma unroll
-    for (int k = 0; k + 2 < S; k++) ahead[k] = ahead[k + 1];
-    ahead[S - 2] = w.page_of(i, S - 1);  // none behind the last
-    issue(i + S - 1, ahead[S - 2], MASKED ? w.block_of(i, S - 1) : 0);
-    if (!n_rows || page == kNone) continue;
+  float low[NT][2];  // L, of the general form
+  // Cell i, which has arrived, in the usual form or the general one. False: the
+  // usual form does not do for it, and has left it.
+  auto take = [&](auto general, uint32_t i, uint32_t page, uint32_t block) -> bool {
+    constexpr bool kGeneral = decltype(general)::value;
+    if (!n_rows || page == kNone) return true;
     uint8_t* cell = ring + (i % S) * CB;
     const uint64_t pos = uint64_t(block) * kPage + w.half(i) * kCell;
-    if (pos >= u.len) continue;
+    if (pos >= u.len) return true;
     if (FMT == kE4M3 && pos + kCell > u.len) {
       // bytes behind the sequence's last row may be e4m3's NaN, which no weight of
       // 0 takes away; every warp of a team writes the zeros that it will read
@@ -328,16 +376,22 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
       }
       __syncwarp();
     }
+    const float* scales = reinterpret_cast<const float*>(cell + 2 * kCell * D);
+    bool apart;  // the lane's row has an unusual scale, or is one of zeros
     {
-      const float* scales = reinterpret_cast<const float*>(cell + 2 * kCell * D);
       const float vs = scales[kCell + lane];
-      const uint32_t e = min(max(__float_as_uint(vs) >> 23, uint32_t(127 + kLeastExp)), 253u);
+      const uint32_t e = min(max(__float_as_uint(vs) >> 23, kGeneral ? 27u : kLeastExp), 253u);
       KeyInfo k;
       k.re = pow2_biased(254u - e);
       k.f = vs * k.re;
       k.a = scales[lane];
       k.e = float(int(e) - 127);
-      if (pos + lane >= open_end) k = KeyInfo{0.0f, -INFINITY, 0.0f, 0.0f};
+      if (kGeneral && vs == kLeastScale && zero_row<D, FMT>(cell + (kCell + lane) * D)) k.e = -INFINITY;
+      apart = e - (kLeastExp + 1) >= kMostExp - kLeastExp;
+      if (pos + lane >= open_end) {
+        k = KeyInfo{0.0f, -INFINITY, 0.0f, 0.0f};
+        apart = false;
+      }
       info[lane] = k;
     }
     float s[NT][2][4];
@@ -351,9 +405,10 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
 #pragma unroll
       for (int t = 0; t < NT; t++) {
         float* x = &s[t][j / 2][2 * (j % 2)];
-        const float2 y = halves(fma2(mul2(pair(x[0], x[1]), ka), pair(q.unit[t][0], q.unit[t][1]), ke));
-        x[0] = y.x;
-        x[1] = y.y;
+        const Pair y = mul2(pair(x[0], x[1]), ka), unit = pair(q.unit[t][0], q.unit[t][1]);
+        const float2 z = halves(kGeneral ? mul2(y, unit) : fma2(y, unit, ke));
+        x[0] = kGeneral && key[j].re == 0.0f ? -INFINITY : z.x;
+        x[1] = kGeneral && key[j].re == 0.0f ? -INFINITY : z.y;
       }
     }
     if (MASKED) {
@@ -374,8 +429,10 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
           for (int h = 0; h < 2; h++) {
             const float was = top[t][h];
             top[t][h] = fmaxf(was, row_most(most[h]));
-            if (was != top[t][h])  // M is measured from the new one
+            if (was != top[t][h]) {  // M is measured from the new one, and L
               high[t][h] = was == -INFINITY ? -INFINITY : high[t][h] + (was - top[t][h]);
+              if (kGeneral) low[t][h] = was == -INFINITY ? -INFINITY : low[t][h] + (was - top[t][h]);
+            }
           }
         }
 #pragma unroll
@@ -389,8 +446,27 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
         }
       }
     }
+    if (kGeneral) {
+#pragma unroll
+      for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          float now = low[t][h];
+          now = fmaxf(now, row_most(fmaxf(fmaxf(s[t][0][h], s[t][0][2 + h]), fmaxf(s[t][1][h], s[t][1][2 + h]))));
+          if (now > -INFINITY) {
+            sum[t][h] *= ex2(low[t][h] - now);
+            low[t][h] = now;
+          }
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            float& y = s[t][j / 2][2 * (j % 2) + h];
+            if (y > -INFINITY) sum[t][h] += ex2(y - now);
+            y += key[j].e;
+          }
+        }
+    }
     float most[NT][2];
-    bool above = false;
+    bool above = apart && !kGeneral;
 #pragma unroll
     for (int t = 0; t < NT; t++)
 #pragma unroll
@@ -399,6 +475,10 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
         above |= most[t][h] > high[t][h] + kSlack;
       }
     if (__any_sync(0xffffffffu, above)) {
+      if (!kGeneral) {  // rows of zeros are taken as they are
+        if (apart && scales[kCell + lane] == kLeastScale) apart = !zero_row<D, FMT>(cell + (kCell + lane) * D);
+        if (__any_sync(0xffffffffu, apart)) return false;
+      }
 #pragma unroll
       for (int t = 0; t < NT; t++) {
         float keep[2];
@@ -407,7 +487,7 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
           const float now = fmaxf(high[t][h], row_most(most[t][h]));
           keep[h] = now == high[t][h] ? 1.0f : ex2(high[t][h] - now);
           high[t][h] = now;
-          sum[t][h] *= keep[h];
+          if (!kGeneral) sum[t][h] *= keep[h];
         }
 #pragma unroll
         for (int m = 0; m < MT; m++)
@@ -417,7 +497,7 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
     }
     // f32 outputs: a cell's products are summed by themselves. The tensor cores'
     // sums truncate, and one sum over 16 cells was off by 1.2e-6, this by 4e-7.
-    float part_o[kApart ? NT : 1][kApart ? MT : 1][4] = {};
+    [[maybe_unused]] float part_o[kApart ? NT : 1][kApart ? MT : 1][4] = {};
 #pragma unroll
     for (int v = 0; v < 2; v++) {
       uint32_t hi[NT][2], lo[kTwo ? NT : 1][2];
@@ -431,7 +511,7 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
           const KeyInfo& k = key[2 * v + j];
           const float2 y = halves(add2(pair(s[t][v][2 * j], s[t][v][2 * j + 1]), less));
           const Pair x = pair(ex2(y.x), ex2(y.y));
-          l = fma2(x, pair(k.re, k.re), l);
+          if (!kGeneral) l = fma2(x, pair(k.re, k.re), l);
           const Pair w = mul2(x, pair(k.f, k.f));
           const float2 wf = halves(w);
           const uint32_t h = pack(wf.x, wf.y);
@@ -461,6 +541,41 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
           }
     }
     __syncwarp();
+    return true;
+  };
+  auto arrive = [&](uint32_t i) {  // of the team; cell i + S - 1 is sent for
+    w.advance(i);
+    copy_wait<S - 2>();
+    meet(team, sh.mg);
+    const uint32_t page = ahead[0];
+#pragma unroll
+    for (int k = 0; k + 2 < S; k++) ahead[k] = ahead[k + 1];
+    ahead[S - 2] = w.page_of(i, S - 1);  // none behind the last
+    issue(i + S - 1, ahead[S - 2], MASKED ? w.block_of(i, S - 1) : 0);
+    return page;
+  };
+  uint32_t i = 0;
+  for (; i < n; i++) {
+    const uint32_t page = arrive(i);
+    if (!take(std::false_type{}, i, page, w.block_of(i, 0))) break;
+  }
+  const bool general = i < n;
+  if (general) {
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        low[t][h] = high[t][h] - kLift;
+        bool some = false;
+#pragma unroll
+        for (int m = 0; m < MT; m++) some |= o[t][m][h] != 0.0f || o[t][m][2 + h] != 0.0f;
+        // a row that has seen rows of zeros alone has no M
+        if (!(__ballot_sync(0xffffffffu, some) & (0x11111111u << c))) high[t][h] = -INFINITY;
+      }
+    for (uint32_t page = w.page_of(i, 0);; page = arrive(i)) {
+      take(std::true_type{}, i, page, w.block_of(i, 0));
+      if (++i == n) break;
+    }
   }
   copy_wait<0>();
 #pragma unroll
@@ -470,6 +585,9 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
 #pragma unroll
       for (int x = 4; x < 32; x <<= 1) sum[t][h] += __shfl_xor_sync(0xffffffffu, sum[t][h], x);
 
+  auto stat_of = [&](int t, int h) {
+    return Stat{top[t][h], high[t][h], sum[t][h], general ? low[t][h] : high[t][h] - kLift};
+  };
   if (sh.kg == 1) {  // a row has one warp
     const bool wide = (reinterpret_cast<uintptr_t>(a.out) | a.out_pitch * sizeof(T)) % 16 == 0;
 #pragma unroll
@@ -481,18 +599,22 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
         const RowId id = row_id(row0 + r, group);
         const uint64_t question = u.q0 + id.question;
         const uint32_t head = u.kv * group + id.head;
-        const Stat st{top[t][h], high[t][h], sum[t][h]};
+        const Stat st = stat_of(t, h);
         const float unit = parts > 1 ? 1.0f : st.l > 0.0f ? 1.0f / st.l : 0.0f;
         float run[NB];
 #pragma unroll
         for (int k = 0; k < NB; k++) run[k] = o[t][k / 2][2 * (k % 2) + h] * unit;
+        if (general && parts == 1) {
+#pragma unroll
+          for (int k = 0; k < NB; k++) run[k] = st.l > 0.0f ? times_ex2(run[k], st.m - kLift - st.low) : 0.0f;
+        }
         if (parts == 1) {
           put_run(static_cast<T*>(a.out) + question * a.out_pitch + head * uint64_t(D) + g * NB, run, wide);
           if (g == 0) put_lse(a, question, head, st);
         } else {
           float* p = part_of(a, question, head, part);
           put_run(p + g * NB, run, true);
-          if (g == 0) *reinterpret_cast<float4*>(p + D) = make_float4(st.b, st.m, st.l, 0.0f);
+          if (g == 0) *reinterpret_cast<float4*>(p + D) = packed(st);
         }
       }
     return;
@@ -511,41 +633,33 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
 #pragma unroll
       for (int k = 0; k < NB; k++) run[k] = o[t][k / 2][2 * (k % 2) + h];
       put_run(p + g * NB, run, true);
-      if (g == 0) *reinterpret_cast<float4*>(p + D) = make_float4(top[t][h], high[t][h], sum[t][h], 0.0f);
+      if (g == 0) *reinterpret_cast<float4*>(p + D) = packed(stat_of(t, h));
     }
   __syncthreads();
   // the team kgi of a unit's kg takes every kg-th row of its warps'
   const uint32_t kgi = team % sh.kg, base = (team - kgi) * sh.mg + mi;
   for (uint32_t r = kgi; r < n_rows; r += sh.kg) {
-    Stat all{-INFINITY, -INFINITY, 0.0f};
-    for (uint32_t k = 0; k < sh.kg; k++) {
-      const float* p = join + ((base + k * sh.mg) * R + r) * (D + 4);
-      if (p[D + 1] > -INFINITY) all.b = fmaxf(all.b, p[D]);
-    }
-    for (uint32_t k = 0; k < sh.kg; k++) {
-      const float* p = join + ((base + k * sh.mg) * R + r) * (D + 4);
-      if (p[D + 1] > -INFINITY) all.m = fmaxf(all.m, (p[D] - all.b) + p[D + 1]);
-    }
+    auto at = [&](uint32_t k) { return join + ((base + k * sh.mg) * R + r) * (D + 4); };
+    float weight;
+    const Stat all = joined(stat_at(at(lane & (sh.kg - 1)) + D), sh.kg, &weight);
     float acc[D / 32] = {};
     for (uint32_t k = 0; k < sh.kg; k++) {
-      const float* p = join + ((base + k * sh.mg) * R + r) * (D + 4);
-      const float x = weight_of(Stat{p[D], p[D + 1], p[D + 2]}, all.b, all.m);
-      all.l = fmaf(x, p[D + 2], all.l);
+      const float x = __shfl_sync(0xffffffffu, weight, k);
 #pragma unroll
-      for (int e = 0; e < D / 32; e++) acc[e] = fmaf(x, p[lane + 32 * e], acc[e]);
+      for (int e = 0; e < D / 32; e++) acc[e] = fmaf(x, at(k)[lane + 32 * e], acc[e]);
     }
     const RowId id = row_id(row0 + r, group);
     const uint64_t question = u.q0 + id.question;
     const uint32_t head = u.kv * group + id.head;
     if (parts == 1) {
 #pragma unroll
-      for (int e = 0; e < D / 32; e++) put<T, FMT>(a, question, head, lane + 32 * e, acc[e], all.l);
+      for (int e = 0; e < D / 32; e++) put<T, FMT>(a, question, head, lane + 32 * e, acc[e], all);
       if (lane == 0) put_lse(a, question, head, all);
     } else {
       float* p = part_of(a, question, head, part);
 #pragma unroll
       for (int e = 0; e < D / 32; e++) p[lane + 32 * e] = acc[e];
-      if (lane == 0) *reinterpret_cast<float4*>(p + D) = make_float4(all.b, all.m, all.l, 0.0f);
+      if (lane == 0) *reinterpret_cast<float4*>(p + D) = packed(all);
     }
   }
 }
@@ -574,32 +688,26 @@ __global__ __launch_bounds__(kThreads) void k_join(AttendArg a, uint32_t per) {
   const uint32_t all = !live ? 0 : a.blocks ? a.block_count : (length_of(a.t, seq) + kPage - 1) / kPage;
   const uint32_t parts = (all + a.chunk - 1) / a.chunk;
   live = live && parts > 1;
-  Stat st{-INFINITY, -INFINITY, 0.0f};
+  // lanes that the parts fill; the others hold them again
+  const uint32_t width = a.splits > 16 ? 32 : a.splits > 8 ? 16 : a.splits > 4 ? 8 : a.splits > 2 ? 4 : 2;
+  Stat st = nothing();
   float acc[D / 32] = {};
   if (live) {
     const float* p = part_of(a, question, head, 0);
     for (uint32_t k0 = share * 32; k0 < parts; k0 += per * 32) {
-      const uint32_t mine = k0 + lane;
-      Stat other{-INFINITY, -INFINITY, 0.0f};
-      if (mine < parts) {
-        const float4 v = *reinterpret_cast<const float4*>(p + uint64_t(mine) * (D + 4) + D);
-        other = Stat{v.y > -INFINITY ? v.x : -INFINITY, v.y, v.z};
+      const uint32_t mine = k0 + (lane & (width - 1));
+      float add, keep;
+      const Stat other = joined(mine < parts ? stat_at(p + uint64_t(mine) * (D + 4) + D) : nothing(), width, &add);
+      if (k0 == share * 32) {
+        st = other;
+      } else {  // lane by lane what is held and what comes
+        const bool come = lane & 1;
+        st = joined(come ? other : st, 2, &keep);
+        add *= __shfl_sync(0xffffffffu, keep, 1);
+        keep = __shfl_sync(0xffffffffu, keep, 0);
+#pragma unroll
+        for (int e = 0; e < D / 32; e++) acc[e] *= keep;
       }
-      float b = fmaxf(st.b, other.b);
-#pragma unroll
-      for (int o = 16; o; o >>= 1) b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, o));
-      if (b == -INFINITY) continue;
-      float m = fmaxf(st.m == -INFINITY ? -INFINITY : (st.b - b) + st.m,
-                      other.m == -INFINITY ? -INFINITY : (other.b - b) + other.m);
-#pragma unroll
-      for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const float keep = weight_of(st, b, m), add = weight_of(other, b, m);
-      float l = add * other.l;
-#pragma unroll
-      for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-      st = Stat{b, m, fmaf(keep, st.l, l)};
-#pragma unroll
-      for (int e = 0; e < D / 32; e++) acc[e] *= keep;
       const uint32_t n = min(32u, parts - k0);
       const float* x = p + uint64_t(k0) * (D + 4) + lane;
 #pragma unroll 8
@@ -616,23 +724,19 @@ __global__ __launch_bounds__(kThreads) void k_join(AttendArg a, uint32_t per) {
     if (lane == 0) s_stat[warp] = st;
     __syncthreads();
     if (share) return;
-    Stat sum{-INFINITY, -INFINITY, 0.0f};
-    for (uint32_t k = 0; k < per; k++) sum.b = fmaxf(sum.b, s_stat[warp + k].b);
-    for (uint32_t k = 0; k < per; k++)
-      if (s_stat[warp + k].m > -INFINITY) sum.m = fmaxf(sum.m, (s_stat[warp + k].b - sum.b) + s_stat[warp + k].m);
+    float weight;
+    st = joined(s_stat[warp + (lane & (per - 1))], per, &weight);
 #pragma unroll
     for (int e = 0; e < D / 32; e++) acc[e] = 0.0f;
     for (uint32_t k = 0; k < per; k++) {
-      const float x = weight_of(s_stat[warp + k], sum.b, sum.m);
-      sum.l = fmaf(x, s_stat[warp + k].l, sum.l);
+      const float x = __shfl_sync(0xffffffffu, weight, k);
 #pragma unroll
       for (int e = 0; e < D / 32; e++) acc[e] = fmaf(x, s_o[warp + k][lane + 32 * e], acc[e]);
     }
-    st = sum;
   }
   if (!live) return;
 #pragma unroll
-  for (int e = 0; e < D / 32; e++) put<T, FMT>(a, question, head, lane + 32 * e, acc[e], st.l);
+  for (int e = 0; e < D / 32; e++) put<T, FMT>(a, question, head, lane + 32 * e, acc[e], st);
   if (lane == 0) put_lse(a, question, head, st);
 }
 
