@@ -89,7 +89,7 @@ kc_status turn_pass(kc_handle* h, const DevBatch& b, const kc::FrameTotals& tot,
     a.c = bank.mixer[blk];
     a.t = bank.table;
     a.a = ask;
-    a.scale = float(1.0 / std::sqrt(double(d.hd)));
+    a.scale = kc::cache::scale_by(float(1.0 / std::sqrt(double(d.hd))));
     a.out_pitch = H;
     KC_TRY(ensure(h, ws.turn_attend, Q * H * 4), "workspace");
     KC_TRY(ensure(h, ws.turn_work, kc::cache::plan_attend(a, h->sms) * 4 + 16), "workspace");
@@ -109,7 +109,7 @@ kc_status turn_pass(kc_handle* h, const DevBatch& b, const kc::FrameTotals& tot,
   ask.q = ws.sq.p;
   ask.heads = 1;
   const kc::cache::ScoreArg sa{bank.selector, bank.table, ask, out->p, P<uint64_t>(ws.turn_off), b.mask,
-                               float(1.0 / std::sqrt(double(d.h)))};
+                               kc::cache::scale_by(float(1.0 / std::sqrt(double(d.h))))};
   KC_TRY(kc::cache::launch_scores(sa, h->sms, h->stream, &h->launches), "scores launch");
   const kc_sampling whole{1.0f, 0, 1.0f, 0.0f, nullptr, nullptr, nullptr, nullptr};
   const kc_rows_view rows{out->p, nullptr, nullptr, uint32_t(Q), 0, row, 0, KC_DTYPE_F32, KC_ROWS_SCORES};

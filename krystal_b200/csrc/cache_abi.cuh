@@ -112,9 +112,9 @@ kc_status launched(kc_handle* h, cudaError_t e, const char* what) {
   return KC_OK;
 }
 
-kc_status check_scale(kc_handle* h, float scale, uint32_t dim, float* out) {
+kc_status check_scale(kc_handle* h, float scale, uint32_t dim, kc::cache::Scale* out) {
   if (!std::isfinite(scale)) return fail(h, KC_ERR_INVALID_ARG, "scale must be finite");
-  *out = scale != 0.0f ? scale : float(1.0 / std::sqrt(double(dim)));
+  *out = kc::cache::scale_by(scale != 0.0f ? scale : float(1.0 / std::sqrt(double(dim))));
   return KC_OK;
 }
 

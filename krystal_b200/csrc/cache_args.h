@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <cmath>
+
 namespace kc {
 namespace cache {
 
@@ -55,6 +57,17 @@ struct Ask {
   int dtype;
 };
 
+// What scores are multiplied by: m 2^e, |m| in [1/2, 1).
+struct Scale {
+  float m;
+  int e;
+};
+inline Scale scale_by(float x) {
+  Scale s;
+  s.m = std::frexp(x, &s.e);
+  return s;
+}
+
 struct AttendArg {
   Store c;
   Table t;
@@ -66,7 +79,7 @@ struct AttendArg {
   const uint64_t* mask_off;
   const uint32_t* blocks;   // [questions][kv heads][block_count], or null: every block
   uint32_t block_count;
-  float scale;
+  Scale scale;
   float* work;              // partial results of split sequences
   uint32_t splits;          // parts a sequence's rows are cut into at most (1: none)
   uint32_t chunk;           // blocks of a part
@@ -79,7 +92,7 @@ struct ScoreArg {
   float* scores;            // sequence s's [Q_s, R_s] block at off[s]
   const uint64_t* off;
   const float* mask;        // laid out like scores, or null
-  float scale;
+  Scale scale;
 };
 
 struct BlockArg {

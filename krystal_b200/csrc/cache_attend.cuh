@@ -15,12 +15,13 @@
 // while no score lies more than 6 binary orders above it, and B within 32, so that
 // most cells take a vote in place of the rows' maxima.
 //
-// Value scales far apart. x_j leaves f32 where t_j lies more than 134 below M. While
-// all e_j lie in -40 .. 24 (rows whose largest value is 1e-10 to 2e9) a row whose
-// x_j is lost has less than 2^-70 of the sum; rows of zeros count as -40, any
-// exponent is theirs. From the first cell with another scale on (the vote on M
-// finds it) a warp takes its cells in the general form, at two exponentials a
-// score: rows of zeros are left out of M, and the sums have a maximum of their own,
+// The general form. x_j leaves f32 where t_j lies more than 134 below M. While all
+// e_j lie in -40 .. 24 (rows whose largest value is 1e-10 to 2e9) a row whose x_j is
+// lost has less than 2^-70 of the sum; rows of zeros count as -40, any exponent is
+// theirs. From the first cell with another scale on (the vote on M finds it), or for
+// questions whose scores two multiplications do not give (cache_tile.cuh), a warp
+// takes its cells in a form of two exponentials a score: rows of zeros are left out
+// of M, and the sums have a maximum of their own,
 //   l = sum 2^((b_j - B) + s_j - L),  L the largest exponent.
 // Sums that meet, of warps or parts, bring their L (M - 8 where there is none).
 //
@@ -53,7 +54,7 @@ constexpr int kMaskPitch = 36;
 __host__ __device__ constexpr int mask_bytes(int tiles) { return 8 * tiles * kMaskPitch * 4; }
 __host__ __device__ constexpr int stages(int dim, bool masked) { return masked && dim > 32 ? 2 : 3; }
 
-// What a warp needs of one key of a cell: score = product * a * unit + e.
+// What a warp needs of one key of a cell: score = product * unit * a + e.
 struct KeyInfo {
   float a;   // key scale
   float e;   // exponent of the value scale; -infinity: not attended, or (general form) a row of zeros
@@ -334,12 +335,17 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
     }
   }
   QTile<T, D, NT> q;
+  bool general = false;  // the form of the cells
+  volatile int powers[NT][2];  // of the units; in local memory, the general form's alone
   const bool wide_q = (reinterpret_cast<uintptr_t>(a.a.q) | a.a.pitch * sizeof(T)) % 16 == 0;
 #pragma unroll
   for (int t = 0; t < NT; t++) {
     const RowId r = row_id(row0 + 8 * t + g, group);
     const T* at = static_cast<const T*>(a.a.q) + (u.q0 + r.question) * a.a.pitch + (u.kv * group + r.head) * uint64_t(D);
-    q.load(t, uint32_t(8 * t + g) < n_rows ? at : nullptr, wide_q, c, a.scale * kLog2e);
+    int power[2];
+    general |= q.load(t, uint32_t(8 * t + g) < n_rows ? at : nullptr, wide_q, c, a.scale.m * kLog2e, a.scale.e, power);
+    powers[t][0] = power[0];
+    powers[t][1] = power[1];
   }
 
   float o[NT][MT][4], top[NT][2], high[NT][2], sum[NT][2];
@@ -405,10 +411,15 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
 #pragma unroll
       for (int t = 0; t < NT; t++) {
         float* x = &s[t][j / 2][2 * (j % 2)];
-        const Pair y = mul2(pair(x[0], x[1]), ka), unit = pair(q.unit[t][0], q.unit[t][1]);
-        const float2 z = halves(kGeneral ? mul2(y, unit) : fma2(y, unit, ke));
-        x[0] = kGeneral && key[j].re == 0.0f ? -INFINITY : z.x;
-        x[1] = kGeneral && key[j].re == 0.0f ? -INFINITY : z.y;
+        if (kGeneral) {
+#pragma unroll
+          for (int h = 0; h < 2; h++)
+            x[h] = key[j].re == 0.0f ? -INFINITY : far_score(x[h], a.scale.m * kLog2e, powers[t][h], key[j].a);
+        } else {
+          const float2 y = halves(fma2(mul2(pair(x[0], x[1]), pair(q.unit[t][0], q.unit[t][1])), ka, ke));
+          x[0] = y.x;
+          x[1] = y.y;
+        }
       }
     }
     if (MASKED) {
@@ -555,12 +566,12 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
     return page;
   };
   uint32_t i = 0;
-  for (; i < n; i++) {
+  if (general && n) arrive(0);
+  for (; i < n && !general; i += !general) {
     const uint32_t page = arrive(i);
-    if (!take(std::false_type{}, i, page, w.block_of(i, 0))) break;
+    general = !take(std::false_type{}, i, page, w.block_of(i, 0));
   }
-  const bool general = i < n;
-  if (general) {
+  if (general && n) {
 #pragma unroll
     for (int t = 0; t < NT; t++)
 #pragma unroll
@@ -572,7 +583,7 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
         // a row that has seen rows of zeros alone has no M
         if (!(__ballot_sync(0xffffffffu, some) & (0x11111111u << c))) high[t][h] = -INFINITY;
       }
-    for (uint32_t page = w.page_of(i, 0);; page = arrive(i)) {
+    for (uint32_t page = w.page_of(i, 0);; page = arrive(i)) {  // the first has arrived
       take(std::true_type{}, i, page, w.block_of(i, 0));
       if (++i == n) break;
     }
@@ -822,6 +833,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_scores(ScoreArg a, uint32_t mg,
   constexpr int S = 3, KB = int(kCell) * D, CB = KB + int(kCell) * 4;  // keys and their scales
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float s_tile[kWarps][8][kCell + 1];
+  __shared__ int s_power[kWarps][8];  // of the rows' units, where they are far from 1
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   const uint32_t team = warp / mg, mi = warp % mg, kg = kWarps / mg;
   const uint32_t seq = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
@@ -864,8 +876,16 @@ __global__ __launch_bounds__(kThreads, 2) void k_scores(ScoreArg a, uint32_t mg,
     issue(i, ahead[i]);
   }
   QTile<T, D, 1> q;
-  q.load(0, uint32_t(g) < n_rows ? static_cast<const T*>(a.a.q) + (q0 + row0 + g) * a.a.pitch : nullptr,
-         (reinterpret_cast<uintptr_t>(a.a.q) | a.a.pitch * sizeof(T)) % 16 == 0, c, a.scale);
+  int power[2];
+  const bool far = q.load(0, uint32_t(g) < n_rows ? static_cast<const T*>(a.a.q) + (q0 + row0 + g) * a.a.pitch : nullptr,
+                          (reinterpret_cast<uintptr_t>(a.a.q) | a.a.pitch * sizeof(T)) % 16 == 0, c, a.scale.m, a.scale.e, power);
+  if (far) {
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      s_power[warp][2 * c + h] = power[h];
+      q.unit[0][h] = 1.0f;
+    }
+  }
   float (*tile)[kCell + 1] = s_tile[warp];
   const uint64_t at0 = a.off[seq] + row0 * stride;
   for (uint32_t i = 0; i < n; i++) {
@@ -899,6 +919,10 @@ __global__ __launch_bounds__(kThreads, 2) void k_scores(ScoreArg a, uint32_t mg,
         for (int h = 0; h < 2; h++) tile[2 * c + h][8 * j + key_of(g)] = s[0][j / 2][2 * (j % 2) + h] * q.unit[0][h];
     }
     __syncwarp();
+    if (far) {
+      for (int r = 0; r < 8; r++) tile[r][lane] = far_score(tile[r][lane], a.scale.m, s_power[warp][r], unit);
+      unit = 1.0f;
+    }
     if (there) {
       const bool held = page != kNone && pos < len;
       float* out = a.scores + at0 + pos;

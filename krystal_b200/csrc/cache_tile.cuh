@@ -14,7 +14,9 @@
 // Exactness. Codes are exact in f16. A question row is divided by a power of two
 // that brings its largest element into [1, 2); 16-bit questions are then exact
 // (bits 2^-25 below the largest aside), f32 ones are the sum of two f16 (22 bits,
-// two products). Products accumulate in f32.
+// two products). Products accumulate in f32, below 2^17. They are multiplied by the
+// row's unit, then by the key's scale; where the unit lies outside 2^-126 .. 2^108
+// the exponents of both are added as whole numbers first (times_pow2).
 #pragma once
 #include "cache.cuh"
 
@@ -55,6 +57,19 @@ __device__ __forceinline__ uint32_t widen(uint32_t w) {
 
 // 2^x, x an integer in [-126, 127] given as its biased exponent.
 __device__ __forceinline__ float pow2_biased(uint32_t e) { return __uint_as_float(e << 23); }
+
+// x 2^n where the product is in f32's range, though 2^n may not be.
+__device__ __forceinline__ float times_pow2(float x, int n) {
+  n = min(max(n, -252), 252);
+  const int half = n >> 1;
+  return x * pow2_biased(uint32_t(127 + half)) * pow2_biased(uint32_t(127 + n - half));
+}
+
+// s: a product of a row whose unit is m 2^power, key: the key's scale.
+__device__ __forceinline__ float far_score(float s, float m, int power, float key) {
+  const uint32_t bits = __float_as_uint(key);
+  return times_pow2(s * m * __uint_as_float((bits & 0x007fffffu) | 0x3f800000u), power + int(bits >> 23) - 127);
+}
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -112,6 +127,7 @@ struct QTile {
   static constexpr int kSteps = D / 16;
   uint32_t hi[NT][kSteps][2], lo[kTwo ? NT : 1][kTwo ? kSteps : 1][2];
   float unit[NT][2];  // what a product of rows 2c and 2c + 1 of a tile is multiplied by
+  static constexpr int kLeastPower = -126, kMostPower = 108;  // of two that a unit may hold
 
   // Dimension of the first of the 4 elements of lane c's piece of fragment s.
   static __device__ __forceinline__ int dim(int s, int c) {
@@ -120,8 +136,9 @@ struct QTile {
 
   // row: row g of tile t, null where there is none; wide: it begins at 16 bytes, and
   // is read 4 elements at once (515 sequences of 20 questions, 8 heads of 128 in f16
-  // over 2: 118 us, 123 one by one). factor multiplies every score.
-  __device__ __forceinline__ void load(int t, const T* row, bool wide, int c, float factor) {
+  // over 2: 118 us, 123 one by one). m 2^e multiplies every score. power: the units
+  // are m 2^power; true where a unit does not hold one of the tile's.
+  __device__ __forceinline__ bool load(int t, const T* row, bool wide, int c, float m, int e, int (&power)[2]) {
     float x[kSteps][4], top = 0.0f;
 #pragma unroll
     for (int s = 0; s < kSteps; s++) {
@@ -138,16 +155,20 @@ struct QTile {
       }
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        x[s][i] = to_f32(y[i]) * (kTwo ? factor : 1.0f);
+        x[s][i] = to_f32(y[i]);
         top = fmaxf(top, fabsf(x[s][i]));
       }
     }
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const uint32_t e = min(max(__float_as_uint(top) >> 23, 1u), 253u);
-    const float down = pow2_biased(254u - e), own = pow2_biased(e) * (kTwo ? 1.0f : factor);
-    unit[t][0] = __shfl_sync(0xffffffffu, own, 8 * c);
-    unit[t][1] = __shfl_sync(0xffffffffu, own, 8 * c + 4);
+    const uint32_t biased = top == 0.0f ? 127u : min(max(__float_as_uint(top) >> 23, 1u), 253u);
+    const float down = pow2_biased(254u - biased);
+    const int own = int(biased) - 127 + e;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      power[h] = __shfl_sync(0xffffffffu, own, 8 * c + 4 * h);
+      unit[t][h] = m * pow2_biased(uint32_t(127 + min(max(power[h], kLeastPower), 127)));
+    }
 #pragma unroll
     for (int s = 0; s < kSteps; s++)
 #pragma unroll
@@ -159,6 +180,7 @@ struct QTile {
           lo[kTwo ? t : 0][kTwo ? s : 0][p] = pack(y0 - __low2float(h), y1 - __high2float(h));
         }
       }
+    return __any_sync(0xffffffffu, own < kLeastPower || own > kMostPower);
   }
 };
 

@@ -17,7 +17,8 @@ def filled(be, lengths, keys, values, fmt="i8", dtype="f32"):
     """A bank that holds these rows [all, kv, dim]."""
     kv, dim = keys.shape[1:]
     b = Bank(be, lengths, kv, dim, fmt, dtype=dtype)
-    x = cuda(np.stack([keys, values]).astype(np.float32), TYPES[dtype])
+    most = float(np.finfo(np.float32).max)
+    x = cuda(np.clip([keys, values], -most, most).astype(np.float32), TYPES[dtype])
     host = x.float().cpu().numpy()
     torch.cuda.synchronize()
     be.cache_write(b.cache, b.table, kc.cache_rows(x[0].data_ptr(), x[1].data_ptr(), dtype, sum(lengths),
@@ -125,3 +126,48 @@ def test_shares_that_large_values_leave(be, lengths):
     a.mask[0][4, rng.random(n) < 0.8] = -1e30
     a.d_mask = cuda(a.mask[0].reshape(-1))
     close(a, a.attend(mask=True), mask=True)
+
+
+# --- products ---------------------------------------------------------------------
+
+FACTORS = [(2e37, 1e-36, 0.0), (1e38, 3e-38, 0.0), (3e37, 1e-44, 1e6), (1e-28, 1e36, 1e-8), (1e-20, 3e37, 1e-18), (1.0, 1e-30, 1e30),
+           (1.0, 1e30, -1e-30), (1e20, 1e-25, 3e4), (1e-26, 1e-12, 1e38), (1e37, 1e2, 3e-39), (1.0, 1e-38, 1e38), (1e10, 1.0, 1e-10),
+           (1e-28, 3e37, 0.0)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("size,ask,scale", FACTORS)
+def test_scores_whose_factors_are_far_from_one(be, size, ask, scale, dtype):
+    """Keys, questions and a scale that leave f32 two at a time, and whose product
+    does not: attention and pointer scores. Beside what Asked.check counts, factors
+    below 2^-126 are rounded to steps of 2^-149 (a question's) or of the least key
+    scale's codes (in the cached keys already)."""
+    if dtype == "bf16" and ask < 1e-40:
+        pytest.skip("below bf16's smallest")
+    rng = np.random.default_rng(6)
+    lengths, dim = [3, 70, 400], 32
+    n = sum(lengths)
+    b = filled(be, lengths, rng.normal(0, 1, (n, 1, dim)) * size, rng.normal(0, 1, (n, 1, dim)))
+    a = Asked(b, [2, 9, 3], 1, dtype, size=ask)
+    a.masks()
+    assert np.isfinite(a.q).all()
+    for mask in (False, True):
+        out, lse = a.attend(mask=mask, scale=scale)
+        assert np.isfinite(out).all()
+        close(a, (out, lse), scale=scale, mask=mask)
+    scores = torch.full((int(a.mask_off[-1]),), 7.0, device="cuda")
+    for mask in (False, True):
+        torch.cuda.synchronize()
+        be.cache_scores(b.cache, b.table, a.view, scores.data_ptr(), a.d_mask_off.data_ptr(),
+                        a.d_mask.data_ptr() if mask else None, scale)
+        be.synchronize()
+        s = scores.cpu().numpy()
+        sc = scale or float(np.float32(1 / np.sqrt(dim)))
+        for i in range(a.total):
+            q = a.seq[i]
+            at = a.mask_off[q] + (i - a.off[q]) * lengths[q]
+            k, x = b.keys[q][:, 0].astype(np.float64), a.q[i, 0].astype(np.float64)
+            want, ok = ref.masked(k @ x * sc, a.mask[q][i - a.off[q]] if mask else np.zeros(lengths[q]))
+            room = (np.abs(k) @ np.abs(x)) * abs(sc) * (dim * U + 2.0 ** -22) + 4 * U * (np.abs(want) + 16)
+            assert (np.abs(s[at:at + lengths[q]] - want)[ok] <= room[ok]).all(), i
+            assert (s[at:at + lengths[q]][~ok] == np.float32(-1e30)).all()
