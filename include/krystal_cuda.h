@@ -738,8 +738,10 @@ kc_status kc_cache_scores(kc_handle* h, const kc_cache_view* cache, const kc_pag
  * the handle; the banks are 8-bit, so that p lies within a few percent of
  * kc_forward_batch's and close decisions may differ. The call waits for the
  * batch's sizes and for the pipeline's error word, and releases the resident
- * batch. A turn that is refused or fails may have appended: repeat it with the
- * same lengths. Weight changes do not reach rows that are cached. */
+ * batch. When it returns, with an error too, its stream has passed what it queued.
+ * Arguments are refused before anything is appended; a turn that fails later may
+ * have appended: repeat it with the same lengths. Weight changes do not reach rows
+ * that are cached. */
 typedef struct kc_bank_view {
   const kc_cache_view* mixer;  /* HOST [mixer_blocks] */
   kc_cache_view selector;

@@ -52,12 +52,32 @@ kc_status turn_pass(kc_handle* h, const DevBatch& b, const kc::FrameTotals& tot,
   Workspace& ws = h->ws;
   const uint64_t Q = tot.q, R = tot.r, H = d.h;
   const int mix_m = 3 * int(d.enc), sel_m = mix_m + 5 * int(d.mix);
+  const uint64_t row = bank.table.max_len;
+  kc::cache::Ask ask{P<float>(ws.mq), P<uint64_t>(ws.q_off), uint32_t(Q), d.heads, tot.max_q, H, kc::kF32};
+  kc::cache::AttendArg a{};  // of a mixer block: they differ in their caches
+  a.t = bank.table;
+  a.a = ask;
+  a.scale = kc::cache::scale_by(float(1.0 / std::sqrt(double(d.hd))));
+  a.out_pitch = H;
+  // what can be refused is refused before anything is appended
+  if (Q > 0) {
+    if (d.mix) {
+      a.c = bank.mixer[0];
+      KC_TRY(ensure(h, ws.turn_attend, Q * H * 4), "workspace");
+      KC_TRY(ensure(h, ws.turn_work, kc::cache::plan_attend(a, h->sms) * 4 + 16), "workspace");
+      a.out = ws.turn_attend.p;
+      a.work = P<float>(ws.turn_work);
+    }
+    KC_TRY(ensure(h, ws.turn_off, (b.frames + 1) * 8ull), "workspace");
+  }
+  const bool planes = !h->kplanes.empty();
+  if (planes && R > 0) {
+    KC_TRY(ensure(h, ws.sk, h->kplanes.size() * R * H * 4), "workspace");
+    KC_TRY(ensure(h, ws.mv, h->vplanes.size() * R * H * 4), "workspace");
+  }
   KC_CHECK(encode_fast(h, ws, b, tot));
   if (R > 0) {
-    const bool planes = !h->kplanes.empty();
     if (planes) {  // bk through the selector's Wk and every block's Wk, bv through every block's Wv
-      KC_TRY(ensure(h, ws.sk, h->kplanes.size() * R * H * 4), "workspace");
-      KC_TRY(ensure(h, ws.mv, h->vplanes.size() * R * H * 4), "workspace");
       KC_CHECK(tc_gemm_planes(h, P<float>(ws.bk), R, h->kplanes, P<float>(ws.sk)));
       KC_CHECK(tc_gemm_planes(h, P<float>(ws.bv), R, h->vplanes, P<float>(ws.mv)));
     } else {
@@ -80,21 +100,11 @@ kc_status turn_pass(kc_handle* h, const DevBatch& b, const kc::FrameTotals& tot,
     KC_CHECK(append(bank.selector, P<float>(ws.sk), P<float>(ws.bv)));
   }
   if (Q == 0) return KC_OK;
-  const uint64_t row = bank.table.max_len;
-  kc::cache::Ask ask{P<float>(ws.mq), P<uint64_t>(ws.q_off), uint32_t(Q), d.heads, tot.max_q, H, kc::kF32};
   for (uint32_t blk = 0; blk < d.mix; blk++) {
     const int m0 = mix_m + 5 * int(blk);
     KC_CHECK(tc_gemm<kc::tc::kEpiStore>(h, P<float>(ws.qstate), Q, m0, P<float>(ws.mq)));
-    kc::cache::AttendArg a{};
     a.c = bank.mixer[blk];
-    a.t = bank.table;
-    a.a = ask;
-    a.scale = kc::cache::scale_by(float(1.0 / std::sqrt(double(d.hd))));
-    a.out_pitch = H;
-    KC_TRY(ensure(h, ws.turn_attend, Q * H * 4), "workspace");
-    KC_TRY(ensure(h, ws.turn_work, kc::cache::plan_attend(a, h->sms) * 4 + 16), "workspace");
-    a.out = ws.turn_attend.p;
-    a.work = P<float>(ws.turn_work);
+    kc::cache::plan_attend(a, h->sms);
     KC_TRY(kc::cache::launch_attend(a, h->sms, h->stream, &h->launches), "attention launch");
     k_turn_add<<<unsigned((Q * H / 4 + 255) / 256), 256, 0, h->stream>>>(P<float4>(ws.qstate),
                                                                        P<float4>(ws.turn_attend), Q * H / 4);
@@ -103,7 +113,6 @@ kc_status turn_pass(kc_handle* h, const DevBatch& b, const kc::FrameTotals& tot,
     KC_CHECK(tc_gemm<kc::tc::kEpiResid>(h, P<float>(ws.mh), Q, m0 + 4, P<float>(ws.qstate)));
   }
   KC_CHECK(tc_gemm<kc::tc::kEpiStore>(h, P<float>(ws.qstate), Q, sel_m, P<float>(ws.sq)));
-  KC_TRY(ensure(h, ws.turn_off, (b.frames + 1) * 8ull), "workspace");
   k_turn_offsets<<<b.frames / 256 + 1, 256, 0, h->stream>>>(P<uint64_t>(ws.q_off), b.frames, row, P<uint64_t>(ws.turn_off));
   h->launches++;
   ask.q = ws.sq.p;
@@ -136,6 +145,7 @@ extern "C" kc_status kc_bank_turn(kc_handle* h, const kc_batch_view* bv, const k
     return fail(h, KC_ERR_INVALID_ARG, "a cache keeps no schemas or bands: a turn takes an explicit mask");
   if (!aligned(out->p, 4) || !aligned(out->index, 4) || !aligned(out->logp, 4) || !aligned(bv->mask, 4))
     return fail(h, KC_ERR_INVALID_ARG, "a turn's outputs and mask must be 4-byte aligned");
+  if (!aligned(bv->uniforms, 8)) return fail(h, KC_ERR_INVALID_ARG, "uniforms must be 8-byte aligned");
   if (sampling) KC_CHECK(check_sampling(h, sampling, false));
   Bank bank;
   try {
@@ -149,11 +159,17 @@ extern "C" kc_status kc_bank_turn(kc_handle* h, const kc_batch_view* bv, const k
   b.band_ids = bv->band_ids; b.uniforms = bv->uniforms; b.word_ids = bv->word_ids; b.word_alpha = bv->word_alpha;
   b.mask = bv->mask;
   kc::FrameTotals tot;
-  KC_CHECK(pack_batch(h, h->ws, b, &tot));
+  // whatever the call answers, its arrays are the caller's again: nothing that it
+  // queued is left to run
+  auto over = [&](kc_status s) {
+    if (s) (void)wait_stream(h);
+    return s;
+  };
+  KC_CHECK(over(pack_batch(h, h->ws, b, &tot)));
   if (tot.q && (!out->p || out->q_capacity < tot.q))
-    return fail(h, KC_ERR_CAPACITY, "the output rows are fewer than the turn's questions");
+    return over(fail(h, KC_ERR_CAPACITY, "the output rows are fewer than the turn's questions"));
   for (;;) {
-    KC_CHECK(turn_pass(h, b, tot, bank, sampling, out));
+    KC_CHECK(over(turn_pass(h, b, tot, bank, sampling, out)));
     KC_TRY(cudaMemcpyAsync(h->h_err, h->d_err, sizeof(int), cudaMemcpyDeviceToHost, h->stream), "readback");
     KC_TRY(wait_stream(h), "turn");
     const int e = *h->h_err;
