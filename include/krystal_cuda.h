@@ -690,9 +690,11 @@ kc_status kc_cache_blocks(kc_handle* h, const kc_cache_view* cache, const kc_pag
  * twice counts twice; numbers outside the sequence count for nothing). A mask
  * entry at or below -1e29, or NaN, shuts its row out, larger ones than 1e29 count
  * as 1e29; rows behind the mask's end are shut out. Nothing left: out 0, lse
- * -infinity. Scores, sums and statistics are f32; the weights are rounded to 22
- * bits before they meet the values, to 11 for bf16 questions. No output overlaps
- * an input. */
+ * -infinity. Scores, sums and statistics are f32; the weights are rounded before
+ * they meet the values: to 22 bits, to 11 for bf16 questions, or to 2^-33 of the
+ * question's largest product of a weight and its value scale, whichever is coarser
+ * (there a row of zeros counts with a scale of 2^-40). So n rows far below a leading
+ * one add up to n 2^-33 of it too little or too much. No output overlaps an input. */
 typedef struct kc_attend_view {
   void* out;                 /* [questions, heads, head_dim], the questions' type, out_pitch elements apart (0 = dense) */
   uint64_t out_pitch;

@@ -25,6 +25,11 @@
 //   l = sum 2^((b_j - B) + s_j - L),  L the largest exponent.
 // Sums that meet, of warps or parts, bring their L (M - 8 where there is none).
 //
+// Small weights. The least step of f16's pieces is 2^-24, so that x_j f_j is rounded
+// to 2^-33 of 2^M at the finest. (The general form with weights brought up cell by
+// cell, from 8192 rows a warp on, took 3.9 ms where this takes 2.2: 200 banks of
+// 30000 rows, 64 f32 questions.)
+//
 // A cell's bytes are read once by the team of warps that needs them, by 16-byte
 // asynchronous copies two cells ahead (one in masked calls of wide heads).
 //

@@ -171,3 +171,59 @@ def test_scores_whose_factors_are_far_from_one(be, size, ask, scale, dtype):
             room = (np.abs(k) @ np.abs(x)) * abs(sc) * (dim * U + 2.0 ** -22) + 4 * U * (np.abs(want) + 16)
             assert (np.abs(s[at:at + lengths[q]] - want)[ok] <= room[ok]).all(), i
             assert (s[at:at + lengths[q]][~ok] == np.float32(-1e30)).all()
+
+
+# --- small weights ------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("gap,mask", [(14.0, False), (22.0, True), (28.0, False), (45.0, True), (60.0, False)])
+def test_the_tail_behind_one_leading_row(be, gap, mask, dtype):
+    """One row whose score lies `gap` above 20000 others', its values zeros and then
+    ones, under questions enough that each warp has every row. The tail's share is
+    20000 e^-gap: beside zeros it is the output. Room is the header's: a weight is
+    rounded to 22 bits (11) or to 2^-33 of the largest product of a weight and its value
+    scale, a row of zeros counting with 2^-40."""
+    n, dim, nq, heads = 20000, 32, 300, 128
+    rng = np.random.default_rng(8)
+    keys = np.zeros((n, 1, dim))
+    values = rng.normal(1, 0.1, (n, 1, dim))
+    lead = 777
+    for value in (0.0, 1.0):
+        keys[lead], values[lead] = 1.0, value
+        b = filled(be, [n], keys, values)
+        a = Asked(b, [nq], heads, dtype)
+        q = torch.full_like(a.flat, gap / 32 * 32 ** 0.5)
+        q.view(nq * heads, dim)[::7] *= 0.5  # rows of half the gap between
+        a.flat.copy_(q)
+        a.q = q.float().cpu().numpy().reshape(nq, heads, dim)
+        some = [0, 1, 6, 150, 299]
+        if mask:
+            m = rng.normal(0, 0.5, (nq, n)).astype(np.float32)
+            m[:, lead] = 0
+            m[:, 1::3] = -1e30
+            a.mask, a.mask_off = [m], offsets([nq * n])
+            a.d_mask, a.d_mask_off = cuda(m.reshape(-1)), cuda(a.mask_off)
+        out, lse = a.attend(mask=mask)
+        k, v = (x[0][:, 0].astype(np.float64) for x in (b.keys, b.values))
+        half = float(torch.finfo(TYPES[dtype]).eps) / 2
+        weight = 2.0 ** -11 if dtype == "bf16" else 2.0 ** -22
+        sc = float(np.float32(1 / np.sqrt(dim)))
+        for i in some:
+            for h in (0, 1, 7, 64, 127):
+                x = k @ a.q[i, h].astype(np.float64) * sc
+                if mask:
+                    x, ok = ref.masked(x, a.mask[0][i].astype(np.float64))
+                    x = np.where(ok, x, -np.inf)
+                p = np.exp(x - x.max())
+                wl = x.max() + np.log(p.sum())
+                p /= p.sum()
+                want = p @ v
+                # the scores, sums of 32 equal terms, and masks of up to 4 beside them; sums of n terms
+                ds = gap * (dim * U + 2.0 ** -22) + 4 * U * (2 * gap + 16)
+                rel = 4 * ds + weight + (n / 8 + 64) * U
+                least = (p * np.maximum(np.abs(v).max(1), 127 * 2.0 ** -40)).max() * n * 2.0 ** -33
+                assert abs(lse[i, h] - wl) <= 2 * ds + (n / 8 + 64) * U
+                room = (p @ np.abs(v)) * rel + half * np.abs(want) + least
+                if dtype == "f16":
+                    room = room + 2.0 ** -25  # half its smallest step
+                assert (np.abs(out[i, h] - want) <= room).all(), (value, i, h, out[i, h][:3], want[:3])
