@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import collections
 import ctypes as C
+import itertools
 import threading
 from dataclasses import dataclass, field
 from typing import Callable, Sequence
@@ -159,6 +160,10 @@ class CudaBrainBackend:
         self._clips_dropped = collections.deque()  # what dropped lists held that the stream may not have passed,
         self._clips_queued: list = []              # and behind an event
         self._clip_lock = threading.Lock()
+        # Calls on caches take tickets as they begin and as they have queued; the
+        # stream has passed what was queued under tickets up to the last that a
+        # waiting call took before it waited.
+        self._tickets, self._passed = itertools.count(1), 0
 
     # --- BrainBackend -----------------------------------------------------
     def encode(self, frame: HostFrame) -> EncodedFrame:
@@ -414,11 +419,25 @@ class CudaBrainBackend:
         if self._clips_dropped or self._clips_queued:
             self._release_clips()
 
+    def ticket(self) -> int:
+        return next(self._tickets)
+
+    def passed(self, ticket: int) -> bool:
+        return not self._h or ticket <= self._passed
+
+    def _waited(self, ticket: int) -> None:
+        """After a wait for the stream that began behind ``ticket``: it has passed
+        what was queued, and let go of what was dropped, under earlier ones."""
+        with self._clip_lock:
+            self._passed = max(self._passed, ticket)
+            while self._clips_dropped and self._clips_dropped[0][0] <= ticket:
+                self._clips_dropped.popleft()
+
     def hold_clip(self, parts) -> None:
         """Takes what a dropped list or cache held (GradList.__del__,
         BankCache.__del__; no CUDA call: it may run anywhere, in a capture too)."""
         if self._h:
-            self._clips_dropped.append(parts)
+            self._clips_dropped.append((self.ticket(), parts))
 
     def _release_clips(self) -> None:
         """Lets go of the dropped lists whose event has passed. The event is
@@ -438,7 +457,7 @@ class CudaBrainBackend:
                     return
             while self._clips_dropped:
                 event = torch.cuda.Event()
-                self._clips_queued.append((self._clips_dropped.popleft(), event))
+                self._clips_queued.append((self._clips_dropped.popleft()[1], event))
                 event.record(stream)
             self._clips_queued = [c for c in self._clips_queued if not c[1].query()]
 
@@ -451,25 +470,30 @@ class CudaBrainBackend:
             self._release_clips()
         return C.byref(cache.view)
 
+    def _cache_call(self, call, cache: BankCache, *args) -> None:
+        try:
+            abi.check(call(self._h, self._cache(cache), *args), self._h)
+        finally:
+            cache.queued_on(self)  # by now: a wait that another thread began before does not cover it
+
     def cache_write(self, cache: BankCache, table: abi.KcPageTable, rows: abi.KcCacheRows) -> None:
         """kc_cache_write: the rows quantised as the last of their sequences
         (cache.page_table, cache.cache_rows: device pointers); queued on the
         handle's stream, as the other calls on a cache are."""
-        abi.check(self._lib.kc_cache_write(self._h, self._cache(cache), C.byref(table), C.byref(rows)), self._h)
+        self._cache_call(self._lib.kc_cache_write, cache, C.byref(table), C.byref(rows))
 
     def cache_read(self, cache: BankCache, table: abi.KcPageTable, rows: abi.KcCacheRows,
                    starts: int | None = None) -> None:
         """kc_cache_read: the sequences' last rows, or those from ``starts`` (u32
         [sequences], device) on, into rows.keys and rows.values."""
-        abi.check(self._lib.kc_cache_read(self._h, self._cache(cache), C.byref(table), starts, C.byref(rows)), self._h)
+        self._cache_call(self._lib.kc_cache_read, cache, C.byref(table), starts, C.byref(rows))
 
     def cache_blocks(self, cache: BankCache, table: abi.KcPageTable, questions: abi.KcQuestionView, count: int,
                      recent: int, blocks: int) -> None:
         """kc_cache_blocks: the ``count`` pages each question's group of heads looks
         at, the ``recent`` last ones among them, into blocks (u32 [questions,
         kv_heads, count], device)."""
-        abi.check(self._lib.kc_cache_blocks(self._h, self._cache(cache), C.byref(table), C.byref(questions), count,
-                                            recent, blocks), self._h)
+        self._cache_call(self._lib.kc_cache_blocks, cache, C.byref(table), C.byref(questions), count, recent, blocks)
 
     def attend_workspace(self, cache: BankCache, table: abi.KcPageTable, questions: abi.KcQuestionView,
                          block_count: int = 0) -> int:
@@ -487,16 +511,14 @@ class CudaBrainBackend:
         are device pointers."""
         v = abi.KcAttendView(out, out_pitch, lse, mask, mask_off, blocks, block_count, scale, workspace,
                              workspace_bytes)
-        abi.check(self._lib.kc_cache_attend(self._h, self._cache(cache), C.byref(table), C.byref(questions),
-                                            C.byref(v)), self._h)
+        self._cache_call(self._lib.kc_cache_attend, cache, C.byref(table), C.byref(questions), C.byref(v))
 
     def cache_scores(self, cache: BankCache, table: abi.KcPageTable, questions: abi.KcQuestionView, scores: int,
                      off: int, mask: int | None = None, scale: float = 0.0) -> None:
         """kc_cache_scores: pointer scores over a cache of one head, laid out like a
         batch's p at ``off``: rows that ``draw`` and ``policy_loss`` take
         (policy.ragged_rows)."""
-        abi.check(self._lib.kc_cache_scores(self._h, self._cache(cache), C.byref(table), C.byref(questions), off, mask,
-                                            scale, scores), self._h)
+        self._cache_call(self._lib.kc_cache_scores, cache, C.byref(table), C.byref(questions), off, mask, scale, scores)
 
     def bank_turn(self, frames: int, records: int, rec_off: int, token_ids: int, field_roles: int, schema_ids: int,
                   band_ids: int, mixer: Sequence[BankCache], selector: BankCache, table: abi.KcPageTable, p: int,
@@ -509,6 +531,7 @@ class CudaBrainBackend:
             raise ValueError(f"a bank has a cache per mixer block ({self.config.mixer_blocks})")
         for c in (*mixer, selector):
             self._cache(c)
+        ticket = self.ticket()
         views = (abi.KcCacheView * max(1, len(mixer)))(*(c.view for c in mixer))
         bank = abi.KcBankView(views, selector.view, table)
         bv = abi.KcBatchView(frames, records, rec_off, token_ids, field_roles, schema_ids, band_ids, None, None,
@@ -516,6 +539,7 @@ class CudaBrainBackend:
         out = abi.KcBankOut(p, index, logp, q_capacity)
         s = C.byref(sampling.device_struct()) if sampling is not None else None
         abi.check(self._lib.kc_bank_turn(self._h, C.byref(bv), C.byref(bank), s, C.byref(out)), self._h)
+        self._waited(ticket)
         return out
 
     # --- packed ragged batches ------------------------------------------------
@@ -648,7 +672,9 @@ class CudaBrainBackend:
         return int(self._lib.kc_get_stream(self._h) or 0)
 
     def synchronize(self) -> None:
+        ticket = self.ticket()
         abi.check(self._lib.kc_synchronize(self._h), self._h)
+        self._waited(ticket)
         if self._clips_dropped or self._clips_queued:
             self._release_clips()
 

@@ -27,8 +27,9 @@ class BankCache:
     (kc_cache_view). ``storage``: a CUDA uint8 tensor of at least
     ``BankCache.bytes_for(...)`` bytes, or None for one of its own on ``device``.
     A cache dropped while its calls are queued leaves the storage with their
-    backends until the stream has passed them; a captured call's cache has to
-    live as long as its graph."""
+    backends until the stream has passed them; once a call that waits for the
+    stream has returned (synchronize, bank_turn) a drop frees it. A captured
+    call's cache has to live as long as its graph."""
 
     def __init__(self, pages: int, kv_heads: int = 4, head_dim: int = 32, format: str = "i8", storage=None,
                  device: int = 0):
@@ -48,7 +49,7 @@ class BankCache:
         self.storage, self.device = storage, storage.device
         self.view = abi.KcCacheView(storage.data_ptr(), storage.numel(), self.pages, self.kv_heads, self.head_dim,
                                     FORMATS[format])
-        self.backends = []  # weak references to those that queued a call on it
+        self.backends = []  # weak references to those that queued a call on it, and each one's last ticket
 
     @staticmethod
     def bytes_for(pages: int, kv_heads: int = 4, head_dim: int = 32) -> int:
@@ -64,14 +65,18 @@ class BankCache:
         return self.storage[size - n:size].view(torch.float32).view(self.pages, self.kv_heads, 2, self.head_dim)
 
     def queued_on(self, backend) -> None:
-        if not self.backends or self.backends[-1]() is not backend:
-            self.backends = [r for r in self.backends if r() is not None and r() is not backend]
-            self.backends.append(weakref.ref(backend))
+        ticket = backend.ticket()
+        last = self.backends[-1] if self.backends else None
+        if last and last[0]() is backend:
+            last[1] = ticket
+        else:
+            self.backends = [b for b in self.backends if b[0]() is not None and b[0]() is not backend]
+            self.backends.append([weakref.ref(backend), ticket])
 
     def __del__(self):
-        for r in getattr(self, "backends", ()):
+        for r, ticket in getattr(self, "backends", ()):
             backend = r()
-            if backend is not None:
+            if backend is not None and not backend.passed(ticket):
                 backend.hold_clip((self.storage,))
 
 
