@@ -607,7 +607,8 @@ kc_status kc_clip_grads(kc_handle* h, const kc_grad_view* grads, uint64_t count,
  * change places where head_dim is 128 and bit 2 of its row is set; a value's
  * byte b lies at b ^ 32 * (row & 3) for 128 dims and b ^ 32 * ((row >> 1) & 1)
  * for 64. Behind the pages lie their bounds [pages][kv_heads][2][head_dim] f32:
- * the smallest and the largest of the keys that a page holds.
+ * the smallest and the largest of the keys that a page held when it was last
+ * written to. A sequence cut back leaves them: they bound what is left too.
  * A row x of a head is stored as scale = max(f32(max |x| / top), 2^-100) and
  * code = round(f32(x / scale)), halves to the even, top = 127 (KC_CACHE_I8, kept
  * as code + 128) or 448 (KC_CACHE_E4M3); its value is f32(code * scale). NaN

@@ -58,7 +58,7 @@ class BankCache:
 
     def bounds(self):
         """[pages, kv_heads, 2, head_dim] f32, a view of the storage: the smallest
-        and the largest of the keys that each page holds."""
+        and the largest of the keys that each page held when it was last written to."""
         import torch
         n = self.pages * self.kv_heads * 2 * self.head_dim * 4
         size = self.bytes_for(self.pages, self.kv_heads, self.head_dim)

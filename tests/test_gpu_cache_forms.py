@@ -118,3 +118,26 @@ def test_rows_behind_gaps_of_empty_sequences(be, lengths, dtype, kv, dim):
     k, v, _ = read_all(b, counts=counts)
     assert np.array_equal(k, np.concatenate([x[len(x) - c:] for x, c in zip(b.keys, counts)]))
     assert np.array_equal(v, np.concatenate([x[len(x) - c:] for x, c in zip(b.values, counts)]))
+
+
+def test_a_cut_sequence_is_selected_by_the_bounds_of_its_last_write(be):
+    """Cut back and not written to: the last page's bounds still hold the rows that
+    are gone; a row written to it takes them out."""
+    b = Bank(be, [64 * 4 + 40], 1, 32)
+    a = Asked(b, [6])
+    held = b.keys[0]
+    lengths = cuda(np.array([64 * 4 + 3], np.uint32))
+    b.table = kc.page_table(b.d["pages"].data_ptr(), lengths.data_ptr(), 1, b.pitch)
+
+    def check(bounds):
+        got = select(b, a, 2, 0).cpu().numpy().astype(np.uint32)
+        for i in range(6):
+            assert got[i, 0].tolist() == ref.chosen(ref.block_scores(a.q[i], bounds)[0], 2, 0)
+
+    check(ref.bounds(held))
+    x = torch.randn(2, 1, 1, 32, device="cuda")
+    off = cuda(np.array([0, 1]))
+    torch.cuda.synchronize()
+    be.cache_write(b.cache, b.table, kc.cache_rows(x[0].data_ptr(), x[1].data_ptr(), "f32", 1, off.data_ptr()))
+    be.synchronize()
+    check(ref.bounds(np.concatenate([held[:64 * 4 + 2], ref.quantised(x[0].cpu().numpy(), "i8")])))
