@@ -51,7 +51,7 @@ namespace {
 
 constexpr int kThreads = 256, kWarps = 8;
 constexpr float kLift = 8.0f, kSlack = 6.0f, kFar = 32.0f;
-constexpr uint32_t kLeastExp = 127 - 40, kMostExp = 127 + 24;  // biased: usual value scales lie between
+constexpr uint32_t kLeastExp = 127 - 40, kMostExp = 127 + 24;  // biased, of the usual value scales
 
 // Cells a ring holds; a masked call's has the mask entries of each warp's rows
 // beside them, 36 floats apart so that what a warp reads at once lies on different banks.
@@ -391,18 +391,16 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
     bool apart;  // the lane's row has an unusual scale, or is one of zeros
     {
       const float vs = scales[kCell + lane];
-      const uint32_t e = min(max(__float_as_uint(vs) >> 23, kGeneral ? 27u : kLeastExp), 253u);
+      const uint32_t raw = __float_as_uint(vs) >> 23, e = min(max(raw, kGeneral ? 27u : kLeastExp), kGeneral ? 253u : kMostExp);
+      const bool open = pos + lane < open_end;
       KeyInfo k;
       k.re = pow2_biased(254u - e);
       k.f = vs * k.re;
       k.a = scales[lane];
       k.e = float(int(e) - 127);
       if (kGeneral && vs == kLeastScale && zero_row<D, FMT>(cell + (kCell + lane) * D)) k.e = -INFINITY;
-      apart = e - (kLeastExp + 1) >= kMostExp - kLeastExp;
-      if (pos + lane >= open_end) {
-        k = KeyInfo{0.0f, -INFINITY, 0.0f, 0.0f};
-        apart = false;
-      }
+      apart = open && raw != e;
+      if (!open) k = KeyInfo{0.0f, -INFINITY, 0.0f, 0.0f};
       info[lane] = k;
     }
     float s[NT][2][4];
