@@ -33,12 +33,15 @@
 // A cell's bytes are read once by the team of warps that needs them, by 16-byte
 // asynchronous copies two cells ahead (one in masked calls of wide heads).
 //
-// Measured (B200): few question rows are bound by memory: single bf16 tokens of 32
-// sequences of up to 16384 rows (8 key heads of 128, e4m3) take 109 us, 5.2 TB/s;
-// one f16 token over 400003 rows 42 us, 5.1 TB/s. Many are bound by issue, 400 to
-// 900 instructions a cell and warp: 64 f32 questions over 64 masked banks of 4096
-// (4 heads of 32) take 179 us, of which the exponentials need 15 and the tensor
-// cores 30; 4096 banks of 8 to 240 rows with 1 to 16 questions 91 us, 2.1 TB/s.
+// Measured (B200, whole calls): few question rows are bound by memory: single bf16
+// tokens of 32 sequences of up to 16384 rows (8 key heads of 128, e4m3) take 115 us,
+// 4.9 TB/s; one f16 token over 400003 rows 55 us, of which the parts 42 (5.2 TB/s).
+// Many are bound by their instructions, 400 to 900 a cell and warp, and the few
+// warps that hide their latency (2.3 to 2.4 of 4 a cycle with 4 warps a scheduler;
+// most stalls wait for the instruction before): 64 f32 questions over 64 masked
+// banks of 4096 (4 heads of 32) take 183 us, of which the exponentials need 15, the
+// tensor cores 30 and the join of the parts takes 14; 4096 banks of 8 to 240 rows
+// with 1 to 16 questions 86 us, 2.1 TB/s.
 #pragma once
 #include <algorithm>
 #include <type_traits>
@@ -238,12 +241,19 @@ __device__ __forceinline__ bool zero_row(const uint8_t* codes) {
 }
 
 // f16 pieces of a weight: two for f32 questions (22 bits) and for f16 ones, whose
-// output one piece's rounding would reach; bf16 outputs round 8 times more.
+// output one piece's rounding would reach; bf16 outputs round 8 times more. (With one,
+// 7 % of bf16 outputs lie a step from those of f32 weights, with two 0.2 %, both as far
+// from the exact ones; two take single tokens from 115 to 119 us, 20 questions of 64
+// dims from 109 to 166.)
 template <typename T>
 __host__ __device__ constexpr int parts_of_weights() { return std::is_same<T, __nv_bfloat16>::value ? 1 : 2; }
 
-// CTAs of 256 threads that an SM should hold at once: what their rings and their
-// registers (without spilling) leave room for.
+// CTAs of 256 threads that an SM should hold at once: what their rings leave room
+// for. The registers of most forms then spill: 4 to 76 bytes a thread, 72 to 192 in
+// the masked two-tile f32 ones of 32 dims, the masked f32 ones of 64 and the two-tile
+// bf16 ones of 64. One CTA less, which spills nothing, is slower all the same: 64
+// masked banks of 4096 236 us against 183, 300 banks with 20 bf16 questions of 64
+// dims 146 against 109, 512 banks with 8 f32 questions 68 against 60.
 __host__ __device__ constexpr int resident(int dim, int tiles, bool masked, int weights) {
   return dim == 128 || (dim == 64 && tiles == 2 && (masked || weights == 2)) ? 1 : dim == 32 && tiles == 1 && !masked ? 3 : 2;
 }
@@ -678,9 +688,11 @@ __global__ __launch_bounds__(kThreads, resident(D, NT, MASKED, parts_of_weights<
   }
 }
 
-// The parts of every row of a cut sequence, joined (16384 rows of 4 parts: 15 us,
-// launch and latency): `per` warps a question and head, each over its share of the parts, 32 at a time (a lane a part for the
-// weights, then a lane a dimension), then the warps' sums in their order.
+// The parts of every row of a cut sequence, joined (16384 rows of 4 parts: 14 us,
+// launch and latency): `per` warps a question and head, each over its share of the
+// parts, 32 at a time (a lane a part for the weights, then a lane a dimension), then
+// the warps' sums in their order. It may be launched while the last of k_attend's
+// CTAs run, and begins when they have ended.
 template <typename T, int D, int FMT>
 __global__ __launch_bounds__(kThreads) void k_join(AttendArg a, uint32_t per) {
   __shared__ float s_o[kWarps][D];
@@ -829,8 +841,8 @@ cudaError_t attend_tile(const AttendArg& a, int sms, cudaStream_t s, uint64_t* l
 // every 16 questions before, 110 us against 81; 72 since the questions are read 4
 // elements at once). The products pass through shared
 // memory so that masks are read and scores written 32 to a row; the mask's entries
-// are on their way while the cell is multiplied. Bound by issue: 540 instructions a
-// cell and warp, a quarter of them widening i8 keys.
+// are on their way while the cell is multiplied. Bound by 540 instructions a cell and
+// warp, a quarter of them widening i8 keys, at 2.0 of 4 a cycle.
 template <typename T, int D, int FMT>
 __global__ __launch_bounds__(kThreads, 2) void k_scores(ScoreArg a, uint32_t mg, uint32_t chunks, uint32_t cells) {
   constexpr int S = 3, KB = int(kCell) * D, CB = KB + int(kCell) * 4;  // keys and their scales

@@ -171,9 +171,10 @@ __device__ __forceinline__ void widen_bounds(const uint32_t (&w)[2], float scale
 // beforehand; where pages are few, several CTAs share them, each some of the heads.
 // kAhead passes of 8 elements a lane are on their way together (4 a lane took twice
 // the instructions for f32), and no code of the call's rows is read again.
-// 507 000 f32 rows of 4 heads of 32: 157 us, 4.2 TB/s; 250 000 bf16 rows of 8 heads
-// of 128 to e4m3: 489 us, 3.2 TB/s, bound by about 20 instructions an element (the
-// quotient, the code, its value again for the bounds).
+// 507 000 f32 rows of 4 heads of 32: 159 us, 4.2 TB/s; 250 000 bf16 rows of 8 heads
+// of 128 to e4m3: 481 us, 3.2 TB/s. About 20 instructions an element (the quotient, the
+// code, its value again for the bounds) take half of that; the warps wait for memory
+// first, and the registers leave room for 38 % of them.
 constexpr int kWriteThreads = 128;
 
 template <typename T, int D, int FMT, bool WIDE>
@@ -477,8 +478,8 @@ __device__ __forceinline__ Cut cut_of(const unsigned long long* key, uint32_t n,
 // smallest and of the largest keys a lane and step, so that 8 blocks of a warp are
 // on their way at once. The scores go, as keys that order alike, to the shared
 // memory of the CTA that selects for the question, with as many of its warps as the
-// other questions leave (64 banks of 4096 with 16 questions: 24 us; 8 histories of
-// 131072 with 4 questions on 8 key heads of 128, clusters of 4: 61 us, of which the
+// other questions leave (64 banks of 4096 with 16 questions: 21 us; 8 histories of
+// 131072 with 4 questions on 8 key heads of 128, clusters of 4: 58 us, of which the
 // bounds' bytes need 20 and the f64 sums about 15). The newest
 // blocks are the sequence's last, so they follow whatever is selected.
 template <typename T, int D>

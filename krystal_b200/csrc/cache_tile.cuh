@@ -136,7 +136,7 @@ struct QTile {
 
   // row: row g of tile t, null where there is none; wide: it begins at 16 bytes, and
   // is read 4 elements at once (515 sequences of 20 questions, 8 heads of 128 in f16
-  // over 2: 118 us, 123 one by one). m 2^e multiplies every score. power: the units
+  // over 2: 121 us, 5 more one by one). m 2^e multiplies every score. power: the units
   // are m 2^power; true where a unit does not hold one of the tile's.
   __device__ __forceinline__ bool load(int t, const T* row, bool wide, int c, float m, int e, int (&power)[2]) {
     float x[kSteps][4], top = 0.0f;
