@@ -127,7 +127,7 @@ struct QTile {
   static constexpr int kSteps = D / 16;
   uint32_t hi[NT][kSteps][2], lo[kTwo ? NT : 1][kTwo ? kSteps : 1][2];
   float unit[NT][2];  // what a product of rows 2c and 2c + 1 of a tile is multiplied by
-  static constexpr int kLeastPower = -126, kMostPower = 108;  // of two that a unit may hold
+  static constexpr int kLeastPower = -125, kMostPower = 108;  // of two that a unit may hold
 
   // Dimension of the first of the 4 elements of lane c's piece of fragment s.
   static __device__ __forceinline__ int dim(int s, int c) {

@@ -132,7 +132,7 @@ def test_shares_that_large_values_leave(be, lengths):
 
 FACTORS = [(2e37, 1e-36, 0.0), (1e38, 3e-38, 0.0), (3e37, 1e-44, 1e6), (1e-28, 1e36, 1e-8), (1e-20, 3e37, 1e-18), (1.0, 1e-30, 1e30),
            (1.0, 1e30, -1e-30), (1e20, 1e-25, 3e4), (1e-26, 1e-12, 1e38), (1e37, 1e2, 3e-39), (1.0, 1e-38, 1e38), (1e10, 1.0, 1e-10),
-           (1e-28, 3e37, 0.0)]
+           (1e-28, 3e37, 0.0), (6e37, 8e-38, 0.0), (6e37, 4e-38, 0.0), (6e37, 2e-38, 0.0), (1e-3, 3e32, 1e-30)]
 
 
 @pytest.mark.parametrize("dtype,size,ask,scale", [(t, *f) for f in FACTORS for t in ("f32", "bf16")
