@@ -708,6 +708,7 @@ typedef struct kc_attend_view {
   void* workspace;           /* kc_cache_attend_workspace bytes, 16-byte aligned, the call's own while it runs */
   uint64_t workspace_bytes;
 } kc_attend_view;
+/* 0 where none is needed, and for arguments that kc_cache_attend refuses. */
 uint64_t kc_cache_attend_workspace(kc_handle* h, const kc_cache_view* cache, const kc_page_table* table,
                                    const kc_question_view* questions, uint32_t block_count);
 kc_status kc_cache_attend(kc_handle* h, const kc_cache_view* cache, const kc_page_table* table,

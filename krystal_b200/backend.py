@@ -471,8 +471,9 @@ class CudaBrainBackend:
         return C.byref(cache.view)
 
     def _cache_call(self, call, cache: BankCache, *args) -> None:
+        view = self._cache(cache)
         try:
-            abi.check(call(self._h, self._cache(cache), *args), self._h)
+            abi.check(call(self._h, view, *args), self._h)
         finally:
             cache.queued_on(self)  # by now: a wait that another thread began before does not cover it
 

@@ -104,6 +104,14 @@ def test_a_cache_of_two_backends_waits_for_both(be, monkeypatch):
         other._h = None
 
 
+def test_a_refused_device_holds_nothing(be):
+    cache = bare_cache()
+    cache.device = torch.device("cuda", 1)
+    with pytest.raises(ValueError, match="lies on"):
+        write(be, cache)
+    assert cache.backends == []
+
+
 @pytest.mark.gpu
 def test_banks_are_freed_with_their_last_turn():
     """Sessions' caches dropped behind a turn leave the memory at once."""
